@@ -378,6 +378,109 @@ int ttt_b200_pack_layernorm_backward(const void* grad_y, const void* x, const fl
                                      void* grad_x, float* grad_gamma, float* grad_beta, int B, int T, int H,
                                      void* stream);
 
+/* ---- Layer-side sequence operators (no counterpart in the reference): what a layer has around and next to the TTT operator ----
+ * Activations are bf16, fp16 or fp32, all tensors of a call the same (`dtype`); weights, scan states and statistics fp32; everything
+ * between reading and writing is fp32.  Strides are in elements; innermost dimensions are contiguous; any alignment to the element
+ * (rows on 16-byte boundaries are read faster).  Device pointers; stream-ordered, no synchronisation; TTT_B200_* codes.  Outputs may
+ * not overlap inputs or one another.  Sums over tokens or channels have a fixed order: the same call gives the same bits.
+ * `lengths` (may be NULL): int32 [B], the tokens of each sequence of a right-padded batch (clamped to 0..T); those behind are not
+ * read, their y and gradients are zero and they change no state. */
+enum { TTT_B200_BF16 = 0, TTT_B200_FP16 = 1, TTT_B200_FP32 = 2 };
+enum { TTT_B200_ACT_NONE = 0, TTT_B200_ACT_SILU = 1, TTT_B200_ACT_GELU = 2 /* tanh form */, TTT_B200_ACT_SIGMOID = 3 };
+
+/* Short depthwise causal convolution: y[b][t][d] = act(bias[d] + sum_k weight[d][k] x[b][t - K + 1 + k][d]), K = 2, 3 or 4.  Inputs
+ * in front of the first token come from `state` [B][K-1][D] (NULL: zeros); the last K - 1 inputs are left in `final_state`. */
+typedef struct ttt_b200_conv_args {
+  const void* x;              /* [B][T][D], strides x_stride; step: [B][D], x_stride[0] */
+  const float* weight;        /* [D][K] */
+  const float* bias;          /* [D] or NULL */
+  const void* state;          /* [B][K-1][D] or NULL */
+  const int32_t* lengths;     /* [B] or NULL */
+  void* y;                    /* [B][T][D], with `heads` [B][D/64][T][64]; step: [B][D] */
+  void* final_state;          /* [B][K-1][D] or NULL */
+  /* backward: the inputs above, and */
+  const void* grad_y;         /* [B][T][D], strides gy_stride; with `heads` [B][D/64][T][64] contiguous */
+  const void* grad_final_state; /* [B][K-1][D] or NULL */
+  void* grad_x;               /* [B][T][D] */
+  float* grad_weight;         /* [D][K] */
+  float* grad_bias;           /* [D] or NULL */
+  void* grad_state;           /* [B][K-1][D] or NULL */
+  void* scratch;              /* ttt_b200_short_conv_scratch_bytes, 16-byte aligned */
+  uint64_t scratch_bytes;
+  /* step: the table of states, and which of its rows each row of the batch has */
+  void* state_io;             /* [rows][K-1][D], updated in place */
+  const int32_t* slots;       /* [B] or NULL (row b has state b, rows = B) */
+  int64_t x_stride[2], gy_stride[2];
+  int32_t B, T, D, K, rows, dtype, activation /* NONE or SILU */, heads;
+} ttt_b200_conv_args;
+int ttt_b200_short_conv(const ttt_b200_conv_args* args, void* stream);
+int ttt_b200_short_conv_backward(const ttt_b200_conv_args* args, void* stream);
+uint64_t ttt_b200_short_conv_scratch_bytes(const ttt_b200_conv_args* args);
+/* One token per row.  A row whose slot is not in 0..rows-1 is padding: y = 0, no state touched.  Rows that name the same slot are taken
+ * in the order of the rows, like tokens after one another. */
+int ttt_b200_short_conv_step(const ttt_b200_conv_args* args, void* stream);
+
+/* Selective state space scan over D channels of N states, G groups of D / G channels that share B and C:
+ *   delta = softplus(dt + dt_bias) (softplus = 0: dt + dt_bias);  h[d][n] = exp(delta A[d][n]) h[d][n] + delta x B[g][n];
+ *   y = sum_n C[g][n] h[d][n] + Dskip[d] x.   1 <= N <= 64; A finite. */
+enum { TTT_B200_SCAN_INTERVAL = 16 /* tokens between two checkpoints */ };
+typedef struct ttt_b200_scan_args {
+  const void *x, *dt;         /* [B][T][D], strides x_stride, dt_stride; step: [B][D], strides [0] */
+  const float* A;             /* [D][N] */
+  const void *Bm, *Cm;        /* [B][T][G][N], strides B_stride, C_stride; step: [B][G][N], strides [0] and [2] */
+  const float *Dskip, *dt_bias; /* [D] or NULL */
+  const float* state;         /* [B][D][N] or NULL (zeros) */
+  const int32_t* lengths;     /* [B] or NULL */
+  void* y;                    /* [B][T][D]; step: [B][D] */
+  float* final_state;         /* [B][D][N] or NULL */
+  float* checkpoints;         /* [B][ceil(T / 16)][D][N]: states before every 16th token, for the backward; forward: or NULL */
+  /* backward: the inputs and the checkpoints above, and */
+  const void* grad_y;         /* [B][T][D], strides gy_stride */
+  const float* grad_final_state; /* [B][D][N] or NULL */
+  void *grad_x, *grad_dt;     /* [B][T][D] */
+  float* grad_A;              /* [D][N] */
+  void *grad_B, *grad_C;      /* [B][T][G][N] */
+  float *grad_D, *grad_dt_bias; /* [D] or NULL */
+  float* grad_state;          /* [B][D][N] or NULL */
+  void* scratch;              /* ttt_b200_ssm_scan_scratch_bytes, 16-byte aligned; may be NULL where that is 0 */
+  uint64_t scratch_bytes;
+  /* step: the table of states, and which of its rows each row of the batch has */
+  float* state_io;            /* [rows][D][N], updated in place */
+  const int32_t* slots;       /* [B] or NULL (row b has state b, rows = B) */
+  int64_t x_stride[2], dt_stride[2], B_stride[3], C_stride[3], gy_stride[2];
+  int32_t B, T, D, G, N, rows, dtype, softplus;
+} ttt_b200_scan_args;
+int ttt_b200_ssm_scan(const ttt_b200_scan_args* args, void* stream);
+int ttt_b200_ssm_scan_backward(const ttt_b200_scan_args* args, void* stream);
+/* Bytes of scratch the forward (backward = 0) or backward needs; depends on B, T, D, G, N and the GPU. */
+uint64_t ttt_b200_ssm_scan_scratch_bytes(const ttt_b200_scan_args* args, int backward);
+/* One token per row; slots as in ttt_b200_short_conv_step. */
+int ttt_b200_ssm_scan_step(const ttt_b200_scan_args* args, void* stream);
+
+/* The end of a block and the start of the next: u = Norm(o) post_weight + post_bias;  x' = residual + scale u act(gate);
+ * n = Norm(x') pre_weight + pre_bias.  Norm: (v - mean) / sqrt(var + eps) (layer) or v / sqrt(mean(v^2) + eps).  Each part is left out
+ * with its pointer NULL: post_weight (u = o), gate, scale, residual (x' = the rest), pre_weight (no n).  The residual stream has the
+ * activations' type or fp32 (`residual_fp32`).  Rows of D values, 1 <= D <= 8192. */
+typedef struct ttt_b200_block_args {
+  const void *o, *residual, *gate; /* [M][D], strides */
+  const float *post_weight, *post_bias, *scale, *pre_weight, *pre_bias; /* [D] or NULL */
+  void *x, *n;                /* [M][D] */
+  float* stats;               /* [M][4] or NULL: mean and 1 / deviation of o, then of x'; the backward reads it */
+  /* backward: the inputs above, and */
+  const void *grad_x, *grad_n; /* [M][D], strides, either may be NULL */
+  void *grad_o, *grad_residual, *grad_gate; /* [M][D]; the last two NULL where there is none */
+  float *grad_post_weight, *grad_post_bias, *grad_scale, *grad_pre_weight, *grad_pre_bias; /* [D] or NULL */
+  void* scratch;              /* ttt_b200_norm_gate_residual_scratch_bytes, 16-byte aligned */
+  uint64_t scratch_bytes;
+  int64_t o_stride, residual_stride, gate_stride, gx_stride, gn_stride;
+  int64_t M;
+  int32_t D, dtype, residual_fp32, layer, activation;
+  float eps;
+} ttt_b200_block_args;
+int ttt_b200_norm_gate_residual(const ttt_b200_block_args* args, void* stream);
+int ttt_b200_norm_gate_residual_backward(const ttt_b200_block_args* args, void* stream);
+uint64_t ttt_b200_norm_gate_residual_scratch_bytes(const ttt_b200_block_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -68,7 +68,10 @@ class BwdNoAllocArgs(ctypes.Structure):
 EXPORTS = ["ttt_b200_forward", "ttt_b200_linear_forward", "ttt_b200_linear_backward", "ttt_b200_linear_backward_scratch_bytes", "ttt_b200_backward", "ttt_b200_backward_noalloc", "ttt_b200_last_error", "ttt_b200_take_status",
            "ttt_b200_version", "ttt_b200_pick_cluster", "ttt_b200_launch_cluster", "ttt_b200_forward_ctas", "ttt_b200_backward_ctas", "ttt_b200_backward_tail", "ttt_b200_backward_pairs", "ttt_b200_cluster_capacity", "ttt_b200_umma_selftest", "ttt_b200_wait_selftest", "ttt_b200_pack_tokens",
            "ttt_b200_unpack_tokens", "ttt_b200_eta_gate", "ttt_b200_eta_gate_backward", "ttt_b200_unpack_layernorm",
-           "ttt_b200_pack_layernorm_backward"]
+           "ttt_b200_pack_layernorm_backward",
+           "ttt_b200_short_conv", "ttt_b200_short_conv_backward", "ttt_b200_short_conv_step", "ttt_b200_short_conv_scratch_bytes",
+           "ttt_b200_ssm_scan", "ttt_b200_ssm_scan_backward", "ttt_b200_ssm_scan_step", "ttt_b200_ssm_scan_scratch_bytes",
+           "ttt_b200_norm_gate_residual", "ttt_b200_norm_gate_residual_backward", "ttt_b200_norm_gate_residual_scratch_bytes"]
 
 FLAG_SYNC = 1
 FLAG_TEST_LOST_LOAD = 2

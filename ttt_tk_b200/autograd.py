@@ -6,6 +6,7 @@ the state after the last mini-batch is returned so that sequences can be process
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .buffers import GRAD_NAMES, alloc_backward_buffers, alloc_checkpoints
 from .ops import ttt_backward, ttt_forward
@@ -151,3 +152,116 @@ def ttt_linear(XQ, XK, XV, last_eta, ttt_norm_weight, ttt_norm_bias, W1, b1, che
         checkpoint_group_size = max(1, int(math.sqrt(NC)))
     r = TTTLinearFunction.apply(XQ, XK, XV, last_eta, ttt_norm_weight, ttt_norm_bias, W1, b1, checkpoint_group_size)
     return r[0], tuple(r[1:])
+
+
+# ---- layer-side sequence operators (`ttt_tk_b200.ssm`, the block end of `ttt_tk_b200.glue`) ------------------------------------
+def _rows(t):
+    """With a contiguous last dimension (an upstream gradient can be an expanded number)."""
+    return t if t is None or t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
+
+
+def _whole(t, dtype=None):
+    return None if t is None else t.contiguous() if dtype is None else t.to(dtype).contiguous()
+
+
+class ShortConvFunction(torch.autograd.Function):
+    """(y, final state or None) = f(x, weight, bias, state, activation, lengths, heads, return_state)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, state, activation, lengths, heads, return_state):
+        from . import ssm
+        x, weight, bias, state = _rows(x), _whole(weight), _whole(bias), _whole(state)
+        r = ssm.short_conv(x, weight, bias, activation=activation, state=state, lengths=lengths, heads=heads, return_state=return_state)
+        ctx.save_for_backward(x, weight, bias, state, lengths)
+        ctx.kw = dict(activation=activation, heads=heads)
+        ctx.set_materialize_grads(False)
+        return r if return_state else (r, None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy, gf):
+        from . import ssm
+        x, weight, bias, state, lengths = ctx.saved_tensors
+        if gy is None:
+            B, T, D = x.shape
+            gy = x.new_zeros((B, D // 64, T // 64, 64, 64) if ctx.kw["heads"] else (B, T, D))
+        gy = _whole(gy) if ctx.kw["heads"] else _rows(gy)
+        g = ssm.short_conv_backward(gy, x, weight, bias, state=state, lengths=lengths, grad_final_state=_whole(gf), **ctx.kw)
+        return g + (None,) * 4
+
+
+def short_conv(x, weight, bias=None, *, activation=None, state=None, lengths=None, heads=False, return_state=False):
+    """Differentiable `ttt_tk_b200.ssm.short_conv`."""
+    y, end = ShortConvFunction.apply(x, weight, bias, state, activation, lengths, heads, return_state)
+    return (y, end) if return_state else y
+
+
+class SSMScanFunction(torch.autograd.Function):
+    """(y, final state or None) = f(x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state)."""
+
+    @staticmethod
+    def forward(ctx, x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state):
+        from . import ssm
+        x, dt, B, C = (_rows(t) for t in (x, dt, B, C))
+        A, D, dt_bias, state = (_whole(t) for t in (A, D, dt_bias, state))
+        keep = any(ctx.needs_input_grad)
+        r = ssm.ssm_scan(x, dt, A, B, C, D, dt_bias, softplus=softplus, state=state, lengths=lengths, return_state=return_state,
+                         return_checkpoints=keep)
+        r = r if isinstance(r, tuple) else (r,)
+        if keep:
+            ctx.save_for_backward(x, dt, A, B, C, D, dt_bias, lengths, r[-1])
+        ctx.softplus, ctx.has_state = softplus, state is not None
+        ctx.set_materialize_grads(False)
+        return r[0], r[1] if return_state else None
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy, gf):
+        from . import ssm
+        x, dt, A, B, C, D, dt_bias, lengths, ck = ctx.saved_tensors
+        gy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if gy is None else _rows(gy)
+        g = ssm.ssm_scan_backward(gy, x, dt, A, B, C, ck, D, dt_bias, softplus=ctx.softplus, lengths=lengths,
+                                  grad_final_state=_whole(gf))
+        return g[:7] + (g[7] if ctx.has_state else None,) + (None,) * 3
+
+
+def ssm_scan(x, dt, A, B, C, D=None, dt_bias=None, *, softplus=True, state=None, lengths=None, return_state=False):
+    """Differentiable `ttt_tk_b200.ssm.ssm_scan`; the checkpoints are kept for the backward."""
+    y, end = SSMScanFunction.apply(x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state)
+    return (y, end) if return_state else y
+
+
+class NormGateResidualFunction(torch.autograd.Function):
+    """(x, n or None) = f(o, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias, norm, activation, eps); o, residual and
+    gate [tokens, D]."""
+
+    @staticmethod
+    def forward(ctx, o, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias, norm, activation, eps):
+        from .glue import norm_gate_residual as run
+        o, residual, gate = (_rows(t) for t in (o, residual, gate))
+        weights = [_whole(t) for t in (post_weight, post_bias, scale, pre_weight, pre_bias)]
+        ctx.kw = dict(norm=norm, activation=activation, eps=eps)
+        x, n, stats = run(o, residual, gate, **dict(zip(_BLOCK_WEIGHTS, weights)), return_stats=True, **ctx.kw)
+        ctx.save_for_backward(o, residual, gate, stats, *weights)
+        ctx.set_materialize_grads(False)
+        return x, n
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gx, gn):
+        from .glue import norm_gate_residual_backward as run
+        o, residual, gate, stats, *weights = ctx.saved_tensors
+        if gx is None and gn is None:
+            return (None,) * 11
+        return run(_rows(gx), _rows(gn), o, stats, residual, gate, **dict(zip(_BLOCK_WEIGHTS, weights)), **ctx.kw) + (None,) * 3
+
+
+_BLOCK_WEIGHTS = ("post_weight", "post_bias", "scale", "pre_weight", "pre_bias")
+
+
+def norm_gate_residual(o, residual=None, gate=None, *, norm="rms", activation="silu", post_weight=None, post_bias=None, scale=None,
+                       pre_weight=None, pre_bias=None, eps=1e-6):
+    """Differentiable `ttt_tk_b200.glue.norm_gate_residual`."""
+    flat = [None if t is None else t.reshape(-1, t.shape[-1]) for t in (o, residual, gate)]
+    x, n = NormGateResidualFunction.apply(*flat, post_weight, post_bias, scale, pre_weight, pre_bias, norm, activation, eps)
+    return x.view(o.shape), None if n is None else n.view(o.shape)

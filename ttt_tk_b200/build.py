@@ -10,16 +10,18 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libttt_mlp_b200.so")
 SOURCES = ["ttt_capi.cu", "ttt_fwd_sm100.cu", "ttt_fwd_pair_sm100.cu", "ttt_bwd_sm100.cu", "ttt_bwd_pair_sm100.cu", "ttt_fwd_cluster_sm100.cu", "ttt_bwd_cluster_sm100.cu", "ttt_linear_fwd_sm100.cu", "ttt_linear_bwd_sm100.cu",
-           "ttt_layout.cu", "ttt_glue.cu", "umma_selftest.cu"]
-HEADERS = ["sm100_ptx.cuh", "ttt_device.cuh", "ttt_cluster.cuh", "ttt_internal.h", os.path.join("..", "..", "include", "ttt_mlp_b200.h")]
+           "ttt_layout.cu", "ttt_glue.cu", "ttt_short_conv.cu", "ttt_ssm_scan_sm100.cu", "ttt_block_norm.cu", "ttt_sum_parts.cu", "umma_selftest.cu"]
+HEADERS = ["sm100_ptx.cuh", "ttt_device.cuh", "ttt_cluster.cuh", "ttt_elem.cuh", "ttt_sum_parts.h", "ttt_internal.h", os.path.join("..", "..", "include", "ttt_mlp_b200.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-              "-shared", "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
+              "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
 
 
 def _nvcc():
@@ -41,14 +43,23 @@ def build(force=False, verbose=False):
     if not force and not needs_build():
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)
-    cmd = [_nvcc()] + NVCC_FLAGS + ["-o", LIB_PATH] + SOURCES + ["-lcudart"]
-    res = subprocess.run(cmd, cwd=CSRC, capture_output=True, text=True)
-    if verbose or res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed building libttt_mlp_b200.so")
+    logs = []
+
+    def run(args):
+        res = subprocess.run([_nvcc()] + NVCC_FLAGS + args, cwd=CSRC, capture_output=True, text=True)
+        logs.append(res.stdout + res.stderr)
+        if verbose or res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed building libttt_mlp_b200.so")
+
+    with tempfile.TemporaryDirectory() as tmp:       # the sources at the same time, then the link
+        objects = [os.path.join(tmp, s + ".o") for s in SOURCES]
+        with ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+            list(pool.map(run, [["-c", s, "-o", o] for s, o in zip(SOURCES, objects)]))
+        run(["-shared", "-o", LIB_PATH] + objects + ["-lcudart"])
     with open(os.path.join(LIB_DIR, "ptxas.log"), "w") as f:
-        f.write(res.stdout + res.stderr)
+        f.write("".join(logs))
     return LIB_PATH
 
 
@@ -61,6 +72,8 @@ EXT_SOURCE = os.path.join(CSRC, "test_time_training.cpp")
 
 HOST_NAME = "_ttt_host"                      # validation and launch for ttt_tk_b200.ops
 HOST_SOURCE = os.path.join(CSRC, "ttt_host.cpp")
+LAYER_HOST_NAME = "_ttt_layer_host"          # the same for the layer-side sequence operators
+LAYER_HOST_SOURCE = os.path.join(CSRC, "ttt_layer_host.cpp")
 
 
 def _module_path(name):
@@ -108,8 +121,9 @@ def _build_torch_module(name, source, out, force, verbose):
 
 
 def build_extension(force=False, verbose=False):
-    """Compile ttt_tk_b200/lib/test_time_training*.so and ttt_tk_b200/lib/_ttt_host*.so."""
-    _build_torch_module(HOST_NAME, HOST_SOURCE, _module_path(HOST_NAME), force, verbose)
+    """Compile ttt_tk_b200/lib/test_time_training*.so and the native host sides, _ttt_host*.so and _ttt_layer_host*.so."""
+    for name, source in ((HOST_NAME, HOST_SOURCE), (LAYER_HOST_NAME, LAYER_HOST_SOURCE)):
+        _build_torch_module(name, source, _module_path(name), force, verbose)
     return _build_torch_module(EXT_NAME, EXT_SOURCE, extension_path(), force, verbose)
 
 
@@ -129,12 +143,17 @@ def load_extension():
     return mod
 
 
-def load_host():
+def load_host(name=HOST_NAME, source=HOST_SOURCE):
     """Import and return the operators' native host side (building it, and the library, if it is out of date)."""
-    path = _module_path(HOST_NAME)
-    if _module_needs_build(HOST_SOURCE, path):
-        _build_torch_module(HOST_NAME, HOST_SOURCE, path, False, False)
-    return _load(HOST_NAME, path)
+    path = _module_path(name)
+    if _module_needs_build(source, path):
+        _build_torch_module(name, source, path, False, False)
+    return _load(name, path)
+
+
+def load_layer_host():
+    """The same for the layer-side sequence operators."""
+    return load_host(LAYER_HOST_NAME, LAYER_HOST_SOURCE)
 
 
 if __name__ == "__main__":

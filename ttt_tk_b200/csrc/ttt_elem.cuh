@@ -1,0 +1,118 @@
+// Element types, packed fp32 arithmetic and small helpers of the layer-side sequence operators (short convolution,
+// state space scan, block end).  Activations are bf16, fp16 or fp32; everything between reading and writing is fp32.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "ttt_internal.h"
+
+namespace ttt {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+
+template <class T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// Eight consecutive elements, 16-byte aligned: one or two 16-byte accesses.
+template <class T> __device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+  alignas(16) T v[8];
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] = to_f32(v[k]);
+}
+template <class T> __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+  alignas(16) T v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = from_f32<T>(f[k]);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
+}
+
+// Two fp32 operations in one instruction (sm_100): halves the issue slots of fp32-heavy loops.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// 16 bytes global -> shared without registers; `bytes` 0 fills with zeros and reads nothing.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
+  const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending> __device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+// Sums V values over the L lanes that differ in the bits kStride, 2 kStride, ... of the lane index, by exchanging halves:
+// V - V / L exchanges instead of V log2 L.  Value i of the sum ends in the lane whose index bits (lane / kStride) are
+// i / (V / L), as its element i % (V / L); with V < L in the L / V lanes whose index bits are i L / V and on.
+template <int V, int L, int kStride> __device__ __forceinline__ void spread_sum(float (&v)[V], int lane) {
+  int n = V;      // a compile-time value after unrolling
+#pragma unroll
+  for (int m = L / 2; m >= 1; m /= 2) {
+    if (n > 1) {
+      n /= 2;
+      const bool up = (lane / kStride) & m;
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i)
+        if (i < n) {
+          const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, give, m * kStride);
+        }
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], m * kStride);
+    }
+  }
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace ttt
+
+// Runs `body` with `Elem` as the activations' type.
+#define TTT_WITH_TYPE(dtype, body)                                     \
+  switch (dtype) {                                                     \
+    case TTT_B200_BF16: { using Elem = __nv_bfloat16; body; break; }   \
+    case TTT_B200_FP16: { using Elem = __half; body; break; }          \
+    default: { using Elem = float; body; break; }                      \
+  }

@@ -82,3 +82,42 @@ def pack_layernorm_backward(grad_y, out, gamma, stats):
     _lib.call_on(out.device, "ttt_b200_pack_layernorm_backward", grad_y.data_ptr(), out.data_ptr(), gamma.data_ptr(),
                  stats.data_ptr(), grad_out.data_ptr(), g_gamma.data_ptr(), g_beta.data_ptr(), B, T, H)
     return grad_out, g_gamma, g_beta
+
+
+_NORMS = {"rms": False, "layer": True}
+_GATES = {"silu": 1, "gelu": 2, "sigmoid": 3}
+
+
+def _kinds(norm, activation):
+    _need(norm in _NORMS, f"norm must be 'rms' or 'layer', got {norm!r}")
+    _need(activation in _GATES, f"activation must be 'silu', 'gelu' or 'sigmoid', got {activation!r}")
+    return _NORMS[norm], _GATES[activation]
+
+
+def norm_gate_residual(o, residual=None, gate=None, *, norm="rms", activation="silu", post_weight=None, post_bias=None, scale=None,
+                       pre_weight=None, pre_bias=None, eps=1e-6, return_stats=False):
+    """The end of a block and the start of the next in one pass over the tokens:
+
+        u = Norm(o) post_weight + post_bias;   x = residual + scale u act(gate);   n = Norm(x) pre_weight + pre_bias
+
+    `o` [..., D], the block's output (D <= 8192); `gate` like it; `residual` [..., D] of o's type or fp32; weights, biases and `scale`
+    fp32 [D].  `norm` "rms" (v / sqrt(mean(v^2) + eps)) or "layer"; `activation` "silu", "gelu" (tanh form) or "sigmoid".  Each
+    part is left out with its argument None: without `post_weight` u = o, without `residual` x is the rest, without `pre_weight`
+    there is no n.  The first block's norm is the call with `pre_weight` alone.  Types as in `ttt_tk_b200.ssm`; rows may be a slice of a
+    wider tensor.  Returns (x, n or None), with `return_stats` (x, n, stats): fp32 [tokens, 4] for the backward.  n is that of x
+    before x is rounded."""
+    from .ssm import _host
+    layer, act = _kinds(norm, activation)
+    x, n, stats = _host().block(o, residual, gate, layer, act, post_weight, post_bias, scale, pre_weight, pre_bias, eps, return_stats)
+    return (x, n, stats) if return_stats else (x, n)
+
+
+def norm_gate_residual_backward(grad_x, grad_n, o, stats, residual=None, gate=None, *, norm="rms", activation="silu", post_weight=None,
+                                post_bias=None, scale=None, pre_weight=None, pre_bias=None, eps=1e-6):
+    """Gradients of `norm_gate_residual` from its inputs and `stats`: (grad_o, grad_residual, grad_gate, grad_post_weight,
+    grad_post_bias, grad_scale, grad_pre_weight, grad_pre_bias), None where there is no such input.  `grad_x`, `grad_n`: as x
+    and n, either may be None."""
+    from .ssm import _host
+    layer, act = _kinds(norm, activation)
+    return _host().block_backward(grad_x, grad_n, o, stats, residual, gate, layer, act, post_weight, post_bias, scale, pre_weight,
+                                  pre_bias, eps)
