@@ -12,13 +12,14 @@
 // operations.  The exponentials leave at 16 per cycle and SM, four instructions' worth of issue slots each, so the arithmetic
 // is packed two to an instruction and the operands that lanes share (delta, B, C) come from shared memory in fp32.
 //
-// A thread owns four states of a channel (of two channels in the backward) and walks along the tokens; the LN lanes of a
+// A thread owns four states of two channels and walks along the tokens; the LN lanes of a
 // channel add their parts of y by exchanging halves over LN tokens at a time.  Channels, groups and sequences are independent.
 // Where they do not fill the GPU the sequence is split into chunks as well: a first kernel carries each chunk's state from
 // zero, a second one joins the chunks with exp(A sum delta), and the main kernel starts every chunk from its own state.  The
 // backward does the same from the other end.
 #include <algorithm>
 #include <cstdio>
+#include <type_traits>
 
 #include "ttt_elem.cuh"
 #include "ttt_sum_parts.h"
@@ -30,12 +31,12 @@ using namespace ttt;
 constexpr int kTile = TTT_B200_SCAN_INTERVAL;      // tokens staged at a time, and between two checkpoints
 static_assert(kTile == 16, "the kernels unroll over tiles of 16 tokens");
 
-// How a CTA is made up for LN lanes per channel (up to 4 LN states); CH channels per thread.
-template <int LN, int CH> struct Shape {
-  static constexpr int NP = 4 * LN;                                     // states, padded
-  static constexpr int TH = CH == 1 && LN > 4 ? 32 * LN : 128;
-  static constexpr int DC = TH / LN * CH;                               // channels of a CTA
-  static constexpr int CPW = 32 / LN;                                   // channels next to each other in a warp
+// How a CTA is made up for LN lanes per channel (up to 4 LN states); a thread has two channels.
+constexpr int TH = 128;
+template <int LN> struct Shape {
+  static constexpr int NP = 4 * LN;               // states, padded
+  static constexpr int DC = TH / LN * 2;          // channels of a CTA
+  static constexpr int CPW = 32 / LN;             // channels next to each other in a warp
 };
 
 struct Plan {
@@ -44,7 +45,7 @@ struct Plan {
   int chunk;      // tokens of a chunk, a multiple of kTile
   int chunks;
   int nck;        // checkpoints of a sequence
-  bool vec_x, vec_dt, vec_gy, vec_b, vec_c, vec_n;      // 16-byte rows; whole float4 of states
+  bool vec_x, vec_dt, vec_gy, vec_b, vec_c, vec_n, vec_part, pairs;      // 16-byte rows; whole float4 of states; outputs in pairs
   float* state;   // [B][chunks][D][N]: what a chunk starts from (backward: ends with)
   float* delta;   // [B][chunks][D]: sum of delta
   float* part_bc; // backward: [2][tiles][B][T][G][N]
@@ -71,7 +72,7 @@ struct Where {
 };
 
 // `rows` x `cols` elements -> [kTile][W], the rest zeros.
-template <class T, int W, int TH> __device__ __forceinline__ void stage(T* dst, const T* src, int64_t stride, int rows, int cols, bool vec) {
+template <class T, int W> __device__ __forceinline__ void stage(T* dst, const T* src, int64_t stride, int rows, int cols, bool vec) {
   constexpr int PV = 16 / sizeof(T), PR = W / PV;
   if (vec) {
 #pragma unroll
@@ -90,18 +91,81 @@ template <class T, int W, int TH> __device__ __forceinline__ void stage(T* dst, 
   }
 }
 
-// delta and its derivative.  log1p(e) of e = exp(-|v|) in (0, 1] as 2 atanh(e / (2 + e)), whose series in s^2 <= 1/9 is cut
-// where its next term is 2e-8 of the value; log(1 + e) itself would lose the small steps that matter most.
-__device__ __forceinline__ float2 softplus(float v) {
-  const float e = ex2(-fabsf(v) * kLog2e);
-  const float s = e * rcp(2.f + e), q = s * s;
-  float r = fmaf(q, 1.f / 13, 1.f / 11);
-  r = fmaf(q, r, 1.f / 9);
-  r = fmaf(q, r, 1.f / 7);
-  r = fmaf(q, r, 1.f / 5);
-  r = fmaf(q, r, 1.f / 3);
-  r = fmaf(q, r, 1.f);
-  return make_float2(fmaxf(v, 0.f) + 2.f * s * r, (v >= 0.f ? 1.f : e) * rcp(1.f + e));
+// delta of two values, and its derivative.  log1p(e) of e = exp(-|v|) in (0, 1] as 2 atanh(s), s = e / (2 + e), whose series in
+// s^2 <= 1/9 is cut where its next term is 2e-8 of the value; log(1 + e) itself would lose the small steps that matter most.
+__device__ __forceinline__ float2 softplus2(float2 v, float2* slope = nullptr) {
+  const float2 e = make_float2(ex2(-fabsf(v.x) * kLog2e), ex2(-fabsf(v.y) * kLog2e));
+  const float2 d = add2(e, both(2.f)), s = mul2(e, make_float2(rcp(d.x), rcp(d.y))), q = mul2(s, s);
+  float2 r = fma2(q, both(1.f / 13), both(1.f / 11));
+  r = fma2(q, r, both(1.f / 9));
+  r = fma2(q, r, both(1.f / 7));
+  r = fma2(q, r, both(1.f / 5));
+  r = fma2(q, r, both(1.f / 3));
+  r = fma2(q, r, both(1.f));
+  if (slope) {
+    const float2 o = add2(e, both(1.f));
+    *slope = mul2(make_float2(v.x >= 0.f ? 1.f : e.x, v.y >= 0.f ? 1.f : e.y), make_float2(rcp(o.x), rcp(o.y)));
+  }
+  return fma2(add2(s, s), r, make_float2(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f)));
+}
+
+// a or b, both worked out: a branch would keep the arithmetic in front of it from filling the gaps of the walk
+__device__ __forceinline__ float2 choose(bool first, float2 a, float2 b) {
+  float2 r;
+  asm("{ .reg .pred q; setp.ne.s32 q, %6, 0; selp.f32 %0, %2, %4, q; selp.f32 %1, %3, %5, q; }"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "r"(static_cast<int>(first)));
+  return r;
+}
+
+// two neighbouring elements in shared memory
+template <class T> __device__ __forceinline__ float2 pair(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    return *reinterpret_cast<const float2*>(p);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    return __half22float2(*reinterpret_cast<const __half2*>(p));
+  } else {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
+  }
+}
+// two neighbouring values of a row of an output: together where the host has found all its rows aligned for it
+template <class T> __device__ __forceinline__ void put_pair(T* p, float2 v, bool together, bool first, bool second) {
+  if (together) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p) = v;
+    else if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(p) = __floats2half2_rn(v.x, v.y);
+    else *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v.x, v.y);
+  } else {
+    if (first) p[0] = from_f32<T>(v.x);
+    if (second) p[1] = from_f32<T>(v.y);
+  }
+}
+// A thread's share of a tile [kTile][W] of B or C, on its way to fp32.
+template <class T, int W> struct Wide {
+  static constexpr int kPairs = kTile * W / 2, kMine = (kPairs + TH - 1) / TH;
+  float2 v[kMine];
+  __device__ __forceinline__ void load(const T* src) {
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      const int i = k * TH + threadIdx.x;
+      if (kPairs % TH == 0 || i < kPairs) v[k] = pair(src + 2 * i);
+    }
+  }
+  __device__ __forceinline__ void store(float* dst) const {
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      const int i = k * TH + threadIdx.x;
+      if (kPairs % TH == 0 || i < kPairs) *reinterpret_cast<float2*>(dst + 2 * i) = v[k];
+    }
+  }
+};
+
+// exp(delta A) of a pair of states, a2 = A log2(e).  The approximate exponential is 2e-8 low on average for the slow decays
+// (arguments of -0.5 to -0.001), which a state of a thousand tokens adds up; the offset takes the average to a quarter of
+// that and leaves exp(0) = 1, which tokens behind a sequence rely on.
+constexpr float kCentre = 2.2e-8f;
+__device__ __forceinline__ float2 decay(float delta, float2 a2) {
+  const float2 x = fma2(both(delta), a2, both(kCentre));
+  return make_float2(ex2(x.x), ex2(x.y));
 }
 
 // four states of a row [N] of fp32
@@ -128,162 +192,230 @@ __device__ __forceinline__ void split(const float4 v, float2 (&o)[2]) {
   o[1] = make_float2(v.z, v.w);
 }
 
+// A thread's two channels and four states.
+template <int LN> struct Mine {
+  int li, dl, n0, ch[2];
+  long row[2];
+  __device__ __forceinline__ Mine(const Where& w, int N) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    li = lane % LN;
+    dl = lane / LN;
+    n0 = 4 * li;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      ch[e] = (2 * warp + e) * Shape<LN>::CPW + dl;
+      row[e] = static_cast<long>(w.ch0 + ch[e]) * N;
+    }
+  }
+  // of a row [D][N]; a channel behind the last reads nothing
+  __device__ __forceinline__ void read(const float* p, const Where& w, int N, bool vec, float2 (&h)[2][2], float scale = 1.f) const {
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (ch[e] < w.cols) {
+        float v[4];
+        load_states(p + row[e], n0, N, vec, v);
+        h[e][0] = make_float2(v[0] * scale, v[1] * scale);
+        h[e][1] = make_float2(v[2] * scale, v[3] * scale);
+      }
+  }
+  __device__ __forceinline__ void write(float* p, const Where& w, int N, bool vec, const float2 (&h)[2][2]) const {
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (ch[e] < w.cols) {
+        const float v[4] = {h[e][0].x, h[e][0].y, h[e][1].x, h[e][1].y};
+        store_states(p + row[e], n0, N, vec, v);
+      }
+  }
+};
+
+// Where elements are worked on one by one a thread has two neighbouring channels, the same in every row.
+template <int DC> struct Pair {
+  int c, t0;      // channel; first row, the next ones kStep further
+  static constexpr int kStep = 2 * TH / DC, kRows = kTile / kStep;
+  bool first, second, together;
+  float2 bias, skip;
+  __device__ __forceinline__ Pair(const ttt_b200_scan_args& p, const Plan& q, const Where& w) {
+    c = threadIdx.x % (DC / 2) * 2;
+    t0 = threadIdx.x / (DC / 2);
+    first = c < w.cols;
+    second = c + 1 < w.cols;
+    together = second && q.pairs && w.ch0 % 2 == 0;
+    bias = skip = both(0.f);
+    if (p.dt_bias) bias = make_float2(first ? p.dt_bias[w.ch0 + c] : 0.f, second ? p.dt_bias[w.ch0 + c + 1] : 0.f);
+    if (p.Dskip) skip = make_float2(first ? p.Dskip[w.ch0 + c] : 0.f, second ? p.Dskip[w.ch0 + c + 1] : 0.f);
+  }
+};
+
 // ---- forward ---------------------------------------------------------------------------------------------------------
 template <class T, int LN> struct FwdSmem {
-  using S = Shape<LN, 1>;
+  using S = Shape<LN>;
   static constexpr int YW = S::DC + S::CPW;      // the y of a warp's channels and LN tokens in different banks
   alignas(16) T x[2][kTile * S::DC];
   alignas(16) T dt[2][kTile * S::DC];
   alignas(16) T b[2][kTile * S::NP];
   alignas(16) T c[2][kTile * S::NP];
-  alignas(16) float2 u[kTile * S::DC];      // delta, delta x
-  alignas(16) float fb[kTile * S::NP];
-  alignas(16) float fc[kTile * S::NP];
-  float y[kTile * YW];
+  alignas(16) float2 u[2][kTile * S::DC];      // delta, delta x
+  alignas(16) float fb[2][kTile * S::NP];
+  alignas(16) float fc[2][kTile * S::NP];
+  alignas(16) float y[2][kTile * YW];          // D x, then y
 };
 
-template <class T, int LN> __global__ void __launch_bounds__(Shape<LN, 1>::TH) scan_forward_kernel(const ttt_b200_scan_args p, const Plan q) {
-  using S = Shape<LN, 1>;
-  constexpr int TH = S::TH, DC = S::DC, NP = S::NP, U = LN < 4 ? 4 : LN, YW = FwdSmem<T, LN>::YW;
+// One barrier to a tile: between two of them the states walk over tile k, tile k + 1 goes from its copy to fp32 (in registers
+// first, so that its arithmetic fills the gaps of the walk), tile k - 1 leaves, and the copy of tile k + 2 is on its way.
+template <class T, int LN> __global__ void __launch_bounds__(TH, 4) scan_forward_kernel(const ttt_b200_scan_args p, const Plan q) {
+  using S = Shape<LN>;
+  constexpr int DC = S::DC, NP = S::NP, U = LN < 4 ? 4 : LN, YW = FwdSmem<T, LN>::YW;
   extern __shared__ __align__(16) unsigned char raw[];
   FwdSmem<T, LN>& m = *reinterpret_cast<FwdSmem<T, LN>*>(raw);
   const Where w(p, q, DC);
-  const int lane = threadIdx.x & 31, li = lane % LN, ch = threadIdx.x / LN, n0 = 4 * li;
-  const bool live = ch < w.cols;
-  const long row = static_cast<long>(w.ch0 + ch) * p.N, DN = static_cast<long>(p.D) * p.N;
+  const Mine<LN> me(w, p.N);
+  const Pair<DC> el(p, q, w);
+  const int lane = threadIdx.x & 31;
+  const long DN = static_cast<long>(p.D) * p.N;
 
-  float2 a2[2] = {}, h[2] = {};
-  if (live) {
-    float v[4];
-    load_states(p.A + row, n0, p.N, q.vec_n, v);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] *= kLog2e;
-    split(make_float4(v[0], v[1], v[2], v[3]), a2);
-    const float* from = q.chunks > 1 ? q.state + w.bc * DN : p.state ? p.state + w.b * DN : nullptr;
-    if (from) {
-      load_states(from + row, n0, p.N, q.vec_n, v);
-      split(make_float4(v[0], v[1], v[2], v[3]), h);
-    }
-  }
-  // this thread's channel where elements are worked on one at a time
-  const int ec = threadIdx.x % DC;
-  const float bias = p.dt_bias && ec < w.cols ? p.dt_bias[w.ch0 + ec] : 0.f;
-  const float skip = p.Dskip && ec < w.cols ? p.Dskip[w.ch0 + ec] : 0.f;
-
-  const int begin = w.c * q.chunk, end = min(begin + q.chunk, p.T);
+  const int begin = w.c * q.chunk, end = min(begin + q.chunk, p.T), stop = min(end, w.len);
+  const int count = stop > begin ? (stop - begin + kTile - 1) / kTile : 0;
   const T* xs = static_cast<const T*>(p.x) + w.b * p.x_stride[0] + w.ch0;
   const T* ds = static_cast<const T*>(p.dt) + w.b * p.dt_stride[0] + w.ch0;
   const T* bs = static_cast<const T*>(p.Bm) + w.b * p.B_stride[0] + w.g * p.B_stride[2];
   const T* cs = static_cast<const T*>(p.Cm) + w.b * p.C_stride[0] + w.g * p.C_stride[2];
-  T* ys = static_cast<T*>(p.y) + static_cast<long>(w.b) * p.T * p.D + w.ch0;
-  auto fetch = [&](int t0, int buf) {
-    const int rows = min(w.len - t0, kTile);
-    if (t0 < end && rows > 0) {
-      stage<T, DC, TH>(m.x[buf], xs + t0 * p.x_stride[1], p.x_stride[1], rows, w.cols, q.vec_x);
-      stage<T, DC, TH>(m.dt[buf], ds + t0 * p.dt_stride[1], p.dt_stride[1], rows, w.cols, q.vec_dt);
-      stage<T, NP, TH>(m.b[buf], bs + t0 * p.B_stride[1], p.B_stride[1], rows, p.N, q.vec_b);
-      stage<T, NP, TH>(m.c[buf], cs + t0 * p.C_stride[1], p.C_stride[1], rows, p.N, q.vec_c);
+  T* ys = static_cast<T*>(p.y) + static_cast<long>(w.b) * p.T * p.D + w.ch0 + el.c;
+  auto fetch = [&](int k) {
+    if (k < count) {
+      const int t0 = begin + k * kTile, rows = min(stop - t0, kTile), buf = k & 1;
+      stage<T, DC>(m.x[buf], xs + t0 * p.x_stride[1], p.x_stride[1], rows, w.cols, q.vec_x);
+      stage<T, DC>(m.dt[buf], ds + t0 * p.dt_stride[1], p.dt_stride[1], rows, w.cols, q.vec_dt);
+      stage<T, NP>(m.b[buf], bs + t0 * p.B_stride[1], p.B_stride[1], rows, p.N, q.vec_b);
+      stage<T, NP>(m.c[buf], cs + t0 * p.C_stride[1], p.C_stride[1], rows, p.N, q.vec_c);
     }
     cp_async_commit();
   };
-
-  fetch(begin, 0);
-  int buf = 0;
-  for (int t0 = begin; t0 < end; t0 += kTile, buf ^= 1) {
-    const int rows = min(w.len - t0, kTile);
-    if (rows <= 0) {      // behind the sequence: zeros, and the state stays
-      for (int i = threadIdx.x; i < kTile * DC; i += TH)
-        if (t0 + i / DC < end && ec < w.cols) ys[static_cast<long>(t0 + i / DC) * p.D + ec] = from_f32<T>(0.f);
-      continue;
-    }
-    cp_async_wait<0>();
-    __syncthreads();      // the tile has landed, and no thread reads the other buffer any more
-    fetch(t0 + kTile, buf ^ 1);
+  auto leave = [&](int k) {      // the y of a tile, with zeros behind the sequence
 #pragma unroll
-    for (int i0 = 0; i0 < kTile * DC; i0 += TH) {
-      const int i = i0 + threadIdx.x;
-      const float v = to_f32(m.dt[buf][i]) + bias;
-      const float d = i / DC < rows ? (p.softplus ? softplus(v).x : v) : 0.f;
-      m.u[i] = make_float2(d, d * to_f32(m.x[buf][i]));
+    for (int i = 0; i < el.kRows; ++i) {
+      const int r = el.t0 + i * el.kStep, t = begin + k * kTile + r;
+      if (t < end)
+        put_pair(ys + static_cast<long>(t) * p.D, t < stop ? *reinterpret_cast<const float2*>(m.y[k & 1] + r * YW + el.c) : both(0.f),
+                 el.together, el.first, el.second);
     }
-    for (int i = threadIdx.x; i < kTile * NP; i += TH) {
-      m.fb[i] = to_f32(m.b[buf][i]);
-      m.fc[i] = to_f32(m.c[buf][i]);
+  };
+  struct Next {      // a tile on its way to fp32
+    float2 x[Pair<DC>::kRows], dt[Pair<DC>::kRows];
+    Wide<T, NP> b, c;
+  };
+  auto pick_up = [&](int k, Next& n) {
+    const int buf = k & 1;
+#pragma unroll
+    for (int i = 0; i < el.kRows; ++i) {
+      const int at = (el.t0 + i * el.kStep) * DC + el.c;
+      n.x[i] = pair(m.x[buf] + at);
+      n.dt[i] = pair(m.dt[buf] + at);
     }
-    __syncthreads();
-    if (p.checkpoints && live) {
-      const float v[4] = {h[0].x, h[0].y, h[1].x, h[1].y};
-      store_states(p.checkpoints + (static_cast<long>(w.b) * q.nck + t0 / kTile) * DN + row, n0, p.N, q.vec_n, v);
+    n.b.load(m.b[buf]);
+    n.c.load(m.c[buf]);
+  };
+  auto work_out = [&](int k, Next& n) {
+    const int rows = stop - (begin + k * kTile);
+#pragma unroll
+    for (int i = 0; i < el.kRows; ++i) {
+      const float2 v = add2(n.dt[i], el.bias);
+      n.dt[i] = choose(p.softplus, softplus2(v), v);
+      n.dt[i] = choose(el.t0 + i * el.kStep < rows, n.dt[i], both(0.f));
     }
+  };
+  auto put_down = [&](int k, const Next& n) {
+    const int buf = k & 1;
+#pragma unroll
+    for (int i = 0; i < el.kRows; ++i) {
+      const int r = el.t0 + i * el.kStep;
+      const float2 dx = mul2(n.dt[i], n.x[i]);
+      *reinterpret_cast<float4*>(m.u[buf] + r * DC + el.c) = make_float4(n.dt[i].x, dx.x, n.dt[i].y, dx.y);
+      *reinterpret_cast<float2*>(m.y[buf] + r * YW + el.c) = mul2(el.skip, n.x[i]);
+    }
+    n.b.store(m.fb[buf]);
+    n.c.store(m.fc[buf]);
+  };
+
+  fetch(0);
+  float2 a2[2][2] = {}, h[2][2] = {};
+  me.read(p.A, w, p.N, q.vec_n, a2, kLog2e);
+  if (q.chunks > 1) me.read(q.state + w.bc * DN, w, p.N, q.vec_n, h);
+  else if (p.state) me.read(p.state + w.b * DN, w, p.N, q.vec_n, h);
+  Next next;
+  cp_async_wait<0>();
+  __syncthreads();
+  fetch(1);
+  if (count > 0) {
+    pick_up(0, next);
+    work_out(0, next);
+    put_down(0, next);
+  }
+  for (int k = 0; k < count; ++k) {
+    cp_async_wait<0>();
+    __syncthreads();      // tile k + 1 has landed, tile k is ready, and no thread is behind
+    fetch(k + 2);
+    if (k > 0) leave(k - 1);
+    if (p.checkpoints) me.write(p.checkpoints + (static_cast<long>(w.b) * q.nck + begin / kTile + k) * DN, w, p.N, q.vec_n, h);
+    pick_up(k + 1, next);      // (behind the last tile: what is there, for nothing)
+    work_out(k + 1, next);
+    const float2* u = m.u[k & 1];
+    const float *fb = m.fb[k & 1] + me.n0, *fc = m.fc[k & 1] + me.n0;
+    float* y = m.y[k & 1];
 #pragma unroll
     for (int s = 0; s < kTile; s += U) {
-      float acc[U];
+      float acc[2][U];
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int t = s + k;
-        const float2 du = m.u[t * DC + ch];
+      for (int i = 0; i < U; ++i) {
+        const int t = s + i;
         float2 b[2], c[2];
-        split(*reinterpret_cast<const float4*>(m.fb + t * NP + n0), b);
-        split(*reinterpret_cast<const float4*>(m.fc + t * NP + n0), c);
-        float2 y;
+        split(*reinterpret_cast<const float4*>(fb + t * NP), b);
+        split(*reinterpret_cast<const float4*>(fc + t * NP), c);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float2 e = mul2(both(du.x), a2[j]);
-          h[j] = fma2(make_float2(ex2(e.x), ex2(e.y)), h[j], mul2(both(du.y), b[j]));
-          y = j ? fma2(h[j], c[j], y) : mul2(h[j], c[j]);
+        for (int e = 0; e < 2; ++e) {
+          const float2 du = u[t * DC + me.ch[e]];
+          float2 o;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            h[e][j] = fma2(decay(du.x, a2[e][j]), h[e][j], mul2(both(du.y), b[j]));
+            o = j ? fma2(h[e][j], c[j], o) : mul2(h[e][j], c[j]);
+          }
+          acc[e][i] = o.x + o.y;
         }
-        acc[k] = y.x + y.y;
       }
-      spread_sum<U, LN, 1>(acc, lane);
 #pragma unroll
-      for (int k = 0; k < U / LN; ++k) m.y[(s + li * (U / LN) + k) * YW + ch] = acc[k];
-    }
-    __syncthreads();
+      for (int e = 0; e < 2; ++e) {
+        spread_sum<U, LN, 1>(acc[e], lane);
 #pragma unroll
-    for (int i0 = 0; i0 < kTile * DC; i0 += TH) {
-      const int t = (i0 + threadIdx.x) / DC;
-      if (t0 + t < end && ec < w.cols) {
-        const float y = t < rows ? fmaf(skip, to_f32(m.x[buf][t * DC + ec]), m.y[t * YW + ec]) : 0.f;
-        ys[static_cast<long>(t0 + t) * p.D + ec] = from_f32<T>(y);
+        for (int i = 0; i < U / LN; ++i) y[(s + me.li * (U / LN) + i) * YW + me.ch[e]] += acc[e][i];
       }
     }
+    put_down(k + 1, next);
   }
-  if (p.final_state && w.c == q.chunks - 1 && live) {
-    const float v[4] = {h[0].x, h[0].y, h[1].x, h[1].y};
-    store_states(p.final_state + w.b * DN + row, n0, p.N, q.vec_n, v);
-  }
+  __syncthreads();
+  if (count > 0) leave(count - 1);
+  for (int k = count; begin + k * kTile < end; ++k) leave(k);
+  if (p.final_state && w.c == q.chunks - 1) me.write(p.final_state + w.b * DN, w, p.N, q.vec_n, h);
 }
 
 // ---- a chunk's state by itself, from zero: forwards h <- a h + delta x B; backwards (kRev) c <- a (c + dy C) -----------
 template <class T, int LN> struct StateSmem {
-  using S = Shape<LN, 1>;
+  using S = Shape<LN>;
   alignas(16) T v[2][kTile * S::DC];      // x or dy
   alignas(16) T dt[2][kTile * S::DC];
   alignas(16) T n[2][kTile * S::NP];      // B or C
-  alignas(16) float2 u[kTile * S::DC];
-  alignas(16) float fn[kTile * S::NP];
+  alignas(16) float2 u[2][kTile * S::DC];
+  alignas(16) float fn[2][kTile * S::NP];
 };
 
-template <class T, int LN, bool kRev>
-__global__ void __launch_bounds__(Shape<LN, 1>::TH) scan_state_kernel(const ttt_b200_scan_args p, const Plan q) {
-  using S = Shape<LN, 1>;
-  constexpr int TH = S::TH, DC = S::DC, NP = S::NP;
+template <class T, int LN, bool kRev> __global__ void __launch_bounds__(TH, 4) scan_state_kernel(const ttt_b200_scan_args p, const Plan q) {
+  using S = Shape<LN>;
+  constexpr int DC = S::DC, NP = S::NP;
   extern __shared__ __align__(16) unsigned char raw[];
   StateSmem<T, LN>& m = *reinterpret_cast<StateSmem<T, LN>*>(raw);
   const Where w(p, q, DC);
-  const int li = threadIdx.x % LN, ch = threadIdx.x / LN, n0 = 4 * li;
-  const bool live = ch < w.cols;
-  const long row = static_cast<long>(w.ch0 + ch) * p.N, DN = static_cast<long>(p.D) * p.N;
-  float2 a2[2] = {}, h[2] = {};
-  if (live) {
-    float v[4];
-    load_states(p.A + row, n0, p.N, q.vec_n, v);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] *= kLog2e;
-    split(make_float4(v[0], v[1], v[2], v[3]), a2);
-  }
-  const int ec = threadIdx.x % DC;
-  const float bias = p.dt_bias && ec < w.cols ? p.dt_bias[w.ch0 + ec] : 0.f;
+  const Mine<LN> me(w, p.N);
+  const Pair<DC> el(p, q, w);
+  const long DN = static_cast<long>(p.D) * p.N;
   const int64_t* vst = kRev ? p.gy_stride : p.x_stride;
   const int64_t* nst = kRev ? p.C_stride : p.B_stride;
   const T* vs = static_cast<const T*>(kRev ? p.grad_y : p.x) + w.b * vst[0] + w.ch0;
@@ -292,51 +424,90 @@ __global__ void __launch_bounds__(Shape<LN, 1>::TH) scan_state_kernel(const ttt_
   const int begin = w.c * q.chunk, end = min(begin + q.chunk, w.len);
   const int count = end > begin ? (end - begin + kTile - 1) / kTile : 0;
   auto at = [&](int k) { return begin + (kRev ? count - 1 - k : k) * kTile; };
-  auto fetch = [&](int k, int buf) {
+  auto fetch = [&](int k) {
     if (k < count) {
-      const int t0 = at(k), rows = min(end - t0, kTile);
-      stage<T, DC, TH>(m.v[buf], vs + t0 * vst[1], vst[1], rows, w.cols, kRev ? q.vec_gy : q.vec_x);
-      stage<T, DC, TH>(m.dt[buf], ds + t0 * p.dt_stride[1], p.dt_stride[1], rows, w.cols, q.vec_dt);
-      stage<T, NP, TH>(m.n[buf], ns + t0 * nst[1], nst[1], rows, p.N, kRev ? q.vec_c : q.vec_b);
+      const int t0 = at(k), rows = min(end - t0, kTile), buf = k & 1;
+      stage<T, DC>(m.v[buf], vs + t0 * vst[1], vst[1], rows, w.cols, kRev ? q.vec_gy : q.vec_x);
+      stage<T, DC>(m.dt[buf], ds + t0 * p.dt_stride[1], p.dt_stride[1], rows, w.cols, q.vec_dt);
+      stage<T, NP>(m.n[buf], ns + t0 * nst[1], nst[1], rows, p.N, kRev ? q.vec_c : q.vec_b);
     }
     cp_async_commit();
   };
-  float total = 0.f;
-  fetch(0, 0);
+  struct Next {
+    float2 v[Pair<DC>::kRows], dt[Pair<DC>::kRows];
+    Wide<T, NP> n;
+  };
+  auto pick_up = [&](int k, Next& n) {
+    const int buf = k & 1;
+#pragma unroll
+    for (int i = 0; i < el.kRows; ++i) {
+      const int o = (el.t0 + i * el.kStep) * DC + el.c;
+      n.v[i] = pair(m.v[buf] + o);
+      n.dt[i] = pair(m.dt[buf] + o);
+    }
+    n.n.load(m.n[buf]);
+  };
+  auto work_out = [&](int k, Next& n) {
+    const int rows = end - at(k);
+#pragma unroll
+    for (int i = 0; i < el.kRows; ++i) {
+      const float2 v = add2(n.dt[i], el.bias);
+      n.dt[i] = choose(p.softplus, softplus2(v), v);
+      n.dt[i] = choose(el.t0 + i * el.kStep < rows, n.dt[i], both(0.f));
+      if (!kRev) n.v[i] = mul2(n.dt[i], n.v[i]);
+    }
+  };
+  auto put_down = [&](int k, const Next& n) {
+    const int buf = k & 1;
+#pragma unroll
+    for (int i = 0; i < el.kRows; ++i)
+      *reinterpret_cast<float4*>(m.u[buf] + (el.t0 + i * el.kStep) * DC + el.c) = make_float4(n.dt[i].x, n.v[i].x, n.dt[i].y, n.v[i].y);
+    n.n.store(m.fn[buf]);
+  };
+
+  fetch(0);
+  float2 a2[2][2] = {}, h[2][2] = {};
+  me.read(p.A, w, p.N, q.vec_n, a2, kLog2e);
+  float2 total = both(0.f);
+  Next next;
+  cp_async_wait<0>();
+  __syncthreads();
+  fetch(1);
+  if (count > 0) {
+    pick_up(0, next);
+    work_out(0, next);
+    put_down(0, next);
+  }
   for (int k = 0; k < count; ++k) {
-    const int buf = k & 1, rows = min(end - at(k), kTile);
     cp_async_wait<0>();
     __syncthreads();
-    fetch(k + 1, buf ^ 1);
+    fetch(k + 2);
+    pick_up(k + 1, next);      // (behind the last tile: what is there, for nothing)
+    work_out(k + 1, next);
+    const float2* u = m.u[k & 1];
+    const float* fn = m.fn[k & 1] + me.n0;
 #pragma unroll
-    for (int i0 = 0; i0 < kTile * DC; i0 += TH) {
-      const int i = i0 + threadIdx.x;
-      const float v = to_f32(m.dt[buf][i]) + bias;
-      const float d = i / DC < rows ? (p.softplus ? softplus(v).x : v) : 0.f;
-      m.u[i] = make_float2(d, kRev ? to_f32(m.v[buf][i]) : d * to_f32(m.v[buf][i]));
-    }
-    for (int i = threadIdx.x; i < kTile * NP; i += TH) m.fn[i] = to_f32(m.n[buf][i]);
-    __syncthreads();
-#pragma unroll 4
     for (int s = 0; s < kTile; ++s) {
       const int t = kRev ? kTile - 1 - s : s;
-      const float2 du = m.u[t * DC + ch];
       float2 b[2];
-      split(*reinterpret_cast<const float4*>(m.fn + t * NP + n0), b);
-      total += du.x;
+      split(*reinterpret_cast<const float4*>(fn + t * NP), b);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float2 e = mul2(both(du.x), a2[j]);
-        const float2 f = make_float2(ex2(e.x), ex2(e.y));
-        h[j] = kRev ? mul2(f, fma2(both(du.y), b[j], h[j])) : fma2(f, h[j], mul2(both(du.y), b[j]));
+      for (int e = 0; e < 2; ++e) {
+        const float2 du = u[t * DC + me.ch[e]];
+        (e ? total.y : total.x) += du.x;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float2 f = decay(du.x, a2[e][j]);
+          h[e][j] = kRev ? mul2(f, fma2(both(du.y), b[j], h[e][j])) : fma2(f, h[e][j], mul2(both(du.y), b[j]));
+        }
       }
     }
+    put_down(k + 1, next);
   }
-  if (live) {
-    const float v[4] = {h[0].x, h[0].y, h[1].x, h[1].y};
-    store_states(q.state + w.bc * DN + row, n0, p.N, q.vec_n, v);
-    if (li == 0) q.delta[w.bc * p.D + w.ch0 + ch] = total;
-  }
+  me.write(q.state + w.bc * DN, w, p.N, q.vec_n, h);
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (me.li == 0 && me.ch[e] < w.cols) q.delta[w.bc * p.D + w.ch0 + me.ch[e]] = e ? total.y : total.x;
 }
 
 // The chunks' own states -> the states that they start from (kRev: that they end with), in place, in the order of time.
@@ -355,7 +526,7 @@ template <bool kRev> __global__ void __launch_bounds__(256) scan_join_kernel(con
     for (int k = 0; k < kAhead; ++k) {
       const long c = b * q.chunks + (kRev ? q.chunks - 1 - min(c0 + k, q.chunks - 1) : min(c0 + k, q.chunks - 1));
       s[k] = q.state[c * DN + dn];
-      f[k] = ex2(a2 * q.delta[c * p.D + d]);
+      f[k] = ex2(fmaf(a2, q.delta[c * p.D + d], kCentre));
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
@@ -371,53 +542,36 @@ template <bool kRev> __global__ void __launch_bounds__(256) scan_join_kernel(con
 constexpr int kSub = 4;      // tokens whose states and factors are in registers at a time
 
 template <class T, int LN> struct BwdSmem {
-  using S = Shape<LN, 2>;
-  static constexpr int OW = S::DC + S::CPW;
+  using S = Shape<LN>;
   alignas(16) T x[2][kTile * S::DC];
   alignas(16) T dt[2][kTile * S::DC];
   alignas(16) T gy[2][kTile * S::DC];
   alignas(16) T b[2][kTile * S::NP];
   alignas(16) T c[2][kTile * S::NP];
-  alignas(16) float4 u[kTile * S::DC];      // delta, delta x, dy, d delta / d dt
+  alignas(16) float4 u[kTile * S::DC];      // delta, delta x, dy, d delta / d dt; then sum_n dh A exp(delta A) h (in base 2) and
+                                            // sum_n dh B in the place of delta x and dy, which only the warp of the channel reads
   alignas(16) float fb[kTile * S::NP];
   alignas(16) float fc[kTile * S::NP];
-  alignas(16) float4 start[kTile / kSub][2][S::TH];      // each thread's states at the starts of the runs of kSub tokens
-  float bc[kTile][S::TH / 32][2 * S::NP];     // each warp's part of dB and dC
-  float o[2][kTile * OW];                   // sum_n dh A exp(delta A) h (in base 2), sum_n dh B
+  alignas(16) float4 start[kTile / kSub - 1][2][TH];      // each thread's states at the starts of the later runs of kSub tokens
+  alignas(16) float bc[kTile][TH / 32][2 * S::NP];     // each warp's part of dB and dC
 };
 
 template <class T, int LN>
-__global__ void __launch_bounds__(Shape<LN, 2>::TH, 3) scan_backward_kernel(const ttt_b200_scan_args p, const Plan q) {
-  using S = Shape<LN, 2>;
-  constexpr int TH = S::TH, DC = S::DC, NP = S::NP, CPW = S::CPW, OW = BwdSmem<T, LN>::OW, ND = 32 / LN;
+__global__ void __launch_bounds__(TH, 3) scan_backward_kernel(const ttt_b200_scan_args p, const Plan q) {
+  using S = Shape<LN>;
+  constexpr int DC = S::DC, NP = S::NP, ND = 32 / LN;
   extern __shared__ __align__(16) unsigned char raw[];
   BwdSmem<T, LN>& m = *reinterpret_cast<BwdSmem<T, LN>*>(raw);
   const Where w(p, q, DC);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, li = lane % LN, dl = lane / LN, n0 = 4 * li;
-  const int ch[2] = {warp * 2 * CPW + dl, warp * 2 * CPW + CPW + dl};
+  const Mine<LN> me(w, p.N);
+  const Pair<DC> el(p, q, w);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long DN = static_cast<long>(p.D) * p.N;
-  long row[2];
   float2 a2[2][2] = {}, carry[2][2] = {}, da[2][2] = {};
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    row[e] = static_cast<long>(w.ch0 + ch[e]) * p.N;
-    if (ch[e] >= w.cols) continue;
-    float v[4];
-    load_states(p.A + row[e], n0, p.N, q.vec_n, v);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] *= kLog2e;
-    split(make_float4(v[0], v[1], v[2], v[3]), a2[e]);
-    const float* from = q.chunks > 1 ? q.state + w.bc * DN : p.grad_final_state ? p.grad_final_state + w.b * DN : nullptr;
-    if (from) {
-      load_states(from + row[e], n0, p.N, q.vec_n, v);
-      split(make_float4(v[0], v[1], v[2], v[3]), carry[e]);
-    }
-  }
-  const int ec = threadIdx.x % DC;
-  const bool elive = ec < w.cols;
-  const float bias = p.dt_bias && elive ? p.dt_bias[w.ch0 + ec] : 0.f;
-  const float skip = p.Dskip && elive ? p.Dskip[w.ch0 + ec] : 0.f;
-  float sum_d = 0.f, sum_bias = 0.f;
+  me.read(p.A, w, p.N, q.vec_n, a2, kLog2e);
+  if (q.chunks > 1) me.read(q.state + w.bc * DN, w, p.N, q.vec_n, carry);
+  else if (p.grad_final_state) me.read(p.grad_final_state + w.b * DN, w, p.N, q.vec_n, carry);
+  float2 sum_d = both(0.f), sum_bias = both(0.f);
 
   const int begin = w.c * q.chunk, end = min(begin + q.chunk, p.T);
   const T* xs = static_cast<const T*>(p.x) + w.b * p.x_stride[0] + w.ch0;
@@ -425,7 +579,7 @@ __global__ void __launch_bounds__(Shape<LN, 2>::TH, 3) scan_backward_kernel(cons
   const T* gs = static_cast<const T*>(p.grad_y) + w.b * p.gy_stride[0] + w.ch0;
   const T* bs = static_cast<const T*>(p.Bm) + w.b * p.B_stride[0] + w.g * p.B_stride[2];
   const T* cs = static_cast<const T*>(p.Cm) + w.b * p.C_stride[0] + w.g * p.C_stride[2];
-  const long out0 = static_cast<long>(w.b) * p.T * p.D + w.ch0;
+  const long out0 = static_cast<long>(w.b) * p.T * p.D + w.ch0 + el.c;
   T* gxs = static_cast<T*>(p.grad_x) + out0;
   T* gds = static_cast<T*>(p.grad_dt) + out0;
   const long GN = static_cast<long>(p.G) * p.N, BTGN = static_cast<long>(p.B) * p.T * GN;
@@ -434,11 +588,11 @@ __global__ void __launch_bounds__(Shape<LN, 2>::TH, 3) scan_backward_kernel(cons
   auto fetch = [&](int t0, int buf) {
     const int rows = min(w.len - t0, kTile);
     if (t0 >= begin && rows > 0) {
-      stage<T, DC, TH>(m.x[buf], xs + t0 * p.x_stride[1], p.x_stride[1], rows, w.cols, q.vec_x);
-      stage<T, DC, TH>(m.dt[buf], ds + t0 * p.dt_stride[1], p.dt_stride[1], rows, w.cols, q.vec_dt);
-      stage<T, DC, TH>(m.gy[buf], gs + t0 * p.gy_stride[1], p.gy_stride[1], rows, w.cols, q.vec_gy);
-      stage<T, NP, TH>(m.b[buf], bs + t0 * p.B_stride[1], p.B_stride[1], rows, p.N, q.vec_b);
-      stage<T, NP, TH>(m.c[buf], cs + t0 * p.C_stride[1], p.C_stride[1], rows, p.N, q.vec_c);
+      stage<T, DC>(m.x[buf], xs + t0 * p.x_stride[1], p.x_stride[1], rows, w.cols, q.vec_x);
+      stage<T, DC>(m.dt[buf], ds + t0 * p.dt_stride[1], p.dt_stride[1], rows, w.cols, q.vec_dt);
+      stage<T, DC>(m.gy[buf], gs + t0 * p.gy_stride[1], p.gy_stride[1], rows, w.cols, q.vec_gy);
+      stage<T, NP>(m.b[buf], bs + t0 * p.B_stride[1], p.B_stride[1], rows, p.N, q.vec_b);
+      stage<T, NP>(m.c[buf], cs + t0 * p.C_stride[1], p.C_stride[1], rows, p.N, q.vec_c);
     }
     cp_async_commit();
   };
@@ -449,10 +603,11 @@ __global__ void __launch_bounds__(Shape<LN, 2>::TH, 3) scan_backward_kernel(cons
   for (int t0 = last; t0 >= begin; t0 -= kTile, buf ^= 1) {
     const int rows = min(w.len - t0, kTile);
     if (rows <= 0) {      // behind the sequence: zeros, and the gradient of the state passes through
-      for (int i = threadIdx.x; i < kTile * DC; i += TH)
-        if (t0 + i / DC < end && elive) {
-          gxs[static_cast<long>(t0 + i / DC) * p.D + ec] = from_f32<T>(0.f);
-          gds[static_cast<long>(t0 + i / DC) * p.D + ec] = from_f32<T>(0.f);
+#pragma unroll
+      for (int t = el.t0; t < kTile; t += el.kStep)
+        if (t0 + t < end) {
+          put_pair(gxs + static_cast<long>(t0 + t) * p.D, both(0.f), el.together, el.first, el.second);
+          put_pair(gds + static_cast<long>(t0 + t) * p.D, both(0.f), el.together, el.first, el.second);
         }
       for (int i = threadIdx.x; i < kTile * NP; i += TH)
         if (t0 + i / NP < end && i % NP < p.N) {
@@ -463,70 +618,68 @@ __global__ void __launch_bounds__(Shape<LN, 2>::TH, 3) scan_backward_kernel(cons
       continue;
     }
     float2 h0[2][2] = {};      // the state before the tile
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (ch[e] < w.cols) {
-        float v[4];
-        load_states(p.checkpoints + (static_cast<long>(w.b) * q.nck + t0 / kTile) * DN + row[e], n0, p.N, q.vec_n, v);
-        split(make_float4(v[0], v[1], v[2], v[3]), h0[e]);
-      }
+    me.read(p.checkpoints + (static_cast<long>(w.b) * q.nck + t0 / kTile) * DN, w, p.N, q.vec_n, h0);
     cp_async_wait<0>();
     __syncthreads();      // the tile has landed, and no thread reads the other buffer any more
     fetch(t0 - kTile, buf ^ 1);
 #pragma unroll
-    for (int i0 = 0; i0 < kTile * DC; i0 += TH) {
-      const int i = i0 + threadIdx.x;
-      const float v = to_f32(m.dt[buf][i]) + bias;
-      float2 d = p.softplus ? softplus(v) : make_float2(v, 1.f);
-      if (i / DC >= rows) d = make_float2(0.f, 0.f);
-      m.u[i] = make_float4(d.x, d.x * to_f32(m.x[buf][i]), to_f32(m.gy[buf][i]), d.y);
+    for (int t = el.t0; t < kTile; t += el.kStep) {
+      const float2 x = pair(m.x[buf] + t * DC + el.c), v = add2(pair(m.dt[buf] + t * DC + el.c), el.bias);
+      const float2 gy = pair(m.gy[buf] + t * DC + el.c);
+      float2 slope = both(1.f), d = p.softplus ? softplus2(v, &slope) : v;
+      if (t >= rows) d = slope = both(0.f);
+      const float2 dx = mul2(d, x);
+      m.u[t * DC + el.c] = make_float4(d.x, dx.x, gy.x, slope.x);
+      m.u[t * DC + el.c + 1] = make_float4(d.y, dx.y, gy.y, slope.y);
     }
-    for (int i = threadIdx.x; i < kTile * NP; i += TH) {
-      m.fb[i] = to_f32(m.b[buf][i]);
-      m.fc[i] = to_f32(m.c[buf][i]);
-    }
+    Wide<T, NP> wide;
+    wide.load(m.b[buf]);
+    wide.store(m.fb);
+    wide.load(m.c[buf]);
+    wide.store(m.fc);
     __syncthreads();
     {      // the states at the starts of the runs
       float2 h[2][2] = {{h0[0][0], h0[0][1]}, {h0[1][0], h0[1][1]}};
 #pragma unroll 1
-      for (int s = 0;; ++s) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) m.start[s][e][threadIdx.x] = make_float4(h[e][0].x, h[e][0].y, h[e][1].x, h[e][1].y);
-        if (s == kTile / kSub - 1) break;
+      for (int s = 0; s < kTile / kSub - 1; ++s) {
 #pragma unroll
         for (int k = 0; k < kSub; ++k) {
           const int t = s * kSub + k;
           float2 b[2];
-          split(*reinterpret_cast<const float4*>(m.fb + t * NP + n0), b);
+          split(*reinterpret_cast<const float4*>(m.fb + t * NP + me.n0), b);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float4 u = m.u[t * DC + ch[e]];
+            const float2 u = *reinterpret_cast<const float2*>(m.u + t * DC + me.ch[e]);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const float2 x = mul2(both(u.x), a2[e][j]);
-              h[e][j] = fma2(make_float2(ex2(x.x), ex2(x.y)), h[e][j], mul2(both(u.y), b[j]));
+              h[e][j] = fma2(decay(u.x, a2[e][j]), h[e][j], mul2(both(u.y), b[j]));
             }
           }
         }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) m.start[s][e][threadIdx.x] = make_float4(h[e][0].x, h[e][0].y, h[e][1].x, h[e][1].y);
       }
     }
 #pragma unroll 1
     for (int s = kTile / kSub - 1; s >= 0; --s) {
       float2 f[2][kSub][2], h[2][kSub + 1][2];      // factors; states before token k of the run
 #pragma unroll
-      for (int e = 0; e < 2; ++e) split(m.start[s][e][threadIdx.x], h[e][0]);
+      for (int e = 0; e < 2; ++e) {
+        h[e][0][0] = h0[e][0];
+        h[e][0][1] = h0[e][1];
+        if (s > 0) split(m.start[s - 1][e][threadIdx.x], h[e][0]);
+      }
 #pragma unroll
       for (int k = 0; k < kSub; ++k) {
         const int t = s * kSub + k;
         float2 b[2];
-        split(*reinterpret_cast<const float4*>(m.fb + t * NP + n0), b);
+        split(*reinterpret_cast<const float4*>(m.fb + t * NP + me.n0), b);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float4 u = m.u[t * DC + ch[e]];
+          const float2 u = *reinterpret_cast<const float2*>(m.u + t * DC + me.ch[e]);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float2 x = mul2(both(u.x), a2[e][j]);
-            f[e][k][j] = make_float2(ex2(x.x), ex2(x.y));
+            f[e][k][j] = decay(u.x, a2[e][j]);
             h[e][k + 1][j] = fma2(f[e][k][j], h[e][k][j], mul2(both(u.y), b[j]));
           }
         }
@@ -535,18 +688,19 @@ __global__ void __launch_bounds__(Shape<LN, 2>::TH, 3) scan_backward_kernel(cons
       for (int k = kSub - 1; k >= 0; --k) {
         const int t = s * kSub + k;
         float2 b[2], c[2], vb[2], vc[2];
-        split(*reinterpret_cast<const float4*>(m.fb + t * NP + n0), b);
-        split(*reinterpret_cast<const float4*>(m.fc + t * NP + n0), c);
+        split(*reinterpret_cast<const float4*>(m.fb + t * NP + me.n0), b);
+        split(*reinterpret_cast<const float4*>(m.fc + t * NP + me.n0), c);
         float o[4];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float4 u = m.u[t * DC + ch[e]];
+          const float2 u = *reinterpret_cast<const float2*>(m.u + t * DC + me.ch[e]);
+          const float gy = m.u[t * DC + me.ch[e]].z;
           float2 qa, gb;
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float2 g = fma2(both(u.z), c[j], carry[e][j]);
+            const float2 g = fma2(both(gy), c[j], carry[e][j]);
             vb[j] = e ? fma2(both(u.y), g, vb[j]) : mul2(both(u.y), g);
-            vc[j] = e ? fma2(both(u.z), h[e][k + 1][j], vc[j]) : mul2(both(u.z), h[e][k + 1][j]);
+            vc[j] = e ? fma2(both(gy), h[e][k + 1][j], vc[j]) : mul2(both(gy), h[e][k + 1][j]);
             gb = j ? fma2(g, b[j], gb) : mul2(g, b[j]);
             carry[e][j] = mul2(f[e][k][j], g);
             const float2 r = mul2(carry[e][j], h[e][k][j]);
@@ -561,12 +715,12 @@ __global__ void __launch_bounds__(Shape<LN, 2>::TH, 3) scan_backward_kernel(cons
         if constexpr (LN <= 4) {
 #pragma unroll
           for (int r = 0; r < 4 / LN; ++r) {
-            const int i = li * (4 / LN) + r;
-            m.o[i >> 1][t * OW + (i & 1 ? ch[1] : ch[0])] = o[r];
+            const int i = me.li * (4 / LN) + r;
+            reinterpret_cast<float*>(m.u + t * DC + (i & 1 ? me.ch[1] : me.ch[0]))[1 + (i >> 1)] = o[r];
           }
         } else {
-          const int i = li / (LN / 4);
-          if (li % (LN / 4) == 0) m.o[i >> 1][t * OW + (i & 1 ? ch[1] : ch[0])] = o[0];
+          const int i = me.li / (LN / 4);
+          if (me.li % (LN / 4) == 0) reinterpret_cast<float*>(m.u + t * DC + (i & 1 ? me.ch[1] : me.ch[0]))[1 + (i >> 1)] = o[0];
         }
         // dB and dC: over the warp's channels
         float v[8] = {vb[0].x, vb[0].y, vb[1].x, vb[1].y, vc[0].x, vc[0].y, vc[1].x, vc[1].y};
@@ -574,64 +728,61 @@ __global__ void __launch_bounds__(Shape<LN, 2>::TH, 3) scan_backward_kernel(cons
         if constexpr (ND <= 8) {
 #pragma unroll
           for (int r = 0; r < 8 / ND; ++r) {
-            const int i = dl * (8 / ND) + r;
-            m.bc[t][warp][(i >> 2) * NP + n0 + (i & 3)] = v[r];
+            const int i = me.dl * (8 / ND) + r;
+            m.bc[t][warp][(i >> 2) * NP + me.n0 + (i & 3)] = v[r];
           }
         } else {
-          const int i = dl / (ND / 8);
-          if (dl % (ND / 8) == 0) m.bc[t][warp][(i >> 2) * NP + n0 + (i & 3)] = v[0];
+          const int i = me.dl / (ND / 8);
+          if (me.dl % (ND / 8) == 0) m.bc[t][warp][(i >> 2) * NP + me.n0 + (i & 3)] = v[0];
         }
       }
     }
     __syncthreads();
 #pragma unroll
-    for (int i0 = 0; i0 < kTile * DC; i0 += TH) {
-      const int t = (i0 + threadIdx.x) / DC;
-      if (t0 + t < end && elive) {
-        const float4 u = m.u[t * DC + ec];
-        const float x = to_f32(m.x[buf][t * DC + ec]), gb = m.o[1][t * OW + ec];
-        const float gx = fmaf(u.x, gb, skip * u.z), gd = u.w * fmaf(kLn2, m.o[0][t * OW + ec], x * gb);
-        const bool in = t < rows;
-        gxs[static_cast<long>(t0 + t) * p.D + ec] = from_f32<T>(in ? gx : 0.f);
-        gds[static_cast<long>(t0 + t) * p.D + ec] = from_f32<T>(in ? gd : 0.f);
-        if (in) {
-          sum_d = fmaf(u.z, x, sum_d);
-          sum_bias += gd;
+    for (int t = el.t0; t < kTile; t += el.kStep) {
+      if (t0 + t >= end) break;
+      const float4 u0 = m.u[t * DC + el.c], u1 = m.u[t * DC + el.c + 1];
+      const float2 d = make_float2(u0.x, u1.x), slope = make_float2(u0.w, u1.w), qa = make_float2(u0.y, u1.y), gb = make_float2(u0.z, u1.z);
+      const float2 x = pair(m.x[buf] + t * DC + el.c), gy = pair(m.gy[buf] + t * DC + el.c);
+      const float2 gx = fma2(d, gb, mul2(el.skip, gy)), gd = mul2(slope, fma2(both(kLn2), qa, mul2(x, gb)));
+      const bool in = t < rows;
+      put_pair(gxs + static_cast<long>(t0 + t) * p.D, in ? gx : both(0.f), el.together, el.first, el.second);
+      put_pair(gds + static_cast<long>(t0 + t) * p.D, in ? gd : both(0.f), el.together, el.first, el.second);
+      if (in) {
+        sum_d = fma2(gy, x, sum_d);
+        sum_bias = add2(sum_bias, gd);
+      }
+    }
+    for (int i = threadIdx.x; i < kTile * NP / 2; i += TH) {      // four values of dB or dC, over the warps
+      const int t = i / (NP / 2), k = i % (NP / 2) * 4, n = k % NP;
+      if (t0 + t >= end || n >= p.N) continue;
+      float v[4] = {};
+      if (t < rows) {
+#pragma unroll
+        for (int r = 0; r < TH / 32; ++r) {
+          const float4 o = *reinterpret_cast<const float4*>(&m.bc[t][r][k]);
+          v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
         }
       }
-    }
-    for (int i = threadIdx.x; i < kTile * NP * 2; i += TH) {
-      const int t = i / (2 * NP), k = i % (2 * NP);
-      float v = 0.f;
-#pragma unroll
-      for (int r = 0; r < S::TH / 32; ++r) v += m.bc[t][r][k];
-      const int n = k % NP;
-      if (t0 + t < end && n < p.N) (k < NP ? pb : pc)[(t0 + t) * GN + n] = t < rows ? v : 0.f;
+      store_states((k < NP ? pb : pc) + (t0 + t) * GN, n, p.N, q.vec_part, v);
     }
   }
-#pragma unroll
-  for (int e = 0; e < 2; ++e)
-    if (ch[e] < w.cols) {
-      const float v[4] = {da[e][0].x, da[e][0].y, da[e][1].x, da[e][1].y};
-      store_states(q.part_a + w.bc * DN + row[e], n0, p.N, q.vec_n, v);
-      if (w.c == 0 && p.grad_state) {
-        const float g[4] = {carry[e][0].x, carry[e][0].y, carry[e][1].x, carry[e][1].y};
-        store_states(p.grad_state + w.b * DN + row[e], n0, p.N, q.vec_n, g);
-      }
-    }
+  me.write(q.part_a + w.bc * DN, w, p.N, q.vec_n, da);
+  if (w.c == 0 && p.grad_state) me.write(p.grad_state + w.b * DN, w, p.N, q.vec_n, carry);
   __syncthreads();
-  float* red = m.o[0];      // [TH] pairs: what the threads of a channel have summed
+  float2* red = reinterpret_cast<float2*>(m.u);      // [2][TH]: what the threads of a pair of channels have summed
   red[threadIdx.x] = sum_d;
   red[TH + threadIdx.x] = sum_bias;
   __syncthreads();
-  if (threadIdx.x < DC && elive) {
-    for (int r = threadIdx.x + DC; r < TH; r += DC) {
-      sum_d += red[r];
-      sum_bias += red[TH + r];
+  if (threadIdx.x < DC / 2) {
+    for (int r = threadIdx.x + DC / 2; r < TH; r += DC / 2) {
+      sum_d = add2(sum_d, red[r]);
+      sum_bias = add2(sum_bias, red[TH + r]);
     }
-    const long BCD = static_cast<long>(p.B) * q.chunks * p.D, i = w.bc * p.D + w.ch0 + ec;
-    q.part_d[i] = sum_d;
-    q.part_d[BCD + i] = sum_bias;
+    const long BCD = static_cast<long>(p.B) * q.chunks * p.D;
+    float* to = q.part_d + w.bc * p.D + w.ch0 + el.c;
+    put_pair(to, sum_d, el.together, el.first, el.second);
+    put_pair(to + BCD, sum_bias, el.together, el.first, el.second);
   }
 }
 
@@ -671,13 +822,13 @@ template <class T, int LN> __global__ void __launch_bounds__(128) scan_step_kern
     if (live) {
       x = to_f32(static_cast<const T*>(p.x)[b * p.x_stride[0] + d]);
       const float v = to_f32(static_cast<const T*>(p.dt)[b * p.dt_stride[0] + d]) + bias;
-      const float dl = p.softplus ? softplus(v).x : v;
+      const float dl = p.softplus ? softplus2(both(v)).x : v;
       const T* bs = static_cast<const T*>(p.Bm) + b * p.B_stride[0] + g * p.B_stride[2];
       const T* cs = static_cast<const T*>(p.Cm) + b * p.C_stride[0] + g * p.C_stride[2];
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         if (n0 + k < p.N) {
-          h[k] = fmaf(ex2(dl * (a[k] * kLog2e)), h[k], dl * x * to_f32(bs[n0 + k]));
+          h[k] = fmaf(ex2(fmaf(dl, a[k] * kLog2e, kCentre)), h[k], dl * x * to_f32(bs[n0 + k]));
           y = fmaf(h[k], to_f32(cs[n0 + k]), y);
         }
     }
@@ -710,19 +861,20 @@ int check(const ttt_b200_scan_args* p) {
   return TTT_B200_OK;
 }
 
-// Tokens to a chunk: see the measurements at the forward's and backward's launch.
+// Tokens to a chunk.  Without chunks the kernels need an SM's worth of CTAs next to each other to cover their latencies; with them
+// every token's exponentials are worked out once more, by the state kernel.  Measured at 2048 tokens of N = 16, us without / with
+// chunks: forward of 96 CTAs 244 / 164, of 256 301 / 393; backward of 96 CTAs 680 / 350, of 256 915 / 850, of 384 1160 / 1390.  So
+// the forward is split below one CTA to an SM, the backward below two, into some eight to an SM (four to sixteen are within 5 %), and
+// short sequences into single tiles (512 tokens of 256 channels, 32 chunks: 62 -> 20); the joining kernel walks over the chunks, at
+// most 128 of them.
 void plan_chunks(Plan& q, const ttt_b200_scan_args& p, bool backward) {
-  const int LN = lanes_of(p.N), ch = backward ? 2 : 1;
-  const int th = ch == 1 && LN > 4 ? 32 * LN : 128;
-  const int dc = th / LN * ch;
+  const int dc = TH / lanes_of(p.N) * 2;
   q.per = p.D / p.G;
   q.tiles = (q.per + dc - 1) / dc;
   q.nck = (p.T + kTile - 1) / kTile;
-  const long ctas = static_cast<long>(p.B) * p.G * q.tiles, warps = ctas * (th / 32);
-  const long want = static_cast<long>(sm_count()) * (backward ? 8 : 16);
+  const long ctas = static_cast<long>(p.B) * p.G * q.tiles, sms = sm_count();
   long chunks = 1;
-  if (warps * 2 < want) chunks = std::min<long>((want + warps - 1) / warps, (q.nck + 3) / 4);
-  chunks = std::max<long>(1, std::min<long>(chunks, 64));
+  if (ctas < (backward ? 2 : 1) * sms) chunks = std::max<long>(1, std::min<long>({(8 * sms + ctas - 1) / ctas, q.nck, 128}));
   const int per = static_cast<int>((q.nck + chunks - 1) / chunks);
   q.chunk = std::max(per, 1) * kTile;
   q.chunks = std::max(1, (p.T + q.chunk - 1) / q.chunk);
@@ -769,7 +921,10 @@ int prepare(Plan& q, const ttt_b200_scan_args& p, bool backward) {
   q.vec_gy = backward && rows16(p.grad_y, p.gy_stride, 2, es, inner);
   q.vec_b = rows16(p.Bm, p.B_stride, 3, es, p.N);
   q.vec_c = rows16(p.Cm, p.C_stride, 3, es, p.N);
-  q.vec_n = p.N % 4 == 0;
+  q.vec_n = q.vec_part = p.N % 4 == 0;      // (the scratch is aligned)
+  q.pairs = p.D % 2 == 0;
+  for (const void* o : {static_cast<const void*>(p.y), static_cast<const void*>(p.grad_x), static_cast<const void*>(p.grad_dt)})
+    q.pairs = q.pairs && reinterpret_cast<uintptr_t>(o) % (2 * es) == 0;
   for (const void* s : {static_cast<const void*>(p.A), static_cast<const void*>(p.state), static_cast<const void*>(p.final_state),
                         static_cast<const void*>(p.checkpoints), static_cast<const void*>(p.grad_final_state),
                         static_cast<const void*>(p.grad_state)})
@@ -785,37 +940,34 @@ int launched(const char* what) {
   return ttt_set_error(TTT_B200_ERR_LAUNCH, buf);
 }
 
-template <class K> int launch(K kernel, size_t smem, long grid, int threads, cudaStream_t s, const ttt_b200_scan_args& p, const Plan& q) {
+template <class K> int launch(K kernel, size_t smem, long grid, cudaStream_t s, const ttt_b200_scan_args& p, const Plan& q) {
   if (grid > 0x7fffffffL) return fail("ssm scan: too many CTAs");
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return ttt_set_error(TTT_B200_ERR_LAUNCH, cudaGetErrorString(e));
   }
-  kernel<<<static_cast<unsigned>(grid), threads, smem, s>>>(p, q);
+  kernel<<<static_cast<unsigned>(grid), TH, smem, s>>>(p, q);
   return launched("ssm scan");
 }
 
 template <class T, int LN> int forward(const ttt_b200_scan_args& p, const Plan& q, cudaStream_t s) {
   const long grid = static_cast<long>(p.B) * q.chunks * p.G * q.tiles;
   if (q.chunks > 1) {
-    if (int rc = launch(scan_state_kernel<T, LN, false>, sizeof(StateSmem<T, LN>), grid, Shape<LN, 1>::TH, s, p, q)) return rc;
+    if (int rc = launch(scan_state_kernel<T, LN, false>, sizeof(StateSmem<T, LN>), grid, s, p, q)) return rc;
     const long n = static_cast<long>(p.B) * p.D * p.N;
     scan_join_kernel<false><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(p, q);
   }
-  return launch(scan_forward_kernel<T, LN>, sizeof(FwdSmem<T, LN>), grid, Shape<LN, 1>::TH, s, p, q);
+  return launch(scan_forward_kernel<T, LN>, sizeof(FwdSmem<T, LN>), grid, s, p, q);
 }
 
 template <class T, int LN> int backward(const ttt_b200_scan_args& p, const Plan& q, cudaStream_t s) {
+  const long grid = static_cast<long>(p.B) * q.chunks * p.G * q.tiles;
   if (q.chunks > 1) {
-    Plan f = q;      // one channel per thread here: other tiles of the same chunks
-    f.tiles = (q.per + Shape<LN, 1>::DC - 1) / Shape<LN, 1>::DC;
-    const long grid = static_cast<long>(p.B) * q.chunks * p.G * f.tiles;
-    if (int rc = launch(scan_state_kernel<T, LN, true>, sizeof(StateSmem<T, LN>), grid, Shape<LN, 1>::TH, s, p, f)) return rc;
+    if (int rc = launch(scan_state_kernel<T, LN, true>, sizeof(StateSmem<T, LN>), grid, s, p, q)) return rc;
     const long n = static_cast<long>(p.B) * p.D * p.N;
     scan_join_kernel<true><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(p, q);
   }
-  const long grid = static_cast<long>(p.B) * q.chunks * p.G * q.tiles;
-  if (int rc = launch(scan_backward_kernel<T, LN>, sizeof(BwdSmem<T, LN>), grid, Shape<LN, 2>::TH, s, p, q)) return rc;
+  if (int rc = launch(scan_backward_kernel<T, LN>, sizeof(BwdSmem<T, LN>), grid, s, p, q)) return rc;
   const long BTGN = static_cast<long>(p.B) * p.T * p.G * p.N, DN = static_cast<long>(p.D) * p.N, BCD = static_cast<long>(p.B) * q.chunks * p.D;
   const int bc = p.B * q.chunks;
   const ttt_sum_job jobs[] = {{q.part_bc, p.grad_B, BTGN, BTGN, q.tiles, p.dtype, 0},
