@@ -3,12 +3,14 @@
 //   y[b][t][d] = act(bias[d] + sum_k w[d][k] x[b][t - K + 1 + k][d])
 //   g = dy act'(pre);  dx[s] = sum_k w[d][k] g[s + K - 1 - k];  dw[d][k] = sum_t g[t] x[t - K + 1 + k];  db = sum_t g[t]
 //
-// Bound by memory: 2 K operations per value that is read and written once.  A thread owns V neighbouring channels (eight, as
-// 16-byte accesses, or one where rows do not start on 16-byte boundaries) and walks along a run of tokens with the last K - 1
-// inputs in registers, so that an input is read once per run; the K - 1 in front of a run come from the cache.  The backward
+// Bound by memory: 2 K operations per value that is read and written once.  A thread owns two neighbouring channels
+// (one where rows do not start on a pair's boundary) and walks along a run of tokens with the last K - 1 inputs in registers, so that
+// an input is read once per run; the K - 1 in front of a run come from the cache.  Eight rows are requested ahead of the eight that
+// are worked on: a warp's row is 128 bytes, and it takes some 40 KB in flight to keep an SM's share of the memory busy.  The backward
 // keeps the last K values of g as well and leaves dx with a delay of K - 1 tokens.
 #include <algorithm>
 #include <cstdio>
+#include <type_traits>
 
 #include "ttt_elem.cuh"
 #include "ttt_sum_parts.h"
@@ -20,209 +22,345 @@ using namespace ttt;
 struct Plan {
   int groups;      // V channels each
   int run;         // tokens of a thread
-  int runs;        // of a sequence; backward: of a CTA's warps together
+  int runs;        // CTAs along a sequence, kWarps runs each
   long y_batch, y_head, y_token;      // strides of y (dy with heads)
   float* part;     // backward: [B][runs][K + 1][D]
 };
 
-template <class T, int V> __device__ __forceinline__ void load(const T* p, float (&f)[V]) {
-  if constexpr (V == 8) {
-    load8(p, f);
-  } else {
-    static_assert(V == 1, "one channel or eight");
-    f[0] = to_f32(*p);
-  }
-}
-template <class T, int V> __device__ __forceinline__ void store(T* p, const float (&f)[V]) {
-  if constexpr (V == 8) store8(p, f);
-  else *p = from_f32<T>(f[0]);
-}
-template <int V> __device__ __forceinline__ void clear(float (&f)[V]) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) f[i] = 0.f;
-}
+constexpr int kWarps = 4;      // of a CTA: runs of tokens after one another, of the same 32 V channels
 
-// weights [k][channel] and bias of a thread's channels
-template <int K, int V> __device__ __forceinline__ void load_weights(const ttt_b200_conv_args& p, int d, float (&w)[K][V], float (&bias)[V]) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) w[k][i] = p.weight[static_cast<long>(d + i) * K + k];
-    bias[i] = p.bias ? p.bias[d + i] : 0.f;
+// What a thread works on.
+struct At {
+  int tile, group, row, b, run;      // `row`: the CTA among those of its channels, over all sequences
+  __device__ __forceinline__ explicit At(const Plan& q) {
+    const int tiles = (q.groups + 31) / 32;
+    tile = blockIdx.x % tiles;
+    row = blockIdx.x / tiles;
+    b = row / q.runs;
+    run = row % q.runs * kWarps + threadIdx.x / 32;
+    group = tile * 32 + threadIdx.x % 32;
   }
+};
+
+// V = 1 or 2 neighbouring channels of a thread: their values as float or float2, and as they lie in memory.
+template <int V> struct Channels;
+template <> struct Channels<1> {
+  using F = float;
+};
+template <> struct Channels<2> {
+  using F = float2;
+};
+template <class T, int V> struct alignas(V * sizeof(T)) Raw {
+  T v[V];
+};
+__device__ __forceinline__ float mac(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float2 mac(float2 a, float2 b, float2 c) { return fma2(a, b, c); }
+__device__ __forceinline__ float times(float a, float b) { return a * b; }
+__device__ __forceinline__ float2 times(float2 a, float2 b) { return mul2(a, b); }
+__device__ __forceinline__ float plus(float a, float b) { return a + b; }
+__device__ __forceinline__ float2 plus(float2 a, float2 b) { return add2(a, b); }
+template <class F> __device__ __forceinline__ F all(float v) {
+  if constexpr (sizeof(F) == 8) return both(v);
+  else return v;
+}
+// 1 / (1 + exp(-v)); far on the left exp is infinite and the result 0
+__device__ __forceinline__ float sigmoid(float v) { return rcp(1.f + ex2(-v * kLog2e)); }
+__device__ __forceinline__ float2 sigmoid(float2 v) {
+  const float2 x = mul2(v, both(-kLog2e)), d = add2(make_float2(ex2(x.x), ex2(x.y)), both(1.f));
+  return make_float2(rcp(d.x), rcp(d.y));
+}
+template <class T, int V> __device__ __forceinline__ typename Channels<V>::F wide(const Raw<T, V>& r) {
+  if constexpr (V == 1) return to_f32(r.v[0]);
+  else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __bfloat1622float2(reinterpret_cast<const __nv_bfloat162&>(r));
+  else if constexpr (std::is_same<T, __half>::value) return __half22float2(reinterpret_cast<const __half2&>(r));
+  else return make_float2(r.v[0], r.v[1]);
+}
+template <class T, int V> __device__ __forceinline__ Raw<T, V> narrow(typename Channels<V>::F f) {
+  Raw<T, V> r;
+  if constexpr (V == 1) r.v[0] = from_f32<T>(f);
+  else if constexpr (std::is_same<T, __nv_bfloat16>::value) reinterpret_cast<__nv_bfloat162&>(r) = __float22bfloat162_rn(f);
+  else if constexpr (std::is_same<T, __half>::value) reinterpret_cast<__half2&>(r) = __float22half2_rn(f);
+  else r.v[0] = f.x, r.v[1] = f.y;
+  return r;
+}
+template <class T, int V> __device__ __forceinline__ Raw<T, V> nothing() { return narrow<T, V>(all<typename Channels<V>::F>(0.f)); }
+template <class T, int V> __device__ __forceinline__ Raw<T, V> load(const T* p) { return *reinterpret_cast<const Raw<T, V>*>(p); }
+template <class T, int V> __device__ __forceinline__ void store(T* p, Raw<T, V> r) { *reinterpret_cast<Raw<T, V>*>(p) = r; }
+
+// weights [k] and bias of a thread's channels, whose K V weights are next to each other
+template <int K, int V>
+__device__ __forceinline__ void load_weights(const ttt_b200_conv_args& p, int d, typename Channels<V>::F (&w)[K], typename Channels<V>::F& bias) {
+  float f[K * V];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const Raw<float, V> r = load<float, V>(p.weight + static_cast<long>(d) * K + k * V);
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[k * V + i] = r.v[i];
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if constexpr (V == 2) w[k] = make_float2(f[k], f[K + k]);
+    else w[k] = f[k];
+  }
+  bias = p.bias ? wide<float, V>(load<float, V>(p.bias + d)) : all<typename Channels<V>::F>(0.f);
 }
 
 // The input at position t, which may lie in front of the sequence (the state) but not behind it.
-template <class T, int K, int V> __device__ __forceinline__ void input(const ttt_b200_conv_args& p, int b, int d, int t, float (&f)[V]) {
-  if (t >= 0) load<T, V>(static_cast<const T*>(p.x) + b * p.x_stride[0] + t * p.x_stride[1] + d, f);
-  else if (p.state && t >= 1 - K) load<T, V>(static_cast<const T*>(p.state) + (static_cast<long>(b) * (K - 1) + t + K - 1) * p.D + d, f);
-  else clear<V>(f);
+template <class T, int K, int V> __device__ __forceinline__ Raw<T, V> input(const ttt_b200_conv_args& p, int b, int d, int t) {
+  if (t >= 0) return load<T, V>(static_cast<const T*>(p.x) + b * p.x_stride[0] + t * p.x_stride[1] + d);
+  if (p.state && t >= 1 - K) return load<T, V>(static_cast<const T*>(p.state) + (static_cast<long>(b) * (K - 1) + t + K - 1) * p.D + d);
+  return nothing<T, V>();
 }
-
-__device__ __forceinline__ float sigmoid(float v) { return rcp(1.f + ex2(fminf(-v * kLog2e, 126.f))); }
 
 __device__ __forceinline__ int length_of(const ttt_b200_conv_args& p, int b) {
   return p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
 }
 
-template <class T, int K, int V> __global__ void __launch_bounds__(128) conv_forward_kernel(const ttt_b200_conv_args p, const Plan q) {
-  const long id = static_cast<long>(blockIdx.x) * 128 + threadIdx.x;
-  const int d = static_cast<int>(id % q.groups) * V;
-  const long bt = id / q.groups;
-  const int b = static_cast<int>(bt / q.runs), r = static_cast<int>(bt % q.runs);
-  if (b >= p.B) return;
-  const int len = length_of(p, b), begin = r * q.run, end = min(begin + q.run, p.T);
-  float w[K][V], bias[V], x[K][V];
+constexpr int U = 8;      // tokens of a block, which are requested together
+
+// The rows of a tensor that a warp walks along, a block of U tokens at a time, requested ahead of the block that is worked on; those
+// from `stop` on are not read.  Pairs of channels go through a ring in shared memory (asynchronous 16-byte copies: what is
+// in flight costs no registers), single channels through registers.  All lanes of a warp call `start` and `turn` together.
+template <class T, int V> struct Rows;
+template <class T> struct Rows<T, 2> {
+  static constexpr int kSlots = sizeof(T) == 2 ? 4 : 2, kWidth = 64, kBytes = kSlots * U * kWidth * sizeof(T);
+  static constexpr int kPiece = 16 / sizeof(T), kPieces = kWidth / kPiece, kMine = U * kPieces / 32;      // pieces of a block, of a lane
+  T* ring;
+  const T *from, *next;      // of this lane's first piece: the first block's and the next one's
+  int64_t stride;
+  int bytes, t, stop, block;      // bytes of a piece; first token of the next block to request
+  __device__ __forceinline__ Rows(void* smem, const T* tile, int64_t stride, int cols) : ring(static_cast<T*>(smem)), from(tile), stride(stride) {
+    const int c = (threadIdx.x & 31) % kPieces * kPiece, n = min(max(cols - c, 0), kPiece);
+    bytes = n * static_cast<int>(sizeof(T));
+    if (n > 0) from += c;
+  }
+  __device__ __forceinline__ void issue(int slot) {
+    if (t < stop) {
+      const int u = (threadIdx.x & 31) / kPieces;
+      T* to = ring + slot * (U * kWidth) + (threadIdx.x & 31) * kPiece;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const bool in = t + u + i * (32 / kPieces) < stop;
+        cp_async16(to + i * 32 * kPiece, in ? next + i * (32 / kPieces) * stride : from, in ? bytes : 0);
+      }
+      next += U * stride;
+      t += U;
+    }
+    cp_async_commit();
+  }
+  __device__ __forceinline__ void start(int begin, int stop_) {
+    t = begin;
+    stop = stop_;
+    block = -1;
+    next = from + (begin + (threadIdx.x & 31) / kPieces) * stride;
+#pragma unroll
+    for (int k = 0; k < kSlots - 1; ++k) issue(k);
+  }
+  // to the next block
+  __device__ __forceinline__ void turn() {
+    ++block;
+    cp_async_wait<kSlots - 2>();
+    __syncwarp();      // the block has landed for all lanes, and all are through with the one before
+    issue((block + kSlots - 1) % kSlots);
+  }
+  // row u of the block; `at`: where there are that many before `stop`
+  __device__ __forceinline__ Raw<T, 2> at(int u) const { return load<T, 2>(ring + (block % kSlots * U + u) * kWidth + 2 * (threadIdx.x & 31)); }
+};
+template <class T> struct Rows<T, 1> {
+  static constexpr int kBytes = 0;
+  const T* next;      // of this lane's channel (behind the last channel: of the tile's first)
+  int64_t stride;
+  int t, stop;
+  Raw<T, 1> now[U], then[U];
+  __device__ __forceinline__ Rows(void*, const T* tile, int64_t stride, int cols)
+      : next(tile + (static_cast<int>(threadIdx.x & 31) < cols ? threadIdx.x & 31 : 0)), stride(stride) {}
+  __device__ __forceinline__ void ask() {
+    if (t + U <= stop) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) then[u] = load<T, 1>(next + u * stride);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (t + u < stop) then[u] = load<T, 1>(next + u * stride);
+    }
+    next += U * stride;
+    t += U;
+  }
+  __device__ __forceinline__ void start(int begin, int stop_) {
+    t = begin;
+    stop = stop_;
+    next += begin * stride;
+    ask();
+  }
+  __device__ __forceinline__ void turn() {
+#pragma unroll
+    for (int u = 0; u < U; ++u) now[u] = then[u];
+    ask();
+  }
+  __device__ __forceinline__ Raw<T, 1> at(int u) const { return now[u]; }
+};
+
+template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(32 * kWarps) conv_forward_kernel(const ttt_b200_conv_args p, const Plan q) {
+  using F = typename Channels<V>::F;
+  __shared__ __align__(16) unsigned char rings[kWarps][Rows<T, V>::kBytes + 16];
+  const At at(q);
+  const int b = at.b, d0 = at.tile * 32 * V, begin = min(at.run * q.run, p.T), end = min(begin + q.run, p.T);
+  if (begin == end) return;
+  const bool mine = at.group < q.groups;
+  const int d = mine ? at.group * V : d0;      // (a lane behind the last channel reads the tile's first)
+  const int len = length_of(p, b), stop = min(len, end);
+  Rows<T, V> rows(rings[threadIdx.x / 32], static_cast<const T*>(p.x) + b * p.x_stride[0] + d0, p.x_stride[1], p.D - d0);
+  rows.start(begin, stop);
+  T* y = static_cast<T*>(p.y) + b * q.y_batch + d / 64 * q.y_head + d % 64;
+  F w[K], bias, x[K];
   load_weights<K, V>(p, d, w, bias);
 #pragma unroll
   for (int k = 0; k < K - 1; ++k) {
-    if (begin - K + 1 + k < len) input<T, K, V>(p, b, d, begin - K + 1 + k, x[k]);
-    else clear<V>(x[k]);
+    const int t = begin - K + 1 + k;
+    x[k] = wide<T, V>(t < len ? input<T, K, V>(p, b, d, t) : nothing<T, V>());
   }
-  T* y = static_cast<T*>(p.y) + b * q.y_batch + d / 64 * q.y_head + d % 64;
-  constexpr int U = 4;      // rows requested together
+  auto one = [&](const Raw<T, V>& row) {
+    x[K - 1] = wide<T, V>(row);
+    F v = bias;
+#pragma unroll
+    for (int k = 0; k < K; ++k) v = mac(w[k], x[k], v);
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) x[k] = x[k + 1];
+    return kSilu ? times(v, sigmoid(v)) : v;
+  };
   for (int t0 = begin; t0 < end; t0 += U) {
-    float in[U][V];
+    rows.turn();
+    T* to = y + t0 * q.y_token;
+    if (t0 + U <= stop) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (t0 + u < min(len, end)) load<T, V>(static_cast<const T*>(p.x) + b * p.x_stride[0] + (t0 + u) * p.x_stride[1] + d, in[u]);
-      else clear<V>(in[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int t = t0 + u;
-      float o[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        x[K - 1][i] = in[u][i];
-        float v = bias[i];
-#pragma unroll
-        for (int k = 0; k < K; ++k) v = fmaf(w[k][i], x[k][i], v);
-        if (p.activation == TTT_B200_ACT_SILU) v *= sigmoid(v);
-        o[i] = t < len ? v : 0.f;
-#pragma unroll
-        for (int k = 0; k < K - 1; ++k) x[k][i] = x[k + 1][i];
+      for (int u = 0; u < U; ++u) {
+        const Raw<T, V> o = narrow<T, V>(one(rows.at(u)));
+        if (mine) store<T, V>(to, o);
+        to += q.y_token;
       }
-      if (t < end) store<T, V>(y + t * q.y_token, o);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const F v = one(t0 + u < stop ? rows.at(u) : nothing<T, V>());
+        if (mine && t0 + u < end) store<T, V>(to, t0 + u < stop ? narrow<T, V>(v) : nothing<T, V>());
+        to += q.y_token;
+      }
     }
   }
-  if (r == 0 && p.final_state) {
+  if (begin == 0 && p.final_state && mine) {
     T* f = static_cast<T*>(p.final_state) + static_cast<long>(b) * (K - 1) * p.D + d;
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) {
-      float v[V];
-      input<T, K, V>(p, b, d, len - K + 1 + k, v);
-      store<T, V>(f + static_cast<long>(k) * p.D, v);
-    }
+    for (int k = 0; k < K - 1; ++k) store<T, V>(f + static_cast<long>(k) * p.D, input<T, K, V>(p, b, d, len - K + 1 + k));
   }
 }
 
-constexpr int kWarps = 4;      // of a backward CTA: runs of tokens after one another, of the same 32 V channels
-
-template <class T, int K, int V> __global__ void __launch_bounds__(32 * kWarps) conv_backward_kernel(const ttt_b200_conv_args p, const Plan q) {
-  __shared__ float sums[kWarps][(K + 1) * V][32];
+template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(32 * kWarps) conv_backward_kernel(const ttt_b200_conv_args p, const Plan q) {
+  using F = typename Channels<V>::F;
+  __shared__ __align__(16) unsigned char rings[2][kWarps][Rows<T, V>::kBytes + 16];
+  __shared__ float sums[kWarps][K + 1][32 * V];
+  const At at(q);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int tiles = (q.groups + 31) / 32;
-  const int group = blockIdx.x % tiles * 32 + lane, d = group * V;
-  const long bt = blockIdx.x / tiles;
-  const int b = static_cast<int>(bt / q.runs), r = static_cast<int>(bt % q.runs);
-  const int begin = min((r * kWarps + warp) * q.run, p.T), end = min(begin + q.run, p.T);
-  const bool live = group < q.groups;
-  float dw[K][V], db[V];
+  const int b = at.b, d0 = at.tile * 32 * V, begin = min(at.run * q.run, p.T), end = min(begin + q.run, p.T);
+  F dw[K], db = all<F>(0.f);
 #pragma unroll
-  for (int k = 0; k < K; ++k) clear<V>(dw[k]);
-  clear<V>(db);
-  if (live && begin < end) {
+  for (int k = 0; k < K; ++k) dw[k] = db;
+  if (begin < end) {
+    const bool mine = at.group < q.groups;
+    const int d = mine ? at.group * V : d0;      // (a lane behind the last channel reads the tile's first)
     const int len = length_of(p, b);
-    float w[K][V], bias[V], x[K][V], g[K][V];
-    load_weights<K, V>(p, d, w, bias);
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      clear<V>(g[k]);
-      if (k < K - 1 && begin - K + 1 + k < len) input<T, K, V>(p, b, d, begin - K + 1 + k, x[k]);
-      else clear<V>(x[k]);
-    }
+    // token t finishes the gradient of position t - K + 1, in front of the sequence the state's
+    const int live = min(len, end + K - 1), whole = min(len, end);
     const bool heads = p.heads != 0;
-    const T* gy = static_cast<const T*>(p.grad_y) + (heads ? b * q.y_batch + d / 64 * q.y_head + d % 64 : b * p.gy_stride[0] + d);
-    const long gy_token = heads ? q.y_token : p.gy_stride[1];
+    Rows<T, V> rows(rings[0][warp], static_cast<const T*>(p.x) + b * p.x_stride[0] + d0, p.x_stride[1], p.D - d0);
+    Rows<T, V> ups(rings[1][warp], static_cast<const T*>(p.grad_y) + (heads ? b * q.y_batch + d0 / 64 * q.y_head + d0 % 64 : b * p.gy_stride[0] + d0),
+                   heads ? q.y_token : p.gy_stride[1], p.D - d0);
+    rows.start(begin, live);
+    ups.start(begin, live);
     const T* gf = p.grad_final_state ? static_cast<const T*>(p.grad_final_state) + static_cast<long>(b) * (K - 1) * p.D + d : nullptr;
     T* gx = static_cast<T*>(p.grad_x) + static_cast<long>(b) * p.T * p.D + d;
     T* gs = p.grad_state ? static_cast<T*>(p.grad_state) + static_cast<long>(b) * (K - 1) * p.D + d : nullptr;
-    // g[j] is g at token t - j; token t finishes the gradient of position t - K + 1, in front of the sequence the state's
-    const int stop = end + K - 1;
-    constexpr int U = 4;
-    for (int t0 = begin; t0 < stop; t0 += U) {
-      float in[U][V], dy[U][V];
+    F w[K], bias, x[K], g[K];      // g[j] is g at token t - j
+    load_weights<K, V>(p, d, w, bias);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int t = t0 + u;
-        if (t < min(len, stop)) {
-          load<T, V>(static_cast<const T*>(p.x) + b * p.x_stride[0] + t * p.x_stride[1] + d, in[u]);
-          load<T, V>(gy + t * gy_token, dy[u]);
-        } else {
-          clear<V>(in[u]);
-          clear<V>(dy[u]);
-        }
+    for (int k = 0; k < K; ++k) {
+      const int t = begin - K + 1 + k;
+      g[k] = x[k] = all<F>(0.f);
+      if (k < K - 1 && t < len) x[k] = wide<T, V>(input<T, K, V>(p, b, d, t));
+    }
+    auto one = [&](const Raw<T, V>& row, const Raw<T, V>& up, bool own) {
+      x[K - 1] = wide<T, V>(row);
+      F v = wide<T, V>(up);
+      if constexpr (kSilu) {
+        F pre = bias;
+#pragma unroll
+        for (int k = 0; k < K; ++k) pre = mac(w[k], x[k], pre);
+        const F s = sigmoid(pre);
+        v = times(v, mac(times(pre, s), mac(s, all<F>(-1.f), all<F>(1.f)), s));
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int t = t0 + u;
-        if (t >= stop) break;
-        const bool own = t < end;
-        float o[V];
+      for (int k = K - 1; k > 0; --k) g[k] = g[k - 1];
+      g[0] = v;
+      F o = times(w[0], g[0]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          x[K - 1][i] = in[u][i];
-          float v = dy[u][i];
-          if (p.activation == TTT_B200_ACT_SILU) {
-            float pre = bias[i];
+      for (int k = 1; k < K; ++k) o = mac(w[k], g[k], o);
+      if (own) {
+        db = plus(db, v);
 #pragma unroll
-            for (int k = 0; k < K; ++k) pre = fmaf(w[k][i], x[k][i], pre);
-            const float s = sigmoid(pre);
-            v *= fmaf(pre * s, 1.f - s, s);
-          }
-#pragma unroll
-          for (int k = K - 1; k > 0; --k) g[k][i] = g[k - 1][i];
-          g[0][i] = v;
-          const float mine = own ? v : 0.f;
-          db[i] += mine;
-          o[i] = 0.f;
-#pragma unroll
-          for (int k = 0; k < K; ++k) {
-            dw[k][i] = fmaf(mine, x[k][i], dw[k][i]);
-            o[i] = fmaf(w[k][i], g[k][i], o[i]);
-          }
-#pragma unroll
-          for (int k = 0; k < K - 1; ++k) x[k][i] = x[k + 1][i];
-        }
-        const int s = t - K + 1;
-        if (s >= begin || (begin == 0 && gs)) {
-          const int j = s - len + K - 1;      // its place among the last K - 1 inputs
-          if (gf && j >= 0 && j < K - 1) {
-            float f[V];
-            load<T, V>(gf + static_cast<long>(j) * p.D, f);
-#pragma unroll
-            for (int i = 0; i < V; ++i) o[i] += f[i];
-          }
-          store<T, V>(s >= 0 ? gx + static_cast<long>(s) * p.D : gs + static_cast<long>(s + K - 1) * p.D, o);
-        }
+        for (int k = 0; k < K; ++k) dw[k] = mac(v, x[k], dw[k]);
       }
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k) x[k] = x[k + 1];
+      return o;
+    };
+    auto place = [&](int s, F o) {      // the gradient of position s, where it may be the state's or among the last K - 1 inputs
+      if (!mine || (s < begin && !(begin == 0 && gs))) return;
+      const int j = s - len + K - 1;
+      if (gf && j >= 0 && j < K - 1) o = plus(o, wide<T, V>(load<T, V>(gf + static_cast<long>(j) * p.D)));
+      store<T, V>(s >= 0 ? gx + static_cast<long>(s) * p.D : gs + static_cast<long>(s + K - 1) * p.D, narrow<T, V>(o));
+    };
+    for (int t0 = begin; t0 < end; t0 += U) {
+      rows.turn();
+      ups.turn();
+      if (t0 + U <= whole) {
+        T* to = gx + static_cast<long>(t0 - K + 1) * p.D;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const Raw<T, V> o = narrow<T, V>(one(rows.at(u), ups.at(u), true));
+          if (mine && (u >= K - 1 || t0 > begin)) store<T, V>(to, o);
+          else if (mine && begin == 0 && gs) store<T, V>(gs + static_cast<long>(u) * p.D, o);      // (t0 = 0, and len is beyond)
+          to += p.D;
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (t0 + u < end) {
+            const bool in = t0 + u < live;
+            place(t0 + u - K + 1, one(in ? rows.at(u) : nothing<T, V>(), in ? ups.at(u) : nothing<T, V>(), true));
+          }
+      }
+    }
+    // the K - 1 tokens behind the run, for the gradients of its last inputs; where there are any the run ends with a block
+    if (end < live) {
+      rows.turn();
+      ups.turn();
+    }
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) {
+      const bool in = end + k < live;
+      place(end + k - K + 1, one(in ? rows.at(k) : nothing<T, V>(), in ? ups.at(k) : nothing<T, V>(), false));
     }
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) sums[warp][k * V + i][lane] = dw[k][i];
-    sums[warp][K * V + i][lane] = db[i];
-  }
+  for (int k = 0; k < K; ++k) reinterpret_cast<F*>(sums[warp][k])[lane] = dw[k];
+  reinterpret_cast<F*>(sums[warp][K])[lane] = db;
   __syncthreads();
-  float* part = q.part + bt * (K + 1) * p.D;
+  float* part = q.part + static_cast<long>(at.row) * (K + 1) * p.D;
   for (int i = threadIdx.x; i < (K + 1) * V * 32; i += 32 * kWarps) {
-    const int c = i % (V * 32), k = i / (V * 32), at = blockIdx.x % tiles * 32 * V + c;
+    const int c = i % (V * 32), k = i / (V * 32), ch = at.tile * 32 * V + c;
     float s = 0.f;
 #pragma unroll
-    for (int v = 0; v < kWarps; ++v) s += sums[v][k * V + c % V][c / V];
-    if (at < p.D) part[static_cast<long>(k) * p.D + at] = s;
+    for (int v = 0; v < kWarps; ++v) s += sums[v][k][c];
+    if (ch < p.D) part[static_cast<long>(k) * p.D + ch] = s;
   }
 }
 
@@ -236,9 +374,7 @@ template <class T, int K, int V> __global__ void __launch_bounds__(128) conv_ste
   if (p.slots) {
     slot = p.slots[b0];
     if (slot < 0 || slot >= p.rows) {
-      float o[V];
-      clear<V>(o);
-      if (live) store<T, V>(ys + static_cast<long>(b0) * p.D + d, o);
+      if (live) store<T, V>(ys + static_cast<long>(b0) * p.D + d, nothing<T, V>());
       return;
     }
     int before = 0, after = 0;
@@ -248,25 +384,23 @@ template <class T, int K, int V> __global__ void __launch_bounds__(128) conv_ste
     more = __syncthreads_or(after);
   }
   if (!live) return;
-  float w[K][V], bias[V], x[K][V];
+  using F = typename Channels<V>::F;
+  F w[K], bias;
+  Raw<T, V> x[K];
   load_weights<K, V>(p, d, w, bias);
   T* st = static_cast<T*>(p.state_io) + static_cast<long>(slot) * (K - 1) * p.D + d;
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) load<T, V>(st + static_cast<long>(k) * p.D, x[k]);
+  for (int k = 0; k < K - 1; ++k) x[k] = load<T, V>(st + static_cast<long>(k) * p.D);
   for (int b = b0; b < p.B; ++b) {
     if (b != b0 && p.slots[b] != slot) continue;
-    load<T, V>(static_cast<const T*>(p.x) + b * p.x_stride[0] + d, x[K - 1]);
-    float o[V];
+    x[K - 1] = load<T, V>(static_cast<const T*>(p.x) + b * p.x_stride[0] + d);
+    F v = bias;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float v = bias[i];
+    for (int k = 0; k < K; ++k) v = mac(w[k], wide<T, V>(x[k]), v);
+    if (p.activation == TTT_B200_ACT_SILU) v = times(v, sigmoid(v));
+    store<T, V>(ys + static_cast<long>(b) * p.D + d, narrow<T, V>(v));
 #pragma unroll
-      for (int k = 0; k < K; ++k) v = fmaf(w[k][i], x[k][i], v);
-      o[i] = p.activation == TTT_B200_ACT_SILU ? v * sigmoid(v) : v;
-#pragma unroll
-      for (int k = 0; k < K - 1; ++k) x[k][i] = x[k + 1][i];
-    }
-    store<T, V>(ys + static_cast<long>(b) * p.D + d, o);
+    for (int k = 0; k < K - 1; ++k) x[k] = x[k + 1];
     if (!more) break;
   }
 #pragma unroll
@@ -300,51 +434,61 @@ int launched(const char* what) {
   return ttt_set_error(TTT_B200_ERR_LAUNCH, buf);
 }
 
+// whether channels can be taken in pairs
+bool paired(const ttt_b200_conv_args& p, const void* a, const int64_t* st) {
+  const uintptr_t two = p.dtype == TTT_B200_FP32 ? 8 : 4;
+  return reinterpret_cast<uintptr_t>(a) % two == 0 && (!st || (st[0] % 2 == 0 && st[1] % 2 == 0));
+}
+// and whether its rows can be copied in pieces of 16 bytes
 bool rows16(const ttt_b200_conv_args& p, const void* a, const int64_t* st) {
   const int64_t es = p.dtype == TTT_B200_FP32 ? 4 : 2;
   return aligned16(a) && (!st || (st[0] * es % 16 == 0 && st[1] * es % 16 == 0));
 }
+bool paired_weights(const ttt_b200_conv_args& p) {
+  return p.D % 2 == 0 && ((reinterpret_cast<uintptr_t>(p.weight) | reinterpret_cast<uintptr_t>(p.bias)) & 7) == 0;
+}
 
-void fill(Plan& q, const ttt_b200_conv_args& p, int V) {
+// Tokens of a warp's run: as many as leave four to five CTAs to an SM, since each run reads K - 1 tokens more and has its weights to
+// fetch.  Measured, us, forward / backward with runs of 16, 32, 64, 128: 4 x 2048 tokens of 2048 channels 18.7 / 49.7, 16.7 / 43.4,
+// 15.7 / 37.3, 17.7 / 37.3; 2048 tokens of 768 channels 6.1 / 12.6, 6.3 / 14.7, 6.5 / 16.7, 9.9 / 22.9.
+void plan_runs(Plan& q, const ttt_b200_conv_args& p, int V) {
   q.groups = p.D / V;
+  const long tiles = (q.groups + 31) / 32, sms = sm_count();
+  for (q.run = 128; q.run > 16; q.run /= 2)
+    if (2 * tiles * p.B * ((p.T + q.run * kWarps - 1) / (q.run * kWarps)) >= 9 * sms) break;
+  q.runs = (p.T + q.run * kWarps - 1) / (q.run * kWarps);
   q.y_batch = static_cast<long>(p.T) * p.D;
   q.y_head = p.heads ? 64L * p.T : 64;
   q.y_token = p.heads ? 64 : p.D;
 }
 
-// Backward: tokens of a warp's run.
-void plan_backward(Plan& q, const ttt_b200_conv_args& p) {
-  q.run = 32;
-  q.runs = (p.T + q.run * kWarps - 1) / (q.run * kWarps);
-}
-
 template <class T, int K> int forward(const ttt_b200_conv_args& p, cudaStream_t s) {
   Plan q = {};
-  const bool vec = p.D % 8 == 0 && rows16(p, p.x, p.x_stride) && rows16(p, p.y, nullptr) && rows16(p, p.state, nullptr) &&
-                   rows16(p, p.final_state, nullptr);
-  fill(q, p, vec ? 8 : 1);
-  const long want = static_cast<long>(sm_count()) * 1024, tokens = static_cast<long>(p.B) * p.T * q.groups;
-  q.run = tokens / 32 >= want ? 32 : tokens / 16 >= want ? 16 : 8;
-  q.runs = (p.T + q.run - 1) / q.run;
-  const long grid = (static_cast<long>(p.B) * q.runs * q.groups + 127) / 128;
+  const bool vec = paired_weights(p) && rows16(p, p.x, p.x_stride) && paired(p, p.y, nullptr) && paired(p, p.state, nullptr) &&
+                   paired(p, p.final_state, nullptr);
+  plan_runs(q, p, vec ? 2 : 1);
+  const long grid = static_cast<long>(p.B) * q.runs * ((q.groups + 31) / 32);
   if (grid > 0x7fffffffL) return fail("short conv: too many CTAs");
-  if (vec) conv_forward_kernel<T, K, 8><<<static_cast<unsigned>(grid), 128, 0, s>>>(p, q);
-  else conv_forward_kernel<T, K, 1><<<static_cast<unsigned>(grid), 128, 0, s>>>(p, q);
+  const bool silu = p.activation == TTT_B200_ACT_SILU;
+  const auto kernel = vec ? (silu ? conv_forward_kernel<T, K, 2, true> : conv_forward_kernel<T, K, 2, false>)
+                          : (silu ? conv_forward_kernel<T, K, 1, true> : conv_forward_kernel<T, K, 1, false>);
+  kernel<<<static_cast<unsigned>(grid), 32 * kWarps, 0, s>>>(p, q);
   return launched("short conv");
 }
 
 template <class T, int K> int backward(const ttt_b200_conv_args& p, cudaStream_t s) {
   Plan q = {};
-  const bool vec = p.D % 8 == 0 && rows16(p, p.x, p.x_stride) && rows16(p, p.grad_y, p.heads ? nullptr : p.gy_stride) &&
-                   rows16(p, p.state, nullptr) && rows16(p, p.grad_final_state, nullptr) && rows16(p, p.grad_x, nullptr) &&
-                   rows16(p, p.grad_state, nullptr);
-  fill(q, p, vec ? 8 : 1);
-  plan_backward(q, p);
+  const bool vec = paired_weights(p) && rows16(p, p.x, p.x_stride) && rows16(p, p.grad_y, p.heads ? nullptr : p.gy_stride) &&
+                   paired(p, p.state, nullptr) && paired(p, p.grad_final_state, nullptr) && paired(p, p.grad_x, nullptr) &&
+                   paired(p, p.grad_state, nullptr);
+  plan_runs(q, p, vec ? 2 : 1);
   q.part = static_cast<float*>(p.scratch);
   const long grid = static_cast<long>(p.B) * q.runs * ((q.groups + 31) / 32);
   if (grid > 0x7fffffffL) return fail("short conv backward: too many CTAs");
-  if (vec) conv_backward_kernel<T, K, 8><<<static_cast<unsigned>(grid), 32 * kWarps, 0, s>>>(p, q);
-  else conv_backward_kernel<T, K, 1><<<static_cast<unsigned>(grid), 32 * kWarps, 0, s>>>(p, q);
+  const bool silu = p.activation == TTT_B200_ACT_SILU;
+  const auto kernel = vec ? (silu ? conv_backward_kernel<T, K, 2, true> : conv_backward_kernel<T, K, 2, false>)
+                          : (silu ? conv_backward_kernel<T, K, 1, true> : conv_backward_kernel<T, K, 1, false>);
+  kernel<<<static_cast<unsigned>(grid), 32 * kWarps, 0, s>>>(p, q);
   if (int rc = launched("short conv backward")) return rc;
   const long row = static_cast<long>(K + 1) * p.D, KD = static_cast<long>(K) * p.D;
   const int parts = p.B * q.runs;
@@ -355,11 +499,11 @@ template <class T, int K> int backward(const ttt_b200_conv_args& p, cudaStream_t
 
 template <class T, int K> int step(const ttt_b200_conv_args& p, cudaStream_t s) {
   const int64_t st[2] = {p.x_stride[0], 0};
-  const bool vec = p.D % 8 == 0 && rows16(p, p.x, st) && rows16(p, p.y, nullptr) && rows16(p, p.state_io, nullptr);
-  const int tiles = (p.D / (vec ? 8 : 1) + 127) / 128;
+  const bool vec = paired_weights(p) && paired(p, p.x, st) && paired(p, p.y, nullptr) && paired(p, p.state_io, nullptr);
+  const int tiles = (p.D / (vec ? 2 : 1) + 127) / 128;
   const long grid = static_cast<long>(p.B) * tiles;
   if (grid > 0x7fffffffL) return fail("short conv step: too many CTAs");
-  if (vec) conv_step_kernel<T, K, 8><<<static_cast<unsigned>(grid), 128, 0, s>>>(p, tiles);
+  if (vec) conv_step_kernel<T, K, 2><<<static_cast<unsigned>(grid), 128, 0, s>>>(p, tiles);
   else conv_step_kernel<T, K, 1><<<static_cast<unsigned>(grid), 128, 0, s>>>(p, tiles);
   return launched("short conv step");
 }
@@ -375,9 +519,10 @@ template <class T, int K> int step(const ttt_b200_conv_args& p, cudaStream_t s) 
 
 extern "C" uint64_t ttt_b200_short_conv_scratch_bytes(const ttt_b200_conv_args* p) {
   if (check(p) || p->B == 0 || p->T == 0) return 0;
-  Plan q = {};
-  plan_backward(q, *p);
-  return static_cast<uint64_t>(p->B) * q.runs * (p->K + 1) * p->D * sizeof(float);
+  Plan one = {}, two = {};      // single channels or pairs: the pointers say which
+  plan_runs(one, *p, 1);
+  plan_runs(two, *p, 2);
+  return static_cast<uint64_t>(p->B) * std::max(one.runs, two.runs) * (p->K + 1) * p->D * sizeof(float);
 }
 
 extern "C" int ttt_b200_short_conv(const ttt_b200_conv_args* p, void* stream) {
