@@ -13,6 +13,7 @@
 // sums over tokens of its columns to itself over all its tokens and leaves them as one part per CTA for an ordered sum.
 #include <algorithm>
 #include <cstdio>
+#include <type_traits>
 
 #include "ttt_elem.cuh"
 #include "ttt_sum_parts.h"
@@ -28,30 +29,98 @@ struct Plan {
   float* part;    // backward: [ctas * side][5][D]
 };
 
-template <class T, int V> __device__ __forceinline__ void load(const T* p, float (&f)[V]) {
-  if constexpr (V == 8) load8(p, f);
-  else f[0] = to_f32(*p);
+// A vector of a thread: eight neighbouring values as four pairs, or, where rows do not start on 16-byte boundaries, one value.
+template <int V> struct Vec;
+template <> struct Vec<8> {
+  using F = float2;
+  static constexpr int N = 4;
+};
+template <> struct Vec<1> {
+  using F = float;
+  static constexpr int N = 1;
+};
+template <int V> using Of = typename Vec<V>::F;
+
+template <class T> __device__ __forceinline__ void widen(const uint4 (&r)[sizeof(T) / 2], float2 (&f)[4]) {
+  const T* v = reinterpret_cast<const T*>(r);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) f[k] = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(v)[k]);
+    else if constexpr (std::is_same<T, __half>::value) f[k] = __half22float2(reinterpret_cast<const __half2*>(v)[k]);
+    else f[k] = make_float2(v[2 * k], v[2 * k + 1]);
+  }
 }
-template <class T, int V> __device__ __forceinline__ void store(T* p, const float (&f)[V]) {
-  if constexpr (V == 8) store8(p, f);
-  else *p = from_f32<T>(f[0]);
+template <class T, int V> __device__ __forceinline__ void load(const T* p, Of<V> (&f)[Vec<V>::N]) {
+  if constexpr (V == 8) {
+    uint4 r[sizeof(T) / 2];
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) r[i] = reinterpret_cast<const uint4*>(p)[i];
+    widen<T>(r, f);
+  } else {
+    f[0] = to_f32(*p);
+  }
+}
+template <class T, int V> __device__ __forceinline__ void store(T* p, const Of<V> (&f)[Vec<V>::N]) {
+  if constexpr (V == 8) {
+    uint4 r[sizeof(T) / 2];
+    T* v = reinterpret_cast<T*>(r);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) reinterpret_cast<__nv_bfloat162*>(v)[k] = __float22bfloat162_rn(f[k]);
+      else if constexpr (std::is_same<T, __half>::value) reinterpret_cast<__half2*>(v)[k] = __float22half2_rn(f[k]);
+      else v[2 * k] = f[k].x, v[2 * k + 1] = f[k].y;
+    }
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r[i];
+  } else {
+    *p = from_f32<T>(f[0]);
+  }
+}
+// a weight's values at column d, or `none` where there is no such weight
+template <int V> __device__ __forceinline__ void weights(const float* p, int d, bool in, float none, Of<V> (&f)[Vec<V>::N]) {
+  if (p && in) {
+    load<float, V>(p + d, f);
+  } else {
+#pragma unroll
+    for (int k = 0; k < Vec<V>::N; ++k) f[k] = all<Of<V>>(none);
+  }
 }
 
-struct Gate {
-  float v, s;      // value and slope
-};
-__device__ __forceinline__ Gate act(int kind, float x) {
-  // sigmoid of a and its complement; the exponent is bounded so that neither becomes 0 times infinity
-  float a = x, da = 1.f;
-  if (kind == TTT_B200_ACT_GELU) {      // x sigmoid(2 u): no 1 + tanh(u), which cancels on the left
-    constexpr float k = 1.5957691216057308f, c = 0.044715f;      // 2 sqrt(2 / pi)
-    const float q = x * x;
-    a = k * x * fmaf(c, q, 1.f);
-    da = k * fmaf(3.f * c, q, 1.f);
+// The gate: its value, and with kSlope its derivative.  GELU as x sigmoid(2 u): no 1 + tanh(u), which cancels on the left.  The
+// derivative needs 1 - sigmoid without its cancellation on the right, which is e times sigmoid; the exponent is bounded there so
+// that this is not infinity times 0.
+template <int kKind, bool kSlope, class F> __device__ __forceinline__ void gate_one(F x, F& v, F& s) {
+  constexpr float k = 1.5957691216057308f, c = 0.044715f;      // 2 sqrt(2 / pi)
+  F e;
+  const F q = times(x, x);
+  if constexpr (kKind == TTT_B200_ACT_GELU) e = times(times(x, all<F>(-k * kLog2e)), mac(q, all<F>(c), all<F>(1.f)));
+  else e = times(x, all<F>(-kLog2e));
+  if constexpr (kSlope) e = least(e, 126.f);
+  e = ex2(e);
+  const F g = rcp(plus(e, all<F>(1.f)));
+  if constexpr (kKind == TTT_B200_ACT_SIGMOID) {
+    v = g;
+    if constexpr (kSlope) s = times(g, times(e, g));
+  } else {
+    v = times(x, g);
+    if constexpr (kSlope) {
+      F o = times(e, g);
+      if constexpr (kKind == TTT_B200_ACT_GELU) o = times(o, mac(q, all<F>(3.f * c * k), all<F>(k)));
+      s = mac(v, o, g);
+    }
   }
-  const float e = ex2(fminf(-a * kLog2e, 126.f)), s = rcp(1.f + e), o = e * s;
-  if (kind == TTT_B200_ACT_SIGMOID) return {s, s * o};
-  return {x * s, fmaf(x * s, o * da, s)};
+}
+template <bool kSlope, class F, int N> __device__ __forceinline__ void gate(int kind, const F (&x)[N], F (&v)[N], F (&s)[N]) {
+  if (kind == TTT_B200_ACT_SILU) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) gate_one<TTT_B200_ACT_SILU, kSlope>(x[k], v[k], s[k]);
+  } else if (kind == TTT_B200_ACT_GELU) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) gate_one<TTT_B200_ACT_GELU, kSlope>(x[k], v[k], s[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) gate_one<TTT_B200_ACT_SIGMOID, kSlope>(x[k], v[k], s[k]);
+  }
 }
 
 // The sum of two values over the threads of a token, in all of them.  `buf` alternates between calls: a barrier lies between two
@@ -80,237 +149,357 @@ __device__ __forceinline__ float2 row_sum(float2 v, float2 (*smem)[32], int& buf
 // column of vector j of this thread
 template <int V> __device__ __forceinline__ int column(int j, int lane, int width) { return (j * width + lane) * V; }
 
+// A thread's values of a tensor's rows.  With kAhead (vectors of eight) the next row is copied into the thread's own places in shared memory
+// while it works on this one: no barrier, no registers, and past the L1, which keeps the weights.
+template <class T, int V, int NV, bool kAhead> struct Feed {
+  static constexpr int kPieces = V * static_cast<int>(sizeof(T)) / 16 * NV;      // of 16 bytes, per thread
+  const T* base;      // NULL: all zeros
+  int64_t stride;
+  uint4* own;         // this thread's first piece of the first stage
+  static size_t bytes(int threads) { return kAhead ? static_cast<size_t>(2) * kPieces * 16 * threads : 0; }
+  __device__ __forceinline__ Feed(const void* p, int64_t stride, unsigned char*& smem) : base(static_cast<const T*>(p)), stride(stride) {
+    if constexpr (kAhead) {
+      own = reinterpret_cast<uint4*>(smem) + threadIdx.x;
+      if (base) smem += 2 * kPieces * 16 * blockDim.x;
+    }
+  }
+  __device__ __forceinline__ void ahead(long m, bool live, int stage, int lane, int width, int D) const {
+    if constexpr (kAhead) {
+      if (!base) return;
+      const T* row = live ? base + m * stride : base;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int j = i / (kPieces / NV), d = column<V>(j, lane, width);
+        const bool in = live && d < D;
+        cp_async16(own + (stage * kPieces + i) * blockDim.x, in ? row + d + i % (kPieces / NV) * (16 / static_cast<int>(sizeof(T))) : base, in ? 16 : 0);
+      }
+    }
+  }
+  __device__ __forceinline__ void get(long m, bool live, int stage, int j, int d, int D, Of<V> (&f)[Vec<V>::N]) const {
+    if (kAhead && base) {
+      if constexpr (kAhead) {
+        uint4 r[sizeof(T) / 2];
+#pragma unroll
+        for (int i = 0; i < kPieces / NV; ++i) r[i] = own[(stage * kPieces + j * (kPieces / NV) + i) * blockDim.x];
+        widen<T>(r, f);
+      }
+    } else if (!kAhead && base && live && d < D) {
+      load<T, V>(base + m * stride + d, f);
+    } else {
+#pragma unroll
+      for (int k = 0; k < Vec<V>::N; ++k) f[k] = all<Of<V>>(0.f);
+    }
+  }
+};
+
+// What the threads of a token share: partial sums, in two halves that alternate (a barrier lies between two uses of the same
+// one), and how many columns each of its warps has.
+struct Shared {
+  float2 part[2][32];
+  float columns[32];
+};
+template <int V, int NV> __device__ __forceinline__ void count_columns(Shared& sh, int width, int D) {
+  if (threadIdx.x < 32) {
+    int n = 0;      // of warp threadIdx.x of a token: NV runs of 32 V
+#pragma unroll
+    for (int j = 0; j < NV; ++j) n += min(max(D - (j * width + 32 * static_cast<int>(threadIdx.x)) * V, 0), 32 * V);
+    sh.columns[threadIdx.x] = static_cast<float>(n);
+  }
+  __syncthreads();
+}
+
+// Mean and 1 / deviation of a row with one barrier: each warp's mean and its squares about it, joined as
+// sum over warps of (squares + columns (mean of the warp - mean)^2).
 template <int V, int NV>
-__device__ __forceinline__ float2 statistics(const float (&a)[NV][V], const ttt_b200_block_args& p, int lane, int width, float2 (*smem)[32], int& buf) {
+__device__ __forceinline__ float2 statistics(const Of<V> (&a)[NV][Vec<V>::N], const ttt_b200_block_args& p, int lane, int width, Shared& sh, int& buf) {
+  using F = Of<V>;
   const float inv = 1.f / static_cast<float>(p.D);
   float mean = 0.f;
   if (p.layer) {
-    float s = 0.f;
+    F s = all<F>(0.f);
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      if (column<V>(j, lane, width) < p.D) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) s += a[j][i];
-      }
-    mean = row_sum(make_float2(s, 0.f), smem, buf, width).x * inv;
+      for (int k = 0; k < Vec<V>::N; ++k) s = plus(s, a[j][k]);      // (zeros behind the last column)
+    mean = fold(s);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
+    mean *= rcp(fmaxf(sh.columns[lane >> 5], 1.f));
   }
-  float s = 0.f;
+  F sq = all<F>(0.f);
 #pragma unroll
   for (int j = 0; j < NV; ++j)
     if (column<V>(j, lane, width) < p.D) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) s = fmaf(a[j][i] - mean, a[j][i] - mean, s);
-    }
-  s = row_sum(make_float2(s, 0.f), smem, buf, width).x;
-  return make_float2(mean, rsqrtf(fmaf(s, inv, p.eps)));
-}
-
-template <class T, class R, int V, int NV>
-__global__ void __launch_bounds__(1024) block_forward_kernel(const ttt_b200_block_args p, const Plan q) {
-  __shared__ float2 smem[2][32];
-  int buf = 0;
-  const int lane = threadIdx.x % q.width;
-  const long m = static_cast<long>(blockIdx.x) * q.side + threadIdx.x / q.width;
-  const bool live = m < p.M;
-  float a[NV][V], z[NV][V];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int d = column<V>(j, lane, q.width);
-#pragma unroll
-    for (int i = 0; i < V; ++i) a[j][i] = z[j][i] = 0.f;
-    if (live && d < p.D) {
-      load<T, V>(static_cast<const T*>(p.o) + m * p.o_stride + d, a[j]);
-      if (p.residual) load<R, V>(static_cast<const R*>(p.residual) + m * p.residual_stride + d, z[j]);
-      if (p.gate && !p.post_weight) {
-        float g[V];
-        load<T, V>(static_cast<const T*>(p.gate) + m * p.gate_stride + d, g);
-#pragma unroll
-        for (int i = 0; i < V; ++i) a[j][i] *= act(p.activation, g[i]).v;
+      for (int k = 0; k < Vec<V>::N; ++k) {
+        const F v = plus(a[j][k], all<F>(-mean));
+        sq = mac(v, v, sq);
       }
     }
+  float q = fold(sq);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+  if (width > 32) {
+    const int warp = threadIdx.x >> 5, warps = width >> 5, home = warp & -warps;
+    if ((threadIdx.x & 31) == 0) sh.part[buf][warp] = make_float2(mean, q);
+    __syncthreads();
+    q = 0.f;
+    if (p.layer) {
+      mean = 0.f;
+      for (int i = 0; i < warps; ++i) mean = fmaf(sh.part[buf][home + i].x, sh.columns[i], mean);
+      mean *= inv;
+    }
+    for (int i = 0; i < warps; ++i) {
+      const float2 v = sh.part[buf][home + i];
+      const float d = v.x - mean;
+      q += fmaf(sh.columns[i] * d, d, v.y);
+    }
+    buf ^= 1;
   }
-  float2 s1 = make_float2(0.f, 1.f), s2 = s1;
-  if (p.post_weight) {
-    // the gate is requested before the statistics, which wait for o
-    float g[NV][V];
-    if (p.gate) {
+  return make_float2(mean, rsqrtf(fmaf(q, inv, p.eps)));
+}
+
+template <class T, class R, int V, int NV, int kThreads>
+__global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 1024 / kThreads : 1) block_forward_kernel(const ttt_b200_block_args p, const Plan q) {
+  using F = Of<V>;
+  constexpr bool kAhead = V == 8;
+  constexpr int N = Vec<V>::N;
+  __shared__ Shared sh;
+  extern __shared__ __align__(16) unsigned char stages[];
+  int buf = 0;
+  const int lane = threadIdx.x % q.width, sub = threadIdx.x / q.width;
+  unsigned char* at = stages;
+  const Feed<T, V, NV, kAhead> fo(p.o, p.o_stride, at), fg(p.gate, p.gate_stride, at);
+  const Feed<R, V, NV, kAhead> fx(p.residual, p.residual_stride, at);
+  auto ahead = [&](long m, int stage) {
+    fo.ahead(m, m < p.M, stage, lane, q.width, p.D);
+    fg.ahead(m, m < p.M, stage, lane, q.width, p.D);
+    fx.ahead(m, m < p.M, stage, lane, q.width, p.D);
+    cp_async_commit();
+  };
+  const long step = static_cast<long>(q.ctas) * q.side;
+  int stage = 0;
+  ahead(static_cast<long>(blockIdx.x) * q.side + sub, 0);
+  count_columns<V, NV>(sh, q.width, p.D);
+  for (long base = static_cast<long>(blockIdx.x) * q.side; base < p.M; base += step, stage ^= 1) {
+    const long m = base + sub;
+    const bool live = m < p.M;
+    ahead(m + step, stage ^ 1);
+    cp_async_wait<1>();
+    F a[NV][N], z[NV][N];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) fo.get(m, live, stage, j, column<V>(j, lane, q.width), p.D, a[j]);
+    float2 s1 = make_float2(0.f, 1.f), s2 = s1;
+    if (p.post_weight) s1 = statistics<V, NV>(a, p, lane, q.width, sh, buf);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int d = column<V>(j, lane, q.width);
+      const bool in = d < p.D;
+      F w[N], b[N];
+      if (p.post_weight) {
+        weights<V>(p.post_weight, d, in, 0.f, w);
+        weights<V>(p.post_bias, d, in, 0.f, b);
+#pragma unroll
+        for (int k = 0; k < N; ++k) a[j][k] = mac(times(plus(a[j][k], all<F>(-s1.x)), all<F>(s1.y)), w[k], b[k]);
+      }
+      if (p.gate) {
+        F g[N];
+        fg.get(m, live, stage, j, d, p.D, g);
+        gate<false>(p.activation, g, g, w);
+#pragma unroll
+        for (int k = 0; k < N; ++k) a[j][k] = times(a[j][k], g[k]);
+      }
+      fx.get(m, live, stage, j, d, p.D, z[j]);
+      weights<V>(p.scale, d, in, 1.f, w);
+#pragma unroll
+      for (int k = 0; k < N; ++k) z[j][k] = in ? mac(w[k], a[j][k], z[j][k]) : all<F>(0.f);
+      if (live && in) store<R, V>(static_cast<R*>(p.x) + m * p.D + d, z[j]);
+    }
+    if (p.pre_weight) {
+      s2 = statistics<V, NV>(z, p, lane, q.width, sh, buf);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int d = column<V>(j, lane, q.width);
-        if (live && d < p.D) load<T, V>(static_cast<const T*>(p.gate) + m * p.gate_stride + d, g[j]);
-      }
-    }
-    s1 = statistics<V, NV>(a, p, lane, q.width, smem, buf);
+        if (live && d < p.D) {
+          F w[N], b[N];
+          weights<V>(p.pre_weight, d, true, 0.f, w);
+          weights<V>(p.pre_bias, d, true, 0.f, b);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int d = column<V>(j, lane, q.width);
-      if (live && d < p.D) {
-        float w[V], b[V];
-        load<float, V>(p.post_weight + d, w);
-        if (p.post_bias) load<float, V>(p.post_bias + d, b);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          a[j][i] = fmaf((a[j][i] - s1.x) * s1.y, w[i], p.post_bias ? b[i] : 0.f);
-          if (p.gate) a[j][i] *= act(p.activation, g[j][i]).v;
+          for (int k = 0; k < N; ++k) z[j][k] = mac(times(plus(z[j][k], all<F>(-s2.x)), all<F>(s2.y)), w[k], b[k]);
+          store<T, V>(static_cast<T*>(p.n) + m * p.D + d, z[j]);
         }
       }
     }
+    if (p.stats && live && lane == 0) reinterpret_cast<float4*>(p.stats)[m] = make_float4(s1.x, s1.y, s2.x, s2.y);
   }
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int d = column<V>(j, lane, q.width);
-    if (live && d < p.D) {
-      float sc[V];
-      if (p.scale) load<float, V>(p.scale + d, sc);
-#pragma unroll
-      for (int i = 0; i < V; ++i) z[j][i] = fmaf(p.scale ? sc[i] : 1.f, a[j][i], z[j][i]);
-      store<R, V>(static_cast<R*>(p.x) + m * p.D + d, z[j]);
-    }
-  }
-  if (p.pre_weight) {
-    s2 = statistics<V, NV>(z, p, lane, q.width, smem, buf);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int d = column<V>(j, lane, q.width);
-      if (live && d < p.D) {
-        float w[V], b[V];
-        load<float, V>(p.pre_weight + d, w);
-        if (p.pre_bias) load<float, V>(p.pre_bias + d, b);
-#pragma unroll
-        for (int i = 0; i < V; ++i) z[j][i] = fmaf((z[j][i] - s2.x) * s2.y, w[i], p.pre_bias ? b[i] : 0.f);
-        store<T, V>(static_cast<T*>(p.n) + m * p.D + d, z[j]);
-      }
-    }
-  }
-  if (p.stats && live && lane == 0) reinterpret_cast<float4*>(p.stats)[m] = make_float4(s1.x, s1.y, s2.x, s2.y);
 }
 
 // Sums over tokens of a thread's columns: in registers, or, of sixteen columns, in shared memory.
 enum { kDw1, kDb1, kDsc, kDw2, kDb2, kSums };
 template <int V, int NV, bool kShared> struct Sums {
-  float r[kShared ? 1 : kSums][NV][V];
+  using F = Of<V>;
+  F r[kShared ? 1 : kSums][NV][Vec<V>::N];
   float* s;
   int D;
-  __device__ __forceinline__ void add(int k, int j, int i, int d, float v) {
-    if constexpr (kShared) s[k * D + d + i] += v;
-    else r[k][j][i] += v;
-  }
-  __device__ __forceinline__ float get(int k, int j, int i, int d) const {
-    if constexpr (kShared) return s[k * D + d + i];
+  __device__ __forceinline__ F& at(int k, int j, int i, int d) {
+    if constexpr (kShared) return reinterpret_cast<F*>(s + k * D + d)[i];
     else return r[k][j][i];
+  }
+  __device__ __forceinline__ void add(int k, int j, int i, int d, F v) {
+    F& t = at(k, j, i, d);
+    t = plus(t, v);
+  }
+  __device__ __forceinline__ void add(int k, int j, int i, int d, F a, F b) {
+    F& t = at(k, j, i, d);
+    t = mac(a, b, t);
   }
 };
 
-template <class T, class R, int V, int NV, bool kShared>
-__global__ void __launch_bounds__(512) block_backward_kernel(const ttt_b200_block_args p, const Plan q) {
-  __shared__ float2 smem[2][32];
-  extern __shared__ float shared_sums[];
+template <class T, class R, int V, int NV, bool kShared, int kThreads>
+__global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 512 / kThreads : 1) block_backward_kernel(const ttt_b200_block_args p, const Plan q) {
+  using F = Of<V>;
+  constexpr bool kAhead = V == 8 && !kShared;
+  constexpr int N = Vec<V>::N;
+  __shared__ Shared sh;
+  extern __shared__ __align__(16) unsigned char stages[];
   int buf = 0;
   const int lane = threadIdx.x % q.width, sub = threadIdx.x / q.width;
+  unsigned char* at = stages;
+  const Feed<T, V, NV, kAhead> fo(p.o, p.o_stride, at), fg(p.gate, p.gate_stride, at), fn(p.pre_weight ? p.grad_n : nullptr, p.gn_stride, at);
+  const Feed<R, V, NV, kAhead> fx(p.pre_weight ? p.residual : nullptr, p.residual_stride, at), fd(p.grad_x, p.gx_stride, at);
+  auto ahead = [&](long m, int stage) {
+    fo.ahead(m, m < p.M, stage, lane, q.width, p.D);
+    fg.ahead(m, m < p.M, stage, lane, q.width, p.D);
+    fn.ahead(m, m < p.M, stage, lane, q.width, p.D);
+    fx.ahead(m, m < p.M, stage, lane, q.width, p.D);
+    fd.ahead(m, m < p.M, stage, lane, q.width, p.D);
+    cp_async_commit();
+  };
   const float inv = 1.f / static_cast<float>(p.D);
   Sums<V, NV, kShared> sums;
-  sums.s = shared_sums;
+  sums.s = reinterpret_cast<float*>(stages);
   sums.D = p.D;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int d = column<V>(j, lane, q.width);
 #pragma unroll
-    for (int i = 0; i < V; ++i)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int k = 0; k < kSums; ++k) {
-        if constexpr (kShared) {
-          if (d < p.D) shared_sums[k * p.D + d + i] = 0.f;
-        } else {
-          sums.r[k][j][i] = 0.f;
-        }
-      }
+      for (int k = 0; k < kSums; ++k)
+        if (!kShared || d < p.D) sums.at(k, j, i, d) = all<F>(0.f);
   }
-  for (long base = static_cast<long>(blockIdx.x) * q.side; base < p.M; base += static_cast<long>(q.ctas) * q.side) {
+  const long step = static_cast<long>(q.ctas) * q.side;
+  int stage = 0;
+  ahead(static_cast<long>(blockIdx.x) * q.side + sub, 0);
+  for (long base = static_cast<long>(blockIdx.x) * q.side; base < p.M; base += step, stage ^= 1) {
     const long m = base + sub;
     const bool live = m < p.M;
-    float o[NV][V], z[NV][V], g[NV][V], d2[NV][V], gn[NV][V];
+    ahead(m + step, stage ^ 1);
     float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
     if (live) st = reinterpret_cast<const float4*>(p.stats)[m];
+    cp_async_wait<1>();
+    F o[NV][N], z[NV][N], gn[NV][N], d2[NV][N];
+    // u (with its norm: oh) and z again, as the forward had them; z is its normalised value
+    F sx = all<F>(0.f), sy = sx;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int d = column<V>(j, lane, q.width);
+      const bool in = live && d < p.D;
+      fo.get(m, live, stage, j, d, p.D, o[j]);
+      if (p.post_weight) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) o[j][i] = z[j][i] = g[j][i] = d2[j][i] = gn[j][i] = 0.f;
-      if (live && d < p.D) {
-        load<T, V>(static_cast<const T*>(p.o) + m * p.o_stride + d, o[j]);
-        if (p.gate) load<T, V>(static_cast<const T*>(p.gate) + m * p.gate_stride + d, g[j]);
-        if (p.residual && p.pre_weight) load<R, V>(static_cast<const R*>(p.residual) + m * p.residual_stride + d, z[j]);
-        if (p.grad_x) load<R, V>(static_cast<const R*>(p.grad_x) + m * p.gx_stride + d, d2[j]);
-        if (p.grad_n && p.pre_weight) load<T, V>(static_cast<const T*>(p.grad_n) + m * p.gn_stride + d, gn[j]);
+        for (int i = 0; i < N; ++i) o[j][i] = times(plus(o[j][i], all<F>(-st.x)), all<F>(st.y));
+      }
+      if (!p.pre_weight || !in) continue;
+      F u[N], w[N], b[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) u[i] = o[j][i];
+      if (p.post_weight) {
+        weights<V>(p.post_weight, d, true, 0.f, w);
+        weights<V>(p.post_bias, d, true, 0.f, b);
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = mac(o[j][i], w[i], b[i]);
+      }
+      if (p.gate) {
+        fg.get(m, live, stage, j, d, p.D, w);
+        gate<false>(p.activation, w, w, b);
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = times(u[i], w[i]);
+      }
+      weights<V>(p.scale, d, true, 1.f, w);
+      fx.get(m, live, stage, j, d, p.D, z[j]);
+#pragma unroll
+      for (int i = 0; i < N; ++i) z[j][i] = times(plus(mac(w[i], u[i], z[j][i]), all<F>(-st.z)), all<F>(st.w));
+      fn.get(m, live, stage, j, d, p.D, gn[j]);
+      weights<V>(p.pre_weight, d, true, 0.f, w);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        sums.add(kDw2, j, i, d, gn[j][i], z[j][i]);
+        sums.add(kDb2, j, i, d, gn[j][i]);
+        gn[j][i] = times(gn[j][i], w[i]);
+        sx = plus(sx, gn[j][i]);
+        sy = mac(gn[j][i], z[j][i], sy);
       }
     }
-    // u (with its norm: oh) and z again, as the forward had them; from here on z is its normalised value
-    float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int d = column<V>(j, lane, q.width);
-      if (!(live && d < p.D)) continue;
-      float w[V], b[V], sc[V], w2[V];
-      if (p.post_weight) load<float, V>(p.post_weight + d, w);
-      if (p.post_bias) load<float, V>(p.post_bias + d, b);
-      if (p.scale) load<float, V>(p.scale + d, sc);
-      if (p.pre_weight) load<float, V>(p.pre_weight + d, w2);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (p.post_weight) o[j][i] = (o[j][i] - st.x) * st.y;
-        if (p.pre_weight) {
-          const float u = p.post_weight ? fmaf(o[j][i], w[i], p.post_bias ? b[i] : 0.f) : o[j][i];
-          const float v = p.gate ? u * act(p.activation, g[j][i]).v : u;
-          z[j][i] = (fmaf(p.scale ? sc[i] : 1.f, v, z[j][i]) - st.z) * st.w;
-          sums.add(kDw2, j, i, d, gn[j][i] * z[j][i]);
-          sums.add(kDb2, j, i, d, gn[j][i]);
-          gn[j][i] *= w2[i];
-          s.x += gn[j][i];
-          s.y = fmaf(gn[j][i], z[j][i], s.y);
-        }
-      }
-    }
-    if (p.pre_weight) {
-      s = row_sum(s, smem, buf, q.width);
-      const float m1 = p.layer ? s.x * inv : 0.f, m2 = s.y * inv;
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) d2[j][i] = fmaf(st.w, gn[j][i] - m1 - z[j][i] * m2, d2[j][i]);
-    }
-    s = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int d = column<V>(j, lane, q.width);
-      if (!(live && d < p.D)) continue;
-      if (p.grad_residual) store<R, V>(static_cast<R*>(p.grad_residual) + m * p.D + d, d2[j]);
-      float w[V], b[V], sc[V];
-      if (p.post_weight) load<float, V>(p.post_weight + d, w);
-      if (p.post_bias) load<float, V>(p.post_bias + d, b);
-      if (p.scale) load<float, V>(p.scale + d, sc);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float u = p.post_weight ? fmaf(o[j][i], w[i], p.post_bias ? b[i] : 0.f) : o[j][i];
-        Gate a = {1.f, 0.f};
-        if (p.gate) a = act(p.activation, g[j][i]);
-        sums.add(kDsc, j, i, d, d2[j][i] * (u * a.v));
-        const float dv = p.scale ? d2[j][i] * sc[i] : d2[j][i];
-        g[j][i] = dv * u * a.s;
-        float du = dv * a.v;
-        if (p.post_weight) {
-          sums.add(kDw1, j, i, d, du * o[j][i]);
-          sums.add(kDb1, j, i, d, du);
-          du *= w[i];
-          s.x += du;
-          s.y = fmaf(du, o[j][i], s.y);
-        }
-        d2[j][i] = du;
-      }
-      if (p.grad_gate) store<T, V>(static_cast<T*>(p.grad_gate) + m * p.D + d, g[j]);
-    }
+    float2 s = make_float2(fold(sx), fold(sy));
     float m1 = 0.f, m2 = 0.f;
+    if (p.pre_weight) {
+      s = row_sum(s, sh.part, buf, q.width);
+      m1 = p.layer ? s.x * inv : 0.f;
+      m2 = s.y * inv;
+    }
+    sx = sy = all<F>(0.f);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int d = column<V>(j, lane, q.width);
+      if (!(live && d < p.D)) continue;
+      fd.get(m, live, stage, j, d, p.D, d2[j]);
+      if (p.pre_weight) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) d2[j][i] = mac(all<F>(st.w), mac(z[j][i], all<F>(-m2), plus(gn[j][i], all<F>(-m1))), d2[j][i]);
+      }
+      if (p.grad_residual) store<R, V>(static_cast<R*>(p.grad_residual) + m * p.D + d, d2[j]);
+      F u[N], w[N], b[N], v[N], g[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) u[i] = o[j][i];
+      if (p.post_weight) {
+        weights<V>(p.post_weight, d, true, 0.f, w);
+        weights<V>(p.post_bias, d, true, 0.f, b);
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = mac(o[j][i], w[i], b[i]);
+      }
+      weights<V>(p.scale, d, true, 1.f, b);
+      if (p.gate) {
+        fg.get(m, live, stage, j, d, p.D, g);
+        gate<true>(p.activation, g, v, g);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          sums.add(kDsc, j, i, d, d2[j][i], times(u[i], v[i]));
+          d2[j][i] = times(d2[j][i], b[i]);
+          g[i] = times(times(d2[j][i], u[i]), g[i]);
+          d2[j][i] = times(d2[j][i], v[i]);
+        }
+        store<T, V>(static_cast<T*>(p.grad_gate) + m * p.D + d, g);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          sums.add(kDsc, j, i, d, d2[j][i], u[i]);
+          d2[j][i] = times(d2[j][i], b[i]);
+        }
+      }
+      if (p.post_weight) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          sums.add(kDw1, j, i, d, d2[j][i], o[j][i]);
+          sums.add(kDb1, j, i, d, d2[j][i]);
+          d2[j][i] = times(d2[j][i], w[i]);
+          sx = plus(sx, d2[j][i]);
+          sy = mac(d2[j][i], o[j][i], sy);
+        }
+      }
+    }
     if (p.post_weight) {
-      s = row_sum(s, smem, buf, q.width);
+      s = row_sum(make_float2(fold(sx), fold(sy)), sh.part, buf, q.width);
       m1 = p.layer ? s.x * inv : 0.f;
       m2 = s.y * inv;
     }
@@ -320,7 +509,7 @@ __global__ void __launch_bounds__(512) block_backward_kernel(const ttt_b200_bloc
       if (!(live && d < p.D)) continue;
       if (p.post_weight) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) d2[j][i] = st.y * (d2[j][i] - m1 - o[j][i] * m2);
+        for (int i = 0; i < N; ++i) d2[j][i] = times(all<F>(st.y), mac(o[j][i], all<F>(-m2), plus(d2[j][i], all<F>(-m1))));
       }
       store<T, V>(static_cast<T*>(p.grad_o) + m * p.D + d, d2[j]);
     }
@@ -332,9 +521,9 @@ __global__ void __launch_bounds__(512) block_backward_kernel(const ttt_b200_bloc
     if (d >= p.D) continue;
 #pragma unroll
     for (int k = 0; k < kSums; ++k) {
-      float v[V];
+      F v[N];
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = sums.get(k, j, i, d);
+      for (int i = 0; i < N; ++i) v[i] = sums.at(k, j, i, d);
       store<float, V>(part + static_cast<long>(k) * p.D + d, v);
     }
   }
@@ -368,10 +557,11 @@ int width_of(int D, int values) {
 }
 constexpr int kWide = 4096;      // backward: from here on sixteen values to a thread, the sums over tokens in shared memory
 
-void plan_backward(Plan& q, const ttt_b200_block_args& p) {
-  q.width = width_of(p.D, p.D > kWide ? 16 : 8);
+// CTAs that are resident together and walk over the tokens: forward 1024 threads to an SM, backward 512.
+void plan(Plan& q, const ttt_b200_block_args& p, bool backward) {
+  q.width = width_of(p.D, backward && p.D > kWide ? 16 : 8);
   q.side = std::max(1, 128 / q.width);
-  const long most = static_cast<long>(sm_count()) * 2;
+  const long most = static_cast<long>(sm_count()) * std::max(1, (backward ? 512 : 1024) / (q.width * q.side));
   q.ctas = static_cast<int>(std::min<long>(most, (p.M + q.side - 1) / q.side));
 }
 
@@ -395,38 +585,53 @@ int launched(const char* what) {
   return ttt_set_error(TTT_B200_ERR_LAUNCH, buf);
 }
 
-template <class T, class R> int forward(const ttt_b200_block_args& p, cudaStream_t s) {
-  Plan q = {};
-  q.width = width_of(p.D, 8);
-  q.side = std::max(1, 128 / q.width);
-  const long grid = (p.M + q.side - 1) / q.side;
-  if (grid > 0x7fffffffL) return fail("block norm: too many tokens");
-  q.ctas = static_cast<int>(grid);
-  const int threads = q.width * q.side;
-  if (vectors(p, false)) block_forward_kernel<T, R, 8, 1><<<q.ctas, threads, 0, s>>>(p, q);
-  else block_forward_kernel<T, R, 1, 8><<<q.ctas, threads, 0, s>>>(p, q);
-  return launched("block norm");
-}
-
-template <class T, class R, int V, int NV, bool kShared> int backward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
-  const auto kernel = block_backward_kernel<T, R, V, NV, kShared>;
-  const size_t bytes = kShared ? static_cast<size_t>(kSums) * p.D * sizeof(float) : 0;
-  if (bytes > 48 * 1024) {
+template <class K> int launch(K kernel, const Plan& q, size_t bytes, cudaStream_t s, const ttt_b200_block_args& p, const char* what) {
+  if (bytes > 40 * 1024) {      // (with the static part 48 KB is the most without asking)
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
     if (e != cudaSuccess) return ttt_set_error(TTT_B200_ERR_LAUNCH, cudaGetErrorString(e));
   }
   kernel<<<q.ctas, q.width * q.side, bytes, s>>>(p, q);
-  return launched("block norm backward");
+  return launched(what);
+}
+
+template <class T, class R, int V, int NV, int kThreads> int forward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
+  const int n = q.width * q.side;
+  const size_t bytes = Feed<T, V, NV, V == 8>::bytes(n) * (1 + (p.gate != nullptr)) + Feed<R, V, NV, V == 8>::bytes(n) * (p.residual != nullptr);
+  return launch(block_forward_kernel<T, R, V, NV, kThreads>, q, bytes, s, p, "block norm");
+}
+
+template <class T, class R> int forward(const ttt_b200_block_args& p, cudaStream_t s) {
+  Plan q = {};
+  plan(q, p, false);
+  const int n = q.width * q.side;
+  if (vectors(p, false)) {
+    if (n <= 128) return forward_as<T, R, 8, 1, 128>(p, q, s);
+    return n <= 256 ? forward_as<T, R, 8, 1, 256>(p, q, s) : forward_as<T, R, 8, 1, 1024>(p, q, s);
+  }
+  if (n <= 128) return forward_as<T, R, 1, 8, 128>(p, q, s);
+  return n <= 256 ? forward_as<T, R, 1, 8, 256>(p, q, s) : forward_as<T, R, 1, 8, 1024>(p, q, s);
+}
+
+template <class T, class R, int V, int NV, bool kShared, int kThreads> int backward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
+  constexpr bool kAhead = V == 8 && !kShared;
+  const int n = q.width * q.side;
+  const size_t bytes = kShared ? static_cast<size_t>(kSums) * p.D * sizeof(float)
+                               : Feed<T, V, NV, kAhead>::bytes(n) * (1 + (p.gate != nullptr) + (p.pre_weight && p.grad_n)) +
+                                     Feed<R, V, NV, kAhead>::bytes(n) * ((p.pre_weight && p.residual) + (p.grad_x != nullptr));
+  return launch(block_backward_kernel<T, R, V, NV, kShared, kThreads>, q, bytes, s, p, "block norm backward");
 }
 
 template <class T, class R> int backward(const ttt_b200_block_args& p, cudaStream_t s) {
   Plan q = {};
-  plan_backward(q, p);
+  plan(q, p, true);
   q.part = static_cast<float*>(p.scratch);
   const bool vec = vectors(p, true);
+  const int n = q.width * q.side;
   int rc;
-  if (p.D > kWide) rc = vec ? backward_as<T, R, 8, 2, true>(p, q, s) : backward_as<T, R, 1, 16, true>(p, q, s);
-  else rc = vec ? backward_as<T, R, 8, 1, false>(p, q, s) : backward_as<T, R, 1, 8, false>(p, q, s);
+  if (p.D > kWide) rc = vec ? backward_as<T, R, 8, 2, true, 512>(p, q, s) : backward_as<T, R, 1, 16, true, 512>(p, q, s);
+  else if (n <= 128) rc = vec ? backward_as<T, R, 8, 1, false, 128>(p, q, s) : backward_as<T, R, 1, 8, false, 128>(p, q, s);
+  else if (n <= 256) rc = vec ? backward_as<T, R, 8, 1, false, 256>(p, q, s) : backward_as<T, R, 1, 8, false, 256>(p, q, s);
+  else rc = vec ? backward_as<T, R, 8, 1, false, 512>(p, q, s) : backward_as<T, R, 1, 8, false, 512>(p, q, s);
   if (rc) return rc;
   const long row = static_cast<long>(kSums) * p.D;
   float* dst[kSums] = {p.grad_post_weight, p.grad_post_bias, p.grad_scale, p.grad_pre_weight, p.grad_pre_bias};
@@ -441,7 +646,7 @@ template <class T, class R> int backward(const ttt_b200_block_args& p, cudaStrea
 extern "C" uint64_t ttt_b200_norm_gate_residual_scratch_bytes(const ttt_b200_block_args* p) {
   if (check(p) || p->M == 0) return 0;
   Plan q = {};
-  plan_backward(q, *p);
+  plan(q, *p, true);
   return static_cast<uint64_t>(q.ctas) * q.side * kSums * p->D * sizeof(float);
 }
 

@@ -60,6 +60,20 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
+// The same names for one value and for two, for code that takes either.
+__device__ __forceinline__ float mac(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float2 mac(float2 a, float2 b, float2 c) { return fma2(a, b, c); }
+__device__ __forceinline__ float times(float a, float b) { return a * b; }
+__device__ __forceinline__ float2 times(float2 a, float2 b) { return mul2(a, b); }
+__device__ __forceinline__ float plus(float a, float b) { return a + b; }
+__device__ __forceinline__ float2 plus(float2 a, float2 b) { return add2(a, b); }
+template <class F> __device__ __forceinline__ F all(float v) {
+  if constexpr (sizeof(F) == 8) return both(v);
+  else return v;
+}
+__device__ __forceinline__ float fold(float v) { return v; }
+__device__ __forceinline__ float fold(float2 v) { return v.x + v.y; }
+
 __device__ __forceinline__ float ex2(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -70,6 +84,11 @@ __device__ __forceinline__ float rcp(float v) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+
+__device__ __forceinline__ float2 ex2(float2 v) { return make_float2(ex2(v.x), ex2(v.y)); }
+__device__ __forceinline__ float2 rcp(float2 v) { return make_float2(rcp(v.x), rcp(v.y)); }
+__device__ __forceinline__ float least(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ float2 least(float2 a, float b) { return make_float2(fminf(a.x, b), fminf(a.y, b)); }
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 

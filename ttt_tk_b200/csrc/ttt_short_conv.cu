@@ -53,22 +53,8 @@ template <> struct Channels<2> {
 template <class T, int V> struct alignas(V * sizeof(T)) Raw {
   T v[V];
 };
-__device__ __forceinline__ float mac(float a, float b, float c) { return fmaf(a, b, c); }
-__device__ __forceinline__ float2 mac(float2 a, float2 b, float2 c) { return fma2(a, b, c); }
-__device__ __forceinline__ float times(float a, float b) { return a * b; }
-__device__ __forceinline__ float2 times(float2 a, float2 b) { return mul2(a, b); }
-__device__ __forceinline__ float plus(float a, float b) { return a + b; }
-__device__ __forceinline__ float2 plus(float2 a, float2 b) { return add2(a, b); }
-template <class F> __device__ __forceinline__ F all(float v) {
-  if constexpr (sizeof(F) == 8) return both(v);
-  else return v;
-}
 // 1 / (1 + exp(-v)); far on the left exp is infinite and the result 0
-__device__ __forceinline__ float sigmoid(float v) { return rcp(1.f + ex2(-v * kLog2e)); }
-__device__ __forceinline__ float2 sigmoid(float2 v) {
-  const float2 x = mul2(v, both(-kLog2e)), d = add2(make_float2(ex2(x.x), ex2(x.y)), both(1.f));
-  return make_float2(rcp(d.x), rcp(d.y));
-}
+template <class F> __device__ __forceinline__ F sigmoid(F v) { return rcp(plus(ex2(times(v, all<F>(-kLog2e))), all<F>(1.f))); }
 template <class T, int V> __device__ __forceinline__ typename Channels<V>::F wide(const Raw<T, V>& r) {
   if constexpr (V == 1) return to_f32(r.v[0]);
   else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __bfloat1622float2(reinterpret_cast<const __nv_bfloat162&>(r));

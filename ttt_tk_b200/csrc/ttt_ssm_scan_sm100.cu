@@ -942,7 +942,7 @@ int launched(const char* what) {
 
 template <class K> int launch(K kernel, size_t smem, long grid, cudaStream_t s, const ttt_b200_scan_args& p, const Plan& q) {
   if (grid > 0x7fffffffL) return fail("ssm scan: too many CTAs");
-  if (smem > 48 * 1024) {
+  if (smem > 40 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return ttt_set_error(TTT_B200_ERR_LAUNCH, cudaGetErrorString(e));
   }
