@@ -41,44 +41,52 @@ template <> struct Vec<1> {
 };
 template <int V> using Of = typename Vec<V>::F;
 
-template <class T> __device__ __forceinline__ void widen(const uint4 (&r)[sizeof(T) / 2], float2 (&f)[4]) {
-  const T* v = reinterpret_cast<const T*>(r);
+// eight neighbouring values as they lie in memory
+template <class T, int V> struct Raw {
+  static constexpr int kPieces = V * static_cast<int>(sizeof(T)) / 16;
+  alignas(16) T v[V];
+};
+template <class T, int V> __device__ __forceinline__ void widen(const Raw<T, V>& r, Of<V> (&f)[Vec<V>::N]) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) f[k] = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(v)[k]);
-    else if constexpr (std::is_same<T, __half>::value) f[k] = __half22float2(reinterpret_cast<const __half2*>(v)[k]);
-    else f[k] = make_float2(v[2 * k], v[2 * k + 1]);
+  for (int k = 0; k < Vec<V>::N; ++k) {
+    if constexpr (V == 1) f[k] = to_f32(r.v[k]);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) f[k] = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(r.v)[k]);
+    else if constexpr (std::is_same<T, __half>::value) f[k] = __half22float2(reinterpret_cast<const __half2*>(r.v)[k]);
+    else f[k] = make_float2(r.v[2 * k], r.v[2 * k + 1]);
   }
 }
 template <class T, int V> __device__ __forceinline__ void load(const T* p, Of<V> (&f)[Vec<V>::N]) {
-  if constexpr (V == 8) {
-    uint4 r[sizeof(T) / 2];
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) r[i] = reinterpret_cast<const uint4*>(p)[i];
-    widen<T>(r, f);
-  } else {
+  if constexpr (V == 1) {
     f[0] = to_f32(*p);
+  } else {
+    Raw<T, V> r;
+#pragma unroll
+    for (int i = 0; i < Raw<T, V>::kPieces; ++i) {
+      reinterpret_cast<uint4*>(r.v)[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
+    widen<T, V>(r, f);
   }
 }
 template <class T, int V> __device__ __forceinline__ void store(T* p, const Of<V> (&f)[Vec<V>::N]) {
-  if constexpr (V == 8) {
-    uint4 r[sizeof(T) / 2];
-    T* v = reinterpret_cast<T*>(r);
+  if constexpr (V == 1) {
+    *p = from_f32<T>(f[0]);
+  } else {
+    Raw<T, V> r;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) reinterpret_cast<__nv_bfloat162*>(v)[k] = __float22bfloat162_rn(f[k]);
-      else if constexpr (std::is_same<T, __half>::value) reinterpret_cast<__half2*>(v)[k] = __float22half2_rn(f[k]);
-      else v[2 * k] = f[k].x, v[2 * k + 1] = f[k].y;
+    for (int k = 0; k < Vec<V>::N; ++k) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) reinterpret_cast<__nv_bfloat162*>(r.v)[k] = __float22bfloat162_rn(f[k]);
+      else if constexpr (std::is_same<T, __half>::value) reinterpret_cast<__half2*>(r.v)[k] = __float22half2_rn(f[k]);
+      else r.v[2 * k] = f[k].x, r.v[2 * k + 1] = f[k].y;
     }
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r[i];
-  } else {
-    *p = from_f32<T>(f[0]);
+    for (int i = 0; i < Raw<T, V>::kPieces; ++i) {
+      reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(r.v)[i];
+    }
   }
 }
 // a weight's values at column d, or `none` where there is no such weight
-template <int V> __device__ __forceinline__ void weights(const float* p, int d, bool in, float none, Of<V> (&f)[Vec<V>::N]) {
-  if (p && in) {
+template <int V> __device__ __forceinline__ void weights(const float* p, int d, float none, Of<V> (&f)[Vec<V>::N]) {
+  if (p) {
     load<float, V>(p + d, f);
   } else {
 #pragma unroll
@@ -123,71 +131,82 @@ template <bool kSlope, class F, int N> __device__ __forceinline__ void gate(int 
   }
 }
 
-// The sum of two values over the threads of a token, in all of them.  `buf` alternates between calls: a barrier lies between two
-// uses of the same half.
+// The sums of two values over the threads of a token, in all of them.  `buf` alternates between calls: a barrier lies between two
+// uses of the same half.  The lower half of a warp takes the first value, the upper the second, here and across the warps.
 __device__ __forceinline__ float2 row_sum(float2 v, float2 (*smem)[32], int& buf, int width) {
+  const bool up = threadIdx.x & 16;
+  float s = (up ? v.y : v.x) + __shfl_xor_sync(0xffffffffu, up ? v.x : v.y, 16);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-  }
+  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (width > 32) {
-    const int warp = threadIdx.x >> 5, warps = width >> 5, first = warp / warps * warps;
-    if ((threadIdx.x & 31) == 0) smem[buf][warp] = v;
+    const int warp = threadIdx.x >> 5, warps = width >> 5, first = warp & -warps, i = threadIdx.x & 15;
+    float* part = reinterpret_cast<float*>(smem[buf]);
+    if (i == 0) part[2 * warp + up] = s;
     __syncthreads();
-    v = make_float2(0.f, 0.f);
-    for (int i = 0; i < warps; ++i) {
-      const float2 a = smem[buf][first + i];
-      v.x += a.x;
-      v.y += a.y;
-    }
+    s = i < warps ? part[2 * (first + i) + up] : 0.f;
+    if (warps > 16) s += part[2 * (first + 16 + i) + up];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     buf ^= 1;
   }
-  return v;
+  const float other = __shfl_xor_sync(0xffffffffu, s, 16);
+  return up ? make_float2(other, s) : make_float2(s, other);
 }
 
 // column of vector j of this thread
 template <int V> __device__ __forceinline__ int column(int j, int lane, int width) { return (j * width + lane) * V; }
 
-// A thread's values of a tensor's rows.  With kAhead (vectors of eight) the next row is copied into the thread's own places in shared memory
-// while it works on this one: no barrier, no registers, and past the L1, which keeps the weights.
-template <class T, int V, int NV, bool kAhead> struct Feed {
-  static constexpr int kPieces = V * static_cast<int>(sizeof(T)) / 16 * NV;      // of 16 bytes, per thread
-  const T* base;      // NULL: all zeros
+// A thread's values of a tensor's rows, token after token at a fixed distance; a tensor that is not there is all zeros.
+//   kOwn     vectors of eight: the next row is copied into the thread's own places in shared memory while it works on this one: no
+//            barrier, no registers, and past the L1, which keeps the weights
+//   kWindow  single values: the next row's 16-byte blocks are copied by the token's threads together (the first and the last may hold
+//            neighbours of the row as well), and each value is picked out at the row's offset; needs a barrier in front of `get`
+//   kDirect  from global memory
+enum { kDirect, kOwn, kWindow };
+template <class T, int V, int NV, int kMode> struct Feed {
+  static_assert(kMode != kOwn || (V == 8 && NV == 1), "one vector of eight to a thread");
+  const T* base;      // NULL: no such tensor
   int64_t stride;
-  uint4* own;         // this thread's first piece of the first stage
-  static size_t bytes(int threads) { return kAhead ? static_cast<size_t>(2) * kPieces * 16 * threads : 0; }
-  __device__ __forceinline__ Feed(const void* p, int64_t stride, unsigned char*& smem) : base(static_cast<const T*>(p)), stride(stride) {
-    if constexpr (kAhead) {
-      own = reinterpret_cast<uint4*>(smem) + threadIdx.x;
-      if (base) smem += 2 * kPieces * 16 * blockDim.x;
+  uint32_t slot;      // shared address of the first stage, the same for all threads
+  __host__ __device__ static constexpr uint32_t window(int D) { return (static_cast<uint32_t>(D) * sizeof(T) + 30) / 16 * 16; }
+  // bytes of one stage
+  __host__ __device__ static uint32_t bytes(int threads, int side, int D) {
+    return kMode == kOwn ? V * static_cast<int>(sizeof(T)) * threads : kMode == kWindow ? side * window(D) : 0;
+  }
+  __device__ __forceinline__ Feed(const void* p, int64_t stride, uint32_t& smem, int side, int D) : base(static_cast<const T*>(p)), stride(stride), slot(smem) {
+    if (base) smem += 2 * bytes(blockDim.x, side, D);
+  }
+  __device__ __forceinline__ static uint32_t place(int sub, int D) { return kMode == kOwn ? threadIdx.x * 16 : sub * window(D); }
+  // row m into a stage; `some`: this thread has columns
+  __device__ __forceinline__ void ahead(long m, bool some, uint32_t to, int lane, int sub, int width, int D) const {
+    if (!base) return;
+    to += slot + place(sub, D);
+    if constexpr (kMode == kOwn) {
+      if (!some) return;
+      const T* from = base + m * stride + lane * V;
+#pragma unroll
+      for (int i = 0; i < Raw<T, V>::kPieces; ++i) cp_async16_at(to + i * 16 * blockDim.x, from + i * (16 / static_cast<int>(sizeof(T))));
+    } else if constexpr (kMode == kWindow) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(base + m * stride), begin = at & ~static_cast<uintptr_t>(15);
+      const int span = D * static_cast<int>(sizeof(T)) + static_cast<int>(at - begin);
+      for (int c = 16 * lane; c < span; c += 16 * width) cp_async16_at(to + c, reinterpret_cast<const char*>(begin) + c, min(16, span - c));
     }
   }
-  __device__ __forceinline__ void ahead(long m, bool live, int stage, int lane, int width, int D) const {
-    if constexpr (kAhead) {
-      if (!base) return;
-      const T* row = live ? base + m * stride : base;
-#pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const int j = i / (kPieces / NV), d = column<V>(j, lane, width);
-        const bool in = live && d < D;
-        cp_async16(own + (stage * kPieces + i) * blockDim.x, in ? row + d + i % (kPieces / NV) * (16 / static_cast<int>(sizeof(T))) : base, in ? 16 : 0);
-      }
-    }
-  }
-  __device__ __forceinline__ void get(long m, bool live, int stage, int j, int d, int D, Of<V> (&f)[Vec<V>::N]) const {
-    if (kAhead && base) {
-      if constexpr (kAhead) {
-        uint4 r[sizeof(T) / 2];
-#pragma unroll
-        for (int i = 0; i < kPieces / NV; ++i) r[i] = own[(stage * kPieces + j * (kPieces / NV) + i) * blockDim.x];
-        widen<T>(r, f);
-      }
-    } else if (!kAhead && base && live && d < D) {
-      load<T, V>(base + m * stride + d, f);
-    } else {
+  // vector of row m at column d, which is there
+  __device__ __forceinline__ void get(long m, uint32_t from, int d, int sub, int D, Of<V> (&f)[Vec<V>::N]) const {
+    if (!base) {
 #pragma unroll
       for (int k = 0; k < Vec<V>::N; ++k) f[k] = all<Of<V>>(0.f);
+    } else if constexpr (kMode == kOwn) {
+      Raw<T, V> r;
+#pragma unroll
+      for (int i = 0; i < Raw<T, V>::kPieces; ++i) reinterpret_cast<uint4*>(r.v)[i] = shared_load16(slot + from + place(sub, D) + i * 16 * blockDim.x);
+      widen<T, V>(r, f);
+    } else if constexpr (kMode == kWindow) {
+      const uint32_t offset = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base + m * stride)) & 15;
+      f[0] = shared_load<T>(slot + from + place(sub, D) + offset + d * static_cast<int>(sizeof(T)));
+    } else {
+      load<T, V>(base + m * stride + d, f);
     }
   }
 };
@@ -195,14 +214,16 @@ template <class T, int V, int NV, bool kAhead> struct Feed {
 // What the threads of a token share: partial sums, in two halves that alternate (a barrier lies between two uses of the same
 // one), and how many columns each of its warps has.
 struct Shared {
-  float2 part[2][32];
+  alignas(16) float2 part[2][32];
   float columns[32];
+  float4 stats[2][32];      // backward: each warp's token's
 };
 template <int V, int NV> __device__ __forceinline__ void count_columns(Shared& sh, int width, int D) {
   if (threadIdx.x < 32) {
     int n = 0;      // of warp threadIdx.x of a token: NV runs of 32 V
 #pragma unroll
-    for (int j = 0; j < NV; ++j) n += min(max(D - (j * width + 32 * static_cast<int>(threadIdx.x)) * V, 0), 32 * V);
+    for (int j = 0; j < NV; ++j)
+      if (32 * static_cast<int>(threadIdx.x) < width) n += min(max(D - (j * width + 32 * static_cast<int>(threadIdx.x)) * V, 0), 32 * V);
     sh.columns[threadIdx.x] = static_cast<float>(n);
   }
   __syncthreads();
@@ -240,80 +261,91 @@ __device__ __forceinline__ float2 statistics(const Of<V> (&a)[NV][Vec<V>::N], co
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
   if (width > 32) {
-    const int warp = threadIdx.x >> 5, warps = width >> 5, home = warp & -warps;
-    if ((threadIdx.x & 31) == 0) sh.part[buf][warp] = make_float2(mean, q);
+    const int warp = threadIdx.x >> 5, warps = width >> 5, home = warp & -warps, i = threadIdx.x & 31;
+    if (i == 0) sh.part[buf][warp] = make_float2(mean, q);
     __syncthreads();
-    q = 0.f;
+    const float2 v = i < warps ? sh.part[buf][home + i] : make_float2(0.f, 0.f);      // a lane for each warp
+    q = v.y;
     if (p.layer) {
-      mean = 0.f;
-      for (int i = 0; i < warps; ++i) mean = fmaf(sh.part[buf][home + i].x, sh.columns[i], mean);
+      const float n = sh.columns[i];      // (0 behind the last warp)
+      mean = n * v.x;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
       mean *= inv;
+      q = fmaf(n * (v.x - mean), v.x - mean, q);
     }
-    for (int i = 0; i < warps; ++i) {
-      const float2 v = sh.part[buf][home + i];
-      const float d = v.x - mean;
-      q += fmaf(sh.columns[i] * d, d, v.y);
-    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
     buf ^= 1;
   }
   return make_float2(mean, rsqrtf(fmaf(q, inv, p.eps)));
 }
 
 template <class T, class R, int V, int NV, int kThreads>
-__global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 1024 / kThreads : 1) block_forward_kernel(const ttt_b200_block_args p, const Plan q) {
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kernel(const ttt_b200_block_args p, const Plan q) {
   using F = Of<V>;
-  constexpr bool kAhead = V == 8;
+  constexpr int kMode = V > 1 ? kOwn : kWindow;
   constexpr int N = Vec<V>::N;
   __shared__ Shared sh;
   extern __shared__ __align__(16) unsigned char stages[];
+  uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(stages));
   int buf = 0;
   const int lane = threadIdx.x % q.width, sub = threadIdx.x / q.width;
-  unsigned char* at = stages;
-  const Feed<T, V, NV, kAhead> fo(p.o, p.o_stride, at), fg(p.gate, p.gate_stride, at);
-  const Feed<R, V, NV, kAhead> fx(p.residual, p.residual_stride, at);
+  const long step = static_cast<long>(q.ctas) * q.side;
+  const Feed<T, V, NV, kMode> fo(p.o, p.o_stride, at, q.side, p.D), fg(p.gate, p.gate_stride, at, q.side, p.D);
+  const Feed<R, V, NV, kMode> fx(p.residual, p.residual_stride, at, q.side, p.D);
+  const uint32_t small = Feed<T, V, NV, kMode>::bytes(blockDim.x, q.side, p.D), large = Feed<R, V, NV, kMode>::bytes(blockDim.x, q.side, p.D);
+  const bool some = lane * V < p.D;      // this thread has columns
   auto ahead = [&](long m, int stage) {
-    fo.ahead(m, m < p.M, stage, lane, q.width, p.D);
-    fg.ahead(m, m < p.M, stage, lane, q.width, p.D);
-    fx.ahead(m, m < p.M, stage, lane, q.width, p.D);
+    if (m < p.M) {
+      fo.ahead(m, some, stage * small, lane, sub, q.width, p.D);
+      fg.ahead(m, some, stage * small, lane, sub, q.width, p.D);
+      fx.ahead(m, some, stage * large, lane, sub, q.width, p.D);
+    }
     cp_async_commit();
   };
-  const long step = static_cast<long>(q.ctas) * q.side;
-  int stage = 0;
-  ahead(static_cast<long>(blockIdx.x) * q.side + sub, 0);
+  long m = static_cast<long>(blockIdx.x) * q.side + sub;
+  ahead(m, 0);
   count_columns<V, NV>(sh, q.width, p.D);
-  for (long base = static_cast<long>(blockIdx.x) * q.side; base < p.M; base += step, stage ^= 1) {
-    const long m = base + sub;
+  int stage = 0;
+  for (long base = static_cast<long>(blockIdx.x) * q.side; base < p.M; base += step, stage ^= 1, m += step) {
     const bool live = m < p.M;
+    cp_async_wait<0>();
+    if constexpr (kMode == kWindow) __syncthreads();
     ahead(m + step, stage ^ 1);
-    cp_async_wait<1>();
     F a[NV][N], z[NV][N];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) fo.get(m, live, stage, j, column<V>(j, lane, q.width), p.D, a[j]);
+    for (int j = 0; j < NV; ++j) {
+      const int d = column<V>(j, lane, q.width);
+#pragma unroll
+      for (int k = 0; k < N; ++k) a[j][k] = z[j][k] = all<F>(0.f);
+      if (live && d < p.D) fo.get(m, stage * small, d, sub, p.D, a[j]);
+    }
     float2 s1 = make_float2(0.f, 1.f), s2 = s1;
     if (p.post_weight) s1 = statistics<V, NV>(a, p, lane, q.width, sh, buf);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int d = column<V>(j, lane, q.width);
-      const bool in = d < p.D;
+      if (!(live && d < p.D)) continue;
       F w[N], b[N];
       if (p.post_weight) {
-        weights<V>(p.post_weight, d, in, 0.f, w);
-        weights<V>(p.post_bias, d, in, 0.f, b);
+        weights<V>(p.post_weight, d, 0.f, w);
+        weights<V>(p.post_bias, d, 0.f, b);
 #pragma unroll
         for (int k = 0; k < N; ++k) a[j][k] = mac(times(plus(a[j][k], all<F>(-s1.x)), all<F>(s1.y)), w[k], b[k]);
       }
       if (p.gate) {
         F g[N];
-        fg.get(m, live, stage, j, d, p.D, g);
+        fg.get(m, stage * small, d, sub, p.D, g);
         gate<false>(p.activation, g, g, w);
 #pragma unroll
         for (int k = 0; k < N; ++k) a[j][k] = times(a[j][k], g[k]);
       }
-      fx.get(m, live, stage, j, d, p.D, z[j]);
-      weights<V>(p.scale, d, in, 1.f, w);
+      fx.get(m, stage * large, d, sub, p.D, z[j]);
+      weights<V>(p.scale, d, 1.f, w);
 #pragma unroll
-      for (int k = 0; k < N; ++k) z[j][k] = in ? mac(w[k], a[j][k], z[j][k]) : all<F>(0.f);
-      if (live && in) store<R, V>(static_cast<R*>(p.x) + m * p.D + d, z[j]);
+      for (int k = 0; k < N; ++k) z[j][k] = mac(w[k], a[j][k], z[j][k]);
+      store<R, V>(static_cast<R*>(p.x) + m * p.D + d, z[j]);
     }
     if (p.pre_weight) {
       s2 = statistics<V, NV>(z, p, lane, q.width, sh, buf);
@@ -322,8 +354,8 @@ __global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 1024 / kThreads : 
         const int d = column<V>(j, lane, q.width);
         if (live && d < p.D) {
           F w[N], b[N];
-          weights<V>(p.pre_weight, d, true, 0.f, w);
-          weights<V>(p.pre_bias, d, true, 0.f, b);
+          weights<V>(p.pre_weight, d, 0.f, w);
+          weights<V>(p.pre_bias, d, 0.f, b);
 #pragma unroll
           for (int k = 0; k < N; ++k) z[j][k] = mac(times(plus(z[j][k], all<F>(-s2.x)), all<F>(s2.y)), w[k], b[k]);
           store<T, V>(static_cast<T*>(p.n) + m * p.D + d, z[j]);
@@ -356,23 +388,32 @@ template <int V, int NV, bool kShared> struct Sums {
 };
 
 template <class T, class R, int V, int NV, bool kShared, int kThreads>
-__global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 512 / kThreads : 1) block_backward_kernel(const ttt_b200_block_args p, const Plan q) {
+__global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1) block_backward_kernel(const ttt_b200_block_args p, const Plan q) {
   using F = Of<V>;
-  constexpr bool kAhead = V == 8 && !kShared;
+  constexpr int kMode = kShared ? kDirect : V > 1 ? kOwn : kWindow;
   constexpr int N = Vec<V>::N;
   __shared__ Shared sh;
   extern __shared__ __align__(16) unsigned char stages[];
+  uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(stages));
   int buf = 0;
   const int lane = threadIdx.x % q.width, sub = threadIdx.x / q.width;
-  unsigned char* at = stages;
-  const Feed<T, V, NV, kAhead> fo(p.o, p.o_stride, at), fg(p.gate, p.gate_stride, at), fn(p.pre_weight ? p.grad_n : nullptr, p.gn_stride, at);
-  const Feed<R, V, NV, kAhead> fx(p.pre_weight ? p.residual : nullptr, p.residual_stride, at), fd(p.grad_x, p.gx_stride, at);
+  const long step = static_cast<long>(q.ctas) * q.side;
+  const Feed<T, V, NV, kMode> fo(p.o, p.o_stride, at, q.side, p.D), fg(p.gate, p.gate_stride, at, q.side, p.D);
+  const Feed<T, V, NV, kMode> fn(p.pre_weight ? p.grad_n : nullptr, p.gn_stride, at, q.side, p.D);
+  const Feed<R, V, NV, kMode> fx(p.pre_weight ? p.residual : nullptr, p.residual_stride, at, q.side, p.D);
+  const Feed<R, V, NV, kMode> fd(p.grad_x, p.gx_stride, at, q.side, p.D);
+  const uint32_t small = Feed<T, V, NV, kMode>::bytes(blockDim.x, q.side, p.D), large = Feed<R, V, NV, kMode>::bytes(blockDim.x, q.side, p.D);
+  const bool some = lane * V < p.D;
+  const uint32_t stats = static_cast<uint32_t>(__cvta_generic_to_shared(&sh.stats[0][threadIdx.x >> 5]));
   auto ahead = [&](long m, int stage) {
-    fo.ahead(m, m < p.M, stage, lane, q.width, p.D);
-    fg.ahead(m, m < p.M, stage, lane, q.width, p.D);
-    fn.ahead(m, m < p.M, stage, lane, q.width, p.D);
-    fx.ahead(m, m < p.M, stage, lane, q.width, p.D);
-    fd.ahead(m, m < p.M, stage, lane, q.width, p.D);
+    if (m < p.M) {
+      if ((threadIdx.x & 31) == 0) cp_async16_at(stats + stage * static_cast<uint32_t>(sizeof(sh.stats[0])), p.stats + 4 * m);
+      fo.ahead(m, some, stage * small, lane, sub, q.width, p.D);
+      fg.ahead(m, some, stage * small, lane, sub, q.width, p.D);
+      fn.ahead(m, some, stage * small, lane, sub, q.width, p.D);
+      fx.ahead(m, some, stage * large, lane, sub, q.width, p.D);
+      fd.ahead(m, some, stage * large, lane, sub, q.width, p.D);
+    }
     cp_async_commit();
   };
   const float inv = 1.f / static_cast<float>(p.D);
@@ -388,16 +429,17 @@ __global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 512 / kThreads : 1
       for (int k = 0; k < kSums; ++k)
         if (!kShared || d < p.D) sums.at(k, j, i, d) = all<F>(0.f);
   }
-  const long step = static_cast<long>(q.ctas) * q.side;
+  long m = static_cast<long>(blockIdx.x) * q.side + sub;
+  ahead(m, 0);
   int stage = 0;
-  ahead(static_cast<long>(blockIdx.x) * q.side + sub, 0);
-  for (long base = static_cast<long>(blockIdx.x) * q.side; base < p.M; base += step, stage ^= 1) {
-    const long m = base + sub;
+  for (long base = static_cast<long>(blockIdx.x) * q.side; base < p.M; base += step, stage ^= 1, m += step) {
     const bool live = m < p.M;
+    cp_async_wait<0>();
+    if constexpr (kMode == kWindow) __syncthreads();
+    else __syncwarp();
     ahead(m + step, stage ^ 1);
     float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (live) st = reinterpret_cast<const float4*>(p.stats)[m];
-    cp_async_wait<1>();
+    if (live) st = sh.stats[stage][threadIdx.x >> 5];
     F o[NV][N], z[NV][N], gn[NV][N], d2[NV][N];
     // u (with its norm: oh) and z again, as the forward had them; z is its normalised value
     F sx = all<F>(0.f), sy = sx;
@@ -405,7 +447,9 @@ __global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 512 / kThreads : 1
     for (int j = 0; j < NV; ++j) {
       const int d = column<V>(j, lane, q.width);
       const bool in = live && d < p.D;
-      fo.get(m, live, stage, j, d, p.D, o[j]);
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[j][i] = all<F>(0.f);
+      if (in) fo.get(m, stage * small, d, sub, p.D, o[j]);
       if (p.post_weight) {
 #pragma unroll
         for (int i = 0; i < N; ++i) o[j][i] = times(plus(o[j][i], all<F>(-st.x)), all<F>(st.y));
@@ -415,23 +459,23 @@ __global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 512 / kThreads : 1
 #pragma unroll
       for (int i = 0; i < N; ++i) u[i] = o[j][i];
       if (p.post_weight) {
-        weights<V>(p.post_weight, d, true, 0.f, w);
-        weights<V>(p.post_bias, d, true, 0.f, b);
+        weights<V>(p.post_weight, d, 0.f, w);
+        weights<V>(p.post_bias, d, 0.f, b);
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = mac(o[j][i], w[i], b[i]);
       }
       if (p.gate) {
-        fg.get(m, live, stage, j, d, p.D, w);
+        fg.get(m, stage * small, d, sub, p.D, w);
         gate<false>(p.activation, w, w, b);
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = times(u[i], w[i]);
       }
-      weights<V>(p.scale, d, true, 1.f, w);
-      fx.get(m, live, stage, j, d, p.D, z[j]);
+      weights<V>(p.scale, d, 1.f, w);
+      fx.get(m, stage * large, d, sub, p.D, z[j]);
 #pragma unroll
       for (int i = 0; i < N; ++i) z[j][i] = times(plus(mac(w[i], u[i], z[j][i]), all<F>(-st.z)), all<F>(st.w));
-      fn.get(m, live, stage, j, d, p.D, gn[j]);
-      weights<V>(p.pre_weight, d, true, 0.f, w);
+      fn.get(m, stage * small, d, sub, p.D, gn[j]);
+      weights<V>(p.pre_weight, d, 0.f, w);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         sums.add(kDw2, j, i, d, gn[j][i], z[j][i]);
@@ -453,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 512 / kThreads : 1
     for (int j = 0; j < NV; ++j) {
       const int d = column<V>(j, lane, q.width);
       if (!(live && d < p.D)) continue;
-      fd.get(m, live, stage, j, d, p.D, d2[j]);
+      fd.get(m, stage * large, d, sub, p.D, d2[j]);
       if (p.pre_weight) {
 #pragma unroll
         for (int i = 0; i < N; ++i) d2[j][i] = mac(all<F>(st.w), mac(z[j][i], all<F>(-m2), plus(gn[j][i], all<F>(-m1))), d2[j][i]);
@@ -463,14 +507,14 @@ __global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 512 / kThreads : 1
 #pragma unroll
       for (int i = 0; i < N; ++i) u[i] = o[j][i];
       if (p.post_weight) {
-        weights<V>(p.post_weight, d, true, 0.f, w);
-        weights<V>(p.post_bias, d, true, 0.f, b);
+        weights<V>(p.post_weight, d, 0.f, w);
+        weights<V>(p.post_bias, d, 0.f, b);
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = mac(o[j][i], w[i], b[i]);
       }
-      weights<V>(p.scale, d, true, 1.f, b);
+      weights<V>(p.scale, d, 1.f, b);
       if (p.gate) {
-        fg.get(m, live, stage, j, d, p.D, g);
+        fg.get(m, stage * small, d, sub, p.D, g);
         gate<true>(p.activation, g, v, g);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -555,11 +599,12 @@ int width_of(int D, int values) {
   while (w * values < D) w *= 2;
   return w;
 }
-constexpr int kWide = 4096;      // backward: from here on sixteen values to a thread, the sums over tokens in shared memory
+constexpr int kWide = 4096;      // backward of wider rows: sixteen values to a thread, the sums over tokens in shared memory
 
-// CTAs that are resident together and walk over the tokens: forward 1024 threads to an SM, backward 512.
+// CTAs that are resident together and walk over the tokens: 1024 threads to an SM, backward 512.
 void plan(Plan& q, const ttt_b200_block_args& p, bool backward) {
-  q.width = width_of(p.D, backward && p.D > kWide ? 16 : 8);
+  const bool wide = p.D > kWide;
+  q.width = width_of(p.D, wide && backward ? 16 : 8);
   q.side = std::max(1, 128 / q.width);
   const long most = static_cast<long>(sm_count()) * std::max(1, (backward ? 512 : 1024) / (q.width * q.side));
   q.ctas = static_cast<int>(std::min<long>(most, (p.M + q.side - 1) / q.side));
@@ -595,8 +640,10 @@ template <class K> int launch(K kernel, const Plan& q, size_t bytes, cudaStream_
 }
 
 template <class T, class R, int V, int NV, int kThreads> int forward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
+  constexpr int kMode = V > 1 ? kOwn : kWindow;
   const int n = q.width * q.side;
-  const size_t bytes = Feed<T, V, NV, V == 8>::bytes(n) * (1 + (p.gate != nullptr)) + Feed<R, V, NV, V == 8>::bytes(n) * (p.residual != nullptr);
+  const size_t bytes = 2 * (Feed<T, V, NV, kMode>::bytes(n, q.side, p.D) * (1 + (p.gate != nullptr)) +
+                            Feed<R, V, NV, kMode>::bytes(n, q.side, p.D) * (p.residual != nullptr));
   return launch(block_forward_kernel<T, R, V, NV, kThreads>, q, bytes, s, p, "block norm");
 }
 
@@ -604,20 +651,18 @@ template <class T, class R> int forward(const ttt_b200_block_args& p, cudaStream
   Plan q = {};
   plan(q, p, false);
   const int n = q.width * q.side;
-  if (vectors(p, false)) {
-    if (n <= 128) return forward_as<T, R, 8, 1, 128>(p, q, s);
-    return n <= 256 ? forward_as<T, R, 8, 1, 256>(p, q, s) : forward_as<T, R, 8, 1, 1024>(p, q, s);
-  }
-  if (n <= 128) return forward_as<T, R, 1, 8, 128>(p, q, s);
-  return n <= 256 ? forward_as<T, R, 1, 8, 256>(p, q, s) : forward_as<T, R, 1, 8, 1024>(p, q, s);
+  const bool vec = vectors(p, false);
+  if (n <= 128) return vec ? forward_as<T, R, 8, 1, 128>(p, q, s) : forward_as<T, R, 1, 8, 128>(p, q, s);
+  if (n <= 256) return vec ? forward_as<T, R, 8, 1, 256>(p, q, s) : forward_as<T, R, 1, 8, 256>(p, q, s);
+  return vec ? forward_as<T, R, 8, 1, 1024>(p, q, s) : forward_as<T, R, 1, 8, 1024>(p, q, s);
 }
 
 template <class T, class R, int V, int NV, bool kShared, int kThreads> int backward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
-  constexpr bool kAhead = V == 8 && !kShared;
+  constexpr int kMode = kShared ? kDirect : V > 1 ? kOwn : kWindow;
   const int n = q.width * q.side;
   const size_t bytes = kShared ? static_cast<size_t>(kSums) * p.D * sizeof(float)
-                               : Feed<T, V, NV, kAhead>::bytes(n) * (1 + (p.gate != nullptr) + (p.pre_weight && p.grad_n)) +
-                                     Feed<R, V, NV, kAhead>::bytes(n) * ((p.pre_weight && p.residual) + (p.grad_x != nullptr));
+                               : 2 * (Feed<T, V, NV, kMode>::bytes(n, q.side, p.D) * (1 + (p.gate != nullptr) + (p.pre_weight && p.grad_n)) +
+                                          Feed<R, V, NV, kMode>::bytes(n, q.side, p.D) * ((p.pre_weight && p.residual) + (p.grad_x != nullptr)));
   return launch(block_backward_kernel<T, R, V, NV, kShared, kThreads>, q, bytes, s, p, "block norm backward");
 }
 

@@ -92,10 +92,32 @@ __device__ __forceinline__ float2 least(float2 a, float b) { return make_float2(
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// 16 bytes global -> shared without registers; `bytes` 0 fills with zeros and reads nothing.
+// 16 bytes global -> shared without registers, to a shared address; of a piece of `bytes` the rest becomes zeros and is not read.
+__device__ __forceinline__ void cp_async16_at(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16_at(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
-  const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(bytes) : "memory");
+  cp_async16_at(static_cast<uint32_t>(__cvta_generic_to_shared(dst)), src, bytes);
+}
+// from a shared address
+__device__ __forceinline__ uint4 shared_load16(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
+  return r;
+}
+template <class T> __device__ __forceinline__ float shared_load(uint32_t at) {
+  if constexpr (sizeof(T) == 4) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+  } else {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+    return to_f32(reinterpret_cast<T&>(v));
+  }
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kPending> __device__ __forceinline__ void cp_async_wait() {
