@@ -458,6 +458,7 @@ PyObject* scan_step(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
 // ---- block end -------------------------------------------------------------------------------------------------------------
 // rows [..., D] that are one after another at a fixed distance: that distance
 int64_t row_stride(const Call& c, const Tensor& t, const char* msg) {
+  if (t.numel() == 0) return 0;
   int64_t stride = 0, below = 1;      // `below`: tokens of the dimensions further in
   for (int64_t i = t.dim() - 2; i >= 0; --i) {
     if (t.size(i) == 1) continue;

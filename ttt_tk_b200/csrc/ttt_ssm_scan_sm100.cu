@@ -787,57 +787,97 @@ __global__ void __launch_bounds__(TH, 3) scan_backward_kernel(const ttt_b200_sca
 }
 
 // ---- one token ---------------------------------------------------------------------------------------------------------
-// A row of the batch and up to 128 / LN channels to a CTA, each state read and written once.  Rows that name the same slot are
-// taken in their order by the CTA of the first of them, so that no two CTAs touch a state.
-template <class T, int LN> __global__ void __launch_bounds__(128) scan_step_kernel(const ttt_b200_scan_args p, bool vec_n, int tiles) {
-  constexpr int DC = 128 / LN;
-  const int b0 = blockIdx.x / tiles, d = (blockIdx.x % tiles) * DC + threadIdx.x / LN;
-  const int li = threadIdx.x % LN, n0 = 4 * li;
-  const bool live = d < p.D;
+// A row of the batch and up to 256 / LN channels to a CTA, two per thread, each state read and written once.  What does not depend on
+// the slot is requested in front of it, and the state in front of the search for rows that share it: two round trips to memory in all.
+// Rows that name the same slot are taken in their order by the CTA of the first of them, so that no two CTAs touch a state.
+template <class T, int LN> __global__ void __launch_bounds__(TH) scan_step_kernel(const ttt_b200_scan_args p, bool vec_n, int tiles) {
+  constexpr int DC = TH / LN;
+  const int b0 = blockIdx.x / tiles, li = threadIdx.x % LN, n0 = 4 * li;
+  int d[2];
+  bool live[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    d[e] = (blockIdx.x % tiles * 2 + e) * DC + threadIdx.x / LN;
+    live[e] = d[e] < p.D;
+    if (!live[e]) d[e] = 0;      // (reads there, writes nothing)
+  }
   T* ys = static_cast<T*>(p.y);
-  int slot = b0, more = 0;
+  const int per = p.D / p.G;
+  struct Token {
+    float x[2], dt[2], b[2][4], c[2][4];
+  };
+  auto read = [&](int b, Token& t) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      t.x[e] = to_f32(static_cast<const T*>(p.x)[b * p.x_stride[0] + d[e]]);
+      t.dt[e] = to_f32(static_cast<const T*>(p.dt)[b * p.dt_stride[0] + d[e]]);
+      const int g = p.G > 1 ? d[e] / per : 0;
+      const T* bs = static_cast<const T*>(p.Bm) + b * p.B_stride[0] + g * p.B_stride[2] + n0;
+      const T* cs = static_cast<const T*>(p.Cm) + b * p.C_stride[0] + g * p.C_stride[2] + n0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        t.b[e][k] = n0 + k < p.N ? to_f32(bs[k]) : 0.f;
+        t.c[e][k] = n0 + k < p.N ? to_f32(cs[k]) : 0.f;
+      }
+    }
+  };
+  int slot = p.slots ? p.slots[b0] : b0, more = 0;
+  Token t;
+  read(b0, t);
+  float a[2][4], bias[2], skip[2], h[2][4];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    load_states(p.A + static_cast<long>(d[e]) * p.N, n0, p.N, vec_n, a[e]);
+    bias[e] = p.dt_bias ? p.dt_bias[d[e]] : 0.f;
+    skip[e] = p.Dskip ? p.Dskip[d[e]] : 0.f;
+  }
+  if (p.slots && (slot < 0 || slot >= p.rows)) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (live[e] && li == 0) ys[static_cast<long>(b0) * p.D + d[e]] = from_f32<T>(0.f);
+    return;
+  }
+  float* st = p.state_io + static_cast<long>(slot) * p.D * p.N;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) load_states(st + static_cast<long>(d[e]) * p.N, n0, p.N, vec_n, h[e]);
   if (p.slots) {
-    slot = p.slots[b0];
-    if (slot < 0 || slot >= p.rows) {
-      if (live && li == 0) ys[static_cast<long>(b0) * p.D + d] = from_f32<T>(0.f);
-      return;
+    int found = 0;      // 1: in a row before, 2: in one behind
+    for (int r = threadIdx.x; r < p.B; r += TH)
+      if (r != b0 && p.slots[r] == slot) found |= r < b0 ? 1 : 2;
+    if (__syncthreads_or(found)) {      // (rarely: which of the two)
+      if (__syncthreads_or(found & 1)) return;
+      more = 1;
     }
-    int before = 0, after = 0;
-    for (int r = threadIdx.x; r < p.B; r += 128)
-      if (r != b0 && p.slots[r] == slot) (r < b0 ? before : after) = 1;
-    if (__syncthreads_or(before)) return;
-    more = __syncthreads_or(after);
   }
-  const int g = live ? d / (p.D / p.G) : 0;
-  float a[4] = {}, h[4] = {};
-  float* st = p.state_io + (static_cast<long>(slot) * p.D + d) * p.N;
-  if (live) {
-    load_states(p.A + static_cast<long>(d) * p.N, n0, p.N, vec_n, a);
-    load_states(st, n0, p.N, vec_n, h);
-  }
-  const float bias = live && p.dt_bias ? p.dt_bias[d] : 0.f, skip = live && p.Dskip ? p.Dskip[d] : 0.f;
-  for (int b = b0; b < p.B; ++b) {
-    if (b != b0 && p.slots[b] != slot) continue;
-    float y = 0.f, x = 0.f;
-    if (live) {
-      x = to_f32(static_cast<const T*>(p.x)[b * p.x_stride[0] + d]);
-      const float v = to_f32(static_cast<const T*>(p.dt)[b * p.dt_stride[0] + d]) + bias;
-      const float dl = p.softplus ? softplus2(both(v)).x : v;
-      const T* bs = static_cast<const T*>(p.Bm) + b * p.B_stride[0] + g * p.B_stride[2];
-      const T* cs = static_cast<const T*>(p.Cm) + b * p.C_stride[0] + g * p.C_stride[2];
+  for (int b = b0;;) {
+    float y[2];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (n0 + k < p.N) {
-          h[k] = fmaf(ex2(fmaf(dl, a[k] * kLog2e, kCentre)), h[k], dl * x * to_f32(bs[n0 + k]));
-          y = fmaf(h[k], to_f32(cs[n0 + k]), y);
-        }
+    for (int e = 0; e < 2; ++e) {
+      const float v = t.dt[e] + bias[e], dl = p.softplus ? softplus2(both(v)).x : v, dx = dl * t.x[e];
+      y[e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        h[e][k] = fmaf(ex2(fmaf(dl, a[e][k] * kLog2e, kCentre)), h[e][k], dx * t.b[e][k]);
+        y[e] = fmaf(h[e][k], t.c[e][k], y[e]);
+      }
     }
 #pragma unroll
-    for (int o = LN / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (live && li == 0) ys[static_cast<long>(b) * p.D + d] = from_f32<T>(fmaf(skip, x, y));
+    for (int o = LN / 2; o > 0; o >>= 1) {
+      y[0] += __shfl_xor_sync(0xffffffffu, y[0], o);
+      y[1] += __shfl_xor_sync(0xffffffffu, y[1], o);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (live[e] && li == 0) ys[static_cast<long>(b) * p.D + d[e]] = from_f32<T>(fmaf(skip[e], t.x[e], y[e]));
     if (!more) break;
+    do ++b;
+    while (b < p.B && p.slots[b] != slot);
+    if (b >= p.B) break;
+    read(b, t);
   }
-  if (live) store_states(st, n0, p.N, vec_n, h);
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (live[e]) store_states(st + static_cast<long>(d[e]) * p.N, n0, p.N, vec_n, h[e]);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
@@ -979,11 +1019,11 @@ template <class T, int LN> int backward(const ttt_b200_scan_args& p, const Plan&
 }
 
 template <class T, int LN> int step(const ttt_b200_scan_args& p, cudaStream_t s) {
-  const int tiles = (p.D + 128 / LN - 1) / (128 / LN);
+  const int tiles = (p.D + 2 * TH / LN - 1) / (2 * TH / LN);
   const bool vec = p.N % 4 == 0 && aligned16(p.A) && aligned16(p.state_io);
   const long grid = static_cast<long>(p.B) * tiles;
   if (grid > 0x7fffffffL) return fail("ssm scan: too many CTAs");
-  scan_step_kernel<T, LN><<<static_cast<unsigned>(grid), 128, 0, s>>>(p, vec, tiles);
+  scan_step_kernel<T, LN><<<static_cast<unsigned>(grid), TH, 0, s>>>(p, vec, tiles);
   return launched("ssm scan step");
 }
 

@@ -12,7 +12,7 @@ import ctypes
 
 import torch
 
-from . import _lib
+from . import _lib, ssm
 
 
 def _need(cond, msg):
@@ -106,9 +106,8 @@ def norm_gate_residual(o, residual=None, gate=None, *, norm="rms", activation="s
     there is no n.  The first block's norm is the call with `pre_weight` alone.  Types as in `ttt_tk_b200.ssm`; rows may be a slice of a
     wider tensor.  Returns (x, n or None), with `return_stats` (x, n, stats): fp32 [tokens, 4] for the backward.  n is that of x
     before x is rounded."""
-    from .ssm import _host
     layer, act = _kinds(norm, activation)
-    x, n, stats = _host().block(o, residual, gate, layer, act, post_weight, post_bias, scale, pre_weight, pre_bias, eps, return_stats)
+    x, n, stats = ssm._host().block(o, residual, gate, layer, act, post_weight, post_bias, scale, pre_weight, pre_bias, eps, return_stats)
     return (x, n, stats) if return_stats else (x, n)
 
 
@@ -117,7 +116,6 @@ def norm_gate_residual_backward(grad_x, grad_n, o, stats, residual=None, gate=No
     """Gradients of `norm_gate_residual` from its inputs and `stats`: (grad_o, grad_residual, grad_gate, grad_post_weight,
     grad_post_bias, grad_scale, grad_pre_weight, grad_pre_bias), None where there is no such input.  `grad_x`, `grad_n`: as x
     and n, either may be None."""
-    from .ssm import _host
     layer, act = _kinds(norm, activation)
-    return _host().block_backward(grad_x, grad_n, o, stats, residual, gate, layer, act, post_weight, post_bias, scale, pre_weight,
+    return ssm._host().block_backward(grad_x, grad_n, o, stats, residual, gate, layer, act, post_weight, post_bias, scale, pre_weight,
                                   pre_bias, eps)
