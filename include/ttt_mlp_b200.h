@@ -384,7 +384,7 @@ int ttt_b200_pack_layernorm_backward(const void* grad_y, const void* x, const fl
  * (rows on 16-byte boundaries are read faster).  Device pointers; stream-ordered, no synchronisation; TTT_B200_* codes.  Outputs may
  * not overlap inputs or one another.  Sums over tokens or channels have a fixed order: the same call gives the same bits.
  * `lengths` (may be NULL): int32 [B], the tokens of each sequence of a right-padded batch (clamped to 0..T); those behind are not
- * read, their y and gradients are zero and they change no state. */
+ * read, their y and gradients are zero and they change no state.  T and D at most 2^30. */
 enum { TTT_B200_BF16 = 0, TTT_B200_FP16 = 1, TTT_B200_FP32 = 2 };
 enum { TTT_B200_ACT_NONE = 0, TTT_B200_ACT_SILU = 1, TTT_B200_ACT_GELU = 2 /* tanh form */, TTT_B200_ACT_SIGMOID = 3 };
 

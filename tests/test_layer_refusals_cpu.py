@@ -165,3 +165,13 @@ def test_the_c_abi_refuses_null_and_bad_sizes():
         assert fn(None, None) == 1
         assert b"NULL" in lib.ttt_b200_last_error()
         assert fn(ctypes.byref(ctypes.create_string_buffer(1024)), None) == 1      # a struct of zeros
+
+
+def test_sizes_that_indices_could_not_hold():
+    """Expanded tensors hold nothing of their own; their sizes are refused before anything is read."""
+    one = torch.zeros(1, 1, 1, dtype=BF)
+    with pytest.raises(ValueError, match="too large"):
+        ssm.short_conv(one.expand(1, (1 << 30) + 1, 1), torch.zeros(1, 2))
+    with pytest.raises(ValueError, match="too large"):
+        x = one.expand(1, (1 << 30) + 1, 1)
+        ssm.ssm_scan(x, x, torch.zeros(1, 1), x.unsqueeze(-1), x.unsqueeze(-1))

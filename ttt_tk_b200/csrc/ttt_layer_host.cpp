@@ -105,8 +105,8 @@ class Call {
   void need(bool ok, const char* msg) const {
     if (!ok) refuse(std::string(what_) + ": " + msg);
   }
-  void int32_sized(int64_t v, const char* name) const {
-    if (v > INT32_MAX) refuse(std::string(what_) + ": " + name + " is too large");
+  void sized(int64_t v, const char* name) const {
+    if (v > (1 << 30)) refuse(std::string(what_) + ": " + name + " is too large");
   }
 
  private:
@@ -195,7 +195,7 @@ void conv_weights(Call& c, ttt_b200_conv_args& a, PyObject* w, PyObject* b) {
 // x [B, T, D] and what the forward and the backward share: v = weight, bias, activation, state, lengths, heads
 void conv_inputs(Call& c, ttt_b200_conv_args& a, PyObject* x, PyObject* const* v) {
   const Tensor& t = *c.first(x, "x", 3, "[B, T, D]");
-  for (int i = 0; i < 3; ++i) c.int32_sized(t.size(i), "a dimension of x");
+  for (int i = 0; i < 3; ++i) c.sized(t.size(i), "a dimension of x");
   a.B = static_cast<int32_t>(t.size(0));
   a.T = static_cast<int32_t>(t.size(1));
   a.D = static_cast<int32_t>(t.size(2));
@@ -277,7 +277,7 @@ PyObject* conv_backward(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
 int64_t table(Call& c, PyObject* state, int64_t dims, PyObject* slots, int64_t B) {
   c.need(THPVariable_Check(state) && THPVariable_Unpack(state).dim() == dims, "state has the wrong number of dimensions");
   const int64_t rows = THPVariable_Unpack(state).size(0);
-  c.int32_sized(rows, "the state");
+  c.sized(rows, "the state");
   c.need(slots != Py_None || rows == B, "without slots the state must have a row for each row of x");
   c.need(slots == Py_None || rows >= 1 || B == 0, "the state has no rows");
   return rows;
@@ -289,7 +289,7 @@ PyObject* conv_step(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     Call c("short_conv_step");
     ttt_b200_conv_args a = {};
     const Tensor& t = *c.first(v[0], "x", 2, "[B, D]");
-    for (int i = 0; i < 2; ++i) c.int32_sized(t.size(i), "a dimension of x");
+    for (int i = 0; i < 2; ++i) c.sized(t.size(i), "a dimension of x");
     a.B = static_cast<int32_t>(t.size(0));
     a.T = 1;
     a.D = static_cast<int32_t>(t.size(1));
@@ -315,7 +315,7 @@ PyObject* conv_step(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
 // v = x, dt, A, B, C, D, dt_bias, softplus; a step has no tokens' dimension
 void scan_inputs(Call& c, ttt_b200_scan_args& a, PyObject* const* v, bool step) {
   const Tensor& x = *c.first(v[0], "x", step ? 2 : 3, step ? "[B, D]" : "[B, T, D]");
-  for (int64_t i = 0; i < x.dim(); ++i) c.int32_sized(x.size(i), "a dimension of x");
+  for (int64_t i = 0; i < x.dim(); ++i) c.sized(x.size(i), "a dimension of x");
   a.B = static_cast<int32_t>(x.size(0));
   a.T = step ? 1 : static_cast<int32_t>(x.size(1));
   a.D = static_cast<int32_t>(x.size(-1));

@@ -398,7 +398,8 @@ int fail(const char* msg) { return ttt_set_error(TTT_B200_ERR_BAD_ARGS, msg); }
 
 int check(const ttt_b200_conv_args* p) {
   if (!p) return fail("short conv: NULL argument struct");
-  if (p->B < 0 || p->T < 0 || p->D < 1 || p->K < 2 || p->K > 4) return fail("short conv: B, T >= 0, D >= 1 and a width of 2, 3 or 4");
+  if (p->B < 0 || p->T < 0 || p->T > 1 << 30 || p->D < 1 || p->D > 1 << 30 || p->K < 2 || p->K > 4)
+    return fail("short conv: B, T >= 0, D >= 1, T and D at most 2^30, and a width of 2, 3 or 4");
   if (p->dtype < TTT_B200_BF16 || p->dtype > TTT_B200_FP32) return fail("short conv: unknown element type");
   if (p->activation != TTT_B200_ACT_NONE && p->activation != TTT_B200_ACT_SILU) return fail("short conv: activation is none or silu");
   if (p->heads && (p->D % 64 || p->T % 64)) return fail("short conv: heads need multiples of 64 channels and tokens");

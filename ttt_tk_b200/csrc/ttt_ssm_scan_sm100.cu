@@ -48,7 +48,7 @@ struct Plan {
   bool vec_x, vec_dt, vec_gy, vec_b, vec_c, vec_n, vec_part, pairs;      // 16-byte rows; whole float4 of states; outputs in pairs
   float* state;   // [B][chunks][D][N]: what a chunk starts from (backward: ends with)
   float* delta;   // [B][chunks][D]: sum of delta
-  float* part_bc; // backward: [2][tiles][B][T][G][N]
+  float* part_bc; // backward: [2][tiles][B][T][G][N], where a group has several tiles
   float* part_a;  // backward: [B][chunks][D][N]
   float* part_d;  // backward: [2][B][chunks][D]: grad_D, grad_dt_bias
 };
@@ -519,20 +519,29 @@ template <bool kRev> __global__ void __launch_bounds__(256) scan_join_kernel(con
   const float a2 = p.A[dn] * kLog2e;
   const float* from = kRev ? p.grad_final_state : p.state;
   float h = from ? from[i] : 0.f;
-  constexpr int kAhead = 8;
-  for (int c0 = 0; c0 < q.chunks; c0 += kAhead) {
-    float s[kAhead], f[kAhead];
+  constexpr int kAhead = 8;      // chunks requested ahead of those that are worked on
+  auto chunk = [&](int c) { return b * q.chunks + (kRev ? q.chunks - 1 - c : c); };
+  float s[kAhead], f[kAhead], s2[kAhead], f2[kAhead];
+  auto request = [&](int c0) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const long c = b * q.chunks + (kRev ? q.chunks - 1 - min(c0 + k, q.chunks - 1) : min(c0 + k, q.chunks - 1));
-      s[k] = q.state[c * DN + dn];
-      f[k] = ex2(fmaf(a2, q.delta[c * p.D + d], kCentre));
+      const long c = chunk(min(c0 + k, q.chunks - 1));
+      s2[k] = q.state[c * DN + dn];
+      f2[k] = q.delta[c * p.D + d];
     }
+  };
+  request(0);
+  for (int c0 = 0; c0 < q.chunks; c0 += kAhead) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      s[k] = s2[k];
+      f[k] = ex2(fmaf(a2, f2[k], kCentre));
+    }
+    request(c0 + kAhead);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
       if (c0 + k < q.chunks) {
-        const long c = b * q.chunks + (kRev ? q.chunks - 1 - (c0 + k) : c0 + k);
-        q.state[c * DN + dn] = h;
+        q.state[chunk(c0 + k) * DN + dn] = h;
         h = fmaf(f[k], h, s[k]);
       }
   }
@@ -585,6 +594,7 @@ __global__ void __launch_bounds__(TH, 3) scan_backward_kernel(const ttt_b200_sca
   const long GN = static_cast<long>(p.G) * p.N, BTGN = static_cast<long>(p.B) * p.T * GN;
   float* pb = q.part_bc + w.tile * BTGN + static_cast<long>(w.b) * p.T * GN + w.g * p.N;
   float* pc = pb + q.tiles * BTGN;
+  T *tb = static_cast<T*>(p.grad_B) + static_cast<long>(w.b) * p.T * GN + w.g * p.N, *tc = static_cast<T*>(p.grad_C) + static_cast<long>(w.b) * p.T * GN + w.g * p.N;
   auto fetch = [&](int t0, int buf) {
     const int rows = min(w.len - t0, kTile);
     if (t0 >= begin && rows > 0) {
@@ -611,8 +621,9 @@ __global__ void __launch_bounds__(TH, 3) scan_backward_kernel(const ttt_b200_sca
         }
       for (int i = threadIdx.x; i < kTile * NP; i += TH)
         if (t0 + i / NP < end && i % NP < p.N) {
-          pb[(t0 + i / NP) * GN + i % NP] = 0.f;
-          pc[(t0 + i / NP) * GN + i % NP] = 0.f;
+          const long at = (t0 + i / NP) * GN + i % NP;
+          if (q.tiles > 1) pb[at] = pc[at] = 0.f;
+          else tb[at] = tc[at] = from_f32<T>(0.f);
         }
       fetch(t0 - kTile, buf ^ 1);
       continue;
@@ -764,7 +775,13 @@ __global__ void __launch_bounds__(TH, 3) scan_backward_kernel(const ttt_b200_sca
           v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
         }
       }
-      store_states((k < NP ? pb : pc) + (t0 + t) * GN, n, p.N, q.vec_part, v);
+      if (q.tiles > 1) {
+        store_states((k < NP ? pb : pc) + (t0 + t) * GN, n, p.N, q.vec_part, v);
+      } else {      // all of the group's channels are here
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n + r < p.N) (k < NP ? tb : tc)[(t0 + t) * GN + n + r] = from_f32<T>(v[r]);
+      }
     }
   }
   me.write(q.part_a + w.bc * DN, w, p.N, q.vec_n, da);
@@ -894,8 +911,8 @@ int fail(const char* msg) { return ttt_set_error(TTT_B200_ERR_BAD_ARGS, msg); }
 
 int check(const ttt_b200_scan_args* p) {
   if (!p) return fail("ssm scan: NULL argument struct");
-  if (p->B < 0 || p->T < 0 || p->D < 1 || p->G < 1 || p->N < 1 || p->N > 64)
-    return fail("ssm scan: B, T >= 0, D, G >= 1 and 1 to 64 states");
+  if (p->B < 0 || p->T < 0 || p->T > 1 << 30 || p->D < 1 || p->D > 1 << 30 || p->G < 1 || p->N < 1 || p->N > 64)
+    return fail("ssm scan: B, T >= 0, D, G >= 1, T and D at most 2^30, and 1 to 64 states");
   if (p->D % p->G) return fail("ssm scan: the groups must divide the channels");
   if (p->dtype < TTT_B200_BF16 || p->dtype > TTT_B200_FP32) return fail("ssm scan: unknown element type");
   return TTT_B200_OK;
@@ -934,7 +951,7 @@ size_t lay_out(Plan& q, const ttt_b200_scan_args& p, bool backward, float* base)
   q.state = q.chunks > 1 ? take(BC * DN) : nullptr;
   q.delta = q.chunks > 1 ? take(BC * p.D) : nullptr;
   if (backward) {
-    q.part_bc = take(2 * static_cast<size_t>(q.tiles) * p.B * p.T * p.G * p.N);
+    q.part_bc = take(q.tiles > 1 ? 2 * static_cast<size_t>(q.tiles) * p.B * p.T * p.G * p.N : 0);
     q.part_a = take(BC * DN);
     q.part_d = take(2 * BC * p.D);
   }
@@ -1010,8 +1027,9 @@ template <class T, int LN> int backward(const ttt_b200_scan_args& p, const Plan&
   if (int rc = launch(scan_backward_kernel<T, LN>, sizeof(BwdSmem<T, LN>), grid, s, p, q)) return rc;
   const long BTGN = static_cast<long>(p.B) * p.T * p.G * p.N, DN = static_cast<long>(p.D) * p.N, BCD = static_cast<long>(p.B) * q.chunks * p.D;
   const int bc = p.B * q.chunks;
-  const ttt_sum_job jobs[] = {{q.part_bc, p.grad_B, BTGN, BTGN, q.tiles, p.dtype, 0},
-                              {q.part_bc + q.tiles * BTGN, p.grad_C, BTGN, BTGN, q.tiles, p.dtype, 0},
+  const bool parts = q.tiles > 1;
+  const ttt_sum_job jobs[] = {{q.part_bc, parts ? p.grad_B : nullptr, BTGN, BTGN, q.tiles, p.dtype, 0},
+                              {q.part_bc + q.tiles * BTGN, parts ? p.grad_C : nullptr, BTGN, BTGN, q.tiles, p.dtype, 0},
                               {q.part_a, p.grad_A, DN, DN, bc, TTT_B200_FP32, 0},
                               {q.part_d, p.grad_D, p.D, p.D, bc, TTT_B200_FP32, 0},
                               {q.part_d + BCD, p.grad_dt_bias, p.D, p.D, bc, TTT_B200_FP32, 0}};
