@@ -565,8 +565,11 @@ template <class T, int LN> struct BwdSmem {
   alignas(16) float bc[kTile][TH / 32][2 * S::NP];     // each warp's part of dB and dC
 };
 
+// With up to 16 states the factors exp(delta A) are worked out once more on the way back instead of kept, and four CTAs fit an SM
+// instead of three (4 x 2048 x 1536 x 16: 348 -> 332 us); with 64 the exponentials cost more than that gives (191 -> 208).
 template <class T, int LN>
-__global__ void __launch_bounds__(TH, 3) scan_backward_kernel(const ttt_b200_scan_args p, const Plan q) {
+__global__ void __launch_bounds__(TH, LN <= 4 ? 4 : 3) scan_backward_kernel(const ttt_b200_scan_args p, const Plan q) {
+  constexpr bool kKeep = LN > 4;
   using S = Shape<LN>;
   constexpr int DC = S::DC, NP = S::NP, ND = 32 / LN;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -673,7 +676,7 @@ __global__ void __launch_bounds__(TH, 3) scan_backward_kernel(const ttt_b200_sca
     }
 #pragma unroll 1
     for (int s = kTile / kSub - 1; s >= 0; --s) {
-      float2 f[2][kSub][2], h[2][kSub + 1][2];      // factors; states before token k of the run
+      float2 f[2][kKeep ? kSub : 1][2], h[2][kSub + 1][2];      // factors; states before token k of the run
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         h[e][0][0] = h0[e][0];
@@ -690,8 +693,9 @@ __global__ void __launch_bounds__(TH, 3) scan_backward_kernel(const ttt_b200_sca
           const float2 u = *reinterpret_cast<const float2*>(m.u + t * DC + me.ch[e]);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            f[e][k][j] = decay(u.x, a2[e][j]);
-            h[e][k + 1][j] = fma2(f[e][k][j], h[e][k][j], mul2(both(u.y), b[j]));
+            const float2 r = decay(u.x, a2[e][j]);
+            if constexpr (kKeep) f[e][k][j] = r;
+            h[e][k + 1][j] = fma2(r, h[e][k][j], mul2(both(u.y), b[j]));
           }
         }
       }
@@ -713,7 +717,7 @@ __global__ void __launch_bounds__(TH, 3) scan_backward_kernel(const ttt_b200_sca
             vb[j] = e ? fma2(both(u.y), g, vb[j]) : mul2(both(u.y), g);
             vc[j] = e ? fma2(both(gy), h[e][k + 1][j], vc[j]) : mul2(both(gy), h[e][k + 1][j]);
             gb = j ? fma2(g, b[j], gb) : mul2(g, b[j]);
-            carry[e][j] = mul2(f[e][k][j], g);
+            carry[e][j] = mul2(kKeep ? f[e][kKeep ? k : 0][j] : decay(u.x, a2[e][j]), g);
             const float2 r = mul2(carry[e][j], h[e][k][j]);
             qa = j ? fma2(r, a2[e][j], qa) : mul2(r, a2[e][j]);
             da[e][j] = fma2(both(u.x), r, da[e][j]);
@@ -920,20 +924,30 @@ int check(const ttt_b200_scan_args* p) {
 
 // Tokens to a chunk.  Without chunks the kernels need an SM's worth of CTAs next to each other to cover their latencies; with them
 // every token's exponentials are worked out once more, by the state kernel.  Measured at 2048 tokens of N = 16, us without / with
-// chunks: forward of 96 CTAs 244 / 164, of 256 301 / 393; backward of 96 CTAs 680 / 350, of 256 915 / 850, of 384 1160 / 1390.  So
-// the forward is split below one CTA to an SM, the backward below two, into some eight to an SM (four to sixteen are within 5 %), and
-// short sequences into single tiles (512 tokens of 256 channels, 32 chunks: 62 -> 20); the joining kernel walks over the chunks, at
-// most 128 of them.
+// chunks: forward of 96 CTAs 244 / 160, of 256 282 / 374; backward of 96 CTAs 680 / 332, of 256 928 / 799, of 384 1160 / 1390.  So the
+// forward is split below one CTA to an SM, the backward below two: into six to sixteen CTAs to an SM, of these the count that leaves
+// the fullest SM least to do (96 CTAs of 128 tiles, backward with 12, 13, 16, 24 chunks: 333, 354, 332, 330), and where there are not
+// that many tiles into single ones (512 tokens of 256 channels: 62 -> 20).  At most 128, which the joining kernel walks over.
 void plan_chunks(Plan& q, const ttt_b200_scan_args& p, bool backward) {
   const int dc = TH / lanes_of(p.N) * 2;
   q.per = p.D / p.G;
   q.tiles = (q.per + dc - 1) / dc;
   q.nck = (p.T + kTile - 1) / kTile;
   const long ctas = static_cast<long>(p.B) * p.G * q.tiles, sms = sm_count();
-  long chunks = 1;
-  if (ctas < (backward ? 2 : 1) * sms) chunks = std::max<long>(1, std::min<long>({(8 * sms + ctas - 1) / ctas, q.nck, 128}));
-  const int per = static_cast<int>((q.nck + chunks - 1) / chunks);
-  q.chunk = std::max(per, 1) * kTile;
+  int per = std::max(q.nck, 1);      // tiles of a chunk
+  if (ctas < (backward ? 2 : 1) * sms && q.nck > 1) {
+    const int least = (q.nck + 127) / 128;
+    per = least;
+    long best = 0;
+    for (int t = least; t <= q.nck; ++t) {
+      const long all = ctas * ((q.nck + t - 1) / t);
+      if (all > 16 * sms) continue;
+      if (all < 6 * sms) break;
+      const long cost = (all + sms - 1) / sms * t;
+      if (!best || cost <= best) best = cost, per = t;
+    }
+  }
+  q.chunk = per * kTile;
   q.chunks = std::max(1, (p.T + q.chunk - 1) / q.chunk);
 }
 
