@@ -29,75 +29,79 @@ struct Plan {
   float* part;    // backward: [ctas * side][5][D]
 };
 
-// A vector of a thread: eight neighbouring values as four pairs, or, where rows do not start on 16-byte boundaries, one value.
-template <int V> struct Vec;
-template <> struct Vec<8> {
-  using F = float2;
-  static constexpr int N = 4;
+// A thread holds a token's values in vectors of eight, as four pairs.  Where all rows start on 16-byte boundaries (kVec) a vector is
+// eight neighbours, moved as such; otherwise its values are a token's width of threads apart, each moved by itself with the
+// warp's others next to it, and some of the last vector's may not be there.
+constexpr int N = 4;
+using F = float2;
+
+struct Cols {
+  int lane, width, D;      // thread among the token's; those; values of a token
+  template <bool kVec> __device__ __forceinline__ int at(int j, int e) const {      // column of value e of vector j
+    return kVec ? (j * width + lane) * 8 + e : (j * 8 + e) * width + lane;
+  }
+  template <bool kVec> __device__ __forceinline__ bool in(int j, int e = 0) const { return at<kVec>(j, e) < D; }
 };
-template <> struct Vec<1> {
-  using F = float;
-  static constexpr int N = 1;
-};
-template <int V> using Of = typename Vec<V>::F;
+
+__device__ __forceinline__ float& half_of(F& f, int e) { return e ? f.y : f.x; }
+__device__ __forceinline__ float half_of(const F& f, int e) { return e ? f.y : f.x; }
+__device__ __forceinline__ void fill(F (&f)[N], float v) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) f[k] = both(v);
+}
 
 // eight neighbouring values as they lie in memory
-template <class T, int V> struct Raw {
-  static constexpr int kPieces = V * static_cast<int>(sizeof(T)) / 16;
-  alignas(16) T v[V];
+template <class T> struct Raw {
+  static constexpr int kPieces = static_cast<int>(sizeof(T)) / 2;      // of 16 bytes
+  alignas(16) T v[8];
 };
-template <class T, int V> __device__ __forceinline__ void widen(const Raw<T, V>& r, Of<V> (&f)[Vec<V>::N]) {
+template <class T> __device__ __forceinline__ void widen(const Raw<T>& r, F (&f)[N]) {
 #pragma unroll
-  for (int k = 0; k < Vec<V>::N; ++k) {
-    if constexpr (V == 1) f[k] = to_f32(r.v[k]);
-    else if constexpr (std::is_same<T, __nv_bfloat16>::value) f[k] = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(r.v)[k]);
+  for (int k = 0; k < N; ++k) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) f[k] = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(r.v)[k]);
     else if constexpr (std::is_same<T, __half>::value) f[k] = __half22float2(reinterpret_cast<const __half2*>(r.v)[k]);
     else f[k] = make_float2(r.v[2 * k], r.v[2 * k + 1]);
   }
 }
-template <class T, int V> __device__ __forceinline__ void load(const T* p, Of<V> (&f)[Vec<V>::N]) {
-  if constexpr (V == 1) {
-    f[0] = to_f32(*p);
-  } else {
-    Raw<T, V> r;
+// vector j of a row; values that are not there become `none`
+template <bool kVec, class T> __device__ __forceinline__ void load(const T* row, const Cols& c, int j, F (&f)[N], float none = 0.f) {
+  if constexpr (kVec) {
+    Raw<T> r;
 #pragma unroll
-    for (int i = 0; i < Raw<T, V>::kPieces; ++i) {
-      reinterpret_cast<uint4*>(r.v)[i] = reinterpret_cast<const uint4*>(p)[i];
-    }
-    widen<T, V>(r, f);
+    for (int i = 0; i < Raw<T>::kPieces; ++i) reinterpret_cast<uint4*>(r.v)[i] = reinterpret_cast<const uint4*>(row + c.at<true>(j, 0))[i];
+    widen(r, f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) half_of(f[e / 2], e % 2) = c.in<false>(j, e) ? to_f32(row[c.at<false>(j, e)]) : none;
   }
 }
-template <class T, int V> __device__ __forceinline__ void store(T* p, const Of<V> (&f)[Vec<V>::N]) {
-  if constexpr (V == 1) {
-    *p = from_f32<T>(f[0]);
-  } else {
-    Raw<T, V> r;
+template <bool kVec, class T> __device__ __forceinline__ void store(T* row, const Cols& c, int j, const F (&f)[N]) {
+  if constexpr (kVec) {
+    Raw<T> r;
 #pragma unroll
-    for (int k = 0; k < Vec<V>::N; ++k) {
+    for (int k = 0; k < N; ++k) {
       if constexpr (std::is_same<T, __nv_bfloat16>::value) reinterpret_cast<__nv_bfloat162*>(r.v)[k] = __float22bfloat162_rn(f[k]);
       else if constexpr (std::is_same<T, __half>::value) reinterpret_cast<__half2*>(r.v)[k] = __float22half2_rn(f[k]);
       else r.v[2 * k] = f[k].x, r.v[2 * k + 1] = f[k].y;
     }
 #pragma unroll
-    for (int i = 0; i < Raw<T, V>::kPieces; ++i) {
-      reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(r.v)[i];
-    }
-  }
-}
-// a weight's values at column d, or `none` where there is no such weight
-template <int V> __device__ __forceinline__ void weights(const float* p, int d, float none, Of<V> (&f)[Vec<V>::N]) {
-  if (p) {
-    load<float, V>(p + d, f);
+    for (int i = 0; i < Raw<T>::kPieces; ++i) reinterpret_cast<uint4*>(row + c.at<true>(j, 0))[i] = reinterpret_cast<const uint4*>(r.v)[i];
   } else {
 #pragma unroll
-    for (int k = 0; k < Vec<V>::N; ++k) f[k] = all<Of<V>>(none);
+    for (int e = 0; e < 8; ++e)
+      if (c.in<false>(j, e)) row[c.at<false>(j, e)] = from_f32<T>(half_of(f[e / 2], e % 2));
   }
+}
+// a weight's values, or `none` where there is no such weight
+template <bool kVec> __device__ __forceinline__ void weights(const float* p, const Cols& c, int j, float none, F (&f)[N]) {
+  if (p) load<kVec>(p, c, j, f, none);
+  else fill(f, none);
 }
 
 // The gate: its value, and with kSlope its derivative.  GELU as x sigmoid(2 u): no 1 + tanh(u), which cancels on the left.  The
 // derivative needs 1 - sigmoid without its cancellation on the right, which is e times sigmoid; the exponent is bounded there so
 // that this is not infinity times 0.
-template <int kKind, bool kSlope, class F> __device__ __forceinline__ void gate_one(F x, F& v, F& s) {
+template <int kKind, bool kSlope> __device__ __forceinline__ void gate_one(F x, F& v, F& s) {
   constexpr float k = 1.5957691216057308f, c = 0.044715f;      // 2 sqrt(2 / pi)
   F e;
   const F q = times(x, x);
@@ -118,7 +122,7 @@ template <int kKind, bool kSlope, class F> __device__ __forceinline__ void gate_
     }
   }
 }
-template <bool kSlope, class F, int N> __device__ __forceinline__ void gate(int kind, const F (&x)[N], F (&v)[N], F (&s)[N]) {
+template <bool kSlope> __device__ __forceinline__ void gate(int kind, const F (&x)[N], F (&v)[N], F (&s)[N]) {
   if (kind == TTT_B200_ACT_SILU) {
 #pragma unroll
     for (int k = 0; k < N; ++k) gate_one<TTT_B200_ACT_SILU, kSlope>(x[k], v[k], s[k]);
@@ -153,9 +157,6 @@ __device__ __forceinline__ float2 row_sum(float2 v, float2 (*smem)[32], int& buf
   return up ? make_float2(other, s) : make_float2(s, other);
 }
 
-// column of vector j of this thread
-template <int V> __device__ __forceinline__ int column(int j, int lane, int width) { return (j * width + lane) * V; }
-
 // A thread's values of a tensor's rows, token after token at a fixed distance; a tensor that is not there is all zeros.
 //   kOwn     vectors of eight: the next row is copied into the thread's own places in shared memory while it works on this one: no
 //            barrier, no registers, and past the L1, which keeps the weights
@@ -163,50 +164,50 @@ template <int V> __device__ __forceinline__ int column(int j, int lane, int widt
 //            neighbours of the row as well), and each value is picked out at the row's offset; needs a barrier in front of `get`
 //   kDirect  from global memory
 enum { kDirect, kOwn, kWindow };
-template <class T, int V, int NV, int kMode> struct Feed {
-  static_assert(kMode != kOwn || (V == 8 && NV == 1), "one vector of eight to a thread");
+template <class T, bool kVec, int kMode> struct Feed {
   const T* base;      // NULL: no such tensor
   int64_t stride;
   uint32_t slot;      // shared address of the first stage, the same for all threads
   __host__ __device__ static constexpr uint32_t window(int D) { return (static_cast<uint32_t>(D) * sizeof(T) + 30) / 16 * 16; }
   // bytes of one stage
   __host__ __device__ static uint32_t bytes(int threads, int side, int D) {
-    return kMode == kOwn ? V * static_cast<int>(sizeof(T)) * threads : kMode == kWindow ? side * window(D) : 0;
+    return kMode == kOwn ? 8 * static_cast<int>(sizeof(T)) * threads : kMode == kWindow ? side * window(D) : 0;
   }
   __device__ __forceinline__ Feed(const void* p, int64_t stride, uint32_t& smem, int side, int D) : base(static_cast<const T*>(p)), stride(stride), slot(smem) {
     if (base) smem += 2 * bytes(blockDim.x, side, D);
   }
   __device__ __forceinline__ static uint32_t place(int sub, int D) { return kMode == kOwn ? threadIdx.x * 16 : sub * window(D); }
-  // row m into a stage; `some`: this thread has columns
-  __device__ __forceinline__ void ahead(long m, bool some, uint32_t to, int lane, int sub, int width, int D) const {
+  // row m into a stage
+  __device__ __forceinline__ void ahead(long m, uint32_t to, const Cols& c, int sub) const {
     if (!base) return;
-    to += slot + place(sub, D);
-    if constexpr (kMode == kOwn) {
-      if (!some) return;
-      const T* from = base + m * stride + lane * V;
+    to += slot + place(sub, c.D);
+    if constexpr (kMode == kOwn) {      // (one vector to a thread)
+      if (!c.in<true>(0)) return;
+      const T* from = base + m * stride + c.at<true>(0, 0);
 #pragma unroll
-      for (int i = 0; i < Raw<T, V>::kPieces; ++i) cp_async16_at(to + i * 16 * blockDim.x, from + i * (16 / static_cast<int>(sizeof(T))));
+      for (int i = 0; i < Raw<T>::kPieces; ++i) cp_async16_at(to + i * 16 * blockDim.x, from + i * (16 / static_cast<int>(sizeof(T))));
     } else if constexpr (kMode == kWindow) {
       const uintptr_t at = reinterpret_cast<uintptr_t>(base + m * stride), begin = at & ~static_cast<uintptr_t>(15);
-      const int span = D * static_cast<int>(sizeof(T)) + static_cast<int>(at - begin);
-      for (int c = 16 * lane; c < span; c += 16 * width) cp_async16_at(to + c, reinterpret_cast<const char*>(begin) + c, min(16, span - c));
+      const int span = c.D * static_cast<int>(sizeof(T)) + static_cast<int>(at - begin);
+      for (int o = 16 * c.lane; o < span; o += 16 * c.width) cp_async16_at(to + o, reinterpret_cast<const char*>(begin) + o, min(16, span - o));
     }
   }
-  // vector of row m at column d, which is there
-  __device__ __forceinline__ void get(long m, uint32_t from, int d, int sub, int D, Of<V> (&f)[Vec<V>::N]) const {
+  // vector j of row m, of which this thread has some
+  __device__ __forceinline__ void get(long m, uint32_t from, const Cols& c, int j, int sub, F (&f)[N]) const {
     if (!base) {
-#pragma unroll
-      for (int k = 0; k < Vec<V>::N; ++k) f[k] = all<Of<V>>(0.f);
+      fill(f, 0.f);
     } else if constexpr (kMode == kOwn) {
-      Raw<T, V> r;
+      Raw<T> r;
 #pragma unroll
-      for (int i = 0; i < Raw<T, V>::kPieces; ++i) reinterpret_cast<uint4*>(r.v)[i] = shared_load16(slot + from + place(sub, D) + i * 16 * blockDim.x);
-      widen<T, V>(r, f);
+      for (int i = 0; i < Raw<T>::kPieces; ++i) reinterpret_cast<uint4*>(r.v)[i] = shared_load16(slot + from + place(sub, c.D) + i * 16 * blockDim.x);
+      widen(r, f);
     } else if constexpr (kMode == kWindow) {
-      const uint32_t offset = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base + m * stride)) & 15;
-      f[0] = shared_load<T>(slot + from + place(sub, D) + offset + d * static_cast<int>(sizeof(T)));
+      const uint32_t at = slot + from + place(sub, c.D) + (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base + m * stride)) & 15);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        half_of(f[e / 2], e % 2) = c.in<false>(j, e) ? shared_load<T>(at + c.at<false>(j, e) * static_cast<int>(sizeof(T))) : 0.f;
     } else {
-      load<T, V>(base + m * stride + d, f);
+      load<kVec>(base + m * stride, c, j, f);
     }
   }
 };
@@ -218,12 +219,14 @@ struct Shared {
   float columns[32];
   float4 stats[2][32];      // backward: each warp's token's
 };
-template <int V, int NV> __device__ __forceinline__ void count_columns(Shared& sh, int width, int D) {
+template <bool kVec, int NV> __device__ __forceinline__ void count_columns(Shared& sh, const Cols& c) {
   if (threadIdx.x < 32) {
-    int n = 0;      // of warp threadIdx.x of a token: NV runs of 32 V
+    const int first = 32 * static_cast<int>(threadIdx.x);
+    int n = 0;      // of warp threadIdx.x of a token: NV runs of 256, or 8 NV of 32
+    if (first < c.width) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (32 * static_cast<int>(threadIdx.x) < width) n += min(max(D - (j * width + 32 * static_cast<int>(threadIdx.x)) * V, 0), 32 * V);
+      for (int j = 0; j < (kVec ? NV : 8 * NV); ++j) n += min(max(c.D - (j * c.width + first) * (kVec ? 8 : 1), 0), kVec ? 256 : 32);
+    }
     sh.columns[threadIdx.x] = static_cast<float>(n);
   }
   __syncthreads();
@@ -231,9 +234,9 @@ template <int V, int NV> __device__ __forceinline__ void count_columns(Shared& s
 
 // Mean and 1 / deviation of a row with one barrier: each warp's mean and its squares about it, joined as
 // sum over warps of (squares + columns (mean of the warp - mean)^2).
-template <int V, int NV>
-__device__ __forceinline__ float2 statistics(const Of<V> (&a)[NV][Vec<V>::N], const ttt_b200_block_args& p, int lane, int width, Shared& sh, int& buf) {
-  using F = Of<V>;
+template <bool kVec, int NV>
+__device__ __forceinline__ float2 statistics(const F (&a)[NV][N], const ttt_b200_block_args& p, const Cols& c, Shared& sh, int& buf) {
+  const int width = c.width;
   const float inv = 1.f / static_cast<float>(p.D);
   float mean = 0.f;
   if (p.layer) {
@@ -241,20 +244,21 @@ __device__ __forceinline__ float2 statistics(const Of<V> (&a)[NV][Vec<V>::N], co
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int k = 0; k < Vec<V>::N; ++k) s = plus(s, a[j][k]);      // (zeros behind the last column)
+      for (int k = 0; k < N; ++k) s = plus(s, a[j][k]);      // (zeros behind the last column)
     mean = fold(s);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
-    mean *= rcp(fmaxf(sh.columns[lane >> 5], 1.f));
+    mean *= rcp(fmaxf(sh.columns[c.lane >> 5], 1.f));
   }
-  F sq = all<F>(0.f);
+  F sq = both(0.f);
 #pragma unroll
   for (int j = 0; j < NV; ++j)
-    if (column<V>(j, lane, width) < p.D) {
+    if (c.in<kVec>(j)) {
 #pragma unroll
-      for (int k = 0; k < Vec<V>::N; ++k) {
-        const F v = plus(a[j][k], all<F>(-mean));
-        sq = mac(v, v, sq);
+      for (int k = 0; k < N; ++k) {
+        F v = add2(a[j][k], both(-mean));
+        if (!kVec) v = make_float2(c.in<kVec>(j, 2 * k) ? v.x : 0.f, c.in<kVec>(j, 2 * k + 1) ? v.y : 0.f);
+        sq = fma2(v, v, sq);
       }
     }
   float q = fold(sq);
@@ -281,32 +285,30 @@ __device__ __forceinline__ float2 statistics(const Of<V> (&a)[NV][Vec<V>::N], co
   return make_float2(mean, rsqrtf(fmaf(q, inv, p.eps)));
 }
 
-template <class T, class R, int V, int NV, int kThreads>
+template <class T, class R, bool kVec, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kernel(const ttt_b200_block_args p, const Plan q) {
-  using F = Of<V>;
-  constexpr int kMode = V > 1 ? kOwn : kWindow;
-  constexpr int N = Vec<V>::N;
+  constexpr int kMode = kVec ? kOwn : kWindow, NV = 1;
   __shared__ Shared sh;
   extern __shared__ __align__(16) unsigned char stages[];
   uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(stages));
   int buf = 0;
   const int lane = threadIdx.x % q.width, sub = threadIdx.x / q.width;
+  const Cols c = {lane, q.width, p.D};
   const long step = static_cast<long>(q.ctas) * q.side;
-  const Feed<T, V, NV, kMode> fo(p.o, p.o_stride, at, q.side, p.D), fg(p.gate, p.gate_stride, at, q.side, p.D);
-  const Feed<R, V, NV, kMode> fx(p.residual, p.residual_stride, at, q.side, p.D);
-  const uint32_t small = Feed<T, V, NV, kMode>::bytes(blockDim.x, q.side, p.D), large = Feed<R, V, NV, kMode>::bytes(blockDim.x, q.side, p.D);
-  const bool some = lane * V < p.D;      // this thread has columns
+  const Feed<T, kVec, kMode> fo(p.o, p.o_stride, at, q.side, p.D), fg(p.gate, p.gate_stride, at, q.side, p.D);
+  const Feed<R, kVec, kMode> fx(p.residual, p.residual_stride, at, q.side, p.D);
+  const uint32_t small = Feed<T, kVec, kMode>::bytes(blockDim.x, q.side, p.D), large = Feed<R, kVec, kMode>::bytes(blockDim.x, q.side, p.D);
   auto ahead = [&](long m, int stage) {
     if (m < p.M) {
-      fo.ahead(m, some, stage * small, lane, sub, q.width, p.D);
-      fg.ahead(m, some, stage * small, lane, sub, q.width, p.D);
-      fx.ahead(m, some, stage * large, lane, sub, q.width, p.D);
+      fo.ahead(m, stage * small, c, sub);
+      fg.ahead(m, stage * small, c, sub);
+      fx.ahead(m, stage * large, c, sub);
     }
     cp_async_commit();
   };
   long m = static_cast<long>(blockIdx.x) * q.side + sub;
   ahead(m, 0);
-  count_columns<V, NV>(sh, q.width, p.D);
+  count_columns<kVec, NV>(sh, c);
   int stage = 0;
   for (long base = static_cast<long>(blockIdx.x) * q.side; base < p.M; base += step, stage ^= 1, m += step) {
     const bool live = m < p.M;
@@ -316,49 +318,46 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kerne
     F a[NV][N], z[NV][N];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int d = column<V>(j, lane, q.width);
 #pragma unroll
-      for (int k = 0; k < N; ++k) a[j][k] = z[j][k] = all<F>(0.f);
-      if (live && d < p.D) fo.get(m, stage * small, d, sub, p.D, a[j]);
+      for (int k = 0; k < N; ++k) a[j][k] = z[j][k] = both(0.f);
+      if (live && c.in<kVec>(j)) fo.get(m, stage * small, c, j, sub, a[j]);
     }
     float2 s1 = make_float2(0.f, 1.f), s2 = s1;
-    if (p.post_weight) s1 = statistics<V, NV>(a, p, lane, q.width, sh, buf);
+    if (p.post_weight) s1 = statistics<kVec, NV>(a, p, c, sh, buf);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int d = column<V>(j, lane, q.width);
-      if (!(live && d < p.D)) continue;
+      if (!(live && c.in<kVec>(j))) continue;
       F w[N], b[N];
       if (p.post_weight) {
-        weights<V>(p.post_weight, d, 0.f, w);
-        weights<V>(p.post_bias, d, 0.f, b);
+        weights<kVec>(p.post_weight, c, j, 0.f, w);
+        weights<kVec>(p.post_bias, c, j, 0.f, b);
 #pragma unroll
-        for (int k = 0; k < N; ++k) a[j][k] = mac(times(plus(a[j][k], all<F>(-s1.x)), all<F>(s1.y)), w[k], b[k]);
+        for (int k = 0; k < N; ++k) a[j][k] = mac(times(plus(a[j][k], both(-s1.x)), both(s1.y)), w[k], b[k]);
       }
       if (p.gate) {
         F g[N];
-        fg.get(m, stage * small, d, sub, p.D, g);
+        fg.get(m, stage * small, c, j, sub, g);
         gate<false>(p.activation, g, g, w);
 #pragma unroll
         for (int k = 0; k < N; ++k) a[j][k] = times(a[j][k], g[k]);
       }
-      fx.get(m, stage * large, d, sub, p.D, z[j]);
-      weights<V>(p.scale, d, 1.f, w);
+      fx.get(m, stage * large, c, j, sub, z[j]);
+      weights<kVec>(p.scale, c, j, 1.f, w);
 #pragma unroll
       for (int k = 0; k < N; ++k) z[j][k] = mac(w[k], a[j][k], z[j][k]);
-      store<R, V>(static_cast<R*>(p.x) + m * p.D + d, z[j]);
+      store<kVec>(static_cast<R*>(p.x) + m * p.D, c, j, z[j]);
     }
     if (p.pre_weight) {
-      s2 = statistics<V, NV>(z, p, lane, q.width, sh, buf);
+      s2 = statistics<kVec, NV>(z, p, c, sh, buf);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int d = column<V>(j, lane, q.width);
-        if (live && d < p.D) {
+        if (live && c.in<kVec>(j)) {
           F w[N], b[N];
-          weights<V>(p.pre_weight, d, 0.f, w);
-          weights<V>(p.pre_bias, d, 0.f, b);
+          weights<kVec>(p.pre_weight, c, j, 0.f, w);
+          weights<kVec>(p.pre_bias, c, j, 0.f, b);
 #pragma unroll
-          for (int k = 0; k < N; ++k) z[j][k] = mac(times(plus(z[j][k], all<F>(-s2.x)), all<F>(s2.y)), w[k], b[k]);
-          store<T, V>(static_cast<T*>(p.n) + m * p.D + d, z[j]);
+          for (int k = 0; k < N; ++k) z[j][k] = mac(times(plus(z[j][k], both(-s2.x)), both(s2.y)), w[k], b[k]);
+          store<kVec>(static_cast<T*>(p.n) + m * p.D, c, j, z[j]);
         }
       }
     }
@@ -368,67 +367,66 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kerne
 
 // Sums over tokens of a thread's columns: in registers, or, of sixteen columns, in shared memory.
 enum { kDw1, kDb1, kDsc, kDw2, kDb2, kSums };
-template <int V, int NV, bool kShared> struct Sums {
-  using F = Of<V>;
-  F r[kShared ? 1 : kSums][NV][Vec<V>::N];
+template <bool kVec, int NV, bool kShared> struct Sums {
+  F r[kShared ? 1 : kSums][NV][N];
   float* s;
-  int D;
-  __device__ __forceinline__ F& at(int k, int j, int i, int d) {
-    if constexpr (kShared) return reinterpret_cast<F*>(s + k * D + d)[i];
-    else return r[k][j][i];
+  __device__ __forceinline__ F get(int k, int j, int i, const Cols& c) const {
+    if constexpr (!kShared) return r[k][j][i];
+    else if constexpr (kVec) return *reinterpret_cast<const F*>(s + k * c.D + c.at<true>(j, 2 * i));
+    else return make_float2(c.in<false>(j, 2 * i) ? s[k * c.D + c.at<false>(j, 2 * i)] : 0.f, c.in<false>(j, 2 * i + 1) ? s[k * c.D + c.at<false>(j, 2 * i + 1)] : 0.f);
   }
-  __device__ __forceinline__ void add(int k, int j, int i, int d, F v) {
-    F& t = at(k, j, i, d);
-    t = plus(t, v);
+  __device__ __forceinline__ void set(int k, int j, int i, const Cols& c, F v) {
+    if constexpr (!kShared) {
+      r[k][j][i] = v;
+    } else if constexpr (kVec) {
+      *reinterpret_cast<F*>(s + k * c.D + c.at<true>(j, 2 * i)) = v;
+    } else {
+      if (c.in<false>(j, 2 * i)) s[k * c.D + c.at<false>(j, 2 * i)] = v.x;
+      if (c.in<false>(j, 2 * i + 1)) s[k * c.D + c.at<false>(j, 2 * i + 1)] = v.y;
+    }
   }
-  __device__ __forceinline__ void add(int k, int j, int i, int d, F a, F b) {
-    F& t = at(k, j, i, d);
-    t = mac(a, b, t);
-  }
+  __device__ __forceinline__ void add(int k, int j, int i, const Cols& c, F v) { set(k, j, i, c, add2(get(k, j, i, c), v)); }
+  __device__ __forceinline__ void add(int k, int j, int i, const Cols& c, F a, F b) { set(k, j, i, c, fma2(a, b, get(k, j, i, c))); }
 };
 
-template <class T, class R, int V, int NV, bool kShared, int kThreads>
+template <class T, class R, bool kVec, int NV, bool kShared, int kThreads>
 __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1) block_backward_kernel(const ttt_b200_block_args p, const Plan q) {
-  using F = Of<V>;
-  constexpr int kMode = kShared ? kDirect : V > 1 ? kOwn : kWindow;
-  constexpr int N = Vec<V>::N;
+  constexpr int kMode = kShared ? kDirect : kVec ? kOwn : kWindow;
   __shared__ Shared sh;
   extern __shared__ __align__(16) unsigned char stages[];
   uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(stages));
   int buf = 0;
   const int lane = threadIdx.x % q.width, sub = threadIdx.x / q.width;
+  const Cols c = {lane, q.width, p.D};
   const long step = static_cast<long>(q.ctas) * q.side;
-  const Feed<T, V, NV, kMode> fo(p.o, p.o_stride, at, q.side, p.D), fg(p.gate, p.gate_stride, at, q.side, p.D);
-  const Feed<T, V, NV, kMode> fn(p.pre_weight ? p.grad_n : nullptr, p.gn_stride, at, q.side, p.D);
-  const Feed<R, V, NV, kMode> fx(p.pre_weight ? p.residual : nullptr, p.residual_stride, at, q.side, p.D);
-  const Feed<R, V, NV, kMode> fd(p.grad_x, p.gx_stride, at, q.side, p.D);
-  const uint32_t small = Feed<T, V, NV, kMode>::bytes(blockDim.x, q.side, p.D), large = Feed<R, V, NV, kMode>::bytes(blockDim.x, q.side, p.D);
-  const bool some = lane * V < p.D;
+  const Feed<T, kVec, kMode> fo(p.o, p.o_stride, at, q.side, p.D), fg(p.gate, p.gate_stride, at, q.side, p.D);
+  const Feed<T, kVec, kMode> fn(p.pre_weight ? p.grad_n : nullptr, p.gn_stride, at, q.side, p.D);
+  const Feed<R, kVec, kMode> fx(p.pre_weight ? p.residual : nullptr, p.residual_stride, at, q.side, p.D);
+  const Feed<R, kVec, kMode> fd(p.grad_x, p.gx_stride, at, q.side, p.D);
+  const uint32_t small = Feed<T, kVec, kMode>::bytes(blockDim.x, q.side, p.D), large = Feed<R, kVec, kMode>::bytes(blockDim.x, q.side, p.D);
   const uint32_t stats = static_cast<uint32_t>(__cvta_generic_to_shared(&sh.stats[0][threadIdx.x >> 5]));
   auto ahead = [&](long m, int stage) {
     if (m < p.M) {
       if ((threadIdx.x & 31) == 0) cp_async16_at(stats + stage * static_cast<uint32_t>(sizeof(sh.stats[0])), p.stats + 4 * m);
-      fo.ahead(m, some, stage * small, lane, sub, q.width, p.D);
-      fg.ahead(m, some, stage * small, lane, sub, q.width, p.D);
-      fn.ahead(m, some, stage * small, lane, sub, q.width, p.D);
-      fx.ahead(m, some, stage * large, lane, sub, q.width, p.D);
-      fd.ahead(m, some, stage * large, lane, sub, q.width, p.D);
+      fo.ahead(m, stage * small, c, sub);
+      fg.ahead(m, stage * small, c, sub);
+      fn.ahead(m, stage * small, c, sub);
+      fx.ahead(m, stage * large, c, sub);
+      fd.ahead(m, stage * large, c, sub);
     }
     cp_async_commit();
   };
   const float inv = 1.f / static_cast<float>(p.D);
-  Sums<V, NV, kShared> sums;
+  Sums<kVec, NV, kShared> sums;
   sums.s = reinterpret_cast<float*>(stages);
-  sums.D = p.D;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int d = column<V>(j, lane, q.width);
+  for (int j = 0; j < NV; ++j)
+    if (!kShared || c.in<kVec>(j)) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+      for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int k = 0; k < kSums; ++k)
-        if (!kShared || d < p.D) sums.at(k, j, i, d) = all<F>(0.f);
-  }
+        for (int k = 0; k < kSums; ++k) sums.set(k, j, i, c, both(0.f));
+    }
   long m = static_cast<long>(blockIdx.x) * q.side + sub;
   ahead(m, 0);
   int stage = 0;
@@ -442,44 +440,43 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
     if (live) st = sh.stats[stage][threadIdx.x >> 5];
     F o[NV][N], z[NV][N], gn[NV][N], d2[NV][N];
     // u (with its norm: oh) and z again, as the forward had them; z is its normalised value
-    F sx = all<F>(0.f), sy = sx;
+    F sx = both(0.f), sy = sx;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int d = column<V>(j, lane, q.width);
-      const bool in = live && d < p.D;
+      const bool in = live && c.in<kVec>(j);
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[j][i] = all<F>(0.f);
-      if (in) fo.get(m, stage * small, d, sub, p.D, o[j]);
+      for (int i = 0; i < N; ++i) o[j][i] = both(0.f);
+      if (in) fo.get(m, stage * small, c, j, sub, o[j]);
       if (p.post_weight) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) o[j][i] = times(plus(o[j][i], all<F>(-st.x)), all<F>(st.y));
+        for (int i = 0; i < N; ++i) o[j][i] = times(plus(o[j][i], both(-st.x)), both(st.y));
       }
       if (!p.pre_weight || !in) continue;
       F u[N], w[N], b[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) u[i] = o[j][i];
       if (p.post_weight) {
-        weights<V>(p.post_weight, d, 0.f, w);
-        weights<V>(p.post_bias, d, 0.f, b);
+        weights<kVec>(p.post_weight, c, j, 0.f, w);
+        weights<kVec>(p.post_bias, c, j, 0.f, b);
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = mac(o[j][i], w[i], b[i]);
       }
       if (p.gate) {
-        fg.get(m, stage * small, d, sub, p.D, w);
+        fg.get(m, stage * small, c, j, sub, w);
         gate<false>(p.activation, w, w, b);
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = times(u[i], w[i]);
       }
-      weights<V>(p.scale, d, 1.f, w);
-      fx.get(m, stage * large, d, sub, p.D, z[j]);
+      weights<kVec>(p.scale, c, j, 1.f, w);
+      fx.get(m, stage * large, c, j, sub, z[j]);
 #pragma unroll
-      for (int i = 0; i < N; ++i) z[j][i] = times(plus(mac(w[i], u[i], z[j][i]), all<F>(-st.z)), all<F>(st.w));
-      fn.get(m, stage * small, d, sub, p.D, gn[j]);
-      weights<V>(p.pre_weight, d, 0.f, w);
+      for (int i = 0; i < N; ++i) z[j][i] = times(plus(mac(w[i], u[i], z[j][i]), both(-st.z)), both(st.w));
+      fn.get(m, stage * small, c, j, sub, gn[j]);
+      weights<kVec>(p.pre_weight, c, j, 0.f, w);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        sums.add(kDw2, j, i, d, gn[j][i], z[j][i]);
-        sums.add(kDb2, j, i, d, gn[j][i]);
+        sums.add(kDw2, j, i, c, gn[j][i], z[j][i]);
+        sums.add(kDb2, j, i, c, gn[j][i]);
         gn[j][i] = times(gn[j][i], w[i]);
         sx = plus(sx, gn[j][i]);
         sy = mac(gn[j][i], z[j][i], sy);
@@ -492,50 +489,49 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
       m1 = p.layer ? s.x * inv : 0.f;
       m2 = s.y * inv;
     }
-    sx = sy = all<F>(0.f);
+    sx = sy = both(0.f);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int d = column<V>(j, lane, q.width);
-      if (!(live && d < p.D)) continue;
-      fd.get(m, stage * large, d, sub, p.D, d2[j]);
+      if (!(live && c.in<kVec>(j))) continue;
+      fd.get(m, stage * large, c, j, sub, d2[j]);
       if (p.pre_weight) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) d2[j][i] = mac(all<F>(st.w), mac(z[j][i], all<F>(-m2), plus(gn[j][i], all<F>(-m1))), d2[j][i]);
+        for (int i = 0; i < N; ++i) d2[j][i] = mac(both(st.w), mac(z[j][i], both(-m2), plus(gn[j][i], both(-m1))), d2[j][i]);
       }
-      if (p.grad_residual) store<R, V>(static_cast<R*>(p.grad_residual) + m * p.D + d, d2[j]);
+      if (p.grad_residual) store<kVec>(static_cast<R*>(p.grad_residual) + m * p.D, c, j, d2[j]);
       F u[N], w[N], b[N], v[N], g[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) u[i] = o[j][i];
       if (p.post_weight) {
-        weights<V>(p.post_weight, d, 0.f, w);
-        weights<V>(p.post_bias, d, 0.f, b);
+        weights<kVec>(p.post_weight, c, j, 0.f, w);
+        weights<kVec>(p.post_bias, c, j, 0.f, b);
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = mac(o[j][i], w[i], b[i]);
       }
-      weights<V>(p.scale, d, 1.f, b);
+      weights<kVec>(p.scale, c, j, 1.f, b);
       if (p.gate) {
-        fg.get(m, stage * small, d, sub, p.D, g);
+        fg.get(m, stage * small, c, j, sub, g);
         gate<true>(p.activation, g, v, g);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          sums.add(kDsc, j, i, d, d2[j][i], times(u[i], v[i]));
+          sums.add(kDsc, j, i, c, d2[j][i], times(u[i], v[i]));
           d2[j][i] = times(d2[j][i], b[i]);
           g[i] = times(times(d2[j][i], u[i]), g[i]);
           d2[j][i] = times(d2[j][i], v[i]);
         }
-        store<T, V>(static_cast<T*>(p.grad_gate) + m * p.D + d, g);
+        store<kVec>(static_cast<T*>(p.grad_gate) + m * p.D, c, j, g);
       } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          sums.add(kDsc, j, i, d, d2[j][i], u[i]);
+          sums.add(kDsc, j, i, c, d2[j][i], u[i]);
           d2[j][i] = times(d2[j][i], b[i]);
         }
       }
       if (p.post_weight) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          sums.add(kDw1, j, i, d, d2[j][i], o[j][i]);
-          sums.add(kDb1, j, i, d, d2[j][i]);
+          sums.add(kDw1, j, i, c, d2[j][i], o[j][i]);
+          sums.add(kDb1, j, i, c, d2[j][i]);
           d2[j][i] = times(d2[j][i], w[i]);
           sx = plus(sx, d2[j][i]);
           sy = mac(d2[j][i], o[j][i], sy);
@@ -549,26 +545,24 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int d = column<V>(j, lane, q.width);
-      if (!(live && d < p.D)) continue;
+      if (!(live && c.in<kVec>(j))) continue;
       if (p.post_weight) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) d2[j][i] = times(all<F>(st.y), mac(o[j][i], all<F>(-m2), plus(d2[j][i], all<F>(-m1))));
+        for (int i = 0; i < N; ++i) d2[j][i] = times(both(st.y), mac(o[j][i], both(-m2), plus(d2[j][i], both(-m1))));
       }
-      store<T, V>(static_cast<T*>(p.grad_o) + m * p.D + d, d2[j]);
+      store<kVec>(static_cast<T*>(p.grad_o) + m * p.D, c, j, d2[j]);
     }
   }
   float* part = q.part + (static_cast<long>(blockIdx.x) * q.side + sub) * kSums * p.D;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int d = column<V>(j, lane, q.width);
-    if (d >= p.D) continue;
+    if (!c.in<kVec>(j)) continue;
 #pragma unroll
     for (int k = 0; k < kSums; ++k) {
       F v[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = sums.at(k, j, i, d);
-      store<float, V>(part + static_cast<long>(k) * p.D + d, v);
+      for (int i = 0; i < N; ++i) v[i] = sums.get(k, j, i, c);
+      store<kVec>(part + static_cast<long>(k) * p.D, c, j, v);
     }
   }
 }
@@ -639,12 +633,12 @@ template <class K> int launch(K kernel, const Plan& q, size_t bytes, cudaStream_
   return launched(what);
 }
 
-template <class T, class R, int V, int NV, int kThreads> int forward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
-  constexpr int kMode = V > 1 ? kOwn : kWindow;
+template <class T, class R, bool kVec, int kThreads> int forward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
+  constexpr int kMode = kVec ? kOwn : kWindow;
   const int n = q.width * q.side;
-  const size_t bytes = 2 * (Feed<T, V, NV, kMode>::bytes(n, q.side, p.D) * (1 + (p.gate != nullptr)) +
-                            Feed<R, V, NV, kMode>::bytes(n, q.side, p.D) * (p.residual != nullptr));
-  return launch(block_forward_kernel<T, R, V, NV, kThreads>, q, bytes, s, p, "block norm");
+  const size_t bytes = 2 * (Feed<T, kVec, kMode>::bytes(n, q.side, p.D) * (1 + (p.gate != nullptr)) +
+                            Feed<R, kVec, kMode>::bytes(n, q.side, p.D) * (p.residual != nullptr));
+  return launch(block_forward_kernel<T, R, kVec, kThreads>, q, bytes, s, p, "block norm");
 }
 
 template <class T, class R> int forward(const ttt_b200_block_args& p, cudaStream_t s) {
@@ -652,18 +646,18 @@ template <class T, class R> int forward(const ttt_b200_block_args& p, cudaStream
   plan(q, p, false);
   const int n = q.width * q.side;
   const bool vec = vectors(p, false);
-  if (n <= 128) return vec ? forward_as<T, R, 8, 1, 128>(p, q, s) : forward_as<T, R, 1, 8, 128>(p, q, s);
-  if (n <= 256) return vec ? forward_as<T, R, 8, 1, 256>(p, q, s) : forward_as<T, R, 1, 8, 256>(p, q, s);
-  return vec ? forward_as<T, R, 8, 1, 1024>(p, q, s) : forward_as<T, R, 1, 8, 1024>(p, q, s);
+  if (n <= 128) return vec ? forward_as<T, R, true, 128>(p, q, s) : forward_as<T, R, false, 128>(p, q, s);
+  if (n <= 256) return vec ? forward_as<T, R, true, 256>(p, q, s) : forward_as<T, R, false, 256>(p, q, s);
+  return vec ? forward_as<T, R, true, 1024>(p, q, s) : forward_as<T, R, false, 1024>(p, q, s);
 }
 
-template <class T, class R, int V, int NV, bool kShared, int kThreads> int backward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
-  constexpr int kMode = kShared ? kDirect : V > 1 ? kOwn : kWindow;
+template <class T, class R, bool kVec, int NV, bool kShared, int kThreads> int backward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
+  constexpr int kMode = kShared ? kDirect : kVec ? kOwn : kWindow;
   const int n = q.width * q.side;
   const size_t bytes = kShared ? static_cast<size_t>(kSums) * p.D * sizeof(float)
-                               : 2 * (Feed<T, V, NV, kMode>::bytes(n, q.side, p.D) * (1 + (p.gate != nullptr) + (p.pre_weight && p.grad_n)) +
-                                          Feed<R, V, NV, kMode>::bytes(n, q.side, p.D) * ((p.pre_weight && p.residual) + (p.grad_x != nullptr)));
-  return launch(block_backward_kernel<T, R, V, NV, kShared, kThreads>, q, bytes, s, p, "block norm backward");
+                               : 2 * (Feed<T, kVec, kMode>::bytes(n, q.side, p.D) * (1 + (p.gate != nullptr) + (p.pre_weight && p.grad_n)) +
+                                          Feed<R, kVec, kMode>::bytes(n, q.side, p.D) * ((p.pre_weight && p.residual) + (p.grad_x != nullptr)));
+  return launch(block_backward_kernel<T, R, kVec, NV, kShared, kThreads>, q, bytes, s, p, "block norm backward");
 }
 
 template <class T, class R> int backward(const ttt_b200_block_args& p, cudaStream_t s) {
@@ -673,10 +667,10 @@ template <class T, class R> int backward(const ttt_b200_block_args& p, cudaStrea
   const bool vec = vectors(p, true);
   const int n = q.width * q.side;
   int rc;
-  if (p.D > kWide) rc = vec ? backward_as<T, R, 8, 2, true, 512>(p, q, s) : backward_as<T, R, 1, 16, true, 512>(p, q, s);
-  else if (n <= 128) rc = vec ? backward_as<T, R, 8, 1, false, 128>(p, q, s) : backward_as<T, R, 1, 8, false, 128>(p, q, s);
-  else if (n <= 256) rc = vec ? backward_as<T, R, 8, 1, false, 256>(p, q, s) : backward_as<T, R, 1, 8, false, 256>(p, q, s);
-  else rc = vec ? backward_as<T, R, 8, 1, false, 512>(p, q, s) : backward_as<T, R, 1, 8, false, 512>(p, q, s);
+  if (p.D > kWide) rc = vec ? backward_as<T, R, true, 2, true, 512>(p, q, s) : backward_as<T, R, false, 2, true, 512>(p, q, s);
+  else if (n <= 128) rc = vec ? backward_as<T, R, true, 1, false, 128>(p, q, s) : backward_as<T, R, false, 1, false, 128>(p, q, s);
+  else if (n <= 256) rc = vec ? backward_as<T, R, true, 1, false, 256>(p, q, s) : backward_as<T, R, false, 1, false, 256>(p, q, s);
+  else rc = vec ? backward_as<T, R, true, 1, false, 512>(p, q, s) : backward_as<T, R, false, 1, false, 512>(p, q, s);
   if (rc) return rc;
   const long row = static_cast<long>(kSums) * p.D;
   float* dst[kSums] = {p.grad_post_weight, p.grad_post_bias, p.grad_scale, p.grad_pre_weight, p.grad_pre_bias};
