@@ -287,6 +287,7 @@ __device__ __forceinline__ float2 statistics(const F (&a)[NV][N], const ttt_b200
 
 template <class T, class R, bool kVec, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kernel(const ttt_b200_block_args p, const Plan q) {
+  wait_for_predecessor();
   constexpr int kMode = kVec ? kOwn : kWindow, NV = 1;
   __shared__ Shared sh;
   extern __shared__ __align__(16) unsigned char stages[];
@@ -391,6 +392,7 @@ template <bool kVec, int NV, bool kShared> struct Sums {
 
 template <class T, class R, bool kVec, int NV, bool kShared, int kThreads>
 __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1) block_backward_kernel(const ttt_b200_block_args p, const Plan q) {
+  wait_for_predecessor();
   constexpr int kMode = kShared ? kDirect : kVec ? kOwn : kWindow;
   __shared__ Shared sh;
   extern __shared__ __align__(16) unsigned char stages[];
@@ -629,7 +631,7 @@ template <class K> int launch(K kernel, const Plan& q, size_t bytes, cudaStream_
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
     if (e != cudaSuccess) return ttt_set_error(TTT_B200_ERR_LAUNCH, cudaGetErrorString(e));
   }
-  kernel<<<q.ctas, q.width * q.side, bytes, s>>>(p, q);
+  ttt_launch_overlapped(kernel, q.ctas, q.width * q.side, static_cast<uint32_t>(bytes), s, p, q);
   return launched(what);
 }
 

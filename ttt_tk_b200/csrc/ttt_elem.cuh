@@ -11,6 +11,10 @@
 
 namespace ttt {
 
+// First statement of every kernel here: the launch may have come before the one in front of it in the stream is through
+// (ttt_launch_overlapped), and nothing global is touched until it is.
+__device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }

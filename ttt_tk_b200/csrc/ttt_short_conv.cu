@@ -187,6 +187,7 @@ template <class T> struct Rows<T, 1> {
 };
 
 template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(32 * kWarps) conv_forward_kernel(const ttt_b200_conv_args p, const Plan q) {
+  wait_for_predecessor();
   using F = typename Channels<V>::F;
   __shared__ __align__(16) unsigned char rings[kWarps][Rows<T, V>::kBytes + 16];
   const At at(q);
@@ -241,6 +242,7 @@ template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(3
 }
 
 template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(32 * kWarps) conv_backward_kernel(const ttt_b200_conv_args p, const Plan q) {
+  wait_for_predecessor();
   using F = typename Channels<V>::F;
   __shared__ __align__(16) unsigned char rings[2][kWarps][Rows<T, V>::kBytes + 16];
   __shared__ float sums[kWarps][K + 1][32 * V];
@@ -353,6 +355,7 @@ template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(3
 // A row of the batch and 128 V channels to a CTA.  Rows that name the same slot are taken in their order by the CTA of the first of
 // them, so that no two CTAs touch a state.
 template <class T, int K, int V> __global__ void __launch_bounds__(128) conv_step_kernel(const ttt_b200_conv_args p, int tiles) {
+  wait_for_predecessor();
   const int b0 = blockIdx.x / tiles, d = (blockIdx.x % tiles * 128 + threadIdx.x) * V;
   const bool live = d < p.D;
   T* ys = static_cast<T*>(p.y);
@@ -459,7 +462,7 @@ template <class T, int K> int forward(const ttt_b200_conv_args& p, cudaStream_t 
   const bool silu = p.activation == TTT_B200_ACT_SILU;
   const auto kernel = vec ? (silu ? conv_forward_kernel<T, K, 2, true> : conv_forward_kernel<T, K, 2, false>)
                           : (silu ? conv_forward_kernel<T, K, 1, true> : conv_forward_kernel<T, K, 1, false>);
-  kernel<<<static_cast<unsigned>(grid), 32 * kWarps, 0, s>>>(p, q);
+  ttt_launch_overlapped(kernel, static_cast<int>(grid), 32 * kWarps, 0, s, p, q);
   return launched("short conv");
 }
 
@@ -475,7 +478,7 @@ template <class T, int K> int backward(const ttt_b200_conv_args& p, cudaStream_t
   const bool silu = p.activation == TTT_B200_ACT_SILU;
   const auto kernel = vec ? (silu ? conv_backward_kernel<T, K, 2, true> : conv_backward_kernel<T, K, 2, false>)
                           : (silu ? conv_backward_kernel<T, K, 1, true> : conv_backward_kernel<T, K, 1, false>);
-  kernel<<<static_cast<unsigned>(grid), 32 * kWarps, 0, s>>>(p, q);
+  ttt_launch_overlapped(kernel, static_cast<int>(grid), 32 * kWarps, 0, s, p, q);
   if (int rc = launched("short conv backward")) return rc;
   const long row = static_cast<long>(K + 1) * p.D, KD = static_cast<long>(K) * p.D;
   const int parts = p.B * q.runs;
@@ -490,8 +493,7 @@ template <class T, int K> int step(const ttt_b200_conv_args& p, cudaStream_t s) 
   const int tiles = (p.D / (vec ? 2 : 1) + 127) / 128;
   const long grid = static_cast<long>(p.B) * tiles;
   if (grid > 0x7fffffffL) return fail("short conv step: too many CTAs");
-  if (vec) conv_step_kernel<T, K, 2><<<static_cast<unsigned>(grid), 128, 0, s>>>(p, tiles);
-  else conv_step_kernel<T, K, 1><<<static_cast<unsigned>(grid), 128, 0, s>>>(p, tiles);
+  ttt_launch_overlapped(vec ? conv_step_kernel<T, K, 2> : conv_step_kernel<T, K, 1>, static_cast<int>(grid), 128, 0, s, p, tiles);
   return launched("short conv step");
 }
 

@@ -263,6 +263,7 @@ template <class T, int LN> struct FwdSmem {
 // One barrier to a tile: between two of them the states walk over tile k, tile k + 1 goes from its copy to fp32 (in registers
 // first, so that its arithmetic fills the gaps of the walk), tile k - 1 leaves, and the copy of tile k + 2 is on its way.
 template <class T, int LN> __global__ void __launch_bounds__(TH, 4) scan_forward_kernel(const ttt_b200_scan_args p, const Plan q) {
+  wait_for_predecessor();
   using S = Shape<LN>;
   constexpr int DC = S::DC, NP = S::NP, U = LN < 4 ? 4 : LN, YW = FwdSmem<T, LN>::YW;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -408,6 +409,7 @@ template <class T, int LN> struct StateSmem {
 };
 
 template <class T, int LN, bool kRev> __global__ void __launch_bounds__(TH, 4) scan_state_kernel(const ttt_b200_scan_args p, const Plan q) {
+  wait_for_predecessor();
   using S = Shape<LN>;
   constexpr int DC = S::DC, NP = S::NP;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -512,6 +514,7 @@ template <class T, int LN, bool kRev> __global__ void __launch_bounds__(TH, 4) s
 
 // The chunks' own states -> the states that they start from (kRev: that they end with), in place, in the order of time.
 template <bool kRev> __global__ void __launch_bounds__(256) scan_join_kernel(const ttt_b200_scan_args p, const Plan q) {
+  wait_for_predecessor();
   const long DN = static_cast<long>(p.D) * p.N;
   const long i = static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (i >= p.B * DN) return;
@@ -569,6 +572,7 @@ template <class T, int LN> struct BwdSmem {
 // instead of three (4 x 2048 x 1536 x 16: 348 -> 332 us); with 64 the exponentials cost more than that gives (191 -> 208).
 template <class T, int LN>
 __global__ void __launch_bounds__(TH, LN <= 4 ? 4 : 3) scan_backward_kernel(const ttt_b200_scan_args p, const Plan q) {
+  wait_for_predecessor();
   constexpr bool kKeep = LN > 4;
   using S = Shape<LN>;
   constexpr int DC = S::DC, NP = S::NP, ND = 32 / LN;
@@ -812,6 +816,7 @@ __global__ void __launch_bounds__(TH, LN <= 4 ? 4 : 3) scan_backward_kernel(cons
 // the slot is requested in front of it, and the state in front of the search for rows that share it: two round trips to memory in all.
 // Rows that name the same slot are taken in their order by the CTA of the first of them, so that no two CTAs touch a state.
 template <class T, int LN> __global__ void __launch_bounds__(TH) scan_step_kernel(const ttt_b200_scan_args p, bool vec_n, int tiles) {
+  wait_for_predecessor();
   constexpr int DC = TH / LN;
   const int b0 = blockIdx.x / tiles, li = threadIdx.x % LN, n0 = 4 * li;
   int d[2];
@@ -1017,7 +1022,7 @@ template <class K> int launch(K kernel, size_t smem, long grid, cudaStream_t s, 
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return ttt_set_error(TTT_B200_ERR_LAUNCH, cudaGetErrorString(e));
   }
-  kernel<<<static_cast<unsigned>(grid), TH, smem, s>>>(p, q);
+  ttt_launch_overlapped(kernel, static_cast<int>(grid), TH, static_cast<uint32_t>(smem), s, p, q);
   return launched("ssm scan");
 }
 
@@ -1026,7 +1031,7 @@ template <class T, int LN> int forward(const ttt_b200_scan_args& p, const Plan& 
   if (q.chunks > 1) {
     if (int rc = launch(scan_state_kernel<T, LN, false>, sizeof(StateSmem<T, LN>), grid, s, p, q)) return rc;
     const long n = static_cast<long>(p.B) * p.D * p.N;
-    scan_join_kernel<false><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(p, q);
+    ttt_launch_overlapped(scan_join_kernel<false>, static_cast<int>((n + 255) / 256), 256, 0, s, p, q);
   }
   return launch(scan_forward_kernel<T, LN>, sizeof(FwdSmem<T, LN>), grid, s, p, q);
 }
@@ -1036,7 +1041,7 @@ template <class T, int LN> int backward(const ttt_b200_scan_args& p, const Plan&
   if (q.chunks > 1) {
     if (int rc = launch(scan_state_kernel<T, LN, true>, sizeof(StateSmem<T, LN>), grid, s, p, q)) return rc;
     const long n = static_cast<long>(p.B) * p.D * p.N;
-    scan_join_kernel<true><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(p, q);
+    ttt_launch_overlapped(scan_join_kernel<true>, static_cast<int>((n + 255) / 256), 256, 0, s, p, q);
   }
   if (int rc = launch(scan_backward_kernel<T, LN>, sizeof(BwdSmem<T, LN>), grid, s, p, q)) return rc;
   const long BTGN = static_cast<long>(p.B) * p.T * p.G * p.N, DN = static_cast<long>(p.D) * p.N, BCD = static_cast<long>(p.B) * q.chunks * p.D;
@@ -1055,7 +1060,7 @@ template <class T, int LN> int step(const ttt_b200_scan_args& p, cudaStream_t s)
   const bool vec = p.N % 4 == 0 && aligned16(p.A) && aligned16(p.state_io);
   const long grid = static_cast<long>(p.B) * tiles;
   if (grid > 0x7fffffffL) return fail("ssm scan: too many CTAs");
-  scan_step_kernel<T, LN><<<static_cast<unsigned>(grid), TH, 0, s>>>(p, vec, tiles);
+  ttt_launch_overlapped(scan_step_kernel<T, LN>, static_cast<int>(grid), TH, 0, s, p, vec, tiles);
   return launched("ssm scan step");
 }
 

@@ -70,6 +70,7 @@ template <int W> __device__ __forceinline__ void add_up(const ttt_sum_job& j, in
 }
 
 __global__ void __launch_bounds__(256) sum_parts_kernel(const Jobs jobs) {
+  wait_for_predecessor();
   __shared__ float4 rows[256];
   int k = 0;
   while (static_cast<int>(blockIdx.x) >= jobs.first[k + 1]) ++k;
@@ -101,7 +102,7 @@ int ttt_sum_parts(const ttt_sum_job* job, int count, cudaStream_t stream) {
     jobs.first[c + 1] = static_cast<int>(blocks);
   }
   if (!jobs.count) return TTT_B200_OK;
-  sum_parts_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(jobs);
+  ttt_launch_overlapped(sum_parts_kernel, static_cast<int>(blocks), 256, 0, stream, jobs);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? TTT_B200_OK : ttt_set_error(TTT_B200_ERR_LAUNCH, cudaGetErrorString(e));
 }
