@@ -103,6 +103,9 @@ __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp_async4_at(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
   cp_async16_at(static_cast<uint32_t>(__cvta_generic_to_shared(dst)), src, bytes);
 }
