@@ -235,6 +235,10 @@ BLOCK = [
     ("fp16", 12, 640, "layer", "gelu", False, True, True, False, True, True, False),
     ("fp32", 12, 640, "rms", "sigmoid", False, False, True, True, False, False, False),
     ("bf16", 12, 88, "rms", "silu", True, True, False, True, True, False, False),
+    ("bf16", 9, 1036, "layer", "gelu", True, True, True, True, True, True, False),       # runs of four, the last vector has one
+    ("fp32", 5, 516, "rms", "sigmoid", False, True, True, True, True, True, False),
+    ("fp16", 3, 4100, "layer", "silu", True, True, True, True, True, True, False),
+    ("fp16", 6, 300, "rms", "gelu", False, True, True, True, True, True, False),       # a 16-bit stream: one by one
 ]
 
 

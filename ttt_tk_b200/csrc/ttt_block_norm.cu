@@ -7,10 +7,14 @@
 //   d residual = d;  d scale = sum d v;  dv = d scale;  d gate = dv u act'(gate);  du = dv act(gate)
 //   do = r1 (g1 - mean(g1) - oh mean(g1 oh)),  g1 = du w1, oh = Norm(o);  dw, db: sums over the tokens
 //
-// Bound by memory.  A token belongs to the fewest threads (a warp or a power of two of them) that hold it with eight values each,
-// so that it is read once and its statistics are two passes over registers; tokens of up to 8192 values take sixteen.  The
-// backward computes z again from what the forward read (not from the z it wrote, whose rounding would be in the sums), keeps the
-// sums over tokens of its columns to itself over all its tokens and leaves them as one part per CTA for an ordered sum.
+// A token belongs to the fewest threads (a warp or a power of two of them) that hold it with eight values each (backward of more
+// than 4096: sixteen), so that it is read once and its statistics are two passes over registers.  The backward computes z again from
+// what the forward read (not from the z it wrote, whose rounding would be in the sums), keeps the sums over tokens of its columns to
+// itself over all its tokens and leaves them as one part per CTA for an ordered sum.
+//
+// Measured, fp32 residual stream, layer norms, all weights, tanh gate, 16384 x 2048 bf16: forward 117 us (4.0 TB/s), backward 229 us
+// (3.2 TB/s); bf16 residual, RMS norms 78 us (4.3) and 210 us (2.5).  Not memory but issued instructions and the wait at a token's
+// barriers hold them: 1024 threads to an SM forward (56 registers), 512 backward (128 registers, 20 of them sums over tokens).
 #include <algorithm>
 #include <cstdio>
 #include <type_traits>
@@ -29,18 +33,22 @@ struct Plan {
   float* part;    // backward: [ctas * side][5][D]
 };
 
-// A thread holds a token's values in vectors of eight, as four pairs.  Where all rows start on 16-byte boundaries (kVec) a vector is
-// eight neighbours, moved as such; otherwise its values are a token's width of threads apart, each moved by itself with the
-// warp's others next to it, and some of the last vector's may not be there.
+// A thread holds a token's values in vectors of eight, as four pairs: V neighbours, a token's width of threads from the next V.
+//   V = 8  where nothing but the weights is fp32
+//   V = 4  with an fp32 residual stream: a warp's 16-byte accesses to fp32 are then whole lines, where eight neighbours took the L1
+//          twice as many cycles.  16384 x 2048, forward and backward: 128 -> 118 and 262 -> 230 us; with a bf16 residual, whose
+//          rows then take twice as many accesses, 78 -> 95 and 209 -> 241 us, so there V stays 8.
+//   V = 1  where a row does not start on a boundary of V values
+// The last runs of a token may not be there.
 constexpr int N = 4;
 using F = float2;
 
 struct Cols {
   int lane, width, D;      // thread among the token's; those; values of a token
-  template <bool kVec> __device__ __forceinline__ int at(int j, int e) const {      // column of value e of vector j
-    return kVec ? (j * width + lane) * 8 + e : (j * 8 + e) * width + lane;
+  template <int V> __device__ __forceinline__ int at(int j, int e) const {      // column of value e of vector j
+    return ((j * (8 / V) + e / V) * width + lane) * V + e % V;
   }
-  template <bool kVec> __device__ __forceinline__ bool in(int j, int e = 0) const { return at<kVec>(j, e) < D; }
+  template <int V> __device__ __forceinline__ bool in(int j, int e = 0) const { return at<V>(j, e - e % V) < D; }
 };
 
 __device__ __forceinline__ float& half_of(F& f, int e) { return e ? f.y : f.x; }
@@ -50,51 +58,62 @@ __device__ __forceinline__ void fill(F (&f)[N], float v) {
   for (int k = 0; k < N; ++k) f[k] = both(v);
 }
 
-// eight neighbouring values as they lie in memory
-template <class T> struct Raw {
-  static constexpr int kPieces = static_cast<int>(sizeof(T)) / 2;      // of 16 bytes
-  alignas(16) T v[8];
-};
-template <class T> __device__ __forceinline__ void widen(const Raw<T>& r, F (&f)[N]) {
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) f[k] = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(r.v)[k]);
-    else if constexpr (std::is_same<T, __half>::value) f[k] = __half22float2(reinterpret_cast<const __half2*>(r.v)[k]);
-    else f[k] = make_float2(r.v[2 * k], r.v[2 * k + 1]);
+// V neighbouring values as they lie in memory, in pieces of up to 16 bytes
+template <class T, int V> struct Raw {
+  using Piece = typename std::conditional<V * sizeof(T) >= 16, uint4, uint2>::type;
+  static constexpr int kPieces = V * sizeof(T) / sizeof(Piece);
+  alignas(16) T v[V];
+  __device__ __forceinline__ Piece& piece(int i) { return reinterpret_cast<Piece*>(v)[i]; }
+  __device__ __forceinline__ F pair(int k) const {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) return __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(v)[k]);
+    else if constexpr (std::is_same<T, __half>::value) return __half22float2(reinterpret_cast<const __half2*>(v)[k]);
+    else return make_float2(v[2 * k], v[2 * k + 1]);
   }
-}
+  __device__ __forceinline__ void pair(int k, F f) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) reinterpret_cast<__nv_bfloat162*>(v)[k] = __float22bfloat162_rn(f);
+    else if constexpr (std::is_same<T, __half>::value) reinterpret_cast<__half2*>(v)[k] = __float22half2_rn(f);
+    else v[2 * k] = f.x, v[2 * k + 1] = f.y;
+  }
+};
 // vector j of a row; values that are not there become `none`
-template <bool kVec, class T> __device__ __forceinline__ void load(const T* row, const Cols& c, int j, F (&f)[N], float none = 0.f) {
-  if constexpr (kVec) {
-    Raw<T> r;
+template <int V, class T> __device__ __forceinline__ void load(const T* row, const Cols& c, int j, F (&f)[N], float none = 0.f) {
+  if constexpr (V > 1) {
 #pragma unroll
-    for (int i = 0; i < Raw<T>::kPieces; ++i) reinterpret_cast<uint4*>(r.v)[i] = reinterpret_cast<const uint4*>(row + c.at<true>(j, 0))[i];
-    widen(r, f);
+    for (int e = 0; e < 8; e += V) {
+      Raw<T, V> r;
+      const bool in = V == 8 || c.in<V>(j, e);      // (the first run of a vector is there)
+      if (in) {
+#pragma unroll
+        for (int i = 0; i < r.kPieces; ++i) r.piece(i) = reinterpret_cast<const typename Raw<T, V>::Piece*>(row + c.at<V>(j, e))[i];
+      }
+#pragma unroll
+      for (int k = 0; k < V / 2; ++k) f[e / 2 + k] = in ? r.pair(k) : both(none);
+    }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) half_of(f[e / 2], e % 2) = c.in<false>(j, e) ? to_f32(row[c.at<false>(j, e)]) : none;
+    for (int e = 0; e < 8; ++e) half_of(f[e / 2], e % 2) = c.in<V>(j, e) ? to_f32(row[c.at<V>(j, e)]) : none;
   }
 }
-template <bool kVec, class T> __device__ __forceinline__ void store(T* row, const Cols& c, int j, const F (&f)[N]) {
-  if constexpr (kVec) {
-    Raw<T> r;
+template <int V, class T> __device__ __forceinline__ void store(T* row, const Cols& c, int j, const F (&f)[N]) {
+  if constexpr (V > 1) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) reinterpret_cast<__nv_bfloat162*>(r.v)[k] = __float22bfloat162_rn(f[k]);
-      else if constexpr (std::is_same<T, __half>::value) reinterpret_cast<__half2*>(r.v)[k] = __float22half2_rn(f[k]);
-      else r.v[2 * k] = f[k].x, r.v[2 * k + 1] = f[k].y;
+    for (int e = 0; e < 8; e += V) {
+      if (V < 8 && !c.in<V>(j, e)) continue;
+      Raw<T, V> r;
+#pragma unroll
+      for (int k = 0; k < V / 2; ++k) r.pair(k, f[e / 2 + k]);
+#pragma unroll
+      for (int i = 0; i < r.kPieces; ++i) reinterpret_cast<typename Raw<T, V>::Piece*>(row + c.at<V>(j, e))[i] = r.piece(i);
     }
-#pragma unroll
-    for (int i = 0; i < Raw<T>::kPieces; ++i) reinterpret_cast<uint4*>(row + c.at<true>(j, 0))[i] = reinterpret_cast<const uint4*>(r.v)[i];
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (c.in<false>(j, e)) row[c.at<false>(j, e)] = from_f32<T>(half_of(f[e / 2], e % 2));
+      if (c.in<V>(j, e)) row[c.at<V>(j, e)] = from_f32<T>(half_of(f[e / 2], e % 2));
   }
 }
 // a weight's values, or `none` where there is no such weight
-template <bool kVec> __device__ __forceinline__ void weights(const float* p, const Cols& c, int j, float none, F (&f)[N]) {
-  if (p) load<kVec>(p, c, j, f, none);
+template <int V> __device__ __forceinline__ void weights(const float* p, const Cols& c, int j, float none, F (&f)[N]) {
+  if (p) load<V>(p, c, j, f, none);
   else fill(f, none);
 }
 
@@ -158,13 +177,15 @@ __device__ __forceinline__ float2 row_sum(float2 v, float2 (*smem)[32], int& buf
 }
 
 // A thread's values of a tensor's rows, token after token at a fixed distance; a tensor that is not there is all zeros.
-//   kOwn     vectors of eight: the next row is copied into the thread's own places in shared memory while it works on this one: no
+//   kOwn     vectors: the next row is copied into the thread's own places in shared memory while it works on this one: no
 //            barrier, no registers, and past the L1, which keeps the weights
-//   kWindow  single values: the next row's 16-byte blocks are copied by the token's threads together (the first and the last may hold
+//   kWindow  V = 1: the next row's 16-byte blocks are copied by the token's threads together (the first and the last may hold
 //            neighbours of the row as well), and each value is picked out at the row's offset; needs a barrier in front of `get`
 //   kDirect  from global memory
 enum { kDirect, kOwn, kWindow };
-template <class T, bool kVec, int kMode> struct Feed {
+template <class T, int V, int kMode> struct Feed {
+  static constexpr int kRun = V * static_cast<int>(sizeof(T));      // kOwn: 8 or 16 bytes
+  static_assert(kMode != kOwn || kRun == 8 || kRun == 16, "a run is one copy");
   const T* base;      // NULL: no such tensor
   int64_t stride;
   uint32_t slot;      // shared address of the first stage, the same for all threads
@@ -176,16 +197,19 @@ template <class T, bool kVec, int kMode> struct Feed {
   __device__ __forceinline__ Feed(const void* p, int64_t stride, uint32_t& smem, int side, int D) : base(static_cast<const T*>(p)), stride(stride), slot(smem) {
     if (base) smem += 2 * bytes(blockDim.x, side, D);
   }
-  __device__ __forceinline__ static uint32_t place(int sub, int D) { return kMode == kOwn ? threadIdx.x * 16 : sub * window(D); }
+  __device__ __forceinline__ static uint32_t place(int sub, int D) { return kMode == kOwn ? threadIdx.x * kRun : sub * window(D); }
   // row m into a stage
   __device__ __forceinline__ void ahead(long m, uint32_t to, const Cols& c, int sub) const {
     if (!base) return;
     to += slot + place(sub, c.D);
     if constexpr (kMode == kOwn) {      // (one vector to a thread)
-      if (!c.in<true>(0)) return;
-      const T* from = base + m * stride + c.at<true>(0, 0);
 #pragma unroll
-      for (int i = 0; i < Raw<T>::kPieces; ++i) cp_async16_at(to + i * 16 * blockDim.x, from + i * (16 / static_cast<int>(sizeof(T))));
+      for (int e = 0; e < 8; e += V) {
+        if (!c.in<V>(0, e)) continue;
+        const T* from = base + m * stride + c.at<V>(0, e);
+        if constexpr (kRun == 16) cp_async16_at(to + e / V * kRun * blockDim.x, from);
+        else cp_async8_at(to + e / V * kRun * blockDim.x, from);
+      }
     } else if constexpr (kMode == kWindow) {
       const uintptr_t at = reinterpret_cast<uintptr_t>(base + m * stride), begin = at & ~static_cast<uintptr_t>(15);
       const int span = c.D * static_cast<int>(sizeof(T)) + static_cast<int>(at - begin);
@@ -197,17 +221,21 @@ template <class T, bool kVec, int kMode> struct Feed {
     if (!base) {
       fill(f, 0.f);
     } else if constexpr (kMode == kOwn) {
-      Raw<T> r;
 #pragma unroll
-      for (int i = 0; i < Raw<T>::kPieces; ++i) reinterpret_cast<uint4*>(r.v)[i] = shared_load16(slot + from + place(sub, c.D) + i * 16 * blockDim.x);
-      widen(r, f);
+      for (int e = 0; e < 8; e += V) {
+        Raw<T, V> r;
+        const uint32_t at = slot + from + place(sub, c.D) + e / V * kRun * blockDim.x;
+        if constexpr (kRun == 16) r.piece(0) = shared_load16(at);
+        else r.piece(0) = shared_load8(at);
+#pragma unroll
+        for (int k = 0; k < V / 2; ++k) f[e / 2 + k] = V == 8 || c.in<V>(0, e) ? r.pair(k) : both(0.f);
+      }
     } else if constexpr (kMode == kWindow) {
       const uint32_t at = slot + from + place(sub, c.D) + (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base + m * stride)) & 15);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        half_of(f[e / 2], e % 2) = c.in<false>(j, e) ? shared_load<T>(at + c.at<false>(j, e) * static_cast<int>(sizeof(T))) : 0.f;
+      for (int e = 0; e < 8; ++e) half_of(f[e / 2], e % 2) = c.in<V>(j, e) ? shared_load<T>(at + c.at<V>(j, e) * static_cast<int>(sizeof(T))) : 0.f;
     } else {
-      load<kVec>(base + m * stride, c, j, f);
+      load<V>(base + m * stride, c, j, f);
     }
   }
 };
@@ -219,13 +247,13 @@ struct Shared {
   float columns[32];
   float4 stats[2][32];      // backward: each warp's token's
 };
-template <bool kVec, int NV> __device__ __forceinline__ void count_columns(Shared& sh, const Cols& c) {
+template <int V, int NV> __device__ __forceinline__ void count_columns(Shared& sh, const Cols& c) {
   if (threadIdx.x < 32) {
     const int first = 32 * static_cast<int>(threadIdx.x);
-    int n = 0;      // of warp threadIdx.x of a token: NV runs of 256, or 8 NV of 32
+    int n = 0;      // of warp threadIdx.x of a token: runs of 32 threads' values
     if (first < c.width) {
 #pragma unroll
-      for (int j = 0; j < (kVec ? NV : 8 * NV); ++j) n += min(max(c.D - (j * c.width + first) * (kVec ? 8 : 1), 0), kVec ? 256 : 32);
+      for (int j = 0; j < 8 / V * NV; ++j) n += min(max(c.D - (j * c.width + first) * V, 0), 32 * V);
     }
     sh.columns[threadIdx.x] = static_cast<float>(n);
   }
@@ -234,7 +262,7 @@ template <bool kVec, int NV> __device__ __forceinline__ void count_columns(Share
 
 // Mean and 1 / deviation of a row with one barrier: each warp's mean and its squares about it, joined as
 // sum over warps of (squares + columns (mean of the warp - mean)^2).
-template <bool kVec, int NV>
+template <int V, int NV>
 __device__ __forceinline__ float2 statistics(const F (&a)[NV][N], const ttt_b200_block_args& p, const Cols& c, Shared& sh, int& buf) {
   const int width = c.width;
   const float inv = 1.f / static_cast<float>(p.D);
@@ -253,11 +281,11 @@ __device__ __forceinline__ float2 statistics(const F (&a)[NV][N], const ttt_b200
   F sq = both(0.f);
 #pragma unroll
   for (int j = 0; j < NV; ++j)
-    if (c.in<kVec>(j)) {
+    if (c.in<V>(j)) {
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         F v = add2(a[j][k], both(-mean));
-        if (!kVec) v = make_float2(c.in<kVec>(j, 2 * k) ? v.x : 0.f, c.in<kVec>(j, 2 * k + 1) ? v.y : 0.f);
+        if (2 * k + 1 >= V) v = make_float2(c.in<V>(j, 2 * k) ? v.x : 0.f, c.in<V>(j, 2 * k + 1) ? v.y : 0.f);      // (the first run is there)
         sq = fma2(v, v, sq);
       }
     }
@@ -285,10 +313,10 @@ __device__ __forceinline__ float2 statistics(const F (&a)[NV][N], const ttt_b200
   return make_float2(mean, rsqrtf(fmaf(q, inv, p.eps)));
 }
 
-template <class T, class R, bool kVec, int kThreads>
+template <class T, class R, int V, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kernel(const ttt_b200_block_args p, const Plan q) {
   wait_for_predecessor();
-  constexpr int kMode = kVec ? kOwn : kWindow, NV = 1;
+  constexpr int kMode = V > 1 ? kOwn : kWindow, NV = 1;
   __shared__ Shared sh;
   extern __shared__ __align__(16) unsigned char stages[];
   uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(stages));
@@ -296,9 +324,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kerne
   const int lane = threadIdx.x % q.width, sub = threadIdx.x / q.width;
   const Cols c = {lane, q.width, p.D};
   const long step = static_cast<long>(q.ctas) * q.side;
-  const Feed<T, kVec, kMode> fo(p.o, p.o_stride, at, q.side, p.D), fg(p.gate, p.gate_stride, at, q.side, p.D);
-  const Feed<R, kVec, kMode> fx(p.residual, p.residual_stride, at, q.side, p.D);
-  const uint32_t small = Feed<T, kVec, kMode>::bytes(blockDim.x, q.side, p.D), large = Feed<R, kVec, kMode>::bytes(blockDim.x, q.side, p.D);
+  const Feed<T, V, kMode> fo(p.o, p.o_stride, at, q.side, p.D), fg(p.gate, p.gate_stride, at, q.side, p.D);
+  const Feed<R, V, kMode> fx(p.residual, p.residual_stride, at, q.side, p.D);
+  const uint32_t small = Feed<T, V, kMode>::bytes(blockDim.x, q.side, p.D), large = Feed<R, V, kMode>::bytes(blockDim.x, q.side, p.D);
   auto ahead = [&](long m, int stage) {
     if (m < p.M) {
       fo.ahead(m, stage * small, c, sub);
@@ -309,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kerne
   };
   long m = static_cast<long>(blockIdx.x) * q.side + sub;
   ahead(m, 0);
-  count_columns<kVec, NV>(sh, c);
+  count_columns<V, NV>(sh, c);
   int stage = 0;
   for (long base = static_cast<long>(blockIdx.x) * q.side; base < p.M; base += step, stage ^= 1, m += step) {
     const bool live = m < p.M;
@@ -321,17 +349,17 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kerne
     for (int j = 0; j < NV; ++j) {
 #pragma unroll
       for (int k = 0; k < N; ++k) a[j][k] = z[j][k] = both(0.f);
-      if (live && c.in<kVec>(j)) fo.get(m, stage * small, c, j, sub, a[j]);
+      if (live && c.in<V>(j)) fo.get(m, stage * small, c, j, sub, a[j]);
     }
     float2 s1 = make_float2(0.f, 1.f), s2 = s1;
-    if (p.post_weight) s1 = statistics<kVec, NV>(a, p, c, sh, buf);
+    if (p.post_weight) s1 = statistics<V, NV>(a, p, c, sh, buf);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (!(live && c.in<kVec>(j))) continue;
+      if (!(live && c.in<V>(j))) continue;
       F w[N], b[N];
       if (p.post_weight) {
-        weights<kVec>(p.post_weight, c, j, 0.f, w);
-        weights<kVec>(p.post_bias, c, j, 0.f, b);
+        weights<V>(p.post_weight, c, j, 0.f, w);
+        weights<V>(p.post_bias, c, j, 0.f, b);
 #pragma unroll
         for (int k = 0; k < N; ++k) a[j][k] = mac(times(plus(a[j][k], both(-s1.x)), both(s1.y)), w[k], b[k]);
       }
@@ -343,22 +371,22 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kerne
         for (int k = 0; k < N; ++k) a[j][k] = times(a[j][k], g[k]);
       }
       fx.get(m, stage * large, c, j, sub, z[j]);
-      weights<kVec>(p.scale, c, j, 1.f, w);
+      weights<V>(p.scale, c, j, 1.f, w);
 #pragma unroll
       for (int k = 0; k < N; ++k) z[j][k] = mac(w[k], a[j][k], z[j][k]);
-      store<kVec>(static_cast<R*>(p.x) + m * p.D, c, j, z[j]);
+      store<V>(static_cast<R*>(p.x) + m * p.D, c, j, z[j]);
     }
     if (p.pre_weight) {
-      s2 = statistics<kVec, NV>(z, p, c, sh, buf);
+      s2 = statistics<V, NV>(z, p, c, sh, buf);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (live && c.in<kVec>(j)) {
+        if (live && c.in<V>(j)) {
           F w[N], b[N];
-          weights<kVec>(p.pre_weight, c, j, 0.f, w);
-          weights<kVec>(p.pre_bias, c, j, 0.f, b);
+          weights<V>(p.pre_weight, c, j, 0.f, w);
+          weights<V>(p.pre_bias, c, j, 0.f, b);
 #pragma unroll
           for (int k = 0; k < N; ++k) z[j][k] = mac(times(plus(z[j][k], both(-s2.x)), both(s2.y)), w[k], b[k]);
-          store<kVec>(static_cast<T*>(p.n) + m * p.D, c, j, z[j]);
+          store<V>(static_cast<T*>(p.n) + m * p.D, c, j, z[j]);
         }
       }
     }
@@ -368,32 +396,32 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kerne
 
 // Sums over tokens of a thread's columns: in registers, or, of sixteen columns, in shared memory.
 enum { kDw1, kDb1, kDsc, kDw2, kDb2, kSums };
-template <bool kVec, int NV, bool kShared> struct Sums {
+template <int V, int NV, bool kShared> struct Sums {
   F r[kShared ? 1 : kSums][NV][N];
   float* s;
   __device__ __forceinline__ F get(int k, int j, int i, const Cols& c) const {
     if constexpr (!kShared) return r[k][j][i];
-    else if constexpr (kVec) return *reinterpret_cast<const F*>(s + k * c.D + c.at<true>(j, 2 * i));
-    else return make_float2(c.in<false>(j, 2 * i) ? s[k * c.D + c.at<false>(j, 2 * i)] : 0.f, c.in<false>(j, 2 * i + 1) ? s[k * c.D + c.at<false>(j, 2 * i + 1)] : 0.f);
+    else if constexpr (V > 1) return c.in<V>(j, 2 * i) ? *reinterpret_cast<const F*>(s + k * c.D + c.at<V>(j, 2 * i)) : both(0.f);
+    else return make_float2(c.in<V>(j, 2 * i) ? s[k * c.D + c.at<V>(j, 2 * i)] : 0.f, c.in<V>(j, 2 * i + 1) ? s[k * c.D + c.at<V>(j, 2 * i + 1)] : 0.f);
   }
   __device__ __forceinline__ void set(int k, int j, int i, const Cols& c, F v) {
     if constexpr (!kShared) {
       r[k][j][i] = v;
-    } else if constexpr (kVec) {
-      *reinterpret_cast<F*>(s + k * c.D + c.at<true>(j, 2 * i)) = v;
+    } else if constexpr (V > 1) {
+      if (c.in<V>(j, 2 * i)) *reinterpret_cast<F*>(s + k * c.D + c.at<V>(j, 2 * i)) = v;
     } else {
-      if (c.in<false>(j, 2 * i)) s[k * c.D + c.at<false>(j, 2 * i)] = v.x;
-      if (c.in<false>(j, 2 * i + 1)) s[k * c.D + c.at<false>(j, 2 * i + 1)] = v.y;
+      if (c.in<V>(j, 2 * i)) s[k * c.D + c.at<V>(j, 2 * i)] = v.x;
+      if (c.in<V>(j, 2 * i + 1)) s[k * c.D + c.at<V>(j, 2 * i + 1)] = v.y;
     }
   }
   __device__ __forceinline__ void add(int k, int j, int i, const Cols& c, F v) { set(k, j, i, c, add2(get(k, j, i, c), v)); }
   __device__ __forceinline__ void add(int k, int j, int i, const Cols& c, F a, F b) { set(k, j, i, c, fma2(a, b, get(k, j, i, c))); }
 };
 
-template <class T, class R, bool kVec, int NV, bool kShared, int kThreads>
+template <class T, class R, int V, int NV, bool kShared, int kThreads>
 __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1) block_backward_kernel(const ttt_b200_block_args p, const Plan q) {
   wait_for_predecessor();
-  constexpr int kMode = kShared ? kDirect : kVec ? kOwn : kWindow;
+  constexpr int kMode = kShared ? kDirect : V > 1 ? kOwn : kWindow;
   __shared__ Shared sh;
   extern __shared__ __align__(16) unsigned char stages[];
   uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(stages));
@@ -401,11 +429,11 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
   const int lane = threadIdx.x % q.width, sub = threadIdx.x / q.width;
   const Cols c = {lane, q.width, p.D};
   const long step = static_cast<long>(q.ctas) * q.side;
-  const Feed<T, kVec, kMode> fo(p.o, p.o_stride, at, q.side, p.D), fg(p.gate, p.gate_stride, at, q.side, p.D);
-  const Feed<T, kVec, kMode> fn(p.pre_weight ? p.grad_n : nullptr, p.gn_stride, at, q.side, p.D);
-  const Feed<R, kVec, kMode> fx(p.pre_weight ? p.residual : nullptr, p.residual_stride, at, q.side, p.D);
-  const Feed<R, kVec, kMode> fd(p.grad_x, p.gx_stride, at, q.side, p.D);
-  const uint32_t small = Feed<T, kVec, kMode>::bytes(blockDim.x, q.side, p.D), large = Feed<R, kVec, kMode>::bytes(blockDim.x, q.side, p.D);
+  const Feed<T, V, kMode> fo(p.o, p.o_stride, at, q.side, p.D), fg(p.gate, p.gate_stride, at, q.side, p.D);
+  const Feed<T, V, kMode> fn(p.pre_weight ? p.grad_n : nullptr, p.gn_stride, at, q.side, p.D);
+  const Feed<R, V, kMode> fx(p.pre_weight ? p.residual : nullptr, p.residual_stride, at, q.side, p.D);
+  const Feed<R, V, kMode> fd(p.grad_x, p.gx_stride, at, q.side, p.D);
+  const uint32_t small = Feed<T, V, kMode>::bytes(blockDim.x, q.side, p.D), large = Feed<R, V, kMode>::bytes(blockDim.x, q.side, p.D);
   const uint32_t stats = static_cast<uint32_t>(__cvta_generic_to_shared(&sh.stats[0][threadIdx.x >> 5]));
   auto ahead = [&](long m, int stage) {
     if (m < p.M) {
@@ -419,11 +447,11 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
     cp_async_commit();
   };
   const float inv = 1.f / static_cast<float>(p.D);
-  Sums<kVec, NV, kShared> sums;
+  Sums<V, NV, kShared> sums;
   sums.s = reinterpret_cast<float*>(stages);
 #pragma unroll
   for (int j = 0; j < NV; ++j)
-    if (!kShared || c.in<kVec>(j)) {
+    if (!kShared || c.in<V>(j)) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -445,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
     F sx = both(0.f), sy = sx;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const bool in = live && c.in<kVec>(j);
+      const bool in = live && c.in<V>(j);
 #pragma unroll
       for (int i = 0; i < N; ++i) o[j][i] = both(0.f);
       if (in) fo.get(m, stage * small, c, j, sub, o[j]);
@@ -458,8 +486,8 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
 #pragma unroll
       for (int i = 0; i < N; ++i) u[i] = o[j][i];
       if (p.post_weight) {
-        weights<kVec>(p.post_weight, c, j, 0.f, w);
-        weights<kVec>(p.post_bias, c, j, 0.f, b);
+        weights<V>(p.post_weight, c, j, 0.f, w);
+        weights<V>(p.post_bias, c, j, 0.f, b);
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = mac(o[j][i], w[i], b[i]);
       }
@@ -469,12 +497,12 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = times(u[i], w[i]);
       }
-      weights<kVec>(p.scale, c, j, 1.f, w);
+      weights<V>(p.scale, c, j, 1.f, w);
       fx.get(m, stage * large, c, j, sub, z[j]);
 #pragma unroll
       for (int i = 0; i < N; ++i) z[j][i] = times(plus(mac(w[i], u[i], z[j][i]), both(-st.z)), both(st.w));
       fn.get(m, stage * small, c, j, sub, gn[j]);
-      weights<kVec>(p.pre_weight, c, j, 0.f, w);
+      weights<V>(p.pre_weight, c, j, 0.f, w);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         sums.add(kDw2, j, i, c, gn[j][i], z[j][i]);
@@ -494,23 +522,23 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
     sx = sy = both(0.f);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (!(live && c.in<kVec>(j))) continue;
+      if (!(live && c.in<V>(j))) continue;
       fd.get(m, stage * large, c, j, sub, d2[j]);
       if (p.pre_weight) {
 #pragma unroll
         for (int i = 0; i < N; ++i) d2[j][i] = mac(both(st.w), mac(z[j][i], both(-m2), plus(gn[j][i], both(-m1))), d2[j][i]);
       }
-      if (p.grad_residual) store<kVec>(static_cast<R*>(p.grad_residual) + m * p.D, c, j, d2[j]);
+      if (p.grad_residual) store<V>(static_cast<R*>(p.grad_residual) + m * p.D, c, j, d2[j]);
       F u[N], w[N], b[N], v[N], g[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) u[i] = o[j][i];
       if (p.post_weight) {
-        weights<kVec>(p.post_weight, c, j, 0.f, w);
-        weights<kVec>(p.post_bias, c, j, 0.f, b);
+        weights<V>(p.post_weight, c, j, 0.f, w);
+        weights<V>(p.post_bias, c, j, 0.f, b);
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = mac(o[j][i], w[i], b[i]);
       }
-      weights<kVec>(p.scale, c, j, 1.f, b);
+      weights<V>(p.scale, c, j, 1.f, b);
       if (p.gate) {
         fg.get(m, stage * small, c, j, sub, g);
         gate<true>(p.activation, g, v, g);
@@ -521,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
           g[i] = times(times(d2[j][i], u[i]), g[i]);
           d2[j][i] = times(d2[j][i], v[i]);
         }
-        store<kVec>(static_cast<T*>(p.grad_gate) + m * p.D, c, j, g);
+        store<V>(static_cast<T*>(p.grad_gate) + m * p.D, c, j, g);
       } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -547,24 +575,24 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (!(live && c.in<kVec>(j))) continue;
+      if (!(live && c.in<V>(j))) continue;
       if (p.post_weight) {
 #pragma unroll
         for (int i = 0; i < N; ++i) d2[j][i] = times(both(st.y), mac(o[j][i], both(-m2), plus(d2[j][i], both(-m1))));
       }
-      store<kVec>(static_cast<T*>(p.grad_o) + m * p.D, c, j, d2[j]);
+      store<V>(static_cast<T*>(p.grad_o) + m * p.D, c, j, d2[j]);
     }
   }
   float* part = q.part + (static_cast<long>(blockIdx.x) * q.side + sub) * kSums * p.D;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    if (!c.in<kVec>(j)) continue;
+    if (!c.in<V>(j)) continue;
 #pragma unroll
     for (int k = 0; k < kSums; ++k) {
       F v[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] = sums.get(k, j, i, c);
-      store<kVec>(part + static_cast<long>(k) * p.D, c, j, v);
+      store<V>(part + static_cast<long>(k) * p.D, c, j, v);
     }
   }
 }
@@ -606,16 +634,18 @@ void plan(Plan& q, const ttt_b200_block_args& p, bool backward) {
   q.ctas = static_cast<int>(std::min<long>(most, (p.M + q.side - 1) / q.side));
 }
 
-bool rows16(const void* p, int64_t stride, size_t es) { return aligned16(p) && stride * static_cast<int64_t>(es) % 16 == 0; }
+template <class R> constexpr int kRun = sizeof(R) == 4 ? 4 : 8;      // V of rows that start on its boundaries
 
-bool vectors(const ttt_b200_block_args& p, bool backward) {
+// whether every row of every tensor starts on a boundary of `run` values
+bool vectors(const ttt_b200_block_args& p, bool backward, int run) {
   const size_t es = p.dtype == TTT_B200_FP32 ? 4 : 2, rs = p.residual_fp32 ? 4 : es;
-  bool ok = p.D % 8 == 0 && rows16(p.o, p.o_stride, es) && rows16(p.residual, p.residual_stride, rs) && rows16(p.gate, p.gate_stride, es);
+  auto rows = [run](const void* a, int64_t stride, size_t bytes) { return reinterpret_cast<uintptr_t>(a) % (run * bytes) == 0 && stride % run == 0; };
+  bool ok = p.D % run == 0 && rows(p.o, p.o_stride, es) && rows(p.residual, p.residual_stride, rs) && rows(p.gate, p.gate_stride, es);
   for (const float* w : {p.post_weight, p.post_bias, p.scale, p.pre_weight, p.pre_bias}) ok = ok && aligned16(w);
   if (backward)
-    return ok && rows16(p.grad_x, p.gx_stride, rs) && rows16(p.grad_n, p.gn_stride, es) && aligned16(p.grad_o) && aligned16(p.grad_residual) &&
-           aligned16(p.grad_gate);
-  return ok && aligned16(p.x) && aligned16(p.n);
+    return ok && rows(p.grad_x, p.gx_stride, rs) && rows(p.grad_n, p.gn_stride, es) && rows(p.grad_o, 0, es) && rows(p.grad_residual, 0, rs) &&
+           rows(p.grad_gate, 0, es);
+  return ok && rows(p.x, 0, rs) && rows(p.n, 0, es);
 }
 
 int launched(const char* what) {
@@ -635,44 +665,44 @@ template <class K> int launch(K kernel, const Plan& q, size_t bytes, cudaStream_
   return launched(what);
 }
 
-template <class T, class R, bool kVec, int kThreads> int forward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
-  constexpr int kMode = kVec ? kOwn : kWindow;
+template <class T, class R, int V, int kThreads> int forward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
+  constexpr int kMode = V > 1 ? kOwn : kWindow;
   const int n = q.width * q.side;
-  const size_t bytes = 2 * (Feed<T, kVec, kMode>::bytes(n, q.side, p.D) * (1 + (p.gate != nullptr)) +
-                            Feed<R, kVec, kMode>::bytes(n, q.side, p.D) * (p.residual != nullptr));
-  return launch(block_forward_kernel<T, R, kVec, kThreads>, q, bytes, s, p, "block norm");
+  const size_t bytes = 2 * (Feed<T, V, kMode>::bytes(n, q.side, p.D) * (1 + (p.gate != nullptr)) +
+                            Feed<R, V, kMode>::bytes(n, q.side, p.D) * (p.residual != nullptr));
+  return launch(block_forward_kernel<T, R, V, kThreads>, q, bytes, s, p, "block norm");
 }
 
 template <class T, class R> int forward(const ttt_b200_block_args& p, cudaStream_t s) {
   Plan q = {};
   plan(q, p, false);
   const int n = q.width * q.side;
-  const bool vec = vectors(p, false);
-  if (n <= 128) return vec ? forward_as<T, R, true, 128>(p, q, s) : forward_as<T, R, false, 128>(p, q, s);
-  if (n <= 256) return vec ? forward_as<T, R, true, 256>(p, q, s) : forward_as<T, R, false, 256>(p, q, s);
-  return vec ? forward_as<T, R, true, 1024>(p, q, s) : forward_as<T, R, false, 1024>(p, q, s);
+  const bool vec = vectors(p, false, kRun<R>);
+  if (n <= 128) return vec ? forward_as<T, R, kRun<R>, 128>(p, q, s) : forward_as<T, R, 1, 128>(p, q, s);
+  if (n <= 256) return vec ? forward_as<T, R, kRun<R>, 256>(p, q, s) : forward_as<T, R, 1, 256>(p, q, s);
+  return vec ? forward_as<T, R, kRun<R>, 1024>(p, q, s) : forward_as<T, R, 1, 1024>(p, q, s);
 }
 
-template <class T, class R, bool kVec, int NV, bool kShared, int kThreads> int backward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
-  constexpr int kMode = kShared ? kDirect : kVec ? kOwn : kWindow;
+template <class T, class R, int V, int NV, bool kShared, int kThreads> int backward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
+  constexpr int kMode = kShared ? kDirect : V > 1 ? kOwn : kWindow;
   const int n = q.width * q.side;
   const size_t bytes = kShared ? static_cast<size_t>(kSums) * p.D * sizeof(float)
-                               : 2 * (Feed<T, kVec, kMode>::bytes(n, q.side, p.D) * (1 + (p.gate != nullptr) + (p.pre_weight && p.grad_n)) +
-                                          Feed<R, kVec, kMode>::bytes(n, q.side, p.D) * ((p.pre_weight && p.residual) + (p.grad_x != nullptr)));
-  return launch(block_backward_kernel<T, R, kVec, NV, kShared, kThreads>, q, bytes, s, p, "block norm backward");
+                               : 2 * (Feed<T, V, kMode>::bytes(n, q.side, p.D) * (1 + (p.gate != nullptr) + (p.pre_weight && p.grad_n)) +
+                                          Feed<R, V, kMode>::bytes(n, q.side, p.D) * ((p.pre_weight && p.residual) + (p.grad_x != nullptr)));
+  return launch(block_backward_kernel<T, R, V, NV, kShared, kThreads>, q, bytes, s, p, "block norm backward");
 }
 
 template <class T, class R> int backward(const ttt_b200_block_args& p, cudaStream_t s) {
   Plan q = {};
   plan(q, p, true);
   q.part = static_cast<float*>(p.scratch);
-  const bool vec = vectors(p, true);
+  const bool vec = vectors(p, true, kRun<R>);
   const int n = q.width * q.side;
   int rc;
-  if (p.D > kWide) rc = vec ? backward_as<T, R, true, 2, true, 512>(p, q, s) : backward_as<T, R, false, 2, true, 512>(p, q, s);
-  else if (n <= 128) rc = vec ? backward_as<T, R, true, 1, false, 128>(p, q, s) : backward_as<T, R, false, 1, false, 128>(p, q, s);
-  else if (n <= 256) rc = vec ? backward_as<T, R, true, 1, false, 256>(p, q, s) : backward_as<T, R, false, 1, false, 256>(p, q, s);
-  else rc = vec ? backward_as<T, R, true, 1, false, 512>(p, q, s) : backward_as<T, R, false, 1, false, 512>(p, q, s);
+  if (p.D > kWide) rc = vec ? backward_as<T, R, kRun<R>, 2, true, 512>(p, q, s) : backward_as<T, R, 1, 2, true, 512>(p, q, s);
+  else if (n <= 128) rc = vec ? backward_as<T, R, kRun<R>, 1, false, 128>(p, q, s) : backward_as<T, R, 1, 1, false, 128>(p, q, s);
+  else if (n <= 256) rc = vec ? backward_as<T, R, kRun<R>, 1, false, 256>(p, q, s) : backward_as<T, R, 1, 1, false, 256>(p, q, s);
+  else rc = vec ? backward_as<T, R, kRun<R>, 1, false, 512>(p, q, s) : backward_as<T, R, 1, 1, false, 512>(p, q, s);
   if (rc) return rc;
   const long row = static_cast<long>(kSums) * p.D;
   float* dst[kSums] = {p.grad_post_weight, p.grad_post_bias, p.grad_scale, p.grad_pre_weight, p.grad_pre_bias};

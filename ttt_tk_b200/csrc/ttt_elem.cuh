@@ -103,6 +103,9 @@ __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp_async8_at(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async4_at(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -113,6 +116,11 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes
 __device__ __forceinline__ uint4 shared_load16(uint32_t at) {
   uint4 r;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
+  return r;
+}
+__device__ __forceinline__ uint2 shared_load8(uint32_t at) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at) : "memory");
   return r;
 }
 template <class T> __device__ __forceinline__ float shared_load(uint32_t at) {
