@@ -12,9 +12,10 @@
 // what the forward read (not from the z it wrote, whose rounding would be in the sums), keeps the sums over tokens of its columns to
 // itself over all its tokens and leaves them as one part per CTA for an ordered sum.
 //
-// Measured, fp32 residual stream, layer norms, all weights, tanh gate, 16384 x 2048 bf16: forward 117 us (4.0 TB/s), backward 229 us
-// (3.2 TB/s); bf16 residual, RMS norms 78 us (4.3) and 210 us (2.5).  Not memory but issued instructions and the wait at a token's
-// barriers hold them: 1024 threads to an SM forward (56 registers), 512 backward (128 registers, 20 of them sums over tokens).
+// Measured, fp32 residual stream, layer norms, all weights, tanh gate, 16384 x 2048 bf16: forward 104 us (4.5 TB/s), backward 211 us
+// (3.5 TB/s); bf16 residual, RMS norms 79 us (4.2) and 187 us (2.9); rows of 2047 118 and 257 us.  Not memory but issued instructions
+// and the wait at a token's barriers hold them: 1024 threads to an SM forward, 512 backward (128 registers, 40 of them sums over
+// tokens).  So the width is a constant of the kernel (118 -> 104 and 230 -> 211 us; rows of 2047 174 -> 118 and 349 -> 257).
 #include <algorithm>
 #include <cstdio>
 #include <type_traits>
@@ -28,10 +29,10 @@ using namespace ttt;
 
 struct Plan {
   int width;      // threads of a token
-  int side;       // tokens next to each other in a CTA
   int ctas;
-  float* part;    // backward: [ctas * side][5][D]
+  float* part;    // backward: [ctas * tokens next to each other][5][D]
 };
+constexpr int side_of(int width) { return width < 128 ? 128 / width : 1; }      // tokens next to each other in a CTA
 
 // A thread holds a token's values in vectors of eight, as four pairs: V neighbours, a token's width of threads from the next V.
 //   V = 8  where nothing but the weights is fp32
@@ -43,12 +44,11 @@ struct Plan {
 constexpr int N = 4;
 using F = float2;
 
-struct Cols {
-  int lane, width, D;      // thread among the token's; those; values of a token
-  template <int V> __device__ __forceinline__ int at(int j, int e) const {      // column of value e of vector j
-    return ((j * (8 / V) + e / V) * width + lane) * V + e % V;
-  }
-  template <int V> __device__ __forceinline__ bool in(int j, int e = 0) const { return at<V>(j, e - e % V) < D; }
+template <int kRun, int kWidth> struct Cols {
+  static constexpr int V = kRun, width = kWidth, side = side_of(kWidth), threads = width * side;
+  int lane, D;      // thread among the token's; values of a token
+  __device__ __forceinline__ int at(int j, int e) const { return ((j * (8 / V) + e / V) * width + lane) * V + e % V; }      // column of value e of vector j
+  __device__ __forceinline__ bool in(int j, int e = 0) const { return at(j, e - e % V) < D; }
 };
 
 __device__ __forceinline__ float& half_of(F& f, int e) { return e ? f.y : f.x; }
@@ -76,44 +76,46 @@ template <class T, int V> struct Raw {
   }
 };
 // vector j of a row; values that are not there become `none`
-template <int V, class T> __device__ __forceinline__ void load(const T* row, const Cols& c, int j, F (&f)[N], float none = 0.f) {
+template <class C, class T> __device__ __forceinline__ void load(const T* row, const C& c, int j, F (&f)[N], float none = 0.f) {
+  constexpr int V = C::V;
   if constexpr (V > 1) {
 #pragma unroll
     for (int e = 0; e < 8; e += V) {
       Raw<T, V> r;
-      const bool in = V == 8 || c.in<V>(j, e);      // (the first run of a vector is there)
+      const bool in = V == 8 || c.in(j, e);      // (the first run of a vector is there)
       if (in) {
 #pragma unroll
-        for (int i = 0; i < r.kPieces; ++i) r.piece(i) = reinterpret_cast<const typename Raw<T, V>::Piece*>(row + c.at<V>(j, e))[i];
+        for (int i = 0; i < r.kPieces; ++i) r.piece(i) = reinterpret_cast<const typename Raw<T, V>::Piece*>(row + c.at(j, e))[i];
       }
 #pragma unroll
       for (int k = 0; k < V / 2; ++k) f[e / 2 + k] = in ? r.pair(k) : both(none);
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) half_of(f[e / 2], e % 2) = c.in<V>(j, e) ? to_f32(row[c.at<V>(j, e)]) : none;
+    for (int e = 0; e < 8; ++e) half_of(f[e / 2], e % 2) = c.in(j, e) ? to_f32(row[c.at(j, e)]) : none;
   }
 }
-template <int V, class T> __device__ __forceinline__ void store(T* row, const Cols& c, int j, const F (&f)[N]) {
+template <class C, class T> __device__ __forceinline__ void store(T* row, const C& c, int j, const F (&f)[N]) {
+  constexpr int V = C::V;
   if constexpr (V > 1) {
 #pragma unroll
     for (int e = 0; e < 8; e += V) {
-      if (V < 8 && !c.in<V>(j, e)) continue;
+      if (V < 8 && !c.in(j, e)) continue;
       Raw<T, V> r;
 #pragma unroll
       for (int k = 0; k < V / 2; ++k) r.pair(k, f[e / 2 + k]);
 #pragma unroll
-      for (int i = 0; i < r.kPieces; ++i) reinterpret_cast<typename Raw<T, V>::Piece*>(row + c.at<V>(j, e))[i] = r.piece(i);
+      for (int i = 0; i < r.kPieces; ++i) reinterpret_cast<typename Raw<T, V>::Piece*>(row + c.at(j, e))[i] = r.piece(i);
     }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (c.in<V>(j, e)) row[c.at<V>(j, e)] = from_f32<T>(half_of(f[e / 2], e % 2));
+      if (c.in(j, e)) row[c.at(j, e)] = from_f32<T>(half_of(f[e / 2], e % 2));
   }
 }
 // a weight's values, or `none` where there is no such weight
-template <int V> __device__ __forceinline__ void weights(const float* p, const Cols& c, int j, float none, F (&f)[N]) {
-  if (p) load<V>(p, c, j, f, none);
+template <class C> __device__ __forceinline__ void weights(const float* p, const C& c, int j, float none, F (&f)[N]) {
+  if (p) load(p, c, j, f, none);
   else fill(f, none);
 }
 
@@ -156,20 +158,21 @@ template <bool kSlope> __device__ __forceinline__ void gate(int kind, const F (&
 
 // The sums of two values over the threads of a token, in all of them.  `buf` alternates between calls: a barrier lies between two
 // uses of the same half.  The lower half of a warp takes the first value, the upper the second, here and across the warps.
-__device__ __forceinline__ float2 row_sum(float2 v, float2 (*smem)[32], int& buf, int width) {
+template <class C> __device__ __forceinline__ float2 row_sum(float2 v, float2 (*smem)[32], int& buf) {
   const bool up = threadIdx.x & 16;
   float s = (up ? v.y : v.x) + __shfl_xor_sync(0xffffffffu, up ? v.x : v.y, 16);
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (width > 32) {
-    const int warp = threadIdx.x >> 5, warps = width >> 5, first = warp & -warps, i = threadIdx.x & 15;
+  if constexpr (C::width > 32) {
+    constexpr int warps = C::width / 32;
+    static_assert(warps <= 16, "half a warp has a lane for each warp");
+    const int warp = threadIdx.x >> 5, first = warp & -warps, i = threadIdx.x & 15;
     float* part = reinterpret_cast<float*>(smem[buf]);
     if (i == 0) part[2 * warp + up] = s;
     __syncthreads();
-    s = i < warps ? part[2 * (first + i) + up] : 0.f;
-    if (warps > 16) s += part[2 * (first + 16 + i) + up];
+    s = part[2 * (first + i % warps) + up];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    for (int o = warps / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     buf ^= 1;
   }
   const float other = __shfl_xor_sync(0xffffffffu, s, 16);
@@ -183,7 +186,8 @@ __device__ __forceinline__ float2 row_sum(float2 v, float2 (*smem)[32], int& buf
 //            neighbours of the row as well), and each value is picked out at the row's offset; needs a barrier in front of `get`
 //   kDirect  from global memory
 enum { kDirect, kOwn, kWindow };
-template <class T, int V, int kMode> struct Feed {
+template <class T, class C, int kMode> struct Feed {
+  static constexpr int V = C::V;
   static constexpr int kRun = V * static_cast<int>(sizeof(T));      // kOwn: 8 or 16 bytes
   static_assert(kMode != kOwn || kRun == 8 || kRun == 16, "a run is one copy");
   const T* base;      // NULL: no such tensor
@@ -191,24 +195,24 @@ template <class T, int V, int kMode> struct Feed {
   uint32_t slot;      // shared address of the first stage, the same for all threads
   __host__ __device__ static constexpr uint32_t window(int D) { return (static_cast<uint32_t>(D) * sizeof(T) + 30) / 16 * 16; }
   // bytes of one stage
-  __host__ __device__ static uint32_t bytes(int threads, int side, int D) {
-    return kMode == kOwn ? 8 * static_cast<int>(sizeof(T)) * threads : kMode == kWindow ? side * window(D) : 0;
+  __host__ __device__ static constexpr uint32_t bytes(int D) {
+    return kMode == kOwn ? 8 * static_cast<int>(sizeof(T)) * C::threads : kMode == kWindow ? C::side * window(D) : 0;
   }
-  __device__ __forceinline__ Feed(const void* p, int64_t stride, uint32_t& smem, int side, int D) : base(static_cast<const T*>(p)), stride(stride), slot(smem) {
-    if (base) smem += 2 * bytes(blockDim.x, side, D);
+  __device__ __forceinline__ Feed(const void* p, int64_t stride, uint32_t& smem, int D) : base(static_cast<const T*>(p)), stride(stride), slot(smem) {
+    if (base) smem += 2 * bytes(D);
   }
   __device__ __forceinline__ static uint32_t place(int sub, int D) { return kMode == kOwn ? threadIdx.x * kRun : sub * window(D); }
   // row m into a stage
-  __device__ __forceinline__ void ahead(long m, uint32_t to, const Cols& c, int sub) const {
+  __device__ __forceinline__ void ahead(long m, uint32_t to, const C& c, int sub) const {
     if (!base) return;
     to += slot + place(sub, c.D);
     if constexpr (kMode == kOwn) {      // (one vector to a thread)
 #pragma unroll
       for (int e = 0; e < 8; e += V) {
-        if (!c.in<V>(0, e)) continue;
-        const T* from = base + m * stride + c.at<V>(0, e);
-        if constexpr (kRun == 16) cp_async16_at(to + e / V * kRun * blockDim.x, from);
-        else cp_async8_at(to + e / V * kRun * blockDim.x, from);
+        if (!c.in(0, e)) continue;
+        const T* from = base + m * stride + c.at(0, e);
+        if constexpr (kRun == 16) cp_async16_at(to + e / V * kRun * C::threads, from);
+        else cp_async8_at(to + e / V * kRun * C::threads, from);
       }
     } else if constexpr (kMode == kWindow) {
       const uintptr_t at = reinterpret_cast<uintptr_t>(base + m * stride), begin = at & ~static_cast<uintptr_t>(15);
@@ -217,25 +221,25 @@ template <class T, int V, int kMode> struct Feed {
     }
   }
   // vector j of row m, of which this thread has some
-  __device__ __forceinline__ void get(long m, uint32_t from, const Cols& c, int j, int sub, F (&f)[N]) const {
+  __device__ __forceinline__ void get(long m, uint32_t from, const C& c, int j, int sub, F (&f)[N]) const {
     if (!base) {
       fill(f, 0.f);
     } else if constexpr (kMode == kOwn) {
 #pragma unroll
       for (int e = 0; e < 8; e += V) {
         Raw<T, V> r;
-        const uint32_t at = slot + from + place(sub, c.D) + e / V * kRun * blockDim.x;
+        const uint32_t at = slot + from + place(sub, c.D) + e / V * kRun * C::threads;
         if constexpr (kRun == 16) r.piece(0) = shared_load16(at);
         else r.piece(0) = shared_load8(at);
 #pragma unroll
-        for (int k = 0; k < V / 2; ++k) f[e / 2 + k] = V == 8 || c.in<V>(0, e) ? r.pair(k) : both(0.f);
+        for (int k = 0; k < V / 2; ++k) f[e / 2 + k] = V == 8 || c.in(0, e) ? r.pair(k) : both(0.f);
       }
     } else if constexpr (kMode == kWindow) {
       const uint32_t at = slot + from + place(sub, c.D) + (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base + m * stride)) & 15);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) half_of(f[e / 2], e % 2) = c.in<V>(j, e) ? shared_load<T>(at + c.at<V>(j, e) * static_cast<int>(sizeof(T))) : 0.f;
+      for (int e = 0; e < 8; ++e) half_of(f[e / 2], e % 2) = c.in(j, e) ? shared_load<T>(at + c.at(j, e) * static_cast<int>(sizeof(T))) : 0.f;
     } else {
-      load<V>(base + m * stride, c, j, f);
+      load(base + m * stride, c, j, f);
     }
   }
 };
@@ -247,7 +251,8 @@ struct Shared {
   float columns[32];
   float4 stats[2][32];      // backward: each warp's token's
 };
-template <int V, int NV> __device__ __forceinline__ void count_columns(Shared& sh, const Cols& c) {
+template <int NV, class C> __device__ __forceinline__ void count_columns(Shared& sh, const C& c) {
+  constexpr int V = C::V;
   if (threadIdx.x < 32) {
     const int first = 32 * static_cast<int>(threadIdx.x);
     int n = 0;      // of warp threadIdx.x of a token: runs of 32 threads' values
@@ -262,9 +267,9 @@ template <int V, int NV> __device__ __forceinline__ void count_columns(Shared& s
 
 // Mean and 1 / deviation of a row with one barrier: each warp's mean and its squares about it, joined as
 // sum over warps of (squares + columns (mean of the warp - mean)^2).
-template <int V, int NV>
-__device__ __forceinline__ float2 statistics(const F (&a)[NV][N], const ttt_b200_block_args& p, const Cols& c, Shared& sh, int& buf) {
-  const int width = c.width;
+template <int NV, class C>
+__device__ __forceinline__ float2 statistics(const F (&a)[NV][N], const ttt_b200_block_args& p, const C& c, Shared& sh, int& buf) {
+  constexpr int V = C::V;
   const float inv = 1.f / static_cast<float>(p.D);
   float mean = 0.f;
   if (p.layer) {
@@ -281,52 +286,53 @@ __device__ __forceinline__ float2 statistics(const F (&a)[NV][N], const ttt_b200
   F sq = both(0.f);
 #pragma unroll
   for (int j = 0; j < NV; ++j)
-    if (c.in<V>(j)) {
+    if (c.in(j)) {
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         F v = add2(a[j][k], both(-mean));
-        if (2 * k + 1 >= V) v = make_float2(c.in<V>(j, 2 * k) ? v.x : 0.f, c.in<V>(j, 2 * k + 1) ? v.y : 0.f);      // (the first run is there)
+        if (2 * k + 1 >= V) v = make_float2(c.in(j, 2 * k) ? v.x : 0.f, c.in(j, 2 * k + 1) ? v.y : 0.f);      // (the first run is there)
         sq = fma2(v, v, sq);
       }
     }
   float q = fold(sq);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
-  if (width > 32) {
-    const int warp = threadIdx.x >> 5, warps = width >> 5, home = warp & -warps, i = threadIdx.x & 31;
-    if (i == 0) sh.part[buf][warp] = make_float2(mean, q);
+  if constexpr (C::width > 32) {
+    constexpr int warps = C::width / 32;
+    const int warp = threadIdx.x >> 5, home = warp & -warps, i = threadIdx.x % warps;
+    if ((threadIdx.x & 31) == 0) sh.part[buf][warp] = make_float2(mean, q);
     __syncthreads();
-    const float2 v = i < warps ? sh.part[buf][home + i] : make_float2(0.f, 0.f);      // a lane for each warp
+    const float2 v = sh.part[buf][home + i];      // a lane for each warp
     q = v.y;
     if (p.layer) {
-      const float n = sh.columns[i];      // (0 behind the last warp)
+      const float n = sh.columns[i];
       mean = n * v.x;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
+      for (int o = warps / 2; o > 0; o >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
       mean *= inv;
       q = fmaf(n * (v.x - mean), v.x - mean, q);
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+    for (int o = warps / 2; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
     buf ^= 1;
   }
   return make_float2(mean, rsqrtf(fmaf(q, inv, p.eps)));
 }
 
-template <class T, class R, int V, int kThreads>
-__global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kernel(const ttt_b200_block_args p, const Plan q) {
+template <class T, class R, class C>
+__global__ void __launch_bounds__(C::threads, 1024 / C::threads) block_forward_kernel(const ttt_b200_block_args p, const Plan q) {
   wait_for_predecessor();
-  constexpr int kMode = V > 1 ? kOwn : kWindow, NV = 1;
+  constexpr int kMode = C::V > 1 ? kOwn : kWindow, NV = 1;
   __shared__ Shared sh;
   extern __shared__ __align__(16) unsigned char stages[];
   uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(stages));
   int buf = 0;
-  const int lane = threadIdx.x % q.width, sub = threadIdx.x / q.width;
-  const Cols c = {lane, q.width, p.D};
-  const long step = static_cast<long>(q.ctas) * q.side;
-  const Feed<T, V, kMode> fo(p.o, p.o_stride, at, q.side, p.D), fg(p.gate, p.gate_stride, at, q.side, p.D);
-  const Feed<R, V, kMode> fx(p.residual, p.residual_stride, at, q.side, p.D);
-  const uint32_t small = Feed<T, V, kMode>::bytes(blockDim.x, q.side, p.D), large = Feed<R, V, kMode>::bytes(blockDim.x, q.side, p.D);
+  const int lane = threadIdx.x % C::width, sub = threadIdx.x / C::width;
+  const C c = {lane, p.D};
+  const long step = static_cast<long>(q.ctas) * C::side;
+  const Feed<T, C, kMode> fo(p.o, p.o_stride, at, p.D), fg(p.gate, p.gate_stride, at, p.D);
+  const Feed<R, C, kMode> fx(p.residual, p.residual_stride, at, p.D);
+  const uint32_t small = Feed<T, C, kMode>::bytes(p.D), large = Feed<R, C, kMode>::bytes(p.D);
   auto ahead = [&](long m, int stage) {
     if (m < p.M) {
       fo.ahead(m, stage * small, c, sub);
@@ -335,11 +341,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kerne
     }
     cp_async_commit();
   };
-  long m = static_cast<long>(blockIdx.x) * q.side + sub;
+  long m = static_cast<long>(blockIdx.x) * C::side + sub;
   ahead(m, 0);
-  count_columns<V, NV>(sh, c);
+  count_columns<NV>(sh, c);
   int stage = 0;
-  for (long base = static_cast<long>(blockIdx.x) * q.side; base < p.M; base += step, stage ^= 1, m += step) {
+  for (long base = static_cast<long>(blockIdx.x) * C::side; base < p.M; base += step, stage ^= 1, m += step) {
     const bool live = m < p.M;
     cp_async_wait<0>();
     if constexpr (kMode == kWindow) __syncthreads();
@@ -349,17 +355,17 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kerne
     for (int j = 0; j < NV; ++j) {
 #pragma unroll
       for (int k = 0; k < N; ++k) a[j][k] = z[j][k] = both(0.f);
-      if (live && c.in<V>(j)) fo.get(m, stage * small, c, j, sub, a[j]);
+      if (live && c.in(j)) fo.get(m, stage * small, c, j, sub, a[j]);
     }
     float2 s1 = make_float2(0.f, 1.f), s2 = s1;
-    if (p.post_weight) s1 = statistics<V, NV>(a, p, c, sh, buf);
+    if (p.post_weight) s1 = statistics<NV>(a, p, c, sh, buf);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (!(live && c.in<V>(j))) continue;
+      if (!(live && c.in(j))) continue;
       F w[N], b[N];
       if (p.post_weight) {
-        weights<V>(p.post_weight, c, j, 0.f, w);
-        weights<V>(p.post_bias, c, j, 0.f, b);
+        weights(p.post_weight, c, j, 0.f, w);
+        weights(p.post_bias, c, j, 0.f, b);
 #pragma unroll
         for (int k = 0; k < N; ++k) a[j][k] = mac(times(plus(a[j][k], both(-s1.x)), both(s1.y)), w[k], b[k]);
       }
@@ -371,22 +377,22 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kerne
         for (int k = 0; k < N; ++k) a[j][k] = times(a[j][k], g[k]);
       }
       fx.get(m, stage * large, c, j, sub, z[j]);
-      weights<V>(p.scale, c, j, 1.f, w);
+      weights(p.scale, c, j, 1.f, w);
 #pragma unroll
       for (int k = 0; k < N; ++k) z[j][k] = mac(w[k], a[j][k], z[j][k]);
-      store<V>(static_cast<R*>(p.x) + m * p.D, c, j, z[j]);
+      store(static_cast<R*>(p.x) + m * p.D, c, j, z[j]);
     }
     if (p.pre_weight) {
-      s2 = statistics<V, NV>(z, p, c, sh, buf);
+      s2 = statistics<NV>(z, p, c, sh, buf);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (live && c.in<V>(j)) {
+        if (live && c.in(j)) {
           F w[N], b[N];
-          weights<V>(p.pre_weight, c, j, 0.f, w);
-          weights<V>(p.pre_bias, c, j, 0.f, b);
+          weights(p.pre_weight, c, j, 0.f, w);
+          weights(p.pre_bias, c, j, 0.f, b);
 #pragma unroll
           for (int k = 0; k < N; ++k) z[j][k] = mac(times(plus(z[j][k], both(-s2.x)), both(s2.y)), w[k], b[k]);
-          store<V>(static_cast<T*>(p.n) + m * p.D, c, j, z[j]);
+          store(static_cast<T*>(p.n) + m * p.D, c, j, z[j]);
         }
       }
     }
@@ -396,44 +402,44 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_forward_kerne
 
 // Sums over tokens of a thread's columns: in registers, or, of sixteen columns, in shared memory.
 enum { kDw1, kDb1, kDsc, kDw2, kDb2, kSums };
-template <int V, int NV, bool kShared> struct Sums {
+template <class C, int NV, bool kShared> struct Sums {
   F r[kShared ? 1 : kSums][NV][N];
   float* s;
-  __device__ __forceinline__ F get(int k, int j, int i, const Cols& c) const {
+  __device__ __forceinline__ F get(int k, int j, int i, const C& c) const {
     if constexpr (!kShared) return r[k][j][i];
-    else if constexpr (V > 1) return c.in<V>(j, 2 * i) ? *reinterpret_cast<const F*>(s + k * c.D + c.at<V>(j, 2 * i)) : both(0.f);
-    else return make_float2(c.in<V>(j, 2 * i) ? s[k * c.D + c.at<V>(j, 2 * i)] : 0.f, c.in<V>(j, 2 * i + 1) ? s[k * c.D + c.at<V>(j, 2 * i + 1)] : 0.f);
+    else if constexpr (C::V > 1) return c.in(j, 2 * i) ? *reinterpret_cast<const F*>(s + k * c.D + c.at(j, 2 * i)) : both(0.f);
+    else return make_float2(c.in(j, 2 * i) ? s[k * c.D + c.at(j, 2 * i)] : 0.f, c.in(j, 2 * i + 1) ? s[k * c.D + c.at(j, 2 * i + 1)] : 0.f);
   }
-  __device__ __forceinline__ void set(int k, int j, int i, const Cols& c, F v) {
+  __device__ __forceinline__ void set(int k, int j, int i, const C& c, F v) {
     if constexpr (!kShared) {
       r[k][j][i] = v;
-    } else if constexpr (V > 1) {
-      if (c.in<V>(j, 2 * i)) *reinterpret_cast<F*>(s + k * c.D + c.at<V>(j, 2 * i)) = v;
+    } else if constexpr (C::V > 1) {
+      if (c.in(j, 2 * i)) *reinterpret_cast<F*>(s + k * c.D + c.at(j, 2 * i)) = v;
     } else {
-      if (c.in<V>(j, 2 * i)) s[k * c.D + c.at<V>(j, 2 * i)] = v.x;
-      if (c.in<V>(j, 2 * i + 1)) s[k * c.D + c.at<V>(j, 2 * i + 1)] = v.y;
+      if (c.in(j, 2 * i)) s[k * c.D + c.at(j, 2 * i)] = v.x;
+      if (c.in(j, 2 * i + 1)) s[k * c.D + c.at(j, 2 * i + 1)] = v.y;
     }
   }
-  __device__ __forceinline__ void add(int k, int j, int i, const Cols& c, F v) { set(k, j, i, c, add2(get(k, j, i, c), v)); }
-  __device__ __forceinline__ void add(int k, int j, int i, const Cols& c, F a, F b) { set(k, j, i, c, fma2(a, b, get(k, j, i, c))); }
+  __device__ __forceinline__ void add(int k, int j, int i, const C& c, F v) { set(k, j, i, c, add2(get(k, j, i, c), v)); }
+  __device__ __forceinline__ void add(int k, int j, int i, const C& c, F a, F b) { set(k, j, i, c, fma2(a, b, get(k, j, i, c))); }
 };
 
-template <class T, class R, int V, int NV, bool kShared, int kThreads>
-__global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1) block_backward_kernel(const ttt_b200_block_args p, const Plan q) {
+template <class T, class R, class C, int NV, bool kShared>
+__global__ void __launch_bounds__(C::threads, 512 / C::threads) block_backward_kernel(const ttt_b200_block_args p, const Plan q) {
   wait_for_predecessor();
-  constexpr int kMode = kShared ? kDirect : V > 1 ? kOwn : kWindow;
+  constexpr int kMode = kShared ? kDirect : C::V > 1 ? kOwn : kWindow;
   __shared__ Shared sh;
   extern __shared__ __align__(16) unsigned char stages[];
   uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(stages));
   int buf = 0;
-  const int lane = threadIdx.x % q.width, sub = threadIdx.x / q.width;
-  const Cols c = {lane, q.width, p.D};
-  const long step = static_cast<long>(q.ctas) * q.side;
-  const Feed<T, V, kMode> fo(p.o, p.o_stride, at, q.side, p.D), fg(p.gate, p.gate_stride, at, q.side, p.D);
-  const Feed<T, V, kMode> fn(p.pre_weight ? p.grad_n : nullptr, p.gn_stride, at, q.side, p.D);
-  const Feed<R, V, kMode> fx(p.pre_weight ? p.residual : nullptr, p.residual_stride, at, q.side, p.D);
-  const Feed<R, V, kMode> fd(p.grad_x, p.gx_stride, at, q.side, p.D);
-  const uint32_t small = Feed<T, V, kMode>::bytes(blockDim.x, q.side, p.D), large = Feed<R, V, kMode>::bytes(blockDim.x, q.side, p.D);
+  const int lane = threadIdx.x % C::width, sub = threadIdx.x / C::width;
+  const C c = {lane, p.D};
+  const long step = static_cast<long>(q.ctas) * C::side;
+  const Feed<T, C, kMode> fo(p.o, p.o_stride, at, p.D), fg(p.gate, p.gate_stride, at, p.D);
+  const Feed<T, C, kMode> fn(p.pre_weight ? p.grad_n : nullptr, p.gn_stride, at, p.D);
+  const Feed<R, C, kMode> fx(p.pre_weight ? p.residual : nullptr, p.residual_stride, at, p.D);
+  const Feed<R, C, kMode> fd(p.grad_x, p.gx_stride, at, p.D);
+  const uint32_t small = Feed<T, C, kMode>::bytes(p.D), large = Feed<R, C, kMode>::bytes(p.D);
   const uint32_t stats = static_cast<uint32_t>(__cvta_generic_to_shared(&sh.stats[0][threadIdx.x >> 5]));
   auto ahead = [&](long m, int stage) {
     if (m < p.M) {
@@ -447,20 +453,20 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
     cp_async_commit();
   };
   const float inv = 1.f / static_cast<float>(p.D);
-  Sums<V, NV, kShared> sums;
+  Sums<C, NV, kShared> sums;
   sums.s = reinterpret_cast<float*>(stages);
 #pragma unroll
   for (int j = 0; j < NV; ++j)
-    if (!kShared || c.in<V>(j)) {
+    if (!kShared || c.in(j)) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int k = 0; k < kSums; ++k) sums.set(k, j, i, c, both(0.f));
     }
-  long m = static_cast<long>(blockIdx.x) * q.side + sub;
+  long m = static_cast<long>(blockIdx.x) * C::side + sub;
   ahead(m, 0);
   int stage = 0;
-  for (long base = static_cast<long>(blockIdx.x) * q.side; base < p.M; base += step, stage ^= 1, m += step) {
+  for (long base = static_cast<long>(blockIdx.x) * C::side; base < p.M; base += step, stage ^= 1, m += step) {
     const bool live = m < p.M;
     cp_async_wait<0>();
     if constexpr (kMode == kWindow) __syncthreads();
@@ -473,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
     F sx = both(0.f), sy = sx;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const bool in = live && c.in<V>(j);
+      const bool in = live && c.in(j);
 #pragma unroll
       for (int i = 0; i < N; ++i) o[j][i] = both(0.f);
       if (in) fo.get(m, stage * small, c, j, sub, o[j]);
@@ -486,8 +492,8 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
 #pragma unroll
       for (int i = 0; i < N; ++i) u[i] = o[j][i];
       if (p.post_weight) {
-        weights<V>(p.post_weight, c, j, 0.f, w);
-        weights<V>(p.post_bias, c, j, 0.f, b);
+        weights(p.post_weight, c, j, 0.f, w);
+        weights(p.post_bias, c, j, 0.f, b);
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = mac(o[j][i], w[i], b[i]);
       }
@@ -497,12 +503,12 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = times(u[i], w[i]);
       }
-      weights<V>(p.scale, c, j, 1.f, w);
+      weights(p.scale, c, j, 1.f, w);
       fx.get(m, stage * large, c, j, sub, z[j]);
 #pragma unroll
       for (int i = 0; i < N; ++i) z[j][i] = times(plus(mac(w[i], u[i], z[j][i]), both(-st.z)), both(st.w));
       fn.get(m, stage * small, c, j, sub, gn[j]);
-      weights<V>(p.pre_weight, c, j, 0.f, w);
+      weights(p.pre_weight, c, j, 0.f, w);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         sums.add(kDw2, j, i, c, gn[j][i], z[j][i]);
@@ -515,30 +521,30 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
     float2 s = make_float2(fold(sx), fold(sy));
     float m1 = 0.f, m2 = 0.f;
     if (p.pre_weight) {
-      s = row_sum(s, sh.part, buf, q.width);
+      s = row_sum<C>(s, sh.part, buf);
       m1 = p.layer ? s.x * inv : 0.f;
       m2 = s.y * inv;
     }
     sx = sy = both(0.f);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (!(live && c.in<V>(j))) continue;
+      if (!(live && c.in(j))) continue;
       fd.get(m, stage * large, c, j, sub, d2[j]);
       if (p.pre_weight) {
 #pragma unroll
         for (int i = 0; i < N; ++i) d2[j][i] = mac(both(st.w), mac(z[j][i], both(-m2), plus(gn[j][i], both(-m1))), d2[j][i]);
       }
-      if (p.grad_residual) store<V>(static_cast<R*>(p.grad_residual) + m * p.D, c, j, d2[j]);
+      if (p.grad_residual) store(static_cast<R*>(p.grad_residual) + m * p.D, c, j, d2[j]);
       F u[N], w[N], b[N], v[N], g[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) u[i] = o[j][i];
       if (p.post_weight) {
-        weights<V>(p.post_weight, c, j, 0.f, w);
-        weights<V>(p.post_bias, c, j, 0.f, b);
+        weights(p.post_weight, c, j, 0.f, w);
+        weights(p.post_bias, c, j, 0.f, b);
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = mac(o[j][i], w[i], b[i]);
       }
-      weights<V>(p.scale, c, j, 1.f, b);
+      weights(p.scale, c, j, 1.f, b);
       if (p.gate) {
         fg.get(m, stage * small, c, j, sub, g);
         gate<true>(p.activation, g, v, g);
@@ -549,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
           g[i] = times(times(d2[j][i], u[i]), g[i]);
           d2[j][i] = times(d2[j][i], v[i]);
         }
-        store<V>(static_cast<T*>(p.grad_gate) + m * p.D, c, j, g);
+        store(static_cast<T*>(p.grad_gate) + m * p.D, c, j, g);
       } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -569,30 +575,30 @@ __global__ void __launch_bounds__(kThreads, kThreads < 512 ? 512 / kThreads : 1)
       }
     }
     if (p.post_weight) {
-      s = row_sum(make_float2(fold(sx), fold(sy)), sh.part, buf, q.width);
+      s = row_sum<C>(make_float2(fold(sx), fold(sy)), sh.part, buf);
       m1 = p.layer ? s.x * inv : 0.f;
       m2 = s.y * inv;
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (!(live && c.in<V>(j))) continue;
+      if (!(live && c.in(j))) continue;
       if (p.post_weight) {
 #pragma unroll
         for (int i = 0; i < N; ++i) d2[j][i] = times(both(st.y), mac(o[j][i], both(-m2), plus(d2[j][i], both(-m1))));
       }
-      store<V>(static_cast<T*>(p.grad_o) + m * p.D, c, j, d2[j]);
+      store(static_cast<T*>(p.grad_o) + m * p.D, c, j, d2[j]);
     }
   }
-  float* part = q.part + (static_cast<long>(blockIdx.x) * q.side + sub) * kSums * p.D;
+  float* part = q.part + (static_cast<long>(blockIdx.x) * C::side + sub) * kSums * p.D;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    if (!c.in<V>(j)) continue;
+    if (!c.in(j)) continue;
 #pragma unroll
     for (int k = 0; k < kSums; ++k) {
       F v[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] = sums.get(k, j, i, c);
-      store<V>(part + static_cast<long>(k) * p.D, c, j, v);
+      store(part + static_cast<long>(k) * p.D, c, j, v);
     }
   }
 }
@@ -629,9 +635,9 @@ constexpr int kWide = 4096;      // backward of wider rows: sixteen values to a 
 void plan(Plan& q, const ttt_b200_block_args& p, bool backward) {
   const bool wide = p.D > kWide;
   q.width = width_of(p.D, wide && backward ? 16 : 8);
-  q.side = std::max(1, 128 / q.width);
-  const long most = static_cast<long>(sm_count()) * std::max(1, (backward ? 512 : 1024) / (q.width * q.side));
-  q.ctas = static_cast<int>(std::min<long>(most, (p.M + q.side - 1) / q.side));
+  const int side = side_of(q.width);
+  const long most = static_cast<long>(sm_count()) * ((backward ? 512 : 1024) / (q.width * side));
+  q.ctas = static_cast<int>(std::min<long>(most, (p.M + side - 1) / side));
 }
 
 template <class R> constexpr int kRun = sizeof(R) == 4 ? 4 : 8;      // V of rows that start on its boundaries
@@ -661,54 +667,65 @@ template <class K> int launch(K kernel, const Plan& q, size_t bytes, cudaStream_
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
     if (e != cudaSuccess) return ttt_set_error(TTT_B200_ERR_LAUNCH, cudaGetErrorString(e));
   }
-  ttt_launch_overlapped(kernel, q.ctas, q.width * q.side, static_cast<uint32_t>(bytes), s, p, q);
+  ttt_launch_overlapped(kernel, q.ctas, q.width * side_of(q.width), static_cast<uint32_t>(bytes), s, p, q);
   return launched(what);
 }
 
-template <class T, class R, int V, int kThreads> int forward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
-  constexpr int kMode = V > 1 ? kOwn : kWindow;
-  const int n = q.width * q.side;
-  const size_t bytes = 2 * (Feed<T, V, kMode>::bytes(n, q.side, p.D) * (1 + (p.gate != nullptr)) +
-                            Feed<R, V, kMode>::bytes(n, q.side, p.D) * (p.residual != nullptr));
-  return launch(block_forward_kernel<T, R, V, kThreads>, q, bytes, s, p, "block norm");
+template <class T, class R, class C> int forward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
+  constexpr int kMode = C::V > 1 ? kOwn : kWindow;
+  const size_t bytes = 2 * (Feed<T, C, kMode>::bytes(p.D) * (1 + (p.gate != nullptr)) + Feed<R, C, kMode>::bytes(p.D) * (p.residual != nullptr));
+  return launch(block_forward_kernel<T, R, C>, q, bytes, s, p, "block norm");
+}
+template <class T, class R, int kWidth> int forward_of(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
+  return vectors(p, false, kRun<R>) ? forward_as<T, R, Cols<kRun<R>, kWidth>>(p, q, s) : forward_as<T, R, Cols<1, kWidth>>(p, q, s);
 }
 
 template <class T, class R> int forward(const ttt_b200_block_args& p, cudaStream_t s) {
   Plan q = {};
   plan(q, p, false);
-  const int n = q.width * q.side;
-  const bool vec = vectors(p, false, kRun<R>);
-  if (n <= 128) return vec ? forward_as<T, R, kRun<R>, 128>(p, q, s) : forward_as<T, R, 1, 128>(p, q, s);
-  if (n <= 256) return vec ? forward_as<T, R, kRun<R>, 256>(p, q, s) : forward_as<T, R, 1, 256>(p, q, s);
-  return vec ? forward_as<T, R, kRun<R>, 1024>(p, q, s) : forward_as<T, R, 1, 1024>(p, q, s);
+  switch (q.width) {
+    case 32: return forward_of<T, R, 32>(p, q, s);
+    case 64: return forward_of<T, R, 64>(p, q, s);
+    case 128: return forward_of<T, R, 128>(p, q, s);
+    case 256: return forward_of<T, R, 256>(p, q, s);
+    case 512: return forward_of<T, R, 512>(p, q, s);
+    default: return forward_of<T, R, 1024>(p, q, s);
+  }
 }
 
-template <class T, class R, int V, int NV, bool kShared, int kThreads> int backward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
-  constexpr int kMode = kShared ? kDirect : V > 1 ? kOwn : kWindow;
-  const int n = q.width * q.side;
+template <class T, class R, class C, int NV, bool kShared> int backward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
+  constexpr int kMode = kShared ? kDirect : C::V > 1 ? kOwn : kWindow;
   const size_t bytes = kShared ? static_cast<size_t>(kSums) * p.D * sizeof(float)
-                               : 2 * (Feed<T, V, kMode>::bytes(n, q.side, p.D) * (1 + (p.gate != nullptr) + (p.pre_weight && p.grad_n)) +
-                                          Feed<R, V, kMode>::bytes(n, q.side, p.D) * ((p.pre_weight && p.residual) + (p.grad_x != nullptr)));
-  return launch(block_backward_kernel<T, R, V, NV, kShared, kThreads>, q, bytes, s, p, "block norm backward");
+                               : 2 * (Feed<T, C, kMode>::bytes(p.D) * (1 + (p.gate != nullptr) + (p.pre_weight && p.grad_n)) +
+                                      Feed<R, C, kMode>::bytes(p.D) * ((p.pre_weight && p.residual) + (p.grad_x != nullptr)));
+  return launch(block_backward_kernel<T, R, C, NV, kShared>, q, bytes, s, p, "block norm backward");
+}
+template <class T, class R, int kWidth, int NV = 1> int backward_of(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
+  return vectors(p, true, kRun<R>) ? backward_as<T, R, Cols<kRun<R>, kWidth>, NV, (NV > 1)>(p, q, s)
+                                   : backward_as<T, R, Cols<1, kWidth>, NV, (NV > 1)>(p, q, s);
+}
+template <class T, class R> int backward_kernel(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
+  if (p.D > kWide) return backward_of<T, R, 512, 2>(p, q, s);
+  switch (q.width) {
+    case 32: return backward_of<T, R, 32>(p, q, s);
+    case 64: return backward_of<T, R, 64>(p, q, s);
+    case 128: return backward_of<T, R, 128>(p, q, s);
+    case 256: return backward_of<T, R, 256>(p, q, s);
+    default: return backward_of<T, R, 512>(p, q, s);
+  }
 }
 
 template <class T, class R> int backward(const ttt_b200_block_args& p, cudaStream_t s) {
   Plan q = {};
   plan(q, p, true);
   q.part = static_cast<float*>(p.scratch);
-  const bool vec = vectors(p, true, kRun<R>);
-  const int n = q.width * q.side;
-  int rc;
-  if (p.D > kWide) rc = vec ? backward_as<T, R, kRun<R>, 2, true, 512>(p, q, s) : backward_as<T, R, 1, 2, true, 512>(p, q, s);
-  else if (n <= 128) rc = vec ? backward_as<T, R, kRun<R>, 1, false, 128>(p, q, s) : backward_as<T, R, 1, 1, false, 128>(p, q, s);
-  else if (n <= 256) rc = vec ? backward_as<T, R, kRun<R>, 1, false, 256>(p, q, s) : backward_as<T, R, 1, 1, false, 256>(p, q, s);
-  else rc = vec ? backward_as<T, R, kRun<R>, 1, false, 512>(p, q, s) : backward_as<T, R, 1, 1, false, 512>(p, q, s);
+  const int rc = backward_kernel<T, R>(p, q, s);
   if (rc) return rc;
   const long row = static_cast<long>(kSums) * p.D;
   float* dst[kSums] = {p.grad_post_weight, p.grad_post_bias, p.grad_scale, p.grad_pre_weight, p.grad_pre_bias};
   ttt_sum_job jobs[kSums];
   for (int k = 0; k < kSums; ++k)
-    jobs[k] = {q.part + static_cast<long>(k) * p.D, dst[k], p.D, row, q.ctas * q.side, TTT_B200_FP32, 0};
+    jobs[k] = {q.part + static_cast<long>(k) * p.D, dst[k], p.D, row, q.ctas * side_of(q.width), TTT_B200_FP32, 0};
   return ttt_sum_parts(jobs, kSums, s);
 }
 
@@ -718,7 +735,7 @@ extern "C" uint64_t ttt_b200_norm_gate_residual_scratch_bytes(const ttt_b200_blo
   if (check(p) || p->M == 0) return 0;
   Plan q = {};
   plan(q, *p, true);
-  return static_cast<uint64_t>(q.ctas) * q.side * kSums * p->D * sizeof(float);
+  return static_cast<uint64_t>(q.ctas) * side_of(q.width) * kSums * p->D * sizeof(float);
 }
 
 extern "C" int ttt_b200_norm_gate_residual(const ttt_b200_block_args* p, void* stream) {
