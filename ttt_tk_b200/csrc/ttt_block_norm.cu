@@ -12,10 +12,11 @@
 // what the forward read (not from the z it wrote, whose rounding would be in the sums), keeps the sums over tokens of its columns to
 // itself over all its tokens and leaves them as one part per CTA for an ordered sum.
 //
-// Measured, fp32 residual stream, layer norms, all weights, tanh gate, 16384 x 2048 bf16: forward 104 us (4.5 TB/s), backward 211 us
-// (3.5 TB/s); bf16 residual, RMS norms 79 us (4.2) and 187 us (2.9); rows of 2047 118 and 257 us.  Not memory but issued instructions
-// and the wait at a token's barriers hold them: 1024 threads to an SM forward, 512 backward (128 registers, 40 of them sums over
-// tokens).  So the width is a constant of the kernel (118 -> 104 and 230 -> 211 us; rows of 2047 174 -> 118 and 349 -> 257).
+// Measured, fp32 residual stream, layer norms, all weights, tanh gate, 16384 x 2048 bf16: forward 97 us (4.8 TB/s), backward 191 us
+// (3.9 TB/s); bf16 residual, RMS norms 77 us (4.4) and 185 us (2.9); rows of 2047 117 and 256 us; 4096 x 8192, layer norms, 114 us
+// (2.9) and 372 us (1.4).  Not memory but issued instructions and the wait at a token's barriers hold them: 1024 threads to an SM
+// forward (1280: 106 us, the L1 has less room for the weights), 512 backward (128 registers, 40 of them sums over tokens).  So the
+// width is a constant of the kernel (118 -> 104 and 230 -> 211 us; rows of 2047 174 -> 118 and 349 -> 257).
 #include <algorithm>
 #include <cstdio>
 #include <type_traits>
@@ -40,15 +41,16 @@ constexpr int side_of(int width) { return width < 128 ? 128 / width : 1; }      
 //          twice as many cycles.  16384 x 2048, forward and backward: 128 -> 118 and 262 -> 230 us; with a bf16 residual, whose
 //          rows then take twice as many accesses, 78 -> 95 and 209 -> 241 us, so there V stays 8.
 //   V = 1  where a row does not start on a boundary of V values
-// The last runs of a token may not be there.
+// The last runs of a token may not be there, unless its values fill its threads (kFull): no comparisons and selections then,
+// forward and backward 104 -> 97 and 211 -> 191 us of the first, 79 -> 77 and 187 -> 185 of the second.
 constexpr int N = 4;
 using F = float2;
 
-template <int kRun, int kWidth> struct Cols {
+template <int kRun, int kWidth, bool kFull> struct Cols {
   static constexpr int V = kRun, width = kWidth, side = side_of(kWidth), threads = width * side;
   int lane, D;      // thread among the token's; values of a token
   __device__ __forceinline__ int at(int j, int e) const { return ((j * (8 / V) + e / V) * width + lane) * V + e % V; }      // column of value e of vector j
-  __device__ __forceinline__ bool in(int j, int e = 0) const { return at(j, e - e % V) < D; }
+  __device__ __forceinline__ bool in(int j, int e = 0) const { return kFull || at(j, e - e % V) < D; }
 };
 
 __device__ __forceinline__ float& half_of(F& f, int e) { return e ? f.y : f.x; }
@@ -677,7 +679,8 @@ template <class T, class R, class C> int forward_as(const ttt_b200_block_args& p
   return launch(block_forward_kernel<T, R, C>, q, bytes, s, p, "block norm");
 }
 template <class T, class R, int kWidth> int forward_of(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
-  return vectors(p, false, kRun<R>) ? forward_as<T, R, Cols<kRun<R>, kWidth>>(p, q, s) : forward_as<T, R, Cols<1, kWidth>>(p, q, s);
+  if (!vectors(p, false, kRun<R>)) return forward_as<T, R, Cols<1, kWidth, false>>(p, q, s);
+  return p.D == 8 * kWidth ? forward_as<T, R, Cols<kRun<R>, kWidth, true>>(p, q, s) : forward_as<T, R, Cols<kRun<R>, kWidth, false>>(p, q, s);
 }
 
 template <class T, class R> int forward(const ttt_b200_block_args& p, cudaStream_t s) {
@@ -701,8 +704,9 @@ template <class T, class R, class C, int NV, bool kShared> int backward_as(const
   return launch(block_backward_kernel<T, R, C, NV, kShared>, q, bytes, s, p, "block norm backward");
 }
 template <class T, class R, int kWidth, int NV = 1> int backward_of(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
-  return vectors(p, true, kRun<R>) ? backward_as<T, R, Cols<kRun<R>, kWidth>, NV, (NV > 1)>(p, q, s)
-                                   : backward_as<T, R, Cols<1, kWidth>, NV, (NV > 1)>(p, q, s);
+  if (!vectors(p, true, kRun<R>)) return backward_as<T, R, Cols<1, kWidth, false>, NV, (NV > 1)>(p, q, s);
+  return p.D == 8 * NV * kWidth ? backward_as<T, R, Cols<kRun<R>, kWidth, true>, NV, (NV > 1)>(p, q, s)
+                                : backward_as<T, R, Cols<kRun<R>, kWidth, false>, NV, (NV > 1)>(p, q, s);
 }
 template <class T, class R> int backward_kernel(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
   if (p.D > kWide) return backward_of<T, R, 512, 2>(p, q, s);
