@@ -239,6 +239,9 @@ BLOCK = [
     ("fp32", 5, 516, "rms", "sigmoid", False, True, True, True, True, True, False),
     ("fp16", 3, 4100, "layer", "silu", True, True, True, True, True, True, False),
     ("fp16", 6, 300, "rms", "gelu", False, True, True, True, True, True, False),       # a 16-bit stream: one by one
+    ("bf16", 7, 512, "layer", "gelu", True, True, True, True, True, True, False),       # rows that fill their threads
+    ("fp16", 5, 1024, "rms", "silu", False, True, True, True, True, True, True),
+    ("bf16", 5, 384, "layer", "sigmoid", False, True, True, True, True, True, False),
 ]
 
 

@@ -175,3 +175,11 @@ def test_sizes_that_indices_could_not_hold():
     with pytest.raises(ValueError, match="too large"):
         x = one.expand(1, (1 << 30) + 1, 1)
         ssm.ssm_scan(x, x, torch.zeros(1, 1), x.unsqueeze(-1), x.unsqueeze(-1))
+
+
+def test_a_flag_that_is_neither_true_nor_false():
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        _conv(heads=torch.ones(2))
+    i = scan_inputs(1, "bf16", 2, 8, 16, 4, 1)
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        ssm.ssm_scan(*[i[k] for k in ("x", "dt", "A", "B", "C")], softplus=torch.ones(2))

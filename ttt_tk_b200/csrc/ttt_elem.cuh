@@ -24,22 +24,6 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// Eight consecutive elements, 16-byte aligned: one or two 16-byte accesses.
-template <class T> __device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
-  alignas(16) T v[8];
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) f[k] = to_f32(v[k]);
-}
-template <class T> __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
-  alignas(16) T v[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = from_f32<T>(f[k]);
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
-}
-
 // Two fp32 operations in one instruction (sm_100): halves the issue slots of fp32-heavy loops.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 r;
@@ -96,7 +80,7 @@ __device__ __forceinline__ float2 least(float2 a, float b) { return make_float2(
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// 16 bytes global -> shared without registers, to a shared address; of a piece of `bytes` the rest becomes zeros and is not read.
+// 16, 8 or 4 bytes global -> shared without registers, to a shared address; of a piece of `bytes` the rest becomes zeros and is not read.
 __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }

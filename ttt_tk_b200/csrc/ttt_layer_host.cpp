@@ -37,6 +37,12 @@ int64_t integer(PyObject* o) {
   return v;
 }
 
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);      // (a tensor of several values is neither)
+  if (v < 0) throw PythonError();
+  return v == 1;
+}
+
 // The tensors of a call: checked one by one against shape and type, their devices at the end.
 class Call {
  public:
@@ -208,7 +214,7 @@ void conv_inputs(Call& c, ttt_b200_conv_args& a, PyObject* x, PyObject* const* v
   a.activation = static_cast<int32_t>(integer(v[2]));
   a.state = c.whole(v[3], "state", c.type(), {a.B, a.K - 1, a.D});
   a.lengths = c.i32(v[4], "lengths", a.B);
-  a.heads = PyObject_IsTrue(v[5]) == 1;
+  a.heads = truth(v[5]);
   if (a.heads) c.need(a.D % 64 == 0 && a.T % 64 == 0, "heads need multiples of 64 channels and tokens");
 }
 
@@ -224,7 +230,7 @@ PyObject* conv(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     const Tensor y = a.heads ? at::empty({a.B, a.D / 64, a.T / 64, 64, 64}, opt) : at::empty({a.B, a.T, a.D}, opt);
     Tensor end;
     const bool none = a.B == 0 || a.T == 0;
-    if (PyObject_IsTrue(v[7]) == 1) {
+    if (truth(v[7])) {
       if (!none) end = at::empty({a.B, a.K - 1, a.D}, opt);
       else end = a.state ? THPVariable_Unpack(v[4]).detach().clone() : at::zeros({a.B, a.K - 1, a.D}, opt);
     }
@@ -358,7 +364,7 @@ void scan_inputs(Call& c, ttt_b200_scan_args& a, PyObject* const* v, bool step) 
   }
   a.Dskip = c.f32(v[5], "D", {a.D});
   a.dt_bias = c.f32(v[6], "dt_bias", {a.D});
-  a.softplus = PyObject_IsTrue(v[7]) == 1;
+  a.softplus = truth(v[7]);
 }
 
 int64_t checkpoints_of(const ttt_b200_scan_args& a) { return (static_cast<int64_t>(a.T) + TTT_B200_SCAN_INTERVAL - 1) / TTT_B200_SCAN_INTERVAL; }
@@ -377,11 +383,11 @@ PyObject* scan(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     const bool none = a.B == 0 || a.T == 0;
     const Tensor y = at::empty({a.B, a.T, a.D}, opt);
     Tensor end, ck;
-    if (PyObject_IsTrue(v[10]) == 1) {
+    if (truth(v[10])) {
       if (!none) end = at::empty({a.B, a.D, a.N}, f32);
       else end = a.state ? THPVariable_Unpack(v[8]).detach().clone() : at::zeros({a.B, a.D, a.N}, f32);
     }
-    if (PyObject_IsTrue(v[11]) == 1) ck = at::empty({a.B, checkpoints_of(a), a.D, a.N}, f32);
+    if (truth(v[11])) ck = at::empty({a.B, checkpoints_of(a), a.D, a.N}, f32);
     if (!none) {
       const Tensor scratch = scratch_of(ttt_b200_ssm_scan_scratch_bytes(&a, 0), dev);
       give(a, scratch);
@@ -497,7 +503,7 @@ const Tensor& block_inputs(Call& c, ttt_b200_block_args& a, PyObject* o, PyObjec
     a.gate = g.data_ptr();
     a.gate_stride = row_stride(c, g, even);
   }
-  a.layer = PyObject_IsTrue(v[2]) == 1;
+  a.layer = truth(v[2]);
   a.activation = static_cast<int32_t>(integer(v[3]));
   a.post_weight = c.f32(v[4], "post_weight", {a.D});
   a.post_bias = c.f32(v[5], "post_bias", {a.D});
@@ -523,7 +529,7 @@ PyObject* block(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     const auto opt = at::TensorOptions().dtype(c.type()).device(dev), f32 = opt.dtype(at::kFloat);
     const Tensor x = at::empty(o.sizes(), a.residual_fp32 ? f32 : opt);
     const Tensor n = a.pre_weight ? at::empty(o.sizes(), opt) : Tensor();
-    const Tensor stats = PyObject_IsTrue(v[11]) == 1 ? at::empty({a.M, 4}, f32) : Tensor();
+    const Tensor stats = truth(v[11]) ? at::empty({a.M, 4}, f32) : Tensor();
     a.x = x.data_ptr();
     a.n = ptr(n);
     a.stats = fptr(stats);
