@@ -202,9 +202,12 @@ def norm_gate_residual_backward(grad_x, grad_n, o, residual=None, gate=None, nor
         gn = m(grad_n) if grad_n is not None else zero
         d = d + back(gn * m(w2), zh, r2)
         g2, gb2 = (gn * m(zh)).sum(0), gn.sum(0)
-    gsc = (d * m(u * gv)).sum(0)
+    # u is a sum itself: worked out with an error of half a step of |oh w1| + |b1|, however near to zero it comes, so these are its
+    # magnitudes (u = 9.7e-7 of two terms of 0.08 is off by up to 2^-24 0.16 / 9.7e-7 = 1 %)
+    ua = (m(oh) * m(w1) + (m(b1) if b1 is not None else 0.0) if w1 is not None else m(o)) if amp else u
+    gsc = (d * m(ua * gv)).sum(0)
     dv = d * m(s)
-    gg = dv * m(u * gs)
+    gg = dv * m(ua * gs)
     du = dv * m(gv)
     g1 = gb1 = None
     go = du
