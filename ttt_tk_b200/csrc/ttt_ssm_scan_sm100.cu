@@ -58,14 +58,16 @@ struct Where {
   int b, c, g, tile, ch0, cols;
   long bc;        // b * chunks + c
   int len;        // tokens of the sequence
-  __device__ Where(const ttt_b200_scan_args& p, const Plan& q, int dc) {
+  // CTAs for `count` chunks of a sequence, from chunk `from` on
+  __device__ Where(const ttt_b200_scan_args& p, const Plan& q, int dc, int count, int from) {
     long i = blockIdx.x;
     tile = static_cast<int>(i % q.tiles);
     i /= q.tiles;
     g = static_cast<int>(i % p.G);
-    bc = i / p.G;
-    c = static_cast<int>(bc % q.chunks);
-    b = static_cast<int>(bc / q.chunks);
+    i /= p.G;
+    c = from + static_cast<int>(i % count);
+    b = static_cast<int>(i / count);
+    bc = static_cast<long>(b) * q.chunks + c;
     ch0 = g * q.per + tile * dc;
     cols = min(q.per - tile * dc, dc);
     len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
@@ -280,7 +282,7 @@ template <class T, int LN> __global__ void __launch_bounds__(TH, 4) scan_forward
   constexpr int DC = S::DC, NP = S::NP, U = LN < 4 ? 4 : LN, YW = FwdSmem<T, LN>::YW;
   extern __shared__ __align__(16) unsigned char raw[];
   FwdSmem<T, LN>& m = *reinterpret_cast<FwdSmem<T, LN>*>(raw);
-  const Where w(p, q, DC);
+  const Where w(p, q, DC, q.chunks, 0);
   const Mine<LN> me(w, p.N);
   const Pair<DC> el(p, q, w);
   const int lane = threadIdx.x & 31;
@@ -411,6 +413,7 @@ template <class T, int LN> __global__ void __launch_bounds__(TH, 4) scan_forward
 }
 
 // ---- a chunk's state by itself, from zero: forwards h <- a h + delta x B; backwards (kRev) c <- a (c + dy C) -----------
+// Not that of the last chunk in the direction of the walk, which none starts from.
 template <class T, int LN> struct StateSmem {
   using S = Shape<LN>;
   alignas(16) T v[2][kTile * S::DC];      // x or dy
@@ -426,7 +429,7 @@ template <class T, int LN, bool kRev> __global__ void __launch_bounds__(TH, 4) s
   constexpr int DC = S::DC, NP = S::NP;
   extern __shared__ __align__(16) unsigned char raw[];
   StateSmem<T, LN>& m = *reinterpret_cast<StateSmem<T, LN>*>(raw);
-  const Where w(p, q, DC);
+  const Where w(p, q, DC, q.chunks - 1, kRev ? 1 : 0);
   const Mine<LN> me(w, p.N);
   const Pair<DC> el(p, q, w);
   const long DN = static_cast<long>(p.D) * p.N;
@@ -540,7 +543,7 @@ template <bool kRev> __global__ void __launch_bounds__(256) scan_join_kernel(con
   auto request = [&](int c0) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const long c = chunk(min(c0 + k, q.chunks - 1));
+      const long c = chunk(min(c0 + k, q.chunks - 2));      // (the last one's own state is not there and not needed)
       s2[k] = q.state[c * DN + dn];
       f2[k] = q.delta[c * p.D + d];
     }
@@ -590,7 +593,7 @@ __global__ void __launch_bounds__(TH, LN <= 4 ? 4 : 3) scan_backward_kernel(cons
   constexpr int DC = S::DC, NP = S::NP, ND = 32 / LN;
   extern __shared__ __align__(16) unsigned char raw[];
   BwdSmem<T, LN>& m = *reinterpret_cast<BwdSmem<T, LN>*>(raw);
-  const Where w(p, q, DC);
+  const Where w(p, q, DC, q.chunks, 0);
   const Mine<LN> me(w, p.N);
   const Pair<DC> el(p, q, w);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -1043,9 +1046,9 @@ template <class K> int launch(K kernel, size_t smem, long grid, cudaStream_t s, 
 }
 
 template <class T, int LN> int forward(const ttt_b200_scan_args& p, const Plan& q, cudaStream_t s) {
-  const long grid = static_cast<long>(p.B) * q.chunks * p.G * q.tiles;
+  const long row = static_cast<long>(p.B) * p.G * q.tiles, grid = row * q.chunks;
   if (q.chunks > 1) {
-    if (int rc = launch(scan_state_kernel<T, LN, false>, sizeof(StateSmem<T, LN>), grid, s, p, q)) return rc;
+    if (int rc = launch(scan_state_kernel<T, LN, false>, sizeof(StateSmem<T, LN>), row * (q.chunks - 1), s, p, q)) return rc;
     const long n = static_cast<long>(p.B) * p.D * p.N;
     ttt_launch_overlapped(scan_join_kernel<false>, static_cast<int>((n + 255) / 256), 256, 0, s, p, q);
   }
@@ -1053,9 +1056,9 @@ template <class T, int LN> int forward(const ttt_b200_scan_args& p, const Plan& 
 }
 
 template <class T, int LN> int backward(const ttt_b200_scan_args& p, const Plan& q, cudaStream_t s) {
-  const long grid = static_cast<long>(p.B) * q.chunks * p.G * q.tiles;
+  const long row = static_cast<long>(p.B) * p.G * q.tiles, grid = row * q.chunks;
   if (q.chunks > 1) {
-    if (int rc = launch(scan_state_kernel<T, LN, true>, sizeof(StateSmem<T, LN>), grid, s, p, q)) return rc;
+    if (int rc = launch(scan_state_kernel<T, LN, true>, sizeof(StateSmem<T, LN>), row * (q.chunks - 1), s, p, q)) return rc;
     const long n = static_cast<long>(p.B) * p.D * p.N;
     ttt_launch_overlapped(scan_join_kernel<true>, static_cast<int>((n + 255) / 256), 256, 0, s, p, q);
   }
