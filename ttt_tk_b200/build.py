@@ -18,8 +18,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libttt_mlp_b200.so")
 SOURCES = ["ttt_capi.cu", "ttt_fwd_sm100.cu", "ttt_fwd_pair_sm100.cu", "ttt_bwd_sm100.cu", "ttt_bwd_pair_sm100.cu", "ttt_fwd_cluster_sm100.cu", "ttt_bwd_cluster_sm100.cu", "ttt_linear_fwd_sm100.cu", "ttt_linear_bwd_sm100.cu",
-           "ttt_layout.cu", "ttt_glue.cu", "ttt_short_conv.cu", "ttt_ssm_scan_sm100.cu", "ttt_block_norm.cu", "ttt_sum_parts.cu", "umma_selftest.cu"]
-HEADERS = ["sm100_ptx.cuh", "ttt_device.cuh", "ttt_cluster.cuh", "ttt_elem.cuh", "ttt_sum_parts.h", "ttt_internal.h", os.path.join("..", "..", "include", "ttt_mlp_b200.h")]
+           "ttt_layout.cu", "ttt_glue.cu", "ttt_short_conv.cu", "ttt_ssm_scan_sm100.cu", "ttt_block_norm.cu", "ttt_block_norm_bwd.cu", "ttt_sum_parts.cu", "umma_selftest.cu"]
+HEADERS = ["sm100_ptx.cuh", "ttt_device.cuh", "ttt_cluster.cuh", "ttt_elem.cuh", "ttt_block_norm.cuh", "ttt_sum_parts.h", "ttt_internal.h", os.path.join("..", "..", "include", "ttt_mlp_b200.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
 
