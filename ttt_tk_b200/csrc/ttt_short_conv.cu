@@ -3,11 +3,15 @@
 //   y[b][t][d] = act(bias[d] + sum_k w[d][k] x[b][t - K + 1 + k][d])
 //   g = dy act'(pre);  dx[s] = sum_k w[d][k] g[s + K - 1 - k];  dw[d][k] = sum_t g[t] x[t - K + 1 + k];  db = sum_t g[t]
 //
-// Bound by memory: 2 K operations per value that is read and written once.  A thread owns two neighbouring channels
-// (one where rows do not start on a pair's boundary) and walks along a run of tokens with the last K - 1 inputs in registers, so that
-// an input is read once per run; the K - 1 in front of a run come from the cache.  Eight rows are requested ahead of the eight that
-// are worked on: a warp's row is 128 bytes, and it takes some 40 KB in flight to keep an SM's share of the memory busy.  The backward
-// keeps the last K values of g as well and leaves dx with a delay of K - 1 tokens.
+// Bound by memory: 2 K operations per value that is read and written once.  A thread owns two neighbouring channels (one where rows
+// do not start on a pair's boundary) and walks along a run of tokens with the last K - 1 inputs in registers, so that an input is read
+// once per run; the K - 1 in front of a run come from the cache.  Rows come through a warp's ring of four blocks of eight rows in shared
+// memory: a warp's row is 128 bytes, and it takes some 40 KB in flight to keep an SM's share of the memory busy, which registers do
+// not hold.  The backward keeps the last K values of g as well and leaves dx with a delay of K - 1 tokens.
+//
+// Measured, 4 x 2048 tokens of 2048 channels, bf16, K = 4, silu: forward 16.6 us (4.0 TB/s), backward 32 us (3.1 TB/s; 52 % of the issue
+// slots, 68 instructions per token and pair).  3 x 1001 x 1003 in fp32, single channels: 5.9 us (4.1 TB/s) and 13.5 us (2.7 TB/s).  The step of
+// 8 rows of 2048: 2.5 us, a launch.
 #include <algorithm>
 #include <cstdio>
 #include <type_traits>

@@ -17,6 +17,10 @@
 // Where they do not fill the GPU the sequence is split into chunks as well: a first kernel carries each chunk's state from
 // zero, a second one joins the chunks with exp(A sum delta), and the main kernel starts every chunk from its own state.  The
 // backward does the same from the other end.
+//
+// Measured, 4 x 2048 tokens of 1536 channels, 16 states, bf16 (24 chunks; 201 M exponentials, 45 us of their unit): states 67 us, join 5,
+// forward 93; backward states 60, join 5, backward 256, sum of parts 11.  8192 tokens of 1024 channels: 46, 7 and 63 us.  The exponential
+// unit is 79, 57, 80 and 49 % busy in states, forward, states and backward, the issue slots 52, 58, 52 and 58 %.
 #include <algorithm>
 #include <cstdio>
 #include <type_traits>
