@@ -183,3 +183,26 @@ def test_a_flag_that_is_neither_true_nor_false():
     i = scan_inputs(1, "bf16", 2, 8, 16, 4, 1)
     with pytest.raises(RuntimeError, match="ambiguous"):
         ssm.ssm_scan(*[i[k] for k in ("x", "dt", "A", "B", "C")], softplus=torch.ones(2))
+
+
+@pytest.mark.parametrize("missing", ["residual", "gate"])
+def test_c_block_backward_without_a_place_for_a_gradient(missing):
+    """An input whose gradient has no place: refused before the scratch is looked at, so nothing is launched."""
+    import ctypes
+    import struct
+
+    from ttt_tk_b200 import _lib
+    lib = _lib.lib()
+    word = ctypes.create_string_buffer(64)
+    at = ctypes.addressof(word) + 15 & ~15      # (never read)
+    p = [0] * 22      # o, residual, gate, weights x 5, x, n, stats, grad_x, grad_n, grad_o, grad_residual, grad_gate, sums x 5, scratch
+    for k in (0, 10, 11, 13, {"residual": 1, "gate": 2}[missing]):
+        p[k] = at
+    args = struct.pack("=22Q Q 6q 5i f", *p, 0, 8, 8, 8, 8, 8, 1, 8, 0, 0, 0, 1, 1e-6)
+    fn = lib.ttt_b200_norm_gate_residual_backward
+    fn.argtypes, fn.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int
+    lib.ttt_b200_last_error.restype = ctypes.c_char_p
+    assert fn(args, None) == 1 and b"null tensor pointer" in lib.ttt_b200_last_error()
+    p[{"residual": 14, "gate": 15}[missing]] = at
+    args = struct.pack("=22Q Q 6q 5i f", *p, 0, 8, 8, 8, 8, 8, 1, 8, 0, 0, 0, 1, 1e-6)
+    assert fn(args, None) == 1 and b"scratch" in lib.ttt_b200_last_error()
