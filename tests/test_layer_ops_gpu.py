@@ -242,6 +242,10 @@ BLOCK = [
     ("bf16", 7, 512, "layer", "gelu", True, True, True, True, True, True, False),       # rows that fill their threads
     ("fp16", 5, 1024, "rms", "silu", False, True, True, True, True, True, True),
     ("bf16", 5, 384, "layer", "sigmoid", False, True, True, True, True, True, False),
+    ("bf16", 150, 512, "rms", "silu", True, True, False, False, False, True, False),       # a residual and the next norm alone
+    ("fp16", 40, 203, "layer", "silu", False, True, False, False, False, True, True),
+    ("fp32", 3, 4100, "layer", "silu", False, True, False, False, False, True, False),
+    ("bf16", 9, 1000, "rms", "silu", False, True, False, False, False, True, False),
 ]
 
 

@@ -1,7 +1,7 @@
 // The end of a block and the start of the next: forward.
 //
 // Measured with all parts, 16384 x 2048 bf16: fp32 residual stream, layer norms, tanh gate 88 us (5.3 TB/s); bf16 residual, RMS norms
-// 67 us (5.0 TB/s); rows of 2047 105 us (3.2).  Issued instructions and the wait at a token's barriers are what is left above the
+// 67 us (5.0 TB/s); rows of 2047 105 us (3.2); a bf16 residual and the next RMS norm alone 44 us (6.2 TB/s).  Issued instructions and the wait at a token's barriers are what is left above the
 // memory: 1024 threads to an SM (1280: 106 us where 1024 had 97, since the L1 has less room for the weights).
 #include "ttt_block_norm.cuh"
 
@@ -21,10 +21,12 @@ __global__ void __launch_bounds__(C::threads, 1024 / C::threads) block_forward_k
   const int lane = threadIdx.x % C::width, sub = threadIdx.x / C::width;
   const C c = {lane, p.D};
   const long step = static_cast<long>(q.ctas) * C::side;
-  const bool post = C::all || p.post_weight, gated = C::all || p.gate, pre = C::all || p.pre_weight;
-  const Feed<T, C, kMode> fo(p.o, p.o_stride, at, p.D), fg(p.gate, p.gate_stride, at, p.D);
-  const Feed<R, C, kMode> fx(p.residual, p.residual_stride, at, p.D);
-  const uint32_t small = Feed<T, C, kMode>::bytes(p.D), large = Feed<R, C, kMode>::bytes(p.D);
+  constexpr bool kMore = C::all || C::bare;
+  const bool post = !C::bare && (C::all || p.post_weight), gated = !C::bare && (C::all || p.gate), pre = kMore || p.pre_weight;
+  const Feed<T, C, kMode, true> fo(p.o, p.o_stride, at, p.D);
+  const Feed<T, C, kMode, C::all> fg(gated ? p.gate : nullptr, p.gate_stride, at, p.D);
+  const Feed<R, C, kMode, kMore> fx(p.residual, p.residual_stride, at, p.D);
+  const uint32_t small = Feed<T, C, kMode, true>::bytes(p.D), large = Feed<R, C, kMode, true>::bytes(p.D);
   auto ahead = [&](long m, int stage) {
     if (m < p.M) {
       fo.ahead(m, stage * small, c, sub);
@@ -69,7 +71,7 @@ __global__ void __launch_bounds__(C::threads, 1024 / C::threads) block_forward_k
         for (int k = 0; k < N; ++k) a[j][k] = times(a[j][k], g[k]);
       }
       fx.get(m, stage * large, c, j, sub, z[j]);
-      weights<C::all>(p.scale, c, j, 1.f, w);
+      weights<C::all>(C::bare ? nullptr : p.scale, c, j, 1.f, w);
 #pragma unroll
       for (int k = 0; k < N; ++k) z[j][k] = mac(w[k], a[j][k], z[j][k]);
       store(static_cast<R*>(p.x) + m * p.D, c, j, z[j]);
@@ -80,7 +82,7 @@ __global__ void __launch_bounds__(C::threads, 1024 / C::threads) block_forward_k
       for (int j = 0; j < NV; ++j) {
         if (live && c.in(j)) {
           F w[N], b[N];
-          weights<C::all>(p.pre_weight, c, j, 0.f, w);
+          weights<kMore>(p.pre_weight, c, j, 0.f, w);
           weights(p.pre_bias, c, j, 0.f, b);
 #pragma unroll
           for (int k = 0; k < N; ++k) z[j][k] = mac(times(plus(z[j][k], both(-s2.x)), both(s2.y)), w[k], b[k]);
@@ -94,16 +96,20 @@ __global__ void __launch_bounds__(C::threads, 1024 / C::threads) block_forward_k
 
 template <class T, class R, class C> int forward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
   constexpr int kMode = C::V > 1 ? kOwn : kWindow;
-  const size_t bytes = 2 * (Feed<T, C, kMode>::bytes(p.D) * (1 + (p.gate != nullptr)) + Feed<R, C, kMode>::bytes(p.D) * (p.residual != nullptr));
+  const size_t bytes = 2 * (Feed<T, C, kMode, true>::bytes(p.D) * (1 + (p.gate != nullptr)) + Feed<R, C, kMode, true>::bytes(p.D) * (p.residual != nullptr));
   return launch(block_forward_kernel<T, R, C>, q, bytes, s, p, "block norm");
 }
-template <class T, class R, int kWidth, bool kAll> int forward_with(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
-  if (!vectors(p, false, kRun<R>)) return forward_as<T, R, Cols<1, kWidth, false, kAll>>(p, q, s);
-  return p.D == 8 * kWidth ? forward_as<T, R, Cols<kRun<R>, kWidth, true, kAll>>(p, q, s)
-                           : forward_as<T, R, Cols<kRun<R>, kWidth, false, kAll>>(p, q, s);
+template <class T, class R, int kWidth, int kParts> int forward_with(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
+  if (!vectors(p, false, kRun<R>)) return forward_as<T, R, Cols<1, kWidth, false, kParts>>(p, q, s);
+  return p.D == 8 * kWidth ? forward_as<T, R, Cols<kRun<R>, kWidth, true, kParts>>(p, q, s)
+                           : forward_as<T, R, Cols<kRun<R>, kWidth, false, kParts>>(p, q, s);
 }
 template <class T, class R, int kWidth> int forward_of(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
-  return all_parts(p) ? forward_with<T, R, kWidth, true>(p, q, s) : forward_with<T, R, kWidth, false>(p, q, s);
+  switch (parts_of(p)) {
+    case kAll: return forward_with<T, R, kWidth, kAll>(p, q, s);
+    case kBare: return forward_with<T, R, kWidth, kBare>(p, q, s);
+    default: return forward_with<T, R, kWidth, kSome>(p, q, s);
+  }
 }
 
 template <class T, class R> int forward(const ttt_b200_block_args& p, cudaStream_t s) {

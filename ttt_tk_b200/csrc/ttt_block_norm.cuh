@@ -43,10 +43,13 @@ constexpr int side_of(int width) { return width < 128 ? 128 / width : 1; }      
 constexpr int N = 4;
 using F = float2;
 
-// kAll: post norm, gate, residual, scale and pre norm are all there, backward both gradients too.  Without a branch around every one of
+// kParts kAll: post norm, gate, residual, scale and pre norm are all there, backward both gradients too.  Without a branch around every one of
 // them the loads of one part overlap the arithmetic of another: 98 -> 89 and 192 -> 169 us of the first, 77 -> 67 and 185 -> 147 of the second.
-template <int kRun, int kWidth, bool kFull, bool kAll> struct Cols {
-  static constexpr bool all = kAll;
+// kBare: a residual and the next norm alone, which is a plain block's end (16384 x 2048 bf16, RMS norm: 49 -> 44 and 107 -> 83 us; rows of 2047,
+// layer norm: 85 -> 76 and 154 -> 119).  kSome: whatever the pointers say.
+enum { kSome, kAll, kBare };
+template <int kRun, int kWidth, bool kFull, int kParts> struct Cols {
+  static constexpr bool all = kParts == kAll, bare = kParts == kBare;
   static constexpr int V = kRun, width = kWidth, side = side_of(kWidth), threads = width * side;
   int lane, D;      // thread among the token's; values of a token
   __device__ __forceinline__ int at(int j, int e) const { return ((j * (8 / V) + e / V) * width + lane) * V + e % V; }      // column of value e of vector j
@@ -188,7 +191,7 @@ template <class C> __device__ __forceinline__ float2 row_sum(float2 v, float2 (*
 //            neighbours of the row as well), and each value is picked out at the row's offset; needs a barrier in front of `get`
 //   kDirect  from global memory
 enum { kDirect, kOwn, kWindow };
-template <class T, class C, int kMode> struct Feed {
+template <class T, class C, int kMode, bool kThere> struct Feed {
   static constexpr int V = C::V;
   static constexpr int kRun = V * static_cast<int>(sizeof(T));      // kOwn: 8 or 16 bytes
   static_assert(kMode != kOwn || kRun == 8 || kRun == 16, "a run is one copy");
@@ -201,12 +204,12 @@ template <class T, class C, int kMode> struct Feed {
     return kMode == kOwn ? 8 * static_cast<int>(sizeof(T)) * C::threads : kMode == kWindow ? C::side * window(D) : 0;
   }
   __device__ __forceinline__ Feed(const void* p, int64_t stride, uint32_t& smem, int D) : base(static_cast<const T*>(p)), stride(stride), slot(smem) {
-    if (C::all || base) smem += 2 * bytes(D);
+    if (kThere || base) smem += 2 * bytes(D);
   }
   __device__ __forceinline__ static uint32_t place(int sub, int D) { return kMode == kOwn ? threadIdx.x * kRun : sub * window(D); }
   // row m into a stage
   __device__ __forceinline__ void ahead(long m, uint32_t to, const C& c, int sub) const {
-    if (!C::all && !base) return;
+    if (!kThere && !base) return;
     to += slot + place(sub, c.D);
     if constexpr (kMode == kOwn) {      // (one vector to a thread)
 #pragma unroll
@@ -224,7 +227,7 @@ template <class T, class C, int kMode> struct Feed {
   }
   // vector j of row m, of which this thread has some
   __device__ __forceinline__ void get(long m, uint32_t from, const C& c, int j, int sub, F (&f)[N]) const {
-    if (!C::all && !base) {
+    if (!kThere && !base) {
       fill(f, 0.f);
     } else if constexpr (kMode == kOwn) {
 #pragma unroll
@@ -372,7 +375,10 @@ inline bool vectors(const ttt_b200_block_args& p, bool backward, int run) {
   return ok && rows(p.x, 0, rs) && rows(p.n, 0, es);
 }
 
-inline bool all_parts(const ttt_b200_block_args& p) { return p.residual && p.gate && p.post_weight && p.scale && p.pre_weight; }
+inline int parts_of(const ttt_b200_block_args& p) {
+  if (p.residual && p.gate && p.post_weight && p.scale && p.pre_weight) return kAll;
+  return p.residual && p.pre_weight && !p.gate && !p.post_weight && !p.scale ? kBare : kSome;
+}
 
 inline int launched(const char* what) {
   const cudaError_t e = cudaGetLastError();

@@ -1,7 +1,7 @@
 // The end of a block and the start of the next: backward.
 //
 // Measured with all parts, 16384 x 2048 bf16: fp32 residual stream, layer norms, tanh gate 168 us (4.4 TB/s); bf16 residual, RMS norms
-// 147 us (3.6 TB/s); rows of 2047 210 us (2.6); 4096 x 8192, layer norms, sums in shared memory, 335 us (1.6).  512 threads to an SM,
+// 147 us (3.6 TB/s), a residual and the next norm alone 83 us (4.9 TB/s); rows of 2047 210 us (2.6); 4096 x 8192, layer norms, sums in shared memory, 335 us (1.6).  512 threads to an SM,
 // since a thread has 128 registers, 40 of them sums over tokens; each wait (two barriers a token, the L1 for the weights) shows.
 #include "ttt_block_norm.cuh"
 
@@ -45,12 +45,14 @@ __global__ void __launch_bounds__(C::threads, 512 / C::threads) block_backward_k
   const int lane = threadIdx.x % C::width, sub = threadIdx.x / C::width;
   const C c = {lane, p.D};
   const long step = static_cast<long>(q.ctas) * C::side;
-  const bool post = C::all || p.post_weight, gated = C::all || p.gate, pre = C::all || p.pre_weight;
-  const Feed<T, C, kMode> fo(p.o, p.o_stride, at, p.D), fg(p.gate, p.gate_stride, at, p.D);
-  const Feed<T, C, kMode> fn(pre ? p.grad_n : nullptr, p.gn_stride, at, p.D);
-  const Feed<R, C, kMode> fx(pre ? p.residual : nullptr, p.residual_stride, at, p.D);
-  const Feed<R, C, kMode> fd(p.grad_x, p.gx_stride, at, p.D);
-  const uint32_t small = Feed<T, C, kMode>::bytes(p.D), large = Feed<R, C, kMode>::bytes(p.D);
+  constexpr bool kMore = C::all || C::bare;
+  const bool post = !C::bare && (C::all || p.post_weight), gated = !C::bare && (C::all || p.gate), pre = kMore || p.pre_weight;
+  const Feed<T, C, kMode, true> fo(p.o, p.o_stride, at, p.D);
+  const Feed<T, C, kMode, C::all> fg(gated ? p.gate : nullptr, p.gate_stride, at, p.D);
+  const Feed<T, C, kMode, kMore> fn(pre ? p.grad_n : nullptr, p.gn_stride, at, p.D);
+  const Feed<R, C, kMode, kMore> fx(pre ? p.residual : nullptr, p.residual_stride, at, p.D);
+  const Feed<R, C, kMode, kMore> fd(p.grad_x, p.gx_stride, at, p.D);
+  const uint32_t small = Feed<T, C, kMode, true>::bytes(p.D), large = Feed<R, C, kMode, true>::bytes(p.D);
   const uint32_t stats = static_cast<uint32_t>(__cvta_generic_to_shared(&sh.stats[0][threadIdx.x >> 5]));
   auto ahead = [&](long m, int stage) {
     if (m < p.M) {
@@ -114,12 +116,12 @@ __global__ void __launch_bounds__(C::threads, 512 / C::threads) block_backward_k
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = times(u[i], w[i]);
       }
-      weights<C::all>(p.scale, c, j, 1.f, w);
+      weights<C::all>(C::bare ? nullptr : p.scale, c, j, 1.f, w);
       fx.get(m, stage * large, c, j, sub, z[j]);
 #pragma unroll
       for (int i = 0; i < N; ++i) z[j][i] = times(plus(mac(w[i], u[i], z[j][i]), both(-st.z)), both(st.w));
       fn.get(m, stage * small, c, j, sub, gn[j]);
-      weights<C::all>(p.pre_weight, c, j, 0.f, w);
+      weights<kMore>(p.pre_weight, c, j, 0.f, w);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         sums.add(kDw2, j, i, c, gn[j][i], z[j][i]);
@@ -145,7 +147,7 @@ __global__ void __launch_bounds__(C::threads, 512 / C::threads) block_backward_k
 #pragma unroll
         for (int i = 0; i < N; ++i) d2[j][i] = mac(both(st.w), mac(z[j][i], both(-m2), plus(gn[j][i], both(-m1))), d2[j][i]);
       }
-      if (C::all || p.grad_residual) store(static_cast<R*>(p.grad_residual) + m * p.D, c, j, d2[j]);
+      if (kMore || p.grad_residual) store(static_cast<R*>(p.grad_residual) + m * p.D, c, j, d2[j]);
       F u[N], w[N], b[N], v[N], g[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) u[i] = o[j][i];
@@ -155,7 +157,7 @@ __global__ void __launch_bounds__(C::threads, 512 / C::threads) block_backward_k
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = mac(o[j][i], w[i], b[i]);
       }
-      weights<C::all>(p.scale, c, j, 1.f, b);
+      weights<C::all>(C::bare ? nullptr : p.scale, c, j, 1.f, b);
       if (gated) {
         fg.get(m, stage * small, c, j, sub, g);
         gate<true>(p.activation, g, v, g);
@@ -170,7 +172,7 @@ __global__ void __launch_bounds__(C::threads, 512 / C::threads) block_backward_k
       } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          sums.add(kDsc, j, i, c, d2[j][i], u[i]);
+          if (!C::bare) sums.add(kDsc, j, i, c, d2[j][i], u[i]);
           d2[j][i] = times(d2[j][i], b[i]);
         }
       }
@@ -217,17 +219,21 @@ __global__ void __launch_bounds__(C::threads, 512 / C::threads) block_backward_k
 template <class T, class R, class C, int NV, bool kShared> int backward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
   constexpr int kMode = kShared ? kDirect : C::V > 1 ? kOwn : kWindow;
   const size_t bytes = kShared ? static_cast<size_t>(kSums) * p.D * sizeof(float)
-                               : 2 * (Feed<T, C, kMode>::bytes(p.D) * (1 + (p.gate != nullptr) + (p.pre_weight && p.grad_n)) +
-                                      Feed<R, C, kMode>::bytes(p.D) * ((p.pre_weight && p.residual) + (p.grad_x != nullptr)));
+                               : 2 * (Feed<T, C, kMode, true>::bytes(p.D) * (1 + (p.gate != nullptr) + (p.pre_weight && p.grad_n)) +
+                                      Feed<R, C, kMode, true>::bytes(p.D) * ((p.pre_weight && p.residual) + (p.grad_x != nullptr)));
   return launch(block_backward_kernel<T, R, C, NV, kShared>, q, bytes, s, p, "block norm backward");
 }
-template <class T, class R, int kWidth, int NV, bool kAll> int backward_with(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
-  if (!vectors(p, true, kRun<R>)) return backward_as<T, R, Cols<1, kWidth, false, kAll>, NV, (NV > 1)>(p, q, s);
-  return p.D == 8 * NV * kWidth ? backward_as<T, R, Cols<kRun<R>, kWidth, true, kAll>, NV, (NV > 1)>(p, q, s)
-                                : backward_as<T, R, Cols<kRun<R>, kWidth, false, kAll>, NV, (NV > 1)>(p, q, s);
+template <class T, class R, int kWidth, int NV, int kParts> int backward_with(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
+  if (!vectors(p, true, kRun<R>)) return backward_as<T, R, Cols<1, kWidth, false, kParts>, NV, (NV > 1)>(p, q, s);
+  return p.D == 8 * NV * kWidth ? backward_as<T, R, Cols<kRun<R>, kWidth, true, kParts>, NV, (NV > 1)>(p, q, s)
+                                : backward_as<T, R, Cols<kRun<R>, kWidth, false, kParts>, NV, (NV > 1)>(p, q, s);
 }
 template <class T, class R, int kWidth, int NV = 1> int backward_of(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
-  return all_parts(p) && p.grad_x && p.grad_n ? backward_with<T, R, kWidth, NV, true>(p, q, s) : backward_with<T, R, kWidth, NV, false>(p, q, s);
+  switch (p.grad_x && p.grad_n ? parts_of(p) : kSome) {
+    case kAll: return backward_with<T, R, kWidth, NV, kAll>(p, q, s);
+    case kBare: return backward_with<T, R, kWidth, NV, kBare>(p, q, s);
+    default: return backward_with<T, R, kWidth, NV, kSome>(p, q, s);
+  }
 }
 template <class T, class R> int backward_kernel(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
   if (p.D > kWide) return backward_of<T, R, 512, 2>(p, q, s);
