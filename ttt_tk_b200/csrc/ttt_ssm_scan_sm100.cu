@@ -748,8 +748,9 @@ __global__ void __launch_bounds__(TH, LN <= 4 ? 4 : 3) scan_backward_kernel(cons
           o[e] = qa.x + qa.y;
           o[2 + e] = gb.x + gb.y;
         }
-        // dx and d delta: over the channel's lanes
+        // dx and d delta: over the channel's lanes, which have all read the token's delta x and dy when one of them overwrites these
         spread_sum<4, LN, 1>(o, lane);
+        __syncwarp();
         if constexpr (LN <= 4) {
 #pragma unroll
           for (int r = 0; r < 4 / LN; ++r) {
