@@ -1,0 +1,33 @@
+"""What the differentiable forms of the layer-side sequence operators refuse and ask of the operators, without a GPU: shapes and types are
+checked before devices, and what is asked is read from the call that arrives."""
+import pytest
+import torch
+
+from ttt_tk_b200 import autograd as ag
+
+BF = torch.bfloat16
+
+
+# ---- block end -----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("name", ["residual", "gate"])
+@pytest.mark.parametrize("shape", [(3, 2, 8), (6, 8), (1, 6, 8), (2, 3, 4), (8,), (1, 1, 8)])
+def test_block_end_takes_no_other_shape_of_as_many_tokens(name, shape):
+    """Tokens in flat order are not the tokens of another shape."""
+    o = torch.zeros(2, 3, 8, dtype=BF)
+    with pytest.raises(ValueError, match=f"{name} must have the shape of o"):
+        ag.norm_gate_residual(o, **{name: torch.zeros(shape, dtype=BF)})
+
+
+def test_block_end_of_equal_shapes_reaches_the_device_check():
+    o = torch.zeros(2, 3, 8, dtype=BF)
+    with pytest.raises(ValueError, match="CUDA"):
+        ag.norm_gate_residual(o, o, o, pre_weight=torch.ones(8))
+    with pytest.raises(ValueError, match="CUDA"):      # a size of one in front, rows that do not follow one another
+        ag.norm_gate_residual(torch.zeros(2, 4, 6, 8, dtype=BF)[:, :3])
+
+
+@pytest.mark.parametrize("o,msg", [(torch.zeros((), dtype=BF), "o must be"), (torch.zeros(3, 0, dtype=BF), "1 to 8192"),
+                                   (torch.zeros(0, 8193, dtype=BF), "1 to 8192")])
+def test_block_end_without_values_to_a_token(o, msg):
+    with pytest.raises(ValueError, match=msg):
+        ag.norm_gate_residual(o)
