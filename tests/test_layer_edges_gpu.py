@@ -1,0 +1,48 @@
+"""The layer-side sequence operators at the ends of their ranges and where calls meet.
+Statements: oracle/layer.py; tolerances: tests/layer_cases.py."""
+import pytest
+import torch
+
+from layer_cases import TYPES, close, gen
+from oracle import layer as ol
+from ttt_tk_b200 import glue
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+# ---- block end: gates of any size -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("ty", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+@pytest.mark.parametrize("parts", ["all", "gate"])
+def test_gradients_at_gates_of_any_size(ty, act, parts):
+    """A closed gate (the type's lowest value, as a mask leaves it) passes no gradient, an open one passes it whole.  The sizes lie away
+    from -87, where 1 / (1 + exp(-v)) leaves fp32: what is below is 0."""
+    t, M, D = TYPES[ty], 6, 64
+    top = torch.finfo(t).max
+    g = gen(4)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    sizes = [-top, -min(top, 1e30), -min(top, 1e25), -min(top, 1e19), -min(top, 1e13), -1e3, -100.0, 0.0, 100.0, 1e3]
+    if parts == "gate":      # (a gate that is open that wide leaves no room for the rest of a row's arithmetic)
+        sizes += [min(top, 1e13), min(top, 1e19), min(top, 1e25), min(top, 1e30), top]
+    gate = torch.tensor(sizes).repeat(M * D // len(sizes) + 1)[:M * D].view(M, D).to(t)
+    small = 2.0 ** -6 if parts == "gate" else 1.0      # products with the widest gate have to be numbers of the type
+    o, res, gx = (r(M, D).clamp(-4, 4) * s for s in (small, 1.0, small))
+    o, res, gx = o.to(t), res.to(t), gx.to(t)
+    w = {} if parts == "gate" else dict(post_weight=1 + 0.1 * r(D), scale=0.3 + 0.1 * r(D), pre_weight=1 + 0.1 * r(D))
+    gn = None if parts == "gate" else r(M, D).to(t)
+    dev = lambda v: None if v is None else v.to(DEV)  # noqa: E731
+    o, res, gate, gx, gn = (dev(v) for v in (o, res, gate, gx, gn))
+    kw = dict(activation=act, **{k: dev(v) for k, v in w.items()})
+    x, n, stats = glue.norm_gate_residual(o, res, gate, return_stats=True, **kw)
+    assert torch.isfinite(x).all() and (n is None or torch.isfinite(n).all())
+    got = glue.norm_gate_residual_backward(gx, gn, o, stats, res, gate, **kw)
+    okw = {("activation_" if k == "activation" else k): v for k, v in kw.items()}
+    want = ol.norm_gate_residual_backward(gx, gn, o, res, gate, **okw)
+    amps = ol.norm_gate_residual_backward(gx, gn, o, res, gate, amp=True, **okw)
+    for k, a, b, m in zip(("o", "residual", "gate", "post_weight", "post_bias", "scale", "pre_weight"), got, want, amps):
+        assert (a is None) == (b is None), k
+        if a is not None:
+            assert torch.isfinite(a).all(), k
+            # (the statistics' sums have up to 28 roundings in a row at this width, and M tokens follow one another in a weight's)
+            close(a, b, m, 4 * (2 * 28 + 120) + M, "grad " + k)

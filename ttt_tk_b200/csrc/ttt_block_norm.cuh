@@ -125,15 +125,16 @@ template <bool kThere = false, class C> __device__ __forceinline__ void weights(
 }
 
 // The gate: its value, and with kSlope its derivative.  GELU as x sigmoid(2 u): no 1 + tanh(u), which cancels on the left.  The
-// derivative needs 1 - sigmoid without its cancellation on the right, which is e times sigmoid; the exponent is bounded there so
-// that this is not infinity times 0.
+// derivative needs 1 - sigmoid without its cancellation on the right, which is e times sigmoid.  Far on the left e is bounded, so that
+// this is not infinity times 0: at 2^127 the reciprocal is below the least normal number and so 0, and with it all that it enters
+// (at 2^126 it is 2^-126, which x = -1e38 takes to -1).  GELU's x^2 is bounded where it meets a factor of 0, beyond |x| = 1e15.
 template <int kKind, bool kSlope> __device__ __forceinline__ void gate_one(F x, F& v, F& s) {
   constexpr float k = 1.5957691216057308f, c = 0.044715f;      // 2 sqrt(2 / pi)
   F e;
   const F q = times(x, x);
   if constexpr (kKind == TTT_B200_ACT_GELU) e = times(times(x, all<F>(-k * kLog2e)), mac(q, all<F>(c), all<F>(1.f)));
   else e = times(x, all<F>(-kLog2e));
-  if constexpr (kSlope) e = least(e, 126.f);
+  if constexpr (kSlope) e = least(e, 127.f);
   e = ex2(e);
   const F g = rcp(plus(e, all<F>(1.f)));
   if constexpr (kKind == TTT_B200_ACT_SIGMOID) {
@@ -143,7 +144,7 @@ template <int kKind, bool kSlope> __device__ __forceinline__ void gate_one(F x, 
     v = times(x, g);
     if constexpr (kSlope) {
       F o = times(e, g);
-      if constexpr (kKind == TTT_B200_ACT_GELU) o = times(o, mac(q, all<F>(3.f * c * k), all<F>(k)));
+      if constexpr (kKind == TTT_B200_ACT_GELU) o = times(o, mac(least(q, 1e30f), all<F>(3.f * c * k), all<F>(k)));
       s = mac(v, o, g);
     }
   }
