@@ -3,9 +3,9 @@ Statements: oracle/layer.py; tolerances: tests/layer_cases.py."""
 import pytest
 import torch
 
-from layer_cases import TYPES, close, gen
+from layer_cases import TYPES, close, conv_inputs, gen
 from oracle import layer as ol
-from ttt_tk_b200 import glue
+from ttt_tk_b200 import glue, ssm
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -46,3 +46,22 @@ def test_gradients_at_gates_of_any_size(ty, act, parts):
             assert torch.isfinite(a).all(), k
             # (the statistics' sums have up to 28 roundings in a row at this width, and M tokens follow one another in a weight's)
             close(a, b, m, 4 * (2 * 28 + 120) + M, "grad " + k)
+
+
+# ---- convolution: what lies behind a sequence is zero ---------------------------------------------------------------------
+@pytest.mark.parametrize("act", [None, "silu"])
+@pytest.mark.parametrize("ty,D,K,T,n", [("bf16", 64, 4, 40, 21), ("fp32", 13, 3, 19, 8), ("fp32", 64, 2, 64, 63), ("fp16", 72, 4, 300, 130)])
+def test_gradients_behind_a_sequence_that_ends_with_infinities(act, ty, D, K, T, n):
+    i = conv_inputs(7, ty, 1, T, D, K, DEV)
+    i["x"][0, n - 1, ::2] = float("inf")
+    i["x"][0, n - 2, 1::4] = float("nan")
+    lengths = torch.tensor([n], dtype=torch.int32, device=DEV)
+    got = ssm.short_conv_backward(i["gy"], i["x"], i["weight"], i["bias"], activation=act, state=i["state"], lengths=lengths,
+                                  grad_final_state=i["gf"])
+    want = ol.short_conv_backward(i["gy"], i["x"], i["weight"], i["bias"], act, i["state"], [n], i["gf"])
+    assert (got[0][0, n:] == 0).all()
+    for k, a, b in zip(("x", "weight", "bias", "state"), got, want):
+        fine = torch.isfinite(b)
+        assert torch.isfinite(a.cpu())[fine].all(), k      # a number wherever the formula has one
+    if act is None:      # nothing but the weights' gradients sees x
+        assert torch.isfinite(got[0]).all() and torch.isfinite(got[2]).all() and torch.isfinite(got[3]).all()

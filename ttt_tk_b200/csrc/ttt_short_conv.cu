@@ -279,7 +279,8 @@ template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(3
       g[k] = x[k] = all<F>(0.f);
       if (k < K - 1 && t < len) x[k] = wide<T, V>(input<T, K, V>(p, b, d, t));
     }
-    auto one = [&](const Raw<T, V>& row, const Raw<T, V>& up, bool own) {
+    // `in`: a token of the sequence; behind it g is zero, and the last inputs, whatever they are, are in no product with it
+    auto one = [&](const Raw<T, V>& row, const Raw<T, V>& up, bool own, bool in) {
       x[K - 1] = wide<T, V>(row);
       F v = wide<T, V>(up);
       if constexpr (kSilu) {
@@ -291,11 +292,12 @@ template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(3
       }
 #pragma unroll
       for (int k = K - 1; k > 0; --k) g[k] = g[k - 1];
+      if (!in) v = all<F>(0.f);
       g[0] = v;
       F o = times(w[0], g[0]);
 #pragma unroll
       for (int k = 1; k < K; ++k) o = mac(w[k], g[k], o);
-      if (own) {
+      if (own && in) {
         db = plus(db, v);
 #pragma unroll
         for (int k = 0; k < K; ++k) dw[k] = mac(v, x[k], dw[k]);
@@ -317,7 +319,7 @@ template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(3
         T* to = gx + static_cast<long>(t0 - K + 1) * p.D;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const Raw<T, V> o = narrow<T, V>(one(rows.at(u), ups.at(u), true));
+          const Raw<T, V> o = narrow<T, V>(one(rows.at(u), ups.at(u), true, true));
           if (mine && (u >= K - 1 || t0 > begin)) store<T, V>(to, o);
           else if (mine && begin == 0 && gs) store<T, V>(gs + static_cast<long>(u) * p.D, o);      // (t0 = 0, and len is beyond)
           to += p.D;
@@ -327,7 +329,7 @@ template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(3
         for (int u = 0; u < U; ++u)
           if (t0 + u < end) {
             const bool in = t0 + u < live;
-            place(t0 + u - K + 1, one(in ? rows.at(u) : nothing<T, V>(), in ? ups.at(u) : nothing<T, V>(), true));
+            place(t0 + u - K + 1, one(in ? rows.at(u) : nothing<T, V>(), in ? ups.at(u) : nothing<T, V>(), true, in));
           }
       }
     }
@@ -339,7 +341,7 @@ template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(3
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
       const bool in = end + k < live;
-      place(end + k - K + 1, one(in ? rows.at(k) : nothing<T, V>(), in ? ups.at(k) : nothing<T, V>(), false));
+      place(end + k - K + 1, one(in ? rows.at(k) : nothing<T, V>(), in ? ups.at(k) : nothing<T, V>(), false, in));
     }
   }
 #pragma unroll
