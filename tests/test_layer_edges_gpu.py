@@ -3,7 +3,7 @@ Statements: oracle/layer.py; tolerances: tests/layer_cases.py."""
 import pytest
 import torch
 
-from layer_cases import TYPES, close, conv_inputs, gen
+from layer_cases import TYPES, close, conv_inputs, gen, scan_inputs
 from oracle import layer as ol
 from ttt_tk_b200 import glue, ssm
 
@@ -65,3 +65,49 @@ def test_gradients_behind_a_sequence_that_ends_with_infinities(act, ty, D, K, T,
         assert torch.isfinite(a.cpu())[fine].all(), k      # a number wherever the formula has one
     if act is None:      # nothing but the weights' gradients sees x
         assert torch.isfinite(got[0]).all() and torch.isfinite(got[2]).all() and torch.isfinite(got[3]).all()
+
+
+# ---- scan: states that grow ----------------------------------------------------------------------------
+def test_chunks_over_which_a_state_grows_beyond_fp32():
+    """Factors of exp(8) a token: over a chunk of 16 more than fp32 holds, while the states themselves are zero or small there."""
+    B, T, D, N = 1, 600, 64, 16      # (one CTA's worth of channels: every tile of 16 tokens is a chunk)
+    i = scan_inputs(9, "fp32", B, T, D, N, 1, DEV, state=False)
+    i["A"] = torch.full((D, N), 2.0, device=DEV)
+    i["dt"] = torch.full((B, T, D), 4.0, device=DEV)
+    i["x"][:, :T - 3] = 0
+    i["gy"][:, 3:] = 0
+    a = [i[k] for k in ("x", "dt", "A", "B", "C")]
+    y, end, ck = ssm.ssm_scan(*a, softplus=False, return_state=True, return_checkpoints=True)
+    ref, rend, _ = ol.ssm_scan(*a, softplus_=False)
+    amp, aend, _ = ol.ssm_scan(*a, softplus_=False, amp=True)
+    close(y, ref, amp, 16 * 8 + N + 40, "y")      # (nothing is there before the last three tokens)
+    close(end, rend, aend, 16 * 8, "state")
+    got = ssm.ssm_scan_backward(i["gy"], *a, ck, softplus=False)
+    want = ol.ssm_scan_backward(i["gy"], *a, softplus_=False)
+    amps = ol.ssm_scan_backward(i["gy"], *a, softplus_=False, amp=True)
+    for k, g, r, m in zip(("x", "dt", "A", "B", "C", "", "", "state"), got, want, amps):
+        if k:
+            close(g, r, m, 32 * 8 + 2 * N + 80 + D, "grad " + k)
+
+
+def test_a_small_state_that_grows_over_a_chunk():
+    B, T, D, N = 1, 18, 64, 16      # two chunks
+    i = scan_inputs(10, "fp32", B, T, D, N, 1, DEV)
+    i["A"] = torch.full((D, N), 2.0, device=DEV)
+    i["dt"] = torch.full((B, T, D), 4.0, device=DEV)
+    i["x"][:] = 0
+    i["state"] = i["state"] * 1e-30
+    i["gy"][:] = 0
+    i["gf"] = i["gf"] * 1e-30
+    a = [i[k] for k in ("x", "dt", "A", "B", "C")]
+    y, end, ck = ssm.ssm_scan(*a, softplus=False, state=i["state"], return_state=True, return_checkpoints=True)
+    ref, rend, _ = ol.ssm_scan(*a, softplus_=False, state=i["state"])
+    amp, aend, _ = ol.ssm_scan(*a, softplus_=False, state=i["state"], amp=True)
+    # a factor's exponent of 8 log2(e) = 11.5 is rounded twice: 12 + 12 roundings of the factor, and 16 as elsewhere
+    close(y, ref, amp, 40 * T + N + 40, "y")
+    close(end, rend, aend, 40 * T, "state")
+    got = ssm.ssm_scan_backward(i["gy"], *a, ck, softplus=False, grad_final_state=i["gf"])
+    want = ol.ssm_scan_backward(i["gy"], *a, softplus_=False, state=i["state"], grad_final_state=i["gf"])
+    amps = ol.ssm_scan_backward(i["gy"], *a, softplus_=False, state=i["state"], grad_final_state=i["gf"], amp=True)
+    for j, k in ((0, "x"), (1, "dt"), (2, "A"), (7, "state")):
+        close(got[j], want[j], amps[j], 80 * T + 2 * N + 80, "grad " + k)

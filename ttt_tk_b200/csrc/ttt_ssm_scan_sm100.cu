@@ -531,6 +531,15 @@ template <class T, int LN, bool kRev> __global__ void __launch_bounds__(TH, 4) s
     if (me.li == 0 && me.ch[e] < w.cols) q.delta[w.bc * p.D + w.ch0 + me.ch[e]] = e ? total.y : total.x;
 }
 
+// 2^x h for x > kStep, h a state that a chunk's decay carries on.  A state that grows (A delta > 0) may do so by more than fp32 holds over a
+// chunk and still be a number, if it is zero or small, so the exponent is taken in steps: three take the least number beyond the greatest.
+constexpr float kStep = 126.f;
+__device__ __forceinline__ float grown(float x, float h) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i, x -= kStep) h *= ex2(fminf(fmaxf(x, 0.f), kStep));
+  return h;
+}
+
 // The chunks' own states -> the states that they start from (kRev: that they end with), in place, in the order of time.
 template <bool kRev> __global__ void __launch_bounds__(256) scan_join_kernel(const ttt_b200_scan_args p, const Plan q) {
   wait_for_predecessor();
@@ -543,7 +552,7 @@ template <bool kRev> __global__ void __launch_bounds__(256) scan_join_kernel(con
   float h = from ? from[i] : 0.f;
   constexpr int kAhead = 8;      // chunks requested ahead of those that are worked on
   auto chunk = [&](int c) { return b * q.chunks + (kRev ? q.chunks - 1 - c : c); };
-  float s[kAhead], f[kAhead], s2[kAhead], f2[kAhead];
+  float s[kAhead], f[kAhead], e[kAhead], s2[kAhead], f2[kAhead];
   auto request = [&](int c0) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
@@ -554,17 +563,20 @@ template <bool kRev> __global__ void __launch_bounds__(256) scan_join_kernel(con
   };
   request(0);
   for (int c0 = 0; c0 < q.chunks; c0 += kAhead) {
+    bool grows = false;
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       s[k] = s2[k];
-      f[k] = ex2(fmaf(a2, f2[k], kCentre));
+      e[k] = fmaf(a2, f2[k], kCentre);
+      f[k] = ex2(e[k]);
+      grows = grows || e[k] > kStep;
     }
     request(c0 + kAhead);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
       if (c0 + k < q.chunks) {
         q.state[chunk(c0 + k) * DN + dn] = h;
-        h = fmaf(f[k], h, s[k]);
+        h = grows && e[k] > kStep ? grown(e[k], h) + s[k] : fmaf(f[k], h, s[k]);
       }
   }
 }
