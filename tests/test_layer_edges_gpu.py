@@ -111,3 +111,28 @@ def test_a_small_state_that_grows_over_a_chunk():
     amps = ol.ssm_scan_backward(i["gy"], *a, softplus_=False, state=i["state"], grad_final_state=i["gf"], amp=True)
     for j, k in ((0, "x"), (1, "dt"), (2, "A"), (7, "state")):
         close(got[j], want[j], amps[j], 80 * T + 2 * N + 80, "grad " + k)
+
+
+# ---- decays: of the lowest value
+@pytest.mark.parametrize("T", [13, 600])
+def test_decays_of_the_lowest_value(T):
+    """A = the lowest fp32 forgets a state wherever delta is not zero, and keeps it where it is: steps of zero and tokens behind a sequence."""
+    B, D, N = 2, 64, 16
+    low = torch.finfo(torch.float32).min
+    i = scan_inputs(11, "fp32", B, T, D, N, 1, DEV)
+    i["A"][:, ::3] = low
+    n = [T - 4, 0]
+    i["dt"] = i["dt"].abs() * 0.1 + 0.01
+    i["dt"][:, T // 3:T // 2] = 0
+    lengths = torch.tensor(n, dtype=torch.int32, device=DEV)
+    a = [i[k] for k in ("x", "dt", "A", "B", "C")]
+    y, end = ssm.ssm_scan(*a, i["D"], softplus=False, state=i["state"], lengths=lengths, return_state=True)
+    ref, rend, _ = ol.ssm_scan(*a, i["D"], softplus_=False, state=i["state"], lengths=n)
+    amp, aend, _ = ol.ssm_scan(*a, i["D"], softplus_=False, state=i["state"], lengths=n, amp=True)
+    close(y, ref, amp, 16 * T + N + 40, "y")
+    close(end, rend, aend, 16 * T + N + 40, "state")
+    st = i["state"].clone()
+    one = [t[:, 0] if t.dim() > 2 else t for t in a]
+    one[1] = torch.zeros_like(one[1])
+    ssm.ssm_scan_step(*one, st, softplus=False)
+    assert torch.equal(st, i["state"])

@@ -181,6 +181,11 @@ template <class T, int W> struct Wide {
 // (arguments of -0.5 to -0.001), which a state of a thousand tokens adds up; the offset takes the average to a quarter of
 // that and leaves exp(0) = 1, which tokens behind a sequence rely on.
 constexpr float kCentre = 2.2e-8f;
+// A log2(e), a number for every A that is one: the lowest would be infinite, and a delta of zero times it no number.
+__device__ __forceinline__ float rate(float a) {
+  const float r = a * kLog2e;
+  return isinf(r) ? copysignf(3.402823466e38f, r) : r;
+}
 __device__ __forceinline__ float2 decay(float delta, float2 a2) {
   const float2 x = fma2(both(delta), a2, both(kCentre));
   return make_float2(ex2(x.x), ex2(x.y));
@@ -226,14 +231,18 @@ template <int LN> struct Mine {
     }
   }
   // of a row [D][N]; a channel behind the last reads nothing
-  __device__ __forceinline__ void read(const float* p, const Where& w, int N, bool vec, float2 (&h)[2][2], float scale = 1.f) const {
+  template <bool kRate = false> __device__ __forceinline__ void read(const float* p, const Where& w, int N, bool vec, float2 (&h)[2][2]) const {
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       if (ch[e] < w.cols) {
         float v[4];
         load_states(p + row[e], n0, N, vec, v);
-        h[e][0] = make_float2(v[0] * scale, v[1] * scale);
-        h[e][1] = make_float2(v[2] * scale, v[3] * scale);
+        if constexpr (kRate) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = rate(v[k]);
+        }
+        h[e][0] = make_float2(v[0], v[1]);
+        h[e][1] = make_float2(v[2], v[3]);
       }
   }
   __device__ __forceinline__ void write(float* p, const Where& w, int N, bool vec, const float2 (&h)[2][2]) const {
@@ -357,7 +366,7 @@ template <class T, int LN> __global__ void __launch_bounds__(TH, 4) scan_forward
 
   fetch(0);
   float2 a2[2][2] = {}, h[2][2] = {};
-  me.read(p.A, w, p.N, q.vec_n, a2, kLog2e);
+  me.template read<true>(p.A, w, p.N, q.vec_n, a2);
   if (q.chunks > 1) me.read(q.state + w.bc * DN, w, p.N, q.vec_n, h);
   else if (p.state) me.read(p.state + w.b * DN, w, p.N, q.vec_n, h);
   Next next;
@@ -488,7 +497,7 @@ template <class T, int LN, bool kRev> __global__ void __launch_bounds__(TH, 4) s
 
   fetch(0);
   float2 a2[2][2] = {}, h[2][2] = {};
-  me.read(p.A, w, p.N, q.vec_n, a2, kLog2e);
+  me.template read<true>(p.A, w, p.N, q.vec_n, a2);
   float2 total = both(0.f);
   Next next;
   cp_async_wait<0>();
@@ -547,7 +556,7 @@ template <bool kRev> __global__ void __launch_bounds__(256) scan_join_kernel(con
   const long i = static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (i >= p.B * DN) return;
   const long b = i / DN, dn = i % DN, d = dn / p.N;
-  const float a2 = p.A[dn] * kLog2e;
+  const float a2 = rate(p.A[dn]);
   const float* from = kRev ? p.grad_final_state : p.state;
   float h = from ? from[i] : 0.f;
   constexpr int kAhead = 8;      // chunks requested ahead of those that are worked on
@@ -615,7 +624,7 @@ __global__ void __launch_bounds__(TH, LN <= 4 ? 4 : 3) scan_backward_kernel(cons
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long DN = static_cast<long>(p.D) * p.N;
   float2 a2[2][2] = {}, carry[2][2] = {}, da[2][2] = {};
-  me.read(p.A, w, p.N, q.vec_n, a2, kLog2e);
+  me.template read<true>(p.A, w, p.N, q.vec_n, a2);
   if (q.chunks > 1) me.read(q.state + w.bc * DN, w, p.N, q.vec_n, carry);
   else if (p.grad_final_state) me.read(p.grad_final_state + w.b * DN, w, p.N, q.vec_n, carry);
   float2 sum_d = both(0.f), sum_bias = both(0.f);
@@ -918,7 +927,7 @@ template <class T, int LN, bool kOne> __global__ void __launch_bounds__(TH, 8) s
       y[e] = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        h[e][k] = fmaf(ex2(fmaf(dl, a[e][k] * kLog2e, kCentre)), h[e][k], dx * t.b[kOne ? 0 : e][k]);
+        h[e][k] = fmaf(ex2(fmaf(dl, rate(a[e][k]), kCentre)), h[e][k], dx * t.b[kOne ? 0 : e][k]);
         y[e] = fmaf(h[e][k], t.c[kOne ? 0 : e][k], y[e]);
       }
     }
