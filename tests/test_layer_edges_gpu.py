@@ -1,11 +1,15 @@
 """The layer-side sequence operators at the ends of their ranges and where calls meet.
 Statements: oracle/layer.py; tolerances: tests/layer_cases.py."""
+import ctypes
+import struct
+import threading
+
 import pytest
 import torch
 
 from layer_cases import TYPES, close, conv_inputs, gen, scan_inputs
 from oracle import layer as ol
-from ttt_tk_b200 import glue, ssm
+from ttt_tk_b200 import _lib, glue, ssm
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -136,3 +140,48 @@ def test_decays_of_the_lowest_value(T):
     one[1] = torch.zeros_like(one[1])
     ssm.ssm_scan_step(*one, st, softplus=False)
     assert torch.equal(st, i["state"])
+
+
+# ---- threads: two of the host -----------------------------------------------------------------------------------------------------
+def test_two_threads_with_different_amounts_of_shared_memory():
+    """The same kernel with 160 KB and 80 KB of shared memory, called through the C entry from two threads."""
+    lib = _lib.lib()
+    fn = lib.ttt_b200_norm_gate_residual_backward
+    fn.argtypes, fn.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int
+    lib.ttt_b200_norm_gate_residual_scratch_bytes.argtypes = [ctypes.c_void_p]
+    lib.ttt_b200_norm_gate_residual_scratch_bytes.restype = ctypes.c_uint64
+
+    def call(D):
+        M = 2
+        o, gx, go = (torch.ones(M, D, device=DEV) for _ in range(3))
+        w, gw = (torch.ones(D, device=DEV) for _ in range(2))
+        _, _, stats = glue.norm_gate_residual(o, post_weight=w, return_stats=True)
+        # o, residual, gate, weights x 5, x, n, stats, grad_x, grad_n, grad_o, grad_residual, grad_gate, sums x 5, scratch
+        p = [0] * 22
+        p[0], p[3], p[10], p[11], p[13], p[16] = (t.data_ptr() for t in (o, w, stats, gx, go, gw))
+        tail = (D, D, D, D, D, M, D, 2, 0, 0, 1, 1e-6)
+        size = lib.ttt_b200_norm_gate_residual_scratch_bytes(struct.pack("=22Q Q 6q 5i f", *p, 0, *tail))
+        scratch = torch.empty(size, dtype=torch.uint8, device=DEV)
+        p[21] = scratch.data_ptr()
+        stream = torch.cuda.Stream()
+        return struct.pack("=22Q Q 6q 5i f", *p, size, *tail), stream, (o, gx, go, w, gw, stats, scratch)
+
+    calls = [call(8188), call(4100)]      # (8192 fills its threads, which is another kernel)
+    torch.cuda.synchronize()
+    codes = [[], []]
+    start = threading.Barrier(2)
+
+    def work(k):
+        args, stream, _ = calls[k]
+        start.wait()
+        for _ in range(3000):
+            codes[k].append(fn(args, stream.cuda_stream))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert len(codes[0]) == len(codes[1]) == 3000
+    assert not any(codes[0]) and not any(codes[1]), [sum(map(bool, c)) for c in codes]

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(C::threads, 1024 / C::threads) block_forward_k
 template <class T, class R, class C> int forward_as(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
   constexpr int kMode = C::V > 1 ? kOwn : kWindow;
   const size_t bytes = 2 * (Feed<T, C, kMode, true>::bytes(p.D) * (1 + (p.gate != nullptr)) + Feed<R, C, kMode, true>::bytes(p.D) * (p.residual != nullptr));
-  return launch(block_forward_kernel<T, R, C>, q, bytes, s, p, "block norm");
+  return launch<block_forward_kernel<T, R, C>>(q, bytes, s, p, "block norm");
 }
 template <class T, class R, int kWidth, int kParts> int forward_with(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
   if (!vectors(p, false, kRun<R>)) return forward_as<T, R, Cols<1, kWidth, false, kParts>>(p, q, s);

@@ -16,6 +16,7 @@
 #pragma once
 
 #include <algorithm>
+#include <atomic>
 #include <cstdio>
 #include <type_traits>
 
@@ -389,12 +390,26 @@ inline int launched(const char* what) {
   return ttt_set_error(TTT_B200_ERR_LAUNCH, buf);
 }
 
-template <class K> int launch(K kernel, const Plan& q, size_t bytes, cudaStream_t s, const ttt_b200_block_args& p, const char* what) {
-  if (bytes > 40 * 1024) {      // (with the static part 48 KB is the most without asking)
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-    if (e != cudaSuccess) return ttt_set_error(TTT_B200_ERR_LAUNCH, cudaGetErrorString(e));
-  }
-  ttt_launch_overlapped(kernel, q.ctas, q.width * side_of(q.width), static_cast<uint32_t>(bytes), s, p, q);
+// More dynamic shared memory than 48 KB has to be asked for, per kernel and device.  All that there is is asked for, once: a limit of a
+// call's own would be lowered by a smaller call of another host thread between this call's asking and its launch.
+template <auto kKernel> int allow_shared() {
+  static std::atomic<uint64_t> done{0};      // a bit for each device
+  int dev = 0, most = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;      // (beyond 64 devices: every time the same)
+  if (e == cudaSuccess && (done.load(std::memory_order_acquire) & bit)) return TTT_B200_OK;
+  cudaFuncAttributes own = {};
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&own, kKernel);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - static_cast<int>(own.sharedSizeBytes));
+  if (e != cudaSuccess) return ttt_set_error(TTT_B200_ERR_LAUNCH, cudaGetErrorString(e));
+  done.fetch_or(bit, std::memory_order_release);
+  return TTT_B200_OK;
+}
+template <auto kKernel> int launch(const Plan& q, size_t bytes, cudaStream_t s, const ttt_b200_block_args& p, const char* what) {
+  if (bytes > 40 * 1024)      // (with the static part 48 KB is the most without asking)
+    if (int rc = allow_shared<kKernel>()) return rc;
+  ttt_launch_overlapped(kKernel, q.ctas, q.width * side_of(q.width), static_cast<uint32_t>(bytes), s, p, q);
   return launched(what);
 }
 

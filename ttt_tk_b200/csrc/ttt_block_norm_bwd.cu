@@ -221,7 +221,7 @@ template <class T, class R, class C, int NV, bool kShared> int backward_as(const
   const size_t bytes = kShared ? static_cast<size_t>(kSums) * p.D * sizeof(float)
                                : 2 * (Feed<T, C, kMode, true>::bytes(p.D) * (1 + (p.gate != nullptr) + (p.pre_weight && p.grad_n)) +
                                       Feed<R, C, kMode, true>::bytes(p.D) * ((p.pre_weight && p.residual) + (p.grad_x != nullptr)));
-  return launch(block_backward_kernel<T, R, C, NV, kShared>, q, bytes, s, p, "block norm backward");
+  return launch<block_backward_kernel<T, R, C, NV, kShared>>(q, bytes, s, p, "block norm backward");
 }
 template <class T, class R, int kWidth, int NV, int kParts> int backward_with(const ttt_b200_block_args& p, const Plan& q, cudaStream_t s) {
   if (!vectors(p, true, kRun<R>)) return backward_as<T, R, Cols<1, kWidth, false, kParts>, NV, (NV > 1)>(p, q, s);
