@@ -185,3 +185,139 @@ def test_two_threads_with_different_amounts_of_shared_memory():
     torch.cuda.synchronize()
     assert len(codes[0]) == len(codes[1]) == 3000
     assert not any(codes[0]) and not any(codes[1]), [sum(map(bool, c)) for c in codes]
+
+
+# ---- bits: tokens behind a sequence
+@pytest.mark.parametrize("ty,B,T,D,N", [("bf16", 2, 16, 64, 16), ("fp32", 2, 333, 20, 8), ("bf16", 3, 700, 64, 16), ("fp16", 1, 400, 130, 64)])
+def test_no_token_changes_no_bit_of_a_state(ty, B, T, D, N):
+    """Sequences without tokens, in one chunk and in several: their states and the gradients of these pass through as they are."""
+    i = scan_inputs(T, ty, B, T, D, N, 1, DEV)
+    zero = torch.zeros(B, dtype=torch.int32, device=DEV)
+    a = [i[k] for k in ("x", "dt", "A", "B", "C")]
+    y, end, ck = ssm.ssm_scan(*a, i["D"], i["dt_bias"], state=i["state"], lengths=zero, return_state=True, return_checkpoints=True)
+    assert torch.equal(end, i["state"]) and (y == 0).all()
+    got = ssm.ssm_scan_backward(i["gy"], *a, ck, i["D"], i["dt_bias"], lengths=zero, grad_final_state=i["gf"])
+    assert torch.equal(got[7], i["gf"])
+    assert all((g == 0).all() for g in got[:7])
+
+
+@pytest.mark.parametrize("T,n", [(16, 9), (16, 15), (32, 17), (700, 689)])
+def test_tokens_behind_a_sequence_change_no_bit_of_its_state(T, n):
+    """As many tiles with and without the tokens behind: the same chunks, the same states."""
+    i = scan_inputs(n, "bf16", 2, T, 64, 16, 1, DEV)
+    a = [i[k] for k in ("x", "dt", "A", "B", "C")]
+    cut = [t[:, :n] if t.dim() > 2 else t for t in a]
+    lengths = torch.full((2,), n, dtype=torch.int32, device=DEV)
+    y, end, ck = ssm.ssm_scan(*a, i["D"], i["dt_bias"], state=i["state"], lengths=lengths, return_state=True, return_checkpoints=True)
+    y1, end1, ck1 = ssm.ssm_scan(*cut, i["D"], i["dt_bias"], state=i["state"], return_state=True, return_checkpoints=True)
+    assert (T + 15) // 16 == (n + 15) // 16 and torch.equal(end, end1) and torch.equal(y[:, :n], y1) and torch.equal(ck, ck1)
+    got = ssm.ssm_scan_backward(i["gy"], *a, ck, i["D"], i["dt_bias"], lengths=lengths, grad_final_state=i["gf"])
+    want = ssm.ssm_scan_backward(i["gy"][:, :n], *cut, ck1, i["D"], i["dt_bias"], grad_final_state=i["gf"])
+    for k in (0, 1, 3, 4):
+        assert torch.equal(got[k][:, :n], want[k]) and (got[k][:, n:] == 0).all()
+    for k in (2, 5, 6, 7):
+        assert torch.equal(got[k], want[k])
+
+# ---- sums that have few roundings in a row -----------------------------------------------------------------------------------
+BLOCK = [
+    # type, M, D, norm, residual fp32, all parts
+    ("fp32", 5, 64, "layer", False, True), ("fp32", 3, 1003, "layer", False, True), ("fp32", 4, 1024, "rms", False, True),
+    ("bf16", 4, 2048, "layer", True, True), ("fp32", 3, 4096, "layer", False, False), ("fp32", 4, 4100, "layer", False, True),
+    ("bf16", 3, 4104, "layer", True, True), ("fp32", 4, 8192, "layer", False, True), ("fp16", 4, 8191, "layer", True, True),
+    ("fp32", 2, 8190, "rms", False, True), ("fp32", 3, 8192, "layer", False, False),
+]
+
+
+def _block_magnitudes(gx, gn, o, res, gate, layer, eps, post_weight=None, scale=None, pre_weight=None):
+    """What the roundings of the block end's gradients are relative to: (o, residual, gate, post_weight, None, scale, pre_weight).  A normalised
+    value (v - mean) r is off by 2^-24 of (|v| + |mean|) r however near to zero it comes (v = 0.3 + 1e-6 about a mean of 0.3: half a step of
+    0.3, 1.5e-8, is 1.5 % of it), so these stand for it in every term; of z = residual + scale u act(gate), |z| is the sum of its terms'."""
+    gx, gn, o, res, gate, w1, sc, w2 = (ol._d(t) for t in (gx, gn, o, res, gate, post_weight, scale, pre_weight))
+    mean = lambda v: v.mean(-1, keepdim=True)  # noqa: E731
+    r1, big = 1.0, o.abs()
+    if w1 is not None:
+        r1 = ol._norm(o, layer, eps)[1]
+        big = (o.abs() + (mean(o).abs() if layer else 0.0)) * r1
+    u = big * (w1.abs() if w1 is not None else 1.0)
+    gv, gs = ol.activation("sigmoid", gate) if gate is not None else (torch.ones_like(o), None)
+    s = sc.abs() if sc is not None else 1.0
+    z = s * u * gv + res.abs()
+    r2 = ol._norm(ol.norm_gate_residual(o, res, gate, "layer" if layer else "rms", "sigmoid", w1, None, sc, w2, None, eps)[0], layer, eps)[1]
+    zn = (z + (mean(z) if layer else 0.0)) * r2
+    back = lambda g, h, r: r * (g + h * mean(g * h) + (mean(g) if layer else 0.0))  # noqa: E731
+    d = gx.abs() + back(gn.abs() * w2.abs(), zn, r2)
+    du = d * s * gv
+    return (back(du * w1.abs(), big, r1) if w1 is not None else du, d, d * s * u * gs if gate is not None else None,
+            (du * big).sum(0) if w1 is not None else None, None, (d * u * gv).sum(0) if sc is not None else None, (gn.abs() * zn).sum(0))
+
+
+@pytest.mark.parametrize("ty,M,D,norm,res32,full", BLOCK)
+def test_the_means_of_the_norms_backward(ty, M, D, norm, res32, full):
+    """Upstream gradients of one sign, so that the means that a norm's backward takes off are as large as what they are taken off, and
+    tolerances that count the roundings in a row of these sums, not their terms: at most eight pairs, their halves, five shuffles, a warp's
+    count and reciprocal (5), four more shuffles and 1 / D: 28, once for the statistics and once for the means."""
+    t, rt, g = TYPES[ty], torch.float32 if res32 else TYPES[ty], gen(D)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    o, res, gate = (r(M, D) * 1.5 + 0.3).to(t).to(DEV), (r(M, D) * 2).to(rt).to(DEV), (1 + r(M, D)).to(t).to(DEV)
+    w = dict(post_weight=1 + 0.1 * r(D), scale=0.5 + 0.1 * r(D), pre_weight=1 + 0.1 * r(D)) if full else dict(pre_weight=1 + 0.1 * r(D))
+    w = {k: v.to(DEV) for k, v in w.items()}
+    gate = gate if full else None
+    kw = dict(norm=norm, activation="sigmoid", eps=1e-5, **w)
+    okw = {("activation_" if k == "activation" else k): v for k, v in kw.items()}
+    x, n, stats = glue.norm_gate_residual(o, res, gate, return_stats=True, **kw)
+    ref, _ = ol.norm_gate_residual(o, res, gate, **okw)
+    zh = ol._norm(ref, norm == "layer", 1e-5)[0]
+    gx = (0.5 + 0.05 * r(M, D)).to(x.dtype).to(DEV)
+    gn = (1 + 0.1 * r(M, D) + 0.5 * zh.float()).to(t).to(DEV)      # (its mean and its mean with the normalised values)
+    got = glue.norm_gate_residual_backward(gx, gn, o, stats, res, gate, **kw)
+    want = ol.norm_gate_residual_backward(gx, gn, o, res, gate, **okw)
+    amps = _block_magnitudes(gx, gn, o, res, gate, norm == "layer", 1e-5, **w)
+    for k, a, b, m in zip(("o", "residual", "gate", "post_weight", "post_bias", "scale", "pre_weight"), got, want, amps):
+        if a is not None:
+            # (4: z's errors once more in its statistics, as for all of these inputs)
+            close(a, b, m, 4 * (2 * 28 + 120) + (M if a.dim() == 1 else 0), "grad " + k)
+
+
+def _bounded(got, ref, bound, what):
+    """`bound`: in roundings of 2^-24"""
+    d = (got.double().cpu() - ref).abs()
+    tol = bound * (1 + 2.0 ** -10) * 2.0 ** -24 + 2.0 ** -24 * ref.abs() + 2.0 ** -126
+    assert (d <= tol).all(), (what, (d / tol).max().item())
+
+
+@pytest.mark.parametrize("B,T,D,N,G", [(1, 700, 64, 16, 1), (4, 64, 2560, 16, 1), (2, 333, 20, 5, 1), (1, 500, 48, 64, 3)])
+def test_errors_of_a_state_decay_with_it(B, T, D, N, G):
+    """The state's error is a recursion of its own: what a token adds decays with the state.  Per token, in roundings of 2^-24: delta
+    2 (|dt| + |bias|) + 16 of itself (its sum; the exponential, two reciprocals and the series); the factor exp(delta A) |delta A| times those of
+    delta, of A log2(e), of the product and of the sum of up to 16 deltas where chunks are joined (16 + 2), and 4 of the exponential;
+    delta x B three products and a sum.  y: 12 for its products, N / 4 lanes' and D x's sums."""
+    i = scan_inputs(T + N, "fp32", B, T, D, N, G, DEV)
+    a = [i[k] for k in ("x", "dt", "A", "B", "C")]
+    y, end, ck = ssm.ssm_scan(*a, i["D"], i["dt_bias"], state=i["state"], return_state=True, return_checkpoints=True)
+    ref, rend, _ = ol.ssm_scan(*a, i["D"], i["dt_bias"], state=i["state"])
+    x, dt, A, Bm, Cm = (t.double().cpu() for t in a)
+    bias, st, gy, gf = (i[k].double().cpu() for k in ("dt_bias", "state", "gy", "gf"))
+    spread = lambda m: m.repeat_interleave(D // G, -2)  # noqa: E731
+    Bm, Cm = spread(Bm).abs(), spread(Cm).abs()
+    delta = ol.softplus(dt + bias)
+    steps = 2 * (dt.abs() + bias.abs()) + 16
+    h, e, by = st.abs(), torch.zeros_like(st), torch.zeros_like(x)
+    for t in range(T):
+        z = delta[:, t, :, None] * A
+        f, u = torch.exp(z), (delta[:, t] * x[:, t].abs())[..., None] * Bm[:, t]
+        e = f * e + f * h * (z.abs() * (steps[:, t, :, None] + 18) + 4) + u * (steps[:, t, :, None] + 4) + (f * h + u)
+        h = f * h + u
+        m = (h * Cm[:, t]).sum(-1) + (i["D"].double().cpu() * x[:, t]).abs()
+        by[:, t] = (e * Cm[:, t]).sum(-1) + 12 * m
+    _bounded(end, rend, e, "state")
+    _bounded(y, ref, by, "y")
+    # the gradient of the first state, the same from the other end
+    got = ssm.ssm_scan_backward(i["gy"], *a, ck, i["D"], i["dt_bias"], grad_final_state=i["gf"])[7]
+    want = ol.ssm_scan_backward(i["gy"], *a, i["D"], i["dt_bias"], state=i["state"], grad_final_state=i["gf"])[7]
+    c, e = gf.abs(), torch.zeros_like(gf)
+    for t in reversed(range(T)):
+        z = delta[:, t, :, None] * A
+        f, u = torch.exp(z), gy[:, t, :, None].abs() * Cm[:, t]
+        e = f * (e + u + (c + u) * (z.abs() * (steps[:, t, :, None] + 18) + 4 + 2))
+        c = f * (c + u)
+    _bounded(got, want, e, "grad state")
