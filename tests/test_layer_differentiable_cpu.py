@@ -31,3 +31,27 @@ def test_block_end_of_equal_shapes_reaches_the_device_check():
 def test_block_end_without_values_to_a_token(o, msg):
     with pytest.raises(ValueError, match=msg):
         ag.norm_gate_residual(o)
+
+
+# ---- scan ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode, torch.enable_grad])
+@pytest.mark.parametrize("leaf", [True, False])
+@pytest.mark.parametrize("state", [True, False])
+def test_checkpoints_are_kept_only_for_a_backward_that_can_come(monkeypatch, mode, leaf, state):
+    """Weights that are parameters ask for a gradient even where none is recorded."""
+    from ttt_tk_b200 import ssm
+    asked = []
+
+    def scan(x, dt, A, B, C, D, dt_bias, softplus, state, lengths, return_state, return_checkpoints):
+        asked.append((return_state, return_checkpoints))
+        return (torch.zeros_like(x), torch.zeros(2, 8, 4) if return_state else None, torch.zeros(2, 1, 8, 4) if return_checkpoints else None)
+
+    monkeypatch.setattr(ssm, "_host", lambda: type("Host", (), {"scan": staticmethod(scan)}))
+    x, B = torch.zeros(2, 5, 8), torch.zeros(2, 5, 1, 4)
+    A, D = (torch.nn.Parameter(torch.zeros(s), requires_grad=leaf) for s in ((8, 4), (8,)))
+    with mode():
+        r = ag.ssm_scan(x, x, A, B, B, D, return_state=state)
+    wanted = leaf and mode is torch.enable_grad
+    assert asked == [(state, wanted)]
+    y = r[0] if state else r
+    assert y.requires_grad == wanted and y.shape == x.shape

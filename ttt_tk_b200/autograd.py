@@ -202,14 +202,17 @@ def short_conv(x, weight, bias=None, *, activation=None, state=None, lengths=Non
 
 
 class SSMScanFunction(torch.autograd.Function):
-    """(y, final state or None) = f(x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state)."""
+    """(y, final state or None) = f(x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state, recorded).
+
+    `recorded`: whether gradients are recorded where it is called, which is not to be seen inside `forward` (and `needs_input_grad` says
+    what the inputs ask for, recorded or not): the checkpoints, fp32 [batch, T / 16, D, N], are written for a backward that can come."""
 
     @staticmethod
-    def forward(ctx, x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state):
+    def forward(ctx, x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state, recorded=True):
         from . import ssm
         x, dt, B, C = (_rows(t) for t in (x, dt, B, C))
         A, D, dt_bias, state = (_whole(t) for t in (A, D, dt_bias, state))
-        keep = any(ctx.needs_input_grad)
+        keep = recorded and any(ctx.needs_input_grad)
         r = ssm.ssm_scan(x, dt, A, B, C, D, dt_bias, softplus=softplus, state=state, lengths=lengths, return_state=return_state,
                          return_checkpoints=keep)
         r = r if isinstance(r, tuple) else (r,)
@@ -227,12 +230,12 @@ class SSMScanFunction(torch.autograd.Function):
         gy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if gy is None else _rows(gy)
         g = ssm.ssm_scan_backward(gy, x, dt, A, B, C, ck, D, dt_bias, softplus=ctx.softplus, lengths=lengths,
                                   grad_final_state=_whole(gf))
-        return g[:7] + (g[7] if ctx.has_state else None,) + (None,) * 3
+        return g[:7] + (g[7] if ctx.has_state else None,) + (None,) * 4
 
 
 def ssm_scan(x, dt, A, B, C, D=None, dt_bias=None, *, softplus=True, state=None, lengths=None, return_state=False):
-    """Differentiable `ttt_tk_b200.ssm.ssm_scan`; the checkpoints are kept for the backward."""
-    y, end = SSMScanFunction.apply(x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state)
+    """Differentiable `ttt_tk_b200.ssm.ssm_scan`; where gradients are recorded, the checkpoints are kept for the backward."""
+    y, end = SSMScanFunction.apply(x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state, torch.is_grad_enabled())
     return (y, end) if return_state else y
 
 
