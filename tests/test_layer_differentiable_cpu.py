@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from ttt_tk_b200 import autograd as ag
+from ttt_tk_b200 import glue, ssm
 
 BF = torch.bfloat16
 
@@ -39,7 +40,6 @@ def test_block_end_without_values_to_a_token(o, msg):
 @pytest.mark.parametrize("state", [True, False])
 def test_checkpoints_are_kept_only_for_a_backward_that_can_come(monkeypatch, mode, leaf, state):
     """Weights that are parameters ask for a gradient even where none is recorded."""
-    from ttt_tk_b200 import ssm
     asked = []
 
     def scan(x, dt, A, B, C, D, dt_bias, softplus, state, lengths, return_state, return_checkpoints):
@@ -55,3 +55,43 @@ def test_checkpoints_are_kept_only_for_a_backward_that_can_come(monkeypatch, mod
     assert asked == [(state, wanted)]
     y = r[0] if state else r
     assert y.requires_grad == wanted and y.shape == x.shape
+
+
+# ---- arguments of another kind --------------------------------------------------------------------------------------------
+def _scan_args(**kw):
+    a = dict(x=torch.zeros(2, 5, 8), dt=torch.zeros(2, 5, 8), A=torch.zeros(8, 4), B=torch.zeros(2, 5, 1, 4), C=torch.zeros(2, 5, 1, 4))
+    return {**a, **kw}
+
+
+@pytest.mark.parametrize("kind", [3, [1.0], "x"])
+def test_what_is_not_a_tensor(kind):
+    o = torch.zeros(2, 3, 8)
+    for call in (lambda: ag.short_conv(kind, torch.zeros(8, 4)), lambda: ag.short_conv(o, kind), lambda: ag.short_conv(o, torch.zeros(8, 4), kind),
+                 lambda: ag.short_conv(o, torch.zeros(8, 4), state=kind), lambda: ag.short_conv(o, torch.zeros(8, 4), lengths=kind),
+                 *[lambda k=k: ag.ssm_scan(**_scan_args(**{k: kind})) for k in ("x", "dt", "A", "B", "C", "D", "dt_bias", "state", "lengths")],
+                 lambda: ag.norm_gate_residual(kind), lambda: ag.norm_gate_residual(o, kind), lambda: ag.norm_gate_residual(o, gate=kind),
+                 lambda: ag.norm_gate_residual(o, pre_weight=kind)):
+        with pytest.raises(ValueError):
+            call()
+
+
+@pytest.mark.parametrize("zero", ["x", "dt", "A", "B", "C", "D", "dt_bias", "state"])
+def test_tensors_without_dimensions(zero):
+    with pytest.raises(ValueError, match="must be"):
+        ag.ssm_scan(**_scan_args(**{zero: torch.zeros(())}))
+
+
+@pytest.mark.parametrize("name", [["silu"], {}, 1, "SILU", torch.zeros(2)])
+def test_names_of_no_activation_or_norm(name):
+    o = torch.zeros(2, 3, 8)
+    for call in (lambda: ssm.short_conv(o, torch.zeros(8, 4), activation=name), lambda: ag.short_conv(o, torch.zeros(8, 4), activation=name),
+                 lambda: ssm.short_conv_step(o[0], torch.zeros(3, 3, 8), torch.zeros(8, 4), activation=name),
+                 lambda: glue.norm_gate_residual(o, activation=name), lambda: ag.norm_gate_residual(o, norm=name)):
+        with pytest.raises(ValueError, match="activation|norm must be"):
+            call()
+
+
+@pytest.mark.parametrize("eps", ["1e-5", None, [1.0], -1e-30])
+def test_an_epsilon_that_is_no_number(eps):
+    with pytest.raises(ValueError, match="eps"):
+        glue.norm_gate_residual(torch.zeros(2, 8), eps=eps)

@@ -155,18 +155,21 @@ def ttt_linear(XQ, XK, XV, last_eta, ttt_norm_weight, ttt_norm_bias, W1, b1, che
 
 
 # ---- layer-side sequence operators (`ttt_tk_b200.ssm`, the block end of `ttt_tk_b200.glue`) ------------------------------------
+# What is no tensor (None among it) passes, for the operator to take or to refuse.
 def _rows(t):
     """With a contiguous last dimension (an upstream gradient can be an expanded number)."""
-    return t if t is None or t.dim() == 0 or t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
+    return t if not isinstance(t, torch.Tensor) or t.dim() == 0 or t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
 
 
-def _whole(t, dtype=None):
-    return None if t is None else t.contiguous() if dtype is None else t.to(dtype).contiguous()
+def _whole(t):
+    return t.contiguous() if isinstance(t, torch.Tensor) else t
 
 
 def _tokens(t):
     """[..., D] as [tokens, D]."""
-    return t if t is None or t.dim() in (0, 2) else t.unsqueeze(0) if t.dim() == 1 else t.flatten(0, -2)
+    if not isinstance(t, torch.Tensor) or t.dim() in (0, 2):
+        return t
+    return t.unsqueeze(0) if t.dim() == 1 else t.flatten(0, -2)
 
 
 class ShortConvFunction(torch.autograd.Function):
@@ -271,7 +274,7 @@ def norm_gate_residual(o, residual=None, gate=None, *, norm="rms", activation="s
                        pre_weight=None, pre_bias=None, eps=1e-6):
     """Differentiable `ttt_tk_b200.glue.norm_gate_residual`, with rows at any distances."""
     for name, t in (("residual", residual), ("gate", gate)):
-        if t is not None and t.shape != o.shape:
+        if isinstance(o, torch.Tensor) and isinstance(t, torch.Tensor) and t.shape != o.shape:
             raise ValueError(f"norm_gate_residual: {name} must have the shape of o, {list(o.shape)}, got {list(t.shape)}")
     x, n = NormGateResidualFunction.apply(*[_tokens(t) for t in (o, residual, gate)], post_weight, post_bias, scale, pre_weight, pre_bias, norm, activation, eps)
     return x.view(o.shape), None if n is None else n.view(o.shape)

@@ -513,7 +513,11 @@ const Tensor& block_inputs(Call& c, ttt_b200_block_args& a, PyObject* o, PyObjec
   c.need(a.post_weight || !a.post_bias, "post_bias needs post_weight");
   c.need(a.pre_weight || !a.pre_bias, "pre_bias needs pre_weight");
   a.eps = static_cast<float>(PyFloat_AsDouble(v[9]));
-  if (PyErr_Occurred()) throw PythonError();
+  if (PyErr_Occurred()) {
+    if (!PyErr_ExceptionMatches(PyExc_TypeError)) throw PythonError();
+    PyErr_Clear();
+    refuse("norm_gate_residual: eps must be a number");
+  }
   c.need(a.eps >= 0.f, "eps must be >= 0");
   return t;
 }

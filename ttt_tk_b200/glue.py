@@ -89,8 +89,8 @@ _GATES = {"silu": 1, "gelu": 2, "sigmoid": 3}
 
 
 def _kinds(norm, activation):
-    _need(norm in _NORMS, f"norm must be 'rms' or 'layer', got {norm!r}")
-    _need(activation in _GATES, f"activation must be 'silu', 'gelu' or 'sigmoid', got {activation!r}")
+    _need(isinstance(norm, str) and norm in _NORMS, f"norm must be 'rms' or 'layer', got {norm!r}")
+    _need(isinstance(activation, str) and activation in _GATES, f"activation must be 'silu', 'gelu' or 'sigmoid', got {activation!r}")
     return _NORMS[norm], _GATES[activation]
 
 

@@ -36,7 +36,7 @@ def _host():
 
 
 def _activation(name):
-    if name not in _ACTIVATIONS:
+    if not (name is None or isinstance(name, str)) or name not in _ACTIVATIONS:
         raise ValueError(f"activation must be None or 'silu', got {name!r}")
     return _ACTIVATIONS[name]
 
