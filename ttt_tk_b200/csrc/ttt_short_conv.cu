@@ -5,12 +5,13 @@
 //
 // Bound by memory: 2 K operations per value that is read and written once.  A thread owns two neighbouring channels (one where rows
 // do not start on a pair's boundary) and walks along a run of tokens with the last K - 1 inputs in registers, so that an input is read
-// once per run; the K - 1 in front of a run come from the cache.  Rows come through a warp's ring of four blocks of eight rows in shared
+// once per run; the K - 1 in front of a run come from the cache.  Rows come through a warp's ring of four blocks of eight rows (two in fp32) in shared
 // memory: a warp's row is 128 bytes, and it takes some 40 KB in flight to keep an SM's share of the memory busy, which registers do
 // not hold.  The backward keeps the last K values of g as well and leaves dx with a delay of K - 1 tokens.
 //
-// Measured, 4 x 2048 tokens of 2048 channels, bf16, K = 4, silu: forward 16.6 us (4.0 TB/s), backward 32 us (3.1 TB/s; 52 % of the issue
-// slots, 68 instructions per token and pair).  3 x 1001 x 1003 in fp32, single channels: 5.9 us (4.1 TB/s) and 13.5 us (2.7 TB/s).  The step of
+// Measured, 4 x 2048 tokens of 2048 channels, K = 4, silu: in bf16 forward 16.2 us (4.1 TB/s), backward 31 us (3.3 TB/s; 52 % of the issue
+// slots, 68 instructions per token and pair), in fp32 20.3 and 45 us.  3 x 1001 x 1003 in fp32, K = 3, single channels: 5.9 us
+// (4.1 TB/s) and 10.8 us (3.3 TB/s).  The step of
 // 8 rows of 2048: 2.5 us, a launch.
 #include <algorithm>
 #include <cstdio>
@@ -110,9 +111,10 @@ constexpr int U = 8;      // tokens of a block, which are requested together
 
 // The rows of a tensor that a warp walks along, a block of U tokens at a time, requested ahead of the block that is worked on; those
 // from `stop` on are not read.  Pairs of channels go through a ring in shared memory (asynchronous 16-byte copies: what is
-// in flight costs no registers), single channels through registers.  All lanes of a warp call `start` and `turn` together.
+// in flight costs no registers), single channels through registers.
 template <class T, int V> struct Rows;
 template <class T> struct Rows<T, 2> {
+  static constexpr bool kRing = true;
   static constexpr int kSlots = sizeof(T) == 2 ? 4 : 2, kWidth = 64, kBytes = kSlots * U * kWidth * sizeof(T);
   static constexpr int kPiece = 16 / sizeof(T), kPieces = kWidth / kPiece, kMine = U * kPieces / 32;      // pieces of a block, of a lane
   T* ring;
@@ -123,6 +125,12 @@ template <class T> struct Rows<T, 2> {
     const int c = (threadIdx.x & 31) % kPieces * kPiece, n = min(max(cols - c, 0), kPiece);
     bytes = n * static_cast<int>(sizeof(T));
     if (n > 0) from += c;
+  }
+  __device__ __forceinline__ void aim(int begin, int stop_) {
+    t = begin;
+    stop = stop_;
+    block = -1;
+    next = from + (begin + (threadIdx.x & 31) / kPieces) * stride;
   }
   __device__ __forceinline__ void issue(int slot) {
     if (t < stop) {
@@ -136,27 +144,16 @@ template <class T> struct Rows<T, 2> {
       next += U * stride;
       t += U;
     }
-    cp_async_commit();
   }
-  __device__ __forceinline__ void start(int begin, int stop_) {
-    t = begin;
-    stop = stop_;
-    block = -1;
-    next = from + (begin + (threadIdx.x & 31) / kPieces) * stride;
-#pragma unroll
-    for (int k = 0; k < kSlots - 1; ++k) issue(k);
-  }
-  // to the next block
-  __device__ __forceinline__ void turn() {
+  __device__ __forceinline__ void advance() {
     ++block;
-    cp_async_wait<kSlots - 2>();
-    __syncwarp();      // the block has landed for all lanes, and all are through with the one before
     issue((block + kSlots - 1) % kSlots);
   }
   // row u of the block; `at`: where there are that many before `stop`
   __device__ __forceinline__ Raw<T, 2> at(int u) const { return load<T, 2>(ring + (block % kSlots * U + u) * kWidth + 2 * (threadIdx.x & 31)); }
 };
 template <class T> struct Rows<T, 1> {
+  static constexpr bool kRing = false;
   static constexpr int kBytes = 0;
   const T* next;      // of this lane's channel (behind the last channel: of the tile's first)
   int64_t stride;
@@ -176,19 +173,43 @@ template <class T> struct Rows<T, 1> {
     next += U * stride;
     t += U;
   }
-  __device__ __forceinline__ void start(int begin, int stop_) {
+  __device__ __forceinline__ void aim(int begin, int stop_) {
     t = begin;
     stop = stop_;
     next += begin * stride;
     ask();
   }
-  __device__ __forceinline__ void turn() {
+  __device__ __forceinline__ void advance() {
 #pragma unroll
     for (int u = 0; u < U; ++u) now[u] = then[u];
     ask();
   }
   __device__ __forceinline__ Raw<T, 1> at(int u) const { return now[u]; }
 };
+
+// Tensors that are walked along together, to their first block and from block to block; all lanes of a warp together.  Copies are waited for
+// by groups, whichever ring they are for, so a block of all rings is one group: kSlots - 2 blocks of each are on their way behind a wait.
+template <class R, class... More> __device__ __forceinline__ void start(int begin, int stop, R& rows, More&... more) {
+  rows.aim(begin, stop);
+  (more.aim(begin, stop), ...);
+  if constexpr (R::kRing) {
+#pragma unroll
+    for (int k = 0; k < R::kSlots - 1; ++k) {
+      rows.issue(k);
+      (more.issue(k), ...);
+      cp_async_commit();
+    }
+  }
+}
+template <class R, class... More> __device__ __forceinline__ void turn(R& rows, More&... more) {
+  if constexpr (R::kRing) {
+    cp_async_wait<R::kSlots - 2>();
+    __syncwarp();      // the block has landed for all lanes, and all are through with the one before, whose place the next one takes
+  }
+  rows.advance();      // (issues the last block of the ring)
+  (more.advance(), ...);
+  if constexpr (R::kRing) cp_async_commit();
+}
 
 template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(32 * kWarps) conv_forward_kernel(const ttt_b200_conv_args p, const Plan q) {
   wait_for_predecessor();
@@ -201,7 +222,7 @@ template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(3
   const int d = mine ? at.group * V : d0;      // (a lane behind the last channel reads the tile's first)
   const int len = length_of(p, b), stop = min(len, end);
   Rows<T, V> rows(rings[threadIdx.x / 32], static_cast<const T*>(p.x) + b * p.x_stride[0] + d0, p.x_stride[1], p.D - d0);
-  rows.start(begin, stop);
+  start(begin, stop, rows);
   T* y = static_cast<T*>(p.y) + b * q.y_batch + d / 64 * q.y_head + d % 64;
   F w[K], bias, x[K];
   load_weights<K, V>(p, d, w, bias);
@@ -220,7 +241,7 @@ template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(3
     return kSilu ? times(v, sigmoid(v)) : v;
   };
   for (int t0 = begin; t0 < end; t0 += U) {
-    rows.turn();
+    turn(rows);
     T* to = y + t0 * q.y_token;
     if (t0 + U <= stop) {
 #pragma unroll
@@ -266,8 +287,7 @@ template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(3
     Rows<T, V> rows(rings[0][warp], static_cast<const T*>(p.x) + b * p.x_stride[0] + d0, p.x_stride[1], p.D - d0);
     Rows<T, V> ups(rings[1][warp], static_cast<const T*>(p.grad_y) + (heads ? b * q.y_batch + d0 / 64 * q.y_head + d0 % 64 : b * p.gy_stride[0] + d0),
                    heads ? q.y_token : p.gy_stride[1], p.D - d0);
-    rows.start(begin, live);
-    ups.start(begin, live);
+    start(begin, live, rows, ups);
     const T* gf = p.grad_final_state ? static_cast<const T*>(p.grad_final_state) + static_cast<long>(b) * (K - 1) * p.D + d : nullptr;
     T* gx = static_cast<T*>(p.grad_x) + static_cast<long>(b) * p.T * p.D + d;
     T* gs = p.grad_state ? static_cast<T*>(p.grad_state) + static_cast<long>(b) * (K - 1) * p.D + d : nullptr;
@@ -313,8 +333,7 @@ template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(3
       store<T, V>(s >= 0 ? gx + static_cast<long>(s) * p.D : gs + static_cast<long>(s + K - 1) * p.D, narrow<T, V>(o));
     };
     for (int t0 = begin; t0 < end; t0 += U) {
-      rows.turn();
-      ups.turn();
+      turn(rows, ups);
       if (t0 + U <= whole) {
         T* to = gx + static_cast<long>(t0 - K + 1) * p.D;
 #pragma unroll
@@ -335,8 +354,7 @@ template <class T, int K, int V, bool kSilu> __global__ void __launch_bounds__(3
     }
     // the K - 1 tokens behind the run, for the gradients of its last inputs; where there are any the run ends with a block
     if (end < live) {
-      rows.turn();
-      ups.turn();
+      turn(rows, ups);
     }
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
@@ -445,8 +463,9 @@ bool paired_weights(const ttt_b200_conv_args& p) {
 }
 
 // Tokens of a warp's run: as many as leave four to five CTAs to an SM, since each run reads K - 1 tokens more and has its weights to
-// fetch.  Measured, us, forward / backward with runs of 16, 32, 64, 128: 4 x 2048 tokens of 2048 channels 18.7 / 49.7, 16.7 / 43.4,
-// 15.7 / 37.3, 17.7 / 37.3; 2048 tokens of 768 channels 6.1 / 12.6, 6.3 / 14.7, 6.5 / 16.7, 9.9 / 22.9.
+// fetch.  Measured, us, forward / backward with its sum of parts, K = 4, bf16, with runs of 16, 32, 64, 128: 4 x 2048 tokens of 2048 channels
+// 19.9 / 46.4, 18.1 / 38.7, 16.2 / 34.6, 18.0 / 36.0 (64 by the rule); 2048 tokens of 768 channels 5.0 / 11.0, 6.3 / 12.2, 7.0 / 14.3, 9.4 / 20.4
+// (16 by the rule).
 void plan_runs(Plan& q, const ttt_b200_conv_args& p, int V) {
   q.groups = p.D / V;
   const long tiles = (q.groups + 31) / 32, sms = sm_count();
