@@ -321,3 +321,34 @@ def test_errors_of_a_state_decay_with_it(B, T, D, N, G):
         e = f * (e + u + (c + u) * (z.abs() * (steps[:, t, :, None] + 18) + 4 + 2))
         c = f * (c + u)
     _bounded(got, want, e, "grad state")
+
+
+# ---- offsets beyond 32 bits ------------------------------------------------------------------------------------------------
+def test_backward_of_more_than_two_to_the_31_values():
+    """Activations, checkpoints and gradients of more than 2^31 values: the gradients at the end are those of a run that starts there."""
+    T, D, N, cut = 1_100_000, 2048, 16, 1_099_008
+    r = lambda *s: torch.randn(*s, device=DEV, dtype=torch.bfloat16)  # noqa: E731
+    rel = lambda a, b: ((a.double() - b.double()).norm() / b.double().norm()).item()  # noqa: E731
+    x, gy = r(1, T, D), r(1, T, D)
+    dt = r(1, T, 1).expand(1, T, D).contiguous()
+    A = -torch.rand(D, N, device=DEV) - 0.5
+    B, C = r(1, T, 1, N), r(1, T, 1, N)
+    y, ck = ssm.ssm_scan(x, dt, A, B, C, return_checkpoints=True)
+    assert min(t.numel() for t in (x, y, ck)) > 2 ** 31
+    del y
+    got = ssm.ssm_scan_backward(gy, x, dt, A, B, C, ck)
+    tail = (x[:, cut:], dt[:, cut:], A, B[:, cut:], C[:, cut:])
+    _, ct = ssm.ssm_scan(*tail, state=ck[:, cut // 16].contiguous(), return_checkpoints=True)
+    want = ssm.ssm_scan_backward(gy[:, cut:], *tail, ct)
+    for k in (0, 1, 3, 4):      # two roundings to bf16 of the same sums
+        assert rel(got[k][:, cut:], want[k]) <= 2 ** -8, k
+    assert all(torch.isfinite(got[k]).all() for k in (2, 7))
+    del got, want, ck, ct, dt, B, C
+    res, gate, gn = r(1, T, D), r(1, T, D), r(1, T, D)
+    w = torch.ones(D, device=DEV)
+    kw = dict(post_weight=w, scale=w, pre_weight=w)
+    _, _, stats = glue.norm_gate_residual(x, res, gate, return_stats=True, **kw)
+    got = glue.norm_gate_residual_backward(gy, gn, x, stats, res, gate, **kw)
+    want = glue.norm_gate_residual_backward(gy[:, cut:], gn[:, cut:], x[:, cut:], stats[cut:], res[:, cut:], gate[:, cut:], **kw)
+    for k in range(3):
+        assert torch.equal(got[k][:, cut:], want[k]), k
