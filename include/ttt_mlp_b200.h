@@ -433,7 +433,8 @@ typedef struct ttt_b200_scan_args {
   const int32_t* lengths;     /* [B] or NULL */
   void* y;                    /* [B][T][D]; step: [B][D] */
   float* final_state;         /* [B][D][N] or NULL */
-  float* checkpoints;         /* [B][ceil(T / 16)][D][N]: states before every 16th token, for the backward; forward: or NULL */
+  float* checkpoints;         /* [B][ceil(T / 16)][D][N]: states before every 16th token, for the backward; forward: or NULL.  Those of
+                               * tokens behind a sequence are neither written nor read */
   /* backward: the inputs and the checkpoints above, and */
   const void* grad_y;         /* [B][T][D], strides gy_stride */
   const float* grad_final_state; /* [B][D][N] or NULL */
@@ -452,7 +453,11 @@ typedef struct ttt_b200_scan_args {
 } ttt_b200_scan_args;
 int ttt_b200_ssm_scan(const ttt_b200_scan_args* args, void* stream);
 int ttt_b200_ssm_scan_backward(const ttt_b200_scan_args* args, void* stream);
-/* Bytes of scratch the forward (backward = 0) or backward needs; depends on B, T, D, G, N and the GPU. */
+/* Bytes of scratch the forward (backward = 0) or backward needs; depends on B, T, D, G, N and the GPU.  What a backward takes grows with
+ * channels x states: beside the checkpoints, N / 4 bytes per token and channel, its scratch holds grad_B and grad_C as fp32 parts, one per
+ * 128, 64, 32 or 16 channels of a group for up to 8, 16, 32 or 64 states, where a group has more channels than that: 1/2, 2, 8 or 32 bytes per token
+ * and channel at 8, 16, 32 and 64 states (and the states of the chunks, which are small beside that).  16 x 8192 tokens of 4096 channels in one
+ * group: 2.1 GB of checkpoints and 1.1 GB of scratch with 16 states, 8.6 and 17 GB with 64, beside 1 GB of x in 16 bits. */
 uint64_t ttt_b200_ssm_scan_scratch_bytes(const ttt_b200_scan_args* args, int backward);
 /* One token per row; slots as in ttt_b200_short_conv_step. */
 int ttt_b200_ssm_scan_step(const ttt_b200_scan_args* args, void* stream);

@@ -76,7 +76,8 @@ def ssm_scan(x, dt, A, B, C, D=None, dt_bias=None, *, softplus=True, state=None,
     `x`, `dt` [batch, T, D]; `A` fp32 [D, N], finite, 1 to 64 states; `B`, `C` [batch, T, G, N], G dividing the channels; `D`,
     `dt_bias` fp32 [D]; `state` fp32 [batch, D, N] in front of the first token (zeros without it).  Returns y [batch, T, D], followed
     by the state behind each sequence's last token where `return_state` asks for it, and by the states before every 16th
-    token, fp32 [batch, ceil(T / 16), D, N], that `ssm_scan_backward` starts from, where `return_checkpoints` does."""
+    token, fp32 [batch, ceil(T / 16), D, N], that `ssm_scan_backward` starts from, where `return_checkpoints` does (those behind a
+    sequence's end hold nothing)."""
     y, end, ck = _host().scan(x, dt, A, B, C, D, dt_bias, softplus, state, lengths, return_state, return_checkpoints)
     if not (return_state or return_checkpoints):
         return y
@@ -87,7 +88,10 @@ def ssm_scan_backward(grad_y, x, dt, A, B, C, checkpoints, D=None, dt_bias=None,
                       grad_final_state=None):
     """Gradients of `ssm_scan` from its inputs and checkpoints: (grad_x, grad_dt, grad_A, grad_B, grad_C, grad_D, grad_dt_bias,
     grad_state); grad_D and grad_dt_bias None where there is none.  Those of the activations have their type, the others are fp32;
-    grad_state fp32 [batch, D, N] is that of the state in front of the first token."""
+    grad_state fp32 [batch, D, N] is that of the state in front of the first token.
+
+    Memory: the checkpoints are N / 4 bytes per token and channel, and its scratch, for grad_B and grad_C, 1/2, 2, 8 or 32 bytes per token and
+    channel at 8, 16, 32 or 64 states, where a group has more than 128, 64, 32 or 16 channels."""
     return _host().scan_backward(grad_y, x, dt, A, B, C, D, dt_bias, softplus, checkpoints, lengths, grad_final_state)
 
 
