@@ -17,7 +17,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <cstdio>
 #include <type_traits>
 
 #include "ttt_elem.cuh"
@@ -327,8 +326,6 @@ __device__ __forceinline__ float2 statistics(const F (&a)[NV][N], const ttt_b200
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
-inline int fail(const char* msg) { return ttt_set_error(TTT_B200_ERR_BAD_ARGS, msg); }
-
 inline int check(const ttt_b200_block_args* p) {
   if (!p) return fail("block norm: NULL argument struct");
   if (p->M < 0 || p->D < 1 || p->D > 8192) return fail("block norm: M >= 0 and 1 <= D <= 8192");
@@ -337,13 +334,6 @@ inline int check(const ttt_b200_block_args* p) {
   if (!(p->eps >= 0.f)) return fail("block norm: eps must be >= 0");
   if ((p->post_bias && !p->post_weight) || (p->pre_bias && !p->pre_weight)) return fail("block norm: a bias without its weight");
   return TTT_B200_OK;
-}
-
-inline int sm_count() {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
 }
 
 // threads of a token: the fewest that hold it with `values` each
@@ -380,14 +370,6 @@ inline bool vectors(const ttt_b200_block_args& p, bool backward, int run) {
 inline int parts_of(const ttt_b200_block_args& p) {
   if (p.residual && p.gate && p.post_weight && p.scale && p.pre_weight) return kAll;
   return p.residual && p.pre_weight && !p.gate && !p.post_weight && !p.scale ? kBare : kSome;
-}
-
-inline int launched(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) return TTT_B200_OK;
-  static thread_local char buf[160];
-  snprintf(buf, sizeof buf, "%s: %s", what, cudaGetErrorString(e));
-  return ttt_set_error(TTT_B200_ERR_LAUNCH, buf);
 }
 
 // More dynamic shared memory than 48 KB has to be asked for, per kernel and device.  All that there is is asked for, once: a limit of a

@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <stdio.h>
 
 #include "ttt_internal.h"
 
@@ -145,6 +146,22 @@ template <int V, int L, int kStride> __device__ __forceinline__ void spread_sum(
   }
 }
 
+// ---- host
+inline int fail(const char* msg) { return ttt_set_error(TTT_B200_ERR_BAD_ARGS, msg); }
+inline int sm_count() {
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+// what the launch in front has come to
+inline int launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return TTT_B200_OK;
+  static thread_local char buf[160];
+  snprintf(buf, sizeof buf, "%s: %s", what, cudaGetErrorString(e));
+  return ttt_set_error(TTT_B200_ERR_LAUNCH, buf);
+}
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace ttt

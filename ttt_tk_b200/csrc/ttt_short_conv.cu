@@ -14,7 +14,6 @@
 // (4.1 TB/s) and 10.8 us (3.3 TB/s).  The step of
 // 8 rows of 2048: 2.5 us, a launch.
 #include <algorithm>
-#include <cstdio>
 #include <type_traits>
 
 #include "ttt_elem.cuh"
@@ -421,8 +420,6 @@ template <class T, int K, int V> __global__ void __launch_bounds__(128) conv_ste
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
-int fail(const char* msg) { return ttt_set_error(TTT_B200_ERR_BAD_ARGS, msg); }
-
 int check(const ttt_b200_conv_args* p) {
   if (!p) return fail("short conv: NULL argument struct");
   if (p->B < 0 || p->T < 0 || p->T > 1 << 30 || p->D < 1 || p->D > 1 << 30 || p->K < 2 || p->K > 4)
@@ -431,21 +428,6 @@ int check(const ttt_b200_conv_args* p) {
   if (p->activation != TTT_B200_ACT_NONE && p->activation != TTT_B200_ACT_SILU) return fail("short conv: activation is none or silu");
   if (p->heads && (p->D % 64 || p->T % 64)) return fail("short conv: heads need multiples of 64 channels and tokens");
   return TTT_B200_OK;
-}
-
-int sm_count() {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
-int launched(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) return TTT_B200_OK;
-  static thread_local char buf[160];
-  snprintf(buf, sizeof buf, "%s: %s", what, cudaGetErrorString(e));
-  return ttt_set_error(TTT_B200_ERR_LAUNCH, buf);
 }
 
 // whether channels can be taken in pairs

@@ -22,7 +22,6 @@
 // forward 93; backward states 60, join 5, backward 256, sum of parts 11.  8192 tokens of 1024 channels: 46, 7 and 63 us.  The exponential
 // unit is 79, 57, 80 and 49 % busy in states, forward, states and backward, the issue slots 52, 58, 52 and 58 %.
 #include <algorithm>
-#include <cstdio>
 #include <type_traits>
 
 #include "ttt_elem.cuh"
@@ -953,15 +952,6 @@ template <class T, int LN, bool kOne> __global__ void __launch_bounds__(TH, 8) s
 // ---- host --------------------------------------------------------------------------------------------------------------
 int lanes_of(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
-int fail(const char* msg) { return ttt_set_error(TTT_B200_ERR_BAD_ARGS, msg); }
-
 int check(const ttt_b200_scan_args* p) {
   if (!p) return fail("ssm scan: NULL argument struct");
   if (p->B < 0 || p->T < 0 || p->T > 1 << 30 || p->D < 1 || p->D > 1 << 30 || p->G < 1 || p->N < 1 || p->N > 64)
@@ -1054,14 +1044,6 @@ int prepare(Plan& q, const ttt_b200_scan_args& p, bool backward) {
                         static_cast<const void*>(p.grad_state)})
     q.vec_n = q.vec_n && aligned16(s);
   return TTT_B200_OK;
-}
-
-int launched(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) return TTT_B200_OK;
-  static thread_local char buf[160];
-  snprintf(buf, sizeof buf, "%s: %s", what, cudaGetErrorString(e));
-  return ttt_set_error(TTT_B200_ERR_LAUNCH, buf);
 }
 
 template <class K> int launch(K kernel, size_t smem, long grid, cudaStream_t s, const ttt_b200_scan_args& p, const Plan& q) {
