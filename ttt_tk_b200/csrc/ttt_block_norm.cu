@@ -1,8 +1,10 @@
 // The end of a block and the start of the next: forward.
 //
-// Measured with all parts, 16384 x 2048 bf16: fp32 residual stream, layer norms, tanh gate 88 us (5.3 TB/s); bf16 residual, RMS norms
-// 67 us (5.0 TB/s); rows of 2047 105 us (3.2); a bf16 residual and the next RMS norm alone 44 us (6.2 TB/s).  Issued instructions and the wait at a token's barriers are what is left above the
-// memory: 1024 threads to an SM (1280: 106 us where 1024 had 97, since the L1 has less room for the weights).
+// Measured with all parts, 16384 x 2048 bf16: fp32 residual stream, layer norms, tanh gate 87 us (5.4 TB/s), all in fp32 102 us (6.6); bf16
+// residual, RMS norms 68 us (4.9 TB/s); rows of 2047 127 us (3.7) and 106 us (3.2); a bf16 residual and the next RMS norm alone 42 us (6.3 TB/s).  Rows
+// that do not fill their threads, fp32 residual: 16384 x 1536 83 us (4.2), 32768 x 768 81 us (4.3); 4096 x 8192 100 us (4.7).  Issued instructions and
+// the wait at a token's barriers are what is left above the memory: 1024 threads to an SM (1280: 106 us where 1024 had 97, since the L1 has less
+// room for the weights).
 #include "ttt_block_norm.cuh"
 
 namespace {

@@ -1,8 +1,11 @@
 // The end of a block and the start of the next: backward.
 //
-// Measured with all parts, 16384 x 2048 bf16: fp32 residual stream, layer norms, tanh gate 168 us (4.4 TB/s); bf16 residual, RMS norms
-// 147 us (3.6 TB/s), a residual and the next norm alone 83 us (4.9 TB/s); rows of 2047 210 us (2.6); 4096 x 8192, layer norms, sums in shared memory, 335 us (1.6).  512 threads to an SM,
-// since a thread has 128 registers, 40 of them sums over tokens; each wait (two barriers a token, the L1 for the weights) shows.
+// Measured with all parts, the kernel by itself (the sum of its parts is 4 to 7 us more, of rows of up to 512 values 13 to 24), 16384 x 2048 bf16: fp32
+// residual stream, layer norms, tanh gate 155 us (4.8 TB/s), all in fp32 177 us (6.1); bf16 residual, RMS norms 141 us (3.8 TB/s), a residual and the
+// next norm alone 81 us (5.0); rows of 2047 216 us (3.4) and 204 us (2.6).  Rows that do not fill their threads, fp32 residual: 16384 x 1536 153 us
+// (3.6), 32768 x 768 142 us (3.9).  65536 x 512, whose kernels spill (up to 132 bytes), 171 us (4.3).  4096 x 8192, layer norms, sums in shared memory and
+// nothing copied ahead: 282 us (2.6), with a bf16 residual 324 us (1.7).  512 threads to an SM, since a thread has 128 registers, 40 of them sums
+// over tokens; each wait (two barriers a token, the L1 for the weights) shows.
 #include "ttt_block_norm.cuh"
 
 namespace {

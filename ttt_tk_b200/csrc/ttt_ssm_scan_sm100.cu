@@ -19,7 +19,7 @@
 // backward does the same from the other end.
 //
 // Measured, 4 x 2048 tokens of 1536 channels, 16 states, bf16 (24 chunks; 201 M exponentials, 45 us of their unit): states 67 us, join 5,
-// forward 93; backward states 60, join 5, backward 256, sum of parts 11.  8192 tokens of 1024 channels: 46, 7 and 63 us.  The exponential
+// forward 93; backward states 60, join 5, backward 255, sum of parts 11.  8192 tokens of 1024 channels: 45, 7 and 64 us.  The exponential
 // unit is 79, 57, 80 and 49 % busy in states, forward, states and backward, the issue slots 52, 58, 52 and 58 %.
 #include <algorithm>
 #include <type_traits>
@@ -286,6 +286,10 @@ template <class T, int LN> struct FwdSmem {
   alignas(16) float y[2][kTile * YW];          // D x, then y
 };
 
+// Four CTAs to an SM, here and in the state kernel, against three, whose 168 registers hold nearly all that 128 spill (us, forward kernel / state
+// kernel): 4 x 2048 x 1536 x 16 in 24 chunks 93 / 67 against 105 / 68, 2 x 1000 x 768 x 64 48 / 31 against 53 / 34; but 8 states in fp32 98 / 54 against
+// 85 / 50, and 8 x 2048 x 2048 x 16, which is not split, 307 against 299.
+//
 // One barrier to a tile: between two of them the states walk over tile k, tile k + 1 goes from its copy to fp32 (in registers
 // first, so that its arithmetic fills the gaps of the walk), tile k - 1 leaves, and the copy of tile k + 2 is on its way.
 template <class T, int LN> __global__ void __launch_bounds__(TH, 4) scan_forward_kernel(const ttt_b200_scan_args p, const Plan q) {
@@ -856,7 +860,8 @@ __global__ void __launch_bounds__(TH, LN <= 4 ? 4 : 3) scan_backward_kernel(cons
 // the slot is requested in front of it, and the state in front of the search for rows that share it: two round trips to memory in all.
 // Rows that name the same slot are taken in their order by the CTA of the first of them, so that no two CTAs touch a state.
 // kOne: a CTA's channels are of one group, whose B and C are then read once, and eight CTAs fit an SM instead of six (64 rows of
-// 2048 x 16: 7.3 -> 6.1 us, 64 of 4096 x 64: 47 -> 37 us, which is 3.6 TB/s; ten or twelve CTAs, with registers spilled, are no faster).
+// 2048 x 16: 7.3 -> 6.1 us with the states in the L2, 7.1 from memory; 64 of 4096 x 64: 47 -> 38 us, which is 3.6 TB/s; ten or twelve CTAs, with
+// registers spilled, are no faster).
 template <class T, int LN, bool kOne> __global__ void __launch_bounds__(TH, 8) scan_step_kernel(const ttt_b200_scan_args p, bool vec_n, int tiles) {
   wait_for_predecessor();
   constexpr int DC = TH / LN;
