@@ -1,7 +1,10 @@
 """The layer-side sequence operators at the ends of their ranges and where calls meet.
 Statements: oracle/layer.py; tolerances: tests/layer_cases.py."""
 import ctypes
+import os
 import struct
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -352,3 +355,89 @@ def test_backward_of_more_than_two_to_the_31_values():
     want = glue.norm_gate_residual_backward(gy[:, cut:], gn[:, cut:], x[:, cut:], stats[cut:], res[:, cut:], gate[:, cut:], **kw)
     for k in range(3):
         assert torch.equal(got[k][:, cut:], want[k]), k
+
+
+# ---- captured steps, first calls in a capture, other streams ----------------------------------------------------------------
+def test_captured_steps_follow_their_slots():
+    """Steps captured once and replayed with other tokens and slots, among them padding and a slot that is named twice."""
+    B, S, D, N, K = 5, 8, 72, 16, 4
+    g = gen(21)
+    r = lambda *s: torch.randn(*s, generator=g).to(DEV)  # noqa: E731
+    A, w, b, skip, bias, one = -r(D, N).abs(), r(D, K), r(D), r(D), r(D) - 3, torch.ones(D, device=DEV)
+    static = dict(x=r(B, D), dt=r(B, D), B=r(B, 1, N), C=r(B, 1, N), slots=torch.zeros(B, dtype=torch.int32, device=DEV))
+    start = (r(S, K - 1, D), r(S, D, N))
+
+    def run(i, ctable, table):
+        u = ssm.short_conv_step(i["x"], ctable, w, b, activation="silu", slots=i["slots"])
+        y = ssm.ssm_scan_step(u, i["dt"], A, i["B"], i["C"], table, skip, bias, slots=i["slots"])
+        return (y, *glue.norm_gate_residual(y, i["x"], u, post_weight=one, scale=one, pre_weight=one))
+
+    steps = [{**{k: r(*v.shape) for k, v in static.items() if k != "slots"}, "slots": torch.tensor(s, dtype=torch.int32, device=DEV)}
+             for s in ([0, 1, 2, 3, 4], [7, -1, 3, 3, 0], [S, 5, 3, 0, 5], [-2, S + 1, -1, 99, -1])]
+    tables = [t.clone() for t in start]
+    run(static, *tables)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(static, *tables)
+    for t, s in zip(tables, start):
+        t.copy_(s)
+    eager = [t.clone() for t in start]
+    for i in steps:
+        for k, v in i.items():
+            static[k].copy_(v)
+        graph.replay()
+        want = run(i, *eager)
+        assert all(torch.equal(p, q) for p, q in zip(out, want))
+        assert all(torch.equal(p, q) for p, q in zip(tables, eager))
+
+
+def test_first_calls_of_a_process_in_a_capture():
+    """Nothing has been loaded or allowed yet when the capture begins; the rows need more than 48 KB of shared memory."""
+    code = """
+import torch
+from ttt_tk_b200 import glue, ssm
+o, gx = (torch.randn(3, 8188, device="cuda") for _ in range(2))
+w = torch.rand(8188, device="cuda") + 0.5
+x = torch.randn(2, 300, 64, device="cuda"); c = torch.randn(64, 4, device="cuda")
+A = -torch.rand(64, 16, device="cuda"); B = torch.randn(2, 300, 1, 16, device="cuda")
+def run():
+    z, n, st = glue.norm_gate_residual(o, o, o, post_weight=w, scale=w, pre_weight=w, return_stats=True)
+    g = glue.norm_gate_residual_backward(gx, n, o, st, o, o, post_weight=w, scale=w, pre_weight=w)
+    y, ck = ssm.ssm_scan(ssm.short_conv(x, c), x, A, B, B, return_checkpoints=True)
+    s = ssm.ssm_scan_backward(y, x, x, A, B, B, ck)
+    return [t for t in (z, n, *g, y, *s, *ssm.short_conv_backward(y, x, c)) if t is not None]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = run()
+graph.replay()
+want = run()
+torch.cuda.synchronize()
+assert all(torch.equal(p, q) and torch.isfinite(p).all() for p, q in zip(got, want))
+print("as eager")
+"""
+    root = os.path.join(os.path.dirname(__file__), "..")
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "as eager" in r.stdout, r.stderr[-2000:]
+
+
+def test_conv_and_block_end_on_streams_of_their_own():
+    i = conv_inputs(5, "bf16", 2, 700, 512, 4, DEV)
+    w = torch.ones(512, device=DEV)
+
+    def run():
+        u = ssm.short_conv(i["x"], i["weight"], i["bias"], activation="silu", state=i["state"])
+        z, n, st = glue.norm_gate_residual(u, i["x"], i["gy"], return_stats=True, post_weight=w, scale=w, pre_weight=w)
+        g = glue.norm_gate_residual_backward(z, n, u, st, i["x"], i["gy"], post_weight=w, scale=w, pre_weight=w)
+        return [u, z, n, *[t for t in g if t is not None],
+                *ssm.short_conv_backward(g[0], i["x"], i["weight"], i["bias"], activation="silu", state=i["state"])]
+
+    want = run()
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(6):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(run())
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for o in outs for p, q in zip(o, want))
