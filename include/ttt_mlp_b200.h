@@ -462,6 +462,43 @@ uint64_t ttt_b200_ssm_scan_scratch_bytes(const ttt_b200_scan_args* args, int bac
 /* One token per row; slots as in ttt_b200_short_conv_step. */
 int ttt_b200_ssm_scan_step(const ttt_b200_scan_args* args, void* stream);
 
+/* Gated linear recurrence over D channels, one state to a channel:
+ *   s = sigmoid(gate + gate_bias);  log a = min(A, 0) s, with A NULL a = s;  b = sqrt(1 - a^2), 1 - a or 1 (mix);
+ *   h[d] = a h[d] + b sigmoid(input_gate + input_bias) x[d]  (input_gate NULL: a h + b x);  y = h.   A finite. */
+enum { TTT_B200_GATED_INTERVAL = 64 /* tokens between two checkpoints */ };
+enum { TTT_B200_MIX_NONE = 0, TTT_B200_MIX_SQRT = 1, TTT_B200_MIX_LINEAR = 2 };
+typedef struct ttt_b200_gated_args {
+  const void *x, *gate, *input_gate; /* [B][T][D], strides; step: [B][D], strides [0]; input_gate or NULL */
+  const float *A, *gate_bias, *input_bias; /* [D] or NULL */
+  const float* state;         /* [B][D] or NULL (zeros) */
+  const int32_t* lengths;     /* [B] or NULL */
+  void* y;                    /* [B][T][D]; step: [B][D] */
+  float* final_state;         /* [B][D] or NULL */
+  float* checkpoints;         /* [B][ceil(T / 64)][D]: states before every 64th token, for the backward; forward: or NULL.  Those of tokens
+                               * behind a sequence are neither written nor read */
+  /* backward: the inputs and the checkpoints above, and */
+  const void* grad_y;         /* [B][T][D], strides gy_stride */
+  const float* grad_final_state; /* [B][D] or NULL */
+  void *grad_x, *grad_gate, *grad_input; /* [B][T][D]; grad_input NULL where there is no input_gate */
+  float *grad_A, *grad_gate_bias, *grad_input_bias; /* [D] or NULL (not wanted) */
+  float* grad_state;          /* [B][D] or NULL */
+  /* backward with `group` 32, 64 or 128: x and the gates are e4m3 bytes of contiguous rows, with a scale for each `group` channels */
+  const float *x_scales, *gate_scales, *input_scales; /* [B][T][ceil(D / group)] */
+  void* scratch;              /* ttt_b200_gated_scan_scratch_bytes, 16-byte aligned */
+  uint64_t scratch_bytes;
+  /* step: the table of states, and which of its rows each row of the batch has */
+  float* state_io;            /* [rows][D], updated in place */
+  const int32_t* slots;       /* [B] or NULL (row b has state b, rows = B) */
+  int64_t x_stride[2], gate_stride[2], input_stride[2], gy_stride[2];
+  int32_t B, T, D, rows, dtype, mix, group;
+} ttt_b200_gated_args;
+int ttt_b200_gated_scan(const ttt_b200_gated_args* args, void* stream);
+int ttt_b200_gated_scan_backward(const ttt_b200_gated_args* args, void* stream);
+/* Bytes of scratch the backward needs: the sums' parts, 12 bytes per channel, sequence and CTA along it (at most 8). */
+uint64_t ttt_b200_gated_scan_scratch_bytes(const ttt_b200_gated_args* args);
+/* One token per row; slots as in ttt_b200_short_conv_step. */
+int ttt_b200_gated_scan_step(const ttt_b200_gated_args* args, void* stream);
+
 /* The end of a block and the start of the next: u = Norm(o) post_weight + post_bias;  x' = residual + scale u act(gate);
  * n = Norm(x') pre_weight + pre_bias.  Norm: (v - mean) / sqrt(var + eps) (layer) or v / sqrt(mean(v^2) + eps).  Each part is left out
  * with its pointer NULL: post_weight (u = o), gate, scale, residual (x' = the rest), pre_weight (no n).  The residual stream has the

@@ -242,6 +242,42 @@ def ssm_scan(x, dt, A, B, C, D=None, dt_bias=None, *, softplus=True, state=None,
     return (y, end) if return_state else y
 
 
+class GatedScanFunction(torch.autograd.Function):
+    """(y, final state or None) = f(x, gate, A, input_gate, gate_bias, input_bias, state, mix, lengths, return_state, recorded); `recorded` as in
+    `SSMScanFunction`."""
+
+    @staticmethod
+    def forward(ctx, x, gate, A, input_gate, gate_bias, input_bias, state, mix, lengths, return_state, recorded=True):
+        from . import ssm
+        x, gate, input_gate = (_rows(t) for t in (x, gate, input_gate))
+        A, gate_bias, input_bias, state = (_whole(t) for t in (A, gate_bias, input_bias, state))
+        keep = recorded and any(ctx.needs_input_grad)
+        r = ssm.gated_scan(x, gate, A, input_gate, gate_bias, input_bias, mix=mix, state=state, lengths=lengths, return_state=return_state,
+                           return_checkpoints=keep)
+        r = r if isinstance(r, tuple) else (r,)
+        if keep:
+            ctx.save_for_backward(x, gate, A, input_gate, gate_bias, input_bias, lengths, r[-1])
+        ctx.mix, ctx.has_state = mix, state is not None
+        ctx.set_materialize_grads(False)
+        return r[0], r[1] if return_state else None
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy, gf):
+        from . import ssm
+        x, gate, A, input_gate, gate_bias, input_bias, lengths, ck = ctx.saved_tensors
+        gy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if gy is None else _rows(gy)
+        g = ssm.gated_scan_backward(gy, x, gate, ck, A, input_gate, gate_bias, input_bias, mix=ctx.mix, lengths=lengths,
+                                    grad_final_state=_whole(gf))
+        return g[:6] + (g[6] if ctx.has_state else None,) + (None,) * 4
+
+
+def gated_scan(x, gate, A=None, input_gate=None, gate_bias=None, input_bias=None, *, mix="sqrt", state=None, lengths=None, return_state=False):
+    """Differentiable `ttt_tk_b200.ssm.gated_scan`; where gradients are recorded, the checkpoints are kept for the backward."""
+    y, end = GatedScanFunction.apply(x, gate, A, input_gate, gate_bias, input_bias, state, mix, lengths, return_state, torch.is_grad_enabled())
+    return (y, end) if return_state else y
+
+
 class NormGateResidualFunction(torch.autograd.Function):
     """(x, n or None) = f(o, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias, norm, activation, eps); o, residual and
     gate [tokens, D]."""

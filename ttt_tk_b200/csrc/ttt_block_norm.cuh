@@ -16,7 +16,6 @@
 #pragma once
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "ttt_elem.cuh"
@@ -372,22 +371,6 @@ inline int parts_of(const ttt_b200_block_args& p) {
   return p.residual && p.pre_weight && !p.gate && !p.post_weight && !p.scale ? kBare : kSome;
 }
 
-// More dynamic shared memory than 48 KB has to be asked for, per kernel and device.  All that there is is asked for, once: a limit of a
-// call's own would be lowered by a smaller call of another host thread between this call's asking and its launch.
-template <auto kKernel> int allow_shared() {
-  static std::atomic<uint64_t> done{0};      // a bit for each device
-  int dev = 0, most = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;      // (beyond 64 devices: every time the same)
-  if (e == cudaSuccess && (done.load(std::memory_order_acquire) & bit)) return TTT_B200_OK;
-  cudaFuncAttributes own = {};
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
-  if (e == cudaSuccess) e = cudaFuncGetAttributes(&own, kKernel);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - static_cast<int>(own.sharedSizeBytes));
-  if (e != cudaSuccess) return ttt_set_error(TTT_B200_ERR_LAUNCH, cudaGetErrorString(e));
-  done.fetch_or(bit, std::memory_order_release);
-  return TTT_B200_OK;
-}
 template <auto kKernel> int launch(const Plan& q, size_t bytes, cudaStream_t s, const ttt_b200_block_args& p, const char* what) {
   if (bytes > 40 * 1024)      // (with the static part 48 KB is the most without asking)
     if (int rc = allow_shared<kKernel>()) return rc;

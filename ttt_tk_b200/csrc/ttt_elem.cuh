@@ -8,6 +8,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "ttt_internal.h"
 
 namespace ttt {
@@ -161,6 +163,22 @@ inline int launched(const char* what) {
   static thread_local char buf[160];
   snprintf(buf, sizeof buf, "%s: %s", what, cudaGetErrorString(e));
   return ttt_set_error(TTT_B200_ERR_LAUNCH, buf);
+}
+// More dynamic shared memory than 48 KB has to be asked for, per kernel and device.  All that there is is asked for, once: a limit of a
+// call's own would be lowered by a smaller call of another host thread between this call's asking and its launch.
+template <auto kKernel> int allow_shared() {
+  static std::atomic<uint64_t> done{0};      // a bit for each device
+  int dev = 0, most = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;      // (beyond 64 devices: every time the same)
+  if (e == cudaSuccess && (done.load(std::memory_order_acquire) & bit)) return TTT_B200_OK;
+  cudaFuncAttributes own = {};
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&own, kKernel);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - static_cast<int>(own.sharedSizeBytes));
+  if (e != cudaSuccess) return ttt_set_error(TTT_B200_ERR_LAUNCH, cudaGetErrorString(e));
+  done.fetch_or(bit, std::memory_order_release);
+  return TTT_B200_OK;
 }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 

@@ -461,6 +461,160 @@ PyObject* scan_step(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
   });
 }
 
+// ---- gated linear recurrence -------------------------------------------------------------------------------------------------
+int64_t gated_checkpoints_of(const ttt_b200_gated_args& a) { return (static_cast<int64_t>(a.T) + TTT_B200_GATED_INTERVAL - 1) / TTT_B200_GATED_INTERVAL; }
+
+void gated_weights(Call& c, ttt_b200_gated_args& a, PyObject* A, PyObject* gate_bias, PyObject* input_bias, PyObject* mix, bool gated) {
+  a.A = c.f32(A, "A", {a.D});
+  a.gate_bias = c.f32(gate_bias, "gate_bias", {a.D});
+  a.input_bias = c.f32(input_bias, "input_bias", {a.D});
+  c.need(gated || !a.input_bias, "input_bias needs input_gate");
+  a.mix = static_cast<int32_t>(integer(mix));
+}
+
+// v = x, gate, A, input_gate, gate_bias, input_bias, mix; a step has no tokens' dimension
+void gated_inputs(Call& c, ttt_b200_gated_args& a, PyObject* const* v, bool step) {
+  const Tensor& x = *c.first(v[0], "x", step ? 2 : 3, step ? "[B, D]" : "[B, T, D]");
+  for (int64_t i = 0; i < x.dim(); ++i) c.sized(x.size(i), "a dimension of x");
+  a.B = static_cast<int32_t>(x.size(0));
+  a.T = step ? 1 : static_cast<int32_t>(x.size(1));
+  a.D = static_cast<int32_t>(x.size(-1));
+  c.need(a.D >= 1, "x has no channels");
+  a.dtype = c.dtype();
+  auto rows = [&](const Tensor& t, const void*& p, int64_t* stride) {
+    p = t.data_ptr();
+    stride[0] = step_of(t, 0);
+    if (!step) stride[1] = step_of(t, 1);
+  };
+  auto like = [&](PyObject* o, const char* name) -> const Tensor& { return step ? *c.act(o, name, {a.B, a.D}) : *c.act(o, name, {a.B, a.T, a.D}); };
+  rows(x, a.x, a.x_stride);
+  rows(like(v[1], "gate"), a.gate, a.gate_stride);
+  if (v[3] != Py_None) rows(like(v[3], "input_gate"), a.input_gate, a.input_stride);
+  gated_weights(c, a, v[2], v[4], v[5], v[6], v[3] != Py_None);
+}
+
+// gated(x, gate, A, input_gate, gate_bias, input_bias, mix, state, lengths, want_state, want_checkpoints) -> (y, final state or None, checkpoints or None)
+PyObject* gated(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  return guarded("gated", nargs, 11, [&]() -> PyObject* {
+    Call c("gated_scan");
+    ttt_b200_gated_args a = {};
+    gated_inputs(c, a, v, false);
+    a.state = c.f32(v[7], "state", {a.B, a.D});
+    a.lengths = c.i32(v[8], "lengths", a.B);
+    const c10::Device dev = c.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    const auto opt = at::TensorOptions().dtype(c.type()).device(dev), f32 = opt.dtype(at::kFloat);
+    const bool none = a.B == 0 || a.T == 0;
+    const Tensor y = at::empty({a.B, a.T, a.D}, opt);
+    Tensor end, ck;
+    if (truth(v[9])) {
+      if (!none) end = at::empty({a.B, a.D}, f32);
+      else end = a.state ? THPVariable_Unpack(v[7]).detach().clone() : at::zeros({a.B, a.D}, f32);
+    }
+    if (truth(v[10])) ck = at::empty({a.B, gated_checkpoints_of(a), a.D}, f32);
+    a.y = y.data_ptr();
+    a.final_state = fptr(end);
+    a.checkpoints = fptr(ck);
+    if (!none) launch(ttt_b200_gated_scan, a, dev);
+    return tuple_of({y, end, ck});
+  });
+}
+
+// 8-bit values of a backward pass, as (values, scales); the first of a call sets the group
+const Tensor& kept(Call& c, ttt_b200_gated_args& a, PyObject* o, const char* name, const void*& p, int64_t* stride, const float*& scales) {
+  const std::string n = name;
+  c.need(PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 2, (n + " must be (values, scales), as the other inputs").c_str());
+  const Tensor& q = *c.shaped(PyTuple_GET_ITEM(o, 0), name, at::kFloat8_e4m3fn, {a.B, a.T, a.D});
+  const Tensor& s = *c.any(PyTuple_GET_ITEM(o, 1), name);
+  c.need(q.is_contiguous() && s.is_contiguous(), (n + "'s values and scales must be contiguous").c_str());
+  int group = 0;
+  for (const int g : {32, 64, 128})
+    if (s.dim() == 3 && s.size(0) == a.B && s.size(1) == a.T && s.size(2) == (a.D + g - 1) / g && (!a.group || a.group == g)) group = g;
+  c.need(group && s.scalar_type() == at::kFloat, (n + "'s scales must be float32 [B, T, D / group], group 32, 64 or 128 and the same for all inputs").c_str());
+  a.group = group;
+  p = q.data_ptr();
+  scales = static_cast<const float*>(s.data_ptr());
+  stride[0] = static_cast<int64_t>(a.T) * a.D;
+  stride[1] = a.D;
+  return q;
+}
+
+// gated_backward(grad_y, x, gate, checkpoints, A, input_gate, gate_bias, input_bias, mix, lengths, grad_final_state)
+//   -> (grad_x, grad_gate, grad_A, grad_input_gate, grad_gate_bias, grad_input_bias, grad_state); x and the gates may be (values, scales) in 8 bits
+PyObject* gated_backward(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  return guarded("gated_backward", nargs, 11, [&]() -> PyObject* {
+    Call c("gated_scan_backward");
+    ttt_b200_gated_args a = {};
+    const Tensor* g;
+    if (PyTuple_Check(v[1])) {
+      g = c.first(v[0], "grad_y", 3, "[B, T, D]");
+      for (int i = 0; i < 3; ++i) c.sized(g->size(i), "a dimension of grad_y");
+      a.B = static_cast<int32_t>(g->size(0));
+      a.T = static_cast<int32_t>(g->size(1));
+      a.D = static_cast<int32_t>(g->size(2));
+      c.need(a.D >= 1, "grad_y has no channels");
+      a.dtype = c.dtype();
+      kept(c, a, v[1], "x", a.x, a.x_stride, a.x_scales);
+      kept(c, a, v[2], "gate", a.gate, a.gate_stride, a.gate_scales);
+      if (v[5] != Py_None) kept(c, a, v[5], "input_gate", a.input_gate, a.input_stride, a.input_scales);
+      gated_weights(c, a, v[4], v[6], v[7], v[8], v[5] != Py_None);
+    } else {
+      PyObject* const in[] = {v[1], v[2], v[4], v[5], v[6], v[7], v[8]};
+      gated_inputs(c, a, in, false);
+      g = c.act(v[0], "grad_y", {a.B, a.T, a.D});
+    }
+    a.grad_y = g->data_ptr();
+    a.gy_stride[0] = step_of(*g, 0);
+    a.gy_stride[1] = step_of(*g, 1);
+    a.checkpoints = c.weight(v[3], "checkpoints", {a.B, gated_checkpoints_of(a), a.D});
+    a.lengths = c.i32(v[9], "lengths", a.B);
+    a.grad_final_state = c.f32(v[10], "grad_final_state", {a.B, a.D});
+    const c10::Device dev = c.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    const auto opt = at::TensorOptions().dtype(c.type()).device(dev), f32 = opt.dtype(at::kFloat);
+    const bool none = a.B == 0 || a.T == 0;
+    auto sum = [&](const float* w) { return !w ? Tensor() : none ? at::zeros({a.D}, f32) : at::empty({a.D}, f32); };
+    const Tensor gx = at::empty({a.B, a.T, a.D}, opt), gg = at::empty({a.B, a.T, a.D}, opt);
+    const Tensor gi = v[5] != Py_None ? at::empty({a.B, a.T, a.D}, opt) : Tensor();
+    const Tensor gA = sum(a.A), gb = sum(a.gate_bias), gib = sum(a.input_bias);
+    Tensor gs;
+    if (none) {
+      gs = a.grad_final_state ? THPVariable_Unpack(v[10]).detach().clone() : at::zeros({a.B, a.D}, f32);
+    } else {
+      gs = at::empty({a.B, a.D}, f32);
+      const Tensor scratch = scratch_of(ttt_b200_gated_scan_scratch_bytes(&a), dev);
+      give(a, scratch);
+      a.grad_x = gx.data_ptr();
+      a.grad_gate = gg.data_ptr();
+      a.grad_input = ptr(gi);
+      a.grad_A = fptr(gA);
+      a.grad_gate_bias = fptr(gb);
+      a.grad_input_bias = fptr(gib);
+      a.grad_state = fptr(gs);
+      launch(ttt_b200_gated_scan_backward, a, dev);
+    }
+    return tuple_of({gx, gg, gA, gi, gb, gib, gs});
+  });
+}
+
+// gated_step(x, gate, A, input_gate, gate_bias, input_bias, mix, state, slots) -> y
+PyObject* gated_step(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  return guarded("gated_step", nargs, 9, [&]() -> PyObject* {
+    Call c("gated_scan_step");
+    ttt_b200_gated_args a = {};
+    gated_inputs(c, a, v, true);
+    a.rows = static_cast<int32_t>(table(c, v[7], 2, v[8], a.B));
+    a.state_io = c.f32(v[7], "state", {a.rows, a.D});
+    a.slots = c.i32(v[8], "slots", a.B);
+    const c10::Device dev = c.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    const Tensor y = at::empty({a.B, a.D}, at::TensorOptions().dtype(c.type()).device(dev));
+    a.y = y.data_ptr();
+    if (a.B > 0) launch(ttt_b200_gated_scan_step, a, dev);
+    return wrap(y);
+  });
+}
+
 // ---- block end -------------------------------------------------------------------------------------------------------------
 // rows [..., D] that are one after another at a fixed distance: that distance
 int64_t row_stride(const Call& c, const Tensor& t, const char* msg) {
@@ -594,6 +748,7 @@ PyObject* block_backward(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
 #define TTT_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {TTT_METHOD(conv),          TTT_METHOD(conv_backward), TTT_METHOD(conv_step), TTT_METHOD(scan),
                           TTT_METHOD(scan_backward), TTT_METHOD(scan_step),     TTT_METHOD(block),     TTT_METHOD(block_backward),
+                          TTT_METHOD(gated),         TTT_METHOD(gated_backward), TTT_METHOD(gated_step),
                           {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_ttt_layer_host", "Validation and launch of the layer-side sequence operators.", -1, kMethods,

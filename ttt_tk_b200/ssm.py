@@ -1,16 +1,19 @@
-"""Layer-side sequence operators with a state of their own (CUDA, `csrc/ttt_short_conv.cu`, `csrc/ttt_ssm_scan_sm100.cu`): the short
-causal convolution in front of a TTT layer's queries and keys or of a state space layer, and the selective state space scan that
-models mix with TTT layers.  Each for prompts, for training and for single tokens.
+"""Layer-side sequence operators with a state of their own (CUDA, `csrc/ttt_short_conv.cu`, `csrc/ttt_ssm_scan_sm100.cu`,
+`csrc/ttt_gated_scan_sm100.cu`): the short causal convolution in front of a TTT layer's queries and keys or of a recurrent layer, and the
+two recurrences that models mix with TTT layers, the selective state space scan and the gated linear recurrence.  Each for prompts, for
+training and for single tokens.
 
     y, state = short_conv(x, weight, bias, activation="silu", return_state=True)       # [B, T, D]
     y, state, ck = ssm_scan(x, dt, A, B, C, D, dt_bias, return_state=True, return_checkpoints=True)
     y = short_conv_step(x, state, weight, bias, activation="silu", slots=slots)        # [B, D], one token; `state` in place
     y = ssm_scan_step(x, dt, A, B, C, state, D, dt_bias, slots=slots)
+    y, state, ck = gated_scan(x, gate, A, input_gate, return_state=True, return_checkpoints=True)
+    y = gated_scan_step(x, gate, state, A, input_gate, slots=slots)
 
 Activations are bf16, fp16 or fp32 (all of a call the same), with any strides but the innermost, so that a slice of a projection's
 output can be passed as it is; weights, biases, A, D, scan states and checkpoints are contiguous fp32.  Everything between reading and
 writing is fp32, and sums have a fixed order: the same call gives the same bits.  Calls are stream-ordered and do not synchronise.
-A bad argument raises ValueError.  Differentiable forms: `ttt_tk_b200.autograd.short_conv` and `ssm_scan`.
+A bad argument raises ValueError.  Differentiable forms: `ttt_tk_b200.autograd.short_conv`, `ssm_scan` and `gated_scan`.
 
 `lengths` (int32 [B], on the GPU): a right-padded batch.  Tokens from a sequence's length on are not read, whatever they hold; their
 outputs and gradients are zero and they change no state.
@@ -23,6 +26,7 @@ from .build import load_layer_host
 
 _HOST = None
 _ACTIVATIONS = {None: 0, "silu": 1}
+_MIXES = {None: 0, "sqrt": 1, "linear": 2}
 
 
 def _host():
@@ -39,6 +43,12 @@ def _activation(name):
     if not (name is None or isinstance(name, str)) or name not in _ACTIVATIONS:
         raise ValueError(f"activation must be None or 'silu', got {name!r}")
     return _ACTIVATIONS[name]
+
+
+def _mix(name):
+    if not (name is None or isinstance(name, str)) or name not in _MIXES:
+        raise ValueError(f"mix must be None, 'sqrt' or 'linear', got {name!r}")
+    return _MIXES[name]
 
 
 def short_conv(x, weight, bias=None, *, activation=None, state=None, lengths=None, heads=False, return_state=False):
@@ -99,3 +109,37 @@ def ssm_scan_step(x, dt, A, B, C, state, D=None, dt_bias=None, *, softplus=True,
     """`ssm_scan` of one token per row: `x`, `dt` [batch, D]; `B`, `C` [batch, G, N]; `state` fp32 [batch, D, N], or with `slots` a
     table [S, D, N], is updated in place.  Returns y [batch, D]."""
     return _host().scan_step(x, dt, A, B, C, D, dt_bias, softplus, state, slots)
+
+
+def gated_scan(x, gate, A=None, input_gate=None, gate_bias=None, input_bias=None, *, mix="sqrt", state=None, lengths=None,
+               return_state=False, return_checkpoints=False):
+    """Gated linear recurrence, one state to a channel:
+
+        s = sigmoid(gate + gate_bias);  log a = min(A[d], 0) s, without A: a = s
+        h[d] = a h[d] + b sigmoid(input_gate + input_bias) x[d];  y[d] = h[d]
+
+    with b = sqrt(1 - a^2) (`mix` "sqrt", under which inputs of unit variance have states of unit variance), 1 - a ("linear", a running
+    mean) or 1 (None).  `x`, `gate`, `input_gate` [batch, T, D] (without an input gate: h = a h + b x); `A`, finite, and the biases fp32 [D];
+    `state` fp32 [batch, D] in front of the first token (zeros without it).  A gate of -inf holds the state, and with a mix lets no
+    input in (with A; without A it forgets the state).  Returns y [batch, T, D], followed by the state behind each sequence's last token
+    where `return_state` asks for it, and by the states before every 64th token, fp32 [batch, ceil(T / 64), D], that `gated_scan_backward`
+    starts from, where `return_checkpoints` does (those behind a sequence's end hold nothing)."""
+    y, end, ck = _host().gated(x, gate, A, input_gate, gate_bias, input_bias, _mix(mix), state, lengths, return_state, return_checkpoints)
+    if not (return_state or return_checkpoints):
+        return y
+    return (y,) + ((end,) if return_state else ()) + ((ck,) if return_checkpoints else ())
+
+
+def gated_scan_backward(grad_y, x, gate, checkpoints, A=None, input_gate=None, gate_bias=None, input_bias=None, *, mix="sqrt", lengths=None,
+                        grad_final_state=None):
+    """Gradients of `gated_scan` from its inputs and checkpoints: (grad_x, grad_gate, grad_A, grad_input_gate, grad_gate_bias,
+    grad_input_bias, grad_state); None where there is no such input.  Those of the activations have their type, the others are fp32;
+    grad_state fp32 [batch, D] is that of the state in front of the first token.  Where 1 - a^2 is below the least normal fp32 the slope of its root counts as 0,
+    and where A is above 0 so does grad_A."""
+    return _host().gated_backward(grad_y, x, gate, checkpoints, A, input_gate, gate_bias, input_bias, _mix(mix), lengths, grad_final_state)
+
+
+def gated_scan_step(x, gate, state, A=None, input_gate=None, gate_bias=None, input_bias=None, *, mix="sqrt", slots=None):
+    """`gated_scan` of one token per row: `x`, `gate`, `input_gate` [batch, D]; `state` fp32 [batch, D], or with `slots` a table [S, D], is
+    updated in place.  Returns y [batch, D]."""
+    return _host().gated_step(x, gate, A, input_gate, gate_bias, input_bias, _mix(mix), state, slots)
