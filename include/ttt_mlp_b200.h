@@ -523,6 +523,55 @@ int ttt_b200_norm_gate_residual(const ttt_b200_block_args* args, void* stream);
 int ttt_b200_norm_gate_residual_backward(const ttt_b200_block_args* args, void* stream);
 uint64_t ttt_b200_norm_gate_residual_scratch_bytes(const ttt_b200_block_args* args);
 
+/* ---- Activations in 8 bits ----
+ * Of each `group` (32, 64 or 128) neighbouring values of a row one fp32 scale, the least power of two with max |v| <= 448 scale (of the finite
+ * values; at least 2^-126), and v / scale in e4m3, ties to even; infinities become 448 scale, NaN stays.  One to four tensors of the same shape. */
+enum { TTT_B200_PACK8_TENSORS = 4 };
+typedef struct ttt_b200_pack8_args {
+  const void* src[TTT_B200_PACK8_TENSORS];  /* pack: [M][D], strides */
+  void* values[TTT_B200_PACK8_TENSORS];     /* [M][D] e4m3; unpack reads them */
+  float* scales[TTT_B200_PACK8_TENSORS];    /* [M][ceil(D / group)] */
+  void* dst[TTT_B200_PACK8_TENSORS];        /* unpack: [M][D], contiguous */
+  int64_t stride[TTT_B200_PACK8_TENSORS];
+  int64_t M;
+  int32_t D, dtype /* of src or dst */, group /* unpack: 0 for one scale to a row */, count;
+} ttt_b200_pack8_args;
+int ttt_b200_pack8(const ttt_b200_pack8_args* args, void* stream);
+int ttt_b200_unpack8(const ttt_b200_pack8_args* args, void* stream);
+
+/* x' = residual + o;  n = Norm(x') weight + bias, left in 8 bits as above, with a scale to each `group` values or to the whole row (group 0).
+ * Norms, types and the residual stream as in ttt_b200_norm_gate_residual; without a residual x' = o and is not written.  1 <= D <= 8192. */
+typedef struct ttt_b200_norm8_args {
+  const void *o, *residual;   /* [M][D], strides; residual or NULL */
+  const float *weight, *bias; /* [D]; bias or NULL */
+  void* x;                    /* [M][D], of the residual's type */
+  void* values;               /* [M][D] e4m3 */
+  float* scales;              /* [M][ceil(D / group)] or [M] */
+  float* stats;               /* [M][4] or NULL: what ttt_b200_norm_gate_residual_backward takes */
+  int64_t o_stride, residual_stride;
+  int64_t M;
+  int32_t D, dtype, residual_fp32, layer, group;
+  float eps;
+} ttt_b200_norm8_args;
+int ttt_b200_norm_residual_8bit(const ttt_b200_norm8_args* args, void* stream);
+
+/* ---- Rows of tables of states ---- up to 16 tables with the same number of rows, each contiguous, not overlapping one another. */
+enum { TTT_B200_TABLES = 16, TTT_B200_TABLE_PAIRS = 4096 };
+typedef struct ttt_b200_tables_args {
+  void* table[TTT_B200_TABLES];
+  int64_t row_bytes[TTT_B200_TABLES];
+  const int32_t *source, *target; /* [pairs]; clear: the rows are `target` */
+  const uint8_t* used;            /* compact: [rows], not 0: in use */
+  int32_t* place;                 /* compact: [rows], where each used row is now, -1 for the others */
+  int32_t count, rows, pairs;
+} ttt_b200_tables_args;
+/* table[target[i]] = table[source[i]], all rows read before one is written; pairs with an index that is no row do nothing; of several pairs with
+ * the same target the last one counts. */
+int ttt_b200_copy_rows(const ttt_b200_tables_args* args, void* stream);
+int ttt_b200_clear_rows(const ttt_b200_tables_args* args, void* stream);
+/* Of n used rows the k-th from row n on moves to the k-th unused one in front of it; what is left behind stays as it is.  At most 8192 rows. */
+int ttt_b200_compact_rows(const ttt_b200_tables_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

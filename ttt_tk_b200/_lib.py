@@ -72,6 +72,8 @@ EXPORTS = ["ttt_b200_forward", "ttt_b200_linear_forward", "ttt_b200_linear_backw
            "ttt_b200_short_conv", "ttt_b200_short_conv_backward", "ttt_b200_short_conv_step", "ttt_b200_short_conv_scratch_bytes",
            "ttt_b200_ssm_scan", "ttt_b200_ssm_scan_backward", "ttt_b200_ssm_scan_step", "ttt_b200_ssm_scan_scratch_bytes",
            "ttt_b200_gated_scan", "ttt_b200_gated_scan_backward", "ttt_b200_gated_scan_step", "ttt_b200_gated_scan_scratch_bytes",
+           "ttt_b200_pack8", "ttt_b200_unpack8", "ttt_b200_norm_residual_8bit", "ttt_b200_copy_rows", "ttt_b200_clear_rows",
+           "ttt_b200_compact_rows",
            "ttt_b200_norm_gate_residual", "ttt_b200_norm_gate_residual_backward", "ttt_b200_norm_gate_residual_scratch_bytes"]
 
 FLAG_SYNC = 1

@@ -172,15 +172,51 @@ def _tokens(t):
     return t.unsqueeze(0) if t.dim() == 1 else t.flatten(0, -2)
 
 
+# `saved`: what a forward keeps of its activations for the backward, None for themselves or "e4m3" for 8 bits (`ttt_tk_b200.saved`).
+def _saved(name):
+    if not (name is None or isinstance(name, str)) or name not in (None, "e4m3"):
+        raise ValueError(f"saved must be None or 'e4m3', got {name!r}")
+    return name is not None and torch.is_grad_enabled()
+
+
+def _even(t):
+    """With rows at a fixed distance."""
+    at_all = t.dim() < 3 or t.size(0) <= 1 or t.size(1) <= 1 or t.stride(0) == t.stride(1) * t.size(1)
+    return t if at_all else t.contiguous()
+
+
+def _pack(*ts):
+    """Tensors of one shape (None among them) in 8 bits, flat: values, scales, values, ...; those of one type in one launch."""
+    from .saved import pack8
+    flat = [None] * (2 * len(ts))
+    for ty in {t.dtype for t in ts if t is not None}:
+        at = [k for k, t in enumerate(ts) if t is not None and t.dtype == ty]
+        for k, p in zip(at, pack8(*[_even(ts[k]) for k in at])):
+            flat[2 * k], flat[2 * k + 1] = p
+    return flat
+
+
+def _unpack(flat, types):
+    """And back, in their types."""
+    from .saved import unpack8
+    ts = [None] * len(types)
+    for ty in set(types) - {None}:
+        at = [k for k, t in enumerate(types) if t == ty]
+        for k, t in zip(at, unpack8(*[(flat[2 * k], flat[2 * k + 1]) for k in at], dtype=ty)):
+            ts[k] = t
+    return ts
+
+
 class ShortConvFunction(torch.autograd.Function):
-    """(y, final state or None) = f(x, weight, bias, state, activation, lengths, heads, return_state)."""
+    """(y, final state or None) = f(x, weight, bias, state, activation, lengths, heads, return_state, packed)."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, state, activation, lengths, heads, return_state):
+    def forward(ctx, x, weight, bias, state, activation, lengths, heads, return_state, packed=False):
         from . import ssm
         x, weight, bias, state = _rows(x), _whole(weight), _whole(bias), _whole(state)
         r = ssm.short_conv(x, weight, bias, activation=activation, state=state, lengths=lengths, heads=heads, return_state=return_state)
-        ctx.save_for_backward(x, weight, bias, state, lengths)
+        ctx.packed = x.dtype if packed and any(ctx.needs_input_grad) else None
+        ctx.save_for_backward(weight, bias, state, lengths, *([x] if ctx.packed is None else _pack(x)))
         ctx.kw = dict(activation=activation, heads=heads)
         ctx.set_materialize_grads(False)
         return r if return_state else (r, None)
@@ -189,29 +225,30 @@ class ShortConvFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gy, gf):
         from . import ssm
-        x, weight, bias, state, lengths = ctx.saved_tensors
+        weight, bias, state, lengths, *kept = ctx.saved_tensors
+        (x,) = kept if ctx.packed is None else _unpack(kept, [ctx.packed])
         if gy is None:
             B, T, D = x.shape
             gy = x.new_zeros((B, D // 64, T // 64, 64, 64) if ctx.kw["heads"] else (B, T, D))
         gy = _whole(gy) if ctx.kw["heads"] else _rows(gy)
         g = ssm.short_conv_backward(gy, x, weight, bias, state=state, lengths=lengths, grad_final_state=_whole(gf), **ctx.kw)
-        return g + (None,) * 4
+        return g + (None,) * 5
 
 
-def short_conv(x, weight, bias=None, *, activation=None, state=None, lengths=None, heads=False, return_state=False):
-    """Differentiable `ttt_tk_b200.ssm.short_conv`."""
-    y, end = ShortConvFunction.apply(x, weight, bias, state, activation, lengths, heads, return_state)
+def short_conv(x, weight, bias=None, *, activation=None, state=None, lengths=None, heads=False, return_state=False, saved=None):
+    """Differentiable `ttt_tk_b200.ssm.short_conv`.  `saved` "e4m3": x is kept in 8 bits, and the gradients are those at what was kept."""
+    y, end = ShortConvFunction.apply(x, weight, bias, state, activation, lengths, heads, return_state, _saved(saved))
     return (y, end) if return_state else y
 
 
 class SSMScanFunction(torch.autograd.Function):
-    """(y, final state or None) = f(x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state, recorded).
+    """(y, final state or None) = f(x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state, recorded, packed).
 
     `recorded`: whether gradients are recorded where it is called, which is not to be seen inside `forward` (and `needs_input_grad` says
     what the inputs ask for, recorded or not): the checkpoints, fp32 [batch, T / 16, D, N], are written for a backward that can come."""
 
     @staticmethod
-    def forward(ctx, x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state, recorded=True):
+    def forward(ctx, x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state, recorded=True, packed=False):
         from . import ssm
         x, dt, B, C = (_rows(t) for t in (x, dt, B, C))
         A, D, dt_bias, state = (_whole(t) for t in (A, D, dt_bias, state))
@@ -219,8 +256,9 @@ class SSMScanFunction(torch.autograd.Function):
         r = ssm.ssm_scan(x, dt, A, B, C, D, dt_bias, softplus=softplus, state=state, lengths=lengths, return_state=return_state,
                          return_checkpoints=keep)
         r = r if isinstance(r, tuple) else (r,)
+        ctx.packed = x.dtype if packed else None
         if keep:
-            ctx.save_for_backward(x, dt, A, B, C, D, dt_bias, lengths, r[-1])
+            ctx.save_for_backward(A, B, C, D, dt_bias, lengths, r[-1], *(_pack(x, dt) if packed else (x, dt)))
         ctx.softplus, ctx.has_state = softplus, state is not None
         ctx.set_materialize_grads(False)
         return r[0], r[1] if return_state else None
@@ -229,25 +267,27 @@ class SSMScanFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gy, gf):
         from . import ssm
-        x, dt, A, B, C, D, dt_bias, lengths, ck = ctx.saved_tensors
+        A, B, C, D, dt_bias, lengths, ck, *kept = ctx.saved_tensors
+        x, dt = kept if ctx.packed is None else _unpack(kept, [ctx.packed] * 2)
         gy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if gy is None else _rows(gy)
         g = ssm.ssm_scan_backward(gy, x, dt, A, B, C, ck, D, dt_bias, softplus=ctx.softplus, lengths=lengths,
                                   grad_final_state=_whole(gf))
-        return g[:7] + (g[7] if ctx.has_state else None,) + (None,) * 4
+        return g[:7] + (g[7] if ctx.has_state else None,) + (None,) * 5
 
 
-def ssm_scan(x, dt, A, B, C, D=None, dt_bias=None, *, softplus=True, state=None, lengths=None, return_state=False):
-    """Differentiable `ttt_tk_b200.ssm.ssm_scan`; where gradients are recorded, the checkpoints are kept for the backward."""
-    y, end = SSMScanFunction.apply(x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state, torch.is_grad_enabled())
+def ssm_scan(x, dt, A, B, C, D=None, dt_bias=None, *, softplus=True, state=None, lengths=None, return_state=False, saved=None):
+    """Differentiable `ttt_tk_b200.ssm.ssm_scan`; where gradients are recorded, the checkpoints are kept for the backward.  `saved` "e4m3": x and dt are
+    kept in 8 bits, and the gradients are those at what was kept, with the checkpoints as the forward has them."""
+    y, end = SSMScanFunction.apply(x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state, torch.is_grad_enabled(), _saved(saved))
     return (y, end) if return_state else y
 
 
 class GatedScanFunction(torch.autograd.Function):
-    """(y, final state or None) = f(x, gate, A, input_gate, gate_bias, input_bias, state, mix, lengths, return_state, recorded); `recorded` as in
-    `SSMScanFunction`."""
+    """(y, final state or None) = f(x, gate, A, input_gate, gate_bias, input_bias, state, mix, lengths, return_state, recorded, packed);
+    `recorded` as in `SSMScanFunction`."""
 
     @staticmethod
-    def forward(ctx, x, gate, A, input_gate, gate_bias, input_bias, state, mix, lengths, return_state, recorded=True):
+    def forward(ctx, x, gate, A, input_gate, gate_bias, input_bias, state, mix, lengths, return_state, recorded=True, packed=False):
         from . import ssm
         x, gate, input_gate = (_rows(t) for t in (x, gate, input_gate))
         A, gate_bias, input_bias, state = (_whole(t) for t in (A, gate_bias, input_bias, state))
@@ -256,8 +296,8 @@ class GatedScanFunction(torch.autograd.Function):
                            return_checkpoints=keep)
         r = r if isinstance(r, tuple) else (r,)
         if keep:
-            ctx.save_for_backward(x, gate, A, input_gate, gate_bias, input_bias, lengths, r[-1])
-        ctx.mix, ctx.has_state = mix, state is not None
+            ctx.save_for_backward(A, gate_bias, input_bias, lengths, r[-1], *(_pack(x, gate, input_gate) if packed else (x, gate, input_gate)))
+        ctx.mix, ctx.has_state, ctx.like = mix, state is not None, (x.shape, x.dtype, x.device)
         ctx.set_materialize_grads(False)
         return r[0], r[1] if return_state else None
 
@@ -265,31 +305,40 @@ class GatedScanFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gy, gf):
         from . import ssm
-        x, gate, A, input_gate, gate_bias, input_bias, lengths, ck = ctx.saved_tensors
-        gy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if gy is None else _rows(gy)
+        A, gate_bias, input_bias, lengths, ck, *kept = ctx.saved_tensors
+        if len(kept) == 6:      # in 8 bits, which the backward takes as they are
+            kept = [(kept[k], kept[k + 1]) if kept[k] is not None else None for k in (0, 2, 4)]
+        x, gate, input_gate = kept
+        shape, dtype, device = ctx.like
+        gy = torch.zeros(shape, dtype=dtype, device=device) if gy is None else _rows(gy)
         g = ssm.gated_scan_backward(gy, x, gate, ck, A, input_gate, gate_bias, input_bias, mix=ctx.mix, lengths=lengths,
                                     grad_final_state=_whole(gf))
-        return g[:6] + (g[6] if ctx.has_state else None,) + (None,) * 4
+        return g[:6] + (g[6] if ctx.has_state else None,) + (None,) * 5
 
 
-def gated_scan(x, gate, A=None, input_gate=None, gate_bias=None, input_bias=None, *, mix="sqrt", state=None, lengths=None, return_state=False):
-    """Differentiable `ttt_tk_b200.ssm.gated_scan`; where gradients are recorded, the checkpoints are kept for the backward."""
-    y, end = GatedScanFunction.apply(x, gate, A, input_gate, gate_bias, input_bias, state, mix, lengths, return_state, torch.is_grad_enabled())
+def gated_scan(x, gate, A=None, input_gate=None, gate_bias=None, input_bias=None, *, mix="sqrt", state=None, lengths=None, return_state=False,
+               saved=None):
+    """Differentiable `ttt_tk_b200.ssm.gated_scan`; where gradients are recorded, the checkpoints are kept for the backward.  `saved` "e4m3": x and the
+    gates are kept in 8 bits, and the gradients are those at what was kept, with the checkpoints as the forward has them."""
+    y, end = GatedScanFunction.apply(x, gate, A, input_gate, gate_bias, input_bias, state, mix, lengths, return_state, torch.is_grad_enabled(),
+                                     _saved(saved))
     return (y, end) if return_state else y
 
 
 class NormGateResidualFunction(torch.autograd.Function):
-    """(x, n or None) = f(o, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias, norm, activation, eps); o, residual and
-    gate [tokens, D]."""
+    """(x, n or None) = f(o, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias, norm, activation, eps, packed); o,
+    residual and gate [tokens, D]."""
 
     @staticmethod
-    def forward(ctx, o, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias, norm, activation, eps):
+    def forward(ctx, o, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias, norm, activation, eps, packed=False):
         from .glue import norm_gate_residual as run
         o, residual, gate = (_rows(t) for t in (o, residual, gate))
         weights = [_whole(t) for t in (post_weight, post_bias, scale, pre_weight, pre_bias)]
         ctx.kw = dict(norm=norm, activation=activation, eps=eps)
         x, n, stats = run(o, residual, gate, **dict(zip(_BLOCK_WEIGHTS, weights)), return_stats=True, **ctx.kw)
-        ctx.save_for_backward(o, residual, gate, stats, *weights)
+        kept = [o, residual, gate]
+        ctx.packed = [None if t is None else t.dtype for t in kept] if packed and any(ctx.needs_input_grad) else None
+        ctx.save_for_backward(stats, *weights, *(kept if ctx.packed is None else _pack(*kept)))
         ctx.set_materialize_grads(False)
         return x, n
 
@@ -297,20 +346,24 @@ class NormGateResidualFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gx, gn):
         from .glue import norm_gate_residual_backward as run
-        o, residual, gate, stats, *weights = ctx.saved_tensors
         if gx is None and gn is None:
-            return (None,) * 11
-        return run(_rows(gx), _rows(gn), o, stats, residual, gate, **dict(zip(_BLOCK_WEIGHTS, weights)), **ctx.kw) + (None,) * 3
+            return (None,) * 12
+        stats, *kept = ctx.saved_tensors
+        weights, kept = kept[:5], kept[5:]
+        o, residual, gate = kept if ctx.packed is None else _unpack(kept, ctx.packed)
+        return run(_rows(gx), _rows(gn), o, stats, residual, gate, **dict(zip(_BLOCK_WEIGHTS, weights)), **ctx.kw) + (None,) * 4
 
 
 _BLOCK_WEIGHTS = ("post_weight", "post_bias", "scale", "pre_weight", "pre_bias")
 
 
 def norm_gate_residual(o, residual=None, gate=None, *, norm="rms", activation="silu", post_weight=None, post_bias=None, scale=None,
-                       pre_weight=None, pre_bias=None, eps=1e-6):
-    """Differentiable `ttt_tk_b200.glue.norm_gate_residual`, with rows at any distances."""
+                       pre_weight=None, pre_bias=None, eps=1e-6, saved=None):
+    """Differentiable `ttt_tk_b200.glue.norm_gate_residual`, with rows at any distances.  `saved` "e4m3": o, residual and gate are kept in 8 bits, and the
+    gradients are those at what was kept, with the statistics as the forward has them."""
     for name, t in (("residual", residual), ("gate", gate)):
         if isinstance(o, torch.Tensor) and isinstance(t, torch.Tensor) and t.shape != o.shape:
             raise ValueError(f"norm_gate_residual: {name} must have the shape of o, {list(o.shape)}, got {list(t.shape)}")
-    x, n = NormGateResidualFunction.apply(*[_tokens(t) for t in (o, residual, gate)], post_weight, post_bias, scale, pre_weight, pre_bias, norm, activation, eps)
+    x, n = NormGateResidualFunction.apply(*[_tokens(t) for t in (o, residual, gate)], post_weight, post_bias, scale, pre_weight, pre_bias, norm, activation, eps,
+                                          _saved(saved))
     return x.view(o.shape), None if n is None else n.view(o.shape)

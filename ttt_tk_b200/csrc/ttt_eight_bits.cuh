@@ -1,0 +1,57 @@
+// Activations in 8 bits: of each group of neighbouring values of a row, one fp32 scale, the least power of two with max |v| <= 448 scale,
+// and v / scale in e4m3 (rounded to the nearest, ties to even).  A power of two divides exactly, so the only rounding is the format's own.
+// Infinities are left out of the maximum and become 448 scale; NaN stays.  A group of zeros has the least scale there is.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include <type_traits>
+
+#include "ttt_elem.cuh"
+
+namespace ttt {
+
+// Largest of the magnitudes so far, infinities and NaN left out.
+__device__ __forceinline__ uint32_t magnitude(uint32_t most, float v) {
+  const uint32_t m = __float_as_uint(v) & 0x7fffffffu;
+  return m < 0x7f800000u && m > most ? m : most;
+}
+// Exponent field of the scale of a group whose largest magnitude has these bits: 8 less than that of amax / 1.75 rounded up, at least 1.
+__device__ __forceinline__ uint32_t scale_exponent(uint32_t most) { return max(static_cast<int>((most + 0x1fffffu) >> 23) - 8, 1); }
+__device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float(e << 23); }
+__device__ __forceinline__ float inverse_of(uint32_t e) { return __uint_as_float((254u - e) << 23); }      // (e is at most 254 - 8: no subnormal)
+
+// Two values to two bytes.
+__device__ __forceinline__ uint32_t two_bytes(float a, float b) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float2 two_values(uint32_t bytes) {
+  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(bytes), __NV_E4M3)));
+}
+
+// Eight neighbouring values in memory, in pieces of up to 16 bytes where they start on a boundary.
+template <class T> struct Eight {
+  alignas(16) T v[8];
+  using Piece = typename std::conditional<sizeof(T) == 1, uint2, uint4>::type;
+  static constexpr int kPieces = 8 * sizeof(T) / sizeof(Piece);
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) reinterpret_cast<Piece*>(v)[i] = reinterpret_cast<const Piece*>(p)[i];
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) reinterpret_cast<Piece*>(p)[i] = reinterpret_cast<const Piece*>(v)[i];
+  }
+  // the first n of them, from and to any boundary
+  __device__ __forceinline__ void load(const T* p, int n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : T();
+  }
+  __device__ __forceinline__ void store(T* p, int n) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = v[i];
+  }
+};
+
+}  // namespace ttt

@@ -31,6 +31,12 @@ using E4 = __nv_fp8_e4m3;
 constexpr int kTile = TTT_B200_GATED_INTERVAL;      // tokens of a CTA's tile, and between two checkpoints
 constexpr int kCols = 64;                           // channels of a CTA
 
+#ifndef TTT_FWD_CTAS
+#define TTT_FWD_CTAS 2
+#define TTT_BWD_CTAS 2
+#define TTT_FWD_S 8
+#define TTT_BWD_S 8
+#endif
 struct Plan {
   int tiles;      // CTAs (clusters) side by side: channels / 64
   int cluster;    // CTAs that have tiles behind one another
@@ -55,37 +61,39 @@ __device__ __forceinline__ float rsqrt_fast(float v) {
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-__device__ __forceinline__ F neg(F a) { return make_float2(-a.x, -a.y); }
+__device__ __forceinline__ F neg(F a) { return mul2(a, both(-1.f)); }
 
-// s = sigmoid(v) and 1 - s, the latter without the cancellation on the right.  The exponent is bounded so that far on the left e s is a
-// number: at 2^127 the reciprocal is below the least normal number and so s = 0 (and e s = 0: it only ever meets the factor s); at 2^126
+// s = sigmoid(v) and, with kBoth, 1 - s without the cancellation on the right.  For 1 - s the exponent is bounded so that far on the left e s
+// is a number: at 2^127 the reciprocal is below the least normal number and so s = 0 (and e s = 0: it only ever meets the factor s); at 2^126
 // s = 2^-126 and e s = 1, which the form without A needs.
-__device__ __forceinline__ void sigmoid(F v, float most, F& s, F& other) {
-  const F t = mul2(v, both(-kLog2e));
-  const F e = make_float2(ex2(min_nan(t.x, most)), ex2(min_nan(t.y, most)));
+// `bias` comes times -log2 e.
+template <bool kBoth> __device__ __forceinline__ void sigmoid(F v, F bias, float most, F& s, F& other) {
+  F t = fma2(v, both(-kLog2e), bias);
+  if constexpr (kBoth) t = make_float2(min_nan(t.x, most), min_nan(t.y, most));
+  const F e = ex2(t);
   s = rcp(add2(e, both(1.f)));
-  other = mul2(e, s);
+  if constexpr (kBoth) other = mul2(e, s);
 }
 
-// exp(v) and exp(v) - 1 for v <= 0: v = k ln 2 + f, |f| <= ln 2 / 2, ln 2 in two parts (Cody and Waite), exp(f) - 1 by its Taylor series to the
-// seventh power (the rest is below 2^-25 of it).  Both from one series: 1 - a keeps its digits where a is close to one, which is where these
+// exp(v) and 1 - exp(v) for v <= 0: v = k ln 2 + f, |f| <= ln 2 / 2, ln 2 in two parts (Cody and Waite), exp(f) - 1 = f + f^2 p(f) with the
+// polynomial of fourth degree that is off by the least part of f (1.6e-8, fitted).  Both from one series: 1 - a keeps its digits where a is close to one, which is where these
 // recurrences are, and the exponential unit, which is close to its limit, is left alone.  Where k comes to -127 the power's
 // bits are those of 0: exp(v) is 0 from there on, as far as A makes v.
-__device__ __forceinline__ void exp_both(F v, F& a, F& m) {
+__device__ __forceinline__ void exp_both(F v, F& a, F& rest) {
   v = make_float2(max_nan(v.x, -88.f), max_nan(v.y, -88.f));
   constexpr float magic = 12582912.f;      // 1.5 2^23: the sum's last bits are the rounded integer
   const F k = fma2(v, both(kLog2e), both(magic)), kf = add2(k, both(-magic));
   F f = fma2(kf, both(-0.693145751953125f), v);
   f = fma2(kf, both(-1.42860682030941723e-6f), f);
-  F q = fma2(f, both(1.f / 5040), both(1.f / 720));
-  q = fma2(q, f, both(1.f / 120));
-  q = fma2(q, f, both(1.f / 24));
-  q = fma2(q, f, both(1.f / 6));
+  F q = fma2(f, both(1.3947017723694444e-3f), both(8.366910740733147e-3f));
+  q = fma2(q, f, both(4.166627302765846e-2f));
+  q = fma2(q, f, both(1.6666540503501892e-1f));
   q = fma2(q, f, both(0.5f));
   q = fma2(mul2(f, f), q, f);
   const F two = make_float2(__int_as_float((__float_as_int(k.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(k.y) << 23) + 0x3f800000));
-  a = fma2(q, two, two);
-  m = fma2(q, two, add2(two, both(-1.f)));
+  q = mul2(q, two);      // exact but where it is below the normal numbers
+  a = add2(q, two);
+  rest = fma2(q, both(-1.f), fma2(two, both(-1.f), both(1.f)));
 }
 
 // What does not change over the tokens of a lane's channels.
@@ -95,68 +103,55 @@ struct Weights {
   bool has_a, gated;
 };
 
-// Of S tokens: a; w = b i; and for the backward  k = d log a / d gate, s, slope = i db/dlog a, rest = 1 - i.  The cases are the same for all
-// threads and decided once for the S tokens.
-template <int S, bool kBack> struct Factors {
-  F a[S], w[S];
-  F k[kBack ? S : 1], s[kBack ? S : 1], slope[kBack ? S : 1], rest[kBack ? S : 1];
-  // gate and input gate are given by functions of the token, so that they are read where they are used
-  template <class Gate, class Input> __device__ __forceinline__ void set(const Weights& z, Gate gate, Input input) {
-    F m[S];      // a - 1
-    if (z.has_a) {
-#pragma unroll
-      for (int t = 0; t < S; ++t) {
-        F s1, o;
-        sigmoid(add2(gate(t), z.gate_bias), 127.f, s1, o);
-        const F la = mul2(s1, z.A);
-        exp_both(la, a[t], m[t]);
-        if constexpr (kBack) s[t] = s1, k[t] = mul2(la, o);
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < S; ++t) {
-        F o;
-        sigmoid(add2(gate(t), z.gate_bias), 126.f, a[t], o);
-        m[t] = neg(o);
-        if constexpr (kBack) s[t] = a[t], k[t] = o;
-      }
-    }
-    if (z.mix == TTT_B200_MIX_SQRT) {
-#pragma unroll
-      for (int t = 0; t < S; ++t) {
-        const F q = mul2(neg(m[t]), add2(m[t], both(2.f)));      // 1 - a^2
-        F r = make_float2(rsqrt_fast(q.x), rsqrt_fast(q.y));
-        r = make_float2(q.x < 1.17549435e-38f ? 0.f : r.x, q.y < 1.17549435e-38f ? 0.f : r.y);      // a = 1: b and its slope are 0
-        w[t] = mul2(q, r);
-        if constexpr (kBack) slope[t] = mul2(neg(mul2(a[t], a[t])), r);
-      }
-    } else if (z.mix == TTT_B200_MIX_LINEAR) {
-#pragma unroll
-      for (int t = 0; t < S; ++t) {
-        w[t] = neg(m[t]);
-        if constexpr (kBack) slope[t] = neg(a[t]);
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < S; ++t) {
-        w[t] = both(1.f);
-        if constexpr (kBack) slope[t] = both(0.f);
-      }
-    }
-    if (z.gated) {
-#pragma unroll
-      for (int t = 0; t < S; ++t) {
-        F i, o;
-        sigmoid(add2(input(t), z.input_bias), 126.f, i, o);
-        w[t] = mul2(w[t], i);
-        if constexpr (kBack) slope[t] = mul2(slope[t], i), rest[t] = o;
-      }
-    } else if constexpr (kBack) {
-#pragma unroll
-      for (int t = 0; t < S; ++t) rest[t] = both(0.f);
-    }
-  }
+// A token's a and w = b i, and for the backward  k = d log a / d gate, s, slope = i db/dlog a, rest = 1 - i.
+template <bool kBack> struct Factors;
+template <> struct Factors<false> {
+  F a, w;
 };
+template <> struct Factors<true> {
+  F a, w, k, s, slope, rest;
+};
+// kUsual: A, the root and an input gate, which leaves nothing to decide for each token.
+template <bool kUsual, bool kBack, class Gate, class Input>
+__device__ __forceinline__ void factors(const Weights& z, Gate gate, Input input, Factors<kBack>& f) {
+  F rest, o;      // 1 - a, 1 - s
+  if (kUsual || z.has_a) {
+    F s;
+    sigmoid<kBack>(gate, z.gate_bias, 127.f, s, o);
+    const F la = mul2(s, z.A);
+    exp_both(la, f.a, rest);
+    if constexpr (kBack) f.s = s, f.k = mul2(la, o);
+  } else {
+    sigmoid<true>(gate, z.gate_bias, 126.f, f.a, rest);
+    if constexpr (kBack) f.s = f.a, f.k = rest;
+  }
+  if (kUsual || z.mix == TTT_B200_MIX_SQRT) {
+    const F q = mul2(rest, fma2(rest, both(-1.f), both(2.f)));      // 1 - a^2
+    // where that is no normal number b is 0, and so is its slope
+    if constexpr (kBack) {
+      F r = make_float2(rsqrt_fast(q.x), rsqrt_fast(q.y));
+      r = make_float2(q.x < 1.17549435e-38f ? 0.f : r.x, q.y < 1.17549435e-38f ? 0.f : r.y);
+      f.w = mul2(q, r);
+      f.slope = mul2(mul2(f.a, f.a), neg(r));
+    } else {
+      f.w = mul2(q, make_float2(rsqrt_fast(max_nan(q.x, 1.17549435e-38f)), rsqrt_fast(max_nan(q.y, 1.17549435e-38f))));
+    }
+  } else if (z.mix == TTT_B200_MIX_LINEAR) {
+    f.w = rest;
+    if constexpr (kBack) f.slope = neg(f.a);
+  } else {
+    f.w = both(1.f);
+    if constexpr (kBack) f.slope = both(0.f);
+  }
+  if (kUsual || z.gated) {
+    F i;
+    sigmoid<kBack>(input(), z.input_bias, 126.f, i, o);
+    f.w = mul2(f.w, i);
+    if constexpr (kBack) f.slope = mul2(f.slope, i), f.rest = o;
+  } else if constexpr (kBack) {
+    f.rest = both(0.f);
+  }
+}
 
 // ---- rows through shared memory ------------------------------------------------------------------------------------------------
 template <class T> __device__ __forceinline__ F pair_of(uint32_t at) {      // shared address
@@ -212,19 +207,32 @@ template <class T, int S, bool kWhole> struct Rows {
   // tokens t .. t + S - 1, those before `stop`, to the shared address `to`
   __device__ __forceinline__ void copy(uint32_t to, int t, int stop) const {
     const int lane = threadIdx.x & 31;
+    if (kWhole && t + S <= stop && cols == kBytes) {      // all of them: nothing to compare
+      static_assert(32 % kPieces == 0 || !kWhole, "a lane's pieces are below one another");
+      const char* from = base + (t + lane / kPieces) * step + lane % kPieces * 16;
+      to += lane * 16;
 #pragma unroll
-    for (int i = 0; i < (S * kPieces + 31) / 32; ++i) {
-      const int n = lane + 32 * i, row = n / kPieces, o = n % kPieces * 16;
-      if (S * kPieces % 32 && n >= S * kPieces) break;
-      const char* from = base + (t + row) * step;
-      int have = cols - o;
-      if constexpr (!kWhole) {
-        const int off = static_cast<int>(reinterpret_cast<uintptr_t>(from) & 15);
-        from -= off;
-        have += off;
+      for (int i = 0; i < (S * kPieces + 31) / 32; ++i) {
+        if (S * kPieces % 32 && lane + 32 * i >= S * kPieces) break;
+        cp_async16_at(to + 512 * i, from);
+        from += 32 / kPieces * step;
       }
-      have = t + row < stop ? min(max(have, 0), 16) : 0;
-      cp_async16_at(to + row * kPitch + o, have ? from + o : reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(base) & ~uintptr_t{15}), have);
+      if constexpr (kScaled) to -= lane * 16;
+    } else {
+#pragma unroll
+      for (int i = 0; i < (S * kPieces + 31) / 32; ++i) {
+        const int n = lane + 32 * i, row = n / kPieces, o = n % kPieces * 16;
+        if (S * kPieces % 32 && n >= S * kPieces) break;
+        const char* from = base + (t + row) * step;
+        int have = cols - o;
+        if constexpr (!kWhole) {
+          const int off = static_cast<int>(reinterpret_cast<uintptr_t>(from) & 15);
+          from -= off;
+          have += off;
+        }
+        have = t + row < stop ? min(max(have, 0), 16) : 0;
+        cp_async16_at(to + row * kPitch + o, have ? from + o : reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(base) & ~uintptr_t{15}), have);
+      }
     }
     if constexpr (kScaled) {
       static_assert(S * 2 <= 32, "a lane for each scale");
@@ -270,8 +278,8 @@ template <bool kWhole> __device__ __forceinline__ Weights weights_of(const ttt_b
   Weights z;
   z.A = load2<kWhole>(p.A, d, p.D, 0.f);
   z.A = make_float2(min_nan(z.A.x, 0.f), min_nan(z.A.y, 0.f));
-  z.gate_bias = load2<kWhole>(p.gate_bias, d, p.D, 0.f);
-  z.input_bias = load2<kWhole>(p.input_bias, d, p.D, 0.f);
+  z.gate_bias = mul2(load2<kWhole>(p.gate_bias, d, p.D, 0.f), both(-kLog2e));
+  z.input_bias = mul2(load2<kWhole>(p.input_bias, d, p.D, 0.f), both(-kLog2e));
   z.mix = p.mix;
   z.has_a = p.A != nullptr;
   z.gated = p.input_gate != nullptr;
@@ -279,7 +287,12 @@ template <bool kWhole> __device__ __forceinline__ Weights weights_of(const ttt_b
 }
 
 // ---- joins -----------------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+// The warp that has written to the other CTAs releases what it wrote, and what the CTA's barrier in front has put in front of it; for the other
+// warps there is nothing to wait for (a release waits for all of a warp's stores, those of y among them).
+__device__ __forceinline__ void cluster_arrive(bool wrote) {
+  if (wrote) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  else asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ int cluster_rank() {
   uint32_t r;
@@ -291,7 +304,7 @@ __device__ __forceinline__ void store_remote(const void* mine, int rank, float4 
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine))), "r"(rank));
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
-constexpr int kMostCluster = 8;
+constexpr int kMostCluster = 16;
 __device__ __forceinline__ F first2(float4 v) { return make_float2(v.x, v.y); }
 __device__ __forceinline__ F second2(float4 v) { return make_float2(v.z, v.w); }
 __device__ __forceinline__ float4 four(F a, F b) { return make_float4(a.x, a.y, b.x, b.y); }
@@ -300,6 +313,7 @@ __device__ __forceinline__ float4 four(F a, F b) { return make_float4(a.x, a.y, 
 // the same one).
 template <int W> struct Steps {
   float4 warp[2][W][32], tile[2][kMostCluster][32];
+  F end[2][32];      // what a tile leaves, where a CTA has all of them
 };
 
 struct At {
@@ -318,7 +332,8 @@ struct At {
 
 constexpr int kStages = 2;
 
-template <class T, bool kWhole, int S, int W> __global__ void __launch_bounds__(32 * W) gated_forward_kernel(const ttt_b200_gated_args p, const Plan q) {
+template <class T, bool kWhole, bool kUsual, int S, int W>
+__global__ void __launch_bounds__(32 * W, TTT_FWD_CTAS) gated_forward_kernel(const ttt_b200_gated_args p, const Plan q) {
   static_assert(S * W == kTile, "the warps' tokens make a tile");
   wait_for_predecessor();
   using R = Rows<T, S, kWhole>;
@@ -337,7 +352,7 @@ template <class T, bool kWhole, int S, int W> __global__ void __launch_bounds__(
       const uint32_t to = ring + j % kStages * (3 * R::kStage);
       rx.copy(to, first + j * hop, at.len);
       rg.copy(to + R::kStage, first + j * hop, at.len);
-      if (z.gated) ri.copy(to + 2 * R::kStage, first + j * hop, at.len);
+      if (kUsual || z.gated) ri.copy(to + 2 * R::kStage, first + j * hop, at.len);
     }
     cp_async_commit();
   };
@@ -351,22 +366,29 @@ template <class T, bool kWhole, int S, int W> __global__ void __launch_bounds__(
     __syncwarp();      // the rows have landed for all lanes, and all are through with the place that the next ones take
     ahead(j + kStages - 1);
     const uint32_t from = ring + j % kStages * (3 * R::kStage);
-    Factors<S, false> f;
-    f.set(z, [&](int t) { return rg.get(from + R::kStage, t, t0 + t); }, [&](int t) { return ri.get(from + 2 * R::kStage, t, t0 + t); });
-    F whole = both(1.f), own = both(0.f);
+    F a[S], u[S], whole = both(1.f), own = both(0.f);
 #pragma unroll
     for (int t = 0; t < S; ++t) {
-      F u = mul2(f.w[t], rx.get(from, t, t0 + t));
-      if (t0 + t >= at.len) f.a[t] = both(1.f), u = both(0.f);
-      f.w[t] = u;
-      own = fma2(f.a[t], own, u);
-      whole = mul2(whole, f.a[t]);
+      Factors<false> f;
+      factors<kUsual, false>(z, rg.get(from + R::kStage, t, t0 + t), [&] { return ri.get(from + 2 * R::kStage, t, t0 + t); }, f);
+      a[t] = f.a;
+      u[t] = mul2(f.w, rx.get(from, t, t0 + t));
+    }
+    if (t0 + S > at.len) {
+#pragma unroll
+      for (int t = 0; t < S; ++t)
+        if (t0 + t >= at.len) a[t] = both(1.f), u[t] = both(0.f);
+    }
+#pragma unroll
+    for (int t = 0; t < S; ++t) {
+      own = fma2(a[t], own, u[t]);
+      whole = mul2(whole, a[t]);
     }
     join.warp[half][at.warp][at.lane] = four(whole, own);
     __syncthreads();
-    F h = carry;
+    F h = C > 1 || j == 0 ? carry : join.end[half ^ 1][at.lane];
     if (C > 1) {
-      if (at.warp < C) {      // warp r tells CTA r
+      if (at.warp == 0) {
         F P = both(1.f), H = both(0.f);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
@@ -374,9 +396,9 @@ template <class T, bool kWhole, int S, int W> __global__ void __launch_bounds__(
           P = mul2(P, first2(v));
           H = fma2(first2(v), H, second2(v));
         }
-        store_remote(&join.tile[half][at.rank][at.lane], at.warp, four(P, H));
+        for (int r = 0; r < C; ++r) store_remote(&join.tile[half][at.rank][at.lane], r, four(P, H));
       }
-      cluster_arrive();
+      cluster_arrive(at.warp == 0);
       cluster_wait();
       F next = carry;
       for (int r = 0; r < C; ++r) {
@@ -388,30 +410,38 @@ template <class T, bool kWhole, int S, int W> __global__ void __launch_bounds__(
     }
     if (at.warp == 0 && p.checkpoints && t0 < at.len)
       store2<float, kWhole>(p.checkpoints + (static_cast<long>(at.b) * q.nck + j * C + at.rank) * p.D, at.d, p.D, h);
-    F mine = h;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      if (C > 1 && w >= at.warp) break;
-      if (w == at.warp) mine = h;
+    for (int w = 0; w < W - 1; ++w) {
+      if (w >= at.warp) break;
       const float4 v = join.warp[half][w][at.lane];
       h = fma2(first2(v), h, second2(v));
     }
-    if (C > 1) mine = h;
-    else carry = h;
-    h = mine;
+    T* to = y + static_cast<long>(t0) * p.D;
+    if (t0 + S <= at.len) {
 #pragma unroll
-    for (int t = 0; t < S; ++t) {
-      h = fma2(f.a[t], h, f.w[t]);
-      if (t0 + t < p.T) store2<T, kWhole>(y + static_cast<long>(t0 + t) * p.D, at.d, p.D, t0 + t < at.len ? h : both(0.f));
+      for (int t = 0; t < S; ++t) {
+        h = fma2(a[t], h, u[t]);
+        store2<T, kWhole>(to, at.d, p.D, h);
+        to += p.D;
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < S; ++t) {
+        h = fma2(a[t], h, u[t]);
+        if (t0 + t < p.T) store2<T, kWhole>(to, at.d, p.D, t0 + t < at.len ? h : both(0.f));
+        to += p.D;
+      }
     }
+    if (C == 1 && at.warp == W - 1) carry = join.end[half][at.lane] = h;
   }
-  if (p.final_state && at.rank == 0 && at.warp == 0) store2<float, kWhole>(p.final_state + static_cast<long>(at.b) * p.D, at.d, p.D, carry);
+  if (p.final_state && at.rank == 0 && at.warp == W - 1) store2<float, kWhole>(p.final_state + static_cast<long>(at.b) * p.D, at.d, p.D, carry);
   for (int t0 = first + rounds * hop; t0 < p.T; t0 += hop)
     for (int t = t0; t < min(t0 + S, p.T); ++t) store2<T, kWhole>(y + static_cast<long>(t) * p.D, at.d, p.D, both(0.f));
 }
 
 // T: the gradients' type; I: that of x and the gates, or 8-bit values
-template <class T, class I, bool kWhole, int S, int W> __global__ void __launch_bounds__(32 * W) gated_backward_kernel(const ttt_b200_gated_args p, const Plan q) {
+template <class T, class I, bool kWhole, bool kUsual, int S, int W>
+__global__ void __launch_bounds__(32 * W, TTT_BWD_CTAS) gated_backward_kernel(const ttt_b200_gated_args p, const Plan q) {
   static_assert(S * W == kTile, "the warps' tokens make a tile");
   wait_for_predecessor();
   using R = Rows<I, S, kWhole>;
@@ -423,6 +453,7 @@ template <class T, class I, bool kWhole, int S, int W> __global__ void __launch_
   const At at(p, q);
   const int d0 = at.tile * kCols, C = q.cluster;
   const Weights z = weights_of<kWhole>(p, at.d);
+  const bool gated = kUsual || z.gated;
   const int groups = p.group ? (p.D + p.group - 1) / p.group : 0;
   const R rx(p.x, p.x_stride[0], p.x_stride[1], at.b, d0, p.D, p.x_scales, groups, p.group, p.T),
       rg(p.gate, p.gate_stride[0], p.gate_stride[1], at.b, d0, p.D, p.gate_scales, groups, p.group, p.T),
@@ -436,7 +467,7 @@ template <class T, class I, bool kWhole, int S, int W> __global__ void __launch_
       const uint32_t to = ring + j % kStages * kStage;
       rx.copy(to, first + j * hop, at.len);
       rg.copy(to + R::kStage, first + j * hop, at.len);
-      if (z.gated) ri.copy(to + 2 * R::kStage, first + j * hop, at.len);
+      if (gated) ri.copy(to + 2 * R::kStage, first + j * hop, at.len);
       ru.copy(to + 3 * R::kStage, first + j * hop, at.len);
     }
     cp_async_commit();
@@ -445,11 +476,10 @@ template <class T, class I, bool kWhole, int S, int W> __global__ void __launch_
   for (int j = 0; j < kStages - 1; ++j) ahead(rounds - 1 - j);
   const long batch = static_cast<long>(at.b) * p.T * p.D;
   T *gx = static_cast<T*>(p.grad_x) + batch, *gg = static_cast<T*>(p.grad_gate) + batch, *gi = static_cast<T*>(p.grad_input) + batch;
-  auto put = [&](int t, F x, F g, F i) {
-    const long o = static_cast<long>(t) * p.D;
+  auto put = [&](long o, F x, F g, F i) {
     store2<T, kWhole>(gx + o, at.d, p.D, x);
     store2<T, kWhole>(gg + o, at.d, p.D, g);
-    if (z.gated) store2<T, kWhole>(gi + o, at.d, p.D, i);
+    if (gated) store2<T, kWhole>(gi + o, at.d, p.D, i);
   };
   F carry = load2<kWhole>(p.grad_final_state ? p.grad_final_state + static_cast<long>(at.b) * p.D : nullptr, at.d, p.D, 0.f);
   F sum_a = both(0.f), sum_g = sum_a, sum_i = sum_a;
@@ -461,54 +491,58 @@ template <class T, class I, bool kWhole, int S, int W> __global__ void __launch_
     __syncwarp();
     ahead(j - kStages + 1);
     const uint32_t from = ring + j % kStages * kStage;
-    Factors<S, true> f;
-    f.set(z, [&](int t) { return rg.get(from + R::kStage, t, t0 + t); }, [&](int t) { return ri.get(from + 2 * R::kStage, t, t0 + t); });
-    F whole = both(1.f), own = both(0.f), left = both(0.f);
+    // of a token: a; w = b i; what there is of d log a / G without the state, which joins it; d log a's factors in d gate and dA; d input / G
+    F a[S], w[S], slope[S], k[S], s[S], in[S], whole = both(1.f), own = both(0.f), left = both(0.f);
 #pragma unroll
     for (int t = 0; t < S; ++t) {
-      const bool in = t0 + t < at.len;
+      Factors<true> f;
+      factors<kUsual, true>(z, rg.get(from + R::kStage, t, t0 + t), [&] { return ri.get(from + 2 * R::kStage, t, t0 + t); }, f);
       const F x = rx.get(from, t, t0 + t);
-      f.slope[t] = mul2(f.slope[t], x);
-      f.rest[t] = mul2(f.rest[t], mul2(f.w[t], x));
-      if (!in) f.a[t] = both(1.f);
-      own = fma2(f.a[t], own, in ? mul2(f.w[t], x) : both(0.f));
-      whole = mul2(whole, f.a[t]);
+      a[t] = f.a, w[t] = f.w, k[t] = f.k, s[t] = f.s;
+      slope[t] = mul2(f.slope, x);
+      in[t] = mul2(f.rest, mul2(f.w, x));
     }
-    F dy[S];
+    if (t0 + S > at.len) {
 #pragma unroll
-    for (int t = S - 1; t >= 0; --t) {
-      dy[t] = t0 + t < at.len ? ru.get(from + 3 * R::kStage, t, t0 + t) : both(0.f);
-      left = mul2(f.a[t], add2(dy[t], left));
+      for (int t = 0; t < S; ++t)
+        if (t0 + t >= at.len) a[t] = both(1.f), w[t] = both(0.f);
     }
+#pragma unroll
+    for (int t = 0; t < S; ++t) {
+      own = fma2(a[t], own, mul2(w[t], rx.get(from, t, t0 + t)));
+      whole = mul2(whole, a[t]);
+    }
+#pragma unroll
+    for (int t = S - 1; t >= 0; --t) left = mul2(a[t], add2(ru.get(from + 3 * R::kStage, t, t0 + t), left));
     join.warp[half][at.warp][at.lane] = four(whole, own);
     back[half][at.warp][at.lane] = left;
     __syncthreads();
-    F c = carry;
+    F c = C > 1 || j == rounds - 1 ? carry : join.end[half ^ 1][at.lane];
     if (C > 1) {
-      if (at.warp < C) {
+      if (at.warp == W - 1) {
         F P = both(1.f), Q = both(0.f);
 #pragma unroll
-        for (int w = W - 1; w >= 0; --w) {
-          const F a = first2(join.warp[half][w][at.lane]);
-          P = mul2(P, a);
-          Q = fma2(a, Q, back[half][w][at.lane]);
+        for (int v = W - 1; v >= 0; --v) {
+          const F f = first2(join.warp[half][v][at.lane]);
+          P = mul2(P, f);
+          Q = fma2(f, Q, back[half][v][at.lane]);
         }
-        store_remote(&join.tile[half][at.rank][at.lane], at.warp, four(P, Q));
+        for (int r = 0; r < C; ++r) store_remote(&join.tile[half][at.rank][at.lane], r, four(P, Q));
       }
-      cluster_arrive();
+      cluster_arrive(at.warp == W - 1);
     }
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      if (w >= at.warp) break;
-      const float4 v = join.warp[half][w][at.lane];
-      h = fma2(first2(v), h, second2(v));
+    for (int v = 0; v < W; ++v) {
+      if (v >= at.warp) break;
+      const float4 f = join.warp[half][v][at.lane];
+      h = fma2(first2(f), h, second2(f));
     }
     // to h_{t-1}, and with it to d log a / G
 #pragma unroll
     for (int t = 0; t < S; ++t) {
-      const F left_of = mul2(f.a[t], h);
-      f.slope[t] = add2(left_of, f.slope[t]);
-      h = fma2(f.w[t], rx.get(from, t, t0 + t), left_of);
+      const F kept = mul2(a[t], h);
+      slope[t] = add2(kept, slope[t]);
+      h = fma2(w[t], rx.get(from, t, t0 + t), kept);
     }
     if (C > 1) {
       cluster_wait();
@@ -520,34 +554,36 @@ template <class T, class I, bool kWhole, int S, int W> __global__ void __launch_
       }
       carry = next;
     }
-    F mine = c;
 #pragma unroll
-    for (int w = W - 1; w >= 0; --w) {
-      if (C > 1 && w <= at.warp) break;
-      if (w == at.warp) mine = c;
-      c = fma2(first2(join.warp[half][w][at.lane]), c, back[half][w][at.lane]);
+    for (int v = W - 1; v > 0; --v) {
+      if (v <= at.warp) break;
+      c = fma2(first2(join.warp[half][v][at.lane]), c, back[half][v][at.lane]);
     }
-    if (C > 1) mine = c;
-    else carry = c;
-    c = mine;
+    long o = static_cast<long>(t0 + S - 1) * p.D;
+    auto one = [&](int t) {
+      const F G = add2(ru.get(from + 3 * R::kStage, t, t0 + t), c);
+      c = mul2(a[t], G);
+      const F dl = mul2(G, slope[t]), dg = mul2(dl, k[t]), di = mul2(G, in[t]);
+      sum_a = fma2(dl, s[t], sum_a);
+      sum_g = add2(sum_g, dg);
+      sum_i = add2(sum_i, di);
+      put(o, mul2(G, w[t]), dg, di);
+    };
+    if (t0 + S <= at.len) {
 #pragma unroll
-    for (int t = S - 1; t >= 0; --t) {
-      const F G = add2(dy[t], c);
-      c = mul2(f.a[t], G);
-      const F dl = mul2(G, f.slope[t]), dg = mul2(dl, f.k[t]), di = mul2(G, f.rest[t]);
-      if (t0 + t < at.len) {
-        sum_a = fma2(dl, f.s[t], sum_a);
-        sum_g = add2(sum_g, dg);
-        sum_i = add2(sum_i, di);
-        put(t0 + t, mul2(G, f.w[t]), dg, di);
-      } else if (t0 + t < p.T) {
-        put(t0 + t, both(0.f), both(0.f), both(0.f));
+      for (int t = S - 1; t >= 0; --t, o -= p.D) one(t);
+    } else {
+#pragma unroll
+      for (int t = S - 1; t >= 0; --t, o -= p.D) {
+        if (t0 + t < at.len) one(t);
+        else if (t0 + t < p.T) put(o, both(0.f), both(0.f), both(0.f));
       }
     }
+    if (C == 1 && at.warp == 0) carry = join.end[half][at.lane] = c;
   }
   if (p.grad_state && at.rank == 0 && at.warp == 0) store2<float, kWhole>(p.grad_state + static_cast<long>(at.b) * p.D, at.d, p.D, carry);
   for (int t0 = first + rounds * hop; t0 < p.T; t0 += hop)
-    for (int t = t0; t < min(t0 + S, p.T); ++t) put(t, both(0.f), both(0.f), both(0.f));
+    for (int t = t0; t < min(t0 + S, p.T); ++t) put(static_cast<long>(t) * p.D, both(0.f), both(0.f), both(0.f));
   // the warps' sums, in their order
   __shared__ F sums[3][W][32];
   sums[0][at.warp][at.lane] = sum_a;
@@ -601,10 +637,10 @@ template <class T, bool kWhole> __global__ void __launch_bounds__(128) gated_ste
   F h = load2<kWhole>(st, d, p.D, 0.f);
   for (int b = b0; b < p.B; ++b) {
     if (b != b0 && p.slots[b] != slot) continue;
-    Factors<1, false> f;
+    Factors<false> f;
     const F x = two(p.x, p.x_stride[0], b);
-    f.set(z, [&](int) { return two(p.gate, p.gate_stride[0], b); }, [&](int) { return two(p.input_gate, p.input_stride[0], b); });
-    h = fma2(f.a[0], h, mul2(f.w[0], x));
+    factors<false, false>(z, two(p.gate, p.gate_stride[0], b), [&] { return two(p.input_gate, p.input_stride[0], b); }, f);
+    h = fma2(f.a, h, mul2(f.w, x));
     store2<T, kWhole>(ys + static_cast<long>(b) * p.D, d, p.D, h);
     if (!more) break;
   }
@@ -640,7 +676,10 @@ void plan(Plan& q, const ttt_b200_gated_args& p) {
   q.tiles = (p.D - 1) / kCols + 1;
   q.nck = (p.T - 1) / kTile + 1;
   const long columns = static_cast<long>(q.tiles) * p.B, sms = sm_count();
-  for (q.cluster = 1; q.cluster < kMostCluster && q.cluster < q.nck && columns * q.cluster < 2 * sms; q.cluster *= 2) {}
+  for (q.cluster = 1; q.cluster < kMostCluster && q.cluster < q.nck && columns * q.cluster < sms; q.cluster *= 2) {}
+#ifdef TTT_PROBE
+  if (getenv("TTT_PROBE_C")) q.cluster = atoi(getenv("TTT_PROBE_C"));
+#endif
 }
 
 template <auto kKernel> int launch(const Plan& q, const ttt_b200_gated_args& p, int threads, uint32_t bytes, cudaStream_t s, const char* what) {
@@ -648,6 +687,8 @@ template <auto kKernel> int launch(const Plan& q, const ttt_b200_gated_args& p, 
   if (grid > 0x7fffffffL) return fail("gated scan: too many CTAs");
   if (bytes > 16 * 1024)      // (with the static part 48 KB is the most without asking)
     if (int rc = allow_shared<kKernel>()) return rc;
+  if (q.cluster > 8)
+    if (cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return ttt_set_error(TTT_B200_ERR_LAUNCH, cudaGetErrorString(e));
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -665,14 +706,19 @@ template <auto kKernel> int launch(const Plan& q, const ttt_b200_gated_args& p, 
   return launched(what);
 }
 
+bool usual(const ttt_b200_gated_args& p) { return p.A && p.input_gate && p.mix == TTT_B200_MIX_SQRT; }
+
 template <class T, bool kWhole> int forward(const ttt_b200_gated_args& p, const Plan& q, cudaStream_t s) {
-  constexpr int S = 8, W = kTile / S;
-  return launch<gated_forward_kernel<T, kWhole, S, W>>(q, p, 32 * W, W * kStages * 3 * Rows<T, S, kWhole>::kStage, s, "gated scan");
+  constexpr int S = TTT_FWD_S, W = kTile / S;
+  constexpr uint32_t bytes = W * kStages * 3 * Rows<T, S, kWhole>::kStage;
+  return usual(p) ? launch<gated_forward_kernel<T, kWhole, true, S, W>>(q, p, 32 * W, bytes, s, "gated scan")
+                  : launch<gated_forward_kernel<T, kWhole, false, S, W>>(q, p, 32 * W, bytes, s, "gated scan");
 }
 template <class T, class I, bool kWhole> int backward_of(const ttt_b200_gated_args& p, const Plan& q, cudaStream_t s) {
-  constexpr int S = 8, W = kTile / S;
-  return launch<gated_backward_kernel<T, I, kWhole, S, W>>(
-      q, p, 32 * W, W * kStages * (3 * Rows<I, S, kWhole>::kStage + Rows<T, S, kWhole>::kStage), s, "gated scan backward");
+  constexpr int S = TTT_BWD_S, W = kTile / S;
+  constexpr uint32_t bytes = W * kStages * (3 * Rows<I, S, kWhole>::kStage + Rows<T, S, kWhole>::kStage);
+  return usual(p) ? launch<gated_backward_kernel<T, I, kWhole, true, S, W>>(q, p, 32 * W, bytes, s, "gated scan backward")
+                  : launch<gated_backward_kernel<T, I, kWhole, false, S, W>>(q, p, 32 * W, bytes, s, "gated scan backward");
 }
 template <class T> int backward(const ttt_b200_gated_args& p, cudaStream_t s) {
   Plan q = {};

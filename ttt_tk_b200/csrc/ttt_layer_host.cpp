@@ -11,6 +11,7 @@
 #include <initializer_list>
 #include <stdexcept>
 #include <string>
+#include <vector>
 
 #include "../../include/ttt_mlp_b200.h"
 
@@ -119,7 +120,7 @@ class Call {
   void rows(const Tensor& t, const char* name) const {
     if (t.size(-1) > 1 && t.stride(-1) != 1) refuse(std::string(what_) + ": the last dimension of " + name + " must be contiguous");
   }
-  static constexpr int kMost = 16;
+  static constexpr int kMost = 20;
   const char* what_;
   const Tensor* seen_[kMost];
   const char* names_[kMost];
@@ -745,10 +746,267 @@ PyObject* block_backward(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
   });
 }
 
+// ---- activations in 8 bits ---------------------------------------------------------------------------------------------------
+std::vector<int64_t> scales_shape(const Tensor& t, int64_t group) {
+  std::vector<int64_t> s(t.sizes().begin(), t.sizes().end());
+  if (group) s.back() = (s.back() + group - 1) / group;
+  else s.pop_back();
+  return s;
+}
+int64_t group_of(const Call& c, PyObject* o) {
+  const int64_t g = integer(o);
+  c.need(g == 32 || g == 64 || g == 128, "group must be 32, 64 or 128");
+  return g;
+}
+PyObject* pair_of(const Tensor& a, const Tensor& b) { return tuple_of({a, b}); }
+
+// a list of what `one` makes for each of n
+template <class Fn> PyObject* list_of(Py_ssize_t n, Fn one) {
+  PyObject* r = PyList_New(n);
+  if (!r) throw PythonError();
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o;
+    try {
+      o = one(i);
+    } catch (...) {
+      Py_DECREF(r);
+      throw;
+    }
+    PyList_SET_ITEM(r, i, o);
+  }
+  return r;
+}
+
+// pack8(tuple of tensors, group) -> [(values, scales), ...]
+PyObject* pack8(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  return guarded("pack8", nargs, 2, [&]() -> PyObject* {
+    Call c("pack8");
+    ttt_b200_pack8_args a = {};
+    const Py_ssize_t n = PyTuple_GET_SIZE(v[0]);
+    c.need(n >= 1 && n <= TTT_B200_PACK8_TENSORS, "one to four tensors");
+    const int64_t group = group_of(c, v[1]);
+    const Tensor* first = nullptr;
+    for (Py_ssize_t k = 0; k < n; ++k) {
+      const Tensor& t = *c.any(PyTuple_GET_ITEM(v[0], k), "a tensor");
+      c.need(t.dim() >= 1, "tensors must be [..., D]");
+      if (!first) {
+        c.first(PyTuple_GET_ITEM(v[0], k), "a tensor", t.dim(), "[..., D]");
+        first = &t;
+      }
+      c.need(t.sizes() == first->sizes() && t.scalar_type() == first->scalar_type(), "tensors of one call must share shape and type");
+      c.need(t.size(-1) <= 1 || t.stride(-1) == 1, "the last dimension of a tensor must be contiguous");
+      a.stride[k] = row_stride(c, t, "the rows of a tensor must be at a fixed distance");
+      a.src[k] = t.data_ptr();
+    }
+    c.sized(first->size(-1), "a row");
+    c.need(first->size(-1) >= 1, "rows have no values");
+    a.D = static_cast<int32_t>(first->size(-1));
+    a.M = first->numel() / a.D;
+    a.dtype = c.dtype();
+    a.group = static_cast<int32_t>(group);
+    a.count = static_cast<int32_t>(n);
+    const c10::Device dev = c.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    const auto opt = at::TensorOptions().device(dev);
+    const std::vector<int64_t> scaled = scales_shape(*first, group);
+    Tensor q[TTT_B200_PACK8_TENSORS], s[TTT_B200_PACK8_TENSORS];
+    for (Py_ssize_t k = 0; k < n; ++k) {
+      q[k] = at::empty(first->sizes(), opt.dtype(at::kFloat8_e4m3fn));
+      s[k] = at::empty(scaled, opt.dtype(at::kFloat));
+      a.values[k] = q[k].data_ptr();
+      a.scales[k] = fptr(s[k]);
+    }
+    if (a.M > 0) launch(ttt_b200_pack8, a, dev);
+    return list_of(n, [&](Py_ssize_t k) { return pair_of(q[k], s[k]); });
+  });
+}
+
+// unpack8(tuple of (values, scales), dtype code) -> [tensor, ...]
+PyObject* unpack8(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  return guarded("unpack8", nargs, 2, [&]() -> PyObject* {
+    Call c("unpack8");
+    ttt_b200_pack8_args a = {};
+    const Py_ssize_t n = PyTuple_GET_SIZE(v[0]);
+    c.need(n >= 1 && n <= TTT_B200_PACK8_TENSORS, "one to four pairs of values and scales");
+    a.dtype = static_cast<int32_t>(integer(v[1]));
+    const Tensor* first = nullptr;
+    int group = -1;
+    for (Py_ssize_t k = 0; k < n; ++k) {
+      PyObject* o = PyTuple_GET_ITEM(v[0], k);
+      c.need(PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 2, "what is unpacked must be (values, scales)");
+      const Tensor &q = *c.any(PyTuple_GET_ITEM(o, 0), "values"), &s = *c.any(PyTuple_GET_ITEM(o, 1), "scales");
+      c.need(q.scalar_type() == at::kFloat8_e4m3fn && q.dim() >= 1 && q.is_contiguous(), "values must be contiguous float8_e4m3fn [..., D]");
+      if (!first) first = &q;
+      c.need(q.sizes() == first->sizes(), "values of one call must share their shape");
+      int found = -1;
+      for (const int g : {0, 32, 64, 128})
+        if (s.sizes() == at::IntArrayRef(scales_shape(q, g)) && (group < 0 || group == g)) found = g;
+      c.need(found >= 0 && s.scalar_type() == at::kFloat && s.is_contiguous(),
+             "scales must be contiguous float32 [..., D / group], group 32, 64 or 128, or [...], and the same for all");
+      group = found;
+      a.values[k] = q.data_ptr();
+      a.scales[k] = static_cast<float*>(s.data_ptr());
+    }
+    c.sized(first->size(-1), "a row");
+    c.need(first->size(-1) >= 1, "rows have no values");
+    a.D = static_cast<int32_t>(first->size(-1));
+    a.M = first->numel() / a.D;
+    a.group = group;
+    a.count = static_cast<int32_t>(n);
+    const c10::Device dev = c.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::ScalarType type = a.dtype == TTT_B200_BF16 ? at::kBFloat16 : a.dtype == TTT_B200_FP16 ? at::kHalf : at::kFloat;
+    Tensor t[TTT_B200_PACK8_TENSORS];
+    for (Py_ssize_t k = 0; k < n; ++k) {
+      t[k] = at::empty(first->sizes(), at::TensorOptions().device(dev).dtype(type));
+      a.dst[k] = t[k].data_ptr();
+    }
+    if (a.M > 0) launch(ttt_b200_unpack8, a, dev);
+    return list_of(n, [&](Py_ssize_t k) { return wrap(t[k]); });
+  });
+}
+
+// norm8(o, residual, weight, bias, layer, group or 0, eps, want_stats) -> (x, values, scales, stats or None)
+PyObject* norm8(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  return guarded("norm8", nargs, 8, [&]() -> PyObject* {
+    Call c("norm_residual_8bit");
+    ttt_b200_norm8_args a = {};
+    const Tensor& o = *c.any(v[0], "o");
+    c.need(o.dim() >= 1, "o must be [..., D]");
+    c.first(v[0], "o", o.dim(), "[..., D]");
+    c.need(o.size(-1) >= 1 && o.size(-1) <= 8192, "o must have 1 to 8192 values to a token");
+    a.D = static_cast<int32_t>(o.size(-1));
+    a.M = o.numel() / a.D;
+    a.dtype = c.dtype();
+    const char* even = "the tokens of o and residual must be at a fixed distance";
+    a.o = o.data_ptr();
+    a.o_stride = row_stride(c, o, even);
+    const bool added = v[1] != Py_None;
+    if (added) {
+      const Tensor& r = *c.any(v[1], "residual");
+      c.need(r.sizes() == o.sizes(), "residual must have the shape of o");
+      c.need(r.scalar_type() == c.type() || r.scalar_type() == at::kFloat, "residual must have the type of o, or float32");
+      c.need(r.size(-1) == 1 || r.stride(-1) == 1, "the last dimension of residual must be contiguous");
+      a.residual_fp32 = r.scalar_type() == at::kFloat && c.type() != at::kFloat;
+      a.residual = r.data_ptr();
+      a.residual_stride = row_stride(c, r, even);
+    }
+    a.weight = c.weight(v[2], "weight", {a.D});
+    a.bias = c.f32(v[3], "bias", {a.D});
+    a.layer = truth(v[4]);
+    const int64_t group = integer(v[5]);
+    c.need(group == 0 || group == 32 || group == 64 || group == 128, "group must be 32, 64, 128 or None");
+    a.group = static_cast<int32_t>(group);
+    a.eps = static_cast<float>(PyFloat_AsDouble(v[6]));
+    if (PyErr_Occurred()) {
+      if (!PyErr_ExceptionMatches(PyExc_TypeError)) throw PythonError();
+      PyErr_Clear();
+      refuse("norm_residual_8bit: eps must be a number");
+    }
+    c.need(a.eps >= 0.f, "eps must be >= 0");
+    const c10::Device dev = c.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    const auto opt = at::TensorOptions().dtype(c.type()).device(dev), f32 = opt.dtype(at::kFloat);
+    const Tensor x = added ? at::empty(o.sizes(), a.residual_fp32 ? f32 : opt) : o;
+    const Tensor q = at::empty(o.sizes(), opt.dtype(at::kFloat8_e4m3fn)), s = at::empty(scales_shape(o, group), f32);
+    const Tensor stats = truth(v[7]) ? at::empty({a.M, 4}, f32) : Tensor();
+    a.x = added ? x.data_ptr() : nullptr;
+    a.values = q.data_ptr();
+    a.scales = fptr(s);
+    a.stats = fptr(stats);
+    if (a.M > 0) launch(ttt_b200_norm_residual_8bit, a, dev);
+    return tuple_of({x, q, s, stats});
+  });
+}
+
+// ---- rows of tables of states --------------------------------------------------------------------------------------------------
+// v: a tuple of tables
+int64_t tables_of(Call& c, ttt_b200_tables_args& a, PyObject* v) {
+  const Py_ssize_t n = PyTuple_GET_SIZE(v);
+  c.need(n >= 1 && n <= TTT_B200_TABLES, "1 to 16 tables");
+  int64_t rows = -1;
+  for (Py_ssize_t k = 0; k < n; ++k) {
+    const Tensor& t = *c.any(PyTuple_GET_ITEM(v, k), "a table");
+    c.need(t.dim() >= 1 && t.is_contiguous(), "a table must be contiguous and have rows");
+    if (rows < 0) rows = t.size(0);
+    c.need(t.size(0) == rows, "tables of one call must have as many rows");
+    const int64_t bytes = rows ? t.numel() / rows * static_cast<int64_t>(t.element_size()) : 0;
+    if (!bytes) continue;
+    for (int j = 0; j < a.count; ++j) {
+      const char *p = static_cast<char*>(t.data_ptr()), *q = static_cast<char*>(a.table[j]);
+      c.need(p + rows * bytes <= q || q + rows * a.row_bytes[j] <= p, "tables of one call must not overlap");
+    }
+    a.table[a.count] = t.data_ptr();
+    a.row_bytes[a.count++] = bytes;
+  }
+  c.sized(rows, "a table");
+  a.rows = static_cast<int32_t>(rows);
+  return rows;
+}
+const int32_t* pairs_of(Call& c, ttt_b200_tables_args& a, PyObject* o, const char* name) {
+  const Tensor& t = *c.any(o, name);
+  c.need(t.dim() == 1 && t.scalar_type() == at::kInt && t.is_contiguous(), (std::string(name) + " must be contiguous int32 [n]").c_str());
+  c.need(t.size(0) <= TTT_B200_TABLE_PAIRS, (std::string("at most 4096 rows in ") + name).c_str());
+  a.pairs = static_cast<int32_t>(t.size(0));
+  return static_cast<const int32_t*>(t.data_ptr());
+}
+
+// copy_rows(tables, source, target)
+PyObject* copy_rows(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  return guarded("copy_rows", nargs, 3, [&]() -> PyObject* {
+    Call c("copy_rows");
+    ttt_b200_tables_args a = {};
+    const int64_t rows = tables_of(c, a, v[0]);
+    a.source = pairs_of(c, a, v[1], "source");
+    const int32_t n = a.pairs;
+    a.target = pairs_of(c, a, v[2], "target");
+    c.need(a.pairs == n, "source and target must have as many rows");
+    const c10::Device dev = c.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    if (rows && n && a.count) launch(ttt_b200_copy_rows, a, dev);
+    Py_RETURN_NONE;
+  });
+}
+
+// clear_rows(tables, rows)
+PyObject* clear_rows(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  return guarded("clear_rows", nargs, 2, [&]() -> PyObject* {
+    Call c("clear_rows");
+    ttt_b200_tables_args a = {};
+    const int64_t rows = tables_of(c, a, v[0]);
+    a.target = pairs_of(c, a, v[1], "rows");
+    const c10::Device dev = c.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    if (rows && a.pairs && a.count) launch(ttt_b200_clear_rows, a, dev);
+    Py_RETURN_NONE;
+  });
+}
+
+// compact_rows(tables, used) -> place
+PyObject* compact_rows(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  return guarded("compact_rows", nargs, 2, [&]() -> PyObject* {
+    Call c("compact_rows");
+    ttt_b200_tables_args a = {};
+    const int64_t rows = tables_of(c, a, v[0]);
+    const Tensor& used = *c.shaped(v[1], "used", at::kBool, {rows});
+    c.need(used.is_contiguous(), "used must be contiguous");
+    c.need(rows <= 8192, "at most 8192 rows");
+    const c10::Device dev = c.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    const Tensor place = at::empty({rows}, at::TensorOptions().dtype(at::kInt).device(dev));
+    a.used = static_cast<const uint8_t*>(used.data_ptr());
+    a.place = static_cast<int32_t*>(place.data_ptr());
+    if (rows) launch(ttt_b200_compact_rows, a, dev);
+    return wrap(place);
+  });
+}
+
 #define TTT_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {TTT_METHOD(conv),          TTT_METHOD(conv_backward), TTT_METHOD(conv_step), TTT_METHOD(scan),
                           TTT_METHOD(scan_backward), TTT_METHOD(scan_step),     TTT_METHOD(block),     TTT_METHOD(block_backward),
                           TTT_METHOD(gated),         TTT_METHOD(gated_backward), TTT_METHOD(gated_step),
+                          TTT_METHOD(pack8),         TTT_METHOD(unpack8),        TTT_METHOD(norm8),
+                          TTT_METHOD(copy_rows),     TTT_METHOD(clear_rows),     TTT_METHOD(compact_rows),
                           {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_ttt_layer_host", "Validation and launch of the layer-side sequence operators.", -1, kMethods,

@@ -111,6 +111,23 @@ def norm_gate_residual(o, residual=None, gate=None, *, norm="rms", activation="s
     return (x, n, stats) if return_stats else (x, n)
 
 
+def norm_residual_8bit(o, residual=None, *, weight, bias=None, norm="rms", group=128, eps=1e-6, return_stats=False):
+    """A residual's addition and the next norm, whose output leaves in 8 bits for an 8-bit projection:
+
+        x = residual + o;   n = Norm(x) weight + bias;   values, scales = n in 8 bits, as `ttt_tk_b200.saved.pack8` has them
+
+    `o` [..., D] (D <= 8192), `residual`, `weight`, `bias`, `norm` and eps as `norm_gate_residual`'s `o`, `residual`, `pre_weight`, `pre_bias`.  `group`: the
+    neighbouring values that share a scale, 32, 64 or 128, or None for one scale to a token.  Returns (x, values, scales): x is `o` itself
+    without a residual, values float8_e4m3fn like o, scales fp32 [..., ceil(D / group)] or [...].  n is that of x before x is rounded, and
+    is rounded once.  With `return_stats` also the fp32 [tokens, 4] from which `norm_gate_residual_backward` (with `pre_weight` and `pre_bias`) takes
+    the gradients for those of x and n."""
+    _need(isinstance(norm, str) and norm in _NORMS, f"norm must be 'rms' or 'layer', got {norm!r}")
+    _need(group is None or (isinstance(group, int) and not isinstance(group, bool) and group in (32, 64, 128)),
+          f"group must be 32, 64, 128 or None, got {group!r}")
+    r = ssm._host().norm8(o, residual, weight, bias, _NORMS[norm], group or 0, eps, return_stats)
+    return r if return_stats else r[:3]
+
+
 def norm_gate_residual_backward(grad_x, grad_n, o, stats, residual=None, gate=None, *, norm="rms", activation="silu", post_weight=None,
                                 post_bias=None, scale=None, pre_weight=None, pre_bias=None, eps=1e-6):
     """Gradients of `norm_gate_residual` from its inputs and `stats`: (grad_o, grad_residual, grad_gate, grad_post_weight,

@@ -1,0 +1,36 @@
+"""Activations that a forward pass keeps for its backward pass in 8 bits (CUDA, `csrc/ttt_eight_bits.cu`), at half the memory of 16 bits.
+
+    (qx, sx), (qg, sg) = pack8(x, gate)                  # values float8_e4m3fn, scales fp32 [..., ceil(D / 128)]
+    x, gate = unpack8((qx, sx), (qg, sg))                # bf16
+
+Of each `group` neighbouring values of a row the scale is the least power of two with max |v| <= 448 scale, and v / scale is kept in e4m3: a
+value is off by at most 2^-4 of itself (and by 2^-10 of the scale where it is below 2^-6 of it), the largest of a group among them.  A power of two divides exactly, so
+the format's rounding is the only one.  Infinities are left out of the maximum and become 448 scale; NaN stays NaN.
+
+`ttt_tk_b200.ssm.gated_scan_backward` takes packed inputs as they are; the differentiable operators of `ttt_tk_b200.autograd` with `saved="e4m3"` keep
+theirs this way.  Calls are stream-ordered and do not synchronise.  A bad argument raises ValueError.
+"""
+from . import ssm
+
+_TYPES = {"torch.bfloat16": 0, "torch.float16": 1, "torch.float32": 2}
+
+
+def pack8(*xs, group=128):
+    """One to four tensors [..., D] of the same shape and type (bf16, fp16 or fp32, rows at a fixed distance) -> a list of (values, scales), one
+    launch.  `group`: 32, 64 or 128."""
+    return ssm._host().pack8(xs, _group(group, "32, 64 or 128"))
+
+
+def unpack8(*packs, dtype=None):
+    """The values that (values, scales) stand for, in `dtype` (bf16 by default, fp16 or fp32), for one to four of the same shape, one launch.  The group is
+    that of the scales' shape; [...] is one scale to a row (`glue.norm_residual_8bit` with group None)."""
+    code = 0 if dtype is None else _TYPES.get(str(dtype)) if str(dtype) in _TYPES and not isinstance(dtype, str) else None
+    if code is None:
+        raise ValueError(f"dtype must be torch.bfloat16, torch.float16 or torch.float32, got {dtype!r}")
+    return ssm._host().unpack8(packs, code)
+
+
+def _group(group, what):
+    if not isinstance(group, int) or isinstance(group, bool) or group < 1 or group > 128:
+        raise ValueError(f"group must be {what}, got {group!r}")
+    return group
