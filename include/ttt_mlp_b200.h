@@ -484,7 +484,7 @@ typedef struct ttt_b200_gated_args {
   float* grad_state;          /* [B][D] or NULL */
   /* backward with `group` 32, 64 or 128: x and the gates are e4m3 bytes of contiguous rows, with a scale for each `group` channels */
   const float *x_scales, *gate_scales, *input_scales; /* [B][T][ceil(D / group)] */
-  void* scratch;              /* ttt_b200_gated_scan_scratch_bytes, 16-byte aligned */
+  void* scratch;              /* ttt_b200_gated_scan_scratch_bytes, 16-byte aligned; may be NULL where that is 0 */
   uint64_t scratch_bytes;
   /* step: the table of states, and which of its rows each row of the batch has */
   float* state_io;            /* [rows][D], updated in place */
@@ -494,8 +494,9 @@ typedef struct ttt_b200_gated_args {
 } ttt_b200_gated_args;
 int ttt_b200_gated_scan(const ttt_b200_gated_args* args, void* stream);
 int ttt_b200_gated_scan_backward(const ttt_b200_gated_args* args, void* stream);
-/* Bytes of scratch the backward needs: the sums' parts, 12 bytes per channel, sequence and CTA along it (at most 8). */
-uint64_t ttt_b200_gated_scan_scratch_bytes(const ttt_b200_gated_args* args);
+/* Bytes of scratch the forward (backward = 0) or backward needs; depends on B, T, D and the GPU: where a sequence is cut into chunks (at most 32) 8 bytes
+ * per channel and chunk, in the backward 12 more per channel and chunk. */
+uint64_t ttt_b200_gated_scan_scratch_bytes(const ttt_b200_gated_args* args, int backward);
 /* One token per row; slots as in ttt_b200_short_conv_step. */
 int ttt_b200_gated_scan_step(const ttt_b200_gated_args* args, void* stream);
 

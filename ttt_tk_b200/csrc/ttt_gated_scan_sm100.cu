@@ -11,9 +11,9 @@
 // operations and six of the exponential unit.  A recurrence of steps h -> p h + q joins: two after one another are p2 p1, p2 q1 + q2.  So a
 // warp has S tokens of 64 channels in registers (two neighbouring channels to a lane), the warps of a CTA have the tokens behind one another
 // of a tile, each takes its tokens from zero, and all join what is in front of them over shared memory: one pass over the data, one barrier.
-// Where channels and sequences do not fill the GPU the CTAs of a cluster have tiles behind one another and join over distributed
-// shared memory, with one cluster barrier more.  The order of the joins is fixed.
-// The backward starts each tile from the state that the forward left of it and joins both directions over the same barrier.
+// The backward starts every 64 tokens from the state that the forward left of them and joins both directions over the same barrier.
+// Where channels and sequences do not fill the GPU the sequence is cut into chunks: a first kernel leaves what each chunk does to a state, and
+// every chunk of the main one begins with the steps of those in front of it.  The order of the joins is fixed.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -28,20 +28,20 @@ using namespace ttt;
 
 using F = float2;
 using E4 = __nv_fp8_e4m3;
-constexpr int kTile = TTT_B200_GATED_INTERVAL;      // tokens of a CTA's tile, and between two checkpoints
+constexpr int kEvery = TTT_B200_GATED_INTERVAL;     // tokens between two checkpoints
+constexpr int S = 8;                                // tokens of a warp's part of a tile; a tile is W of them, 64 tokens or 128
 constexpr int kCols = 64;                           // channels of a CTA
 
-#ifndef TTT_FWD_CTAS
-#define TTT_FWD_CTAS 2
-#define TTT_BWD_CTAS 2
-#define TTT_FWD_S 8
-#define TTT_BWD_S 8
-#endif
+constexpr int kMostChunks = 32;
+
 struct Plan {
-  int tiles;      // CTAs (clusters) side by side: channels / 64
-  int cluster;    // CTAs that have tiles behind one another
-  int nck;        // tiles of a sequence
-  float* part;    // backward: [B * cluster][3][D]
+  int tiles;      // CTAs side by side: channels / 64
+  int nck;        // checkpoints of a sequence
+  int warps;      // of a CTA
+  int chunk;      // tiles that a CTA has
+  int chunks;
+  float* ends;    // [B][chunks][2][D]: p and q of a chunk's step p h + q
+  float* part;    // backward: [B * chunks][3][D]
 };
 
 // ---- arithmetic, two channels at a time ----------------------------------------------------------------------------------------
@@ -59,6 +59,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 __device__ __forceinline__ float rsqrt_fast(float v) {
   float r;
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float sqrt_fast(float v) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
 __device__ __forceinline__ F neg(F a) { return mul2(a, both(-1.f)); }
@@ -134,7 +139,7 @@ __device__ __forceinline__ void factors(const Weights& z, Gate gate, Input input
       f.w = mul2(q, r);
       f.slope = mul2(mul2(f.a, f.a), neg(r));
     } else {
-      f.w = mul2(q, make_float2(rsqrt_fast(max_nan(q.x, 1.17549435e-38f)), rsqrt_fast(max_nan(q.y, 1.17549435e-38f))));
+      f.w = make_float2(sqrt_fast(q.x), sqrt_fast(q.y));
     }
   } else if (z.mix == TTT_B200_MIX_LINEAR) {
     f.w = rest;
@@ -151,6 +156,16 @@ __device__ __forceinline__ void factors(const Weights& z, Gate gate, Input input
   } else if constexpr (kBack) {
     f.rest = both(0.f);
   }
+}
+
+// a alone
+template <bool kUsual> __device__ __forceinline__ F decay(const Weights& z, F gate) {
+  F s, o;
+  sigmoid<false>(gate, z.gate_bias, 0.f, s, o);
+  if (!kUsual && !z.has_a) return s;
+  F a, rest;
+  exp_both(mul2(s, z.A), a, rest);
+  return a;
 }
 
 // ---- rows through shared memory ------------------------------------------------------------------------------------------------
@@ -184,7 +199,7 @@ template <class T> __device__ __forceinline__ float value_of(uint32_t at) {
 //   otherwise the 16-byte blocks that a row touches (the first and the last may hold its neighbours too), from which values are picked one
 //             by one at the row's offset
 // 8-bit values come with their scales, two to a row (one for each 32 channels).
-template <class T, int S, bool kWhole> struct Rows {
+template <class T, bool kWhole> struct Rows {
   static constexpr int es = sizeof(T), kBytes = kCols * es, kPitch = kWhole ? kBytes : kBytes + 16, kPieces = kPitch / 16;
   static constexpr bool kScaled = es == 1;
   static constexpr uint32_t kStage = S * kPitch + (kScaled ? S * 8 : 0);      // bytes
@@ -287,81 +302,166 @@ template <bool kWhole> __device__ __forceinline__ Weights weights_of(const ttt_b
 }
 
 // ---- joins -----------------------------------------------------------------------------------------------------------------------------
-// The warp that has written to the other CTAs releases what it wrote, and what the CTA's barrier in front has put in front of it; for the other
-// warps there is nothing to wait for (a release waits for all of a warp's stores, those of y among them).
-__device__ __forceinline__ void cluster_arrive(bool wrote) {
-  if (wrote) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  else asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ int cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
-  return static_cast<int>(r);
-}
-__device__ __forceinline__ void store_remote(const void* mine, int rank, float4 v) {
-  uint32_t at;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine))), "r"(rank));
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
-}
-constexpr int kMostCluster = 16;
 __device__ __forceinline__ F first2(float4 v) { return make_float2(v.x, v.y); }
 __device__ __forceinline__ F second2(float4 v) { return make_float2(v.z, v.w); }
 __device__ __forceinline__ float4 four(F a, F b) { return make_float4(a.x, a.y, b.x, b.y); }
 
-// Steps p h + q of the warps of a tile and of the tiles of a cluster, in two halves that alternate (a barrier lies between two uses of
-// the same one).
+// Steps p h + q of the warps of a tile, in two halves that alternate (a barrier lies between two uses of the same one).
 template <int W> struct Steps {
-  float4 warp[2][W][32], tile[2][kMostCluster][32];
-  F end[2][32];      // what a tile leaves, where a CTA has all of them
+  float4 warp[2][W][32];
+  F end[2][32];      // what a tile leaves
 };
 
-struct At {
-  int tile, b, rank, d, lane, warp, len;
-  template <class P> __device__ __forceinline__ At(const P& p, const Plan& q) {
-    rank = q.cluster > 1 ? cluster_rank() : 0;
-    const int i = blockIdx.x / q.cluster;
-    tile = i % q.tiles;
-    b = i / q.tiles;
+template <int W> struct At {
+  static constexpr int kTile = S * W;
+  int tile, b, chunk, d, lane, warp, len, first, last;      // `first`, `last`: tiles of the chunk that have tokens, and the one behind them
+  __device__ __forceinline__ At(const ttt_b200_gated_args& p, const Plan& q, int chunks) {
+    const int i = blockIdx.x / q.tiles;
+    tile = blockIdx.x % q.tiles;
+    chunk = i % chunks;
+    b = i / chunks;
     lane = threadIdx.x & 31;
-    warp = threadIdx.x >> 5;
+    warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);      // known to be the same for a warp: addresses in uniform registers
     d = tile * kCols + 2 * lane;
     len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+    first = chunk * q.chunk;
+    last = max(first, min(first + q.chunk, (len + kTile - 1) / kTile));
   }
+  // behind the chunk's last tile
+  __device__ __forceinline__ int end(const Plan& q, int p_T) const { return min((chunk + 1) * q.chunk, (p_T + kTile - 1) / kTile); }
 };
+// Of what stands in front of a chunk (backward: behind it) the steps, one after another.
+template <bool kWhole, bool kBack, class W> __device__ __forceinline__ F join_chunks(const ttt_b200_gated_args& p, const Plan& q, const W& at, F h) {
+  const int n = kBack ? q.chunks - 1 - at.chunk : at.chunk;
+  const float* ends = q.ends + static_cast<long>(at.b) * q.chunks * 2 * p.D;
+#pragma unroll 8
+  for (int k = 0; k < n; ++k) {
+    const float* e = ends + static_cast<long>(kBack ? q.chunks - 1 - k : k) * 2 * p.D;
+    h = fma2(load2<kWhole>(e, at.d, p.D, 1.f), h, load2<kWhole>(e + p.D, at.d, p.D, 0.f));
+  }
+  return h;
+}
 
 constexpr int kStages = 2;
 
-template <class T, bool kWhole, bool kUsual, int S, int W>
-__global__ void __launch_bounds__(32 * W, TTT_FWD_CTAS) gated_forward_kernel(const ttt_b200_gated_args p, const Plan q) {
-  static_assert(S * W == kTile, "the warps' tokens make a tile");
+// Where channels and sequences do not fill the GPU: a chunk's step p h + q, forward (kBack: backward, of which q is c in front of the chunk for
+// nothing behind it).  Each warp has tokens after one another, and nothing to wait for until the end.  What the main kernels compute of a token is
+// computed here before: but for the last chunk (the first one).
+template <class T, class I, bool kWhole, bool kUsual, bool kBack, int W>
+__global__ void __launch_bounds__(32 * W, 16 / W) gated_ends_kernel(const ttt_b200_gated_args p, const Plan q) {
   wait_for_predecessor();
-  using R = Rows<T, S, kWhole>;
+  using R = Rows<I, kWhole>;
+  using U = Rows<T, kWhole>;
+  constexpr uint32_t kStage = kBack ? R::kStage + U::kStage : 3 * R::kStage;
+  __shared__ float4 steps[W][32];
+  extern __shared__ __align__(16) unsigned char rings[];
+  At<W> at(p, q, q.chunks - 1);
+  constexpr int kTile = At<W>::kTile;
+  if constexpr (kBack) {      // all but the first
+    at.first += q.chunk;
+    ++at.chunk;
+    at.last = max(at.first, min(at.first + q.chunk, (at.len + kTile - 1) / kTile));
+  }
+  const int d0 = at.tile * kCols;
+  const Weights z = weights_of<kWhole>(p, at.d);
+  const int groups = p.group ? (p.D + p.group - 1) / p.group : 0;
+  const R rx(p.x, p.x_stride[0], p.x_stride[1], at.b, d0, p.D, p.x_scales, groups, p.group, p.T),
+      rg(p.gate, p.gate_stride[0], p.gate_stride[1], at.b, d0, p.D, p.gate_scales, groups, p.group, p.T),
+      ri(p.input_gate, p.input_stride[0], p.input_stride[1], at.b, d0, p.D, p.input_scales, groups, p.group, p.T);
+  const U ru(p.grad_y, p.gy_stride[0], p.gy_stride[1], at.b, d0, p.D);
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(rings)) + at.warp * (kStages * kStage);
+  const int rounds = at.last - at.first, first = at.first * kTile + at.warp * rounds * S;
+  auto ahead = [&](int j) {
+    if (j < rounds) {
+      const uint32_t to = ring + j % kStages * kStage;
+      const int t = first + j * S;
+      rg.copy(to, t, at.len);
+      if constexpr (kBack) {
+        ru.copy(to + R::kStage, t, at.len);
+      } else {
+        rx.copy(to + R::kStage, t, at.len);
+        if (kUsual || z.gated) ri.copy(to + 2 * R::kStage, t, at.len);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int j = 0; j < kStages - 1; ++j) ahead(j);
+  F whole = both(1.f), own = both(0.f);
+  for (int j = 0; j < rounds; ++j) {
+    cp_async_wait<kStages - 2>();
+    __syncwarp();      // the rows have landed for all lanes, and all are through with the place that the next ones take
+    ahead(j + kStages - 1);
+    const uint32_t from = ring + j % kStages * kStage;
+    const int t0 = first + j * S;
+    F a[S], u[S];
+#pragma unroll
+    for (int t = 0; t < S; ++t) {
+      if constexpr (kBack) {
+        a[t] = decay<kUsual>(z, rg.get(from, t, t0 + t));
+        u[t] = ru.get(from + R::kStage, t, t0 + t);
+      } else {
+        Factors<false> f;
+        factors<kUsual, false>(z, rg.get(from, t, t0 + t), [&] { return ri.get(from + 2 * R::kStage, t, t0 + t); }, f);
+        a[t] = f.a;
+        u[t] = mul2(f.w, rx.get(from + R::kStage, t, t0 + t));
+      }
+    }
+    if (t0 + S > at.len) {
+#pragma unroll
+      for (int t = 0; t < S; ++t)
+        if (t0 + t >= at.len) a[t] = both(1.f), u[t] = both(0.f);
+    }
+#pragma unroll
+    for (int t = 0; t < S; ++t) {
+      whole = mul2(whole, a[t]);
+      own = kBack ? fma2(whole, u[t], own) : fma2(a[t], own, u[t]);
+    }
+  }
+  steps[at.warp][at.lane] = four(whole, own);
+  __syncthreads();
+  if (at.warp) return;
+#pragma unroll
+  for (int w = 1; w < W; ++w) {
+    const float4 v = steps[w][at.lane];
+    own = kBack ? fma2(whole, second2(v), own) : fma2(first2(v), own, second2(v));
+    whole = mul2(whole, first2(v));
+  }
+  float* e = q.ends + (static_cast<long>(at.b) * q.chunks + at.chunk) * 2 * p.D;
+  store2<float, kWhole>(e, at.d, p.D, whole);
+  store2<float, kWhole>(e + p.D, at.d, p.D, own);
+}
+
+template <class T, bool kWhole, bool kUsual, int W>
+__global__ void __launch_bounds__(32 * W, 16 / W) gated_forward_kernel(const ttt_b200_gated_args p, const Plan q) {
+  wait_for_predecessor();
+  using R = Rows<T, kWhole>;
   __shared__ Steps<W> join;
   extern __shared__ __align__(16) unsigned char rings[];
-  const At at(p, q);
-  const int d0 = at.tile * kCols, C = q.cluster;
+  const At<W> at(p, q, q.chunks);
+  constexpr int kTile = At<W>::kTile;
+  const int d0 = at.tile * kCols;
   const Weights z = weights_of<kWhole>(p, at.d);
   const R rx(p.x, p.x_stride[0], p.x_stride[1], at.b, d0, p.D), rg(p.gate, p.gate_stride[0], p.gate_stride[1], at.b, d0, p.D),
       ri(p.input_gate, p.input_stride[0], p.input_stride[1], at.b, d0, p.D);
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(rings)) + at.warp * (kStages * 3 * R::kStage);
-  const int hop = C * kTile, first = at.rank * kTile + at.warp * S;      // tokens from one tile of a CTA to its next; the warp's first
-  const int rounds = (at.len + hop - 1) / hop;
+  const int first = at.first * kTile + at.warp * S, rounds = at.last - at.first;
   auto ahead = [&](int j) {
     if (j < rounds) {
       const uint32_t to = ring + j % kStages * (3 * R::kStage);
-      rx.copy(to, first + j * hop, at.len);
-      rg.copy(to + R::kStage, first + j * hop, at.len);
-      if (kUsual || z.gated) ri.copy(to + 2 * R::kStage, first + j * hop, at.len);
+      rx.copy(to, first + j * kTile, at.len);
+      rg.copy(to + R::kStage, first + j * kTile, at.len);
+      if (kUsual || z.gated) ri.copy(to + 2 * R::kStage, first + j * kTile, at.len);
     }
     cp_async_commit();
   };
 #pragma unroll
   for (int j = 0; j < kStages - 1; ++j) ahead(j);
   F carry = load2<kWhole>(p.state ? p.state + static_cast<long>(at.b) * p.D : nullptr, at.d, p.D, 0.f);
+  carry = join_chunks<kWhole, false>(p, q, at, carry);
   T* y = static_cast<T*>(p.y) + static_cast<long>(at.b) * p.T * p.D;
   for (int j = 0; j < rounds; ++j) {
-    const int t0 = first + j * hop, half = j & 1;
+    const int t0 = first + j * kTile, half = j & 1;
     cp_async_wait<kStages - 2>();
     __syncwarp();      // the rows have landed for all lanes, and all are through with the place that the next ones take
     ahead(j + kStages - 1);
@@ -386,36 +486,15 @@ __global__ void __launch_bounds__(32 * W, TTT_FWD_CTAS) gated_forward_kernel(con
     }
     join.warp[half][at.warp][at.lane] = four(whole, own);
     __syncthreads();
-    F h = C > 1 || j == 0 ? carry : join.end[half ^ 1][at.lane];
-    if (C > 1) {
-      if (at.warp == 0) {
-        F P = both(1.f), H = both(0.f);
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const float4 v = join.warp[half][w][at.lane];
-          P = mul2(P, first2(v));
-          H = fma2(first2(v), H, second2(v));
-        }
-        for (int r = 0; r < C; ++r) store_remote(&join.tile[half][at.rank][at.lane], r, four(P, H));
-      }
-      cluster_arrive(at.warp == 0);
-      cluster_wait();
-      F next = carry;
-      for (int r = 0; r < C; ++r) {
-        if (r == at.rank) h = next;
-        const float4 v = join.tile[half][r][at.lane];
-        next = fma2(first2(v), next, second2(v));
-      }
-      carry = next;
-    }
-    if (at.warp == 0 && p.checkpoints && t0 < at.len)
-      store2<float, kWhole>(p.checkpoints + (static_cast<long>(at.b) * q.nck + j * C + at.rank) * p.D, at.d, p.D, h);
+    F h = j == 0 ? carry : join.end[half ^ 1][at.lane];
 #pragma unroll
     for (int w = 0; w < W - 1; ++w) {
       if (w >= at.warp) break;
       const float4 v = join.warp[half][w][at.lane];
       h = fma2(first2(v), h, second2(v));
     }
+    if (at.warp % (kEvery / S) == 0 && p.checkpoints && t0 < at.len)
+      store2<float, kWhole>(p.checkpoints + (static_cast<long>(at.b) * q.nck + t0 / kEvery) * p.D, at.d, p.D, h);
     T* to = y + static_cast<long>(t0) * p.D;
     if (t0 + S <= at.len) {
 #pragma unroll
@@ -432,26 +511,26 @@ __global__ void __launch_bounds__(32 * W, TTT_FWD_CTAS) gated_forward_kernel(con
         to += p.D;
       }
     }
-    if (C == 1 && at.warp == W - 1) carry = join.end[half][at.lane] = h;
+    if (at.warp == W - 1) carry = join.end[half][at.lane] = h;
   }
-  if (p.final_state && at.rank == 0 && at.warp == W - 1) store2<float, kWhole>(p.final_state + static_cast<long>(at.b) * p.D, at.d, p.D, carry);
-  for (int t0 = first + rounds * hop; t0 < p.T; t0 += hop)
-    for (int t = t0; t < min(t0 + S, p.T); ++t) store2<T, kWhole>(y + static_cast<long>(t) * p.D, at.d, p.D, both(0.f));
+  if (p.final_state && at.chunk == q.chunks - 1 && at.warp == W - 1) store2<float, kWhole>(p.final_state + static_cast<long>(at.b) * p.D, at.d, p.D, carry);
+  for (int j = at.last; j < at.end(q, p.T); ++j)
+    for (int t = j * kTile + at.warp * S; t < min(j * kTile + at.warp * S + S, p.T); ++t) store2<T, kWhole>(y + static_cast<long>(t) * p.D, at.d, p.D, both(0.f));
 }
 
 // T: the gradients' type; I: that of x and the gates, or 8-bit values
-template <class T, class I, bool kWhole, bool kUsual, int S, int W>
-__global__ void __launch_bounds__(32 * W, TTT_BWD_CTAS) gated_backward_kernel(const ttt_b200_gated_args p, const Plan q) {
-  static_assert(S * W == kTile, "the warps' tokens make a tile");
+template <class T, class I, bool kWhole, bool kUsual, int W>
+__global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const ttt_b200_gated_args p, const Plan q) {
   wait_for_predecessor();
-  using R = Rows<I, S, kWhole>;
-  using U = Rows<T, S, kWhole>;
+  using R = Rows<I, kWhole>;
+  using U = Rows<T, kWhole>;
   constexpr uint32_t kStage = 3 * R::kStage + U::kStage;
   __shared__ Steps<W> join;
   __shared__ F back[2][W][32];
   extern __shared__ __align__(16) unsigned char rings[];
-  const At at(p, q);
-  const int d0 = at.tile * kCols, C = q.cluster;
+  const At<W> at(p, q, q.chunks);
+  constexpr int kTile = At<W>::kTile;
+  const int d0 = at.tile * kCols;
   const Weights z = weights_of<kWhole>(p, at.d);
   const bool gated = kUsual || z.gated;
   const int groups = p.group ? (p.D + p.group - 1) / p.group : 0;
@@ -460,15 +539,14 @@ __global__ void __launch_bounds__(32 * W, TTT_BWD_CTAS) gated_backward_kernel(co
       ri(p.input_gate, p.input_stride[0], p.input_stride[1], at.b, d0, p.D, p.input_scales, groups, p.group, p.T);
   const U ru(p.grad_y, p.gy_stride[0], p.gy_stride[1], at.b, d0, p.D);
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(rings)) + at.warp * (kStages * kStage);
-  const int hop = C * kTile, first = at.rank * kTile + at.warp * S;
-  const int rounds = (at.len + hop - 1) / hop;
+  const int first = at.first * kTile + at.warp * S, rounds = at.last - at.first;
   auto ahead = [&](int j) {
     if (j >= 0) {
       const uint32_t to = ring + j % kStages * kStage;
-      rx.copy(to, first + j * hop, at.len);
-      rg.copy(to + R::kStage, first + j * hop, at.len);
-      if (gated) ri.copy(to + 2 * R::kStage, first + j * hop, at.len);
-      ru.copy(to + 3 * R::kStage, first + j * hop, at.len);
+      rx.copy(to, first + j * kTile, at.len);
+      rg.copy(to + R::kStage, first + j * kTile, at.len);
+      if (gated) ri.copy(to + 2 * R::kStage, first + j * kTile, at.len);
+      ru.copy(to + 3 * R::kStage, first + j * kTile, at.len);
     }
     cp_async_commit();
   };
@@ -482,11 +560,12 @@ __global__ void __launch_bounds__(32 * W, TTT_BWD_CTAS) gated_backward_kernel(co
     if (gated) store2<T, kWhole>(gi + o, at.d, p.D, i);
   };
   F carry = load2<kWhole>(p.grad_final_state ? p.grad_final_state + static_cast<long>(at.b) * p.D : nullptr, at.d, p.D, 0.f);
+  carry = join_chunks<kWhole, true>(p, q, at, carry);
   F sum_a = both(0.f), sum_g = sum_a, sum_i = sum_a;
   for (int j = rounds - 1; j >= 0; --j) {
-    const int t0 = first + j * hop, half = j & 1;
-    const bool some = t0 - at.warp * S < at.len;      // of the tile's tokens (else there is no checkpoint)
-    F h = load2<kWhole>(some ? p.checkpoints + (static_cast<long>(at.b) * q.nck + j * C + at.rank) * p.D : nullptr, at.d, p.D, 0.f);
+    const int t0 = first + j * kTile, half = j & 1;
+    const int ck = t0 / kEvery;
+    F h = load2<kWhole>(ck * kEvery < at.len ? p.checkpoints + (static_cast<long>(at.b) * q.nck + ck) * p.D : nullptr, at.d, p.D, 0.f);
     cp_async_wait<kStages - 2>();
     __syncwarp();
     ahead(j - kStages + 1);
@@ -517,24 +596,11 @@ __global__ void __launch_bounds__(32 * W, TTT_BWD_CTAS) gated_backward_kernel(co
     join.warp[half][at.warp][at.lane] = four(whole, own);
     back[half][at.warp][at.lane] = left;
     __syncthreads();
-    F c = C > 1 || j == rounds - 1 ? carry : join.end[half ^ 1][at.lane];
-    if (C > 1) {
-      if (at.warp == W - 1) {
-        F P = both(1.f), Q = both(0.f);
+    F c = j == rounds - 1 ? carry : join.end[half ^ 1][at.lane];
 #pragma unroll
-        for (int v = W - 1; v >= 0; --v) {
-          const F f = first2(join.warp[half][v][at.lane]);
-          P = mul2(P, f);
-          Q = fma2(f, Q, back[half][v][at.lane]);
-        }
-        for (int r = 0; r < C; ++r) store_remote(&join.tile[half][at.rank][at.lane], r, four(P, Q));
-      }
-      cluster_arrive(at.warp == W - 1);
-    }
-#pragma unroll
-    for (int v = 0; v < W; ++v) {
-      if (v >= at.warp) break;
-      const float4 f = join.warp[half][v][at.lane];
+    for (int v = 0; v < kEvery / S - 1; ++v) {
+      if (v >= at.warp % (kEvery / S)) break;
+      const float4 f = join.warp[half][at.warp / (kEvery / S) * (kEvery / S) + v][at.lane];
       h = fma2(first2(f), h, second2(f));
     }
     // to h_{t-1}, and with it to d log a / G
@@ -543,16 +609,6 @@ __global__ void __launch_bounds__(32 * W, TTT_BWD_CTAS) gated_backward_kernel(co
       const F kept = mul2(a[t], h);
       slope[t] = add2(kept, slope[t]);
       h = fma2(w[t], rx.get(from, t, t0 + t), kept);
-    }
-    if (C > 1) {
-      cluster_wait();
-      F next = carry;
-      for (int r = C - 1; r >= 0; --r) {
-        if (r == at.rank) c = next;
-        const float4 v = join.tile[half][r][at.lane];
-        next = fma2(first2(v), next, second2(v));
-      }
-      carry = next;
     }
 #pragma unroll
     for (int v = W - 1; v > 0; --v) {
@@ -579,11 +635,11 @@ __global__ void __launch_bounds__(32 * W, TTT_BWD_CTAS) gated_backward_kernel(co
         else if (t0 + t < p.T) put(o, both(0.f), both(0.f), both(0.f));
       }
     }
-    if (C == 1 && at.warp == 0) carry = join.end[half][at.lane] = c;
+    if (at.warp == 0) carry = join.end[half][at.lane] = c;
   }
-  if (p.grad_state && at.rank == 0 && at.warp == 0) store2<float, kWhole>(p.grad_state + static_cast<long>(at.b) * p.D, at.d, p.D, carry);
-  for (int t0 = first + rounds * hop; t0 < p.T; t0 += hop)
-    for (int t = t0; t < min(t0 + S, p.T); ++t) put(static_cast<long>(t) * p.D, both(0.f), both(0.f), both(0.f));
+  if (p.grad_state && at.chunk == 0 && at.warp == 0) store2<float, kWhole>(p.grad_state + static_cast<long>(at.b) * p.D, at.d, p.D, carry);
+  for (int j = at.last; j < at.end(q, p.T); ++j)
+    for (int t = j * kTile + at.warp * S; t < min(j * kTile + at.warp * S + S, p.T); ++t) put(static_cast<long>(t) * p.D, both(0.f), both(0.f), both(0.f));
   // the warps' sums, in their order
   __shared__ F sums[3][W][32];
   sums[0][at.warp][at.lane] = sum_a;
@@ -598,7 +654,7 @@ __global__ void __launch_bounds__(32 * W, TTT_BWD_CTAS) gated_backward_kernel(co
       const F A = load2<kWhole>(p.A, at.d, p.D, 0.f);
       s = make_float2(A.x > 0.f ? 0.f : s.x, A.y > 0.f ? 0.f : s.y);
     }
-    store2<float, kWhole>(q.part + (static_cast<long>(at.b) * C + at.rank) * 3 * p.D + static_cast<long>(at.warp) * p.D, at.d, p.D, s);
+    store2<float, kWhole>(q.part + (static_cast<long>(at.b) * q.chunks + at.chunk) * 3 * p.D + static_cast<long>(at.warp) * p.D, at.d, p.D, s);
   }
 }
 
@@ -671,65 +727,85 @@ bool whole(const ttt_b200_gated_args& p, bool backward) {
   return ok && rows16(p.grad_y, p.gy_stride, es) && even(p.grad_x, es) && even(p.grad_gate, es) && even(p.grad_input, es);
 }
 
-// CTAs of a cluster: as many as leave two to three CTAs to an SM, and no more than there are tiles.
-void plan(Plan& q, const ttt_b200_gated_args& p) {
+// How many chunks a sequence is cut into, of how many tiles, and whether a CTA has 8 warps (two CTAs to an SM) or 16: by what a round of tiles takes, in
+// tenths of a microsecond, measured with 2048 channels and more or fewer sequences.  A CTA of 8 warps that has an SM for itself 15 (it waits for itself), two
+// of them or one of 16 warps 24; the chunks' steps 0.6 of the main kernel, a launch and a start 30.
+// 16384 tokens of 1024 channels, forward / backward us: one chunk 348 / 673, 8 chunks 89 / 126, 18 (by the rule) 73 / 97, 24 83 / 116.
+void plan(Plan& q, const ttt_b200_gated_args& p, bool backward) {
   q.tiles = (p.D - 1) / kCols + 1;
-  q.nck = (p.T - 1) / kTile + 1;
+  q.nck = (p.T - 1) / kEvery + 1;
   const long columns = static_cast<long>(q.tiles) * p.B, sms = sm_count();
-  for (q.cluster = 1; q.cluster < kMostCluster && q.cluster < q.nck && columns * q.cluster < sms; q.cluster *= 2) {}
+  auto main = [&](long ctas, long rounds) { return 30 + (ctas <= sms ? 15 : 24 * ((ctas + 2 * sms - 1) / (2 * sms))) * rounds; };
+  long best = main(columns, q.nck);
+  q.warps = 8;
+  q.chunk = q.nck;
+  // (16 warps' rows of four fp32 tensors are more than the shared memory holds)
+  if (columns <= sms && p.T > 8 * S && !(backward && p.dtype == TTT_B200_FP32 && !p.group)) {
+    const int rounds = (p.T - 1) / (16 * S) + 1;
+    const long cost = 30 + 24L * rounds;
+    if (cost < best) best = cost, q.warps = 16, q.chunk = rounds;
+  }
+  for (int n = 2; n <= std::min(kMostChunks, q.nck); ++n) {
+    const int chunk = (q.nck + n - 1) / n, chunks = (q.nck + chunk - 1) / chunk;
+    const long cost = main(columns * chunks, chunk) + main(columns * (chunks - 1), chunk) * 6 / 10 + 20;
+    if (cost < best) best = cost, q.warps = 8, q.chunk = chunk;
+  }
 #ifdef TTT_PROBE
-  if (getenv("TTT_PROBE_C")) q.cluster = atoi(getenv("TTT_PROBE_C"));
+  if (getenv("TTT_PROBE_C")) q.warps = 8, q.chunk = (q.nck + atoi(getenv("TTT_PROBE_C")) - 1) / atoi(getenv("TTT_PROBE_C"));
+  if (getenv("TTT_PROBE_W")) q.warps = 16, q.chunk = (p.T - 1) / (16 * S) + 1;
 #endif
+  const int tiles = (p.T - 1) / (q.warps * S) + 1;
+  q.chunks = (tiles + q.chunk - 1) / q.chunk;
 }
+// scratch: the chunks' steps, and behind them the sums' parts
+uint64_t ends_bytes(const Plan& q, const ttt_b200_gated_args& p) { return q.chunks > 1 ? (static_cast<uint64_t>(p.B) * q.chunks * 2 * p.D * sizeof(float) + 15) / 16 * 16 : 0; }
 
-template <auto kKernel> int launch(const Plan& q, const ttt_b200_gated_args& p, int threads, uint32_t bytes, cudaStream_t s, const char* what) {
-  const long grid = static_cast<long>(p.B) * q.tiles * q.cluster;
+template <auto kKernel> int launch(long grid, const Plan& q, const ttt_b200_gated_args& p, int threads, uint32_t bytes, cudaStream_t s, const char* what) {
   if (grid > 0x7fffffffL) return fail("gated scan: too many CTAs");
   if (bytes > 16 * 1024)      // (with the static part 48 KB is the most without asking)
     if (int rc = allow_shared<kKernel>()) return rc;
-  if (q.cluster > 8)
-    if (cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return ttt_set_error(TTT_B200_ERR_LAUNCH, cudaGetErrorString(e));
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = q.cluster;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = bytes;
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = q.cluster > 1 ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, kKernel, p, q);
+  ttt_launch_overlapped(kKernel, static_cast<int>(grid), threads, bytes, s, p, q);
   return launched(what);
 }
 
 bool usual(const ttt_b200_gated_args& p) { return p.A && p.input_gate && p.mix == TTT_B200_MIX_SQRT; }
 
-template <class T, bool kWhole> int forward(const ttt_b200_gated_args& p, const Plan& q, cudaStream_t s) {
-  constexpr int S = TTT_FWD_S, W = kTile / S;
-  constexpr uint32_t bytes = W * kStages * 3 * Rows<T, S, kWhole>::kStage;
-  return usual(p) ? launch<gated_forward_kernel<T, kWhole, true, S, W>>(q, p, 32 * W, bytes, s, "gated scan")
-                  : launch<gated_forward_kernel<T, kWhole, false, S, W>>(q, p, 32 * W, bytes, s, "gated scan");
+template <class T, bool kWhole, bool kUsual> int forward_as(const ttt_b200_gated_args& p, const Plan& q, cudaStream_t s) {
+  constexpr uint32_t bytes = kStages * 3 * Rows<T, kWhole>::kStage;      // of a warp
+  const long columns = static_cast<long>(p.B) * q.tiles;
+  if (q.warps == 16) return launch<gated_forward_kernel<T, kWhole, kUsual, 16>>(columns, q, p, 512, 16 * bytes, s, "gated scan");
+  if (q.chunks > 1)
+    if (int rc = launch<gated_ends_kernel<T, T, kWhole, kUsual, false, 8>>(columns * (q.chunks - 1), q, p, 256, 8 * bytes, s, "gated scan")) return rc;
+  return launch<gated_forward_kernel<T, kWhole, kUsual, 8>>(columns * q.chunks, q, p, 256, 8 * bytes, s, "gated scan");
 }
-template <class T, class I, bool kWhole> int backward_of(const ttt_b200_gated_args& p, const Plan& q, cudaStream_t s) {
-  constexpr int S = TTT_BWD_S, W = kTile / S;
-  constexpr uint32_t bytes = W * kStages * (3 * Rows<I, S, kWhole>::kStage + Rows<T, S, kWhole>::kStage);
-  return usual(p) ? launch<gated_backward_kernel<T, I, kWhole, true, S, W>>(q, p, 32 * W, bytes, s, "gated scan backward")
-                  : launch<gated_backward_kernel<T, I, kWhole, false, S, W>>(q, p, 32 * W, bytes, s, "gated scan backward");
+template <class T> int forward(const ttt_b200_gated_args& p, cudaStream_t s) {
+  Plan q = {};
+  plan(q, p, false);
+  q.ends = static_cast<float*>(p.scratch);
+  if (whole(p, false)) return usual(p) ? forward_as<T, true, true>(p, q, s) : forward_as<T, true, false>(p, q, s);
+  return usual(p) ? forward_as<T, false, true>(p, q, s) : forward_as<T, false, false>(p, q, s);
+}
+template <class T, class I, bool kWhole, bool kUsual> int backward_as(const ttt_b200_gated_args& p, const Plan& q, cudaStream_t s) {
+  constexpr uint32_t in = kStages * Rows<I, kWhole>::kStage, up = kStages * Rows<T, kWhole>::kStage;      // of a warp
+  const long columns = static_cast<long>(p.B) * q.tiles;
+  if constexpr (16 * (3 * in + up) <= 180 * 1024)
+    if (q.warps == 16) return launch<gated_backward_kernel<T, I, kWhole, kUsual, 16>>(columns, q, p, 512, 16 * (3 * in + up), s, "gated scan backward");
+  if (q.chunks > 1)
+    if (int rc = launch<gated_ends_kernel<T, I, kWhole, kUsual, true, 8>>(columns * (q.chunks - 1), q, p, 256, 8 * (in + up), s, "gated scan backward")) return rc;
+  return launch<gated_backward_kernel<T, I, kWhole, kUsual, 8>>(columns * q.chunks, q, p, 256, 8 * (3 * in + up), s, "gated scan backward");
+}
+template <class T, class I> int backward_of(const ttt_b200_gated_args& p, const Plan& q, cudaStream_t s) {
+  if (whole(p, true)) return usual(p) ? backward_as<T, I, true, true>(p, q, s) : backward_as<T, I, true, false>(p, q, s);
+  return usual(p) ? backward_as<T, I, false, true>(p, q, s) : backward_as<T, I, false, false>(p, q, s);
 }
 template <class T> int backward(const ttt_b200_gated_args& p, cudaStream_t s) {
   Plan q = {};
-  plan(q, p);
-  q.part = static_cast<float*>(p.scratch);
-  int rc;
-  if (p.group) rc = whole(p, true) ? backward_of<T, E4, true>(p, q, s) : backward_of<T, E4, false>(p, q, s);
-  else rc = whole(p, true) ? backward_of<T, T, true>(p, q, s) : backward_of<T, T, false>(p, q, s);
-  if (rc) return rc;
+  plan(q, p, true);
+  q.ends = static_cast<float*>(p.scratch);
+  q.part = reinterpret_cast<float*>(static_cast<char*>(p.scratch) + ends_bytes(q, p));
+  if (int rc = p.group ? backward_of<T, E4>(p, q, s) : backward_of<T, T>(p, q, s)) return rc;
   const long D = p.D;
-  const int parts = p.B * q.cluster;
+  const int parts = p.B * q.chunks;
   const ttt_sum_job jobs[] = {{q.part, p.grad_A, D, 3 * D, parts, TTT_B200_FP32, 0},
                               {q.part + D, p.grad_gate_bias, D, 3 * D, parts, TTT_B200_FP32, 0},
                               {q.part + 2 * D, p.grad_input_bias, D, 3 * D, parts, TTT_B200_FP32, 0}};
@@ -749,11 +825,17 @@ template <class T> int step(const ttt_b200_gated_args& p, cudaStream_t s) {
 
 }  // namespace
 
-extern "C" uint64_t ttt_b200_gated_scan_scratch_bytes(const ttt_b200_gated_args* p) {
+extern "C" uint64_t ttt_b200_gated_scan_scratch_bytes(const ttt_b200_gated_args* p, int backward) {
   if (check(p) || p->B == 0 || p->T == 0) return 0;
   Plan q = {};
-  plan(q, *p);
-  return static_cast<uint64_t>(p->B) * q.cluster * 3 * p->D * sizeof(float);
+  plan(q, *p, backward);
+  return ends_bytes(q, *p) + (backward ? static_cast<uint64_t>(p->B) * q.chunks * 3 * p->D * sizeof(float) : 0);
+}
+
+static int check_scratch(const ttt_b200_gated_args* p, int backward) {
+  const uint64_t need = ttt_b200_gated_scan_scratch_bytes(p, backward);
+  if (need && (!p->scratch || p->scratch_bytes < need || !aligned16(p->scratch))) return fail("gated scan: scratch is missing, too small or not 16-byte aligned");
+  return TTT_B200_OK;
 }
 
 extern "C" int ttt_b200_gated_scan(const ttt_b200_gated_args* p, void* stream) {
@@ -762,10 +844,8 @@ extern "C" int ttt_b200_gated_scan(const ttt_b200_gated_args* p, void* stream) {
   if (p->B == 0 || p->T == 0) return fail("gated scan: no tokens");
   if (p->group) return fail("gated scan: 8-bit inputs are for the backward pass");
   if (p->input_bias && !p->input_gate) return fail("gated scan: input_bias without input_gate");
-  Plan q = {};
-  plan(q, *p);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  TTT_WITH_TYPE(p->dtype, return whole(*p, false) ? (forward<Elem, true>(*p, q, s)) : (forward<Elem, false>(*p, q, s)))
+  if (int rc = check_scratch(p, 0)) return rc;
+  TTT_WITH_TYPE(p->dtype, return forward<Elem>(*p, static_cast<cudaStream_t>(stream)))
   return TTT_B200_OK;
 }
 
@@ -776,8 +856,7 @@ extern "C" int ttt_b200_gated_scan_backward(const ttt_b200_gated_args* p, void* 
   if (p->group && (!p->x_scales || !p->gate_scales || (p->input_gate && !p->input_scales))) return fail("gated scan backward: 8-bit inputs without scales");
   if (p->B == 0 || p->T == 0) return fail("gated scan backward: no tokens");
   if ((p->input_bias && !p->input_gate) || (p->grad_A && !p->A)) return fail("gated scan backward: a gradient or bias of what is not there");
-  if (!p->scratch || p->scratch_bytes < ttt_b200_gated_scan_scratch_bytes(p) || !aligned16(p->scratch))
-    return fail("gated scan backward: scratch is missing, too small or not 16-byte aligned");
+  if (int rc = check_scratch(p, 1)) return rc;
   TTT_WITH_TYPE(p->dtype, return backward<Elem>(*p, static_cast<cudaStream_t>(stream)))
   return TTT_B200_OK;
 }

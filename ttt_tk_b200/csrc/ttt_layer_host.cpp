@@ -516,7 +516,11 @@ PyObject* gated(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     a.y = y.data_ptr();
     a.final_state = fptr(end);
     a.checkpoints = fptr(ck);
-    if (!none) launch(ttt_b200_gated_scan, a, dev);
+    if (!none) {
+      const Tensor scratch = scratch_of(ttt_b200_gated_scan_scratch_bytes(&a, 0), dev);
+      give(a, scratch);
+      launch(ttt_b200_gated_scan, a, dev);
+    }
     return tuple_of({y, end, ck});
   });
 }
@@ -583,7 +587,7 @@ PyObject* gated_backward(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
       gs = a.grad_final_state ? THPVariable_Unpack(v[10]).detach().clone() : at::zeros({a.B, a.D}, f32);
     } else {
       gs = at::empty({a.B, a.D}, f32);
-      const Tensor scratch = scratch_of(ttt_b200_gated_scan_scratch_bytes(&a), dev);
+      const Tensor scratch = scratch_of(ttt_b200_gated_scan_scratch_bytes(&a, 1), dev);
       give(a, scratch);
       a.grad_x = gx.data_ptr();
       a.grad_gate = gg.data_ptr();
