@@ -15,94 +15,157 @@ namespace {
 using namespace ttt;
 
 constexpr int kMost = TTT_B200_PACK8_TENSORS;
+constexpr int kNormThreads = 1024;      // of an SM (16384 x 2048, fp32 residual: 63 us; 1536, with registers spilled, 82)
 
 // ---- pack and unpack ----------------------------------------------------------------------------------------------------------------
 struct Many {
   ttt_b200_pack8_args a;
   uint32_t lanes;      // of a row: vectors of eight, whole groups
+  uint32_t magic, shift;      // n / lanes for n < 2^31: the high word of n magic, shifted (Granlund and Montgomery 1994)
   int64_t vectors;     // lanes * rows
 };
+
+// The row of vector i, and which of its lanes it is.
+__device__ __forceinline__ int64_t row_of(const Many& q, int64_t i, int& lane) {
+  const int64_t row = q.lanes == 1 ? i : q.vectors >> 31 ? i / q.lanes : __umulhi(static_cast<uint32_t>(i), q.magic) >> q.shift;
+  lane = static_cast<int>(i - row * q.lanes);
+  return row;
+}
+
+// A thread has several times eight values, a block of threads apart, all requested before the first are worked on: 2048 threads to an SM with 16 bytes each on
+// their way are less than the memory's latency takes.  3 x 32768 x 2048 bf16, packed / unpacked us with one, two and four: 135 / 135, 125 / 116, 119 / 104; 16384 x
+// 2047, whose values come one by one, 45 / 51, 44 / 54, 43 / 61; fp32 16384 x 2048 35 / 41, 33 / 41, 35 / 43.
+template <class T, bool kWhole> constexpr int kEach = kWhole && sizeof(T) == 2 ? 4 : 2;
+
+// Columns of a lane's eight values in a row.  Rows on 16-byte boundaries: neighbours, one access.  Others: of the 256 columns of a warp every 32nd, so that each
+// of eight accesses is the warp's 32 neighbours (eight neighbours to a lane one by one: 16384 x 2047 bf16 packed in 51 us, unpacked in 97).
+template <bool kWhole> __device__ __forceinline__ int column(int lane, int j) { return kWhole ? lane * 8 + j : (lane & ~31) * 8 + j * 32 + (lane & 31); }
+template <bool kWhole, class T> __device__ __forceinline__ void take(const T* row, int lane, int D, Eight<T>& e) {
+  if (kWhole && lane * 8 + 8 <= D) {
+    e.load(row + lane * 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e.v[j] = column<kWhole>(lane, j) < D ? row[column<kWhole>(lane, j)] : T();
+  }
+}
+template <bool kWhole, class T> __device__ __forceinline__ void leave(T* row, int lane, int D, const Eight<T>& e) {
+  if (kWhole && lane * 8 + 8 <= D) {
+    e.store(row + lane * 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (column<kWhole>(lane, j) < D) row[column<kWhole>(lane, j)] = e.v[j];
+  }
+}
+
+// Eight values to 8 bits, with the scales of their groups, of 8 L values each; all lanes of a warp together.  The scale of value j is that of
+// group first + j / (a group's share of a lane's values).
+template <bool kWhole, int L> __device__ __forceinline__ void to_eight(const float (&v)[8], int lane, int groups, bool there, float* scales, Eight<uint8_t>& b) {
+  if constexpr (kWhole) {
+    float most = magnitude(v);
+#pragma unroll
+    for (int o = L / 2; o; o /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const uint32_t x = scale_exponent(most);
+    const float inv = inverse_of(x);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) reinterpret_cast<uint16_t*>(b.v)[j] = static_cast<uint16_t>(two_bytes(v[2 * j] * inv, v[2 * j + 1] * inv));
+    if (there && lane % L == 0 && lane / L < groups) scales[lane / L] = scale_of(x);
+  } else {
+    constexpr int kShare = L / 4;      // of a lane's values in a group of the warp's: 1, 2 or 4
+#pragma unroll
+    for (int g = 0; g < 8; g += kShare) {
+      uint32_t most = 0;      // (magnitudes go by their bits)
+#pragma unroll
+      for (int j = g; j < g + kShare; ++j) most = max(most, fabsf(v[j]) < INFINITY ? __float_as_uint(fabsf(v[j])) : 0u);
+      const uint32_t x = scale_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, most)));
+      const float inv = inverse_of(x);
+#pragma unroll
+      for (int j = g; j < g + kShare; ++j) b.v[j] = static_cast<uint8_t>(two_bytes(v[j] * inv, 0.f));
+      const int at = ((lane & ~31) * 8 + g * 32) / (8 * L);
+      if (there && (lane & 31) == 0 && at < groups) scales[at] = scale_of(x);
+    }
+  }
+}
 
 // L lanes to a group
 template <class T, bool kWhole, int L> __global__ void __launch_bounds__(256) pack8_kernel(const Many q) {
   wait_for_predecessor();
+  constexpr int kN = kEach<T, kWhole>;
   const ttt_b200_pack8_args& a = q.a;
-  const int64_t i = blockIdx.x * 256L + threadIdx.x;      // (whole groups: their lanes leave together)
-  if (i >= q.vectors) return;
-  const int64_t row = q.vectors >> 32 ? i / q.lanes : static_cast<uint32_t>(i) / q.lanes;
-  const int lane = static_cast<int>(i - row * q.lanes), n = a.D - lane * 8, k = blockIdx.y;
-  Eight<T> e;
-  const T* src = static_cast<const T*>(a.src[k]) + row * a.stride[k] + lane * 8;
-  if (kWhole && n >= 8) e.load(src);
-  else e.load(src, n);
-  float v[8];
-  uint32_t most = 0;
+  const int k = blockIdx.y, groups = (a.D + 8 * L - 1) / (8 * L);
+  const int64_t i0 = blockIdx.x * (256L * kN) + threadIdx.x;
+  Eight<T> e[kN];
+  int64_t row[kN];
+  int lane[kN];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    v[j] = to_f32(e.v[j]);
-    most = magnitude(most, v[j]);
+  for (int c = 0; c < kN; ++c) {
+    const int64_t i = i0 + c * 256;
+    row[c] = row_of(q, i, lane[c]);
+    take<kWhole>(static_cast<const T*>(a.src[k]) + row[c] * a.stride[k], lane[c], i < q.vectors ? a.D : 0, e[c]);
   }
-  const int64_t left = q.vectors - (i - threadIdx.x % 32);      // from the warp's first lane on
-  const uint32_t live = left >= 32 ? 0xffffffffu : (1u << left) - 1;
 #pragma unroll
-  for (int o = L / 2; o; o /= 2) most = max(most, __shfl_xor_sync(live, most, o));
-  const uint32_t x = scale_exponent(most);
-  const float inv = inverse_of(x);
-  Eight<uint8_t> b;
+  for (int c = 0; c < kN; ++c) {
+    float v[8];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) reinterpret_cast<uint16_t*>(b.v)[j] = static_cast<uint16_t>(two_bytes(v[2 * j] * inv, v[2 * j + 1] * inv));
-  uint8_t* dst = static_cast<uint8_t*>(a.values[k]) + row * a.D + lane * 8;
-  if (kWhole && n >= 8) b.store(dst);
-  else b.store(dst, n);
-  if (lane % L == 0) a.scales[k][row * (q.lanes / L) + lane / L] = scale_of(x);
+    for (int j = 0; j < 8; ++j) v[j] = to_f32(e[c].v[j]);
+    const bool there = i0 + c * 256 < q.vectors;
+    Eight<uint8_t> b;
+    to_eight<kWhole, L>(v, lane[c], groups, there, a.scales[k] + row[c] * groups, b);
+    if (there) leave<kWhole>(static_cast<uint8_t*>(a.values[k]) + row[c] * a.D, lane[c], a.D, b);
+  }
 }
 
 template <class T, bool kWhole> __global__ void __launch_bounds__(256) unpack8_kernel(const Many q) {
   wait_for_predecessor();
+  constexpr int kN = kEach<T, kWhole>;
   const ttt_b200_pack8_args& a = q.a;
-  const int64_t i = blockIdx.x * 256L + threadIdx.x;
-  if (i >= q.vectors) return;
-  const int64_t row = q.vectors >> 32 ? i / q.lanes : static_cast<uint32_t>(i) / q.lanes;
-  const int lane = static_cast<int>(i - row * q.lanes), n = a.D - lane * 8, k = blockIdx.y;
-  const int groups = a.group ? (a.D + a.group - 1) / a.group : 1;
-  const float scale = a.scales[k][row * groups + (a.group ? lane * 8 / a.group : 0)];
-  Eight<uint8_t> b;
-  const uint8_t* src = static_cast<const uint8_t*>(a.values[k]) + row * a.D + lane * 8;
-  if (kWhole && n >= 8) b.load(src);
-  else b.load(src, n);
-  Eight<T> e;
+  const int groups = a.group ? (a.D + a.group - 1) / a.group : 1, k = blockIdx.y, shift = a.group == 32 ? 5 : a.group == 64 ? 6 : a.group == 128 ? 7 : 31;
+  const int64_t i0 = blockIdx.x * (256L * kN) + threadIdx.x;
+  constexpr int kScales = kWhole ? 1 : 8;
+  Eight<uint8_t> b[kN];
+  float scale[kN][kScales];
+  int64_t row[kN];
+  int lane[kN];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 f = two_values(reinterpret_cast<const uint16_t*>(b.v)[j]);
-    e.v[2 * j] = from_f32<T>(f.x * scale);
-    e.v[2 * j + 1] = from_f32<T>(f.y * scale);
+  for (int c = 0; c < kN; ++c) {
+    const int64_t i = i0 + c * 256;
+    row[c] = row_of(q, i, lane[c]);
+    const int D = i < q.vectors ? a.D : 0;
+    take<kWhole>(static_cast<const uint8_t*>(a.values[k]) + row[c] * a.D, lane[c], D, b[c]);
+#pragma unroll
+    for (int j = 0; j < kScales; ++j) {
+      const int d = column<kWhole>(lane[c], j);
+      scale[c][j] = d < D ? a.scales[k][row[c] * groups + (d >> shift)] : 0.f;
+    }
   }
-  T* dst = static_cast<T*>(a.dst[k]) + row * a.D + lane * 8;
-  if (kWhole && n >= 8) e.store(dst);
-  else e.store(dst, n);
+#pragma unroll
+  for (int c = 0; c < kN; ++c) {
+    if (i0 + c * 256 >= q.vectors) continue;
+    Eight<T> e;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = two_values(reinterpret_cast<const uint16_t*>(b[c].v)[j]);
+      e.v[2 * j] = from_f32<T>(f.x * scale[c][2 * j % kScales]);
+      e.v[2 * j + 1] = from_f32<T>(f.y * scale[c][(2 * j + 1) % kScales]);
+    }
+    leave<kWhole>(static_cast<T*>(a.dst[k]) + row[c] * a.D, lane[c], a.D, e);
+  }
 }
 
 // ---- norm -----------------------------------------------------------------------------------------------------------------------------
-// Threads of a token: the fewest, a power of two from a warp on, that hold it with eight values each.  A CTA walks over tokens with its
+// Threads of a token: the fewest, a power of two from a warp on, that hold it with eight values each, 256 columns to a warp.  A CTA walks over tokens with its
 // columns' weights in registers and the next token's values on their way.
 template <int kWidth> constexpr int kSide = kWidth < 128 ? 128 / kWidth : 1;
-__device__ __forceinline__ float add_up(float a, float b) { return a + b; }
-
-// a value joined over a token's threads, in all of them; `part`: a place for each warp, used again only behind another barrier
-template <int kWidth, class V, class Op> __device__ __forceinline__ V over_token(V v, V* part, Op op) {
+__device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
-  for (int o = 16; o; o /= 2) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if constexpr (kWidth > 32) {
-    constexpr int warps = kWidth / 32;
-    const int warp = threadIdx.x / 32, first = warp & -warps;
-    if (threadIdx.x % 32 == 0) part[warp] = v;
-    __syncthreads();
-    v = part[first + threadIdx.x % warps];
-#pragma unroll
-    for (int o = warps / 2; o; o /= 2) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  }
+  for (int o = 16; o; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// What the warps of a token share: (mean, squares about it) and the largest, tokens by turns: a barrier lies between two uses of the same place.
+struct Shared {
+  float2 part[2][32];
+  float top[2][32];
+};
 
 // 1 / sqrt(v), a step of Newton's behind the fast one: an error of all of a token's values alike takes more of them over a border of their rounding
 // to 4 bits than as many errors that differ (16384 x 2048: 4 times the values that differ from those of 64 bits).
@@ -111,31 +174,62 @@ __device__ __forceinline__ float inverse_root(float v) {
   return e < 1.f ? fmaf(0.5f * r, e, r) : r;      // (v = 0, infinite or NaN: r as it is)
 }
 
-template <class T, class R, int kWidth, bool kWhole>
-__global__ void __launch_bounds__(kWidth* kSide<kWidth>, 1024 / (kWidth * kSide<kWidth>)) norm8_kernel(const ttt_b200_norm8_args p) {
+// Mean and 1 / deviation of a token with one barrier: each warp's mean and its squares about it, joined as
+// sum over warps of (squares + columns (mean of the warp - mean)^2).
+template <int kWidth, bool kWhole> __device__ __forceinline__ float2 statistics(const float (&z)[8], const ttt_b200_norm8_args& p, int lane, Shared& sh, int turn) {
+  auto columns = [&](int warp) { return static_cast<float>(min(max(p.D - warp * 256, 0), 256)); };
+  const float inv = 1.f / static_cast<float>(p.D);
+  float mean = 0.f, sq = 0.f;
+  if (p.layer) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += z[j];      // (zeros behind the last column)
+    mean = warp_sum(s) / fmaxf(columns(lane / 32), 1.f);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float v = column<kWhole>(lane, j) < p.D ? z[j] - mean : 0.f;
+    sq = fmaf(v, v, sq);
+  }
+  sq = warp_sum(sq);
+  if constexpr (kWidth > 32) {
+    constexpr int warps = kWidth / 32;
+    const int warp = threadIdx.x / 32, home = warp & -warps, i = threadIdx.x % warps;
+    if (threadIdx.x % 32 == 0) sh.part[turn][warp] = make_float2(mean, sq);
+    __syncthreads();
+    const float2 v = sh.part[turn][home + i];      // a lane for each warp
+    sq = v.y;
+    if (p.layer) {
+      const float n = columns(i);
+      mean = n * v.x;
+#pragma unroll
+      for (int o = warps / 2; o; o /= 2) mean += __shfl_xor_sync(0xffffffffu, mean, o);
+      mean *= inv;
+      sq = fmaf(n * (v.x - mean), v.x - mean, sq);
+    }
+#pragma unroll
+    for (int o = warps / 2; o; o /= 2) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+  }
+  return make_float2(mean, inverse_root(fmaf(sq, inv, p.eps)));
+}
+
+// L lanes to a group; 0: the token has one scale
+template <class T, class R, int kWidth, bool kWhole, int L>
+__global__ void __launch_bounds__(kWidth* kSide<kWidth>, kNormThreads / (kWidth * kSide<kWidth>)) norm8_kernel(const ttt_b200_norm8_args p) {
   wait_for_predecessor();
   constexpr int side = kSide<kWidth>;
-  __shared__ float parts[2][2][32];      // mean, squares; tokens take turns
-  __shared__ uint32_t tops[2][32];
-  const int lane = threadIdx.x % kWidth, sub = threadIdx.x / kWidth, d = lane * 8, n = p.D - d;
-  const float inv_d = 1.f / static_cast<float>(p.D);
-  const int lanes = p.group / 8, groups = p.group ? (p.D + p.group - 1) / p.group : 1;
-  Eight<float> w, b;
-  w.load(p.weight + d, n);
-  if (p.bias) b.load(p.bias + d, n);
+  __shared__ Shared sh;
+  const int lane = threadIdx.x % kWidth, sub = threadIdx.x / kWidth, groups = L ? (p.D + 8 * L - 1) / (8 * L) : 1;
+  Eight<float> w;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w.v[j] = column<kWhole>(lane, j) < p.D ? p.weight[column<kWhole>(lane, j)] : 0.f;
   const int64_t step = static_cast<int64_t>(gridDim.x) * side;
   Eight<T> o;
   Eight<R> r;
   auto ask = [&](int64_t m) {
     if (m >= p.M) return;
-    const T* po = static_cast<const T*>(p.o) + m * p.o_stride + d;
-    if (kWhole && n >= 8) o.load(po);
-    else o.load(po, n);
-    if (p.residual) {
-      const R* pr = static_cast<const R*>(p.residual) + m * p.residual_stride + d;
-      if (kWhole && n >= 8) r.load(pr);
-      else r.load(pr, n);
-    }
+    take<kWhole>(static_cast<const T*>(p.o) + m * p.o_stride, lane, p.D, o);
+    if (p.residual) take<kWhole>(static_cast<const R*>(p.residual) + m * p.residual_stride, lane, p.D, r);
   };
   int64_t m = static_cast<int64_t>(blockIdx.x) * side + sub;
   ask(m);
@@ -148,48 +242,45 @@ __global__ void __launch_bounds__(kWidth* kSide<kWidth>, 1024 / (kWidth * kSide<
     if (live && p.residual) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) r.v[j] = from_f32<R>(z[j]);
-      R* x = static_cast<R*>(p.x) + m * p.D + d;
-      if (kWhole && n >= 8) r.store(x);
-      else r.store(x, n);
+      leave<kWhole>(static_cast<R*>(p.x) + m * p.D, lane, p.D, r);
     }
     ask(m + step);
-    float mean = 0.f;
-    if (p.layer) {
-      float s = 0.f;
+    const float2 s = statistics<kWidth, kWhole>(z, p, lane, sh, turn);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s += z[j];      // (zeros behind the last column)
-      mean = over_token<kWidth>(s, parts[turn][0], add_up) * inv_d;
-    }
-    float sq = 0.f;
+    for (int j = 0; j < 8; ++j) z[j] = (z[j] - s.x) * s.y * w.v[j];      // (0 behind the last column, as weight and bias)
+    if (p.bias) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      z[j] -= mean;
-      if (kWhole ? n > 0 : j < n) sq = fmaf(z[j], z[j], sq);
+      for (int j = 0; j < 8; ++j) z[j] += column<kWhole>(lane, j) < p.D ? p.bias[column<kWhole>(lane, j)] : 0.f;
     }
-    const float dev = inverse_root(fmaf(over_token<kWidth>(sq, parts[turn][1], add_up), inv_d, p.eps));
-    uint32_t most = 0;
+    if (kWhole ? lane * 8 >= p.D : lane / 32 * 256 >= p.D) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      z[j] = z[j] * dev * w.v[j];
-      if (p.bias) z[j] += b.v[j];
-      if (kWhole ? n > 0 : j < n) most = magnitude(most, z[j]);
+      for (int j = 0; j < 8; ++j) z[j] = 0.f;      // (0 times what a token of infinities has for a deviation)
     }
-    if (p.group) {
-      for (int e = lanes / 2; e; e /= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, e));
-    } else {
-      most = over_token<kWidth>(most, tops[turn], [](uint32_t a, uint32_t b) { return max(a, b); });
-    }
-    if (!live || n <= 0) continue;
-    const uint32_t x = scale_exponent(most);
-    const float inv = inverse_of(x);
     Eight<uint8_t> q;
+    if constexpr (L > 0) {
+      to_eight<kWhole, L>(z, lane, groups, live, p.scales + m * groups, q);
+    } else {
+      float most = magnitude(z);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) reinterpret_cast<uint16_t*>(q.v)[j] = static_cast<uint16_t>(two_bytes(z[2 * j] * inv, z[2 * j + 1] * inv));
-    uint8_t* dst = static_cast<uint8_t*>(p.values) + m * p.D + d;
-    if (kWhole && n >= 8) q.store(dst);
-    else q.store(dst, n);
-    if (p.group ? lane % lanes == 0 : lane == 0) p.scales[m * groups + (p.group ? lane / lanes : 0)] = scale_of(x);
-    if (p.stats && lane == 0) reinterpret_cast<float4*>(p.stats)[m] = make_float4(0.f, 1.f, mean, dev);
+      for (int e = 16; e; e /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, e));
+      if constexpr (kWidth > 32) {
+        constexpr int warps = kWidth / 32;
+        const int warp = threadIdx.x / 32;
+        if (threadIdx.x % 32 == 0) sh.top[turn][warp] = most;
+        __syncthreads();
+        most = sh.top[turn][(warp & -warps) + threadIdx.x % warps];
+#pragma unroll
+        for (int e = warps / 2; e; e /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, e));
+      }
+      const uint32_t x = scale_exponent(most);
+      const float inv = inverse_of(x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) reinterpret_cast<uint16_t*>(q.v)[j] = static_cast<uint16_t>(two_bytes(z[2 * j] * inv, z[2 * j + 1] * inv));
+      if (live && lane == 0) p.scales[m] = scale_of(x);
+    }
+    if (!live) continue;
+    leave<kWhole>(static_cast<uint8_t*>(p.values) + m * p.D, lane, p.D, q);
+    if (p.stats && lane == 0) reinterpret_cast<float4*>(p.stats)[m] = make_float4(0.f, 1.f, s.x, s.y);
   }
 }
 
@@ -209,19 +300,25 @@ int check(const ttt_b200_pack8_args* p, bool back) {
 }
 template <class T> int run(Many& q, bool back, cudaStream_t s) {
   const ttt_b200_pack8_args& a = q.a;
-  const int L = back ? 1 : a.group / 8;
-  const int64_t lanes = (a.D + 8L * L - 1) / (8L * L) * L;
-  q.lanes = static_cast<uint32_t>(lanes);
-  if (a.M > (255L << 31) / lanes) return fail("pack8: too many values");
-  q.vectors = a.M * lanes;
-  const int64_t blocks = (q.vectors + 255) / 256;
   bool whole = true;
   for (int k = 0; k < a.count; ++k)
     whole = whole && rows<uint8_t>(a.values[k], a.D) && (back ? rows<T>(a.dst[k], a.D) : rows<T>(a.src[k], a.stride[k]));
+  const int64_t unit = whole ? (back ? 1 : a.group / 8) : 32;      // lanes that a row has a multiple of: a group's, or a warp
+  const int64_t lanes = (a.D + 8 * unit - 1) / (8 * unit) * unit;
+  q.lanes = static_cast<uint32_t>(lanes);
+  if (a.M > (255L << 31) / lanes) return fail("pack8: too many values");
+  q.vectors = a.M * lanes;
+  int bits = 0;      // 2^bits >= lanes
+  while (int64_t{1} << bits < lanes) ++bits;
+  q.shift = bits ? bits - 1 : 0;
+  q.magic = static_cast<uint32_t>(((uint64_t{1} << (31 + bits)) + lanes - 1) / lanes);
+  const int each = whole ? kEach<T, true> : kEach<T, false>;
+  const int64_t blocks = (q.vectors + 256 * each - 1) / (256 * each);
+  if (blocks > 0x7fffffffL) return fail("pack8: too many values");
   auto kernel = back ? (whole ? unpack8_kernel<T, true> : unpack8_kernel<T, false>)
-              : L == 4 ? (whole ? pack8_kernel<T, true, 4> : pack8_kernel<T, false, 4>)
-              : L == 8 ? (whole ? pack8_kernel<T, true, 8> : pack8_kernel<T, false, 8>)
-                       : (whole ? pack8_kernel<T, true, 16> : pack8_kernel<T, false, 16>);
+              : a.group == 32 ? (whole ? pack8_kernel<T, true, 4> : pack8_kernel<T, false, 4>)
+              : a.group == 64 ? (whole ? pack8_kernel<T, true, 8> : pack8_kernel<T, false, 8>)
+                              : (whole ? pack8_kernel<T, true, 16> : pack8_kernel<T, false, 16>);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -235,12 +332,17 @@ template <class T> int run(Many& q, bool back, cudaStream_t s) {
   return launched(back ? "unpack8" : "pack8");
 }
 
-template <class T, class R, int kWidth> int norm_as(const ttt_b200_norm8_args& p, cudaStream_t s) {
+template <class T, class R, int kWidth, bool kWhole> int norm_with(const ttt_b200_norm8_args& p, cudaStream_t s) {
   constexpr int side = kSide<kWidth>, threads = kWidth * side;
-  const bool whole = p.D % 8 == 0 && rows<T>(p.o, p.o_stride) && rows<R>(p.residual, p.residual_stride) && rows<R>(p.x, p.D) && rows<uint8_t>(p.values, p.D);
-  const int ctas = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(sm_count()) * (1024 / threads), (p.M + side - 1) / side));
-  ttt_launch_overlapped(whole ? norm8_kernel<T, R, kWidth, true> : norm8_kernel<T, R, kWidth, false>, ctas, threads, 0, s, p);
+  const int ctas = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(sm_count()) * (kNormThreads / threads), (p.M + side - 1) / side));
+  const auto kernel = p.group == 0 ? norm8_kernel<T, R, kWidth, kWhole, 0> : p.group == 32 ? norm8_kernel<T, R, kWidth, kWhole, 4>
+                    : p.group == 64 ? norm8_kernel<T, R, kWidth, kWhole, 8> : norm8_kernel<T, R, kWidth, kWhole, 16>;
+  ttt_launch_overlapped(kernel, ctas, threads, 0, s, p);
   return launched("norm8");
+}
+template <class T, class R, int kWidth> int norm_as(const ttt_b200_norm8_args& p, cudaStream_t s) {
+  const bool whole = p.D % 8 == 0 && rows<T>(p.o, p.o_stride) && rows<R>(p.residual, p.residual_stride) && rows<R>(p.x, p.D) && rows<uint8_t>(p.values, p.D);
+  return whole ? norm_with<T, R, kWidth, true>(p, s) : norm_with<T, R, kWidth, false>(p, s);
 }
 template <class T, class R> int norm(const ttt_b200_norm8_args& p, cudaStream_t s) {
   if (p.D <= 256) return norm_as<T, R, 32>(p, s);

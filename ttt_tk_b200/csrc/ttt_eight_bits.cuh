@@ -11,13 +11,20 @@
 
 namespace ttt {
 
-// Largest of the magnitudes so far, infinities and NaN left out.
-__device__ __forceinline__ uint32_t magnitude(uint32_t most, float v) {
-  const uint32_t m = __float_as_uint(v) & 0x7fffffffu;
-  return m < 0x7f800000u && m > most ? m : most;
+// Largest of eight magnitudes.  NaN is left out by the maximum itself; where an infinity comes of it the finite ones are looked for.
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, fabsf(b)); }
+__device__ __forceinline__ float magnitude(const float (&v)[8]) {
+  const float a = larger(larger(fabsf(v[0]), v[1]), v[2]), b = larger(larger(fabsf(v[3]), v[4]), v[5]);
+  float most = fmaxf(larger(larger(a, v[6]), v[7]), b);
+  if (!(most < INFINITY)) {      // (or all of them are NaN)
+    most = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) most = fabsf(v[j]) < INFINITY ? larger(most, v[j]) : most;
+  }
+  return most;
 }
 // Exponent field of the scale of a group whose largest magnitude has these bits: 8 less than that of amax / 1.75 rounded up, at least 1.
-__device__ __forceinline__ uint32_t scale_exponent(uint32_t most) { return max(static_cast<int>((most + 0x1fffffu) >> 23) - 8, 1); }
+__device__ __forceinline__ uint32_t scale_exponent(float most) { return max(static_cast<int>((__float_as_uint(most) + 0x1fffffu) >> 23) - 8, 1); }
 __device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float(e << 23); }
 __device__ __forceinline__ float inverse_of(uint32_t e) { return __uint_as_float((254u - e) << 23); }      // (e is at most 254 - 8: no subnormal)
 

@@ -10,9 +10,11 @@ the format's rounding is the only one.  Infinities are left out of the maximum a
 `ttt_tk_b200.ssm.gated_scan_backward` takes packed inputs as they are; the differentiable operators of `ttt_tk_b200.autograd` with `saved="e4m3"` keep
 theirs this way.  Calls are stream-ordered and do not synchronise.  A bad argument raises ValueError.
 """
+import torch
+
 from . import ssm
 
-_TYPES = {"torch.bfloat16": 0, "torch.float16": 1, "torch.float32": 2}
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def pack8(*xs, group=128):
@@ -21,13 +23,12 @@ def pack8(*xs, group=128):
     return ssm._host().pack8(xs, _group(group, "32, 64 or 128"))
 
 
-def unpack8(*packs, dtype=None):
-    """The values that (values, scales) stand for, in `dtype` (bf16 by default, fp16 or fp32), for one to four of the same shape, one launch.  The group is
+def unpack8(*packs, dtype=torch.bfloat16):
+    """The values that (values, scales) stand for, in `dtype` (bf16, fp16 or fp32), for one to four of the same shape, one launch.  The group is
     that of the scales' shape; [...] is one scale to a row (`glue.norm_residual_8bit` with group None)."""
-    code = 0 if dtype is None else _TYPES.get(str(dtype)) if str(dtype) in _TYPES and not isinstance(dtype, str) else None
-    if code is None:
+    if not isinstance(dtype, torch.dtype) or dtype not in _TYPES:
         raise ValueError(f"dtype must be torch.bfloat16, torch.float16 or torch.float32, got {dtype!r}")
-    return ssm._host().unpack8(packs, code)
+    return ssm._host().unpack8(packs, _TYPES[dtype])
 
 
 def _group(group, what):
