@@ -17,6 +17,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "ttt_elem.cuh"
@@ -80,21 +81,21 @@ template <bool kBoth> __device__ __forceinline__ void sigmoid(F v, F bias, float
   if constexpr (kBoth) other = mul2(e, s);
 }
 
-// exp(v) and 1 - exp(v) for v <= 0: v = k ln 2 + f, |f| <= ln 2 / 2, ln 2 in two parts (Cody and Waite), exp(f) - 1 = f + f^2 p(f) with the
-// polynomial of fourth degree that is off by the least part of f (1.6e-8, fitted).  Both from one series: 1 - a keeps its digits where a is close to one, which is where these
-// recurrences are, and the exponential unit, which is close to its limit, is left alone.  Where k comes to -127 the power's
-// bits are those of 0: exp(v) is 0 from there on, as far as A makes v.
-__device__ __forceinline__ void exp_both(F v, F& a, F& rest) {
-  v = make_float2(max_nan(v.x, -88.f), max_nan(v.y, -88.f));
+// 2^v and 1 - 2^v for v <= 0: v = k + f, |f| <= 1/2, both exact, 2^f - 1 = f p(f) with the polynomial of fifth degree that is off by the least part
+// of it (2.1e-08, fitted).  Both from one series: 1 - a keeps its digits where a is close to one, which is where these recurrences are, and the
+// exponential unit, which is close to its limit, is left alone.  Where k comes to -127 the power's bits are those of 0: 2^v is 0 from there on, as far
+// as A makes v.
+__device__ __forceinline__ void exp2_both(F v, F& a, F& rest) {
+  v = make_float2(max_nan(v.x, -127.f), max_nan(v.y, -127.f));
   constexpr float magic = 12582912.f;      // 1.5 2^23: the sum's last bits are the rounded integer
-  const F k = fma2(v, both(kLog2e), both(magic)), kf = add2(k, both(-magic));
-  F f = fma2(kf, both(-0.693145751953125f), v);
-  f = fma2(kf, both(-1.42860682030941723e-6f), f);
-  F q = fma2(f, both(1.3947017723694444e-3f), both(8.366910740733147e-3f));
-  q = fma2(q, f, both(4.166627302765846e-2f));
-  q = fma2(q, f, both(1.6666540503501892e-1f));
-  q = fma2(q, f, both(0.5f));
-  q = fma2(mul2(f, f), q, f);
+  const F k = add2(v, both(magic));
+  const F f = add2(v, fma2(k, both(-1.f), both(magic)));
+  F q = fma2(f, both(0.00015403512225020677f), both(0.0013390964595600963f));
+  q = fma2(q, f, both(0.009618238545954227f));
+  q = fma2(q, f, both(0.055503569543361664f));
+  q = fma2(q, f, both(0.24022649228572845f));
+  q = fma2(q, f, both(0.6931471824645996f));
+  q = mul2(q, f);
   const F two = make_float2(__int_as_float((__float_as_int(k.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(k.y) << 23) + 0x3f800000));
   q = mul2(q, two);      // exact but where it is below the normal numbers
   a = add2(q, two);
@@ -103,7 +104,7 @@ __device__ __forceinline__ void exp_both(F v, F& a, F& rest) {
 
 // What does not change over the tokens of a lane's channels.
 struct Weights {
-  F A, gate_bias, input_bias;
+  F A, A2, gate_bias, input_bias;      // A2 = A log2 e
   int mix;
   bool has_a, gated;
 };
@@ -123,9 +124,8 @@ __device__ __forceinline__ void factors(const Weights& z, Gate gate, Input input
   if (kUsual || z.has_a) {
     F s;
     sigmoid<kBack>(gate, z.gate_bias, 127.f, s, o);
-    const F la = mul2(s, z.A);
-    exp_both(la, f.a, rest);
-    if constexpr (kBack) f.s = s, f.k = mul2(la, o);
+    exp2_both(mul2(s, z.A2), f.a, rest);
+    if constexpr (kBack) f.s = s, f.k = mul2(mul2(s, z.A), o);
   } else {
     sigmoid<true>(gate, z.gate_bias, 126.f, f.a, rest);
     if constexpr (kBack) f.s = f.a, f.k = rest;
@@ -164,7 +164,7 @@ template <bool kUsual> __device__ __forceinline__ F decay(const Weights& z, F ga
   sigmoid<false>(gate, z.gate_bias, 0.f, s, o);
   if (!kUsual && !z.has_a) return s;
   F a, rest;
-  exp_both(mul2(s, z.A), a, rest);
+  exp2_both(mul2(s, z.A2), a, rest);
   return a;
 }
 
@@ -194,31 +194,22 @@ template <class T> __device__ __forceinline__ float value_of(uint32_t at) {
   }
 }
 
+enum { kSingles, kPairs, kWholeRows };
 // S rows of 64 channels of a tensor, copied ahead by a warp into its own place in shared memory.
-//   kWhole    rows start on 16-byte boundaries: 16-byte pieces, pairs
-//   otherwise the 16-byte blocks that a row touches (the first and the last may hold its neighbours too), from which values are picked one
-//             by one at the row's offset
-// 8-bit values come with their scales, two to a row (one for each 32 channels).
-template <class T, bool kWhole> struct Rows {
+//   kWhole    rows start on 16-byte boundaries: 16-byte pieces
+//   kPairs    rows start on boundaries of two values: the 16-byte blocks that a row touches (the first and the last may hold its neighbours too), from which
+//             pairs are picked at the row's offset
+//   kSingles  the same, and values one by one
+template <class T, int kMode> struct Rows {
+  static constexpr bool kWhole = kMode == kWholeRows;
   static constexpr int es = sizeof(T), kBytes = kCols * es, kPitch = kWhole ? kBytes : kBytes + 16, kPieces = kPitch / 16;
-  static constexpr bool kScaled = es == 1;
-  static constexpr uint32_t kStage = S * kPitch + (kScaled ? S * 8 : 0);      // bytes
+  static constexpr uint32_t kStage = S * kPitch;      // bytes
   static_assert(kStage % 16 == 0, "copies start on 16-byte boundaries");
   const char* base;      // channel d0 of the first token
-  const float* scales;   // its scale
-  int64_t step, scale_step;      // bytes from token to token; scales
-  int cols;      // bytes of a row that there are
-  int second;    // distance of the second 32 channels' scale, 0 or 1; -1: there are none
-  __device__ __forceinline__ Rows(const void* p, int64_t batch, int64_t token, int b, int d0, int D, const float* sc = nullptr, int groups = 0, int group = 32, int T_ = 0) {
-    base = static_cast<const char*>(p) + (b * batch + d0) * es;
-    step = token * es;
-    cols = min(D - d0, kCols) * es;
-    if constexpr (kScaled) {
-      scales = sc + static_cast<int64_t>(b) * T_ * groups + d0 / group;
-      scale_step = groups;
-      second = d0 + 32 < D ? (d0 + 32) / group - d0 / group : -1;
-    }
-  }
+  int64_t step;          // bytes from token to token
+  int cols;              // bytes of a row that there are
+  __device__ __forceinline__ Rows(const void* p, const int64_t (&stride)[2], int b, int d0, int D)
+      : base(static_cast<const char*>(p) + (b * stride[0] + d0) * es), step(stride[1] * es), cols(min(D - d0, kCols) * es) {}
   // tokens t .. t + S - 1, those before `stop`, to the shared address `to`
   __device__ __forceinline__ void copy(uint32_t to, int t, int stop) const {
     const int lane = threadIdx.x & 31;
@@ -232,7 +223,6 @@ template <class T, bool kWhole> struct Rows {
         cp_async16_at(to + 512 * i, from);
         from += 32 / kPieces * step;
       }
-      if constexpr (kScaled) to -= lane * 16;
     } else {
 #pragma unroll
       for (int i = 0; i < (S * kPieces + 31) / 32; ++i) {
@@ -249,38 +239,72 @@ template <class T, bool kWhole> struct Rows {
         cp_async16_at(to + row * kPitch + o, have ? from + o : reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(base) & ~uintptr_t{15}), have);
       }
     }
-    if constexpr (kScaled) {
-      static_assert(S * 2 <= 32, "a lane for each scale");
-      if (lane < 2 * S) {
-        const bool in = t + lane / 2 < stop && !(lane % 2 && second < 0);
-        cp_async4_at(to + S * kPitch + lane * 4, in ? scales + (t + lane / 2) * scale_step + (lane % 2 ? second : 0) : scales, in ? 4 : 0);
-      }
-    }
   }
   // this lane's two channels of token t (row i of those at `from`)
   __device__ __forceinline__ F get(uint32_t from, int i, int t) const {
     const int lane = threadIdx.x & 31;
-    F v;
     if constexpr (kWhole) {
-      v = pair_of<T>(from + i * kPitch + lane * 2 * es);
+      return pair_of<T>(from + i * kPitch + lane * 2 * es);
     } else {
       const uint32_t at = from + i * kPitch + (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base) + t * step) & 15) + lane * 2 * es;
-      v = make_float2(value_of<T>(at), value_of<T>(at + es));
+      if constexpr (kMode == kPairs) return pair_of<T>(at);
+      else return make_float2(value_of<T>(at), value_of<T>(at + es));
     }
-    if constexpr (kScaled) v = mul2(v, both(shared_load<float>(from + S * kPitch + i * 8 + lane / 16 * 4)));
-    return v;
+  }
+};
+// The scales of 8-bit x, gate and input gate, next to one another for a token and each half of the channels; T of another size: there are none.
+template <class T> struct Scales {
+  static constexpr bool kThere = sizeof(T) == 1;
+  static constexpr uint32_t kStage = kThere ? S * 2 * 16 : 0;
+  const float* base[3];      // of channel d0 of the first token, or NULL
+  int64_t step;
+  int second;      // distance of the second 32 channels' scale, 0 or 1; -1: there are none
+  __device__ __forceinline__ Scales(const ttt_b200_gated_args& p, int b, int d0) {
+    if constexpr (kThere) {
+      const int groups = (p.D + p.group - 1) / p.group;
+      const int64_t at = static_cast<int64_t>(b) * p.T * groups + d0 / p.group;
+      base[0] = p.x_scales + at;
+      base[1] = p.gate_scales + at;
+      base[2] = p.input_gate ? p.input_scales + at : nullptr;
+      step = groups;
+      second = d0 + 32 < p.D ? (d0 + 32) / p.group - d0 / p.group : -1;
+    }
+  }
+  __device__ __forceinline__ void copy(uint32_t to, int t, int stop) const {
+    if constexpr (kThere) {
+      static_assert(S * 2 <= 32, "a lane for each half of a token");
+      const int lane = threadIdx.x & 31;
+      if (lane >= 2 * S) return;
+      const bool in = t + lane / 2 < stop && !(lane % 2 && second < 0);
+      const int64_t at = in ? (t + lane / 2) * step + (lane % 2 ? second : 0) : 0;
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        if (base[k]) cp_async4_at(to + lane * 16 + k * 4, base[k] + at, in ? 4 : 0);
+    }
+  }
+  __device__ __forceinline__ float4 get(uint32_t from, int i) const {
+    if constexpr (kThere) {
+      const uint4 r = shared_load16(from + (i * 2 + (threadIdx.x & 31) / 16) * 16);
+      return make_float4(__uint_as_float(r.x), __uint_as_float(r.y), __uint_as_float(r.z), 0.f);
+    } else {
+      return make_float4(1.f, 1.f, 1.f, 0.f);
+    }
+  }
+  static __device__ __forceinline__ F apply(F v, float scale) {
+    if constexpr (kThere) return mul2(v, both(scale));
+    else return v;
   }
 };
 
 // ---- a lane's two channels in global memory -------------------------------------------------------------------------------------------
-template <bool kWhole> __device__ __forceinline__ F load2(const float* p, int d, int D, float none) {
+template <int kMode> __device__ __forceinline__ F load2(const float* p, int d, int D, float none) {
   if (!p || d >= D) return both(none);
-  if constexpr (kWhole) return *reinterpret_cast<const F*>(p + d);
+  if constexpr (kMode != kSingles) return *reinterpret_cast<const F*>(p + d);
   return make_float2(p[d], d + 1 < D ? p[d + 1] : none);
 }
-template <class T, bool kWhole> __device__ __forceinline__ void store2(T* p, int d, int D, F v) {
+template <class T, int kMode> __device__ __forceinline__ void store2(T* p, int d, int D, F v) {
   if (d >= D) return;
-  if constexpr (kWhole) {
+  if constexpr (kMode != kSingles) {
     if constexpr (std::is_same<T, __nv_bfloat16>::value) *reinterpret_cast<__nv_bfloat162*>(p + d) = __float22bfloat162_rn(v);
     else if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(p + d) = __float22half2_rn(v);
     else *reinterpret_cast<F*>(p + d) = v;
@@ -289,12 +313,14 @@ template <class T, bool kWhole> __device__ __forceinline__ void store2(T* p, int
     if (d + 1 < D) p[d + 1] = from_f32<T>(v.y);
   }
 }
-template <bool kWhole> __device__ __forceinline__ Weights weights_of(const ttt_b200_gated_args& p, int d) {
+template <int kMode> __device__ __forceinline__ Weights weights_of(const ttt_b200_gated_args& p, int d) {
   Weights z;
-  z.A = load2<kWhole>(p.A, d, p.D, 0.f);
+  z.A = load2<kMode>(p.A, d, p.D, 0.f);
   z.A = make_float2(min_nan(z.A.x, 0.f), min_nan(z.A.y, 0.f));
-  z.gate_bias = mul2(load2<kWhole>(p.gate_bias, d, p.D, 0.f), both(-kLog2e));
-  z.input_bias = mul2(load2<kWhole>(p.input_bias, d, p.D, 0.f), both(-kLog2e));
+  z.A2 = make_float2(max_nan(z.A.x, -FLT_MAX / 2), max_nan(z.A.y, -FLT_MAX / 2));
+  z.A2 = mul2(z.A2, both(kLog2e));
+  z.gate_bias = mul2(load2<kMode>(p.gate_bias, d, p.D, 0.f), both(-kLog2e));
+  z.input_bias = mul2(load2<kMode>(p.input_bias, d, p.D, 0.f), both(-kLog2e));
   z.mix = p.mix;
   z.has_a = p.A != nullptr;
   z.gated = p.input_gate != nullptr;
@@ -331,13 +357,13 @@ template <int W> struct At {
   __device__ __forceinline__ int end(const Plan& q, int p_T) const { return min((chunk + 1) * q.chunk, (p_T + kTile - 1) / kTile); }
 };
 // Of what stands in front of a chunk (backward: behind it) the steps, one after another.
-template <bool kWhole, bool kBack, class W> __device__ __forceinline__ F join_chunks(const ttt_b200_gated_args& p, const Plan& q, const W& at, F h) {
+template <int kMode, bool kBack, class W> __device__ __forceinline__ F join_chunks(const ttt_b200_gated_args& p, const Plan& q, const W& at, F h) {
   const int n = kBack ? q.chunks - 1 - at.chunk : at.chunk;
   const float* ends = q.ends + static_cast<long>(at.b) * q.chunks * 2 * p.D;
 #pragma unroll 8
   for (int k = 0; k < n; ++k) {
     const float* e = ends + static_cast<long>(kBack ? q.chunks - 1 - k : k) * 2 * p.D;
-    h = fma2(load2<kWhole>(e, at.d, p.D, 1.f), h, load2<kWhole>(e + p.D, at.d, p.D, 0.f));
+    h = fma2(load2<kMode>(e, at.d, p.D, 1.f), h, load2<kMode>(e + p.D, at.d, p.D, 0.f));
   }
   return h;
 }
@@ -347,12 +373,12 @@ constexpr int kStages = 2;
 // Where channels and sequences do not fill the GPU: a chunk's step p h + q, forward (kBack: backward, of which q is c in front of the chunk for
 // nothing behind it).  Each warp has tokens after one another, and nothing to wait for until the end.  What the main kernels compute of a token is
 // computed here before: but for the last chunk (the first one).
-template <class T, class I, bool kWhole, bool kUsual, bool kBack, int W>
+template <class T, class I, int kMode, bool kUsual, bool kBack, int W>
 __global__ void __launch_bounds__(32 * W, 16 / W) gated_ends_kernel(const ttt_b200_gated_args p, const Plan q) {
   wait_for_predecessor();
-  using R = Rows<I, kWhole>;
-  using U = Rows<T, kWhole>;
-  constexpr uint32_t kStage = kBack ? R::kStage + U::kStage : 3 * R::kStage;
+  using R = Rows<I, kMode>;
+  using U = Rows<T, kMode>;
+  constexpr uint32_t kStage = kBack ? R::kStage + U::kStage + Scales<I>::kStage : 3 * R::kStage;
   __shared__ float4 steps[W][32];
   extern __shared__ __align__(16) unsigned char rings[];
   At<W> at(p, q, q.chunks - 1);
@@ -363,12 +389,10 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_ends_kernel(const ttt_b2
     at.last = max(at.first, min(at.first + q.chunk, (at.len + kTile - 1) / kTile));
   }
   const int d0 = at.tile * kCols;
-  const Weights z = weights_of<kWhole>(p, at.d);
-  const int groups = p.group ? (p.D + p.group - 1) / p.group : 0;
-  const R rx(p.x, p.x_stride[0], p.x_stride[1], at.b, d0, p.D, p.x_scales, groups, p.group, p.T),
-      rg(p.gate, p.gate_stride[0], p.gate_stride[1], at.b, d0, p.D, p.gate_scales, groups, p.group, p.T),
-      ri(p.input_gate, p.input_stride[0], p.input_stride[1], at.b, d0, p.D, p.input_scales, groups, p.group, p.T);
-  const U ru(p.grad_y, p.gy_stride[0], p.gy_stride[1], at.b, d0, p.D);
+  const Weights z = weights_of<kMode>(p, at.d);
+  const R rx(p.x, p.x_stride, at.b, d0, p.D), rg(p.gate, p.gate_stride, at.b, d0, p.D), ri(p.input_gate, p.input_stride, at.b, d0, p.D);
+  const U ru(p.grad_y, p.gy_stride, at.b, d0, p.D);
+  const Scales<I> scales(p, at.b, d0);
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(rings)) + at.warp * (kStages * kStage);
   const int rounds = at.last - at.first, first = at.first * kTile + at.warp * rounds * S;
   auto ahead = [&](int j) {
@@ -378,6 +402,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_ends_kernel(const ttt_b2
       rg.copy(to, t, at.len);
       if constexpr (kBack) {
         ru.copy(to + R::kStage, t, at.len);
+        scales.copy(to + R::kStage + U::kStage, t, at.len);
       } else {
         rx.copy(to + R::kStage, t, at.len);
         if (kUsual || z.gated) ri.copy(to + 2 * R::kStage, t, at.len);
@@ -398,7 +423,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_ends_kernel(const ttt_b2
 #pragma unroll
     for (int t = 0; t < S; ++t) {
       if constexpr (kBack) {
-        a[t] = decay<kUsual>(z, rg.get(from, t, t0 + t));
+        a[t] = decay<kUsual>(z, scales.apply(rg.get(from, t, t0 + t), scales.get(from + R::kStage + U::kStage, t).y));
         u[t] = ru.get(from + R::kStage, t, t0 + t);
       } else {
         Factors<false> f;
@@ -428,22 +453,21 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_ends_kernel(const ttt_b2
     whole = mul2(whole, first2(v));
   }
   float* e = q.ends + (static_cast<long>(at.b) * q.chunks + at.chunk) * 2 * p.D;
-  store2<float, kWhole>(e, at.d, p.D, whole);
-  store2<float, kWhole>(e + p.D, at.d, p.D, own);
+  store2<float, kMode>(e, at.d, p.D, whole);
+  store2<float, kMode>(e + p.D, at.d, p.D, own);
 }
 
-template <class T, bool kWhole, bool kUsual, int W>
+template <class T, int kMode, bool kUsual, int W>
 __global__ void __launch_bounds__(32 * W, 16 / W) gated_forward_kernel(const ttt_b200_gated_args p, const Plan q) {
   wait_for_predecessor();
-  using R = Rows<T, kWhole>;
+  using R = Rows<T, kMode>;
   __shared__ Steps<W> join;
   extern __shared__ __align__(16) unsigned char rings[];
   const At<W> at(p, q, q.chunks);
   constexpr int kTile = At<W>::kTile;
   const int d0 = at.tile * kCols;
-  const Weights z = weights_of<kWhole>(p, at.d);
-  const R rx(p.x, p.x_stride[0], p.x_stride[1], at.b, d0, p.D), rg(p.gate, p.gate_stride[0], p.gate_stride[1], at.b, d0, p.D),
-      ri(p.input_gate, p.input_stride[0], p.input_stride[1], at.b, d0, p.D);
+  const Weights z = weights_of<kMode>(p, at.d);
+  const R rx(p.x, p.x_stride, at.b, d0, p.D), rg(p.gate, p.gate_stride, at.b, d0, p.D), ri(p.input_gate, p.input_stride, at.b, d0, p.D);
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(rings)) + at.warp * (kStages * 3 * R::kStage);
   const int first = at.first * kTile + at.warp * S, rounds = at.last - at.first;
   auto ahead = [&](int j) {
@@ -457,8 +481,8 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_forward_kernel(const ttt
   };
 #pragma unroll
   for (int j = 0; j < kStages - 1; ++j) ahead(j);
-  F carry = load2<kWhole>(p.state ? p.state + static_cast<long>(at.b) * p.D : nullptr, at.d, p.D, 0.f);
-  carry = join_chunks<kWhole, false>(p, q, at, carry);
+  F carry = load2<kMode>(p.state ? p.state + static_cast<long>(at.b) * p.D : nullptr, at.d, p.D, 0.f);
+  carry = join_chunks<kMode, false>(p, q, at, carry);
   T* y = static_cast<T*>(p.y) + static_cast<long>(at.b) * p.T * p.D;
   for (int j = 0; j < rounds; ++j) {
     const int t0 = first + j * kTile, half = j & 1;
@@ -494,51 +518,49 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_forward_kernel(const ttt
       h = fma2(first2(v), h, second2(v));
     }
     if (at.warp % (kEvery / S) == 0 && p.checkpoints && t0 < at.len)
-      store2<float, kWhole>(p.checkpoints + (static_cast<long>(at.b) * q.nck + t0 / kEvery) * p.D, at.d, p.D, h);
+      store2<float, kMode>(p.checkpoints + (static_cast<long>(at.b) * q.nck + t0 / kEvery) * p.D, at.d, p.D, h);
     T* to = y + static_cast<long>(t0) * p.D;
     if (t0 + S <= at.len) {
 #pragma unroll
       for (int t = 0; t < S; ++t) {
         h = fma2(a[t], h, u[t]);
-        store2<T, kWhole>(to, at.d, p.D, h);
+        store2<T, kMode>(to, at.d, p.D, h);
         to += p.D;
       }
     } else {
 #pragma unroll
       for (int t = 0; t < S; ++t) {
         h = fma2(a[t], h, u[t]);
-        if (t0 + t < p.T) store2<T, kWhole>(to, at.d, p.D, t0 + t < at.len ? h : both(0.f));
+        if (t0 + t < p.T) store2<T, kMode>(to, at.d, p.D, t0 + t < at.len ? h : both(0.f));
         to += p.D;
       }
     }
     if (at.warp == W - 1) carry = join.end[half][at.lane] = h;
   }
-  if (p.final_state && at.chunk == q.chunks - 1 && at.warp == W - 1) store2<float, kWhole>(p.final_state + static_cast<long>(at.b) * p.D, at.d, p.D, carry);
+  if (p.final_state && at.chunk == q.chunks - 1 && at.warp == W - 1) store2<float, kMode>(p.final_state + static_cast<long>(at.b) * p.D, at.d, p.D, carry);
   for (int j = at.last; j < at.end(q, p.T); ++j)
-    for (int t = j * kTile + at.warp * S; t < min(j * kTile + at.warp * S + S, p.T); ++t) store2<T, kWhole>(y + static_cast<long>(t) * p.D, at.d, p.D, both(0.f));
+    for (int t = j * kTile + at.warp * S; t < min(j * kTile + at.warp * S + S, p.T); ++t) store2<T, kMode>(y + static_cast<long>(t) * p.D, at.d, p.D, both(0.f));
 }
 
 // T: the gradients' type; I: that of x and the gates, or 8-bit values
-template <class T, class I, bool kWhole, bool kUsual, int W>
+template <class T, class I, int kMode, bool kUsual, int W>
 __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const ttt_b200_gated_args p, const Plan q) {
   wait_for_predecessor();
-  using R = Rows<I, kWhole>;
-  using U = Rows<T, kWhole>;
-  constexpr uint32_t kStage = 3 * R::kStage + U::kStage;
+  using R = Rows<I, kMode>;
+  using U = Rows<T, kMode>;
+  constexpr uint32_t kStage = 3 * R::kStage + U::kStage + Scales<I>::kStage, kKept = Scales<I>::kThere ? S * 128 : 0;
   __shared__ Steps<W> join;
   __shared__ F back[2][W][32];
   extern __shared__ __align__(16) unsigned char rings[];
   const At<W> at(p, q, q.chunks);
   constexpr int kTile = At<W>::kTile;
   const int d0 = at.tile * kCols;
-  const Weights z = weights_of<kWhole>(p, at.d);
+  const Weights z = weights_of<kMode>(p, at.d);
   const bool gated = kUsual || z.gated;
-  const int groups = p.group ? (p.D + p.group - 1) / p.group : 0;
-  const R rx(p.x, p.x_stride[0], p.x_stride[1], at.b, d0, p.D, p.x_scales, groups, p.group, p.T),
-      rg(p.gate, p.gate_stride[0], p.gate_stride[1], at.b, d0, p.D, p.gate_scales, groups, p.group, p.T),
-      ri(p.input_gate, p.input_stride[0], p.input_stride[1], at.b, d0, p.D, p.input_scales, groups, p.group, p.T);
-  const U ru(p.grad_y, p.gy_stride[0], p.gy_stride[1], at.b, d0, p.D);
-  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(rings)) + at.warp * (kStages * kStage);
+  const R rx(p.x, p.x_stride, at.b, d0, p.D), rg(p.gate, p.gate_stride, at.b, d0, p.D), ri(p.input_gate, p.input_stride, at.b, d0, p.D);
+  const U ru(p.grad_y, p.gy_stride, at.b, d0, p.D);
+  const Scales<I> scales(p, at.b, d0);
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(rings)) + at.warp * (kStages * kStage + kKept);
   const int first = at.first * kTile + at.warp * S, rounds = at.last - at.first;
   auto ahead = [&](int j) {
     if (j >= 0) {
@@ -547,6 +569,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const tt
       rg.copy(to + R::kStage, first + j * kTile, at.len);
       if (gated) ri.copy(to + 2 * R::kStage, first + j * kTile, at.len);
       ru.copy(to + 3 * R::kStage, first + j * kTile, at.len);
+      scales.copy(to + 3 * R::kStage + U::kStage, first + j * kTile, at.len);
     }
     cp_async_commit();
   };
@@ -555,17 +578,24 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const tt
   const long batch = static_cast<long>(at.b) * p.T * p.D;
   T *gx = static_cast<T*>(p.grad_x) + batch, *gg = static_cast<T*>(p.grad_gate) + batch, *gi = static_cast<T*>(p.grad_input) + batch;
   auto put = [&](long o, F x, F g, F i) {
-    store2<T, kWhole>(gx + o, at.d, p.D, x);
-    store2<T, kWhole>(gg + o, at.d, p.D, g);
-    if (gated) store2<T, kWhole>(gi + o, at.d, p.D, i);
+    store2<T, kMode>(gx + o, at.d, p.D, x);
+    store2<T, kMode>(gg + o, at.d, p.D, g);
+    if (gated) store2<T, kMode>(gi + o, at.d, p.D, i);
   };
-  F carry = load2<kWhole>(p.grad_final_state ? p.grad_final_state + static_cast<long>(at.b) * p.D : nullptr, at.d, p.D, 0.f);
-  carry = join_chunks<kWhole, true>(p, q, at, carry);
+  // x is read three times; of 8 bits the first leaves it in bf16, which holds 4 bits times a power of two
+  const uint32_t mine = ring + kStages * kStage + at.lane * 4;
+  auto keep = [&](int t, F x) {
+    const __nv_bfloat162 v = __float22bfloat162_rn(x);
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(mine + t * 128), "r"(reinterpret_cast<const uint32_t&>(v)) : "memory");
+  };
+  auto x_of = [&](int t, uint32_t from, int t0) { return kKept ? pair_of<__nv_bfloat16>(mine + t * 128) : rx.get(from, t, t0 + t); };
+  F carry = load2<kMode>(p.grad_final_state ? p.grad_final_state + static_cast<long>(at.b) * p.D : nullptr, at.d, p.D, 0.f);
+  carry = join_chunks<kMode, true>(p, q, at, carry);
   F sum_a = both(0.f), sum_g = sum_a, sum_i = sum_a;
   for (int j = rounds - 1; j >= 0; --j) {
     const int t0 = first + j * kTile, half = j & 1;
     const int ck = t0 / kEvery;
-    F h = load2<kWhole>(ck * kEvery < at.len ? p.checkpoints + (static_cast<long>(at.b) * q.nck + ck) * p.D : nullptr, at.d, p.D, 0.f);
+    F h = load2<kMode>(ck * kEvery < at.len ? p.checkpoints + (static_cast<long>(at.b) * q.nck + ck) * p.D : nullptr, at.d, p.D, 0.f);
     cp_async_wait<kStages - 2>();
     __syncwarp();
     ahead(j - kStages + 1);
@@ -575,8 +605,10 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const tt
 #pragma unroll
     for (int t = 0; t < S; ++t) {
       Factors<true> f;
-      factors<kUsual, true>(z, rg.get(from + R::kStage, t, t0 + t), [&] { return ri.get(from + 2 * R::kStage, t, t0 + t); }, f);
-      const F x = rx.get(from, t, t0 + t);
+      const float4 sc = scales.get(from + 3 * R::kStage + U::kStage, t);
+      factors<kUsual, true>(z, scales.apply(rg.get(from + R::kStage, t, t0 + t), sc.y), [&] { return scales.apply(ri.get(from + 2 * R::kStage, t, t0 + t), sc.z); }, f);
+      const F x = scales.apply(rx.get(from, t, t0 + t), sc.x);
+      if constexpr (kKept) keep(t, x);
       a[t] = f.a, w[t] = f.w, k[t] = f.k, s[t] = f.s;
       slope[t] = mul2(f.slope, x);
       in[t] = mul2(f.rest, mul2(f.w, x));
@@ -588,7 +620,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const tt
     }
 #pragma unroll
     for (int t = 0; t < S; ++t) {
-      own = fma2(a[t], own, mul2(w[t], rx.get(from, t, t0 + t)));
+      own = fma2(a[t], own, mul2(w[t], x_of(t, from, t0)));
       whole = mul2(whole, a[t]);
     }
 #pragma unroll
@@ -608,7 +640,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const tt
     for (int t = 0; t < S; ++t) {
       const F kept = mul2(a[t], h);
       slope[t] = add2(kept, slope[t]);
-      h = fma2(w[t], rx.get(from, t, t0 + t), kept);
+      h = fma2(w[t], x_of(t, from, t0), kept);
     }
 #pragma unroll
     for (int v = W - 1; v > 0; --v) {
@@ -637,7 +669,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const tt
     }
     if (at.warp == 0) carry = join.end[half][at.lane] = c;
   }
-  if (p.grad_state && at.chunk == 0 && at.warp == 0) store2<float, kWhole>(p.grad_state + static_cast<long>(at.b) * p.D, at.d, p.D, carry);
+  if (p.grad_state && at.chunk == 0 && at.warp == 0) store2<float, kMode>(p.grad_state + static_cast<long>(at.b) * p.D, at.d, p.D, carry);
   for (int j = at.last; j < at.end(q, p.T); ++j)
     for (int t = j * kTile + at.warp * S; t < min(j * kTile + at.warp * S + S, p.T); ++t) put(static_cast<long>(t) * p.D, both(0.f), both(0.f), both(0.f));
   // the warps' sums, in their order
@@ -651,16 +683,16 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const tt
 #pragma unroll
     for (int w = 1; w < W; ++w) s = add2(s, sums[at.warp][w][at.lane]);
     if (at.warp == 0 && p.A) {      // A counts as 0 where it is above
-      const F A = load2<kWhole>(p.A, at.d, p.D, 0.f);
+      const F A = load2<kMode>(p.A, at.d, p.D, 0.f);
       s = make_float2(A.x > 0.f ? 0.f : s.x, A.y > 0.f ? 0.f : s.y);
     }
-    store2<float, kWhole>(q.part + (static_cast<long>(at.b) * q.chunks + at.chunk) * 3 * p.D + static_cast<long>(at.warp) * p.D, at.d, p.D, s);
+    store2<float, kMode>(q.part + (static_cast<long>(at.b) * q.chunks + at.chunk) * 3 * p.D + static_cast<long>(at.warp) * p.D, at.d, p.D, s);
   }
 }
 
 // A row of the batch and 256 channels to a CTA.  Rows that name the same slot are taken in their order by the CTA of the first of
 // them, so that no two CTAs touch a state.
-template <class T, bool kWhole> __global__ void __launch_bounds__(128) gated_step_kernel(const ttt_b200_gated_args p, int tiles) {
+template <class T, int kMode> __global__ void __launch_bounds__(128) gated_step_kernel(const ttt_b200_gated_args p, int tiles) {
   wait_for_predecessor();
   const int b0 = blockIdx.x / tiles, d = (blockIdx.x % tiles * 128 + threadIdx.x) * 2;
   T* ys = static_cast<T*>(p.y);
@@ -668,7 +700,7 @@ template <class T, bool kWhole> __global__ void __launch_bounds__(128) gated_ste
   if (p.slots) {
     slot = p.slots[b0];
     if (slot < 0 || slot >= p.rows) {
-      store2<T, kWhole>(ys + static_cast<long>(b0) * p.D, d, p.D, both(0.f));
+      store2<T, kMode>(ys + static_cast<long>(b0) * p.D, d, p.D, both(0.f));
       return;
     }
     int before = 0, after = 0;
@@ -680,7 +712,7 @@ template <class T, bool kWhole> __global__ void __launch_bounds__(128) gated_ste
   if (d >= p.D) return;
   auto two = [&](const void* base, int64_t stride, int b) {
     const T* r = static_cast<const T*>(base) + b * stride + d;
-    if constexpr (kWhole) {
+    if constexpr (kMode != kSingles) {
       if constexpr (std::is_same<T, __nv_bfloat16>::value) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(r));
       else if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(r));
       else return *reinterpret_cast<const F*>(r);
@@ -688,19 +720,19 @@ template <class T, bool kWhole> __global__ void __launch_bounds__(128) gated_ste
       return make_float2(to_f32(r[0]), d + 1 < p.D ? to_f32(r[1]) : 0.f);
     }
   };
-  const Weights z = weights_of<kWhole>(p, d);
+  const Weights z = weights_of<kMode>(p, d);
   float* st = p.state_io + static_cast<long>(slot) * p.D;
-  F h = load2<kWhole>(st, d, p.D, 0.f);
+  F h = load2<kMode>(st, d, p.D, 0.f);
   for (int b = b0; b < p.B; ++b) {
     if (b != b0 && p.slots[b] != slot) continue;
     Factors<false> f;
     const F x = two(p.x, p.x_stride[0], b);
     factors<false, false>(z, two(p.gate, p.gate_stride[0], b), [&] { return two(p.input_gate, p.input_stride[0], b); }, f);
     h = fma2(f.a, h, mul2(f.w, x));
-    store2<T, kWhole>(ys + static_cast<long>(b) * p.D, d, p.D, h);
+    store2<T, kMode>(ys + static_cast<long>(b) * p.D, d, p.D, h);
     if (!more) break;
   }
-  store2<float, kWhole>(st, d, p.D, h);
+  store2<float, kMode>(st, d, p.D, h);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
@@ -713,18 +745,25 @@ int check(const ttt_b200_gated_args* p) {
   return TTT_B200_OK;
 }
 
-bool rows16(const void* a, const int64_t* st, int es) { return aligned16(a) && st[0] * es % 16 == 0 && st[1] * es % 16 == 0; }
-bool even(const void* a, int es) { return reinterpret_cast<uintptr_t>(a) % (2 * es) == 0; }
+// how rows of values of `size` bytes start
+int mode_of(const void* a, const int64_t* st, int size) {
+  const uintptr_t all = reinterpret_cast<uintptr_t>(a) | static_cast<uintptr_t>(st[0] * size) | static_cast<uintptr_t>(st[1] * size);
+  return all % 16 == 0 ? kWholeRows : all % (2 * size) == 0 ? kPairs : kSingles;
+}
+bool even(const void* a, int size) { return reinterpret_cast<uintptr_t>(a) % (2 * size) == 0; }
 int size_of(const ttt_b200_gated_args& p) { return p.dtype == TTT_B200_FP32 ? 4 : 2; }
-// whether lanes can take their two channels as a pair, and rows be copied in 16-byte pieces
-bool whole(const ttt_b200_gated_args& p, bool backward) {
+// what all rows that are read allow, and all that is written
+int mode_of(const ttt_b200_gated_args& p, bool backward) {
   const int es = size_of(p), in = p.group ? 1 : es;
-  bool ok = p.D % 2 == 0 && rows16(p.x, p.x_stride, in) && rows16(p.gate, p.gate_stride, in) && (!p.input_gate || rows16(p.input_gate, p.input_stride, in));
+  bool ok = p.D % 2 == 0;
   for (const float* v : {p.A, p.gate_bias, p.input_bias, p.state, static_cast<const float*>(p.final_state), static_cast<const float*>(p.checkpoints), p.grad_final_state,
                          static_cast<const float*>(p.grad_state)})
     ok = ok && even(v, 4);
-  if (!backward) return ok && even(p.y, es);
-  return ok && rows16(p.grad_y, p.gy_stride, es) && even(p.grad_x, es) && even(p.grad_gate, es) && even(p.grad_input, es);
+  ok = ok && (backward ? even(p.grad_x, es) && even(p.grad_gate, es) && even(p.grad_input, es) : even(p.y, es));
+  if (!ok) return kSingles;
+  int mode = std::min(mode_of(p.x, p.x_stride, in), mode_of(p.gate, p.gate_stride, in));
+  if (p.input_gate) mode = std::min(mode, mode_of(p.input_gate, p.input_stride, in));
+  return backward ? std::min(mode, mode_of(p.grad_y, p.gy_stride, es)) : mode;
 }
 
 // How many chunks a sequence is cut into, of how many tiles, and whether a CTA has 8 warps (two CTAs to an SM) or 16: by what a round of tiles takes, in
@@ -735,12 +774,14 @@ void plan(Plan& q, const ttt_b200_gated_args& p, bool backward) {
   q.tiles = (p.D - 1) / kCols + 1;
   q.nck = (p.T - 1) / kEvery + 1;
   const long columns = static_cast<long>(q.tiles) * p.B, sms = sm_count();
-  auto main = [&](long ctas, long rounds) { return 30 + (ctas <= sms ? 15 : 24 * ((ctas + 2 * sms - 1) / (2 * sms))) * rounds; };
+  const bool large = backward && p.dtype == TTT_B200_FP32 && !p.group;      // rows of four fp32 tensors: one CTA of 8 warps to an SM
+  auto main = [&](long ctas, long rounds) {
+    return 30 + (ctas <= sms || large ? 15 * ((ctas + sms - 1) / sms) : 24 * ((ctas + 2 * sms - 1) / (2 * sms))) * rounds;
+  };
   long best = main(columns, q.nck);
   q.warps = 8;
   q.chunk = q.nck;
-  // (16 warps' rows of four fp32 tensors are more than the shared memory holds)
-  if (columns <= sms && p.T > 8 * S && !(backward && p.dtype == TTT_B200_FP32 && !p.group)) {
+  if (columns <= sms && p.T > 8 * S && !large) {
     const int rounds = (p.T - 1) / (16 * S) + 1;
     const long cost = 30 + 24L * rounds;
     if (cost < best) best = cost, q.warps = 16, q.chunk = rounds;
@@ -750,10 +791,6 @@ void plan(Plan& q, const ttt_b200_gated_args& p, bool backward) {
     const long cost = main(columns * chunks, chunk) + main(columns * (chunks - 1), chunk) * 6 / 10 + 20;
     if (cost < best) best = cost, q.warps = 8, q.chunk = chunk;
   }
-#ifdef TTT_PROBE
-  if (getenv("TTT_PROBE_C")) q.warps = 8, q.chunk = (q.nck + atoi(getenv("TTT_PROBE_C")) - 1) / atoi(getenv("TTT_PROBE_C"));
-  if (getenv("TTT_PROBE_W")) q.warps = 16, q.chunk = (p.T - 1) / (16 * S) + 1;
-#endif
   const int tiles = (p.T - 1) / (q.warps * S) + 1;
   q.chunks = (tiles + q.chunk - 1) / q.chunk;
 }
@@ -770,33 +807,40 @@ template <auto kKernel> int launch(long grid, const Plan& q, const ttt_b200_gate
 
 bool usual(const ttt_b200_gated_args& p) { return p.A && p.input_gate && p.mix == TTT_B200_MIX_SQRT; }
 
-template <class T, bool kWhole, bool kUsual> int forward_as(const ttt_b200_gated_args& p, const Plan& q, cudaStream_t s) {
-  constexpr uint32_t bytes = kStages * 3 * Rows<T, kWhole>::kStage;      // of a warp
+template <class T, int kMode, bool kUsual> int forward_as(const ttt_b200_gated_args& p, const Plan& q, cudaStream_t s) {
+  constexpr uint32_t bytes = kStages * 3 * Rows<T, kMode>::kStage;      // of a warp
   const long columns = static_cast<long>(p.B) * q.tiles;
-  if (q.warps == 16) return launch<gated_forward_kernel<T, kWhole, kUsual, 16>>(columns, q, p, 512, 16 * bytes, s, "gated scan");
+  if (q.warps == 16) return launch<gated_forward_kernel<T, kMode, kUsual, 16>>(columns, q, p, 512, 16 * bytes, s, "gated scan");
   if (q.chunks > 1)
-    if (int rc = launch<gated_ends_kernel<T, T, kWhole, kUsual, false, 8>>(columns * (q.chunks - 1), q, p, 256, 8 * bytes, s, "gated scan")) return rc;
-  return launch<gated_forward_kernel<T, kWhole, kUsual, 8>>(columns * q.chunks, q, p, 256, 8 * bytes, s, "gated scan");
+    if (int rc = launch<gated_ends_kernel<T, T, kMode, kUsual, false, 8>>(columns * (q.chunks - 1), q, p, 256, 8 * bytes, s, "gated scan")) return rc;
+  return launch<gated_forward_kernel<T, kMode, kUsual, 8>>(columns * q.chunks, q, p, 256, 8 * bytes, s, "gated scan");
 }
 template <class T> int forward(const ttt_b200_gated_args& p, cudaStream_t s) {
   Plan q = {};
   plan(q, p, false);
   q.ends = static_cast<float*>(p.scratch);
-  if (whole(p, false)) return usual(p) ? forward_as<T, true, true>(p, q, s) : forward_as<T, true, false>(p, q, s);
-  return usual(p) ? forward_as<T, false, true>(p, q, s) : forward_as<T, false, false>(p, q, s);
+  switch (mode_of(p, false)) {
+    case kWholeRows: return usual(p) ? forward_as<T, kWholeRows, true>(p, q, s) : forward_as<T, kWholeRows, false>(p, q, s);
+    case kPairs: return usual(p) ? forward_as<T, kPairs, true>(p, q, s) : forward_as<T, kPairs, false>(p, q, s);
+    default: return usual(p) ? forward_as<T, kSingles, true>(p, q, s) : forward_as<T, kSingles, false>(p, q, s);
+  }
 }
-template <class T, class I, bool kWhole, bool kUsual> int backward_as(const ttt_b200_gated_args& p, const Plan& q, cudaStream_t s) {
-  constexpr uint32_t in = kStages * Rows<I, kWhole>::kStage, up = kStages * Rows<T, kWhole>::kStage;      // of a warp
+template <class T, class I, int kMode, bool kUsual> int backward_as(const ttt_b200_gated_args& p, const Plan& q, cudaStream_t s) {
+  // of a warp
+  constexpr uint32_t in = kStages * Rows<I, kMode>::kStage, up = kStages * (Rows<T, kMode>::kStage + Scales<I>::kStage), kept = Scales<I>::kThere ? S * 128 : 0;
   const long columns = static_cast<long>(p.B) * q.tiles;
-  if constexpr (16 * (3 * in + up) <= 180 * 1024)
-    if (q.warps == 16) return launch<gated_backward_kernel<T, I, kWhole, kUsual, 16>>(columns, q, p, 512, 16 * (3 * in + up), s, "gated scan backward");
+  if constexpr (16 * (3 * in + up + kept) <= 180 * 1024)
+    if (q.warps == 16) return launch<gated_backward_kernel<T, I, kMode, kUsual, 16>>(columns, q, p, 512, 16 * (3 * in + up + kept), s, "gated scan backward");
   if (q.chunks > 1)
-    if (int rc = launch<gated_ends_kernel<T, I, kWhole, kUsual, true, 8>>(columns * (q.chunks - 1), q, p, 256, 8 * (in + up), s, "gated scan backward")) return rc;
-  return launch<gated_backward_kernel<T, I, kWhole, kUsual, 8>>(columns * q.chunks, q, p, 256, 8 * (3 * in + up), s, "gated scan backward");
+    if (int rc = launch<gated_ends_kernel<T, I, kMode, kUsual, true, 8>>(columns * (q.chunks - 1), q, p, 256, 8 * (in + up), s, "gated scan backward")) return rc;
+  return launch<gated_backward_kernel<T, I, kMode, kUsual, 8>>(columns * q.chunks, q, p, 256, 8 * (3 * in + up + kept), s, "gated scan backward");
 }
 template <class T, class I> int backward_of(const ttt_b200_gated_args& p, const Plan& q, cudaStream_t s) {
-  if (whole(p, true)) return usual(p) ? backward_as<T, I, true, true>(p, q, s) : backward_as<T, I, true, false>(p, q, s);
-  return usual(p) ? backward_as<T, I, false, true>(p, q, s) : backward_as<T, I, false, false>(p, q, s);
+  switch (mode_of(p, true)) {
+    case kWholeRows: return usual(p) ? backward_as<T, I, kWholeRows, true>(p, q, s) : backward_as<T, I, kWholeRows, false>(p, q, s);
+    case kPairs: return usual(p) ? backward_as<T, I, kPairs, true>(p, q, s) : backward_as<T, I, kPairs, false>(p, q, s);
+    default: return usual(p) ? backward_as<T, I, kSingles, true>(p, q, s) : backward_as<T, I, kSingles, false>(p, q, s);
+  }
 }
 template <class T> int backward(const ttt_b200_gated_args& p, cudaStream_t s) {
   Plan q = {};
@@ -819,7 +863,7 @@ template <class T> int step(const ttt_b200_gated_args& p, cudaStream_t s) {
   const int tiles = (p.D + 255) / 256;
   const long grid = static_cast<long>(p.B) * tiles;
   if (grid > 0x7fffffffL) return fail("gated scan step: too many CTAs");
-  ttt_launch_overlapped(ok ? gated_step_kernel<T, true> : gated_step_kernel<T, false>, static_cast<int>(grid), 128, 0, s, p, tiles);
+  ttt_launch_overlapped(ok ? gated_step_kernel<T, kPairs> : gated_step_kernel<T, kSingles>, static_cast<int>(grid), 128, 0, s, p, tiles);
   return launched("gated scan step");
 }
 
