@@ -768,27 +768,29 @@ int mode_of(const ttt_b200_gated_args& p, bool backward) {
 
 // How many chunks a sequence is cut into, of how many tiles, and whether a CTA has 8 warps (two CTAs to an SM) or 16: by what a round of tiles takes, in
 // tenths of a microsecond, measured with 2048 channels and more or fewer sequences.  A CTA of 8 warps that has an SM for itself 15 (it waits for itself), two
-// of them or one of 16 warps 24; the chunks' steps 0.6 of the main kernel, a launch and a start 30.
-// 16384 tokens of 1024 channels, forward / backward us: one chunk 348 / 673, 8 chunks 89 / 126, 18 (by the rule) 73 / 97, 24 83 / 116.
+// of them or one of 16 warps 24, one that has it for the size of its four fp32 rows 30; a turn of CTAs over the SMs starts in 20; the chunks' steps take 0.6 of that.
+// 16384 tokens of 1024 channels, forward / backward us: one chunk 348 / 673, 8 chunks 89 / 126, 18 (by the rule) 73 / 97, 24 83 / 116;
+// 2 x 2048 of 2048: one of 8 warps 51 / 95, of 16 45 / 79, 4 chunks (by the rule) 42 / 56, 8 44 / 60.
 void plan(Plan& q, const ttt_b200_gated_args& p, bool backward) {
   q.tiles = (p.D - 1) / kCols + 1;
   q.nck = (p.T - 1) / kEvery + 1;
   const long columns = static_cast<long>(q.tiles) * p.B, sms = sm_count();
-  const bool large = backward && p.dtype == TTT_B200_FP32 && !p.group;      // rows of four fp32 tensors: one CTA of 8 warps to an SM
-  auto main = [&](long ctas, long rounds) {
-    return 30 + (ctas <= sms || large ? 15 * ((ctas + sms - 1) / sms) : 24 * ((ctas + 2 * sms - 1) / (2 * sms))) * rounds;
+  const bool large = backward && p.dtype == TTT_B200_FP32 && !p.group;
+  auto rounds_of = [&](long ctas, long rounds, bool one) {
+    if (!one && ctas <= sms) return 35 + 15 * rounds;
+    return 15 + (one ? (30 * rounds + 20) * ((ctas + sms - 1) / sms) : (24 * rounds + 20) * ((ctas + 2 * sms - 1) / (2 * sms)));
   };
-  long best = main(columns, q.nck);
+  long best = rounds_of(columns, q.nck, large);
   q.warps = 8;
   q.chunk = q.nck;
   if (columns <= sms && p.T > 8 * S && !large) {
     const int rounds = (p.T - 1) / (16 * S) + 1;
-    const long cost = 30 + 24L * rounds;
+    const long cost = 35 + 24L * rounds;
     if (cost < best) best = cost, q.warps = 16, q.chunk = rounds;
   }
   for (int n = 2; n <= std::min(kMostChunks, q.nck); ++n) {
     const int chunk = (q.nck + n - 1) / n, chunks = (q.nck + chunk - 1) / chunk;
-    const long cost = main(columns * chunks, chunk) + main(columns * (chunks - 1), chunk) * 6 / 10 + 20;
+    const long cost = rounds_of(columns * chunks, chunk, large) + rounds_of(columns * (chunks - 1), chunk, false) * 6 / 10 + 20;
     if (cost < best) best = cost, q.warps = 8, q.chunk = chunk;
   }
   const int tiles = (p.T - 1) / (q.warps * S) + 1;
