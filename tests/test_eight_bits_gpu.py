@@ -63,6 +63,13 @@ def test_values_at_the_edges():
     assert y.isnan().all()
 
 
+def test_a_row_alone():
+    x = _rows(3, "bf16", 1, 300)[0]
+    _same(saved.pack8(x, group=64)[0], x, 64)
+    (p,) = saved.pack8(x)
+    assert torch.equal(saved.unpack8((p[0], torch.ones((), device="cuda")))[0], p[0].bfloat16())      # one scale to a row
+
+
 def test_no_rows():
     (p,) = saved.pack8(torch.zeros(0, 5, 40, device="cuda"))
     assert p[0].shape == (0, 5, 40) and p[1].shape == (0, 5, 1)
@@ -186,7 +193,7 @@ def test_norm_backward_from_its_statistics(norm, bias):
 # ---- backward passes from what was kept -------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("ty", ["bf16", "fp32"])
 @pytest.mark.parametrize("group", [32, 64, 128])
-@pytest.mark.parametrize("T,D", [(70, 64), (130, 200), (9, 75), (65, 130), (200, 1040)])
+@pytest.mark.parametrize("T,D", [(70, 64), (130, 200), (9, 75), (65, 130), (200, 1040), (900, 66)])
 def test_gated_backward_from_8_bits(ty, group, T, D):
     for igate, lengths in ((True, None), (False, [T, T // 2])):
         i = gated_inputs(1, ty, 2, T, D, "cuda", igate=igate, lengths=lengths)

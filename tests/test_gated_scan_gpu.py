@@ -98,6 +98,21 @@ def test_few_channels_and_long_sequences(B, T, D):
     _run(10, "bf16", B, T, D, lengths=[T - 37] * B)
 
 
+@pytest.mark.parametrize("ty", ["bf16", "fp32"])
+def test_chunks_without_tokens(ty):
+    """Long sequences in chunks beside short and empty ones, whose later chunks have nothing."""
+    _run(19, ty, 4, 1500, 70, lengths=[1500, 700, 1, 0])
+    _run(20, ty, 3, 900, 128, "linear", A=False, lengths=[130, 900, 64], rows="wide")
+
+
+def test_expanded_inputs():
+    """One gate for all tokens, one sequence for the batch."""
+    i = gated_inputs(21, "bf16", 3, 300, 66, "cuda")
+    i["gate"] = i["gate"][:, :1].expand(3, 300, 66)
+    i["x"] = i["x"][:1].expand(3, 300, 66)
+    hold(i, "sqrt", run_both(i, "sqrt"), "expanded")
+
+
 def test_a_long_sequence_keeps_its_precision():
     i = gated_inputs(11, "fp32", 1, 5000, 64, "cuda")
     i["A"][:] = -1e-3
