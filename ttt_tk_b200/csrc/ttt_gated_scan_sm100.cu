@@ -7,13 +7,20 @@
 // dx = G b i;  d input_gate = G b x i (1 - i);  d log a = G (a h_{t-1} + i x db/dlog a), db/dlog a = -a^2 / b, -a or 0;
 // d gate = d log a times A s (1 - s), without A times 1 - s;  dA = sum d log a s;  dh_{-1} = c_0.
 //
-// Bound by memory: a value is read three times 2 bytes and written once (bf16; backward four and three times), for some 40 fp32
-// operations and six of the exponential unit.  A recurrence of steps h -> p h + q joins: two after one another are p2 p1, p2 q1 + q2.  So a
-// warp has S tokens of 64 channels in registers (two neighbouring channels to a lane), the warps of a CTA have the tokens behind one another
-// of a tile, each takes its tokens from zero, and all join what is in front of them over shared memory: one pass over the data, one barrier.
+// Of a token and pair of channels the forward reads 12 bytes and writes 4 (bf16; backward 16 and 12), for 10 operations of the exponential unit and some 80
+// instructions (backward 180): with every SM full the unit, the heavy half of the fp32 pipe and the issue slots are each 60 % busy, the memory 65 %.
+// A recurrence of steps h -> p h + q joins: two after one another are p2 p1, p2 q1 + q2.  So a warp has S tokens of 64 channels in registers (two
+// neighbouring channels to a lane), the warps of a CTA have the tokens behind one another of a tile, each takes its tokens from zero, and all join
+// what is in front of them over shared memory: one pass over the data, one barrier a tile.
 // The backward starts every 64 tokens from the state that the forward left of them and joins both directions over the same barrier.
 // Where channels and sequences do not fill the GPU the sequence is cut into chunks: a first kernel leaves what each chunk does to a state, and
 // every chunk of the main one begins with the steps of those in front of it.  The order of the joins is fixed.
+//
+// Measured, bf16 with A, root and input gate, us (TB/s of the bytes above), forward / backward / backward from 8-bit inputs: 37 x 1024 tokens of 2048
+// channels 147 (4.2) / 284 (3.8) / 308 (2.8); 8 x 4096 of 2048 149 / 288 / 308, 14 % of it SMs with one CTA for two; 4 x 2048 of 2048 43 / 77 / 86; 16384
+// of 1024, in chunks, 31 + 41 / 22 + 76 / 25 + 79.  Not faster: three or four CTAs to an SM (80 and 64 registers: 147 -> 150 and 162); clusters of CTAs
+// along the sequence, joined over distributed shared memory, in place of chunks (16384 of 1024 102, a tile ahead of the exchange 107); four tokens to a
+// warp; constants as kernel arguments (154 -> 165).
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -33,7 +40,7 @@ constexpr int kEvery = TTT_B200_GATED_INTERVAL;     // tokens between two checkp
 constexpr int S = 8;                                // tokens of a warp's part of a tile; a tile is W of them, 64 tokens or 128
 constexpr int kCols = 64;                           // channels of a CTA
 
-constexpr int kMostChunks = 32;
+constexpr int kMostChunks = 32;                     // that a CTA joins the steps of
 
 struct Plan {
   int tiles;      // CTAs side by side: channels / 64
