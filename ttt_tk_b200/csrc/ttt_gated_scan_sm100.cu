@@ -590,8 +590,10 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_forward_kernel(const ttt
     for (int t = j * kTile + at.warp * S; t < min(j * kTile + at.warp * S + S, p.T); ++t) store2<T, kMode>(y + static_cast<long>(t) * p.D, at.d, p.D, both(0.f));
 }
 
+// kStages: tiles of rows in shared memory.  The next one's are on their way while a CTA works on one; of four fp32 tensors two CTAs to an SM have room for one
+// tile (3 x 1001 x 1003 backward 50 -> 45 us), and a CTA that has the SM for itself for two (4 x 2048 x 2048 108 -> 99).
 // T: the gradients' type; I: that of x and the gates, or 8-bit values
-template <class T, class I, int kMode, bool kUsual, int W>
+template <class T, class I, int kMode, bool kUsual, int W, int kStages>
 __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const ttt_b200_gated_args p, const Plan q) {
   wait_for_predecessor();
   using R = Rows<I, kMode>;
@@ -644,9 +646,16 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const tt
     const int t0 = first + j * kTile, half = j & 1;
     const int ck = t0 / kEvery;
     F h = load2<kMode>(ck * kEvery < at.len ? p.checkpoints + (static_cast<long>(at.b) * q.nck + ck) * p.D : nullptr, at.d, p.D, 0.f);
-    cp_async_wait<kStages - 2>();
-    __syncwarp();
-    ahead(j - kStages + 1);
+    if constexpr (kStages == 1) {
+      __syncwarp();      // all lanes are through with the rows in front
+      ahead(j);
+      cp_async_wait<0>();
+      __syncwarp();
+    } else {
+      cp_async_wait<kStages - 2>();
+      __syncwarp();
+      ahead(j - kStages + 1);
+    }
     const uint32_t from = ring + j % kStages * kStage;
     // of a token: a; w = b i; what there is of d log a / G without the state, which joins it; d log a's factors in d gate and dA; d input / G
     F a[S], w[S], slope[S], k[S], s[S], in[S], whole = both(1.f), own = both(0.f), left = both(0.f);
@@ -817,29 +826,26 @@ int mode_of(const ttt_b200_gated_args& p, bool backward) {
 
 // How many chunks a sequence is cut into, of how many tiles, and whether a CTA has 8 warps (two CTAs to an SM) or 16: by what a round of tiles takes, in
 // tenths of a microsecond, measured with 2048 channels and more or fewer sequences.  A CTA of 8 warps that has an SM for itself 15 (it waits for itself), two
-// of them or one of 16 warps 24, one that has it for the size of its four fp32 rows 30; a turn of CTAs over the SMs starts in 20; the chunks' steps take 0.6 of that.
+// of them or one of 16 warps 24; a turn of CTAs over the SMs starts in 20; the chunks' steps take 0.6 of that.
 // 16384 tokens of 1024 channels, forward / backward us: one chunk 348 / 673, 8 chunks 89 / 126, 18 (by the rule) 73 / 97, 24 83 / 116;
 // 2 x 2048 of 2048: one of 8 warps 51 / 95, of 16 45 / 79, 4 chunks (by the rule) 42 / 56, 8 44 / 60.
 void plan(Plan& q, const ttt_b200_gated_args& p, bool backward) {
   q.tiles = (p.D - 1) / kCols + 1;
   q.nck = (p.T - 1) / kEvery + 1;
   const long columns = static_cast<long>(q.tiles) * p.B, sms = sm_count();
-  const bool large = backward && p.dtype == TTT_B200_FP32 && !p.group;
-  auto rounds_of = [&](long ctas, long rounds, bool one) {
-    if (!one && ctas <= sms) return 35 + 15 * rounds;
-    return 15 + (one ? (30 * rounds + 20) * ((ctas + sms - 1) / sms) : (24 * rounds + 20) * ((ctas + 2 * sms - 1) / (2 * sms)));
-  };
-  long best = rounds_of(columns, q.nck, large);
+  auto rounds_of = [&](long ctas, long rounds) { return ctas <= sms ? 35 + 15 * rounds : 15 + (24 * rounds + 20) * ((ctas + 2 * sms - 1) / (2 * sms)); };
+  long best = rounds_of(columns, q.nck);
   q.warps = 8;
   q.chunk = q.nck;
-  if (columns <= sms && p.T > 8 * S && !large) {
+  // (16 warps' rows of four fp32 tensors: the shared memory has room for one tile, and then 8 warps with two are faster)
+  if (columns <= sms && p.T > 8 * S && !(backward && p.dtype == TTT_B200_FP32 && !p.group)) {
     const int rounds = (p.T - 1) / (16 * S) + 1;
     const long cost = 35 + 24L * rounds;
     if (cost < best) best = cost, q.warps = 16, q.chunk = rounds;
   }
   for (int n = 2; n <= std::min(kMostChunks, q.nck); ++n) {
     const int chunk = (q.nck + n - 1) / n, chunks = (q.nck + chunk - 1) / chunk;
-    const long cost = rounds_of(columns * chunks, chunk, large) + rounds_of(columns * (chunks - 1), chunk, false) * 6 / 10 + 20;
+    const long cost = rounds_of(columns * chunks, chunk) + rounds_of(columns * (chunks - 1), chunk) * 6 / 10 + 20;
     if (cost < best) best = cost, q.warps = 8, q.chunk = chunk;
   }
   const int tiles = (p.T - 1) / (q.warps * S) + 1;
@@ -878,13 +884,18 @@ template <class T> int forward(const ttt_b200_gated_args& p, cudaStream_t s) {
 }
 template <class T, class I, int kMode, bool kUsual> int backward_as(const ttt_b200_gated_args& p, const Plan& q, cudaStream_t s) {
   // of a warp
-  constexpr uint32_t in = kStages * Rows<I, kMode>::kStage, up = kStages * (Rows<T, kMode>::kStage + Scales<I>::kStage), kept = Scales<I>::kThere ? S * 128 : 0;
-  const long columns = static_cast<long>(p.B) * q.tiles;
-  if constexpr (16 * (3 * in + up + kept) <= 180 * 1024)
-    if (q.warps == 16) return launch<gated_backward_kernel<T, I, kMode, kUsual, 16>>(columns, q, p, 512, 16 * (3 * in + up + kept), s, "gated scan backward");
+  constexpr uint32_t in = Rows<I, kMode>::kStage, up = Rows<T, kMode>::kStage + Scales<I>::kStage, kept = Scales<I>::kThere ? S * 128 : 0;
+  constexpr uint32_t one = 3 * in + up + kept, two = 2 * (3 * in + up) + kept;
+  constexpr bool kLarge = sizeof(T) == 4 && sizeof(I) == 4;
+  const char* what = "gated scan backward";
+  const long columns = static_cast<long>(p.B) * q.tiles, ctas = columns * q.chunks;
+  if constexpr (!kLarge)
+    if (q.warps == 16) return launch<gated_backward_kernel<T, I, kMode, kUsual, 16, 2>>(columns, q, p, 512, 16 * two, s, what);
   if (q.chunks > 1)
-    if (int rc = launch<gated_ends_kernel<T, I, kMode, kUsual, true, 8>>(columns * (q.chunks - 1), q, p, 256, 8 * (in + up), s, "gated scan backward")) return rc;
-  return launch<gated_backward_kernel<T, I, kMode, kUsual, 8>>(columns * q.chunks, q, p, 256, 8 * (3 * in + up + kept), s, "gated scan backward");
+    if (int rc = launch<gated_ends_kernel<T, I, kMode, kUsual, true, 8>>(columns * (q.chunks - 1), q, p, 256, 8 * kStages * (in + up), s, what)) return rc;
+  if constexpr (kLarge)
+    if (ctas > sm_count()) return launch<gated_backward_kernel<T, I, kMode, kUsual, 8, 1>>(ctas, q, p, 256, 8 * one, s, what);
+  return launch<gated_backward_kernel<T, I, kMode, kUsual, 8, 2>>(ctas, q, p, 256, 8 * two, s, what);
 }
 template <class T, class I> int backward_of(const ttt_b200_gated_args& p, const Plan& q, cudaStream_t s) {
   switch (mode_of(p, true)) {
