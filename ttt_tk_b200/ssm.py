@@ -134,7 +134,9 @@ def gated_scan_backward(grad_y, x, gate, checkpoints, A=None, input_gate=None, g
                         grad_final_state=None):
     """Gradients of `gated_scan` from its inputs and checkpoints: (grad_x, grad_gate, grad_A, grad_input_gate, grad_gate_bias,
     grad_input_bias, grad_state); None where there is no such input.  Those of the activations have their type, the others are fp32;
-    grad_state fp32 [batch, D] is that of the state in front of the first token.  Where 1 - a^2 is below the least normal fp32 the slope of its root counts as 0,
+    grad_state fp32 [batch, D] is that of the state in front of the first token.  `x`, `gate` and `input_gate` may be (values, scales) of
+    `ttt_tk_b200.saved.pack8`, all of them in the same group: the gradients are then those at the values that 8 bits stand for, with the
+    checkpoints as they are, in grad_y's type.  Where 1 - a^2 is below the least normal fp32 the slope of its root counts as 0,
     and where A is above 0 so does grad_A."""
     return _host().gated_backward(grad_y, x, gate, checkpoints, A, input_gate, gate_bias, input_bias, _mix(mix), lengths, grad_final_state)
 
