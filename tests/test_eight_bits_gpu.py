@@ -268,6 +268,28 @@ def test_the_scan_and_the_block_end_keep_8_bits():
         assert torch.equal(a, c.view_as(a))
 
 
+def test_nothing_to_keep():
+    """No sequences, no tokens: there are 8 bits of nothing, and gradients of nothing."""
+    A = -torch.rand(40, device="cuda")
+    for B, T in ((0, 5), (2, 0)):
+        x = torch.zeros(B, T, 40, device="cuda", requires_grad=True)
+        w = torch.zeros(40, 4, device="cuda", requires_grad=True)
+        for y in (ag.gated_scan(x, x, A, saved="e4m3"), ag.short_conv(x, w, saved="e4m3"), ag.norm_gate_residual(x, pre_weight=A, saved="e4m3")[1]):
+            (g,) = torch.autograd.grad(y.sum(), x)
+            assert g.shape == x.shape
+
+
+def test_backward_twice_and_without_gradients():
+    i = gated_inputs(5, "bf16", 2, 70, 64, "cuda")
+    x = i["x"].clone().requires_grad_(True)
+    y = ag.gated_scan(x, i["gate"], i["A"], saved="e4m3")
+    (a,) = torch.autograd.grad(y, x, i["gy"], retain_graph=True)
+    (b,) = torch.autograd.grad(y, x, i["gy"])
+    assert torch.equal(a, b)
+    with torch.no_grad():
+        assert torch.equal(ag.gated_scan(x, i["gate"], i["A"], saved="e4m3"), y)
+
+
 def test_what_is_kept_is_half():
     x = torch.randn(4, 512, 1024, device="cuda", dtype=torch.bfloat16, requires_grad=True)
     w = torch.randn(1024, 4, device="cuda")

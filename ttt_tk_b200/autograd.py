@@ -157,8 +157,10 @@ def ttt_linear(XQ, XK, XV, last_eta, ttt_norm_weight, ttt_norm_bias, W1, b1, che
 # ---- layer-side sequence operators (`ttt_tk_b200.ssm`, the block end of `ttt_tk_b200.glue`) ------------------------------------
 # What is no tensor (None among it) passes, for the operator to take or to refuse.
 def _rows(t):
-    """With a contiguous last dimension (an upstream gradient can be an expanded number)."""
-    return t if not isinstance(t, torch.Tensor) or t.dim() == 0 or t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
+    """With a contiguous last dimension (an upstream gradient can be an expanded number; of no elements that counts as contiguous as it is)."""
+    if not isinstance(t, torch.Tensor) or t.dim() == 0 or t.stride(-1) == 1 or t.size(-1) == 1:
+        return t
+    return t.contiguous() if t.numel() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _whole(t):

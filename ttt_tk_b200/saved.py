@@ -4,8 +4,8 @@
     x, gate = unpack8((qx, sx), (qg, sg))                # bf16
 
 Of each `group` neighbouring values of a row the scale is the least power of two with max |v| <= 448 scale, and v / scale is kept in e4m3: a
-value is off by at most 2^-4 of itself (and by 2^-10 of the scale where it is below 2^-6 of it), the largest of a group among them.  A power of two divides exactly, so
-the format's rounding is the only one.  Infinities are left out of the maximum and become 448 scale; NaN stays NaN.
+value is off by at most 2^-4 of itself, and where it is below 2^-6 of the scale by at most 2^-10 of that.  A power of two divides exactly, so the
+format's rounding is the only one.  Infinities are left out of the maximum and become 448 scale; NaN stays NaN.
 
 `ttt_tk_b200.ssm.gated_scan_backward` takes packed inputs as they are; the differentiable operators of `ttt_tk_b200.autograd` with `saved="e4m3"` keep
 theirs this way.  Calls are stream-ordered and do not synchronise.  A bad argument raises ValueError.
