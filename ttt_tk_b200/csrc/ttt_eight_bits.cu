@@ -170,16 +170,17 @@ struct Shared {
   float top[2][32];
 };
 
-// 1 / sqrt(v), a step of Newton's behind the fast one: an error of all of a token's values alike takes more of them over a border of their rounding
-// to 4 bits than as many errors that differ (16384 x 2048: 4 times the values that differ from those of 64 bits).
-__device__ __forceinline__ float inverse_root(float v) {
+// 1 / sqrt(v) as a sum: the fast one, and a step of Newton's.  An error that all of a token's values have alike takes more of them over a border of their
+// rounding to 4 bits than as many errors that differ: 16384 x 2048, error of all values against 64 bits 6.6e-5 with the fast one alone, where a root and a
+// division have 1.6e-5; with the sum the same as these (some 20 of 33 million values differ).
+__device__ __forceinline__ float2 inverse_root(float v) {
   const float r = rsqrtf(v), e = fmaf(-v * r, r, 1.f);
-  return e < 1.f ? fmaf(0.5f * r, e, r) : r;      // (v = 0, infinite or NaN: r as it is)
+  return make_float2(r, e < 1.f ? 0.5f * r * e : 0.f);      // (v = 0, infinite or NaN: r as it is)
 }
 
-// Mean and 1 / deviation of a token with one barrier: each warp's mean and its squares about it, joined as
+// Mean and 1 / deviation (in two parts) of a token with one barrier: each warp's mean and its squares about it, joined as
 // sum over warps of (squares + columns (mean of the warp - mean)^2).
-template <int kWidth, bool kWhole> __device__ __forceinline__ float2 statistics(const float (&z)[8], const ttt_b200_norm8_args& p, int lane, Shared& sh, int turn) {
+template <int kWidth, bool kWhole> __device__ __forceinline__ float3 statistics(const float (&z)[8], const ttt_b200_norm8_args& p, int lane, Shared& sh, int turn) {
   auto columns = [&](int warp) { return static_cast<float>(min(max(p.D - warp * 256, 0), 256)); };
   const float inv = 1.f / static_cast<float>(p.D);
   float mean = 0.f, sq = 0.f;
@@ -213,7 +214,8 @@ template <int kWidth, bool kWhole> __device__ __forceinline__ float2 statistics(
 #pragma unroll
     for (int o = warps / 2; o; o /= 2) sq += __shfl_xor_sync(0xffffffffu, sq, o);
   }
-  return make_float2(mean, inverse_root(fmaf(sq, inv, p.eps)));
+  const float2 dev = inverse_root(fmaf(sq, inv, p.eps));
+  return make_float3(mean, dev.x, dev.y);
 }
 
 // L lanes to a group; 0: the token has one scale
@@ -248,9 +250,12 @@ __global__ void __launch_bounds__(kWidth* kSide<kWidth>, kNormThreads / (kWidth 
       leave<kWhole>(static_cast<R*>(p.x) + m * p.D, lane, p.D, r);
     }
     ask(m + step);
-    const float2 s = statistics<kWidth, kWhole>(z, p, lane, sh, turn);
+    const float3 s = statistics<kWidth, kWhole>(z, p, lane, sh, turn);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) z[j] = (z[j] - s.x) * s.y * w.v[j];      // (0 behind the last column, as weight and bias)
+    for (int j = 0; j < 8; ++j) {      // (0 behind the last column, as weight and bias)
+      const float c = z[j] - s.x;
+      z[j] = fmaf(c, s.z, c * s.y) * w.v[j];
+    }
     if (p.bias) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) z[j] += column<kWhole>(lane, j) < p.D ? p.bias[column<kWhole>(lane, j)] : 0.f;
@@ -283,7 +288,7 @@ __global__ void __launch_bounds__(kWidth* kSide<kWidth>, kNormThreads / (kWidth 
     }
     if (!live) continue;
     leave<kWhole>(static_cast<uint8_t*>(p.values) + m * p.D, lane, p.D, q);
-    if (p.stats && lane == 0) reinterpret_cast<float4*>(p.stats)[m] = make_float4(0.f, 1.f, s.x, s.y);
+    if (p.stats && lane == 0) reinterpret_cast<float4*>(p.stats)[m] = make_float4(0.f, 1.f, s.x, s.y + s.z);
   }
 }
 
