@@ -669,17 +669,26 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const tt
       if constexpr (kKept) keep(t, x);
       a[t] = f[t].a, w[t] = f[t].w, k[t] = f[t].k, s[t] = f[t].s;
       slope[t] = mul2(f[t].slope, x);
-      in[t] = mul2(f[t].rest, mul2(f[t].w, x));
+      const F u = mul2(f[t].w, x);
+      in[t] = mul2(f[t].rest, u);
+      if constexpr (kKept) {      // (of 16 bits the registers do not hold this as well: 8 x 4096 x 2048 288 -> 298 us, from 8 bits 308 -> 302)
+        own = fma2(a[t], own, u);
+        whole = mul2(whole, a[t]);
+      }
     }
-    if (t0 + S > at.len) {
+    const bool cut = t0 + S > at.len;
+    if (cut) {
 #pragma unroll
       for (int t = 0; t < S; ++t)
         if (t0 + t >= at.len) a[t] = both(1.f), w[t] = both(0.f);
     }
+    if (!kKept || cut) {
+      own = both(0.f), whole = both(1.f);
 #pragma unroll
-    for (int t = 0; t < S; ++t) {
-      own = fma2(a[t], own, mul2(w[t], x_of(t, from, t0)));
-      whole = mul2(whole, a[t]);
+      for (int t = 0; t < S; ++t) {
+        own = fma2(a[t], own, mul2(w[t], x_of(t, from, t0)));
+        whole = mul2(whole, a[t]);
+      }
     }
 #pragma unroll
     for (int t = S - 1; t >= 0; --t) left = mul2(a[t], add2(ru.get(from + 3 * R::kStage, t, t0 + t), left));
