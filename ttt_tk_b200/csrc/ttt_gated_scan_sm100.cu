@@ -16,11 +16,11 @@
 // Where channels and sequences do not fill the GPU the sequence is cut into chunks: a first kernel leaves what each chunk does to a state, and
 // every chunk of the main one begins with the steps of those in front of it.  The order of the joins is fixed.
 //
-// Measured, bf16 with A, root and input gate, us (TB/s of the bytes above), forward / backward / backward from 8-bit inputs: 37 x 1024 tokens of 2048
-// channels 147 (4.2) / 284 (3.8) / 308 (2.8); 8 x 4096 of 2048 149 / 288 / 308, 14 % of it SMs with one CTA for two; 4 x 2048 of 2048 43 / 77 / 86; 16384
-// of 1024, in chunks, 31 + 41 / 22 + 76 / 25 + 79.  Not faster: three or four CTAs to an SM (80 and 64 registers: 147 -> 150 and 162); clusters of CTAs
-// along the sequence, joined over distributed shared memory, in place of chunks (16384 of 1024 102, a tile ahead of the exchange 107); four tokens to a
-// warp; constants as kernel arguments (154 -> 165).
+// Measured, bf16 with A, root and input gate, us (TB/s of the bytes above), forward / backward with the sum of its parts / the same from 8-bit inputs: 37 x 1024
+// tokens of 2048 channels 147 (4.2) / 276 (3.9) / 292 (2.9); 8 x 4096 of 2048 148 / 275 / 292, 14 % of it SMs with one CTA for two; 4 x 2048 of 2048 45 / 81 /
+// 85; 16384 of 1024, in chunks, 73 / 97 / 101, of which the chunks' steps are 31, 21 and 23.  Not faster: three or four CTAs to an SM (80 and 64
+// registers: 147 -> 150 and 162); clusters of CTAs along the sequence, joined over distributed shared memory, in place of chunks (16384 of 1024 102, a
+// tile ahead of the exchange 107); four tokens to a warp; constants as kernel arguments (154 -> 165).
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -150,7 +150,7 @@ template <bool kBack> __device__ __forceinline__ void let_in(const Weights& z, F
 }
 
 // Those of S tokens; `gate` and `input` give a token's.  kUsual: A, the root and an input gate, which leaves nothing to decide (8 x 4096 x 2048 bf16 158 ->
-// 148 us forward, 323 -> 288 backward).  Otherwise each part is decided once for all of the tokens, whose arithmetic then overlaps as well (decided for each
+// 148 us forward, 323 -> 288 backward at the time).  Otherwise each part is decided once for all of the tokens, whose arithmetic then overlaps as well (decided for each
 // token, 16 x 2048 x 2048 bf16: without A and input gate, linear 111 -> 96 and 230 -> 222 us; with both and no mix 180 -> 145 and 302 -> 296).
 template <bool kUsual, bool kBack, int S, class Gate, class Input>
 __device__ __forceinline__ void factors(const Weights& z, Gate gate, Input input, Factors<kBack> (&f)[S]) {
@@ -598,7 +598,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const tt
   wait_for_predecessor();
   using R = Rows<I, kMode>;
   using U = Rows<T, kMode>;
-  constexpr uint32_t kStage = 3 * R::kStage + U::kStage + Scales<I>::kStage, kKept = Scales<I>::kThere ? S * 128 : 0;
+  constexpr uint32_t kStage = 3 * R::kStage + U::kStage + Scales<I>::kStage, kKept = S * 256;
   __shared__ Steps<W> join;
   __shared__ F back[2][W][32];
   extern __shared__ __align__(16) unsigned char rings[];
@@ -632,13 +632,9 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const tt
     store2<T, kMode>(gg + o, at.d, p.D, g);
     if (gated) store2<T, kMode>(gi + o, at.d, p.D, i);
   };
-  // x is read three times; of 8 bits the first leaves it in bf16, which holds 4 bits times a power of two
-  const uint32_t mine = ring + kStages * kStage + at.lane * 4;
-  auto keep = [&](int t, F x) {
-    const __nv_bfloat162 v = __float22bfloat162_rn(x);
-    asm volatile("st.shared.u32 [%0], %1;" ::"r"(mine + t * 128), "r"(reinterpret_cast<const uint32_t&>(v)) : "memory");
-  };
-  auto x_of = [&](int t, uint32_t from, int t0) { return kKept ? pair_of<__nv_bfloat16>(mine + t * 128) : rx.get(from, t, t0 + t); };
+  // u = b i x of each token, for the second pass over a tile, in a place of the thread's own (worked out again from the rows: 8 x 4096 x 2048 288 us for 275)
+  const uint32_t mine = ring + kStages * kStage + at.lane * 8;
+  auto keep = [&](int t, F u) { asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(mine + t * 256), "f"(u.x), "f"(u.y) : "memory"); };
   F carry = load2<kMode>(p.grad_final_state ? p.grad_final_state + static_cast<long>(at.b) * p.D : nullptr, at.d, p.D, 0.f);
   carry = join_chunks<kMode, true>(p, q, at, carry);
   F sum_a = both(0.f), sum_g = sum_a, sum_i = sum_a;
@@ -665,28 +661,20 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const tt
                     [&](int t) { return scales.apply(ri.get(from + 2 * R::kStage, t, t0 + t), scales.get(sc, t).z); }, f);
 #pragma unroll
     for (int t = 0; t < S; ++t) {
-      const F x = scales.apply(rx.get(from, t, t0 + t), scales.get(sc, t).x);
-      if constexpr (kKept) keep(t, x);
+      const F x = scales.apply(rx.get(from, t, t0 + t), scales.get(sc, t).x), u = mul2(f[t].w, x);
+      keep(t, u);
       a[t] = f[t].a, w[t] = f[t].w, k[t] = f[t].k, s[t] = f[t].s;
       slope[t] = mul2(f[t].slope, x);
-      const F u = mul2(f[t].w, x);
       in[t] = mul2(f[t].rest, u);
-      if constexpr (kKept) {      // (of 16 bits the registers do not hold this as well: 8 x 4096 x 2048 288 -> 298 us, from 8 bits 308 -> 302)
-        own = fma2(a[t], own, u);
-        whole = mul2(whole, a[t]);
-      }
+      own = fma2(a[t], own, u);
+      whole = mul2(whole, a[t]);
     }
-    const bool cut = t0 + S > at.len;
-    if (cut) {
-#pragma unroll
-      for (int t = 0; t < S; ++t)
-        if (t0 + t >= at.len) a[t] = both(1.f), w[t] = both(0.f);
-    }
-    if (!kKept || cut) {
+    if (t0 + S > at.len) {      // once more, with the tokens that there are
       own = both(0.f), whole = both(1.f);
 #pragma unroll
       for (int t = 0; t < S; ++t) {
-        own = fma2(a[t], own, mul2(w[t], x_of(t, from, t0)));
+        if (t0 + t >= at.len) a[t] = both(1.f), keep(t, both(0.f));
+        own = fma2(a[t], own, pair_of<float>(mine + t * 256));
         whole = mul2(whole, a[t]);
       }
     }
@@ -707,7 +695,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const tt
     for (int t = 0; t < S; ++t) {
       const F kept = mul2(a[t], h);
       slope[t] = add2(kept, slope[t]);
-      h = fma2(w[t], x_of(t, from, t0), kept);
+      h = add2(pair_of<float>(mine + t * 256), kept);
     }
 #pragma unroll
     for (int v = W - 1; v > 0; --v) {
@@ -893,7 +881,7 @@ template <class T> int forward(const ttt_b200_gated_args& p, cudaStream_t s) {
 }
 template <class T, class I, int kMode, bool kUsual> int backward_as(const ttt_b200_gated_args& p, const Plan& q, cudaStream_t s) {
   // of a warp
-  constexpr uint32_t in = Rows<I, kMode>::kStage, up = Rows<T, kMode>::kStage + Scales<I>::kStage, kept = Scales<I>::kThere ? S * 128 : 0;
+  constexpr uint32_t in = Rows<I, kMode>::kStage, up = Rows<T, kMode>::kStage + Scales<I>::kStage, kept = S * 256;
   constexpr uint32_t one = 3 * in + up + kept, two = 2 * (3 * in + up) + kept;
   constexpr bool kLarge = sizeof(T) == 4 && sizeof(I) == 4;
   const char* what = "gated scan backward";
