@@ -48,6 +48,20 @@ def test_several_tensors_in_rows_at_other_distances(how):
         assert torch.equal(y.double().cpu(), og.e4m3(x, 128)[0])      # 4 bits are less than bf16 has
 
 
+@pytest.mark.parametrize("ty", ["bf16", "fp32"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("how", ["whole", "wide"])
+def test_rows_of_whole_groups(ty, group, how):
+    """Values and scales that follow one another, sources that do or not, the last block in part."""
+    xs = [_rows(k, ty, 7, 123, 256) for k in range(3)]
+    given = [xs[0], xs[1] if how == "whole" else apart(xs[1], "wide"), xs[2]]
+    packs = saved.pack8(*given, group=group)
+    for p, x in zip(packs, xs):
+        _same(p, x, group)
+    for y, x in zip(saved.unpack8(*packs, dtype=TYPES[ty]), xs):
+        assert torch.equal(y.double().cpu(), og.e4m3(x, group)[0].to(TYPES[ty]).double())
+
+
 def test_values_at_the_edges():
     """Zeros, the largest and least values of each type, infinities, NaN, and maxima on both sides of 448 times a power of two."""
     inf, nan = float("inf"), float("nan")

@@ -7,7 +7,7 @@
 // All bound by memory: 2 + 1 bytes a value (16 bits), the norm 2 + 2 + 2 + 1 or with an fp32 residual stream 2 + 4 + 4 + 1.  A thread has eight
 // neighbouring values, one 16-byte access; the lanes of a group, four, eight or sixteen, exchange their largest magnitudes.
 //
-// Measured, bf16: 3 x 32768 x 2048 packed in 117 us and unpacked in 103 (5.3 and 6.0 TB/s; 75 and 80 % of the issue slots); the norm of 16384 x 2048 with an fp32
+// Measured, bf16: 3 x 32768 x 2048 packed in 111 us and unpacked in 102 (5.5 and 6.0 TB/s); the norm of 16384 x 2048 with an fp32
 // residual, a scale to 128, 56 us (6.6 TB/s), with a bf16 residual, layer norm and a scale to a token 56 (4.2 TB/s; 75 % of the issue slots).
 #include <algorithm>
 
@@ -26,6 +26,8 @@ struct Many {
   uint32_t lanes;      // of a row: vectors of eight, whole groups
   uint32_t magic, shift;      // n / lanes for n < 2^31: the high word of n magic, shifted (Granlund and Montgomery 1994)
   int64_t vectors;     // lanes * rows
+  bool flat;           // rows of whole groups: values and scales follow one another, whatever the row
+  bool rows;           // and so do src's: no row is needed
 };
 
 // The row of vector i, and which of its lanes it is.
@@ -37,7 +39,8 @@ __device__ __forceinline__ int64_t row_of(const Many& q, int64_t i, int& lane) {
 
 // A thread has several times eight values, a block of threads apart, all requested before the first are worked on: 2048 threads to an SM with 16 bytes each on
 // their way are less than the memory's latency takes.  3 x 32768 x 2048 bf16, packed / unpacked us with one, two and four: 135 / 135, 125 / 116, 119 / 104; 16384 x
-// 2047, whose values come one by one, 45 / 51, 44 / 54, 43 / 61; fp32 16384 x 2048 35 / 41, 33 / 41, 35 / 43.
+// 2047, whose values come one by one, 45 / 51, 44 / 54, 43 / 61; fp32 16384 x 2048 35 / 41, 33 / 41, 35 / 43.  Since rows of whole groups need no division to be
+// found (`flat`), the first is 111 / 102.
 template <class T, bool kWhole> constexpr int kEach = kWhole && sizeof(T) == 2 ? 4 : 2;
 
 // Columns of a lane's eight values in a row.  Rows on 16-byte boundaries: neighbours, one access.  Others: of the 256 columns of a warp every 32nd, so that each
@@ -71,7 +74,10 @@ template <bool kWhole, int L> __device__ __forceinline__ void to_eight(const flo
     const uint32_t x = scale_exponent(most);
     const float inv = inverse_of(x);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) reinterpret_cast<uint16_t*>(b.v)[j] = static_cast<uint16_t>(two_bytes(v[2 * j] * inv, v[2 * j + 1] * inv));
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = mul2(make_float2(v[2 * j], v[2 * j + 1]), both(inv));
+      reinterpret_cast<uint16_t*>(b.v)[j] = static_cast<uint16_t>(two_bytes(f.x, f.y));
+    }
     if (there && lane % L == 0 && lane / L < groups) scales[lane / L] = scale_of(x);
   } else {
     constexpr int kShare = L / 4;      // of a lane's values in a group of the warp's: 1, 2 or 4
@@ -103,18 +109,28 @@ template <class T, bool kWhole, int L> __global__ void __launch_bounds__(256) pa
 #pragma unroll
   for (int c = 0; c < kN; ++c) {
     const int64_t i = i0 + c * 256;
-    row[c] = row_of(q, i, lane[c]);
-    take<kWhole>(static_cast<const T*>(a.src[k]) + row[c] * a.stride[k], lane[c], i < q.vectors ? a.D : 0, e[c]);
+    if (kWhole && q.rows) {
+      if (i < q.vectors) e[c].load(static_cast<const T*>(a.src[k]) + i * 8);
+    } else {
+      row[c] = row_of(q, i, lane[c]);
+      take<kWhole>(static_cast<const T*>(a.src[k]) + row[c] * a.stride[k], lane[c], i < q.vectors ? a.D : 0, e[c]);
+    }
   }
 #pragma unroll
   for (int c = 0; c < kN; ++c) {
+    const int64_t i = i0 + c * 256;
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = to_f32(e[c].v[j]);
-    const bool there = i0 + c * 256 < q.vectors;
+    const bool there = i < q.vectors;
     Eight<uint8_t> b;
-    to_eight<kWhole, L>(v, lane[c], groups, there, a.scales[k] + row[c] * groups, b);
-    if (there) leave<kWhole>(static_cast<uint8_t*>(a.values[k]) + row[c] * a.D, lane[c], a.D, b);
+    if (kWhole && q.flat) {      // a row of all of them, as it were
+      to_eight<kWhole, L>(v, threadIdx.x % L, 1, there, a.scales[k] + i / L, b);
+      if (there) b.store(static_cast<uint8_t*>(a.values[k]) + i * 8);
+    } else {
+      to_eight<kWhole, L>(v, lane[c], groups, there, a.scales[k] + row[c] * groups, b);
+      if (there) leave<kWhole>(static_cast<uint8_t*>(a.values[k]) + row[c] * a.D, lane[c], a.D, b);
+    }
   }
 }
 
@@ -132,6 +148,13 @@ template <class T, bool kWhole> __global__ void __launch_bounds__(256) unpack8_k
 #pragma unroll
   for (int c = 0; c < kN; ++c) {
     const int64_t i = i0 + c * 256;
+    if (kWhole && q.flat) {
+      if (i < q.vectors) {
+        b[c].load(static_cast<const uint8_t*>(a.values[k]) + i * 8);
+        scale[c][0] = a.scales[k][i >> (shift - 3)];
+      }
+      continue;
+    }
     row[c] = row_of(q, i, lane[c]);
     const int D = i < q.vectors ? a.D : 0;
     take<kWhole>(static_cast<const uint8_t*>(a.values[k]) + row[c] * a.D, lane[c], D, b[c]);
@@ -143,15 +166,17 @@ template <class T, bool kWhole> __global__ void __launch_bounds__(256) unpack8_k
   }
 #pragma unroll
   for (int c = 0; c < kN; ++c) {
-    if (i0 + c * 256 >= q.vectors) continue;
+    const int64_t i = i0 + c * 256;
+    if (i >= q.vectors) continue;
     Eight<T> e;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 f = two_values(reinterpret_cast<const uint16_t*>(b[c].v)[j]);
-      e.v[2 * j] = from_f32<T>(f.x * scale[c][2 * j % kScales]);
-      e.v[2 * j + 1] = from_f32<T>(f.y * scale[c][(2 * j + 1) % kScales]);
+      const float2 f = mul2(two_values(reinterpret_cast<const uint16_t*>(b[c].v)[j]), make_float2(scale[c][2 * j % kScales], scale[c][(2 * j + 1) % kScales]));
+      e.v[2 * j] = from_f32<T>(f.x);
+      e.v[2 * j + 1] = from_f32<T>(f.y);
     }
-    leave<kWhole>(static_cast<T*>(a.dst[k]) + row[c] * a.D, lane[c], a.D, e);
+    if (kWhole && q.flat) e.store(static_cast<T*>(a.dst[k]) + i * 8);
+    else leave<kWhole>(static_cast<T*>(a.dst[k]) + row[c] * a.D, lane[c], a.D, e);
   }
 }
 
@@ -316,6 +341,9 @@ template <class T> int run(Many& q, bool back, cudaStream_t s) {
   q.lanes = static_cast<uint32_t>(lanes);
   if (a.M > (255L << 31) / lanes) return fail("pack8: too many values");
   q.vectors = a.M * lanes;
+  q.flat = whole && (back ? a.group && a.D % a.group == 0 : a.D == 8 * lanes);
+  q.rows = q.flat && !back;
+  for (int k = 0; k < a.count; ++k) q.rows = q.rows && (a.stride[k] == a.D || a.M == 1);
   int bits = 0;      // 2^bits >= lanes
   while (int64_t{1} << bits < lanes) ++bits;
   q.shift = bits ? bits - 1 : 0;
@@ -364,14 +392,16 @@ template <class T, class R> int norm(const ttt_b200_norm8_args& p, cudaStream_t 
 
 extern "C" int ttt_b200_pack8(const ttt_b200_pack8_args* p, void* stream) {
   if (int rc = check(p, false)) return rc;
-  Many q = {*p, 0, 0};
+  Many q = {};
+  q.a = *p;
   TTT_WITH_TYPE(p->dtype, return run<Elem>(q, false, static_cast<cudaStream_t>(stream)))
   return TTT_B200_OK;
 }
 
 extern "C" int ttt_b200_unpack8(const ttt_b200_pack8_args* p, void* stream) {
   if (int rc = check(p, true)) return rc;
-  Many q = {*p, 0, 0};
+  Many q = {};
+  q.a = *p;
   TTT_WITH_TYPE(p->dtype, return run<Elem>(q, true, static_cast<cudaStream_t>(stream)))
   return TTT_B200_OK;
 }
