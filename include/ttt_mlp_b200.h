@@ -556,7 +556,7 @@ typedef struct ttt_b200_norm8_args {
 } ttt_b200_norm8_args;
 int ttt_b200_norm_residual_8bit(const ttt_b200_norm8_args* args, void* stream);
 
-/* ---- Rows of tables of states ---- up to 16 tables with the same number of rows, each contiguous, not overlapping one another. */
+/* ---- Rows of tables of states ---- up to 16 tables with the same number of rows, each contiguous, not overlapping one another, the rows' numbers or `used`. */
 enum { TTT_B200_TABLES = 16, TTT_B200_TABLE_PAIRS = 4096 };
 typedef struct ttt_b200_tables_args {
   void* table[TTT_B200_TABLES];

@@ -115,6 +115,18 @@ def test_tables_that_overlap():
             tables.copy_rows(ts, I(1), I(1))
 
 
+def test_rows_named_from_within_a_table():
+    """One block of the GPU would read them while another writes that table."""
+    at, used = torch.zeros(4, dtype=torch.int32), torch.zeros(4, dtype=torch.bool)
+    states = torch.zeros(4, 3)
+    for call in (lambda: tables.copy_rows([states, at], at, I(4)), lambda: tables.copy_rows([states, at], I(4), at), lambda: tables.copy_rows([at], at[1:3], I(2)),
+                 lambda: tables.clear_rows([at], at), lambda: tables.compact_rows([states, used], used), lambda: tables.compact_rows(used.view(torch.uint8), used)):
+        with pytest.raises(ValueError, match="overlap a table"):
+            call()
+    with pytest.raises(ValueError, match="CUDA"):      # next to one another
+        tables.copy_rows([states[:2], at[:2]], at[2:], I(2))
+
+
 def test_clear_and_compact():
     t = torch.zeros(4, 3)
     for rows, msg in ((torch.zeros(2), "rows"), (I(4097), "4096"), (None, "tensor"), (I(2), "CUDA")):

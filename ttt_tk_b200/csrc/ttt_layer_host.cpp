@@ -948,11 +948,20 @@ int64_t tables_of(Call& c, ttt_b200_tables_args& a, PyObject* v) {
   a.rows = static_cast<int32_t>(rows);
   return rows;
 }
+// What names the rows is read by every block while others write.
+void apart(const Call& c, const ttt_b200_tables_args& a, const Tensor& t, const char* name) {
+  const char *p = static_cast<char*>(t.data_ptr()), *end = p + t.nbytes();
+  for (int j = 0; j < a.count; ++j) {
+    const char* q = static_cast<char*>(a.table[j]);
+    c.need(end <= q || q + a.rows * a.row_bytes[j] <= p, (std::string(name) + " must not overlap a table").c_str());
+  }
+}
 const int32_t* pairs_of(Call& c, ttt_b200_tables_args& a, PyObject* o, const char* name) {
   const Tensor& t = *c.any(o, name);
   c.need(t.dim() == 1 && t.scalar_type() == at::kInt && t.is_contiguous(), (std::string(name) + " must be contiguous int32 [n]").c_str());
   c.need(t.size(0) <= TTT_B200_TABLE_PAIRS, (std::string("at most 4096 rows in ") + name).c_str());
   a.pairs = static_cast<int32_t>(t.size(0));
+  if (a.pairs) apart(c, a, t, name);
   return static_cast<const int32_t*>(t.data_ptr());
 }
 
@@ -996,6 +1005,7 @@ PyObject* compact_rows(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     const Tensor& used = *c.shaped(v[1], "used", at::kBool, {rows});
     c.need(used.is_contiguous(), "used must be contiguous");
     c.need(rows <= 8192, "at most 8192 rows");
+    apart(c, a, used, "used");
     const c10::Device dev = c.device();
     const c10::cuda::CUDAGuard guard(dev);
     const Tensor place = fresh({rows}, at::kInt, dev);
