@@ -526,7 +526,8 @@ uint64_t ttt_b200_norm_gate_residual_scratch_bytes(const ttt_b200_block_args* ar
 
 /* ---- Activations in 8 bits ----
  * Of each `group` (32, 64 or 128) neighbouring values of a row one fp32 scale, the least power of two with max |v| <= 448 scale (of the finite
- * values; at least 2^-126), and v / scale in e4m3, ties to even; infinities become 448 scale, NaN stays.  One to four tensors of the same shape. */
+ * values; at least 2^-126), and v / scale in e4m3, ties to even; infinities become 448 scale, NaN stays.  One to four tensors of the same shape.
+ * What they stand for is finite: at most 240 2^120, in fp16 65504, also where a magnitude has been rounded up to 2^128 or 2^16. */
 enum { TTT_B200_PACK8_TENSORS = 4 };
 typedef struct ttt_b200_pack8_args {
   const void* src[TTT_B200_PACK8_TENSORS];  /* pack: [M][D], strides */

@@ -1,6 +1,8 @@
 // Activations in 8 bits: of each group of neighbouring values of a row, one fp32 scale, the least power of two with max |v| <= 448 scale,
 // and v / scale in e4m3 (rounded to the nearest, ties to even).  A power of two divides exactly, so the only rounding is the format's own.
 // Infinities are left out of the maximum and become 448 scale; NaN stays.  A group of zeros has the least scale there is.
+// A magnitude just below a power of two rounds up to it, which its type may not have: 256 times the largest scale, 2^120, is no fp32, and 256 times 2^8 no
+// fp16.  What is finite stays so: at the scale of 2^120 240 is the most that a byte stands for, and a value in 16 bits is at most the largest there is.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -35,6 +37,10 @@ __device__ __forceinline__ uint32_t two_bytes(float a, float b) {
 __device__ __forceinline__ float2 two_values(uint32_t bytes) {
   return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(bytes), __NV_E4M3)));
 }
+
+constexpr float kLargestScale = 0x1p120f;
+// The largest magnitude that unpacking gives.
+template <class T> constexpr float kMostOf = std::is_same<T, __half>::value ? 65504.f : 240.f * kLargestScale;
 
 // Eight neighbouring values in memory, in pieces of up to 16 bytes where they start on a boundary.
 template <class T> struct Eight {

@@ -78,6 +78,12 @@ __device__ __forceinline__ float rcp(float v) {
 
 __device__ __forceinline__ float2 ex2(float2 v) { return make_float2(ex2(v.x), ex2(v.y)); }
 __device__ __forceinline__ float2 rcp(float2 v) { return make_float2(rcp(v.x), rcp(v.y)); }
+// The magnitude bounded; NaN stays.
+__device__ __forceinline__ float at_most(float v, float most) {
+  float r;
+  asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(most));
+  return r;
+}
 __device__ __forceinline__ float least(float a, float b) { return fminf(a, b); }
 __device__ __forceinline__ float2 least(float2 a, float b) { return make_float2(fminf(a.x, b), fminf(a.y, b)); }
 

@@ -5,7 +5,8 @@
 
 Of each `group` neighbouring values of a row the scale is the least power of two with max |v| <= 448 scale, and v / scale is kept in e4m3: a
 value is off by at most 2^-4 of itself, and where it is below 2^-6 of the scale by at most 2^-10 of that.  A power of two divides exactly, so the
-format's rounding is the only one.  Infinities are left out of the maximum and become 448 scale; NaN stays NaN.
+format's rounding is the only one.  What is finite comes back finite: a value that rounds up to 2^16 in fp16 or 2^128 in bf16 and fp32 is the type's
+largest, of the last two 240 2^120.  Infinities are left out of the maximum and become 448 scale, or that largest value; NaN stays NaN.
 
 `ttt_tk_b200.ssm.gated_scan_backward` takes packed inputs as they are; the differentiable operators of `ttt_tk_b200.autograd` with `saved="e4m3"` keep
 theirs this way.  Calls are stream-ordered and do not synchronise.  A bad argument raises ValueError.
