@@ -529,6 +529,7 @@ uint64_t ttt_b200_norm_gate_residual_scratch_bytes(const ttt_b200_block_args* ar
  * values; at least 2^-126), and v / scale in e4m3, ties to even; infinities become 448 scale, NaN stays.  One to four tensors of the same shape.
  * What they stand for is finite: at most 240 2^120, in fp16 65504, also where a magnitude has been rounded up to 2^128 or 2^16. */
 enum { TTT_B200_PACK8_TENSORS = 4 };
+enum { TTT_B200_CLAMP_LOW = 1, TTT_B200_CLAMP_BOTH = 2 };
 typedef struct ttt_b200_pack8_args {
   const void* src[TTT_B200_PACK8_TENSORS];  /* pack: [M][D], strides */
   void* values[TTT_B200_PACK8_TENSORS];     /* [M][D] e4m3; unpack reads them */
@@ -537,6 +538,8 @@ typedef struct ttt_b200_pack8_args {
   int64_t stride[TTT_B200_PACK8_TENSORS];
   int64_t M;
   int32_t D, dtype /* of src or dst */, group /* unpack: 0 for one scale to a row */, count;
+  int32_t clamp[TTT_B200_PACK8_TENSORS]; /* pack: 0, or TTT_B200_CLAMP_LOW, _BOTH: values below -448, infinities among them, count as -448, and with
+                                          * _BOTH those above 448 as 448: for gates, whose masks would otherwise take their neighbours' digits */
 } ttt_b200_pack8_args;
 int ttt_b200_pack8(const ttt_b200_pack8_args* args, void* stream);
 int ttt_b200_unpack8(const ttt_b200_pack8_args* args, void* stream);

@@ -187,13 +187,13 @@ def _even(t):
     return t if at_all else t.contiguous()
 
 
-def _pack(*ts):
-    """Tensors of one shape (None among them) in 8 bits, flat: values, scales, values, ...; those of one type in one launch."""
+def _pack(*ts, clamp=None):
+    """Tensors of one shape (None among them) in 8 bits, flat: values, scales, values, ...; those of one type in one launch.  `clamp` as `pack8`'s."""
     from .saved import pack8
-    flat = [None] * (2 * len(ts))
+    flat, clamp = [None] * (2 * len(ts)), clamp or (None,) * len(ts)
     for ty in {t.dtype for t in ts if t is not None}:
         at = [k for k, t in enumerate(ts) if t is not None and t.dtype == ty]
-        for k, p in zip(at, pack8(*[_even(ts[k]) for k in at])):
+        for k, p in zip(at, pack8(*[_even(ts[k]) for k in at], clamp=[clamp[k] for k in at])):
             flat[2 * k], flat[2 * k + 1] = p
     return flat
 
@@ -260,7 +260,7 @@ class SSMScanFunction(torch.autograd.Function):
         r = r if isinstance(r, tuple) else (r,)
         ctx.packed = x.dtype if packed else None
         if keep:
-            ctx.save_for_backward(A, B, C, D, dt_bias, lengths, r[-1], *(_pack(x, dt) if packed else (x, dt)))
+            ctx.save_for_backward(A, B, C, D, dt_bias, lengths, r[-1], *(_pack(x, dt, clamp=(None, "low" if softplus else None)) if packed else (x, dt)))
         ctx.softplus, ctx.has_state = softplus, state is not None
         ctx.set_materialize_grads(False)
         return r[0], r[1] if return_state else None
@@ -279,7 +279,8 @@ class SSMScanFunction(torch.autograd.Function):
 
 def ssm_scan(x, dt, A, B, C, D=None, dt_bias=None, *, softplus=True, state=None, lengths=None, return_state=False, saved=None):
     """Differentiable `ttt_tk_b200.ssm.ssm_scan`; where gradients are recorded, the checkpoints are kept for the backward.  `saved` "e4m3": x and dt are
-    kept in 8 bits, and the gradients are those at what was kept, with the checkpoints as the forward has them."""
+    kept in 8 bits, and the gradients are those at what was kept, with the checkpoints as the forward has them; a dt below -448 (a mask's -inf) is kept as
+    -448, which softplus takes to 0 as well as it."""
     y, end = SSMScanFunction.apply(x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state, torch.is_grad_enabled(), _saved(saved))
     return (y, end) if return_state else y
 
@@ -298,7 +299,8 @@ class GatedScanFunction(torch.autograd.Function):
                            return_checkpoints=keep)
         r = r if isinstance(r, tuple) else (r,)
         if keep:
-            ctx.save_for_backward(A, gate_bias, input_bias, lengths, r[-1], *(_pack(x, gate, input_gate) if packed else (x, gate, input_gate)))
+            kept = (x, gate, input_gate)
+            ctx.save_for_backward(A, gate_bias, input_bias, lengths, r[-1], *(_pack(*kept, clamp=(None, "both", "both")) if packed else kept))
         ctx.mix, ctx.has_state, ctx.like = mix, state is not None, (x.shape, x.dtype, x.device)
         ctx.set_materialize_grads(False)
         return r[0], r[1] if return_state else None
@@ -321,7 +323,8 @@ class GatedScanFunction(torch.autograd.Function):
 def gated_scan(x, gate, A=None, input_gate=None, gate_bias=None, input_bias=None, *, mix="sqrt", state=None, lengths=None, return_state=False,
                saved=None):
     """Differentiable `ttt_tk_b200.ssm.gated_scan`; where gradients are recorded, the checkpoints are kept for the backward.  `saved` "e4m3": x and the
-    gates are kept in 8 bits, and the gradients are those at what was kept, with the checkpoints as the forward has them."""
+    gates are kept in 8 bits, and the gradients are those at what was kept, with the checkpoints as the forward has them.  Gates beyond 448 on either side,
+    infinities among them, are kept as -448 and 448: a closed gate stays closed (with biases of less than 300)."""
     y, end = GatedScanFunction.apply(x, gate, A, input_gate, gate_bias, input_bias, state, mix, lengths, return_state, torch.is_grad_enabled(),
                                      _saved(saved))
     return (y, end) if return_state else y
@@ -340,7 +343,7 @@ class NormGateResidualFunction(torch.autograd.Function):
         x, n, stats = run(o, residual, gate, **dict(zip(_BLOCK_WEIGHTS, weights)), return_stats=True, **ctx.kw)
         kept = [o, residual, gate]
         ctx.packed = [None if t is None else t.dtype for t in kept] if packed and any(ctx.needs_input_grad) else None
-        ctx.save_for_backward(stats, *weights, *(kept if ctx.packed is None else _pack(*kept)))
+        ctx.save_for_backward(stats, *weights, *(kept if ctx.packed is None else _pack(*kept, clamp=(None, None, "both" if activation == "sigmoid" else "low"))))
         ctx.set_materialize_grads(False)
         return x, n
 
@@ -362,7 +365,7 @@ _BLOCK_WEIGHTS = ("post_weight", "post_bias", "scale", "pre_weight", "pre_bias")
 def norm_gate_residual(o, residual=None, gate=None, *, norm="rms", activation="silu", post_weight=None, post_bias=None, scale=None,
                        pre_weight=None, pre_bias=None, eps=1e-6, saved=None):
     """Differentiable `ttt_tk_b200.glue.norm_gate_residual`, with rows at any distances.  `saved` "e4m3": o, residual and gate are kept in 8 bits, and the
-    gradients are those at what was kept, with the statistics as the forward has them."""
+    gradients are those at what was kept, with the statistics as the forward has them; a gate below -448 (a mask) is kept as -448."""
     for name, t in (("residual", residual), ("gate", gate)):
         if isinstance(o, torch.Tensor) and isinstance(t, torch.Tensor) and t.shape != o.shape:
             raise ValueError(f"norm_gate_residual: {name} must have the shape of o, {list(o.shape)}, got {list(t.shape)}")

@@ -784,9 +784,9 @@ template <class Fn> PyObject* list_of(Py_ssize_t n, Fn one) {
   return r;
 }
 
-// pack8(tuple of tensors, group) -> [(values, scales), ...]
+// pack8(tuple of tensors, group, tuple of a clamp for each or None) -> [(values, scales), ...]
 PyObject* pack8(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
-  return guarded("pack8", nargs, 2, [&]() -> PyObject* {
+  return guarded("pack8", nargs, 3, [&]() -> PyObject* {
     Call c("pack8");
     ttt_b200_pack8_args a = {};
     const Py_ssize_t n = PyTuple_GET_SIZE(v[0]);
@@ -804,6 +804,7 @@ PyObject* pack8(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
       c.need(t.size(-1) <= 1 || t.stride(-1) == 1, "the last dimension of a tensor must be contiguous");
       a.stride[k] = row_stride(c, t, "the rows of a tensor must be at a fixed distance");
       a.src[k] = t.data_ptr();
+      if (v[2] != Py_None) a.clamp[k] = static_cast<int32_t>(integer(PyTuple_GET_ITEM(v[2], k)));
     }
     c.sized(first->size(-1), "a row");
     c.need(first->size(-1) >= 1, "rows have no values");
