@@ -167,6 +167,11 @@ template <class Args> void give(Args& a, const Tensor& scratch) {
 }
 // An output, from the allocator itself: at::empty takes 0.2 us longer (decoding has little else).
 Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const c10::Device& dev) { return at::Tensor(at::detail::empty_cuda(sizes, type, dev, c10::nullopt)); }
+// What a call has changed in place says so to autograd: a backward that kept it refuses then (inference tensors have no version).
+void changed(PyObject* o) {
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* fptr(const Tensor& t) { return static_cast<float*>(ptr(t)); }
 
@@ -316,7 +321,10 @@ PyObject* conv_step(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     const c10::cuda::CUDAGuard guard(dev);
     const Tensor y = at::empty({a.B, a.D}, t.options());
     a.y = y.data_ptr();
-    if (a.B > 0) launch(ttt_b200_short_conv_step, a, dev);
+    if (a.B > 0) {
+      launch(ttt_b200_short_conv_step, a, dev);
+      changed(v[1]);
+    }
     return wrap(y);
   });
 }
@@ -460,7 +468,10 @@ PyObject* scan_step(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     const c10::cuda::CUDAGuard guard(dev);
     const Tensor y = at::empty({a.B, a.D}, at::TensorOptions().dtype(c.type()).device(dev));
     a.y = y.data_ptr();
-    if (a.B > 0) launch(ttt_b200_ssm_scan_step, a, dev);
+    if (a.B > 0) {
+      launch(ttt_b200_ssm_scan_step, a, dev);
+      changed(v[8]);
+    }
     return wrap(y);
   });
 }
@@ -618,7 +629,10 @@ PyObject* gated_step(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     const c10::cuda::CUDAGuard guard(dev);
     const Tensor y = fresh({a.B, a.D}, c.type(), dev);
     a.y = y.data_ptr();
-    if (a.B > 0) launch(ttt_b200_gated_scan_step, a, dev);
+    if (a.B > 0) {
+      launch(ttt_b200_gated_scan_step, a, dev);
+      changed(v[7]);
+    }
     return wrap(y);
   });
 }
@@ -949,6 +963,9 @@ int64_t tables_of(Call& c, ttt_b200_tables_args& a, PyObject* v) {
   a.rows = static_cast<int32_t>(rows);
   return rows;
 }
+void changed_tables(PyObject* v) {
+  for (Py_ssize_t k = 0; k < PyTuple_GET_SIZE(v); ++k) changed(PyTuple_GET_ITEM(v, k));
+}
 // What names the rows is read by every block while others write.
 void apart(const Call& c, const ttt_b200_tables_args& a, const Tensor& t, const char* name) {
   const char *p = static_cast<char*>(t.data_ptr()), *end = p + t.nbytes();
@@ -978,7 +995,10 @@ PyObject* copy_rows(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     c.need(a.pairs == n, "source and target must have as many rows");
     const c10::Device dev = c.device();
     const c10::cuda::CUDAGuard guard(dev);
-    if (rows && n && a.count) launch(ttt_b200_copy_rows, a, dev);
+    if (rows && n && a.count) {
+      launch(ttt_b200_copy_rows, a, dev);
+      changed_tables(v[0]);
+    }
     Py_RETURN_NONE;
   });
 }
@@ -992,7 +1012,10 @@ PyObject* clear_rows(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     a.target = pairs_of(c, a, v[1], "rows");
     const c10::Device dev = c.device();
     const c10::cuda::CUDAGuard guard(dev);
-    if (rows && a.pairs && a.count) launch(ttt_b200_clear_rows, a, dev);
+    if (rows && a.pairs && a.count) {
+      launch(ttt_b200_clear_rows, a, dev);
+      changed_tables(v[0]);
+    }
     Py_RETURN_NONE;
   });
 }
@@ -1012,7 +1035,10 @@ PyObject* compact_rows(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     const Tensor place = fresh({rows}, at::kInt, dev);
     a.used = static_cast<const uint8_t*>(used.data_ptr());
     a.place = static_cast<int32_t*>(place.data_ptr());
-    if (rows) launch(ttt_b200_compact_rows, a, dev);
+    if (rows) {
+      launch(ttt_b200_compact_rows, a, dev);
+      changed_tables(v[0]);
+    }
     return wrap(place);
   });
 }

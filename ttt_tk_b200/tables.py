@@ -6,8 +6,8 @@ weights of each sequence.
     place = compact_rows((windows, states), used)     # the used rows in front of the tables
 
 Tables [S, ...] are contiguous, of any types, all of a call (up to 16) with the same number of rows; they change in place, in one launch.  Calls are
-stream-ordered and do not synchronise, so that the rows may be worked out on the GPU, in tensors that are none of the tables.  A bad argument raises
-ValueError.
+stream-ordered and do not synchronise, so that the rows may be worked out on the GPU, in tensors that are none of the tables.  A backward that has kept rows
+of a table from before such a call refuses, as after any change in place.  A bad argument raises ValueError.
 """
 import torch
 
