@@ -371,6 +371,10 @@ __device__ __forceinline__ F first2(float4 v) { return make_float2(v.x, v.y); }
 __device__ __forceinline__ F second2(float4 v) { return make_float2(v.z, v.w); }
 __device__ __forceinline__ float4 four(F a, F b) { return make_float4(a.x, a.y, b.x, b.y); }
 
+// p of a step over several tokens, a product that may be less than fp32 has: never 0, or an infinite h would leave the step as no number, where the tokens one by
+// one leave it as it is.  (The least number times a finite h is at most 2^-21.)
+__device__ __forceinline__ F some(F p) { return make_float2(max_nan(p.x, 0x1p-149f), max_nan(p.y, 0x1p-149f)); }
+
 // Steps p h + q of the warps of a tile, in two halves that alternate (a barrier lies between two uses of the same one).
 template <int W> struct Steps {
   float4 warp[2][W][32];
@@ -495,8 +499,10 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_ends_kernel(const ttt_b2
 #pragma unroll
     for (int t = 0; t < S; ++t) {
       whole = mul2(whole, a[t]);
+      if constexpr (kBack) whole = some(whole);
       own = kBack ? fma2(whole, u[t], own) : fma2(a[t], own, u[t]);
     }
+    whole = some(whole);
   }
   steps[at.warp][at.lane] = four(whole, own);
   __syncthreads();
@@ -505,7 +511,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_ends_kernel(const ttt_b2
   for (int w = 1; w < W; ++w) {
     const float4 v = steps[w][at.lane];
     own = kBack ? fma2(whole, second2(v), own) : fma2(first2(v), own, second2(v));
-    whole = mul2(whole, first2(v));
+    whole = some(mul2(whole, first2(v)));
   }
   float* e = q.ends + (static_cast<long>(at.b) * q.chunks + at.chunk) * 2 * p.D;
   store2<float, kMode>(e, at.d, p.D, whole);
@@ -563,7 +569,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_forward_kernel(const ttt
       own = fma2(a[t], own, u[t]);
       whole = mul2(whole, a[t]);
     }
-    join.warp[half][at.warp][at.lane] = four(whole, own);
+    join.warp[half][at.warp][at.lane] = four(some(whole), own);
     __syncthreads();
     F h = j == 0 ? carry : join.end[half ^ 1][at.lane];
 #pragma unroll
@@ -687,7 +693,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) gated_backward_kernel(const tt
     }
 #pragma unroll
     for (int t = S - 1; t >= 0; --t) left = mul2(a[t], add2(ru.get(from + 3 * R::kStage, t, t0 + t), left));
-    join.warp[half][at.warp][at.lane] = four(whole, own);
+    join.warp[half][at.warp][at.lane] = four(some(whole), own);
     back[half][at.warp][at.lane] = left;
     __syncthreads();
     F c = j == rounds - 1 ? carry : join.end[half ^ 1][at.lane];

@@ -121,7 +121,7 @@ def gated_scan(x, gate, A=None, input_gate=None, gate_bias=None, input_bias=None
     with b = sqrt(1 - a^2) (`mix` "sqrt", under which inputs of unit variance have states of unit variance), 1 - a ("linear", a running
     mean) or 1 (None).  `x`, `gate`, `input_gate` [batch, T, D] (without an input gate: h = a h + b x); `A`, finite, and the biases fp32 [D];
     `state` fp32 [batch, D] in front of the first token (zeros without it).  A gate of -inf holds the state, and with a mix lets no
-    input in (with A; without A it forgets the state).  Returns y [batch, T, D], followed by the state behind each sequence's last token
+    input in (with A; without A it forgets the state).  A state that is infinite stays so (where a is below 2^-126, which counts as 0, it may become NaN).  Returns y [batch, T, D], followed by the state behind each sequence's last token
     where `return_state` asks for it, and by the states before every 64th token, fp32 [batch, ceil(T / 64), D], that `gated_scan_backward`
     starts from, where `return_checkpoints` does (those behind a sequence's end hold nothing)."""
     y, end, ck = _host().gated(x, gate, A, input_gate, gate_bias, input_bias, _mix(mix), state, lengths, return_state, return_checkpoints)
