@@ -10,6 +10,7 @@
 // Measured, bf16: 3 x 32768 x 2048 packed in 111 us and unpacked in 102 (5.5 and 6.0 TB/s); the norm of 16384 x 2048 with an fp32
 // residual, a scale to 128, 56 us (6.6 TB/s), with a bf16 residual, layer norm and a scale to a token 56 (4.2 TB/s; 75 % of the issue slots).
 #include <algorithm>
+#include <cmath>
 
 #include "ttt_eight_bits.cuh"
 
@@ -226,19 +227,19 @@ struct Shared {
   float top[2][32];
 };
 
-// 1 / sqrt(v) as a sum: the fast one, and a step of Newton's.  An error that all of a token's values have alike takes more of them over a border of their
-// rounding to 4 bits than as many errors that differ: 16384 x 2048, error of all values against 64 bits 6.6e-5 with the fast one alone, where a root and a
-// division have 1.6e-5; with the sum the same as these (some 20 of 33 million values differ).
+// 1 / sqrt(v) as a sum: the fast one, and a step of Newton's with 1 - v r^2 from v r in two parts.  An error that all of a token's values have alike takes more of them
+// over a border of their rounding to 4 bits than as many errors that differ.  Of 99 million values (16384 x 2048 twice, 16384 x 1920) 50 are not those of 64 bits; of
+// a root and a division in 32 bits 54.
 __device__ __forceinline__ float2 inverse_root(float v) {
-  const float r = rsqrtf(v), e = fmaf(-v * r, r, 1.f);
+  const float r = rsqrtf(v), p = v * r, e = fmaf(-p, r, 1.f) - fmaf(v, r, -p) * r;
   return make_float2(r, e < 1.f ? 0.5f * r * e : 0.f);      // (v = 0, infinite or NaN: r as it is)
 }
 
 // Mean and 1 / deviation (in two parts) of a token with one barrier: each warp's mean and its squares about it, joined as
 // sum over warps of (squares + columns (mean of the warp - mean)^2).
-template <int kWidth, bool kWhole> __device__ __forceinline__ float3 statistics(const float (&z)[8], const ttt_b200_norm8_args& p, int lane, Shared& sh, int turn) {
+// `inv`: 1 / D in two parts, since rounded to one all tokens would have its error (a division in its place: 16384 x 2048 bf16 43 -> 45 us).
+template <int kWidth, bool kWhole> __device__ __forceinline__ float3 statistics(const float (&z)[8], const ttt_b200_norm8_args& p, float2 inv, int lane, Shared& sh, int turn) {
   auto columns = [&](int warp) { return static_cast<float>(min(max(p.D - warp * 256, 0), 256)); };
-  const float inv = 1.f / static_cast<float>(p.D);
   float mean = 0.f, sq = 0.f;
   if (p.layer) {
     float s = 0.f;
@@ -264,19 +265,19 @@ template <int kWidth, bool kWhole> __device__ __forceinline__ float3 statistics(
       mean = n * v.x;
 #pragma unroll
       for (int o = warps / 2; o; o /= 2) mean += __shfl_xor_sync(0xffffffffu, mean, o);
-      mean *= inv;
+      mean = fmaf(mean, inv.x, mean * inv.y);
       sq = fmaf(n * (v.x - mean), v.x - mean, sq);
     }
 #pragma unroll
     for (int o = warps / 2; o; o /= 2) sq += __shfl_xor_sync(0xffffffffu, sq, o);
   }
-  const float2 dev = inverse_root(fmaf(sq, inv, p.eps));
+  const float2 dev = inverse_root(fmaf(sq, inv.x, fmaf(sq, inv.y, p.eps)));
   return make_float3(mean, dev.x, dev.y);
 }
 
 // L lanes to a group; 0: the token has one scale
 template <class T, class R, int kWidth, bool kWhole, int L>
-__global__ void __launch_bounds__(kWidth* kSide<kWidth>, kNormThreads / (kWidth * kSide<kWidth>)) norm8_kernel(const ttt_b200_norm8_args p) {
+__global__ void __launch_bounds__(kWidth* kSide<kWidth>, kNormThreads / (kWidth * kSide<kWidth>)) norm8_kernel(const ttt_b200_norm8_args p, const float2 inv) {
   wait_for_predecessor();
   constexpr int side = kSide<kWidth>;
   __shared__ Shared sh;
@@ -306,11 +307,11 @@ __global__ void __launch_bounds__(kWidth* kSide<kWidth>, kNormThreads / (kWidth 
       leave<kWhole>(static_cast<R*>(p.x) + m * p.D, lane, p.D, r);
     }
     ask(m + step);
-    const float3 s = statistics<kWidth, kWhole>(z, p, lane, sh, turn);
+    const float3 s = statistics<kWidth, kWhole>(z, p, inv, lane, sh, turn);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {      // (0 behind the last column, as weight and bias)
       const float c = z[j] - s.x;
-      z[j] = fmaf(c, s.z, c * s.y) * w.v[j];
+      z[j] = fmaf(c, s.y, c * s.z) * w.v[j];      // the large product exact: rounded once
     }
     if (p.bias) {
 #pragma unroll
@@ -409,7 +410,10 @@ template <class T, class R, int kWidth, bool kWhole> int norm_with(const ttt_b20
   const int ctas = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(sm_count()) * (kNormThreads / threads), (p.M + side - 1) / side));
   const auto kernel = p.group == 0 ? norm8_kernel<T, R, kWidth, kWhole, 0> : p.group == 32 ? norm8_kernel<T, R, kWidth, kWhole, 4>
                     : p.group == 64 ? norm8_kernel<T, R, kWidth, kWhole, 8> : norm8_kernel<T, R, kWidth, kWhole, 16>;
-  ttt_launch_overlapped(kernel, ctas, threads, 0, s, p);
+  float inv = static_cast<float>(1.0 / p.D);
+  if (inv > 1.0 / p.D) inv = std::nextafter(inv, 0.f);
+  const float rest = std::max(static_cast<float>(1.0 / p.D - inv), 0x1p-149f);      // (above 0, so that infinite squares stay infinite)
+  ttt_launch_overlapped(kernel, ctas, threads, 0, s, p, make_float2(inv, rest));
   return launched("norm8");
 }
 template <class T, class R, int kWidth> int norm_as(const ttt_b200_norm8_args& p, cudaStream_t s) {
