@@ -28,6 +28,7 @@ struct Tables {
   int first[kMost + 1];      // CTA of a table
   int shift;                 // 2^shift units of a row that a CTA has
   int count, rows, pairs;
+  int marks;                 // a copy's with more rows than a CTA marks: 2^marks places, at least twice as many as pairs; else -1
   const int32_t *source, *target;
   const uint8_t* used;
   int32_t* place;
@@ -48,7 +49,14 @@ template <class U> struct Slab {
   }
 };
 
-// A row that two pairs name as their target gets the later one's; `win[i]`: whether pair i is taken.
+// A row that two pairs name as their target gets the later one's: each target has its last pair in shared memory.  Where a CTA can mark all rows, a row's
+// place there is its number.  With more rows it is its number's hash, among at least twice as many places as pairs, and the next one where another row has that: 4096
+// pairs of 8193 rows of 4 KB 71 us, for 2645 with a search of the pairs behind each; of 8192 rows 71 as well, for 37 with a place for each row.
+__device__ __forceinline__ uint32_t place_of(uint32_t row, int bits) {
+  row *= 0x9e3779b1u;
+  row ^= row >> 15;
+  return row * 0x9e3779b1u >> (32 - bits);
+}
 __device__ __forceinline__ bool inside(const Tables& q, int i) {
   return static_cast<uint32_t>(q.target[i]) < static_cast<uint32_t>(q.rows) && static_cast<uint32_t>(q.source[i]) < static_cast<uint32_t>(q.rows);
 }
@@ -59,26 +67,45 @@ template <class U> __global__ void __launch_bounds__(kThreads) copy_rows_kernel(
   const Slab<U> s(q);
   int32_t* from = reinterpret_cast<int32_t*>(memory);      // of a pair that is taken: its rows; else -1
   int32_t* to = from + q.pairs;
-  int32_t* last = to + q.pairs;                            // of a row: its last pair
-  const bool marked = q.rows <= kMarked;
-  if (marked) {
-    for (int r = threadIdx.x; r < q.rows; r += kThreads) last[r] = -1;
-    __syncthreads();
-    for (int i = threadIdx.x; i < q.pairs; i += kThreads)
-      if (inside(q, i)) atomicMax(&last[q.target[i]], i);      // (a maximum does not go by the order)
-    __syncthreads();
+  int32_t* last = to + q.pairs;                            // of a place: its row's last pair
+  const bool hashed = q.marks >= 0;
+  const int places = hashed ? 1 << q.marks : q.rows;
+  int32_t* row = last + places;                            // hashed: and that row
+  for (int k = threadIdx.x; k < places; k += kThreads) {
+    last[k] = -1;
+    if (hashed) row[k] = -1;
   }
+  __syncthreads();
   for (int i = threadIdx.x; i < q.pairs; i += kThreads) {
-    bool take = inside(q, i);
+    if (!inside(q, i)) continue;
     const int t = q.target[i];
-    if (take && marked) take = last[t] == i;
-    else if (take)
-      for (int j = i + 1; j < q.pairs; ++j) take = take && !(q.target[j] == t && inside(q, j));
+    uint32_t k = t;
+    if (hashed) {
+      k = place_of(t, q.marks);
+      for (int tries = 0; tries < places; ++tries, k = (k + 1) & (places - 1)) {      // (half of the places stay free)
+        const int32_t who = atomicCAS(&row[k], -1, t);
+        if (who == -1 || who == t) break;
+      }
+    }
+    atomicMax(&last[k], i);      // (a maximum does not go by the order)
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < q.pairs; i += kThreads) {
+    const int t = q.target[i];
+    bool take = inside(q, i);
+    if (take) {
+      uint32_t k = t;
+      if (hashed) {
+        k = place_of(t, q.marks);
+        for (int tries = 0; tries < places && row[k] != t; ++tries) k = (k + 1) & (places - 1);
+      }
+      take = last[k] == i;
+    }
     from[i] = take ? q.source[i] : -1;
     to[i] = t;
   }
   __syncthreads();
-  U* stage = reinterpret_cast<U*>(memory + (8L * q.pairs + (marked ? 4L * q.rows : 0) + 15) / 16 * 16);
+  U* stage = reinterpret_cast<U*>(memory + (8L * q.pairs + (hashed ? 8L : 4L) * places + 15) / 16 * 16);
   const int total = q.pairs << q.shift;
 #pragma unroll 4
   for (int k = threadIdx.x; k < total; k += kThreads) {
@@ -225,8 +252,11 @@ extern "C" int ttt_b200_copy_rows(const ttt_b200_tables_args* p, void* stream) {
   q.source = p->source;
   q.target = p->target;
   const int unit = unit_of(*p);
-  // shared memory: the pairs, the marks, and the slab of every pair: 32 KB, with many pairs as much as 16 bytes of each take
-  const int64_t lists = (8L * q.pairs + (p->rows <= kMarked ? 4L * p->rows : 0) + 15) / 16 * 16;
+  // shared memory: the pairs, the targets' places, and the slab of every pair: 32 KB, with many pairs as much as 16 bytes of each take
+  q.marks = -1;
+  if (p->rows > kMarked)
+    for (q.marks = 1; 1 << q.marks < 2 * q.pairs;) ++q.marks;
+  const int64_t lists = (8L * q.pairs + (q.marks < 0 ? 4L * p->rows : 8L << q.marks) + 15) / 16 * 16;
   const int64_t room = std::max<int64_t>(32 * 1024, 16L * q.pairs);
   if (int rc = lay_out(q, *p, unit, room / (static_cast<int64_t>(unit) * q.pairs))) return rc;
   const uint32_t bytes = static_cast<uint32_t>(lists + (static_cast<int64_t>(unit) * q.pairs << q.shift));
