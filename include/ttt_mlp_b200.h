@@ -494,8 +494,9 @@ typedef struct ttt_b200_gated_args {
 } ttt_b200_gated_args;
 int ttt_b200_gated_scan(const ttt_b200_gated_args* args, void* stream);
 int ttt_b200_gated_scan_backward(const ttt_b200_gated_args* args, void* stream);
-/* Bytes of scratch the forward (backward = 0) or backward needs; depends on B, T, D and the GPU: where a sequence is cut into chunks (at most 32) 8 bytes
- * per channel and chunk, in the backward 12 more per channel and chunk. */
+/* Bytes of scratch the forward (backward = 0) or backward needs; depends on which it is, on B, T, D and the GPU, in the backward on dtype and group too (fp32 that
+ * is not in 8 bits has another number of chunks): where a sequence is cut into chunks (at most 32) 8 bytes per channel and chunk, in the backward 12 more per
+ * channel and chunk. */
 uint64_t ttt_b200_gated_scan_scratch_bytes(const ttt_b200_gated_args* args, int backward);
 /* One token per row; slots as in ttt_b200_short_conv_step. */
 int ttt_b200_gated_scan_step(const ttt_b200_gated_args* args, void* stream);

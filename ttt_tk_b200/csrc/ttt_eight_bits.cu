@@ -7,8 +7,8 @@
 // All bound by memory: 2 + 1 bytes a value (16 bits), the norm 2 + 2 + 2 + 1 or with an fp32 residual stream 2 + 4 + 4 + 1.  A thread has eight
 // neighbouring values, one 16-byte access; the lanes of a group, four, eight or sixteen, exchange their largest magnitudes.
 //
-// Measured, bf16: 3 x 32768 x 2048 packed in 111 us and unpacked in 102 (5.5 and 6.0 TB/s); the norm of 16384 x 2048 with an fp32
-// residual, a scale to 128, 56 us (6.6 TB/s), with a bf16 residual, layer norm and a scale to a token 56 (4.2 TB/s; 75 % of the issue slots).
+// Measured, bf16, calls back to back: 3 x 32768 x 2048 packed in 104 us and unpacked in 94 (5.9 and 6.5 TB/s); the norm of 16384 x 2048 with an fp32
+// residual, a scale to 128, 57 us (6.4 TB/s), with a bf16 residual 44 (5.4 TB/s), with that, layer norm and a scale to a token 53 (4.4 TB/s; 75 % of the issue slots).
 #include <algorithm>
 #include <cmath>
 
@@ -19,7 +19,9 @@ namespace {
 using namespace ttt;
 
 constexpr int kMost = TTT_B200_PACK8_TENSORS;
-constexpr int kNormThreads = 1024;      // of an SM (16384 x 2048, fp32 residual: 63 us; 1536, with registers spilled, 82)
+// Of an SM (16384 x 2048, fp32 residual: 63 us; 1536, with registers spilled everywhere, 82).  At 1024 those of up to 512 columns spill where rows start on any boundary (4 to
+// 56 bytes), with an fp32 residual on every boundary (8 to 32): four and two tokens to a CTA take their registers.
+constexpr int kNormThreads = 1024;
 
 // ---- pack and unpack ----------------------------------------------------------------------------------------------------------------
 struct Many {

@@ -28,7 +28,7 @@ __device__ __forceinline__ float magnitude(const float (&v)[8]) {
 // Exponent field of the scale of a group whose largest magnitude has these bits: 8 less than that of amax / 1.75 rounded up, at least 1.
 __device__ __forceinline__ uint32_t scale_exponent(float most) { return max(static_cast<int>((__float_as_uint(most) + 0x1fffffu) >> 23) - 8, 1); }
 __device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float(e << 23); }
-__device__ __forceinline__ float inverse_of(uint32_t e) { return __uint_as_float((254u - e) << 23); }      // (e is at most 254 - 8: no subnormal)
+__device__ __forceinline__ float inverse_of(uint32_t e) { return __uint_as_float((254u - e) << 23); }      // (e is at most 255 - 8, of magnitudes above 1.75 2^127: no subnormal)
 
 // Two values to two bytes.
 __device__ __forceinline__ uint32_t two_bytes(float a, float b) {

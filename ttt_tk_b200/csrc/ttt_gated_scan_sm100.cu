@@ -839,6 +839,7 @@ int mode_of(const ttt_b200_gated_args& p, bool backward) {
 // of them or one of 16 warps 24; a turn of CTAs over the SMs starts in 20; the chunks' steps take 0.6 of that.
 // 16384 tokens of 1024 channels, forward / backward us: one chunk 348 / 673, 8 chunks 89 / 126, 18 (by the rule) 73 / 97, 24 83 / 116;
 // 2 x 2048 of 2048: one of 8 warps 51 / 95, of 16 45 / 79, 4 chunks (by the rule) 42 / 56, 8 44 / 60.
+// All of these are bf16 with every part, whole rows; fp32, odd rows and forms with fewer parts go by the same costs, which were not measured for them.
 void plan(Plan& q, const ttt_b200_gated_args& p, bool backward) {
   q.tiles = (p.D - 1) / kCols + 1;
   q.nck = (p.T - 1) / kEvery + 1;
