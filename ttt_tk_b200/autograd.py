@@ -280,7 +280,7 @@ class SSMScanFunction(torch.autograd.Function):
 def ssm_scan(x, dt, A, B, C, D=None, dt_bias=None, *, softplus=True, state=None, lengths=None, return_state=False, saved=None):
     """Differentiable `ttt_tk_b200.ssm.ssm_scan`; where gradients are recorded, the checkpoints are kept for the backward.  `saved` "e4m3": x and dt are
     kept in 8 bits, and the gradients are those at what was kept, with the checkpoints as the forward has them; a dt below -448 (a mask's -inf) is kept as
-    -448, which softplus takes to 0 as well as it."""
+    -448, which softplus takes to 0 as well as it (with a dt_bias of less than 300)."""
     y, end = SSMScanFunction.apply(x, dt, A, B, C, D, dt_bias, state, softplus, lengths, return_state, torch.is_grad_enabled(), _saved(saved))
     return (y, end) if return_state else y
 
